@@ -354,6 +354,8 @@ tl_status tl_profile_reset(tl_ctx* ctx);
 int64_t tl_launch_count(const tl_ctx* ctx);
 /* The context's CUDA stream (a cudaStream_t) for event timing by the caller. */
 void* tl_stream(const tl_ctx* ctx);
+/* The context's device (a CUDA ordinal; -1 without a context). */
+int32_t tl_device(const tl_ctx* ctx);
 
 /* ------------------------------------------------------------------------ */
 /* Allocation-free closure fixpoint.                                         */
@@ -398,6 +400,127 @@ void* tl_stream(const tl_ctx* ctx);
 tl_status tl_closure_noalloc(int64_t n, const int64_t* d_rowptr, const int32_t* d_colidx,
                              uint32_t* d_reach, int32_t max_sweeps, void* stream,
                              int32_t* sweeps_out);
+
+/* ------------------------------------------------------------------------ */
+/* Attention with modified scores, its gradient, and gradient clipping.      */
+/*                                                                           */
+/* No counterpart in the reference, whose attention is the three equations  */
+/* of an attention program (S = Q K, A = softmax(S), O = A V: no heads, no   */
+/* masks, S and A kept) and whose `backward` leaves gradients as they come.  */
+/* These calls work on device arrays: memory of the caller's on the          */
+/* context's device, or the fp32 storage of a program's tensor               */
+/* (tl_tensor_array).                                                        */
+/*                                                                           */
+/* Every call checks its arguments before any device work, queues its work   */
+/* on `stream` (a cudaStream_t of the context's device; NULL = the default   */
+/* stream; tl_stream(ctx) = the context's own) and returns without waiting.   */
+/* A bounded device wait that ran out is reported by the next tl_sync that   */
+/* follows the end of the work.  Like every call on a context they are for   */
+/* one host thread at a time.                                                */
+/*                                                                           */
+/* workspace: device memory of at least the size that the call's             */
+/* _workspace function gives, 256-byte aligned, free for other use when the  */
+/* work is done; two calls that may overlap on the GPU (other streams, two   */
+/* captured graphs) need workspaces of their own.  NULL: the context's       */
+/* buffer for that stream, which it allocates as needed (and keeps for the   */
+/* 16 streams used last); a stream in capture and the per-thread default     */
+/* stream need one of the caller's (TL_ERR_INVALID) unless the size is 0.    */
+/* ------------------------------------------------------------------------ */
+#define TL_TYPE_F32  0
+#define TL_TYPE_F16  1
+#define TL_TYPE_BF16 2
+#define TL_ARRAY_RANK 4
+
+/* A view of device memory: strides in elements, none negative. */
+typedef struct tl_array {
+    void* data;
+    int32_t dtype;                      /* TL_TYPE_*                          */
+    int32_t rank;                       /* 0..TL_ARRAY_RANK                   */
+    int64_t dims[TL_ARRAY_RANK];
+    int64_t strides[TL_ARRAY_RANK];
+} tl_array;
+
+/* A view of a tensor's fp32 dense storage (materialised on demand).  write: */
+/* the caller will write through it, so the other storages are dropped.  Not */
+/* for sharded tensors.  The view holds until the next call that gives the   */
+/* tensor other dims or writes it in another form.                           */
+tl_status tl_tensor_array(tl_tensor* t, int32_t write, tl_array* out);
+
+/*
+ * Query i of sequence b stands at position P_i = q_start[b] + i.  With head h
+ * of the queries reading head h / (Hq / Hkv) of the keys, key j at position j:
+ *
+ *   x = scale q_i . k_j
+ *   y = softcap tanh(x / softcap)            (softcap = 0: y = x)
+ *   s = y - slopes[h] |P_i - j|              (slopes NULL: s = y)
+ *   key j is seen by query i when j < kv_len[b], and (not causal, or j <= P_i,
+ *     or j < prefix_len[b]), and (no documents, or q_doc[b,i] == k_doc[b,j] >= 0)
+ *   o_i = sum over seen j of softmax(s)_j v_j,  lse_i = log sum exp(s)
+ *
+ * A query that sees no key gives o = 0 and lse = -inf, and takes and gives no
+ * gradient.  What k and v hold at and after kv_len[b] and at keys of a negative
+ * document, and q and dout at queries of a negative document, does not matter,
+ * not even infinities or NaN; elsewhere a value that is not finite reaches the
+ * results as it does in the formulas (0 times infinity included).
+ *
+ * Arrays of rank 4, [batch, heads, positions, head size], of one type, head
+ * size 1..256, any strides (k and v may have strides of 0; arrays that are
+ * written may not overlap themselves, one another or an input).  fp32 is
+ * computed in fp32; 16-bit types take their products from 16-bit operands
+ * (scores' exponentials and dx rounded to them) with 32-bit sums, the softmax
+ * and its statistics in 32 bits.
+ * The device arrays slopes [Hq] fp32 (constants: they get no gradient),
+ * prefix_len, kv_len, q_start [batch] int32, q_doc [batch, Nq] and
+ * k_doc [batch, Nk] int32 are contiguous.  kv_len NULL: all Nk keys; its values
+ * are clamped to 0..Nk, those of q_start to +-2^30.  q_start NULL: kv_len[b] - Nq, so that the last query
+ * stands at the last key (a cache that already holds the new tokens); a batch
+ * padded on the right passes zeros.
+ */
+typedef struct tl_attention {
+    tl_array q, k, v, o;                /* o: forward writes, backward reads  */
+    tl_array dout, dq, dk, dv;          /* backward only                      */
+    float* lse;                         /* [batch, Hq, Nq] contiguous fp32;   */
+                                        /* forward: NULL if not wanted        */
+    float scale;
+    float softcap;
+    int32_t causal;
+    int32_t _pad;
+    const float* slopes;
+    const int32_t* prefix_len;          /* with causal only                   */
+    const int32_t* q_doc;               /* both or neither                    */
+    const int32_t* k_doc;
+    const int32_t* kv_len;
+    const int32_t* q_start;
+    void* workspace;
+    int64_t workspace_bytes;
+    void* stream;
+} tl_attention;
+
+/* Forward: writes o, and lse when given.  Few queries over many keys (a token */
+/* of each sequence over its cache) are split over the keys.                  */
+tl_status tl_attention_forward(tl_ctx* ctx, const tl_attention* a);
+/* Backward: dq, dk, dv of sum(o * dout) from the forward's o and lse.  The   */
+/* results do not depend on the order in which blocks run.                    */
+tl_status tl_attention_backward(tl_ctx* ctx, const tl_attention* a);
+/* Bytes of workspace of a forward (backward = 0) or backward call with these */
+/* arrays, or minus the status with which the call would be refused.  Checks  */
+/* the arguments and does no device work; ctx may be NULL (no error text).    */
+int64_t tl_attention_workspace(tl_ctx* ctx, const tl_attention* a, int32_t backward);
+
+/*
+ * norm = sqrt(sum of x^2 over all elements of the n arrays), in 64 bits;
+ * out = x min(1, max_norm / norm).  out NULL: in place (nothing is written when
+ * norm <= max_norm).  A norm that is not finite leaves the values as they are.
+ * The arrays may have different types and ranks; each is dense (its elements
+ * fill their memory in some order) and out[i] has the dims and strides of
+ * grads[i] and any type.  No element may lie in two of the arrays written.
+ * d_norm: device fp32 scalar that receives the norm, or NULL.  max_norm: >= 0,
+ * infinity for the norm alone.
+ */
+tl_status tl_clip_gradients(tl_ctx* ctx, const tl_array* grads, const tl_array* out, int32_t n, double max_norm,
+                            float* d_norm, void* workspace, int64_t workspace_bytes, void* stream);
+/* As tl_attention_workspace, for a tl_clip_gradients call. */
+int64_t tl_clip_workspace(tl_ctx* ctx, const tl_array* grads, const tl_array* out, int32_t n, double max_norm);
 
 #ifdef __cplusplus
 }

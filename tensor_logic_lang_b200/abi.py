@@ -31,6 +31,10 @@ STATUS_NAMES = {
 }
 TL_NOALLOC_MAX_ROWS = 65536
 
+# element types of device arrays
+TL_TYPE_F32, TL_TYPE_F16, TL_TYPE_BF16 = range(3)
+TL_ARRAY_RANK = 4
+
 # index kinds
 IX_NAME, IX_CONST, IX_ADD, IX_SUB, IX_PRIMED, IX_DIV, IX_NORMALIZE, IX_SLICE, IX_VIRTUAL = range(9)
 
@@ -100,6 +104,21 @@ class KernelStats(C.Structure):
                 ("algo_bytes", C.c_double), ("algo_flops", C.c_double)]
 
 
+class Array(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int32), ("rank", C.c_int32),
+                ("dims", C.c_int64 * TL_ARRAY_RANK), ("strides", C.c_int64 * TL_ARRAY_RANK)]
+
+
+class Attention(C.Structure):
+    _fields_ = [("q", Array), ("k", Array), ("v", Array), ("o", Array),
+                ("dout", Array), ("dq", Array), ("dk", Array), ("dv", Array),
+                ("lse", C.c_void_p), ("scale", C.c_float), ("softcap", C.c_float),
+                ("causal", C.c_int32), ("_pad", C.c_int32), ("slopes", C.c_void_p),
+                ("prefix_len", C.c_void_p), ("q_doc", C.c_void_p), ("k_doc", C.c_void_p),
+                ("kv_len", C.c_void_p), ("q_start", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64), ("stream", C.c_void_p)]
+
+
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
 LIB_PATH = os.path.join(PKG_DIR, "libtl_cuda.so")
@@ -114,6 +133,8 @@ EXPORTS = [
     "tl_tensor_download_bits", "tl_tensor_device_ptr", "tl_tensor_set", "tl_sparse_upload",
     "tl_query_format", "tl_program_output", "tl_set_sharding", "tl_profile_enable", "tl_profile_read",
     "tl_profile_reset", "tl_launch_count", "tl_stream", "tl_closure_noalloc",
+    "tl_tensor_array", "tl_attention_forward", "tl_attention_backward", "tl_attention_workspace",
+    "tl_clip_gradients", "tl_clip_workspace", "tl_device",
 ]
 
 
@@ -157,6 +178,13 @@ def _declare(lib):
         "tl_launch_count": (C.c_int64, [vp]),
         "tl_stream": (C.c_void_p, [vp]),
         "tl_closure_noalloc": (C.c_int32, [C.c_int64, vp, vp, vp, C.c_int32, vp, P(C.c_int32)]),
+        "tl_tensor_array": (C.c_int32, [vp, C.c_int32, P(Array)]),
+        "tl_attention_forward": (C.c_int32, [vp, vp]),
+        "tl_attention_backward": (C.c_int32, [vp, vp]),
+        "tl_attention_workspace": (C.c_int64, [vp, vp, C.c_int32]),
+        "tl_clip_gradients": (C.c_int32, [vp, vp, vp, C.c_int32, C.c_double, vp, vp, C.c_int64, vp]),
+        "tl_clip_workspace": (C.c_int64, [vp, vp, vp, C.c_int32, C.c_double]),
+        "tl_device": (C.c_int32, [vp]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)

@@ -24,6 +24,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include "tc_ptx.h"
 #include "tl_internal.h"
 
 namespace tl {
@@ -357,7 +358,6 @@ __global__ void __launch_bounds__(TK_THREADS) k_gemm_thin_k(const __grid_constan
 constexpr int TC_BM = 128;
 constexpr int TC_BK = 32;               // 32 fp32 = 128 bytes = one swizzle row
 constexpr int TC_THREADS = 192;         // warp0 TMA, warp1 MMA, warps 2-5 epilogue
-constexpr uint64_t kWaitLimitNs = 2000000000ull;
 
 struct TcEpi {
     float* C; int64_t scm, scn;
@@ -371,74 +371,6 @@ struct TcEpi {
     int fan_n;
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
-                 : "memory");
-}
-
-__device__ __forceinline__ uint64_t globaltimer_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-// Bounded wait: gives up after ~2 s of device time, flags *err and returns
-// false, so a pipeline that never completes ends the kernel instead of
-// hanging the GPU.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* err) {
-    const uint32_t addr = smem_u32(bar);
-    uint64_t t0 = 0;
-    for (unsigned it = 0;; ++it) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(addr), "r"(parity)
-            : "memory");
-        if (ok) return true;
-        if ((it & 1023u) == 0) {
-            const uint64_t now = globaltimer_ns();
-            if (t0 == 0) t0 = now;
-            else if (now - t0 > kWaitLimitNs) break;
-        }
-    }
-    if (err) atomicExch(err, 1);
-    return false;
-}
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-            smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
-        : "memory");
-}
-
-// UMMA shared-memory descriptor (sm_100 version 1).  Layout type 2 is the
-// 128-byte swizzle of K-major tiles; type 1 is the 128-byte swizzle with a
-// 32-byte atom, the one shared-memory layout MN-major tf32 operands have.
-constexpr uint64_t kLayoutSW128 = 2, kLayoutSW128Base32B = 1;
-__device__ __forceinline__ uint64_t umma_desc(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes,
-                                              uint64_t layout) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr >> 4) & 0x3FFF);
-    d |= (uint64_t)((lbo_bytes >> 4) & 0x3FFF) << 16;
-    d |= (uint64_t)((sbo_bytes >> 4) & 0x3FFF) << 32;
-    d |= (uint64_t)1 << 46;                 // descriptor version (Blackwell)
-    d |= layout << 61;
-    return d;
-}
-
 __device__ __forceinline__ void umma_tf32(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                           uint32_t accumulate) {
     asm volatile(
@@ -446,11 +378,6 @@ __device__ __forceinline__ void umma_tf32(uint32_t tmem_d, uint64_t adesc, uint6
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
-}
-
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
 }
 
 // Epilogue stores through the TMA: a 32 x 32 fp32 tile in shared memory (rows
@@ -475,8 +402,6 @@ __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.comm
 __device__ __forceinline__ void bulk_wait_read_1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_read_0() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
     uint32_t r[16];
     asm volatile(
@@ -905,10 +830,6 @@ struct AttnArgs {
     float* lpart;         // [key tiles][n_q]: row sum of exp(scale * S - m) over the tile
     int* err;             // a bounded pipeline wait ran out
 };
-
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 
 // Every fp32 of [base, base + bytes) rounded to TF32 in place by nthreads threads.
 __device__ __forceinline__ void round_tf32_inplace(uint8_t* base, int bytes, int t, int nthreads) {

@@ -42,10 +42,14 @@ tl_status cuda_fail(tl_ctx* c, cudaError_t e, const char* what) {
                 cudaGetErrorString(e));
 }
 
-void launch_begin(tl_ctx* c, const char* name, double bytes, double flops, cudaEvent_t* ev) {
+void launch_begin_on(tl_ctx* c, cudaStream_t s, const char* name, double bytes, double flops, cudaEvent_t* ev) {
     c->launches++;
     ev[0] = ev[1] = nullptr;
     if (!c->prof) return;
+    if (s != c->stream) {
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(s, &cap) != cudaSuccess || cap != cudaStreamCaptureStatusNone) return;
+    }
     for (int i = 0; i < 2; ++i) {
         if (!c->event_pool.empty()) {
             ev[i] = c->event_pool.back();
@@ -54,16 +58,22 @@ void launch_begin(tl_ctx* c, const char* name, double bytes, double flops, cudaE
             cudaEventCreate(&ev[i]);
         }
     }
-    cudaEventRecord(ev[0], c->stream);
+    cudaEventRecord(ev[0], s);
     c->pending.push_back({name, ev[0], ev[1], bytes, flops});
 }
 
-tl_status launch_end(tl_ctx* c, cudaEvent_t* ev) {
+tl_status launch_end_on(tl_ctx* c, cudaStream_t s, cudaEvent_t* ev) {
     cudaError_t e = cudaGetLastError();
-    if (ev[1]) cudaEventRecord(ev[1], c->stream);
+    if (ev[1]) cudaEventRecord(ev[1], s);
     if (e != cudaSuccess) return cuda_fail(c, e, "kernel launch");
     return TL_OK;
 }
+
+void launch_begin(tl_ctx* c, const char* name, double bytes, double flops, cudaEvent_t* ev) {
+    launch_begin_on(c, c->stream, name, bytes, flops, ev);
+}
+
+tl_status launch_end(tl_ctx* c, cudaEvent_t* ev) { return launch_end_on(c, c->stream, ev); }
 
 tl_status workspace(tl_ctx* c, size_t bytes, void** out, int slot) {
     if (slot < 0 || slot > 3) return fail(c, TL_ERR_INVALID, "bad workspace slot");
@@ -351,6 +361,7 @@ extern "C" tl_status tl_shutdown(tl_ctx* c) {
     comm_sym_release(c, SYM_GNN);
     if (c->comm) comm_destroy(c);
     for (int i = 0; i < 4; ++i) cudaFree(c->ws[i]);
+    for (auto& w : c->op_ws) cudaFree(w.ptr);
     cudaFree(c->aux);
     cudaFree(c->fix_state);
     cudaFree(c->fix_closed);
@@ -406,6 +417,8 @@ extern "C" int32_t tl_last_sweeps(const tl_ctx* c) {
     return m->last_sweeps;
 }
 extern "C" int64_t tl_launch_count(const tl_ctx* c) { return c ? c->launches : 0; }
+extern "C" int32_t tl_device(const tl_ctx* c) { return c ? c->device : -1; }
+
 extern "C" void* tl_stream(const tl_ctx* c) { return c ? (void*)c->stream : nullptr; }
 
 extern "C" tl_status tl_domain(tl_ctx* c, const char* name, int64_t size) {

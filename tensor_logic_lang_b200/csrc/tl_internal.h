@@ -141,6 +141,13 @@ struct BqHost {
     float* snap = nullptr;     // device copy of what it held then (nullptr: zeros)
 };
 
+// scratch of the array operators on one stream (op_workspace)
+struct StreamWs {
+    cudaStream_t stream;
+    void* ptr;
+    size_t cap;
+};
+
 }  // namespace tl
 
 struct tl_tensor : tl::Tensor {};
@@ -166,6 +173,9 @@ struct tl_ctx {
     // device scratch
     void* ws[4] = {nullptr, nullptr, nullptr, nullptr};   // one buffer per tl::WsSlot
     size_t ws_cap[4] = {0, 0, 0, 0};
+    // scratch of the array operators (attention, clipping), one buffer per
+    // stream they ran on, the one used last at the end
+    std::vector<tl::StreamWs> op_ws;
     int* d_flags = nullptr;     // [0..63] changed / error words
     void* aux = nullptr;        // state kept across the sweeps of one fixpoint
     size_t aux_cap = 0;
@@ -241,8 +251,13 @@ tl_status cuda_fail(tl_ctx* c, cudaError_t e, const char* what);
     } while (0)
 
 // launch accounting: every kernel launch of the runtime goes through these
+// (timed by events on the context's stream)
 void launch_begin(tl_ctx* c, const char* name, double bytes, double flops, cudaEvent_t* ev);
 tl_status launch_end(tl_ctx* c, cudaEvent_t* ev);
+// the same for a launch on a stream of the caller's; a stream in capture is
+// counted but not timed
+void launch_begin_on(tl_ctx* c, cudaStream_t s, const char* name, double bytes, double flops, cudaEvent_t* ev);
+tl_status launch_end_on(tl_ctx* c, cudaStream_t s, cudaEvent_t* ev);
 struct LaunchScope {
     tl_ctx* c;
     cudaEvent_t ev[2] = {nullptr, nullptr};

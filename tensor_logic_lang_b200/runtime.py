@@ -7,10 +7,20 @@ lowered `.tl` program the way the reference's emitted `main()` does
 fallback: without the built library or a GPU, construction raises.
 """
 import ctypes as C
+import struct
 
 import numpy as np
 
 from . import abi
+
+
+# tl_array: data, dtype, rank, dims[4], strides[4]
+_ARRAY = struct.Struct("=Qii4q4q")
+_TYPES = {"torch.float32": abi.TL_TYPE_F32, "torch.float16": abi.TL_TYPE_F16, "torch.bfloat16": abi.TL_TYPE_BF16,
+          "float32": abi.TL_TYPE_F32, "float16": abi.TL_TYPE_F16, "bfloat16": abi.TL_TYPE_BF16}
+_type_of = {}          # dtype object -> TL_TYPE_*
+_ATTENTION_AT = {n: getattr(abi.Attention, n).offset for n, _ in abi.Attention._fields_}
+_ATTENTION_TAIL = struct.Struct("=QffiiQQQQQQQqQ")   # lse .. stream
 
 
 class Context:
@@ -34,6 +44,7 @@ class Context:
         if st != abi.TL_OK:
             raise abi.TLError(st, "tl_init failed (no CUDA device or bad options)")
         self.h = h
+        self.device = self.lib.tl_device(h)
 
     def close(self):
         if getattr(self, "h", None):
@@ -158,6 +169,177 @@ class Context:
         buf = C.create_string_buffer(need.value + 1)
         self.check(self.lib.tl_program_output(self.h, buf, len(buf), None), "program output")
         return buf.value.decode()
+
+    # ------------------------------------------------------------------ array operators
+    # Arrays are device tensors (torch's, or any object with data_ptr(), dtype,
+    # shape, stride() and device), or names of this context's tensors, which
+    # stand for their fp32 storage.  stream: a cudaStream_t handle (torch's
+    # current stream: torch.cuda.current_stream().cuda_stream), or None for the
+    # context's own stream, on which its programs run.  Device tensors that
+    # another stream wrote need that stream's work done or waited for first.
+    def _view(self, x, what, write=False):
+        """(data, type, shape, strides) of an array argument."""
+        if isinstance(x, str):
+            a = abi.Array()
+            self.check(self.lib.tl_tensor_array(self._lookup(x), 1 if write else 0, C.byref(a)), f"{what} {x}")
+            return a.data or 0, a.dtype, tuple(a.dims[:a.rank]), tuple(a.strides[:a.rank])
+        dt = x.dtype
+        t = _type_of.get(dt)
+        if t is None:
+            t = _type_of[dt] = _TYPES.get(str(dt), -1)
+        if t < 0:
+            raise abi.TLError(abi.TL_ERR_INVALID, f"{what}: element type {dt}, not float32, float16 or bfloat16")
+        self._on_device(x, what)
+        return x.data_ptr(), t, tuple(x.shape), x.stride()
+
+    def _on_device(self, x, what):
+        d = x.device
+        if d.type != "cuda" or (d.index or 0) != self.device:
+            raise abi.TLError(abi.TL_ERR_INVALID, f"{what} is on {d}, the context on cuda:{self.device}")
+
+    def _heads(self, buf, field, x, what, write=False):
+        """Packs [heads and positions] of rank 2 to 4 as [batch, heads, positions, head size]."""
+        p, t, shape, strides = self._view(x, what, write)
+        r = len(shape)
+        if r != 4:
+            if r < 2 or r > 4:
+                raise abi.TLError(abi.TL_ERR_INVALID, f"attention: {what} has rank {r}, not 2 to 4")
+            shape, strides = (1,) * (4 - r) + shape, (0,) * (4 - r) + tuple(strides)
+        _ARRAY.pack_into(buf, _ATTENTION_AT[field], p, t, 4, *shape, *strides)
+        return shape
+
+    def _plain(self, x, what, kind, shape):
+        """Address of a contiguous device array of one type and shape (0 for None)."""
+        if x is None:
+            return 0
+        if isinstance(x, str):
+            if kind != "float32":
+                raise abi.TLError(abi.TL_ERR_INVALID, f"{what} is an array of {kind}, not a tensor's name")
+            p, _, have, _ = self._view(x, what, what in ("lse", "norm"))
+        else:
+            self._on_device(x, what)
+            if str(x.dtype).rpartition(".")[2] != kind or not x.is_contiguous():
+                raise abi.TLError(abi.TL_ERR_INVALID, f"{what} is not a contiguous array of {kind}")
+            p, have = x.data_ptr(), tuple(x.shape)
+        n = 1
+        for k in shape:
+            n *= k
+        m = 1
+        for k in have:
+            m *= k
+        if m != n or (len(have) == len(shape) and tuple(have) != tuple(shape)):
+            raise abi.TLError(abi.TL_ERR_INVALID, f"{what} is {have}, not {tuple(shape)}")
+        return p
+
+    def _stream(self, stream):
+        return self.lib.tl_stream(self.h) or 0 if stream is None else stream
+
+    def _room(self, workspace):
+        if workspace is None:
+            return 0, 0
+        self._on_device(workspace, "workspace")
+        if not workspace.is_contiguous():
+            raise abi.TLError(abi.TL_ERR_INVALID, "workspace is not contiguous")
+        return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+    def _attention(self, q, k, v, out, lse, grads, scale, softcap, slopes, causal, prefix_len, q_doc, k_doc, kv_len,
+                   q_start, workspace, stream, writes_out):
+        buf = bytearray(C.sizeof(abi.Attention))
+        b, hq, nq, d = self._heads(buf, "q", q, "q")
+        nk = self._heads(buf, "k", k, "k")[2]
+        self._heads(buf, "v", v, "v")
+        self._heads(buf, "o", out, "out", writes_out)
+        if grads:
+            for f, x in zip(("dout", "dq", "dk", "dv"), grads):
+                self._heads(buf, f, x, f, f != "dout")
+        room = self._room(workspace)
+        one = (b,)
+        if scale is None:
+            scale = d ** -0.5 if d else 1.0
+        _ATTENTION_TAIL.pack_into(
+            buf, _ATTENTION_AT["lse"], self._plain(lse, "lse", "float32", (b, hq, nq)),
+            scale, softcap, 1 if causal else 0, 0,
+            self._plain(slopes, "slopes", "float32", (hq,)), self._plain(prefix_len, "prefix_len", "int32", one),
+            self._plain(q_doc, "q_doc", "int32", (b, nq)), self._plain(k_doc, "k_doc", "int32", (b, nk)),
+            self._plain(kv_len, "kv_len", "int32", one), self._plain(q_start, "q_start", "int32", one),
+            *room, self._stream(stream))
+        return (C.c_char * len(buf)).from_buffer(buf)
+
+    def attention(self, q, k, v, out, lse=None, *, scale=None, softcap=0.0, slopes=None, causal=False, prefix_len=None,
+                  q_doc=None, k_doc=None, kv_len=None, q_start=None, workspace=None, stream=None):
+        """out = softmax(scores) v by head, with capped, biased or masked scores (tl_attention_forward).
+
+        q, out [batch, Hq, Nq, d] and k, v [batch, Hkv, Nk, d] (leading dims of 1 may be left out); out is written.
+        scale: of q.k, d^-0.5 when None.  softcap: scores become softcap tanh(score / softcap).  slopes [Hq]: score
+        minus slope times distance.  causal: a query sees the keys up to its position, and those before
+        prefix_len [batch].  q_doc [batch, Nq], k_doc [batch, Nk]: keys of the query's own document alone, a negative
+        one is padding.  kv_len [batch]: keys of each sequence.  q_start [batch]: position of its first query,
+        kv_len - Nq when None.  lse [batch, Hq, Nq] fp32 receives what the backward pass needs.
+        """
+        d = self._attention(q, k, v, out, lse, None, scale, softcap, slopes, causal, prefix_len, q_doc, k_doc, kv_len,
+                            q_start, workspace, stream, True)
+        self.check(self.lib.tl_attention_forward(self.h, d), "attention")
+        return out
+
+    def attention_backward(self, q, k, v, out, lse, dout, dq, dk, dv, *, scale=None, softcap=0.0, slopes=None,
+                           causal=False, prefix_len=None, q_doc=None, k_doc=None, kv_len=None, q_start=None,
+                           workspace=None, stream=None):
+        """Writes dq, dk, dv, the gradient of sum(out * dout) (tl_attention_backward); out and lse are the forward's."""
+        d = self._attention(q, k, v, out, lse, (dout, dq, dk, dv), scale, softcap, slopes, causal, prefix_len, q_doc,
+                            k_doc, kv_len, q_start, workspace, stream, False)
+        self.check(self.lib.tl_attention_backward(self.h, d), "attention_backward")
+        return dq, dk, dv
+
+    def attention_workspace(self, q, k, v, out, lse=None, grads=None, *, scale=None, softcap=0.0, slopes=None,
+                            causal=False, prefix_len=None, q_doc=None, k_doc=None, kv_len=None, q_start=None):
+        """Bytes of workspace of an attention call, with grads = (dout, dq, dk, dv) of its backward pass."""
+        d = self._attention(q, k, v, out, lse, grads, scale, softcap, slopes, causal, prefix_len, q_doc, k_doc, kv_len,
+                            q_start, None, None, grads is None)
+        n = self.lib.tl_attention_workspace(self.h, d, 1 if grads else 0)
+        self.check(max(0, -n), "attention_workspace")
+        return n
+
+    def _list(self, arrays, what, write):
+        buf = bytearray(_ARRAY.size * len(arrays))
+        at = 0
+        for x in arrays:
+            p, t, shape, strides = self._view(x, what, write)
+            r = len(shape)
+            if r > abi.TL_ARRAY_RANK:
+                if not x.is_contiguous():
+                    raise abi.TLError(abi.TL_ERR_INVALID, f"{what}: rank {r} and not contiguous")
+                shape, strides, r = (x.numel(),), (1,), 1
+            pad = (0,) * (4 - r)
+            _ARRAY.pack_into(buf, at, p, t, r, *shape, *pad, *strides, *pad)
+            at += _ARRAY.size
+        return buf
+
+    def _clip_lists(self, grads, out):
+        if out is not None and len(out) != len(grads):
+            raise abi.TLError(abi.TL_ERR_INVALID, f"clip: {len(out)} outputs for {len(grads)} gradients")
+
+        def at(arrays, what, write):
+            buf = self._list(arrays, what, write) or bytearray(1)
+            return (C.c_char * len(buf)).from_buffer(buf)
+        return at(grads, "gradient", out is None), None if out is None else at(out, "output", True)
+
+    def clip_gradients(self, grads, max_norm, out=None, norm=None, workspace=None, stream=None):
+        """Scales the arrays so that their global norm is at most max_norm (tl_clip_gradients).
+
+        In place, or into the arrays of `out` (same dims and strides, any type).  norm: a device fp32 scalar that
+        receives the norm before the scaling.  Nothing is copied to the host.
+        """
+        a, o = self._clip_lists(grads, out)
+        at = self._plain(norm, "norm", "float32", ())
+        self.check(self.lib.tl_clip_gradients(self.h, a, o, len(grads), max_norm, at, *self._room(workspace),
+                                              self._stream(stream)), "clip_gradients")
+        return grads if out is None else out
+
+    def clip_workspace(self, grads, max_norm, out=None):
+        """Bytes of workspace of a clip_gradients call."""
+        n = self.lib.tl_clip_workspace(self.h, *self._clip_lists(grads, out), len(grads), max_norm)
+        self.check(max(0, -n), "clip_workspace")
+        return n
 
     # ------------------------------------------------------------------ profiling
     def profile(self, on=True):

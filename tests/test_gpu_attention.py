@@ -1,0 +1,455 @@
+"""Attention with modified scores and its gradient against 64-bit formulas (attention_ref)."""
+import numpy as np
+import pytest
+
+from attention_ref import TYPES, check, reference
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    from tensor_logic_lang_b200.runtime import Context
+    c = Context(device=0)
+    yield c
+    c.close()
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def heads(gen, b, h, n, d, dtype, layout="bhsd"):
+    """A [b, h, n, d] array in one of several memory layouts."""
+    t = TYPES[dtype]
+
+    def randn(*shape):
+        return torch.randn(shape, generator=gen, device="cuda").to(t)
+    if layout == "bshd":
+        return randn(b, n, h, d).transpose(1, 2)
+    if layout == "packed":                     # a third of a joint projection
+        return randn(b, n, 3, h, d)[:, :, 1].transpose(1, 2)
+    if layout == "odd":                        # rows of d + 1, the array one element off its allocation
+        return randn(b * h * n * (d + 1) + 1)[1:].view(b, h, n, d + 1)[..., :d]
+    if layout == "dim":                        # head size not the contiguous dim
+        return randn(b, h, d, n).transpose(2, 3)
+    if layout == "broadcast":                  # one head's values for all, in every sequence
+        return randn(1, 1, n, d).expand(b, h, n, d)
+    return randn(b, h, n, d)
+
+
+def like(x, layout):
+    """An array to write in, with what it must not keep, in a layout of its own."""
+    b, h, n, d = x.shape
+    if layout in ("bhsd", "broadcast"):
+        y = torch.empty((b, h, n, d), dtype=x.dtype, device=x.device)
+    elif layout == "odd":
+        y = torch.empty((b, h, n, d + 1), dtype=x.dtype, device=x.device)[..., :d]
+    elif layout == "dim":
+        y = torch.empty((b, h, d, n), dtype=x.dtype, device=x.device).transpose(2, 3)
+    else:
+        y = torch.empty((b, n, h, d), dtype=x.dtype, device=x.device).transpose(1, 2)
+    return y.fill_(float("nan"))
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def modifiers(names, b, hq, nq, nk, seed):
+    rng = np.random.default_rng(seed)
+    m = {}
+    if "cap" in names:
+        m["softcap"] = 1.5                      # bends the scores of these inputs well
+    if "slopes" in names:
+        m["slopes"] = torch.tensor([2.0 ** (-8 * (h + 1) / hq) for h in range(hq)], device="cuda")
+    if "causal" in names or "prefix" in names:
+        m["causal"] = True
+    if "prefix" in names:
+        m["prefix_len"] = ints([int(x) for x in rng.integers(0, nk + 2, b)])
+    if "docs" in names:                         # packed documents, padding between and behind them
+        def row(n):
+            r = np.sort(rng.integers(0, 4, n))
+            r[rng.random(n) < 0.1] = -1
+            return r
+        m["q_doc"] = ints(np.stack([row(nq) for _ in range(b)])) if nq else ints(np.zeros((b, 0)))
+        m["k_doc"] = m["q_doc"] if nq == nk else ints(np.stack([row(nk) for _ in range(b)])) if nk else \
+            ints(np.zeros((b, 0)))
+    if "ids" in names:                          # documents in no order
+        m["q_doc"], m["k_doc"] = ints(rng.integers(-1, 3, (b, nq))), ints(rng.integers(-1, 3, (b, nk)))
+    if "len" in names:                          # from no key to more than there are
+        m["kv_len"] = ints([(0, nk, nk // 2 + 1, nk + 5, 1)[i % 5] for i in range(b)])
+    if "start" in names:
+        m["q_start"] = ints([(0, -3, nk // 2, 2 * nk)[i % 4] for i in range(b)])
+    return m
+
+
+def poison(x, ok):
+    """Infinities and NaN where what an array holds must not matter."""
+    if ok is not None and not bool(ok.all()):
+        bad = torch.where(torch.arange(x.shape[2], device=x.device) % 2 == 0, float("nan"), float("inf")).to(x.dtype)
+        x.copy_(torch.where(ok[:, None, :, None], x, bad[None, None, :, None].expand_as(x)))
+
+
+def run(ctx, q, k, v, dout, m, layout="bhsd", **kw):
+    out = like(q, layout)
+    lse = torch.full(q.shape[:3], float("nan"), device="cuda")
+    ctx.attention(q, k, v, out, lse, stream=stream(), **m, **kw)
+    got = {"out": out, "lse": lse}
+    if dout is not None:
+        got["dq"], got["dk"], got["dv"] = like(q, layout), like(k, layout), like(v, layout)
+        ctx.attention_backward(q, k, v, out, lse, dout, got["dq"], got["dk"], got["dv"], stream=stream(), **m, **kw)
+    torch.cuda.synchronize()
+    ctx.sync()
+    return got
+
+
+def compare(ctx, b, hq, hkv, nq, nk, d, dtype, names="", layout="bhsd", seed=0, backward=True, gain=1.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    q = heads(gen, b, hq, nq, d, dtype, "bhsd" if layout == "broadcast" else layout)
+    if gain != 1.0:
+        q.mul_(gain)
+    k, v = heads(gen, b, hkv, nk, d, dtype, layout), heads(gen, b, hkv, nk, d, dtype, layout)
+    dout = heads(gen, b, hq, nq, d, dtype, "bshd") if backward else None
+    m = modifiers(names, b, hq, nq, nk, seed)
+    if layout != "broadcast":
+        k_ok = torch.ones((b, nk), dtype=torch.bool, device="cuda")
+        if "kv_len" in m:
+            k_ok &= torch.arange(nk, device="cuda")[None] < m["kv_len"][:, None]
+        if "k_doc" in m:
+            k_ok &= m["k_doc"] >= 0
+        poison(k, k_ok)
+        poison(v, k_ok)
+    if "q_doc" in m:
+        poison(q, m["q_doc"] >= 0)
+        if backward:
+            poison(dout, m["q_doc"] >= 0)
+    want = reference(q, k, v, dout, **m)
+    got = run(ctx, q, k, v, dout, m, layout)
+    for n in want:
+        check(got[n], want[n], n)
+    return got
+
+
+MODIFIERS = ["", "cap", "slopes", "causal", "prefix", "docs", "ids", "len", "causal start", "cap slopes causal docs",
+             "cap prefix len start", "slopes docs len"]
+SIZES = [(1, 1, 1, 1, 1, 64), (2, 4, 2, 7, 5, 64), (1, 2, 2, 64, 64, 64), (5, 2, 1, 65, 129, 64),
+         (2, 3, 3, 200, 333, 128), (1, 8, 1, 257, 257, 128), (4, 2, 1, 130, 31, 80), (2, 4, 4, 3, 300, 128),
+         (1, 6, 2, 300, 300, 40)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("names", MODIFIERS)
+def test_modifiers(ctx, names, dtype):
+    for i, size in enumerate(SIZES):
+        compare(ctx, *size, dtype, names, seed=i)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [1, 8, 32, 33, 72, 96, 120, 129, 192, 256])
+def test_head_sizes(ctx, d, dtype):
+    compare(ctx, 2, 2, 1, 70, 90, d, dtype, "cap causal", seed=d)
+    compare(ctx, 2, 2, 2, 2, 90, d, dtype, "slopes len", seed=d)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("layout", ["bshd", "packed", "odd", "dim", "broadcast"])
+def test_layouts(ctx, layout, dtype):
+    for nq in (1, 140):
+        compare(ctx, 2, 4, 2, nq, 140, 64, dtype, "cap causal len", layout, seed=3)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq,nk", [(0, 5), (5, 0), (0, 0)])
+def test_nothing_to_attend(ctx, nq, nk, dtype):
+    got = compare(ctx, 2, 2, 1, nq, nk, 64, dtype)
+    for n in ("out", "dq", "dk", "dv"):
+        assert not got[n].float().any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq,nk", [(1, 4097), (2, 1000), (513, 2050), (1500, 1500)])
+def test_longer(ctx, nq, nk, dtype):
+    compare(ctx, 2, 4, 2, nq, nk, 128, dtype, "cap causal", seed=nq, backward=nk < 2048)
+    compare(ctx, 2, 4, 2, nq, nk, 64, dtype, "slopes docs", seed=nq, backward=nk < 2048)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_large_scores(ctx, dtype):
+    # rows whose largest key has nearly all of the weight, met late in the row
+    compare(ctx, 1, 2, 2, 300, 700, 64, dtype, "", seed=1, gain=6.0)
+    compare(ctx, 1, 2, 2, 1, 700, 64, dtype, "", seed=1, gain=6.0)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_small_gradients(ctx, dtype):
+    # dout far below 1, as without a loss scale: the gradients keep their bits
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    q, k, v = (heads(gen, 1, 2, 400, 64, dtype) for _ in range(3))
+    dout = heads(gen, 1, 2, 400, 64, dtype)
+    small = (dout.float() * 2.0 ** -10).to(dout.dtype)
+    m = {"causal": True}
+    want = reference(q, k, v, dout, **m)
+    got = run(ctx, q, k, v, small, m)
+    for n in ("dq", "dk", "dv"):
+        value, bound = want[n]
+        check(got[n], (value * 2.0 ** -10, bound * 2.0 ** -10 + 2.0 ** -24), n)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gradient_against_differences(ctx, dtype):
+    # sum(out * dout) in 64 bits moves along a direction as the gradients say
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    q, k, v, dout = (heads(gen, 1, 2, 40, 16, dtype) for _ in range(4))
+    m = modifiers("cap slopes causal", 1, 2, 40, 40, 0)
+    got = run(ctx, q, k, v, dout, m)
+    for n, x in (("dq", q), ("dk", k), ("dv", v)):
+        step = torch.randn(x.shape, generator=gen, device="cuda").double()
+        ends = []
+        for sign in (1e-4, -1e-4):
+            moved = {"q": q.double(), "k": k.double(), "v": v.double()}
+            moved[n[1]] = moved[n[1]] + sign * step
+            ends.append((reference(moved["q"], moved["k"], moved["v"], **m)["out"][0] * dout.double()).sum().item())
+        slope = (ends[0] - ends[1]) / 2e-4
+        # differences: 1e-8 of the values; the gradient: its bound summed along the direction
+        bound = (reference(q, k, v, dout, **m)[n][1] * step.abs()).sum().item() + 1e-6 * (1 + abs(slope))
+        assert abs((got[n].double() * step).sum().item() - slope) <= bound
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_runs_repeat_bit_for_bit(ctx, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    for nq in (1, 600):
+        q, dout = heads(gen, 2, 8, nq, 64, dtype), heads(gen, 2, 8, nq, 64, dtype)
+        k, v = heads(gen, 2, 2, 1100, 64, dtype), heads(gen, 2, 2, 1100, 64, dtype)
+        first = run(ctx, q, k, v, dout, {"causal": True, "softcap": 5.0})
+        for _ in range(3):
+            again = run(ctx, q, k, v, dout, {"causal": True, "softcap": 5.0})
+            for n in first:
+                assert torch.equal(first[n], again[n]), n
+
+
+@pytest.mark.parametrize("nq", [1, 200])
+def test_captured_and_replayed(ctx, nq):
+    # two graphs with workspaces of their own, replayed side by side on new values
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    kept = []
+    for i in range(2):
+        q, dout = heads(gen, 2, 4, nq, 64, "bf16"), heads(gen, 2, 4, nq, 64, "bf16")
+        k, v = heads(gen, 2, 2, 2000, 64, "bf16"), heads(gen, 2, 2, 2000, 64, "bf16")
+        out, lse = like(q, "bhsd"), torch.empty(q.shape[:3], device="cuda")
+        g = (dout, like(q, "bhsd"), like(k, "bhsd"), like(v, "bhsd"))
+        m = {"causal": True, "softcap": 4.0}
+        ws = torch.empty(256 + max(ctx.attention_workspace(q, k, v, out, lse, **m),
+                                   ctx.attention_workspace(q, k, v, out, lse, g, **m)), dtype=torch.uint8, device="cuda")
+
+        def step():
+            ctx.attention(q, k, v, out, lse, stream=stream(), workspace=ws, **m)
+            ctx.attention_backward(q, k, v, out, lse, *g, stream=stream(), workspace=ws, **m)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        kept.append((graph, q, k, v, out, lse, g, m))
+    streams = [torch.cuda.Stream() for _ in kept]
+    for _ in range(2):
+        for _, q, k, v, out, lse, g, m in kept:
+            for x in (q, k, v, g[0]):
+                x.copy_(torch.randn(x.shape, generator=gen, device="cuda"))
+        torch.cuda.synchronize()
+        for s, (graph, *_) in zip(streams, kept):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, q, k, v, out, lse, g, m in kept:
+            want = reference(q, k, v, g[0], **m)
+            for n, x in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *g[1:])):
+                check(x, want[n], n)
+
+
+def test_capture_needs_a_workspace(ctx):
+    from tensor_logic_lang_b200 import abi
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    q, k, v, dout = (heads(gen, 1, 2, 64, 64, "bf16") for _ in range(4))
+    got = run(ctx, q, k, v, dout, {})
+    graph = torch.cuda.CUDAGraph()
+    said = []
+    with torch.cuda.graph(graph):
+        q.add_(0)
+        try:
+            ctx.attention_backward(q, k, v, got["out"], got["lse"], dout, got["dq"], got["dk"], got["dv"], stream=stream())
+        except abi.TLError as e:
+            said.append(e)
+    assert said and said[0].status == abi.TL_ERR_INVALID and "capture" in str(said[0])
+
+
+def test_workspace_is_checked(ctx):
+    from tensor_logic_lang_b200 import abi
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    q, k, v, dout = (heads(gen, 1, 2, 64, 64, "bf16") for _ in range(4))
+    got = run(ctx, q, k, v, dout, {})
+    need = ctx.attention_workspace(q, k, v, got["out"], got["lse"], (dout, got["dq"], got["dk"], got["dv"]))
+    room = torch.empty(need + 512, dtype=torch.uint8, device="cuda")
+    off = -room.data_ptr() % 256
+    before = room.clone()
+    for ws in (room[off:off + need - 1], room[off + 1:off + 1 + need]):
+        with pytest.raises(abi.TLError):
+            ctx.attention_backward(q, k, v, got["out"], got["lse"], dout, got["dq"], got["dk"], got["dv"], workspace=ws,
+                                   stream=stream())
+    assert torch.equal(before, room)
+    again = run(ctx, q, k, v, dout, {})
+    ctx.attention_backward(q, k, v, got["out"], got["lse"], dout, got["dq"], got["dk"], got["dv"],
+                           workspace=room[off:off + need], stream=stream())
+    torch.cuda.synchronize()
+    for n in got:
+        assert torch.equal(got[n], again[n])
+    assert torch.equal(before[:off], room[:off]) and torch.equal(before[off + need:], room[off + need:])
+
+
+def test_streams_side_by_side(ctx):
+    # the context keeps a workspace for each stream
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    jobs = []
+    for i in range(4):
+        q, dout = heads(gen, 1, 4, 300, 64, "f16"), heads(gen, 1, 4, 300, 64, "f16")
+        k, v = heads(gen, 1, 2, 500, 64, "f16"), heads(gen, 1, 2, 500, 64, "f16")
+        jobs.append((torch.cuda.Stream(), q, k, v, dout))
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(3):
+        results = []
+        for s, q, k, v, dout in jobs:
+            with torch.cuda.stream(s):
+                out, lse = like(q, "bhsd"), torch.empty(q.shape[:3], device="cuda")
+                g = (like(q, "bhsd"), like(k, "bhsd"), like(v, "bhsd"))
+                ctx.attention(q, k, v, out, lse, causal=True, stream=s.cuda_stream)
+                ctx.attention_backward(q, k, v, out, lse, dout, *g, causal=True, stream=s.cuda_stream)
+                results.append((out, lse, *g))
+    torch.cuda.synchronize()
+    for (s, q, k, v, dout), got in zip(jobs, results):
+        want = reference(q, k, v, dout, causal=True)
+        for n, x in zip(("out", "lse", "dq", "dk", "dv"), got):
+            check(x, want[n], n)
+
+
+def test_refusals_do_nothing(ctx):
+    from tensor_logic_lang_b200 import abi
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    q, k, v = (heads(gen, 1, 2, 64, 64, "bf16") for _ in range(3))
+    out = torch.full_like(q, 7.0)
+    for bad in (dict(q=q.cpu()), dict(out=out.float()), dict(v=v[:, :, 1:]), dict(out=q), dict(k=k[..., :32]),
+                dict(q=q.double()), dict(q=q[0, 0, 0])):
+        with pytest.raises(abi.TLError):
+            ctx.attention(bad.get("q", q), bad.get("k", k), bad.get("v", v), bad.get("out", out), stream=stream())
+    for bad in (dict(softcap=-1.0), dict(prefix_len=ints([3])), dict(q_doc=ints([[0] * 64])), dict(kv_len=ints([1, 2])),
+                dict(kv_len=torch.tensor([3], device="cuda")), dict(slopes=torch.ones(2)),
+                dict(slopes=torch.ones(2, dtype=torch.float64, device="cuda")),
+                dict(q_doc=ints([[0] * 128])[:, ::2], k_doc=ints([[0] * 64]))):
+        with pytest.raises(abi.TLError):
+            ctx.attention(q, k, v, out, stream=stream(), **bad)
+    torch.cuda.synchronize()
+    assert (out == 7.0).all()
+
+
+def test_rows_outside_are_left(ctx):
+    # outputs inside larger buffers: what surrounds them stays
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    for nq, nk in ((1, 100), (100, 100), (130, 130)):
+        q, k, v, dout = heads(gen, 2, 2, nq, 72, "bf16"), heads(gen, 2, 2, nk, 72, "bf16"), \
+            heads(gen, 2, 2, nk, 72, "bf16"), heads(gen, 2, 2, nq, 72, "bf16")
+        rooms = [torch.full((2, 2, n + 3, 80), 7.0, device="cuda", dtype=torch.bfloat16) for n in (nq, nq, nk, nk)]
+        out, dq, dk, dv = (r[:, :, 1:-2, :72] for r in rooms)
+        lse = torch.empty((2, 2, nq), device="cuda")
+        ctx.attention(q, k, v, out, lse, stream=stream())
+        ctx.attention_backward(q, k, v, out, lse, dout, dq, dk, dv, stream=stream())
+        torch.cuda.synchronize()
+        want = reference(q, k, v, dout)
+        for n, x in zip(("out", "dq", "dk", "dv"), (out, dq, dk, dv)):
+            check(x, want[n], n)
+            x.fill_(7.0)
+        for r in rooms:
+            assert (r == 7.0).all()
+
+
+def test_named_tensors(ctx):
+    # the storage of a program's tensors, on the context's own stream
+    from tensor_logic_lang_b200 import lang
+    rng = np.random.default_rng(3)
+    s, e, d = 96, 24, 16
+    data = {n: rng.standard_normal(shape) for n, shape in
+            (("X", (s, e)), ("Wq", (e, d)), ("Wk", (e, d)), ("Wv", (e, d)))}
+    src = "".join(f"domain {n}: {k}\n" for n, k in (("s", s), ("e", e), ("d", d)))
+    src += "".join(f"{n}[{ix}] = 0\nload {n} \"{n}.bin\"\n" for n, ix in (("X", "s,e"), ("Wq", "e,d"), ("Wk", "e,d"), ("Wv", "e,d")))
+    src += "".join(f"{n}[s,d] = X[s,e] W{n.lower()}[e,d]\n" for n in "QKV")
+    ctx.run(lang.Program(src, inputs=data))
+    ctx.create("O", (s, d))
+    ctx.create("Lse", (1, s))
+    ctx.attention("Q", "K", "V", "O", "Lse", causal=True, softcap=30.0)
+    q, k, v = (torch.tensor(ctx.tensor(n), device="cuda", dtype=torch.float32)[None, None] for n in "QKV")
+    want = reference(q, k, v, causal=True, softcap=30.0)
+    check(torch.tensor(ctx.tensor("O"), device="cuda")[None, None], want["out"], "O")
+    check(torch.tensor(ctx.tensor("Lse"), device="cuda")[None], want["lse"], "Lse")
+
+
+def test_training_step_of_a_program(ctx):
+    """Projections and their gradients from a program, attention and its gradient between them, the gradients
+    clipped: the calls as a training step makes them, on the context's stream."""
+    from tensor_logic_lang_b200 import lang
+    rng = np.random.default_rng(4)
+    s, e, d = 80, 32, 32
+    x, w = rng.standard_normal((s, e)), {n: rng.standard_normal((e, d)) / e ** 0.5 for n in ("Wq", "Wk", "Wv")}
+    g_out = rng.standard_normal((s, d))
+    doms = "".join(f"domain {n}: {k}\n" for n, k in (("s", s), ("e", e), ("d", d)))
+    src = doms + "X[s,e] = 0\nload X \"x\"\n"
+    src += "".join(f"W{n}[e,d] = 0\nload W{n} \"{n}\"\n{n.upper()}[s,d] = X[s,e] W{n}[e,d]\n" for n in "qkv")
+    ctx.run(lang.Program(src, inputs=dict(w, X=x)))
+    for n, shape in (("O", (s, d)), ("Lse", (1, s)), ("dO", (s, d)), ("dQ", (s, d)), ("dK", (s, d)), ("dV", (s, d))):
+        ctx.create(n, shape)
+    ctx.upload("dO", g_out)
+    m = dict(causal=True, softcap=20.0)
+    ctx.attention("Q", "K", "V", "O", "Lse", **m)
+    ctx.attention_backward("Q", "K", "V", "O", "Lse", "dO", "dQ", "dK", "dV", **m)
+    back = {n: ctx.tensor(n) for n in ("dQ", "dK", "dV")}
+    src = doms + "X[s,e] = 0\nload X \"x\"\n"
+    src += "".join(f"G{n}[s,d] = 0\nload G{n} \"{n}\"\nd{n}[e,d] = X[s,e] G{n}[s,d]\n" for n in "QKV")
+    ctx.run(lang.Program(src, inputs={"X": x, "GQ": back["dQ"], "GK": back["dK"], "GV": back["dV"]}))
+    ctx.create("Norm", (1,))
+    before = {n: ctx.tensor(n) for n in ("dQ", "dK", "dV")}
+    ctx.clip_gradients(["dQ", "dK", "dV"], 0.5, norm="Norm")
+    # the same in 64 bits
+    X = torch.tensor(x, device="cuda")
+    leaf = {n: torch.tensor(v, device="cuda") for n, v in w.items()}
+    q, k, v = (X @ leaf[n] for n in ("Wq", "Wk", "Wv"))
+    ref = reference(q[None, None], k[None, None], v[None, None], torch.tensor(g_out, device="cuda")[None, None], **m)
+    grads = {n: X.T @ ref[n.lower()][0][0, 0] for n in ("dQ", "dK", "dV")}
+    norm = torch.sqrt(sum((t ** 2).sum() for t in grads.values())).item()
+    assert norm > 0.5
+    assert abs(ctx.tensor("Norm")[0] - norm) <= 1e-4 * norm
+    for n, t in grads.items():
+        t = t.cpu().numpy()
+        assert np.abs(before[n] - t).max() <= 1e-3 * np.abs(t).max()
+        assert np.abs(ctx.tensor(n) - t * (0.5 / norm)).max() <= 1e-3 * np.abs(t).max() * 0.5 / norm
+
+
+def test_second_device():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    from tensor_logic_lang_b200.runtime import Context
+    c = Context(device=1)
+    try:
+        torch.cuda.set_device(0)
+        gen = torch.Generator(device="cuda").manual_seed(1)
+        q, k, v = (heads(gen, 1, 2, 70, 64, "bf16").to("cuda:1") for _ in range(3))
+        out = torch.empty_like(q)
+        torch.cuda.synchronize(1)
+        c.attention(q, k, v, out, causal=True)
+        c.sync()
+        assert torch.cuda.current_device() == 0
+        check(out, reference(q, k, v, causal=True)["out"], "out")
+    finally:
+        c.close()
