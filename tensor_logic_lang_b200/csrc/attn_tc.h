@@ -1,0 +1,293 @@
+// Device pieces shared by the tensor-core attention kernels (16-bit operands,
+// head size up to 128).
+//
+// Operand tiles are 128 rows of one head in shared memory as one or two
+// chunks of 64 columns (16 KB each, 128-byte swizzle), which TMA writes from a
+// [batch, heads, positions, head size] tensor map; rows past the array and
+// columns past the head size arrive as zeros.  The same tile is a K-major
+// operand (the head size contracted: q k^T, dout v^T) and an MN-major one (the
+// rows contracted: p v, dx k, p^T dout, dx^T q).
+#pragma once
+
+#include "attention.h"
+#include "tc_ptx.h"
+
+namespace tl {
+
+constexpr int TILE = 128;                 // queries or keys of a tile
+constexpr int CHUNK_BYTES = TILE * 128;   // 64 columns of a tile
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// fp16 probabilities are written 2^6 times larger: the smallest ones keep
+// more bits (fp16 ends at 2^-24), and with the lazy rescaling's 2^8 they stay
+// below 2^15.
+template <typename T> struct Lift { static constexpr float log2 = 0.f; };
+template <> struct Lift<__half> { static constexpr float log2 = 6.f; };
+
+// ---------------------------------------------------------------- tcgen05
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 columns of the warp's 32 lanes; the values are there after tmem_wait_ld
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+          "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+          "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+// Instruction descriptor of kind::f16: fp32 sums, A and B of one 16-bit type,
+// A K-major, M = 128.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t f16_idesc(int n, bool b_mn) {
+    const uint32_t t = TypeOf<T>::id == TL_TYPE_BF16 ? 1u : 0u;
+    return (1u << 4) | (t << 7) | (t << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(TILE >> 4) << 24);
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+// D[128 x 128] = A B^T over the head size (ksteps of 16), both K-major tiles.
+template <typename T>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, int ksteps) {
+    constexpr uint32_t idesc = f16_idesc<T>(TILE, false);
+    for (int k = 0; k < ksteps; ++k) {
+        const uint32_t at = (k >> 2) * CHUNK_BYTES + (k & 3) * 32;
+        umma_f16_ss(d, umma_desc(a + at, 16, 1024, kLayoutSW128), umma_desc(b + at, 16, 1024, kLayoutSW128), idesc,
+                    k > 0);
+    }
+}
+// D[128 x n] (+)= A B: A 128 x 128 16-bit in TMEM (two columns of it to a TMEM
+// column), B the tile's 128 rows as contracted index.
+template <typename T>
+__device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+#pragma unroll
+    for (int k = 0; k < TILE / 16; ++k)
+        umma_f16_ts(d, a + 8 * k, umma_desc(b + k * 2048, CHUNK_BYTES, 1024, kLayoutSW128), idesc, accumulate | (k > 0));
+}
+
+// ---------------------------------------------------------------- TMA
+// One head's rows in a 4-D map; strides of 0 and dims of 1 take coordinate 0.
+struct HeadMap {
+    CUtensorMap map;
+    int mh, mb;   // 1, or 0 where every head (sequence) is the same memory
+};
+__device__ __forceinline__ void tma_tile(uint32_t dst, const HeadMap& m, uint64_t* bar, int chunks, int row, int h, int b) {
+    for (int c = 0; c < chunks; ++c)
+        asm volatile(
+            "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+            ::"r"(dst + c * CHUNK_BYTES),
+            "l"(reinterpret_cast<uint64_t>(&m.map)), "r"(smem_u32(bar)), "r"(64 * c), "r"(row), "r"(h * m.mh), "r"(b * m.mb)
+            : "memory");
+}
+
+// ---------------------------------------------------------------- packed fp32
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2(float lo, float hi) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(f2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+template <typename T> __device__ __forceinline__ uint32_t pack16(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <> __device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// ---------------------------------------------------------------- capped scores
+// softcap tanh(x / softcap) for |x| <= softcap as x P((x / softcap)^2): P is
+// the polynomial of degree 4 that has the least largest relative error for
+// tanh(u) / u on u^2 in [0, 1] (a linear programme over a Chebyshev grid
+// gives it): 6.9e-6, far below the rounding of a 16-bit probability.  Tiles
+// that hold a larger score take tanh u = 1 - 2 / (1 + e^2u).
+constexpr float kTanh0 = 0.999993085861206f, kTanh1 = -0.3329806625843048f, kTanh2 = 0.13036811351776123f,
+                kTanh3 = -0.04481755569577217f, kTanh4 = 0.009036424569785595f;
+
+struct CapCoef {
+    float limit;       // largest |q.k| of the polynomial
+    float k2;          // (scale / softcap)^2
+    float mul;         // scale log2 e
+    float wide;        // 2 log2(e) scale / softcap: 2u in base 2
+    float top;         // softcap log2 e
+};
+__device__ __forceinline__ CapCoef cap_coef(float scale, float cap) {
+    CapCoef c;
+    c.limit = cap / scale;
+    c.k2 = (scale / cap) * (scale / cap);
+    c.mul = scale * kLog2e;
+    c.wide = 2.f * kLog2e * scale / cap;
+    c.top = cap * kLog2e;
+    return c;
+}
+__device__ __forceinline__ float wide_tanh(float x, float wide) { return 1.f - __fdividef(2.f, 1.f + ex2(x * wide)); }
+// tanh(u) / u of a pair of scores within the limit
+__device__ __forceinline__ f2 tanh_ratio(f2 x, f2 k2) {
+    const f2 z = mul2(mul2(x, x), k2);
+    f2 r = fma2(z, pack2(kTanh4, kTanh4), pack2(kTanh3, kTanh3));
+    r = fma2(r, z, pack2(kTanh2, kTanh2));
+    r = fma2(r, z, pack2(kTanh1, kTanh1));
+    return fma2(r, z, pack2(kTanh0, kTanh0));
+}
+
+// ---------------------------------------------------------------- documents
+// Smallest and largest document of a tile of positions (padding apart: none
+// gives lo > hi), and whether it holds padding.
+struct DocRange {
+    int lo, hi, pad, _unused;
+};
+__device__ __forceinline__ DocRange no_docs() { return {0x7fffffff, -1, 0, 0}; }
+__device__ __forceinline__ bool docs_meet(const DocRange& a, const DocRange& b) { return a.lo <= b.hi && b.lo <= a.hi && a.lo <= a.hi && b.lo <= b.hi; }
+__device__ __forceinline__ bool docs_one(const DocRange& a, const DocRange& b) { return a.lo == a.hi && b.lo == b.hi && a.lo == b.lo && !a.pad && !b.pad; }
+
+// The tiles of [begin, end) that a block has to visit, 32 at a time: ballots
+// over a lane per tile.  Every warp of a block walks the same list.
+struct TileWalk {
+    int base, end;
+    int clear_lo, clear_hi;       // tiles within need no mask of positions
+    const DocRange* ranges;       // documents of the tiles, or null
+    DocRange mine;                // documents of the block's own rows
+    uint32_t active, masked;
+    int lane;
+    __device__ __forceinline__ void fill() {
+        const int t = base + lane;
+        bool on = t < end, mk = t < clear_lo || t >= clear_hi;
+        if (ranges && on) {
+            const int4 r4 = __ldg(reinterpret_cast<const int4*>(ranges) + t);
+            const DocRange r = {r4.x, r4.y, r4.z, 0};
+            on = docs_meet(mine, r);
+            mk = mk || !docs_one(mine, r);
+        }
+        active = __ballot_sync(0xffffffffu, on);
+        masked = __ballot_sync(0xffffffffu, mk);
+    }
+    __device__ __forceinline__ void start(int begin, int end_, int lo, int hi, const DocRange* r, const DocRange& m) {
+        base = begin; end = end_; clear_lo = lo; clear_hi = hi; ranges = r; mine = m;
+        lane = threadIdx.x & 31;
+        active = masked = 0;
+        if (base < end) fill();
+    }
+    // the next tile (-1: none), by all lanes of a warp together
+    __device__ __forceinline__ int next(bool* mask) {
+        while (!active) {
+            base += 32;
+            if (base >= end) return -1;
+            fill();
+        }
+        const int bit = __ffs(active) - 1;
+        active &= active - 1;
+        *mask = (masked >> bit) & 1;
+        return base + bit;
+    }
+};
+
+// Bits of the 128 other positions whose document is `doc`, lane by lane: the
+// lane holds the documents of positions lane, 32 + lane, ... in other[4] and
+// wants its own row's doc.  The distinct documents of a warp's rows are few
+// (one ballot each).
+__device__ __forceinline__ void doc_bits(const int (&other)[4], int doc, uint32_t (&bits)[4]) {
+    uint32_t left = 0xffffffffu;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) bits[w] = 0;
+    while (left) {
+        const int d = __shfl_sync(0xffffffffu, doc, __ffs(left) - 1);
+        const bool mine = doc == d;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t m = __ballot_sync(0xffffffffu, other[w] == d && d >= 0);
+            if (mine) bits[w] = m;
+        }
+        left &= ~__ballot_sync(0xffffffffu, mine);
+    }
+}
+// the low n bits of word w of a 128-bit row
+__device__ __forceinline__ uint32_t low_bits(int n, int w) {
+    const int k = n - 32 * w;
+    return k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1;
+}
+
+// Zeros over the rows of a tile that must not count (a warp; the caller
+// fences before the tensor cores read the tile).
+template <typename F>
+__device__ __forceinline__ void clear_rows(uint8_t* tile, int chunks, F bad) {
+    const int lane = threadIdx.x & 31;
+    for (int r = lane; r < TILE; r += 32)
+        if (bad(r))
+            for (int c = 0; c < chunks; ++c)
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    *reinterpret_cast<uint4*>(tile + c * CHUNK_BYTES + r * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
+}
+
+// host: the tensor map of one array (k_attention_tc.cu)
+bool make_head_map(HeadMap* m, const HeadsView& v, int dtype, int b, int h, int64_t n, int d);
+// the arrays a tensor-core kernel takes: 16-bit, head size contiguous, 16-byte
+// aligned rows
+bool tc_array(const HeadsView& v, int b, int h, int64_t n);
+
+}  // namespace tl

@@ -1,0 +1,529 @@
+// Attention forward on the tensor cores: 16-bit operands, head size up to
+// 128, one pass over the keys with a running maximum and sum.
+//
+// A block owns two tiles of 128 queries that read the same keys: the same
+// rows of two heads of a group where the group has an even number of heads
+// (each causal tile then needs exactly the keys the block loads), else
+// neighbouring rows of one head.  Warps:
+//   0-3, 4-7  one query row per thread of tile 0, 1: scores out of TMEM,
+//             softmax statistics, probabilities (16-bit) back into TMEM over
+//             the scores
+//   8         tensor cores: S = Q K^T (SMEM x SMEM), O += P V (TMEM x SMEM)
+//   9         TMA: Q once, then K and V tiles through a ring of four
+// TMEM: S0 S1 (128 columns each, P over their first half), O0 O1.  While one
+// tile's softmax runs, the other tile's products do; S of the next keys is
+// issued right behind P V of these, which orders it after P is read.
+//
+// With m the row's reference maximum, p = 2^(s log2 e - m): O is rescaled only
+// when a row's maximum has grown by more than 2^8 (fp32 sums and 16-bit p have
+// the range), so most tiles touch O not at all.  l sums the unrounded p.
+// P is rounded to the operand type: the tensor cores take 16-bit operands;
+// each p is off by half a step, which weighs like the rounding of v.
+#include <algorithm>
+
+#include "attn_tc.h"
+
+namespace tl {
+namespace {
+
+constexpr int FW_THREADS = 384, FW_STAGES = 4;
+constexpr float kGrow = 8.f;   // rescale when the maximum grew by 2^8
+
+struct FwArgs {
+    AttnCall a;
+    const DocRange* k_ranges;   // [b, key tiles] with documents
+    int pair_heads;             // the block's tiles: heads h, h + 1 (else rows i0, i0 + 128)
+    int key_tiles;
+    int* err;
+};
+
+template <int DP>
+struct FwSmem {
+    static constexpr int CH = DP / 64, TILE_B = CH * CHUNK_BYTES;
+    static constexpr int Q = 0, KV = 2 * TILE_B, BAR = KV + FW_STAGES * TILE_B, DOCS = BAR + 256,
+                         BYTES = DOCS + 64 + 1024;
+};
+
+// the smallest / largest document of each tile of 128 keys (queries), a warp per tile
+__global__ void __launch_bounds__(256) k_doc_ranges(const int32_t* __restrict__ doc, int n, int tiles, int64_t total,
+                                                    DocRange* __restrict__ out) {
+    const int lane = threadIdx.x & 31;
+    const int64_t t = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+    if (t >= total) return;
+    const int64_t b = t / tiles;
+    const int j0 = (int)(t % tiles) * TILE;
+    DocRange r = no_docs();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int j = j0 + 32 * w + lane;
+        const int d = j < n ? doc[b * n + j] : -1;
+        if (d >= 0) { r.lo = min(r.lo, d); r.hi = max(r.hi, d); }
+        else r.pad = 1;
+    }
+    r.lo = __reduce_min_sync(0xffffffffu, r.lo);
+    r.hi = __reduce_max_sync(0xffffffffu, r.hi);
+    r.pad = __reduce_max_sync(0xffffffffu, r.pad);
+    if (lane == 0) out[t] = r;
+}
+
+// One tile of scores of this thread's row: x (q.k) in registers becomes the
+// score in base 2 times c (see below), with -inf where the key is not seen.
+// Returns the row's largest c-scaled score.
+//   !CAP && !BIAS: x is left as it is and c = scale log2 e; else c = 1.
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ float score_row(f2 (&x)[TILE / 2], float c1, const CapCoef& cap, float slope2, int p, int j0,
+                                           bool masked, const uint32_t (&bits)[4]) {
+    if (CAP) {
+        float big = 0.f;
+#pragma unroll
+        for (int i = 0; i < TILE / 2; ++i) {
+            float lo, hi;
+            unpack2(x[i], lo, hi);
+            big = fmaxf(big, fmaxf(fabsf(lo), fabsf(hi)));
+        }
+        if (__any_sync(0xffffffffu, !(big <= cap.limit))) {
+#pragma unroll
+            for (int i = 0; i < TILE / 2; ++i) {
+                float lo, hi;
+                unpack2(x[i], lo, hi);
+                x[i] = pack2(cap.top * wide_tanh(lo, cap.wide), cap.top * wide_tanh(hi, cap.wide));
+            }
+        } else {
+            const f2 k2 = pack2(cap.k2, cap.k2), mul = pack2(cap.mul, cap.mul);
+#pragma unroll
+            for (int i = 0; i < TILE / 2; ++i) x[i] = mul2(mul2(x[i], mul), tanh_ratio(x[i], k2));
+        }
+    }
+    if (BIAS) {
+        // -slope |p - j| is linear in j on either side of p
+        const bool before = __all_sync(0xffffffffu, j0 + TILE - 1 <= p), after = __all_sync(0xffffffffu, j0 >= p);
+        const f2 c = CAP ? pack2(1.f, 1.f) : pack2(c1, c1);
+        if (before || after) {
+            const float k = before ? slope2 : -slope2, kb = k * (float)(j0 - p);
+            const f2 kk = pack2(k, k), base = pack2(kb, kb);
+#pragma unroll
+            for (int i = 0; i < TILE / 2; ++i) {
+                const f2 bias = fma2(kk, pack2((float)(2 * i), (float)(2 * i + 1)), base);
+                x[i] = CAP ? add2(x[i], bias) : fma2(x[i], c, bias);
+            }
+        } else {
+            const float at = (float)(j0 - p);
+#pragma unroll
+            for (int i = 0; i < TILE / 2; ++i) {
+                const f2 bias = pack2(-slope2 * fabsf(at + (float)(2 * i)), -slope2 * fabsf(at + (float)(2 * i + 1)));
+                x[i] = CAP ? add2(x[i], bias) : fma2(x[i], c, bias);
+            }
+        }
+    }
+    if (masked) {
+#pragma unroll
+        for (int i = 0; i < TILE / 2; ++i) {
+            float lo, hi;
+            unpack2(x[i], lo, hi);
+            const uint32_t w = bits[i / 16];
+            lo = (w >> (2 * i % 32)) & 1 ? lo : -INFINITY;
+            hi = (w >> (2 * i % 32 + 1)) & 1 ? hi : -INFINITY;
+            x[i] = pack2(lo, hi);
+        }
+    }
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < TILE / 2; ++i) {
+        float lo, hi;
+        unpack2(x[i], lo, hi);
+        top[i % 4] = fmaxf(top[i % 4], fmaxf(lo, hi));
+    }
+    return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(FW_THREADS, 1)
+    k_attn_tc(const __grid_constant__ HeadMap mq, const __grid_constant__ HeadMap mk, const __grid_constant__ HeadMap mv,
+              const __grid_constant__ FwArgs g) {
+    using L = FwSmem<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::BAR);
+    uint64_t *q_full = bar, *full = bar + 1, *empty = full + FW_STAGES, *s_full = empty + FW_STAGES, *p_full = s_full + 2,
+             *o_done = p_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 24);
+    int* docs = reinterpret_cast<int*>(smem + L::DOCS);   // lo, hi, pad of the block's rows
+    const AttnCall& a = g.a;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+
+    // block -> (rows, heads, sequence); the last rows, which see the most keys
+    // of a causal call, go first
+    const int group = a.hq / a.hkv;
+    const int units = g.pair_heads ? a.hq / 2 : a.hq;
+    const int span = g.pair_heads ? TILE : 2 * TILE;
+    const int row_blocks = (a.nq + span - 1) / span;
+    const unsigned per_row = (unsigned)units * a.b;
+    const int rb = row_blocks - 1 - (int)(blockIdx.x / per_row);
+    const unsigned u = blockIdx.x % per_row;
+    const int b = u / units, h0 = (u % units) * (g.pair_heads ? 2 : 1), kvh = h0 / group;
+    const int i0 = rb * span, rows = min(span, a.nq - i0);
+    const SeqMask mask(a, b);
+    const int32_t* qd = a.q_doc ? a.q_doc + (int64_t)b * a.nq : nullptr;
+    const int32_t* kd = a.k_doc ? a.k_doc + (int64_t)b * a.nk : nullptr;
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        for (int s = 0; s < FW_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&p_full[t], TILE); mbar_init(&o_done[t], 1); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        docs[0] = 0x7fffffff; docs[1] = -1; docs[2] = 0;
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (warp == 9 && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mq.map)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mk.map)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mv.map)) : "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    DocRange mine = no_docs();
+    if (qd) {
+        const int r = threadIdx.x;
+        const int d = r < rows ? qd[i0 + r] : -1;
+        const int lo = __reduce_min_sync(0xffffffffu, d >= 0 ? d : 0x7fffffff), hi = __reduce_max_sync(0xffffffffu, d);
+        const int pad = __any_sync(0xffffffffu, d < 0);
+        if (lane == 0) {
+            atomicMin(&docs[0], lo);
+            atomicMax(&docs[1], hi);
+            if (pad && warp * 32 < rows) docs[2] = 1;
+        }
+        __syncthreads();
+        mine = {docs[0], docs[1], docs[2], 0};
+    }
+    TileWalk walk;
+    {
+        const int end = (max(mask.key_end(i0, rows), 0) + TILE - 1) / TILE;
+        // every row sees the keys that the first one sees
+        const int clear = max(mask.key_end(i0, 1), 0) / TILE;
+        walk.start(0, end, 0, clear, kd ? g.k_ranges + (int64_t)b * g.key_tiles : nullptr, mine);
+    }
+    bool masked, ok = true;
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 9) {
+            // ------------------------------------------------ TMA
+            int kt = walk.next(&masked);
+            int n = 0;   // ring entries filled
+            if (kt >= 0 && lane == 0) {
+                mbar_expect_tx(q_full, 2 * L::TILE_B);
+                for (int t = 0; t < 2; ++t)
+                    tma_tile(smem_u32(smem + L::Q + t * L::TILE_B), mq, q_full, L::CH, i0 + (g.pair_heads ? 0 : t * TILE),
+                             h0 + (g.pair_heads ? t : 0), b);
+            }
+            for (; kt >= 0 && ok; kt = walk.next(&masked)) {
+                for (int w = 0; w < 2 && ok; ++w, ++n) {
+                    const int s = n % FW_STAGES;
+                    ok = n < FW_STAGES || mbar_wait(&empty[s], ((n / FW_STAGES) & 1) ^ 1, g.err);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (ok && lane == 0) {
+                        mbar_expect_tx(&full[s], L::TILE_B);
+                        tma_tile(smem_u32(smem + L::KV + s * L::TILE_B), w ? mv : mk, &full[s], L::CH, kt * TILE, kvh, b);
+                    }
+                }
+            }
+            if (!ok)   // copies in flight land before the block ends
+                for (int e = max(0, n - FW_STAGES); e < n - 1; ++e) mbar_wait(&full[e % FW_STAGES], (e / FW_STAGES) & 1, g.err);
+        } else if (warp == 8) {
+            // ------------------------------------------------ tensor cores
+            const int ksteps = (a.d + 15) / 16;
+            const uint32_t idesc_o = f16_idesc<T>(16 * ksteps, true);
+            int kt = walk.next(&masked);
+            int n = 0;
+            auto wait_full = [&](uint64_t* bars, int i, int stages) {
+                ok = ok && mbar_wait(&bars[i % stages], (i / stages) & 1, g.err);
+                ok = __all_sync(0xffffffffu, ok);
+                tc_fence_after();
+            };
+            auto scores = [&](int t, int stage) {
+                if (ok && lane == 0) {
+                    mma_rows<T>(tmem + t * TILE, smem_u32(smem + L::Q + t * L::TILE_B),
+                                smem_u32(smem + L::KV + stage * L::TILE_B), ksteps);
+                    umma_commit(&s_full[t]);
+                }
+                __syncwarp();
+            };
+            if (kt >= 0) {
+                wait_full(q_full, 0, 1);
+                wait_full(full, n, FW_STAGES);
+                scores(0, n % FW_STAGES);
+                scores(1, n % FW_STAGES);
+                if (ok && lane == 0) umma_commit(&empty[n % FW_STAGES]);
+                ++n;
+            }
+            for (int it = 0; kt >= 0 && ok; ++it) {
+                const int vs = n % FW_STAGES;
+                wait_full(full, n, FW_STAGES);
+                ++n;
+                // rows of V that must not count: 0 probability times what they hold could be NaN
+                if (ok && ((kd && masked) || (mask.kv < a.nk && (kt + 1) * TILE > mask.kv))) {
+                    clear_rows(smem + L::KV + vs * L::TILE_B, L::CH, [&](int r) {
+                        const int j = kt * TILE + r;
+                        return j >= mask.kv || (kd && kd[j] < 0);
+                    });
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                bool next_masked;
+                const int next = walk.next(&next_masked);
+                for (int t = 0; t < 2; ++t) {
+                    ok = ok && mbar_wait(&p_full[t], it & 1, g.err);
+                    ok = __all_sync(0xffffffffu, ok);
+                    tc_fence_after();
+                    if (ok && lane == 0) {
+                        mma_cols<T>(tmem + 2 * TILE + t * DP, tmem + t * TILE, smem_u32(smem + L::KV + vs * L::TILE_B), idesc_o,
+                                    it > 0);
+                        if (next < 0) umma_commit(&o_done[t]);
+                    }
+                    __syncwarp();
+                    if (next >= 0) {
+                        if (t == 0) wait_full(full, n, FW_STAGES);
+                        scores(t, n % FW_STAGES);
+                    }
+                }
+                if (ok && lane == 0) {
+                    umma_commit(&empty[vs]);
+                    if (next >= 0) umma_commit(&empty[n % FW_STAGES]);
+                }
+                __syncwarp();
+                if (next >= 0) ++n;
+                kt = next;
+                masked = next_masked;
+            }
+        }
+    } else {
+        // ---------------------------------------------------- a row per thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int t = warp / 4, r = threadIdx.x % TILE;
+        const int i = i0 + r + (g.pair_heads ? 0 : t * TILE), h = h0 + (g.pair_heads ? t : 0);
+        const int p = mask.p0 + i, limit = mask.key_end(i, 1);
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + t * TILE + lanes, to = tmem + 2 * TILE + t * DP + lanes;
+        const float c1 = a.scale * kLog2e, c = CAP || BIAS ? 1.f : c1;
+        const CapCoef cap = cap_coef(a.scale, CAP ? a.cap : 1.f);
+        const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
+        const int doc = qd && i < a.nq ? qd[i] : -1;
+        float m = -INFINITY, l = 0.f;
+        int it = 0;
+        for (int kt = walk.next(&masked); kt >= 0; kt = walk.next(&masked), ++it) {
+            const int j0 = kt * TILE;
+            uint32_t bits[4];
+            if (masked) {
+                if (kd) {
+                    int other[4];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int j = j0 + 32 * w + lane;
+                        other[w] = j < a.nk ? __ldg(kd + j) : -1;
+                    }
+                    doc_bits(other, doc, bits);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) bits[w] &= low_bits(limit - j0, w);
+                } else {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) bits[w] = low_bits(limit - j0, w);
+                }
+            }
+            ok = ok && mbar_wait(&s_full[t], it & 1, g.err);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc_fence_after();
+            f2 x[TILE / 2];
+            {
+                uint32_t raw[TILE];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tmem_ld32(ts + 32 * k, raw + 32 * k);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < TILE / 2; ++k) x[k] = pack2(__uint_as_float(raw[2 * k]), __uint_as_float(raw[2 * k + 1]));
+            }
+            const float top = c * score_row<CAP, BIAS>(x, c1, cap, slope2, p, j0, masked, bits);
+            // a new reference maximum, for the first seen key of a row or a large step
+            if (__any_sync(0xffffffffu, top > m + kGrow || (m == -INFINITY && top > m))) {
+                const float nm = fmaxf(m, top);
+                const float by = nm == -INFINITY ? 1.f : ex2(m - nm);
+                l *= by;
+                m = nm;
+                if (it > 0) {
+                    const f2 by2 = pack2(by, by);
+                    for (int k = 0; k < DP / 32; ++k) {
+                        uint32_t o[32];
+                        tmem_ld32(to + 32 * k, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) {
+                            float lo, hi;
+                            unpack2(mul2(pack2(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1])), by2), lo, hi);
+                            o[2 * q] = __float_as_uint(lo);
+                            o[2 * q + 1] = __float_as_uint(hi);
+                        }
+                        tmem_st32(to + 32 * k, o);
+                    }
+                }
+            }
+            // p = 2^(c x - m), -inf gives 0; a row with no key yet keeps m = 0 here
+            const float ref = (m == -INFINITY ? 0.f : m) - Lift<T>::log2;
+            const f2 c2 = pack2(c, c), ref2 = pack2(-ref, -ref);
+            f2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t out[16];
+#pragma unroll
+                for (int q = 0; q < 16; ++q) {
+                    float lo, hi;
+                    unpack2(CAP || BIAS ? add2(x[16 * k + q], ref2) : fma2(x[16 * k + q], c2, ref2), lo, hi);
+                    lo = ex2(lo);
+                    hi = ex2(hi);
+                    sum[q & 1] = add2(sum[q & 1], pack2(lo, hi));
+                    out[q] = pack16<T>(lo, hi);
+                }
+                tmem_st16(ts + 16 * k, out);
+            }
+            {
+                float lo, hi;
+                unpack2(add2(sum[0], sum[1]), lo, hi);
+                l += lo + hi;
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&p_full[t]);
+        }
+        // ---------------------------------------------------- o = O / l, lse
+        if (it > 0 && ok) {
+            ok = mbar_wait(&o_done[t], 0, g.err);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+        }
+        const bool none = it == 0 || l == 0.f;   // no key seen
+        const float inv = none ? 0.f : 1.f / l;
+        if (ok) {
+            T* row = static_cast<T*>(a.o.p) + b * a.o.sb + h * a.o.sh + i * a.o.ss;
+            for (int k = 0; k < DP / 32; ++k) {
+                uint32_t o[32];
+                if (it > 0) {
+                    tmem_ld32(to + 32 * k, o);
+                    tmem_wait_ld();
+                }
+                if (i < a.nq)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if (32 * k + 8 * q >= a.d) break;
+                        uint32_t v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            v[e] = none ? 0u : pack16<T>(__uint_as_float(o[8 * q + 2 * e]) * inv,
+                                                         __uint_as_float(o[8 * q + 2 * e + 1]) * inv);
+                        *reinterpret_cast<uint4*>(row + 32 * k + 8 * q) = make_uint4(v[0], v[1], v[2], v[3]);
+                    }
+            }
+            if (a.lse && i < a.nq)
+                a.lse[((int64_t)b * a.hq + h) * a.nq + i] = none ? -INFINITY : (m - Lift<T>::log2) * kLn2 + logf(l);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    }
+}
+
+template <typename T, int DP, bool CAP, bool BIAS>
+tl_status launch(tl_ctx* c, const HeadMap& mq, const HeadMap& mk, const HeadMap& mv, const FwArgs& g, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    constexpr int smem = FwSmem<DP>::BYTES;
+    TL_TRY(kernel_smem(c, k_attn_tc<T, DP, CAP, BIAS>, smem, done));
+    const AttnCall& a = g.a;
+    const int span = g.pair_heads ? TILE : 2 * TILE;
+    const int64_t grid = (int64_t)a.b * (g.pair_heads ? a.hq / 2 : a.hq) * ((a.nq + span - 1) / span);
+    cudaEvent_t ev[2];
+    launch_begin_on(c, s, "attention_tc", 0, 4.0 * a.d * attn_pairs(a), ev);
+    k_attn_tc<T, DP, CAP, BIAS><<<(unsigned)grid, FW_THREADS, smem, s>>>(mq, mk, mv, g);
+    return launch_end_on(c, s, ev);
+}
+
+}  // namespace
+
+bool tc_array(const HeadsView& v, int b, int h, int64_t n) {
+    auto fits = [](int64_t count, int64_t stride) { return count <= 1 || (stride % 8 == 0 && stride < (int64_t(1) << 38)); };
+    return v.sd == 1 && reinterpret_cast<uintptr_t>(v.p) % 16 == 0 && fits(n, v.ss) && v.ss != 0 && fits(h, v.sh) && fits(b, v.sb);
+}
+
+bool attn_tc_takes(const AttnCall& a) {
+    // positions within an int32 tile coordinate; a scale that keeps the order of
+    // the scores (the row maximum is taken before scaling)
+    return a.dtype != TL_TYPE_F32 && a.d % 8 == 0 && a.d <= 128 && a.scale > 0.f && tc_array(a.q, a.b, a.hq, a.nq) &&
+           tc_array(a.k, a.b, a.hkv, a.nk) && tc_array(a.v, a.b, a.hkv, a.nk) && tc_array(a.o, a.b, a.hq, a.nq) && a.nk > 0;
+}
+
+bool make_head_map(HeadMap* m, const HeadsView& v, int dtype, int b, int h, int64_t n, int d) {
+    typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode enc = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool got = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                         q == cudaDriverEntryPointSuccess;
+        return reinterpret_cast<Encode>(got ? p : nullptr);
+    }();
+    if (!enc) return false;
+    // a dim of 1, or one whose stride is 0, is mapped as one element
+    m->mh = h > 1 && v.sh != 0;
+    m->mb = b > 1 && v.sb != 0;
+    cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)n, m->mh ? (cuuint64_t)h : 1, m->mb ? (cuuint64_t)b : 1};
+    const int64_t row = n > 1 ? v.ss : (d + 7) / 8 * 8;
+    cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)(m->mh ? v.sh : row) * 2, (cuuint64_t)(m->mb ? v.sb : row) * 2};
+    cuuint32_t box[4] = {64, TILE, 1, 1}, one[4] = {1, 1, 1, 1};
+    return enc(&m->map, dtype == TL_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, v.p, dims,
+               strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// documents: the ranges of the key tiles
+size_t attn_tc_workspace(const AttnCall& a) {
+    return a.k_doc ? (size_t)a.b * ((a.nk + TILE - 1) / TILE) * sizeof(DocRange) : 0;
+}
+
+tl_status launch_doc_ranges(tl_ctx* c, const int32_t* doc, int b, int n, DocRange* out, cudaStream_t s) {
+    const int tiles = (n + TILE - 1) / TILE;
+    const int64_t total = (int64_t)b * tiles;
+    cudaEvent_t ev[2];
+    launch_begin_on(c, s, "attention_doc_ranges", 4.0 * b * n, 0, ev);
+    k_doc_ranges<<<(unsigned)((total + 7) / 8), 256, 0, s>>>(doc, n, tiles, total, out);
+    return launch_end_on(c, s, ev);
+}
+
+tl_status launch_attn_tc(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s) {
+    FwArgs g;
+    g.a = a;
+    g.k_ranges = static_cast<DocRange*>(ws);
+    g.pair_heads = a.hq / a.hkv % 2 == 0;
+    g.key_tiles = (a.nk + TILE - 1) / TILE;
+    g.err = c->d_flags + 8;
+    HeadMap mq, mk, mv;
+    if (!make_head_map(&mq, a.q, a.dtype, a.b, a.hq, a.nq, a.d) || !make_head_map(&mk, a.k, a.dtype, a.b, a.hkv, a.nk, a.d) ||
+        !make_head_map(&mv, a.v, a.dtype, a.b, a.hkv, a.nk, a.d))
+        return fail(c, TL_ERR_CUDA, "attention: tensor maps");
+    if (a.k_doc) TL_TRY(launch_doc_ranges(c, a.k_doc, a.b, a.nk, static_cast<DocRange*>(ws), s));
+    c->flags_armed = true;
+#define TL_ATTN(T, DP)                                                                     \
+    (a.cap > 0.f ? (a.slopes ? launch<T, DP, true, true>(c, mq, mk, mv, g, s)              \
+                             : launch<T, DP, true, false>(c, mq, mk, mv, g, s))            \
+                 : (a.slopes ? launch<T, DP, false, true>(c, mq, mk, mv, g, s)             \
+                             : launch<T, DP, false, false>(c, mq, mk, mv, g, s)))
+    if (a.dtype == TL_TYPE_F16) return a.d <= 64 ? TL_ATTN(__half, 64) : TL_ATTN(__half, 128);
+    return a.d <= 64 ? TL_ATTN(__nv_bfloat16, 64) : TL_ATTN(__nv_bfloat16, 128);
+#undef TL_ATTN
+}
+
+}  // namespace tl

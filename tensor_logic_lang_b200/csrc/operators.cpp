@@ -237,7 +237,10 @@ tl_status check_attention(tl_ctx* c, const tl_attention& t, bool backward, AttnC
     return TL_OK;
 }
 
-size_t attention_need(const AttnCall& a, bool backward) { return attn_general_workspace(a, backward); }
+size_t attention_need(const AttnCall& a, bool backward) {
+    if (!backward && attn_tc_takes(a)) return attn_tc_workspace(a);
+    return attn_general_workspace(a, backward);
+}
 
 tl_status run_attention(tl_ctx* c, const tl_attention* t, bool backward) {
     if (!t) return fail(c, TL_ERR_INVALID, "attention: no descriptor");
@@ -252,7 +255,8 @@ tl_status run_attention(tl_ctx* c, const tl_attention* t, bool backward) {
     TL_TRY(check_stream(c, s, &capturing));
     void* ws = nullptr;
     TL_TRY(op_workspace(c, s, capturing, attention_need(a, backward), t->workspace, t->workspace_bytes, &ws));
-    return backward ? launch_attn_general_backward(c, a, ws, s) : launch_attn_general(c, a, ws, s);
+    if (backward) return launch_attn_general_backward(c, a, ws, s);
+    return attn_tc_takes(a) ? launch_attn_tc(c, a, ws, s) : launch_attn_general(c, a, ws, s);
 }
 
 // ---------------------------------------------------------------------------
