@@ -91,6 +91,11 @@ bool attn_tc_takes(const AttnCall& a);
 size_t attn_tc_workspace(const AttnCall& a);
 tl_status launch_attn_tc(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s);
 
+// k_attention_tc_bwd.cu
+bool attn_tc_backward_takes(const AttnCall& a);
+size_t attn_tc_backward_workspace(const AttnCall& a);
+tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s);
+
 // k_clip.cu
 struct ClipItem {
     const void* in;

@@ -289,5 +289,6 @@ bool make_head_map(HeadMap* m, const HeadsView& v, int dtype, int b, int h, int6
 // the arrays a tensor-core kernel takes: 16-bit, head size contiguous, 16-byte
 // aligned rows
 bool tc_array(const HeadsView& v, int b, int h, int64_t n);
+tl_status launch_doc_ranges(tl_ctx* c, const int32_t* doc, int b, int n, DocRange* out, cudaStream_t s);
 
 }  // namespace tl

@@ -1,0 +1,886 @@
+// Attention backward on the tensor cores: 16-bit operands, head size up to
+// 128.  With p = exp(s - lse), dp = dout v^T, D = dout . o by row,
+//   dx = p (dp - D) (1 - tanh^2),  dq = scale dx k,  dk = scale dx^T q,  dv = p^T dout
+// the scores are taken again from q and k (S is never stored), twice:
+//
+//   k_attn_prep    by tile of 128 queries: log2(e) lse and D, ready for the
+//                  kernels below; the largest row norms of dout and v (fp16)
+//   k_attn_tc_dkv  a block per (key tile, head): dk and dv stay in TMEM while
+//                  the query tiles pass; the heads of a group form a cluster
+//                  and add their sums through distributed shared memory in a
+//                  fixed order
+//   k_attn_tc_dq   a block per (query tile, head): dq stays in TMEM while the
+//                  key tiles pass
+//
+// Seven products where one kernel for all three would need five, but no
+// atomics on dq: the results do not depend on the order of the blocks, and
+// there is no fp32 copy of dq in memory.  Two warpgroups take 64 columns of
+// the 128 x 128 scores each; P (dx) goes back to TMEM as a 16-bit operand over
+// the half of S (dp) its warpgroup has read.  While the exponentials of one
+// tile run, the products of the tile before and the scores of the next do.
+//
+// 16-bit roundings: p and dx as operands of the last products (tensor cores
+// take 16-bit operands), each off by half a step of its own size.  fp16 ends
+// at 2^-24, so p is written 2^14 larger, and dx times the power of two that
+// puts its bound, 2 max|dout_i| max|v_j| (norms; |dp| and |D| are at most half
+// of it), at 2^15: neither can overflow, and small gradients keep their bits.
+#include <algorithm>
+
+#include "attn_tc.h"
+
+namespace tl {
+namespace {
+
+constexpr int BW_THREADS = 384, BW_STAGES = 2;
+constexpr int STAT_BYTES = 2 * TILE * 4;   // of a query tile: -log2(e) lse (+ lift), -D
+
+template <typename T> struct PLift { static constexpr float log2 = 0.f, back = 1.f; };
+template <> struct PLift<__half> { static constexpr float log2 = 14.f, back = 1.f / 16384.f; };
+
+struct BwArgs {
+    AttnCall a;
+    const float* stats;          // [b, hq, query tiles][2][128]
+    const uint32_t* norms;       // fp16: [b, hkv][2] largest |dout_i|^2, |v_j|^2 as bits
+    const DocRange *q_ranges, *k_ranges;
+    int q_tiles, k_tiles, cluster;
+    int* err;
+};
+
+template <int DP>
+struct BwSmem {
+    static constexpr int CH = DP / 64, TILE_B = CH * CHUNK_BYTES;
+    // two resident tiles, stages of two tiles and the statistics
+    static constexpr int FIX = 0, RING = 2 * TILE_B, STAT = RING + BW_STAGES * 2 * TILE_B, BAR = STAT + BW_STAGES * STAT_BYTES,
+                         DOCS = BAR + 256, BYTES = DOCS + 64 + 1024;
+    // the cluster's sums: dv and dk as fp32 rows padded by 16 bytes, over the tiles
+    static constexpr int SUM_LD = DP + 4;
+    static_assert(2 * TILE * SUM_LD * 4 <= STAT, "the sums lie over the tiles");
+};
+
+// ---------------------------------------------------------------- preparation
+// |row|^2 of 8 columns, and the dot product with another row
+template <typename T>
+__device__ __forceinline__ void dot8(const uint4& x, const uint4& y, float& xy, float& xx) {
+    const T* a = reinterpret_cast<const T*>(&x);
+    const T* b = reinterpret_cast<const T*>(&y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float u = to_f32(a[i]);
+        xy = fmaf(u, to_f32(b[i]), xy);
+        xx = fmaf(u, u, xx);
+    }
+}
+
+// Blocks of a tile of 128 rows, 16 lanes a row, 8 rows of a half warp in
+// flight: first the query tiles, then (fp16) the key tiles' norms of v.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    k_attn_prep(const __grid_constant__ AttnCall a, float* __restrict__ stats, uint32_t* __restrict__ norms, int q_tiles, int k_tiles) {
+    const int half = threadIdx.x / 16, sub = threadIdx.x % 16, c0 = sub * 8;
+    int64_t blk = blockIdx.x;
+    const int64_t n_q = (int64_t)a.b * a.hq * q_tiles;
+    float top = 0.f;
+    const bool keys = blk >= n_q;
+    int group_of;
+    if (!keys) {
+        const int qt = (int)(blk % q_tiles);
+        const int h = (int)(blk / q_tiles % a.hq), b = (int)(blk / q_tiles / a.hq);
+        group_of = b * a.hkv + h / (a.hq / a.hkv);
+        const T* dout = static_cast<const T*>(a.dout.p) + b * a.dout.sb + h * a.dout.sh + c0;
+        const T* o = static_cast<const T*>(a.o.p) + b * a.o.sb + h * a.o.sh + c0;
+        uint4 x[8], y[8];
+        bool on[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = qt * TILE + half * 8 + k;
+            on[k] = i < a.nq && (!a.q_doc || a.q_doc[(int64_t)b * a.nq + i] >= 0);
+            x[k] = y[k] = make_uint4(0, 0, 0, 0);
+            if (on[k] && c0 < a.d) {
+                x[k] = *reinterpret_cast<const uint4*>(dout + i * a.dout.ss);
+                y[k] = *reinterpret_cast<const uint4*>(o + i * a.o.ss);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            float xy = 0.f, xx = 0.f;
+            dot8<T>(x[k], y[k], xy, xx);
+#pragma unroll
+            for (int w = 8; w; w >>= 1) {
+                xy += __shfl_xor_sync(0xffffffffu, xy, w);
+                xx += __shfl_xor_sync(0xffffffffu, xx, w);
+            }
+            top = fmaxf(top, xx);
+            if (sub == 0) {
+                const int r = half * 8 + k, i = qt * TILE + r;
+                float* st = stats + blk * 2 * TILE;
+                const float lse = on[k] ? a.lse[((int64_t)b * a.hq + h) * a.nq + i] : -INFINITY;
+                // a row that sees nothing has p = 2^-inf = 0 everywhere
+                st[r] = lse == -INFINITY ? -INFINITY : PLift<T>::log2 - lse * kLog2e;
+                st[TILE + r] = -xy;
+            }
+        }
+    } else {
+        blk -= n_q;
+        const int kt = (int)(blk % k_tiles);
+        const int h = (int)(blk / k_tiles % a.hkv), b = (int)(blk / k_tiles / a.hkv);
+        group_of = b * a.hkv + h;
+        const int kv = a.kv_len ? min(max(a.kv_len[b], 0), a.nk) : a.nk;
+        const T* v = static_cast<const T*>(a.v.p) + b * a.v.sb + h * a.v.sh + c0;
+        uint4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int j = kt * TILE + half * 8 + k;
+            x[k] = make_uint4(0, 0, 0, 0);
+            if (j < kv && (!a.k_doc || a.k_doc[(int64_t)b * a.nk + j] >= 0) && c0 < a.d)
+                x[k] = *reinterpret_cast<const uint4*>(v + j * a.v.ss);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            float xy = 0.f, xx = 0.f;
+            dot8<T>(x[k], x[k], xy, xx);
+#pragma unroll
+            for (int w = 8; w; w >>= 1) xx += __shfl_xor_sync(0xffffffffu, xx, w);
+            top = fmaxf(top, xx);
+        }
+    }
+    if (norms) {
+        // non-negative floats order like their bits; a maximum does not depend on the order
+        const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+        if ((threadIdx.x & 31) == 0) atomicMax(&norms[2 * group_of + (keys ? 1 : 0)], m);
+    }
+}
+
+// The power of two that dx is written with (see the top of the file).
+template <typename T>
+__device__ __forceinline__ float dx_lift(const BwArgs& g, int b, int kvh) {
+    if (PLift<T>::log2 == 0.f) return 1.f;
+    const uint32_t* n = g.norms + 2 * ((int64_t)b * g.a.hkv + kvh);
+    const float bound = 2.f * sqrtf(__uint_as_float(n[0])) * sqrtf(__uint_as_float(n[1]));
+    if (!(bound > 0.f) || bound > 3e38f) return 1.f;
+    return exp2f(fminf(fmaxf(floorf(15.f - log2f(bound)), -100.f), 100.f));
+}
+
+// ---------------------------------------------------------------- elements
+// 64 scores q.k of a row -> p in base 2 (16-bit pairs) and p (1 - tanh^2).
+// off: position of column 0 relative to the row's (|off + c| is the distance);
+// nl(i): minus log2(e) lse of the columns 2i, 2i + 1.
+template <typename T, bool CAP, bool BIAS, typename NL>
+__device__ __forceinline__ void grad_row(f2 (&x)[32], uint32_t (&p16)[32], float c1, const CapCoef& cap, float slope2, int off,
+                                         bool masked, uint32_t bits0, uint32_t bits1, NL nl) {
+    f2 bend[CAP ? 32 : 1];
+    if (CAP) {
+        float big = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            float lo, hi;
+            unpack2(x[i], lo, hi);
+            big = fmaxf(big, fmaxf(fabsf(lo), fabsf(hi)));
+        }
+        const f2 one = pack2(1.f, 1.f);
+        if (__any_sync(0xffffffffu, !(big <= cap.limit))) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                float lo, hi;
+                unpack2(x[i], lo, hi);
+                lo = wide_tanh(lo, cap.wide);
+                hi = wide_tanh(hi, cap.wide);
+                bend[i] = fma2(pack2(-lo, -hi), pack2(lo, hi), one);
+                x[i] = pack2(cap.top * lo, cap.top * hi);
+            }
+        } else {
+            const f2 k2 = pack2(cap.k2, cap.k2), mul = pack2(cap.mul, cap.mul), neg = pack2(-cap.k2, -cap.k2);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const f2 r = tanh_ratio(x[i], k2), xr = mul2(x[i], r);
+                bend[i] = fma2(mul2(xr, neg), xr, one);
+                x[i] = mul2(xr, mul);
+            }
+        }
+    }
+    const f2 c = CAP ? pack2(1.f, 1.f) : pack2(c1, c1);
+    if (BIAS) {
+        const bool after = __all_sync(0xffffffffu, off >= 0), before = __all_sync(0xffffffffu, off + 63 <= 0);
+        if (after || before) {
+            const float k = after ? -slope2 : slope2, kb = k * (float)off;
+            const f2 kk = pack2(k, k), base = pack2(kb, kb);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = fma2(x[i], c, fma2(kk, pack2((float)(2 * i), (float)(2 * i + 1)), base));
+        } else {
+            const float at = (float)off;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                x[i] = fma2(x[i], c, pack2(-slope2 * fabsf(at + (float)(2 * i)), -slope2 * fabsf(at + (float)(2 * i + 1))));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        float lo, hi;
+        unpack2(CAP || BIAS ? add2(x[i], nl(i)) : fma2(x[i], c, nl(i)), lo, hi);
+        if (masked) {
+            const uint32_t w = i < 16 ? bits0 : bits1;
+            lo = (w >> (2 * i % 32)) & 1 ? lo : -INFINITY;
+            hi = (w >> (2 * i % 32 + 1)) & 1 ? hi : -INFINITY;
+        }
+        lo = ex2(lo);
+        hi = ex2(hi);
+        p16[i] = pack16<T>(lo, hi);
+        x[i] = pack2(lo, hi);
+        if (CAP) x[i] = mul2(x[i], bend[i]);
+    }
+}
+
+// dx = pb (dp - D), zero where the key is not seen (there dp may be anything)
+template <typename T, typename ND>
+__device__ __forceinline__ void grad_dx(const f2 (&pb)[32], const uint32_t (&dp)[64], uint32_t (&out)[32], float lift, bool masked,
+                                        uint32_t bits0, uint32_t bits1, ND nd) {
+    const f2 up = pack2(lift, lift);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const f2 d2 = pack2(__uint_as_float(dp[2 * i]), __uint_as_float(dp[2 * i + 1]));
+        float lo, hi;
+        unpack2(mul2(pb[i], PLift<T>::log2 == 0.f ? add2(d2, nd(i)) : fma2(d2, up, nd(i))), lo, hi);
+        if (masked) {
+            const uint32_t w = i < 16 ? bits0 : bits1;
+            lo = (w >> (2 * i % 32)) & 1 ? lo : 0.f;
+            hi = (w >> (2 * i % 32 + 1)) & 1 ? hi : 0.f;
+        }
+        out[i] = pack16<T>(lo, hi);
+    }
+}
+
+__device__ __forceinline__ void load64(uint32_t taddr, uint32_t (&raw)[64]) {
+    tmem_ld32(taddr, raw);
+    tmem_ld32(taddr + 32, raw + 32);
+    tmem_wait_ld();
+}
+__device__ __forceinline__ void load64(uint32_t taddr, f2 (&x)[32]) {
+    uint32_t raw[64];
+    load64(taddr, raw);
+#pragma unroll
+    for (int k = 0; k < 32; ++k) x[k] = pack2(__uint_as_float(raw[2 * k]), __uint_as_float(raw[2 * k + 1]));
+}
+
+// D[128 x n] (+)= A B as mma_cols, A in two halves of 64 columns of the
+// contracted index, 32 TMEM columns each, 64 columns apart
+template <typename T>
+__device__ __forceinline__ void mma_halves(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+#pragma unroll
+    for (int k = 0; k < TILE / 16; ++k)
+        umma_f16_ts(d, a + (k / 4) * 64 + (k % 4) * 8, umma_desc(b + k * 2048, CHUNK_BYTES, 1024, kLayoutSW128), idesc,
+                    accumulate | (k > 0));
+}
+
+// A row of DP fp32 sums in TMEM, scaled, as 16-bit values of an array.
+template <typename T, int DP>
+__device__ __forceinline__ void store_row(const HeadsView& v, int b, int h, int64_t row, bool on, int d, uint32_t taddr, bool any, float mul) {
+    T* p = static_cast<T*>(v.p) + b * v.sb + h * v.sh + row * v.ss;
+    for (int k = 0; k < DP / 32; ++k) {
+        uint32_t o[32];
+        if (any) {
+            tmem_ld32(taddr + 32 * k, o);
+            tmem_wait_ld();
+        }
+        if (on)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (32 * k + 8 * q >= d) break;
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    w[e] = any ? pack16<T>(__uint_as_float(o[8 * q + 2 * e]) * mul, __uint_as_float(o[8 * q + 2 * e + 1]) * mul) : 0u;
+                *reinterpret_cast<uint4*>(p + 32 * k + 8 * q) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+    }
+}
+
+// What the two gradient kernels share: barriers, TMEM, the documents of the block's rows.
+struct BwBlock {
+    uint64_t *fix, *full, *empty, *s_full, *p_full, *dp_full, *dx_full, *done;
+    uint32_t* tmem_slot;
+    int* docs;
+    __device__ __forceinline__ BwBlock(uint8_t* bars, uint8_t* docs_at) {
+        uint64_t* bar = reinterpret_cast<uint64_t*>(bars);
+        fix = bar;
+        full = bar + 1;
+        empty = full + BW_STAGES;
+        s_full = empty + BW_STAGES;   // two in the dq kernel
+        p_full = s_full + 2;
+        dp_full = p_full + 1;
+        dx_full = dp_full + 1;
+        done = dx_full + 1;
+        tmem_slot = reinterpret_cast<uint32_t*>(bar + 24);
+        docs = reinterpret_cast<int*>(docs_at);
+    }
+    // returns the TMEM base; `doc`: documents of the block's rows, or null
+    __device__ __forceinline__ uint32_t setup(const int32_t* doc, int rows, DocRange* mine) {
+        const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+        if (threadIdx.x == 0) {
+            mbar_init(fix, 1);
+            for (int s = 0; s < BW_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+            mbar_init(&s_full[0], 1); mbar_init(&s_full[1], 1);
+            mbar_init(p_full, 2 * TILE); mbar_init(dp_full, 1); mbar_init(dx_full, 2 * TILE); mbar_init(done, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            docs[0] = 0x7fffffff; docs[1] = -1; docs[2] = 0;
+        }
+        if (warp == 8) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        *mine = no_docs();
+        if (doc) {
+            const int r = threadIdx.x;
+            const int d = r < rows ? doc[r] : -1;
+            const int lo = __reduce_min_sync(0xffffffffu, d >= 0 ? d : 0x7fffffff), hi = __reduce_max_sync(0xffffffffu, d);
+            const int pad = __any_sync(0xffffffffu, d < 0);
+            if (lane == 0) {
+                atomicMin(&docs[0], lo);
+                atomicMax(&docs[1], hi);
+                if (pad && warp * 32 < rows) docs[2] = 1;
+            }
+            __syncthreads();
+            *mine = {docs[0], docs[1], docs[2], 0};
+        }
+        return *tmem_slot;
+    }
+    __device__ __forceinline__ void finish(uint32_t tmem) {
+        tc_fence_before();
+        __syncthreads();
+        if (threadIdx.x / 32 == 8) {
+            tc_fence_after();
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+        }
+    }
+};
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, bool ok, int* err) {
+    ok = ok && mbar_wait(bar, parity, err);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    return ok;
+}
+
+// ---------------------------------------------------------------- dk, dv
+// TMEM: S^T (P^T) 0..127, dp^T (dx^T) 128..255, dv, dk (DP columns each).
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(BW_THREADS, 1)
+    k_attn_tc_dkv(const __grid_constant__ HeadMap mq, const __grid_constant__ HeadMap mk, const __grid_constant__ HeadMap mv,
+                  const __grid_constant__ HeadMap mdo, const __grid_constant__ BwArgs g) {
+    using L = BwSmem<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const AttnCall& a = g.a;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    // block -> (key tile, sequence and key head, head of the group); a causal
+    // call's first keys are seen by the most queries and go first
+    const int group = a.hq / a.hkv, rank = blockIdx.x % g.cluster;
+    const unsigned unit = blockIdx.x / g.cluster, bhs = (unsigned)a.b * a.hkv;
+    const int kt = (int)(unit / bhs), kvh = (int)(unit % bhs % a.hkv), b = (int)(unit % bhs / a.hkv);
+    const int j0 = kt * TILE;
+    const SeqMask mask(a, b);
+    const int32_t* qd = a.q_doc ? a.q_doc + (int64_t)b * a.nq : nullptr;
+    const int32_t* kd = a.k_doc ? a.k_doc + (int64_t)b * a.nk : nullptr;
+    BwBlock bb(smem + L::BAR, smem + L::DOCS);
+    DocRange mine;
+    const uint32_t tmem = bb.setup(kd ? kd + j0 : nullptr, min(TILE, a.nk - j0), &mine);
+    const uint32_t t_s = tmem, t_dp = tmem + TILE, t_dv = tmem + 2 * TILE, t_dk = tmem + 2 * TILE + DP;
+
+    // query tiles that see some of the keys; from `clear` on they see all of them
+    int begin = 0, end = g.q_tiles, clear = 0;
+    if (mask.causal && j0 >= mask.prefix) begin = max(0, j0 - mask.p0) / TILE;
+    if (mask.causal && j0 + TILE > mask.prefix) clear = max(0, j0 + TILE - 1 - mask.p0 + TILE - 1) / TILE;
+    if (j0 >= mask.kv) end = 0;
+    if (mask.kv < a.nk && j0 + TILE > mask.kv) clear = end;
+    const DocRange* ranges = qd ? g.q_ranges + (int64_t)b * g.q_tiles : nullptr;
+    TileWalk walk;
+    bool masked, ok = true;
+    // (head, query tile) pairs in order; qt < 0 after the last
+    int h = kvh * group + rank - g.cluster;
+    int qt = -1;
+    auto first = [&]() { walk.start(0, 0, 0, 0, ranges, mine); };
+    auto next = [&]() {
+        qt = walk.next(&masked);
+        while (qt < 0) {
+            h += g.cluster;
+            if (h >= (kvh + 1) * group) return;
+            walk.start(begin, end, clear, end, ranges, mine);
+            qt = walk.next(&masked);
+        }
+    };
+    first();
+    next();
+    const bool any = qt >= 0;   // the same for every head
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 9) {
+            // ------------------------------------------------ TMA
+            if (any && lane == 0) {
+                mbar_expect_tx(bb.fix, 2 * L::TILE_B);
+                tma_tile(smem_u32(smem + L::FIX), mk, bb.fix, L::CH, j0, kvh, b);
+                tma_tile(smem_u32(smem + L::FIX + L::TILE_B), mv, bb.fix, L::CH, j0, kvh, b);
+            }
+            int n = 0;
+            for (; qt >= 0 && ok; next(), ++n) {
+                const int s = n % BW_STAGES;
+                if (n >= BW_STAGES) ok = warp_wait(&bb.empty[s], ((n / BW_STAGES) & 1) ^ 1, ok, g.err);
+                if (ok && lane == 0) {
+                    mbar_expect_tx(&bb.full[s], 2 * L::TILE_B + STAT_BYTES);
+                    const uint32_t at = smem_u32(smem + L::RING + s * 2 * L::TILE_B);
+                    tma_tile(at, mq, &bb.full[s], L::CH, qt * TILE, h, b);
+                    tma_tile(at + L::TILE_B, mdo, &bb.full[s], L::CH, qt * TILE, h, b);
+                    const float* st = g.stats + (((int64_t)b * a.hq + h) * g.q_tiles + qt) * 2 * TILE;
+                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                     smem_u32(smem + L::STAT + s * STAT_BYTES)),
+                                 "l"(st), "r"(STAT_BYTES), "r"(smem_u32(&bb.full[s]))
+                                 : "memory");
+                }
+            }
+            if (!ok)   // copies in flight land before the block ends
+                for (int e = max(0, n - 1 - BW_STAGES); e < n - 1; ++e)
+                    mbar_wait(&bb.full[e % BW_STAGES], (e / BW_STAGES) & 1, g.err);
+        } else if (warp == 8) {
+            // ------------------------------------------------ tensor cores
+            const int ksteps = (a.d + 15) / 16;
+            const uint32_t idesc = f16_idesc<T>(16 * ksteps, true);
+            const uint32_t sk = smem_u32(smem + L::FIX), sv = sk + L::TILE_B;
+            // query rows of negative documents: 0 times what they hold could be NaN
+            auto clean = [&](int s) {
+                if (!qd || !masked) return;
+                auto bad = [&](int r) { const int i = qt * TILE + r; return i < a.nq && qd[i] < 0; };
+                clear_rows(smem + L::RING + s * 2 * L::TILE_B, L::CH, bad);
+                clear_rows(smem + L::RING + s * 2 * L::TILE_B + L::TILE_B, L::CH, bad);
+                fence_proxy_async_smem();
+                __syncwarp();
+            };
+            int n = 0;
+            if (any) {
+                ok = warp_wait(bb.fix, 0, ok, g.err);
+                ok = warp_wait(&bb.full[0], 0, ok, g.err);
+                if (ok) clean(0);
+                const uint32_t sq = smem_u32(smem + L::RING);
+                if (ok && lane == 0) {
+                    mma_rows<T>(t_s, sk, sq, ksteps);
+                    umma_commit(&bb.s_full[0]);
+                    mma_rows<T>(t_dp, sv, sq + L::TILE_B, ksteps);
+                    umma_commit(bb.dp_full);
+                }
+                __syncwarp();
+            }
+            while (qt >= 0 && ok) {
+                const int s = n % BW_STAGES, s1 = (n + 1) % BW_STAGES;
+                const uint32_t sq = smem_u32(smem + L::RING + s * 2 * L::TILE_B);
+                const uint32_t sq1 = smem_u32(smem + L::RING + s1 * 2 * L::TILE_B);
+                ok = warp_wait(bb.p_full, n & 1, ok, g.err);
+                if (ok && lane == 0) mma_halves<T>(t_dv, t_s, sq + L::TILE_B, idesc, n > 0);
+                __syncwarp();
+                next();
+                if (qt >= 0) {
+                    ok = warp_wait(&bb.full[s1], ((n + 1) / BW_STAGES) & 1, ok, g.err);
+                    if (ok) clean(s1);
+                    if (ok && lane == 0) {
+                        mma_rows<T>(t_s, sk, sq1, ksteps);
+                        umma_commit(&bb.s_full[0]);
+                    }
+                    __syncwarp();
+                }
+                ok = warp_wait(bb.dx_full, n & 1, ok, g.err);
+                if (ok && lane == 0) {
+                    mma_halves<T>(t_dk, t_dp, sq, idesc, n > 0);
+                    umma_commit(&bb.empty[s]);
+                    if (qt >= 0) {
+                        mma_rows<T>(t_dp, sv, sq1 + L::TILE_B, ksteps);
+                        umma_commit(bb.dp_full);
+                    } else {
+                        umma_commit(bb.done);
+                    }
+                }
+                __syncwarp();
+                ++n;
+            }
+        }
+    } else {
+        // ---------------------------------------------------- a key per thread, 64 queries
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int wg = warp / 4, r = threadIdx.x % TILE, j = j0 + r;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const float c1 = a.scale * kLog2e;
+        const CapCoef cap = cap_coef(a.scale, CAP ? a.cap : 1.f);
+        const float lift = dx_lift<T>(g, b, kvh), up = lift * PLift<T>::back;
+        const int doc = kd && j < a.nk ? kd[j] : -1;
+        int n = 0;
+        for (; qt >= 0 && ok; next(), ++n) {
+            const int i0 = qt * TILE + wg * 64;
+            uint32_t bits0 = 0xffffffffu, bits1 = 0xffffffffu;
+            if (masked) {
+                // queries from `from` on see the key
+                int from = mask.causal && j >= mask.prefix ? j - mask.p0 - i0 : 0;
+                if (j >= mask.kv) from = 64;
+                bits0 = ~low_bits(from, 0);
+                bits1 = ~low_bits(from, 1);
+                if (qd) {
+                    const int other[4] = {i0 + lane < a.nq ? __ldg(qd + i0 + lane) : -1,
+                                          i0 + 32 + lane < a.nq ? __ldg(qd + i0 + 32 + lane) : -1, -1, -1};
+                    uint32_t same[4];
+                    doc_bits(other, doc, same);
+                    bits0 &= same[0];
+                    bits1 &= same[1];
+                }
+            }
+            const float slope2 = BIAS ? __ldg(a.slopes + h) * kLog2e : 0.f;
+            const float* st = reinterpret_cast<const float*>(smem + L::STAT + (n % BW_STAGES) * STAT_BYTES) + wg * 64;
+            ok = warp_wait(&bb.full[n % BW_STAGES], (n / BW_STAGES) & 1, ok, g.err);   // the statistics
+            ok = warp_wait(&bb.s_full[0], n & 1, ok, g.err);
+            if (!ok) break;
+            f2 x[32];
+            {
+                load64(t_s + lanes + wg * 64, x);
+                uint32_t p16[32];
+                grad_row<T, CAP, BIAS>(x, p16, c1, cap, slope2, mask.p0 + i0 - j, masked, bits0, bits1,
+                                       [&](int i) { return *reinterpret_cast<const f2*>(st + 2 * i); });
+                tmem_st32(t_s + lanes + wg * 64, p16);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(bb.p_full);
+            ok = warp_wait(bb.dp_full, n & 1, ok, g.err);
+            if (!ok) break;
+            {
+                uint32_t dp[64], dx[32];
+                load64(t_dp + lanes + wg * 64, dp);
+                const f2 up2 = pack2(up, up);
+                grad_dx<T>(x, dp, dx, up, masked, bits0, bits1, [&](int i) {
+                    const f2 d = *reinterpret_cast<const f2*>(st + TILE + 2 * i);
+                    return PLift<T>::log2 == 0.f ? d : mul2(d, up2);
+                });
+                tmem_st32(t_dp + lanes + wg * 64, dx);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(bb.dx_full);
+        }
+        if (any) ok = warp_wait(bb.done, 0, ok, g.err);
+        const uint32_t mine_at = (wg ? t_dk : t_dv) + lanes;
+        const float mul = wg ? a.scale / lift : PLift<T>::back;
+        if (g.cluster == 1) {
+            if (ok) store_row<T, DP>(wg ? a.dk : a.dv, b, kvh, j, j < a.nk, a.d, mine_at, any, mul);
+        } else if (any && ok) {
+            float* row = reinterpret_cast<float*>(smem) + (wg * TILE + r) * L::SUM_LD;
+            for (int k = 0; k < DP / 32; ++k) {
+                uint32_t o[32];
+                tmem_ld32(mine_at + 32 * k, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    *reinterpret_cast<float4*>(row + 32 * k + 4 * q) =
+                        make_float4(__uint_as_float(o[4 * q]) * mul, __uint_as_float(o[4 * q + 1]) * mul,
+                                    __uint_as_float(o[4 * q + 2]) * mul, __uint_as_float(o[4 * q + 3]) * mul);
+            }
+        }
+    }
+    __syncwarp();
+    if (g.cluster > 1) {
+        // each block adds its share of the rows over the cluster, in the order of the heads
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (warp < 8) {
+            const int share = TILE / g.cluster, r0 = rank * share;
+            const uint32_t sums = smem_u32(smem);
+            constexpr int V = DP / 4;
+            for (int e = threadIdx.x; e < 2 * share * V; e += 2 * TILE) {
+                const int c = e % V, r = r0 + e / V % share, wg = e / V / share;
+                if (j0 + r >= a.nk || 4 * c >= a.d) continue;
+                float s[4] = {0.f, 0.f, 0.f, 0.f};
+                if (any)
+                    for (int q = 0; q < g.cluster; ++q) {
+                        uint32_t at;
+                        float x, y, z, w;
+                        asm("mapa.shared::cluster.u32 %0, %1, %2;"
+                            : "=r"(at)
+                            : "r"(sums + ((wg * TILE + r) * L::SUM_LD + 4 * c) * 4), "r"(q));
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(x), "=f"(y), "=f"(z), "=f"(w)
+                                     : "r"(at));
+                        s[0] += x; s[1] += y; s[2] += z; s[3] += w;
+                    }
+                const HeadsView& v = wg ? a.dk : a.dv;
+                T* p = static_cast<T*>(v.p) + b * v.sb + kvh * v.sh + (int64_t)(j0 + r) * v.ss + 4 * c;
+                *reinterpret_cast<uint2*>(p) = make_uint2(pack16<T>(s[0], s[1]), pack16<T>(s[2], s[3]));
+            }
+        }
+        __syncwarp();
+        // a block's sums stay until the others have read them
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    bb.finish(tmem);
+}
+
+// ---------------------------------------------------------------- dq
+// TMEM: S of two tiles 0..255, dp (dx) 256..383, dq 384..511.
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(BW_THREADS, 1)
+    k_attn_tc_dq(const __grid_constant__ HeadMap mq, const __grid_constant__ HeadMap mk, const __grid_constant__ HeadMap mv,
+                 const __grid_constant__ HeadMap mdo, const __grid_constant__ BwArgs g) {
+    using L = BwSmem<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const AttnCall& a = g.a;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const unsigned bhs = (unsigned)a.b * a.hq;
+    const int qt = g.q_tiles - 1 - (int)(blockIdx.x / bhs);
+    const int h = (int)(blockIdx.x % bhs % a.hq), b = (int)(blockIdx.x % bhs / a.hq), kvh = h / (a.hq / a.hkv);
+    const int i0 = qt * TILE, rows = min(TILE, a.nq - i0);
+    const SeqMask mask(a, b);
+    const int32_t* qd = a.q_doc ? a.q_doc + (int64_t)b * a.nq : nullptr;
+    const int32_t* kd = a.k_doc ? a.k_doc + (int64_t)b * a.nk : nullptr;
+    BwBlock bb(smem + L::BAR, smem + L::DOCS);
+    DocRange mine;
+    const uint32_t tmem = bb.setup(qd ? qd + i0 : nullptr, rows, &mine);
+    const uint32_t t_dp = tmem + 2 * TILE, t_dq = tmem + 3 * TILE;
+    TileWalk walk;
+    walk.start(0, (max(mask.key_end(i0, rows), 0) + TILE - 1) / TILE, 0, max(mask.key_end(i0, 1), 0) / TILE,
+               kd ? g.k_ranges + (int64_t)b * g.k_tiles : nullptr, mine);
+    bool masked, ok = true;
+    int kt = walk.next(&masked);
+    const bool any = kt >= 0;
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 9) {
+            // ------------------------------------------------ TMA
+            if (any && lane == 0) {
+                mbar_expect_tx(bb.fix, 2 * L::TILE_B);
+                tma_tile(smem_u32(smem + L::FIX), mq, bb.fix, L::CH, i0, h, b);
+                tma_tile(smem_u32(smem + L::FIX + L::TILE_B), mdo, bb.fix, L::CH, i0, h, b);
+            }
+            int n = 0;
+            for (; kt >= 0 && ok; kt = walk.next(&masked), ++n) {
+                const int s = n % BW_STAGES;
+                if (n >= BW_STAGES) ok = warp_wait(&bb.empty[s], ((n / BW_STAGES) & 1) ^ 1, ok, g.err);
+                if (ok && lane == 0) {
+                    mbar_expect_tx(&bb.full[s], 2 * L::TILE_B);
+                    const uint32_t at = smem_u32(smem + L::RING + s * 2 * L::TILE_B);
+                    tma_tile(at, mk, &bb.full[s], L::CH, kt * TILE, kvh, b);
+                    tma_tile(at + L::TILE_B, mv, &bb.full[s], L::CH, kt * TILE, kvh, b);
+                }
+            }
+            if (!ok)
+                for (int e = max(0, n - 1 - BW_STAGES); e < n - 1; ++e)
+                    mbar_wait(&bb.full[e % BW_STAGES], (e / BW_STAGES) & 1, g.err);
+        } else if (warp == 8) {
+            // ------------------------------------------------ tensor cores
+            const int ksteps = (a.d + 15) / 16;
+            const uint32_t idesc = f16_idesc<T>(16 * ksteps, true);
+            const uint32_t sq = smem_u32(smem + L::FIX), sdo = sq + L::TILE_B;
+            // keys that must not count: 0 times what they hold could be NaN
+            auto clean = [&](int s) {
+                if (!((kd && masked) || (mask.kv < a.nk && (kt + 1) * TILE > mask.kv))) return;
+                clear_rows(smem + L::RING + s * 2 * L::TILE_B, L::CH, [&](int r) {
+                    const int j = kt * TILE + r;
+                    return j >= mask.kv || (kd && kd[j] < 0);
+                });
+                fence_proxy_async_smem();
+                __syncwarp();
+            };
+            int n = 0;
+            if (any) {
+                ok = warp_wait(bb.fix, 0, ok, g.err);
+                ok = warp_wait(&bb.full[0], 0, ok, g.err);
+                if (ok) clean(0);
+                const uint32_t sk = smem_u32(smem + L::RING);
+                if (ok && lane == 0) {
+                    mma_rows<T>(tmem, sq, sk, ksteps);
+                    umma_commit(&bb.s_full[0]);
+                    mma_rows<T>(t_dp, sdo, sk + L::TILE_B, ksteps);
+                    umma_commit(bb.dp_full);
+                }
+                __syncwarp();
+            }
+            while (kt >= 0 && ok) {
+                const int s = n % BW_STAGES, s1 = (n + 1) % BW_STAGES;
+                const uint32_t sk = smem_u32(smem + L::RING + s * 2 * L::TILE_B);
+                const uint32_t sk1 = smem_u32(smem + L::RING + s1 * 2 * L::TILE_B);
+                kt = walk.next(&masked);
+                if (kt >= 0) {
+                    ok = warp_wait(&bb.full[s1], ((n + 1) / BW_STAGES) & 1, ok, g.err);
+                    if (ok) clean(s1);
+                    // the scores before last have been read: their dx came before
+                    if (ok && lane == 0) {
+                        mma_rows<T>(tmem + ((n + 1) & 1) * TILE, sq, sk1, ksteps);
+                        umma_commit(&bb.s_full[(n + 1) & 1]);
+                    }
+                    __syncwarp();
+                }
+                ok = warp_wait(bb.dx_full, n & 1, ok, g.err);
+                if (ok && lane == 0) {
+                    mma_halves<T>(t_dq, t_dp, sk, idesc, n > 0);
+                    umma_commit(&bb.empty[s]);
+                    if (kt >= 0) {
+                        mma_rows<T>(t_dp, sdo, sk1 + L::TILE_B, ksteps);
+                        umma_commit(bb.dp_full);
+                    } else {
+                        umma_commit(bb.done);
+                    }
+                }
+                __syncwarp();
+                ++n;
+            }
+        }
+    } else {
+        // ---------------------------------------------------- a query per thread, 64 keys
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int wg = warp / 4, r = threadIdx.x % TILE, i = i0 + r;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const float c1 = a.scale * kLog2e;
+        const CapCoef cap = cap_coef(a.scale, CAP ? a.cap : 1.f);
+        const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
+        const float lift = dx_lift<T>(g, b, kvh), up = lift * PLift<T>::back;
+        const float* st = g.stats + (((int64_t)b * a.hq + h) * g.q_tiles + qt) * 2 * TILE;
+        const float nl = st[r], nd = st[TILE + r] * up;
+        const f2 nl2 = pack2(nl, nl), nd2 = pack2(nd, nd);
+        const int doc = qd && i < a.nq ? qd[i] : -1, limit = mask.key_end(i, 1);
+        int n = 0;
+        for (; kt >= 0 && ok; kt = walk.next(&masked), ++n) {
+            const int jw = kt * TILE + wg * 64;
+            uint32_t bits0 = 0xffffffffu, bits1 = 0xffffffffu;
+            if (masked) {
+                bits0 = low_bits(limit - jw, 0);
+                bits1 = low_bits(limit - jw, 1);
+                if (kd) {
+                    const int other[4] = {jw + lane < a.nk ? __ldg(kd + jw + lane) : -1,
+                                          jw + 32 + lane < a.nk ? __ldg(kd + jw + 32 + lane) : -1, -1, -1};
+                    uint32_t same[4];
+                    doc_bits(other, doc, same);
+                    bits0 &= same[0];
+                    bits1 &= same[1];
+                }
+            }
+            ok = warp_wait(&bb.s_full[n & 1], (n / 2) & 1, ok, g.err);
+            if (!ok) break;
+            f2 x[32];
+            load64(tmem + (n & 1) * TILE + lanes + wg * 64, x);
+            {
+                uint32_t unused[32];
+                grad_row<T, CAP, BIAS>(x, unused, c1, cap, slope2, jw - (mask.p0 + i), masked, bits0, bits1,
+                                       [&](int) { return nl2; });
+            }
+            ok = warp_wait(bb.dp_full, n & 1, ok, g.err);
+            if (!ok) break;
+            {
+                uint32_t dp[64], dx[32];
+                load64(t_dp + lanes + wg * 64, dp);
+                grad_dx<T>(x, dp, dx, up, masked, bits0, bits1, [&](int) { return nd2; });
+                tmem_st32(t_dp + lanes + wg * 64, dx);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(bb.dx_full);
+        }
+        if (any) ok = warp_wait(bb.done, 0, ok, g.err);
+        // each warpgroup writes half of the columns
+        if (ok) {
+            constexpr int HALF = DP / 2;
+            HeadsView v = a.dq;
+            v.p = static_cast<T*>(v.p) + wg * HALF;
+            store_row<T, HALF>(v, b, h, i, i < a.nq, a.d - wg * HALF, t_dq + lanes + wg * HALF, any, a.scale / lift);
+        }
+    }
+    bb.finish(tmem);
+}
+
+struct BwPlan {
+    int q_tiles, k_tiles;
+    size_t stats, norms, q_ranges, k_ranges, bytes;
+    explicit BwPlan(const AttnCall& a) {
+        q_tiles = (a.nq + TILE - 1) / TILE;
+        k_tiles = (a.nk + TILE - 1) / TILE;
+        auto take = [&](size_t n) { const size_t at = bytes; bytes += (n + 255) / 256 * 256; return at; };
+        bytes = 0;
+        stats = take((size_t)a.b * a.hq * q_tiles * STAT_BYTES);
+        norms = take(a.dtype == TL_TYPE_F16 ? (size_t)a.b * a.hkv * 8 : 0);
+        q_ranges = take(a.q_doc ? (size_t)a.b * q_tiles * sizeof(DocRange) : 0);
+        k_ranges = take(a.q_doc ? (size_t)a.b * k_tiles * sizeof(DocRange) : 0);
+    }
+};
+
+template <typename T, int DP, bool CAP, bool BIAS>
+tl_status launch(tl_ctx* c, const HeadMap& mq, const HeadMap& mk, const HeadMap& mv, const HeadMap& mdo, const BwArgs& g, cudaStream_t s) {
+    static std::atomic<uint64_t> done_kv{0}, done_q{0};
+    constexpr int smem = BwSmem<DP>::BYTES;
+    TL_TRY(kernel_smem(c, k_attn_tc_dkv<T, DP, CAP, BIAS>, smem, done_kv));
+    TL_TRY(kernel_smem(c, k_attn_tc_dq<T, DP, CAP, BIAS>, smem, done_q));
+    const AttnCall& a = g.a;
+    cudaEvent_t ev[2];
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = g.cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)((int64_t)g.k_tiles * a.b * a.hkv * g.cluster));
+    cfg.blockDim = dim3(BW_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    launch_begin_on(c, s, "attention_tc_dkv", 0, 8.0 * a.d * attn_pairs(a), ev);
+    TL_CK(c, cudaLaunchKernelEx(&cfg, k_attn_tc_dkv<T, DP, CAP, BIAS>, mq, mk, mv, mdo, g));
+    TL_TRY(launch_end_on(c, s, ev));
+    launch_begin_on(c, s, "attention_tc_dq", 0, 6.0 * a.d * attn_pairs(a), ev);
+    k_attn_tc_dq<T, DP, CAP, BIAS><<<(unsigned)((int64_t)g.q_tiles * a.b * a.hq), BW_THREADS, smem, s>>>(mq, mk, mv, mdo, g);
+    return launch_end_on(c, s, ev);
+}
+
+}  // namespace
+
+bool attn_tc_backward_takes(const AttnCall& a) {
+    return attn_tc_takes(a) && a.nq > 0 && tc_array(a.dout, a.b, a.hq, a.nq) && tc_array(a.dq, a.b, a.hq, a.nq) &&
+           tc_array(a.dk, a.b, a.hkv, a.nk) && tc_array(a.dv, a.b, a.hkv, a.nk);
+}
+
+size_t attn_tc_backward_workspace(const AttnCall& a) { return BwPlan(a).bytes; }
+
+tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s) {
+    const BwPlan plan(a);
+    uint8_t* w = static_cast<uint8_t*>(ws);
+    float* stats = reinterpret_cast<float*>(w + plan.stats);
+    uint32_t* norms = a.dtype == TL_TYPE_F16 ? reinterpret_cast<uint32_t*>(w + plan.norms) : nullptr;
+    BwArgs g;
+    g.a = a;
+    g.stats = stats;
+    g.norms = norms;
+    g.q_ranges = reinterpret_cast<DocRange*>(w + plan.q_ranges);
+    g.k_ranges = reinterpret_cast<DocRange*>(w + plan.k_ranges);
+    g.q_tiles = plan.q_tiles;
+    g.k_tiles = plan.k_tiles;
+    const int group = a.hq / a.hkv;
+    g.cluster = group % 8 == 0 ? 8 : group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+    g.err = c->d_flags + 8;
+    HeadMap mq, mk, mv, mdo;
+    if (!make_head_map(&mq, a.q, a.dtype, a.b, a.hq, a.nq, a.d) || !make_head_map(&mk, a.k, a.dtype, a.b, a.hkv, a.nk, a.d) ||
+        !make_head_map(&mv, a.v, a.dtype, a.b, a.hkv, a.nk, a.d) || !make_head_map(&mdo, a.dout, a.dtype, a.b, a.hq, a.nq, a.d))
+        return fail(c, TL_ERR_CUDA, "attention: tensor maps");
+    c->flags_armed = true;
+    if (norms) TL_CK(c, cudaMemsetAsync(norms, 0, (size_t)a.b * a.hkv * 8, s));
+    if (a.q_doc) {
+        TL_TRY(launch_doc_ranges(c, a.q_doc, a.b, a.nq, reinterpret_cast<DocRange*>(w + plan.q_ranges), s));
+        TL_TRY(launch_doc_ranges(c, a.k_doc, a.b, a.nk, reinterpret_cast<DocRange*>(w + plan.k_ranges), s));
+    }
+    const int64_t blocks = (int64_t)a.b * a.hq * plan.q_tiles + (norms ? (int64_t)a.b * a.hkv * plan.k_tiles : 0);
+    const double rows = (double)a.b * a.hq * a.nq;
+    cudaEvent_t ev[2];
+    launch_begin_on(c, s, "attention_prep", 4.0 * rows * a.d, 2.0 * rows * a.d, ev);
+    if (a.dtype == TL_TYPE_F16) k_attn_prep<__half><<<(unsigned)blocks, 256, 0, s>>>(a, stats, norms, plan.q_tiles, plan.k_tiles);
+    else k_attn_prep<__nv_bfloat16><<<(unsigned)blocks, 256, 0, s>>>(a, stats, norms, plan.q_tiles, plan.k_tiles);
+    TL_TRY(launch_end_on(c, s, ev));
+#define TL_ATTN(T, DP)                                                                  \
+    (a.cap > 0.f ? (a.slopes ? launch<T, DP, true, true>(c, mq, mk, mv, mdo, g, s)      \
+                             : launch<T, DP, true, false>(c, mq, mk, mv, mdo, g, s))    \
+                 : (a.slopes ? launch<T, DP, false, true>(c, mq, mk, mv, mdo, g, s)     \
+                             : launch<T, DP, false, false>(c, mq, mk, mv, mdo, g, s)))
+    if (a.dtype == TL_TYPE_F16) return a.d <= 64 ? TL_ATTN(__half, 64) : TL_ATTN(__half, 128);
+    return a.d <= 64 ? TL_ATTN(__nv_bfloat16, 64) : TL_ATTN(__nv_bfloat16, 128);
+#undef TL_ATTN
+}
+
+}  // namespace tl

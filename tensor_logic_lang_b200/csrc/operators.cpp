@@ -238,6 +238,7 @@ tl_status check_attention(tl_ctx* c, const tl_attention& t, bool backward, AttnC
 }
 
 size_t attention_need(const AttnCall& a, bool backward) {
+    if (backward && attn_tc_backward_takes(a)) return attn_tc_backward_workspace(a);
     if (!backward && attn_tc_takes(a)) return attn_tc_workspace(a);
     return attn_general_workspace(a, backward);
 }
@@ -255,7 +256,8 @@ tl_status run_attention(tl_ctx* c, const tl_attention* t, bool backward) {
     TL_TRY(check_stream(c, s, &capturing));
     void* ws = nullptr;
     TL_TRY(op_workspace(c, s, capturing, attention_need(a, backward), t->workspace, t->workspace_bytes, &ws));
-    if (backward) return launch_attn_general_backward(c, a, ws, s);
+    if (backward)
+        return attn_tc_backward_takes(a) ? launch_attn_tc_backward(c, a, ws, s) : launch_attn_general_backward(c, a, ws, s);
     return attn_tc_takes(a) ? launch_attn_tc(c, a, ws, s) : launch_attn_general(c, a, ws, s);
 }
 
