@@ -96,6 +96,11 @@ bool attn_tc_backward_takes(const AttnCall& a);
 size_t attn_tc_backward_workspace(const AttnCall& a);
 tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s);
 
+// k_attention_decode.cu: few queries over many keys, any type
+bool attn_few_takes(const AttnCall& a);
+size_t attn_few_workspace(const AttnCall& a);
+tl_status launch_attn_few(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s);
+
 // k_clip.cu
 struct ClipItem {
     const void* in;

@@ -1,0 +1,865 @@
+// Attention of few queries over many keys (a token or a few of each sequence
+// over its cache): bound by reading the cache once.
+//
+// The queries of a group's heads that read one key head are the rows of a
+// unit (16 or 32 of them; more rows make more units).  A unit's keys are cut
+// into tiles of 64, the tiles of all units form one line, and each block takes
+// an equal piece of it, whatever the sequences' lengths: all blocks run at
+// once and end together.  A piece that covers a unit whole writes its output;
+// the pieces of a unit that lies over several blocks leave their sums,
+// maxima and unnormalised outputs in the workspace (at most two a block), and
+// k_decode_join adds them in the order of the keys.
+//
+//   k_decode_mma   16-bit types with aligned rows and head sizes up to 128: TMA
+//                  tiles (128-byte swizzle) through a ring; each of four
+//                  warps takes 16 keys of a tile for all rows, with
+//                  mma.sync.m16n8k16 (at a few rows a key the tensor work is a
+//                  fraction of the time the key's bytes take)
+//   k_decode_any   any type, stride and head size: tiles as fp32 in shared
+//                  memory, FFMA
+#include <algorithm>
+
+#include "attn_tc.h"
+
+namespace tl {
+namespace {
+
+constexpr int DT = 64;                // keys of a tile
+constexpr int JOIN_THREADS = 256;
+
+struct DecArgs {
+    AttnCall a;
+    int rows;          // of a unit: 16 or 32
+    int row_blocks;    // units of a key head
+    int blocks;        // of the kernel that reads the cache
+    const int2* spans; // [b] with documents: the first and one past the last key that may be seen
+    float* part;       // [blocks][2][rows][d + 2]: o, m, l of a piece
+    int* err;
+};
+
+__device__ __forceinline__ int2 seq_tiles(const DecArgs& g, int b) {
+    const SeqMask mask(g.a, b);
+    int end = max(mask.key_end(0, g.a.nq), 0), begin = 0;
+    if (g.spans) {
+        const int2 s = g.spans[b];
+        begin = min(s.x, end);
+        end = min(s.y, end);
+    }
+    if (end <= begin) return make_int2(0, 0);
+    return make_int2(begin / DT, (end + DT - 1) / DT);
+}
+
+// Sum over the block; every thread gets it.  NW warps, red[NW] words.
+template <int NW>
+__device__ __forceinline__ int64_t block_total(int64_t v, int64_t* red) {
+#pragma unroll
+    for (int w = 16; w; w >>= 1) v += __shfl_xor_sync(0xffffffffu, v, w);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    int64_t s = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) s += red[w];
+    return s;
+}
+
+// Tiles of all sequences, and of those before `upto`.
+template <int NW>
+__device__ __forceinline__ int64_t tiles_before(const DecArgs& g, int upto, int64_t* all, int64_t* red) {
+    int64_t t = 0, p = 0;
+    for (int b = threadIdx.x; b < g.a.b; b += NW * 32) {
+        const int2 s = seq_tiles(g, b);
+        t += s.y - s.x;
+        if (b < upto) p += s.y - s.x;
+    }
+    *all = block_total<NW>(t, red);
+    return block_total<NW>(p, red);
+}
+
+// The line of tiles, from a place on: sequence, unit within it, tile of it.
+struct Place {
+    int b, unit;       // unit of the sequence: key head * row_blocks + row block
+    int2 span;         // its tiles
+    int64_t tile;      // next tile (span.x ..)
+};
+
+// The place of tile number `at` of the line (at < all tiles); any thread count.
+template <int NW>
+__device__ __forceinline__ Place find_place(const DecArgs& g, int64_t at, int64_t* red, int64_t* found) {
+    const int units = g.a.hkv * g.row_blocks, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    int64_t before = 0;
+    for (int b0 = 0; b0 < g.a.b; b0 += NW * 32) {
+        const int b = b0 + threadIdx.x;
+        int64_t n = 0;
+        if (b < g.a.b) {
+            const int2 s = seq_tiles(g, b);
+            n = (int64_t)(s.y - s.x) * units;
+        }
+        int64_t sum = n;   // inclusive over the warp
+#pragma unroll
+        for (int w = 1; w < 32; w <<= 1) {
+            const int64_t o = __shfl_up_sync(0xffffffffu, sum, w);
+            if (lane >= w) sum += o;
+        }
+        __syncthreads();
+        if (lane == 31) red[warp] = sum;
+        if (threadIdx.x == 0) found[0] = -1;
+        __syncthreads();
+        int64_t base = before, total = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            if (w < warp) base += red[w];
+            total += red[w];
+        }
+        const int64_t lo = base + sum - n, hi = base + sum;
+        if (lo <= at && at < hi) { found[0] = b; found[1] = lo; }
+        __syncthreads();
+        if (found[0] >= 0) break;
+        before += total;
+    }
+    Place p;
+    p.b = (int)found[0];
+    p.span = seq_tiles(g, p.b);
+    const int n = p.span.y - p.span.x;
+    const int64_t in = at - found[1];
+    p.unit = (int)(in / n);
+    p.tile = p.span.x + in % n;
+    return p;
+}
+
+// One piece: the tiles [t0, t1) of a unit, and where its sums go.
+struct Piece {
+    int b, kvh, rb, t0, t1;
+    bool whole;       // all of the unit's tiles
+    int slot;
+};
+
+// The pieces of a block, in order; every thread (and warp role) walks the same ones.
+struct PieceWalk {
+    Place at;
+    int64_t left;      // tiles left for this block
+    bool first;
+    __device__ __forceinline__ bool next(const DecArgs& g, Piece* p) {
+        if (left <= 0) return false;
+        const int units = g.a.hkv * g.row_blocks;
+        while (at.tile >= at.span.y || at.span.x >= at.span.y) {   // the next unit with tiles
+            if (at.span.x < at.span.y && at.unit + 1 < units) {
+                ++at.unit;
+            } else {
+                if (at.b + 1 >= g.a.b) return false;
+                ++at.b;
+                at.unit = 0;
+                at.span = seq_tiles(g, at.b);
+            }
+            at.tile = at.span.x;
+        }
+        p->b = at.b;
+        p->kvh = at.unit / g.row_blocks;
+        p->rb = at.unit % g.row_blocks;
+        p->t0 = (int)at.tile;
+        p->t1 = (int)min((int64_t)at.span.y, at.tile + left);
+        p->whole = p->t0 == at.span.x && p->t1 == at.span.y;
+        p->slot = first ? 0 : 1;
+        first = false;
+        left -= p->t1 - p->t0;
+        at.tile = p->t1;
+        return true;
+    }
+};
+
+template <int NW>
+__device__ __forceinline__ PieceWalk block_pieces(const DecArgs& g, int64_t* red, int64_t* found) {
+    PieceWalk w;
+    int64_t all;
+    tiles_before<NW>(g, 0, &all, red);
+    all *= (int64_t)g.a.hkv * g.row_blocks;
+    const int64_t per = (all + g.blocks - 1) / g.blocks, from = per * blockIdx.x;
+    w.first = true;
+    w.left = min(per, all - from);
+    if (w.left > 0) w.at = find_place<NW>(g, from, red, found);
+    return w;
+}
+
+// Row r of a unit: query i of head h.
+__device__ __forceinline__ void unit_row(const AttnCall& a, int kvh, int row, int* i, int* h) {
+    const int group = a.hq / a.hkv;
+    *i = row / group;
+    *h = kvh * group + row % group;
+}
+
+// What a row needs to score and mask keys.
+struct DecRow {
+    int p, limit, doc;
+    float slope2;
+    bool on;
+    __device__ __forceinline__ void set(const AttnCall& a, const SeqMask& mask, int b, int kvh, int row) {
+        on = row < a.nq * (a.hq / a.hkv);
+        int i, h;
+        unit_row(a, kvh, on ? row : 0, &i, &h);
+        p = mask.p0 + i;
+        limit = on ? mask.key_end(i, 1) : 0;
+        doc = a.q_doc ? a.q_doc[(int64_t)b * a.nq + i] : -1;
+        slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
+    }
+    // q.k -> score in base 2, -inf when not seen
+    __device__ __forceinline__ float score(float x, int j, int jdoc, const AttnCall& a, const CapCoef& cap) const {
+        float y = a.cap > 0.f ? cap.top * wide_tanh(x, cap.wide) : x * cap.mul;
+        y -= slope2 * fabsf((float)(p - j));
+        return j < limit && (!a.k_doc || (doc >= 0 && jdoc == doc)) ? y : -INFINITY;
+    }
+};
+
+// The end of a piece: `warps` sums of o (rows x ld fp32 each), m, l in shared
+// memory -> the output, or the block's part.
+template <typename T>
+__device__ __forceinline__ void finish_piece(const DecArgs& g, const Piece& pc, const float* o, int warps, int wstride, int ld,
+                                             const float* m, const float* l, int row0, int rows, int thread, int threads) {
+    const AttnCall& a = g.a;
+    const int total_rows = a.nq * (a.hq / a.hkv);
+    const int d2 = a.d + 2;
+    for (int e = thread; e < rows * a.d; e += threads) {
+        const int r = e / a.d, c = e % a.d;
+        const int row = pc.rb * g.rows + row0 + r;
+        if (row >= total_rows) continue;
+        float top = -INFINITY;
+        for (int w = 0; w < warps; ++w) top = fmaxf(top, m[w * rows + r]);
+        float sum = 0.f, out = 0.f;
+        for (int w = 0; w < warps; ++w) {
+            const float by = m[w * rows + r] == -INFINITY && top == -INFINITY ? 0.f : ex2(m[w * rows + r] - top);
+            sum = fmaf(by, l[w * rows + r], sum);
+            out = fmaf(by, o[(size_t)w * wstride + r * ld + c], out);
+        }
+        if (pc.whole) {
+            int i, h;
+            unit_row(a, pc.kvh, row, &i, &h);
+            const bool none = sum == 0.f;
+            static_cast<T*>(a.o.p)[pc.b * a.o.sb + h * a.o.sh + i * a.o.ss + c * a.o.sd] = from_f32<T>(none ? 0.f : out / sum);
+            if (a.lse && c == 0)
+                a.lse[((int64_t)pc.b * a.hq + h) * a.nq + i] = none ? -INFINITY : top * kLn2 + logf(sum);
+        } else {
+            float* part = g.part + ((size_t)(blockIdx.x * 2 + pc.slot) * g.rows + row0 + r) * d2;
+            part[c] = out;
+            if (c == 0) { part[a.d] = top; part[a.d + 1] = sum; }
+        }
+    }
+}
+
+// Rows of a unit that lies over several blocks, and of sequences without keys.
+template <typename T>
+__global__ void __launch_bounds__(JOIN_THREADS) k_decode_join(const __grid_constant__ DecArgs g) {
+    __shared__ int64_t red[JOIN_THREADS / 32];
+    const AttnCall& a = g.a;
+    const int units = a.hkv * g.row_blocks;
+    const int b = blockIdx.x / units, unit = blockIdx.x % units, kvh = unit / g.row_blocks, rb = unit % g.row_blocks;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int64_t all;
+    const int64_t before = tiles_before<JOIN_THREADS / 32>(g, b, &all, red) * units;
+    all *= units;
+    const int2 span = seq_tiles(g, b);
+    const int n = span.y - span.x;
+    const int64_t per = max((int64_t)1, (all + g.blocks - 1) / g.blocks);
+    const int64_t u0 = before + (int64_t)unit * n, u1 = u0 + n;
+    const int first = (int)(u0 / per), last = n ? (int)((u1 - 1) / per) : first;
+    if (n && first == last) return;   // one block wrote it
+    const int total_rows = a.nq * (a.hq / a.hkv), d2 = a.d + 2;
+    for (int e = threadIdx.x; e < g.rows * a.d; e += JOIN_THREADS) {
+        const int r = e / a.d, c = e % a.d, row = rb * g.rows + r;
+        if (row >= total_rows) continue;
+        float top = -INFINITY, sum = 0.f, out = 0.f;
+        // a block's second piece is the one that starts inside it
+        auto part = [&](int q) { return g.part + ((size_t)(q * 2 + ((int64_t)q * per < u0 ? 1 : 0)) * g.rows + r) * d2; };
+        if (n) {
+            for (int q = first; q <= last; ++q) top = fmaxf(top, part(q)[a.d]);
+            for (int q = first; q <= last; ++q) {
+                const float* p = part(q);
+                const float by = top == -INFINITY ? 0.f : ex2(p[a.d] - top);
+                sum = fmaf(by, p[a.d + 1], sum);
+                out = fmaf(by, p[c], out);
+            }
+        }
+        int i, h;
+        unit_row(a, kvh, row, &i, &h);
+        const bool none = sum == 0.f;
+        static_cast<T*>(a.o.p)[b * a.o.sb + h * a.o.sh + i * a.o.ss + c * a.o.sd] = from_f32<T>(none ? 0.f : out / sum);
+        if (a.lse && c == 0) a.lse[((int64_t)b * a.hq + h) * a.nq + i] = none ? -INFINITY : top * kLn2 + logf(sum);
+    }
+}
+
+// First and one past the last key whose document is one of a sequence's
+// queries' (a document that lies in one piece is all of that).
+__global__ void __launch_bounds__(256) k_doc_spans(const __grid_constant__ AttnCall a, int2* __restrict__ spans) {
+    __shared__ int lo, hi, dlo, dhi;
+    const int b = blockIdx.x;
+    if (threadIdx.x == 0) { lo = 0x7fffffff; hi = 0; dlo = 0x7fffffff; dhi = -1; }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.nq; i += 256) {
+        const int d = a.q_doc[(int64_t)b * a.nq + i];
+        if (d >= 0) { atomicMin(&dlo, d); atomicMax(&dhi, d); }
+    }
+    __syncthreads();
+    int first = 0x7fffffff, last = 0;
+    const int32_t* kd = a.k_doc + (int64_t)b * a.nk;
+#pragma unroll 8
+    for (int j = threadIdx.x; j < a.nk; j += 256) {
+        const int d = __ldg(kd + j);
+        if (d >= dlo && d <= dhi) { first = min(first, j); last = max(last, j + 1); }
+    }
+    atomicMin(&lo, first);
+    atomicMax(&hi, last);
+    __syncthreads();
+    if (threadIdx.x == 0) spans[b] = make_int2(min(lo, hi), hi);
+}
+
+// ---------------------------------------------------------------- tensor cores
+constexpr int DM_THREADS = 160;   // four warps of keys, one of TMA
+
+template <int DP, int MT>
+struct DmSmem {
+    static constexpr int CH = DP / 64, CHUNK = DT * 128, TILE_B = CH * CHUNK, STAGES = DP == 64 ? 8 : 4;
+    static constexpr int LQ = DP + 8;   // 16-bit query rows, padded by 16 bytes
+    static constexpr int KV = 0, Q = STAGES * 2 * TILE_B, MERGE = Q + 16 * MT * LQ * 2, LO = DP + 4,
+                         STAT = MERGE + 4 * 16 * LO * 4, BAR = STAT + 2 * 4 * 16 * MT * 4, BYTES = BAR + 256 + 1024;
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t at, uint32_t* r) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t at, uint32_t* r) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    if (TypeOf<T>::id == TL_TYPE_BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// MT: tiles of 16 rows of a unit
+template <typename T, int DP, int MT>
+__global__ void __launch_bounds__(DM_THREADS, 1)
+    k_decode_mma(const __grid_constant__ HeadMap mk, const __grid_constant__ HeadMap mv, const __grid_constant__ DecArgs g) {
+    using L = DmSmem<DP, MT>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR);
+    uint64_t* empty = full + L::STAGES;
+    __shared__ int64_t red[DM_THREADS / 32], found[2];
+    const AttnCall& a = g.a;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < L::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 4); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    PieceWalk walk = block_pieces<DM_THREADS / 32>(g, red, found);
+    __syncthreads();
+    Piece pc;
+    int n = 0;
+    bool ok = true;
+    if (warp == 4) {
+        while (ok && walk.next(g, &pc))
+            for (int t = pc.t0; t < pc.t1 && ok; ++t, ++n) {
+                const int s = n % L::STAGES;
+                if (n >= L::STAGES) ok = mbar_wait(&empty[s], ((n / L::STAGES) & 1) ^ 1, g.err);
+                ok = __all_sync(0xffffffffu, ok);
+                if (ok && lane == 0) {
+                    mbar_expect_tx(&full[s], 2 * L::TILE_B);
+                    for (int w = 0; w < 2; ++w)
+                        for (int c = 0; c < L::CH; ++c) {
+                            const HeadMap& m = w ? mv : mk;
+                            asm volatile(
+                                "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, "
+                                "%6}], [%2];" ::"r"(smem_u32(smem + L::KV + (2 * s + w) * L::TILE_B + c * L::CHUNK)),
+                                "l"(reinterpret_cast<uint64_t>(&m.map)), "r"(smem_u32(&full[s])), "r"(64 * c), "r"(t * DT),
+                                "r"(pc.kvh * m.mh), "r"(pc.b * m.mb)
+                                : "memory");
+                        }
+                }
+                __syncwarp();
+            }
+        if (!ok)
+            for (int e = max(0, n - 1 - L::STAGES); e < n - 1; ++e) mbar_wait(&full[e % L::STAGES], (e / L::STAGES) & 1, g.err);
+        return;
+    }
+
+    const CapCoef cap = cap_coef(a.scale, a.cap > 0.f ? a.cap : 1.f);
+    const int gid = lane >> 2, tid = lane & 3, mi = lane >> 3, mr = lane & 7;
+    const int ksteps = (a.d + 15) / 16;
+    T* qs = reinterpret_cast<T*>(smem + L::Q);
+    float* merge = reinterpret_cast<float*>(smem + L::MERGE);
+    float *m_s = reinterpret_cast<float*>(smem + L::STAT), *l_s = m_s + 4 * 16;
+    while (walk.next(g, &pc)) {
+        const SeqMask mask(a, pc.b);
+        const int32_t* kd = a.k_doc ? a.k_doc + (int64_t)pc.b * a.nk : nullptr;
+        // the unit's query rows (zeros past the last one and past the head size)
+        for (int e = threadIdx.x; e < 16 * MT * DP / 8; e += 128) {
+            const int r = e / (DP / 8), c = e % (DP / 8) * 8, row = pc.rb * g.rows + r;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (row < a.nq * (a.hq / a.hkv) && c < a.d) {
+                int i, h;
+                unit_row(a, pc.kvh, row, &i, &h);
+                v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.p) + pc.b * a.q.sb + h * a.q.sh + i * a.q.ss + c);
+            }
+            *reinterpret_cast<uint4*>(qs + r * L::LQ + c) = v;
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        DecRow row[MT][2];
+        float m[MT][2], l[MT][2], o[MT][DP / 8][4];
+#pragma unroll
+        for (int u = 0; u < MT; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                row[u][e].set(a, mask, pc.b, pc.kvh, pc.rb * g.rows + 16 * u + gid + 8 * e);
+                m[u][e] = -INFINITY;
+                l[u][e] = 0.f;
+            }
+#pragma unroll
+        for (int u = 0; u < MT; ++u)
+#pragma unroll
+            for (int c = 0; c < DP / 8; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[u][c][e] = 0.f;
+        for (int t = pc.t0; t < pc.t1 && ok; ++t, ++n) {
+            const int st = n % L::STAGES, j0 = t * DT + warp * 16;
+            ok = mbar_wait(&full[st], (n / L::STAGES) & 1, g.err);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            uint8_t* kt = smem + L::KV + 2 * st * L::TILE_B;
+            uint8_t* vt = kt + L::TILE_B;
+            // keys whose values must not count: 0 times what they hold could be NaN
+            const int jl = j0 + (lane & 15);
+            const int jdoc = kd && jl < a.nk ? __ldg(kd + jl) : -1;
+            const bool bad = jl >= mask.kv || (kd && jdoc < 0);
+            const bool dirty = __any_sync(0xffffffffu, bad);
+            if (dirty) {
+                if (bad && lane < 16)
+                    for (int c = 0; c < L::CH; ++c)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            *reinterpret_cast<uint4*>(vt + c * L::CHUNK + (warp * 16 + lane) * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
+                __syncwarp();
+            }
+            // scores of 16 keys: two tiles of 8 columns
+            float s[MT][2][4];
+#pragma unroll
+            for (int u = 0; u < MT; ++u)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[u][e / 4][e % 4] = 0.f;
+            {
+                const int key = warp * 16 + (mi >> 1) * 8 + mr;
+                const uint32_t kb = smem_u32(kt) + key * 128;
+                const uint32_t qb = smem_u32(qs) + ((mi & 1) * 8 + mr) * (L::LQ * 2) + (mi >> 1) * 16;
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) {
+                    if (k >= ksteps) break;
+                    const int c16 = 2 * (k % 4) + (mi & 1);
+                    uint32_t kf[4];
+                    ldsm4(kb + (k / 4) * L::CHUNK + ((c16 ^ (key & 7)) << 4), kf);
+#pragma unroll
+                    for (int u = 0; u < MT; ++u) {
+                        uint32_t qf[4];
+                        ldsm4(qb + u * 16 * L::LQ * 2 + k * 32, qf);
+                        mma16816<T>(s[u][0], qf, kf[0], kf[1]);
+                        mma16816<T>(s[u][1], qf, kf[2], kf[3]);
+                    }
+                }
+            }
+            uint32_t p[MT][4];
+#pragma unroll
+            for (int u = 0; u < MT; ++u) {
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int col = 8 * x + 2 * tid + (e & 1);
+                        const int cdoc = kd ? __shfl_sync(0xffffffffu, jdoc, col) : -1;
+                        s[u][x][e] = row[u][e >> 1].score(s[u][x][e], j0 + col, cdoc, a, cap);
+                        top[e >> 1] = fmaxf(top[e >> 1], s[u][x][e]);
+                    }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+                    top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
+                }
+                // the reference maximum moves for a row's first key and by steps of 2^8
+                const bool move = top[0] > m[u][0] + 8.f || top[1] > m[u][1] + 8.f || (m[u][0] == -INFINITY && top[0] > m[u][0]) ||
+                                  (m[u][1] == -INFINITY && top[1] > m[u][1]);
+                if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float nm = fmaxf(m[u][e], top[e]);
+                        const float by = nm == -INFINITY ? 1.f : ex2(m[u][e] - nm);
+                        m[u][e] = nm;
+                        l[u][e] *= by;
+#pragma unroll
+                        for (int c = 0; c < DP / 8; ++c) {
+                            o[u][c][2 * e] *= by;
+                            o[u][c][2 * e + 1] *= by;
+                        }
+                    }
+                }
+                float pr[2][4];
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float ref = (m[u][e >> 1] == -INFINITY ? 0.f : m[u][e >> 1]) - Lift<T>::log2;
+                        pr[x][e] = ex2(s[u][x][e] - ref);
+                        l[u][e >> 1] += pr[x][e];
+                    }
+                p[u][0] = pack16<T>(pr[0][0], pr[0][1]);
+                p[u][1] = pack16<T>(pr[0][2], pr[0][3]);
+                p[u][2] = pack16<T>(pr[1][0], pr[1][1]);
+                p[u][3] = pack16<T>(pr[1][2], pr[1][3]);
+            }
+            {
+                const int key = warp * 16 + (mi & 1) * 8 + mr;
+                const uint32_t vb = smem_u32(vt) + key * 128;
+#pragma unroll
+                for (int c = 0; c < DP / 8; c += 2) {
+                    if (8 * c >= a.d) break;
+                    const int c16 = c % 8 + (mi >> 1);
+                    uint32_t vf[4];
+                    ldsm4t(vb + (c / 8) * L::CHUNK + ((c16 ^ (key & 7)) << 4), vf);
+#pragma unroll
+                    for (int u = 0; u < MT; ++u) {
+                        mma16816<T>(o[u][c], p[u], vf[0], vf[1]);
+                        mma16816<T>(o[u][c + 1], p[u], vf[2], vf[3]);
+                    }
+                }
+            }
+            if (dirty) fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
+        }
+        // the four warps' sums, 16 rows at a time
+#pragma unroll
+        for (int u = 0; u < MT; ++u) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                l[u][e] += __shfl_xor_sync(0xffffffffu, l[u][e], 1);
+                l[u][e] += __shfl_xor_sync(0xffffffffu, l[u][e], 2);
+                if (tid == 0) {
+                    m_s[warp * 16 + gid + 8 * e] = m[u][e] == -INFINITY ? -INFINITY : m[u][e] - Lift<T>::log2;
+                    l_s[warp * 16 + gid + 8 * e] = l[u][e];
+                }
+            }
+            float* mw = merge + warp * 16 * L::LO;
+#pragma unroll
+            for (int c = 0; c < DP / 8; ++c) {
+                *reinterpret_cast<float2*>(mw + gid * L::LO + 8 * c + 2 * tid) = make_float2(o[u][c][0], o[u][c][1]);
+                *reinterpret_cast<float2*>(mw + (gid + 8) * L::LO + 8 * c + 2 * tid) = make_float2(o[u][c][2], o[u][c][3]);
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (ok) finish_piece<T>(g, pc, merge, 4, 16 * L::LO, L::LO, m_s, l_s, 16 * u, 16, threadIdx.x, 128);
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+        }
+    }
+}
+
+// ---------------------------------------------------------------- any type
+constexpr int DA_THREADS = 256;
+
+template <int DP, int RB>
+struct DaSmem {
+    static constexpr int LD = DP + 16;   // rows half of the banks apart
+    static constexpr int K = 0, V = K + DT * LD * 4, Q = V + DT * LD * 4, P = Q + RB * DP * 4, STAT = P + DT * RB * 4,
+                         BYTES = STAT + 3 * RB * 4;
+    static_assert(8 * RB * DP <= 2 * DT * LD, "the warps' sums lie over the tiles");
+};
+
+// Scores: four threads a key, each a quarter of its columns for all rows.
+// Sums: warp w takes keys w, w + 8, ... of the tile, a lane 4 columns of every
+// 128, for all rows.
+template <typename T, int DP, int RB>
+__global__ void __launch_bounds__(DA_THREADS) k_decode_any(const __grid_constant__ DecArgs g) {
+    using L = DaSmem<DP, RB>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    float *K = reinterpret_cast<float*>(smem + L::K), *V = reinterpret_cast<float*>(smem + L::V);
+    float *Q = reinterpret_cast<float*>(smem + L::Q), *P = reinterpret_cast<float*>(smem + L::P);
+    float *m_s = reinterpret_cast<float*>(smem + L::STAT), *l_s = m_s + RB, *by_s = l_s + RB;
+    __shared__ int64_t red[DA_THREADS / 32], found[2];
+    const AttnCall& a = g.a;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    PieceWalk walk = block_pieces<DA_THREADS / 32>(g, red, found);
+    const CapCoef cap = cap_coef(a.scale == 0.f ? 1.f : a.scale, a.cap > 0.f ? a.cap : 1.f);
+    const int group = a.hq / a.hkv;
+    constexpr int NC = DP >= 128 ? DP / 128 : 1, LANES = DP >= 128 ? 32 : DP / 4;
+    Piece pc;
+    while (walk.next(g, &pc)) {
+        const SeqMask mask(a, pc.b);
+        const int32_t* kd = a.k_doc ? a.k_doc + (int64_t)pc.b * a.nk : nullptr;
+        __syncthreads();
+        for (int e = threadIdx.x; e < RB * DP; e += DA_THREADS) {
+            const int r = e / DP, c = e % DP, row = pc.rb * g.rows + r;
+            float v = 0.f;
+            if (row < a.nq * group && c < a.d) {
+                int i, h;
+                unit_row(a, pc.kvh, row, &i, &h);
+                v = to_f32(static_cast<const T*>(a.q.p)[pc.b * a.q.sb + h * a.q.sh + i * a.q.ss + c * a.q.sd]);
+            }
+            Q[r * DP + c] = v;
+        }
+        if (threadIdx.x < RB) { m_s[threadIdx.x] = -INFINITY; l_s[threadIdx.x] = 0.f; }
+        float o[RB][NC][4];
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[r][c][e] = 0.f;
+        const T* kp = static_cast<const T*>(a.k.p) + pc.b * a.k.sb + pc.kvh * a.k.sh;
+        const T* vp = static_cast<const T*>(a.v.p) + pc.b * a.v.sb + pc.kvh * a.v.sh;
+        for (int t = pc.t0; t < pc.t1; ++t) {
+            const int j0 = t * DT;
+            __syncthreads();
+#pragma unroll 4
+            for (int e = threadIdx.x; e < DT * DP; e += DA_THREADS) {
+                const int r = e / DP, c = e % DP;
+                const int64_t j = j0 + r;
+                const bool on = j < mask.kv && c < a.d && (!kd || kd[j] >= 0);
+                K[r * L::LD + c] = on ? to_f32(kp[j * a.k.ss + c * a.k.sd]) : 0.f;
+                V[r * L::LD + c] = on ? to_f32(vp[j * a.v.ss + c * a.v.sd]) : 0.f;
+            }
+            __syncthreads();
+            {
+                const int key = threadIdx.x / 4, part = threadIdx.x % 4;
+                float s[RB];
+#pragma unroll
+                for (int r = 0; r < RB; ++r) s[r] = 0.f;
+#pragma unroll 4
+                for (int c = 4 * part; c < DP; c += 16) {
+                    const float4 k = *reinterpret_cast<const float4*>(K + key * L::LD + c);
+#pragma unroll
+                    for (int r = 0; r < RB; ++r) {
+                        const float4 q = *reinterpret_cast<const float4*>(Q + r * DP + c);
+                        s[r] = fmaf(k.x, q.x, fmaf(k.y, q.y, fmaf(k.z, q.z, fmaf(k.w, q.w, s[r]))));
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < RB; ++r) {
+                    s[r] += __shfl_xor_sync(0xffffffffu, s[r], 1);
+                    s[r] += __shfl_xor_sync(0xffffffffu, s[r], 2);
+                }
+                const int j = j0 + key, jdoc = kd && j < mask.kv ? kd[j] : -1;
+#pragma unroll
+                for (int r = 0; r < RB; ++r)
+                    if (r % 4 == part) {
+                        DecRow row;
+                        row.set(a, mask, pc.b, pc.kvh, pc.rb * g.rows + r);
+                        float x = s[r];
+                        float y = a.cap > 0.f ? a.cap * kLog2e * tanhf(x * (a.scale / a.cap)) : x * (a.scale * kLog2e);
+                        y -= row.slope2 * fabsf((float)(row.p - j));
+                        P[key * RB + r] = j < row.limit && (!kd || (row.doc >= 0 && jdoc == row.doc)) ? y : -INFINITY;
+                    }
+            }
+            __syncthreads();
+            // a warp's rows: maximum, exponentials, sum
+            for (int r = warp; r < RB; r += DA_THREADS / 32) {
+                const float x0 = P[lane * RB + r], x1 = P[(lane + 32) * RB + r];
+                float top = fmaxf(x0, x1);
+#pragma unroll
+                for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                const float old = m_s[r], nm = fmaxf(old, top), ref = nm == -INFINITY ? 0.f : nm;
+                const float e0 = exp2f(x0 - ref), e1 = exp2f(x1 - ref);
+                P[lane * RB + r] = e0;
+                P[(lane + 32) * RB + r] = e1;
+                float sum = e0 + e1;
+#pragma unroll
+                for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+                __syncwarp();
+                if (lane == 0) {
+                    const float by = nm == -INFINITY ? 1.f : exp2f(old - nm);
+                    by_s[r] = by;
+                    l_s[r] = l_s[r] * by + sum;
+                    m_s[r] = nm;
+                }
+            }
+            __syncthreads();
+            if (lane < LANES) {
+#pragma unroll
+                for (int r = 0; r < RB; ++r) {
+                    const float by = by_s[r];
+                    if (by != 1.f)
+#pragma unroll
+                        for (int c = 0; c < NC; ++c)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[r][c][e] *= by;
+                }
+#pragma unroll 2
+                for (int key = warp; key < DT; key += DA_THREADS / 32) {
+                    float4 v[NC];
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) v[c] = *reinterpret_cast<const float4*>(V + key * L::LD + 128 * c + 4 * lane);
+#pragma unroll
+                    for (int r = 0; r < RB; ++r) {
+                        const float p = P[key * RB + r];
+#pragma unroll
+                        for (int c = 0; c < NC; ++c) {
+                            o[r][c][0] = fmaf(p, v[c].x, o[r][c][0]);
+                            o[r][c][1] = fmaf(p, v[c].y, o[r][c][1]);
+                            o[r][c][2] = fmaf(p, v[c].z, o[r][c][2]);
+                            o[r][c][3] = fmaf(p, v[c].w, o[r][c][3]);
+                        }
+                    }
+                }
+            }
+        }
+        // the warps' sums over the tiles' memory; one maximum and sum for all
+        __syncthreads();
+        float* merge = K;
+        if (lane < LANES)
+#pragma unroll
+            for (int r = 0; r < RB; ++r)
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+                    *reinterpret_cast<float4*>(merge + (warp * RB + r) * DP + 128 * c + 4 * lane) =
+                        make_float4(o[r][c][0], o[r][c][1], o[r][c][2], o[r][c][3]);
+        __syncthreads();
+        for (int e = threadIdx.x; e < RB * DP; e += DA_THREADS) {
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) s += merge[w * RB * DP + e];
+            Q[e] = s;
+        }
+        __syncthreads();
+        finish_piece<T>(g, pc, Q, 1, 0, DP, m_s, l_s, 0, RB, threadIdx.x, DA_THREADS);
+    }
+}
+
+bool few_takes_mma(const AttnCall& a) { return attn_tc_takes(a); }
+int few_rows(const AttnCall& a) {
+    const int64_t rows = (int64_t)a.nq * (a.hq / a.hkv);
+    if (few_takes_mma(a)) return rows <= 16 ? 16 : 32;
+    return rows <= 4 ? 4 : 16;
+}
+constexpr int kSms = 148;
+int few_blocks(const AttnCall& a) { return few_takes_mma(a) || a.d > 128 ? kSms : 2 * kSms; }
+
+struct DecPlan {
+    size_t part, spans, bytes;
+    explicit DecPlan(const AttnCall& a) {
+        part = 0;
+        bytes = ((size_t)few_blocks(a) * 2 * few_rows(a) * (a.d + 2) * 4 + 255) / 256 * 256;
+        spans = bytes;
+        if (a.k_doc) bytes += ((size_t)a.b * sizeof(int2) + 255) / 256 * 256;
+    }
+};
+
+// Launches after `first`, whose blocks let the next kernel's start early.
+template <typename F, typename... A>
+cudaError_t launch_after(F* kernel, unsigned grid, int threads, int smem, cudaStream_t s, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename T, int DP, int MT>
+tl_status launch_mma(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    constexpr int smem = DmSmem<DP, MT>::BYTES;
+    TL_TRY(kernel_smem(c, k_decode_mma<T, DP, MT>, smem, done));
+    const AttnCall& a = g.a;
+    HeadMap mk, mv;
+    if (!make_head_map(&mk, a.k, a.dtype, a.b, a.hkv, a.nk, a.d, DT) || !make_head_map(&mv, a.v, a.dtype, a.b, a.hkv, a.nk, a.d, DT))
+        return fail(c, TL_ERR_CUDA, "attention: tensor maps");
+    c->flags_armed = true;
+    k_decode_mma<T, DP, MT><<<g.blocks, DM_THREADS, smem, s>>>(mk, mv, g);
+    return TL_OK;
+}
+
+template <typename T, int DP, int RB>
+tl_status launch_any(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    constexpr int smem = DaSmem<DP, RB>::BYTES;
+    TL_TRY(kernel_smem(c, k_decode_any<T, DP, RB>, smem, done));
+    k_decode_any<T, DP, RB><<<g.blocks, DA_THREADS, smem, s>>>(g);
+    return TL_OK;
+}
+
+template <typename T>
+tl_status launch_type(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
+    const AttnCall& a = g.a;
+    cudaEvent_t ev[2];
+    launch_begin_on(c, s, "attention_decode", 2.0 * a.b * a.hkv * (double)a.nk * a.d * sizeof(T), 4.0 * a.d * attn_pairs(a), ev);
+    if constexpr (!std::is_same<T, float>::value) {
+        if (few_takes_mma(a)) {
+            if (a.d <= 64) TL_TRY((g.rows == 16 ? launch_mma<T, 64, 1>(c, g, s) : launch_mma<T, 64, 2>(c, g, s)));
+            else TL_TRY((g.rows == 16 ? launch_mma<T, 128, 1>(c, g, s) : launch_mma<T, 128, 2>(c, g, s)));
+            return launch_end_on(c, s, ev);
+        }
+    }
+    if (a.d <= 64) TL_TRY((g.rows == 4 ? launch_any<T, 64, 4>(c, g, s) : launch_any<T, 64, 16>(c, g, s)));
+    else if (a.d <= 128) TL_TRY((g.rows == 4 ? launch_any<T, 128, 4>(c, g, s) : launch_any<T, 128, 16>(c, g, s)));
+    else TL_TRY((g.rows == 4 ? launch_any<T, 256, 4>(c, g, s) : launch_any<T, 256, 16>(c, g, s)));
+    return launch_end_on(c, s, ev);
+}
+
+}  // namespace
+
+bool attn_few_takes(const AttnCall& a) {
+    const int64_t rows = (int64_t)a.nq * (a.hq / a.hkv);
+    return a.nk > 0 && rows <= 64;
+}
+
+size_t attn_few_workspace(const AttnCall& a) { return DecPlan(a).bytes; }
+
+tl_status launch_attn_few(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s) {
+    const DecPlan plan(a);
+    uint8_t* w = static_cast<uint8_t*>(ws);
+    DecArgs g;
+    g.a = a;
+    g.rows = few_rows(a);
+    g.row_blocks = (int)(((int64_t)a.nq * (a.hq / a.hkv) + g.rows - 1) / g.rows);
+    g.part = reinterpret_cast<float*>(w + plan.part);
+    g.spans = nullptr;
+    g.err = c->d_flags + 8;
+    // no more blocks than tiles there can be
+    const int64_t units = (int64_t)a.b * a.hkv * g.row_blocks;
+    g.blocks = (int)std::min<int64_t>(few_blocks(a), units * ((a.nk + DT - 1) / DT));
+    cudaEvent_t ev[2];
+    if (a.k_doc) {
+        int2* spans = reinterpret_cast<int2*>(w + plan.spans);
+        g.spans = spans;
+        launch_begin_on(c, s, "attention_doc_spans", 4.0 * a.b * a.nk, 0, ev);
+        k_doc_spans<<<a.b, 256, 0, s>>>(a, spans);
+        TL_TRY(launch_end_on(c, s, ev));
+    }
+    switch (a.dtype) {
+    case TL_TYPE_F32: TL_TRY(launch_type<float>(c, g, s)); break;
+    case TL_TYPE_F16: TL_TRY(launch_type<__half>(c, g, s)); break;
+    default: TL_TRY(launch_type<__nv_bfloat16>(c, g, s));
+    }
+    launch_begin_on(c, s, "attention_decode_join", 0, 0, ev);
+    cudaError_t e;
+    switch (a.dtype) {
+    case TL_TYPE_F32: e = launch_after(k_decode_join<float>, (unsigned)units, JOIN_THREADS, 0, s, g); break;
+    case TL_TYPE_F16: e = launch_after(k_decode_join<__half>, (unsigned)units, JOIN_THREADS, 0, s, g); break;
+    default: e = launch_after(k_decode_join<__nv_bfloat16>, (unsigned)units, JOIN_THREADS, 0, s, g);
+    }
+    TL_CK(c, e);
+    return launch_end_on(c, s, ev);
+}
+
+}  // namespace tl

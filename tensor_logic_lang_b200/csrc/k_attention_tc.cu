@@ -465,7 +465,7 @@ bool attn_tc_takes(const AttnCall& a) {
            tc_array(a.k, a.b, a.hkv, a.nk) && tc_array(a.v, a.b, a.hkv, a.nk) && tc_array(a.o, a.b, a.hq, a.nq) && a.nk > 0;
 }
 
-bool make_head_map(HeadMap* m, const HeadsView& v, int dtype, int b, int h, int64_t n, int d) {
+bool make_head_map(HeadMap* m, const HeadsView& v, int dtype, int b, int h, int64_t n, int d, int box_rows) {
     typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -483,7 +483,7 @@ bool make_head_map(HeadMap* m, const HeadsView& v, int dtype, int b, int h, int6
     cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)n, m->mh ? (cuuint64_t)h : 1, m->mb ? (cuuint64_t)b : 1};
     const int64_t row = n > 1 ? v.ss : (d + 7) / 8 * 8;
     cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)(m->mh ? v.sh : row) * 2, (cuuint64_t)(m->mb ? v.sb : row) * 2};
-    cuuint32_t box[4] = {64, TILE, 1, 1}, one[4] = {1, 1, 1, 1};
+    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, one[4] = {1, 1, 1, 1};
     return enc(&m->map, dtype == TL_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, v.p, dims,
                strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;

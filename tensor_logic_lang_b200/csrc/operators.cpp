@@ -239,6 +239,7 @@ tl_status check_attention(tl_ctx* c, const tl_attention& t, bool backward, AttnC
 
 size_t attention_need(const AttnCall& a, bool backward) {
     if (backward && attn_tc_backward_takes(a)) return attn_tc_backward_workspace(a);
+    if (!backward && attn_few_takes(a)) return attn_few_workspace(a);
     if (!backward && attn_tc_takes(a)) return attn_tc_workspace(a);
     return attn_general_workspace(a, backward);
 }
@@ -258,6 +259,7 @@ tl_status run_attention(tl_ctx* c, const tl_attention* t, bool backward) {
     TL_TRY(op_workspace(c, s, capturing, attention_need(a, backward), t->workspace, t->workspace_bytes, &ws));
     if (backward)
         return attn_tc_backward_takes(a) ? launch_attn_tc_backward(c, a, ws, s) : launch_attn_general_backward(c, a, ws, s);
+    if (attn_few_takes(a)) return launch_attn_few(c, a, ws, s);
     return attn_tc_takes(a) ? launch_attn_tc(c, a, ws, s) : launch_attn_general(c, a, ws, s);
 }
 
