@@ -74,6 +74,24 @@ tl_status kernel_smem(tl_ctx* c, F* kernel, int bytes, std::atomic<uint64_t>& do
     return TL_OK;
 }
 
+// A launch whose blocks may start when every block of the kernel before it in
+// the stream has said griddepcontrol.launch_dependents; they wait for its
+// results with griddepcontrol.wait.
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), unsigned grid, int threads, int smem, cudaStream_t s, const A&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 inline size_t type_size(int dtype) { return dtype == TL_TYPE_F32 ? 4 : 2; }
 
 // algorithmic work of a call for the profile: every pair of a query and a key

@@ -12,8 +12,8 @@
 //
 //   k_decode_mma   16-bit types with aligned rows and head sizes up to 128: TMA
 //                  tiles (128-byte swizzle) through a ring; each of four
-//                  warps takes 16 keys of a tile for all rows, with
-//                  mma.sync.m16n8k16 (at a few rows a key the tensor work is a
+//                  warps takes 16 keys of a tile for all rows (two sets of
+//                  four take the tiles in turn), with mma.sync.m16n8k16 (at a few rows a key the tensor work is a
 //                  fraction of the time the key's bytes take)
 //   k_decode_any   any type, stride and head size: tiles as fp32 in shared
 //                  memory, FFMA
@@ -25,7 +25,7 @@ namespace tl {
 namespace {
 
 constexpr int DT = 64;                // keys of a tile
-constexpr int JOIN_THREADS = 256;
+constexpr int JOIN_THREADS = 128;
 
 struct DecArgs {
     AttnCall a;
@@ -72,6 +72,14 @@ __device__ __forceinline__ int64_t tiles_before(const DecArgs& g, int upto, int6
         t += s.y - s.x;
         if (b < upto) p += s.y - s.x;
     }
+    // two sums in one reduction: a sequence has less than 2^24 tiles of 64 keys
+    // and a call at most 2^29 sequences, so the halves are taken apart only
+    // where both fit (else one after the other)
+    if (g.a.b <= 256) {
+        const int64_t both = block_total<NW>(t << 32 | p, red);
+        *all = both >> 32;
+        return both & 0xffffffff;
+    }
     *all = block_total<NW>(t, red);
     return block_total<NW>(p, red);
 }
@@ -83,11 +91,24 @@ struct Place {
     int64_t tile;      // next tile (span.x ..)
 };
 
-// The place of tile number `at` of the line (at < all tiles); any thread count.
+// The place where a block's share of the line starts, and its length (0: it
+// has none).  The shares are equal, in the order of the blocks.
 template <int NW>
-__device__ __forceinline__ Place find_place(const DecArgs& g, int64_t at, int64_t* red, int64_t* found) {
+__device__ __forceinline__ Place find_place(const DecArgs& g, int64_t* left, int64_t* red, int64_t* found) {
     const int units = g.a.hkv * g.row_blocks, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    int64_t before = 0;
+    const bool once = g.a.b <= NW * 32;   // one sequence a thread: the sum of all comes with the scan
+    int64_t all = 0, before = 0, at = 0;
+    if (!once) {
+        int64_t t = 0;
+        for (int b = threadIdx.x; b < g.a.b; b += NW * 32) {
+            const int2 s = seq_tiles(g, b);
+            t += s.y - s.x;
+        }
+        all = block_total<NW>(t, red) * units;
+    }
+    Place p;
+    p.b = 0; p.unit = 0; p.span = make_int2(0, 0); p.tile = 0;
+    *left = 0;
     for (int b0 = 0; b0 < g.a.b; b0 += NW * 32) {
         const int b = b0 + threadIdx.x;
         int64_t n = 0;
@@ -111,13 +132,19 @@ __device__ __forceinline__ Place find_place(const DecArgs& g, int64_t at, int64_
             if (w < warp) base += red[w];
             total += red[w];
         }
+        if (once) all = total;
+        if (b0 == 0) {
+            const int64_t per = (all + g.blocks - 1) / g.blocks;
+            at = per * blockIdx.x;
+            *left = min(per, all - at);
+            if (*left <= 0) return p;
+        }
         const int64_t lo = base + sum - n, hi = base + sum;
         if (lo <= at && at < hi) { found[0] = b; found[1] = lo; }
         __syncthreads();
         if (found[0] >= 0) break;
         before += total;
     }
-    Place p;
     p.b = (int)found[0];
     p.span = seq_tiles(g, p.b);
     const int n = p.span.y - p.span.x;
@@ -170,13 +197,8 @@ struct PieceWalk {
 template <int NW>
 __device__ __forceinline__ PieceWalk block_pieces(const DecArgs& g, int64_t* red, int64_t* found) {
     PieceWalk w;
-    int64_t all;
-    tiles_before<NW>(g, 0, &all, red);
-    all *= (int64_t)g.a.hkv * g.row_blocks;
-    const int64_t per = (all + g.blocks - 1) / g.blocks, from = per * blockIdx.x;
     w.first = true;
-    w.left = min(per, all - from);
-    if (w.left > 0) w.at = find_place<NW>(g, from, red, found);
+    w.at = find_place<NW>(g, &w.left, red, found);
     return w;
 }
 
@@ -215,12 +237,10 @@ template <typename T>
 __device__ __forceinline__ void finish_piece(const DecArgs& g, const Piece& pc, const float* o, int warps, int wstride, int ld,
                                              const float* m, const float* l, int row0, int rows, int thread, int threads) {
     const AttnCall& a = g.a;
-    const int total_rows = a.nq * (a.hq / a.hkv);
-    const int d2 = a.d + 2;
-    for (int e = thread; e < rows * a.d; e += threads) {
+    const int d2 = a.d + 2, used = min(rows, a.nq * (a.hq / a.hkv) - pc.rb * g.rows - row0);
+    for (int e = thread; e < used * a.d; e += threads) {
         const int r = e / a.d, c = e % a.d;
         const int row = pc.rb * g.rows + row0 + r;
-        if (row >= total_rows) continue;
         float top = -INFINITY;
         for (int w = 0; w < warps; ++w) top = fmaxf(top, m[w * rows + r]);
         float sum = 0.f, out = 0.f;
@@ -244,32 +264,35 @@ __device__ __forceinline__ void finish_piece(const DecArgs& g, const Piece& pc, 
     }
 }
 
-// Rows of a unit that lies over several blocks, and of sequences without keys.
+// A block a row: rows of units that lie over several blocks, and of sequences
+// without keys.
 template <typename T>
 __global__ void __launch_bounds__(JOIN_THREADS) k_decode_join(const __grid_constant__ DecArgs g) {
     __shared__ int64_t red[JOIN_THREADS / 32];
     const AttnCall& a = g.a;
-    const int units = a.hkv * g.row_blocks;
-    const int b = blockIdx.x / units, unit = blockIdx.x % units, kvh = unit / g.row_blocks, rb = unit % g.row_blocks;
+    const int rows = a.nq * (a.hq / a.hkv), units = a.hkv * g.row_blocks;
+    const int row = blockIdx.x % rows, kvh = blockIdx.x / rows % a.hkv, b = blockIdx.x / rows / a.hkv;
+    const int unit = kvh * g.row_blocks + row / g.rows, r = row % g.rows;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     int64_t all;
     const int64_t before = tiles_before<JOIN_THREADS / 32>(g, b, &all, red) * units;
     all *= units;
     const int2 span = seq_tiles(g, b);
-    const int n = span.y - span.x;
+    const int n = span.y - span.x, d2 = a.d + 2;
     const int64_t per = max((int64_t)1, (all + g.blocks - 1) / g.blocks);
     const int64_t u0 = before + (int64_t)unit * n, u1 = u0 + n;
     const int first = (int)(u0 / per), last = n ? (int)((u1 - 1) / per) : first;
     if (n && first == last) return;   // one block wrote it
-    const int total_rows = a.nq * (a.hq / a.hkv), d2 = a.d + 2;
-    for (int e = threadIdx.x; e < g.rows * a.d; e += JOIN_THREADS) {
-        const int r = e / a.d, c = e % a.d, row = rb * g.rows + r;
-        if (row >= total_rows) continue;
+    int i, h;
+    unit_row(a, kvh, row, &i, &h);
+    // a block's second piece is the one that starts inside it
+    auto part = [&](int q) { return g.part + ((size_t)(q * 2 + ((int64_t)q * per < u0 ? 1 : 0)) * g.rows + r) * d2; };
+    for (int c = threadIdx.x; c < a.d; c += JOIN_THREADS) {
         float top = -INFINITY, sum = 0.f, out = 0.f;
-        // a block's second piece is the one that starts inside it
-        auto part = [&](int q) { return g.part + ((size_t)(q * 2 + ((int64_t)q * per < u0 ? 1 : 0)) * g.rows + r) * d2; };
         if (n) {
+#pragma unroll 4
             for (int q = first; q <= last; ++q) top = fmaxf(top, part(q)[a.d]);
+#pragma unroll 4
             for (int q = first; q <= last; ++q) {
                 const float* p = part(q);
                 const float by = top == -INFINITY ? 0.f : ex2(p[a.d] - top);
@@ -277,8 +300,6 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_decode_join(const __grid_const
                 out = fmaf(by, p[c], out);
             }
         }
-        int i, h;
-        unit_row(a, kvh, row, &i, &h);
         const bool none = sum == 0.f;
         static_cast<T*>(a.o.p)[b * a.o.sb + h * a.o.sh + i * a.o.ss + c * a.o.sd] = from_f32<T>(none ? 0.f : out / sum);
         if (a.lse && c == 0) a.lse[((int64_t)b * a.hq + h) * a.nq + i] = none ? -INFINITY : top * kLn2 + logf(sum);
@@ -311,14 +332,15 @@ __global__ void __launch_bounds__(256) k_doc_spans(const __grid_constant__ AttnC
 }
 
 // ---------------------------------------------------------------- tensor cores
-constexpr int DM_THREADS = 160;   // four warps of keys, one of TMA
+constexpr int DM_SETS = 2, DM_WARPS = 4 * DM_SETS;   // sets of four warps take the tiles in turn
+constexpr int DM_THREADS = 32 * (DM_WARPS + 1);      // and one warp of TMA
 
 template <int DP, int MT>
 struct DmSmem {
     static constexpr int CH = DP / 64, CHUNK = DT * 128, TILE_B = CH * CHUNK, STAGES = DP == 64 ? 8 : 4;
     static constexpr int LQ = DP + 8;   // 16-bit query rows, padded by 16 bytes
     static constexpr int KV = 0, Q = STAGES * 2 * TILE_B, MERGE = Q + 16 * MT * LQ * 2, LO = DP + 4,
-                         STAT = MERGE + 4 * 16 * LO * 4, BAR = STAT + 2 * 4 * 16 * MT * 4, BYTES = BAR + 256 + 1024;
+                         STAT = MERGE + DM_WARPS * 16 * LO * 4, BAR = STAT + 2 * DM_WARPS * 16 * 4, BYTES = BAR + 256 + 1024;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t at, uint32_t* r) {
@@ -367,7 +389,7 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
     Piece pc;
     int n = 0;
     bool ok = true;
-    if (warp == 4) {
+    if (warp == DM_WARPS) {
         while (ok && walk.next(g, &pc))
             for (int t = pc.t0; t < pc.t1 && ok; ++t, ++n) {
                 const int s = n % L::STAGES;
@@ -398,12 +420,13 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
     const int ksteps = (a.d + 15) / 16;
     T* qs = reinterpret_cast<T*>(smem + L::Q);
     float* merge = reinterpret_cast<float*>(smem + L::MERGE);
-    float *m_s = reinterpret_cast<float*>(smem + L::STAT), *l_s = m_s + 4 * 16;
+    float *m_s = reinterpret_cast<float*>(smem + L::STAT), *l_s = m_s + DM_WARPS * 16;
+    const int set = warp / 4, sub = warp % 4;
     while (walk.next(g, &pc)) {
         const SeqMask mask(a, pc.b);
         const int32_t* kd = a.k_doc ? a.k_doc + (int64_t)pc.b * a.nk : nullptr;
         // the unit's query rows (zeros past the last one and past the head size)
-        for (int e = threadIdx.x; e < 16 * MT * DP / 8; e += 128) {
+        for (int e = threadIdx.x; e < 16 * MT * DP / 8; e += 32 * DM_WARPS) {
             const int r = e / (DP / 8), c = e % (DP / 8) * 8, row = pc.rb * g.rows + r;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (row < a.nq * (a.hq / a.hkv) && c < a.d) {
@@ -413,7 +436,7 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
             }
             *reinterpret_cast<uint4*>(qs + r * L::LQ + c) = v;
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * DM_WARPS) : "memory");
         DecRow row[MT][2];
         float m[MT][2], l[MT][2], o[MT][DP / 8][4];
 #pragma unroll
@@ -431,7 +454,8 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[u][c][e] = 0.f;
         for (int t = pc.t0; t < pc.t1 && ok; ++t, ++n) {
-            const int st = n % L::STAGES, j0 = t * DT + warp * 16;
+            if (n % DM_SETS != set) continue;
+            const int st = n % L::STAGES, j0 = t * DT + sub * 16;
             ok = mbar_wait(&full[st], (n / L::STAGES) & 1, g.err);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -447,7 +471,7 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
                     for (int c = 0; c < L::CH; ++c)
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
-                            *reinterpret_cast<uint4*>(vt + c * L::CHUNK + (warp * 16 + lane) * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(vt + c * L::CHUNK + (sub * 16 + lane) * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
                 __syncwarp();
             }
             // scores of 16 keys: two tiles of 8 columns
@@ -457,7 +481,7 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[u][e / 4][e % 4] = 0.f;
             {
-                const int key = warp * 16 + (mi >> 1) * 8 + mr;
+                const int key = sub * 16 + (mi >> 1) * 8 + mr;
                 const uint32_t kb = smem_u32(kt) + key * 128;
                 const uint32_t qb = smem_u32(qs) + ((mi & 1) * 8 + mr) * (L::LQ * 2) + (mi >> 1) * 16;
 #pragma unroll
@@ -525,7 +549,7 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
                 p[u][3] = pack16<T>(pr[1][2], pr[1][3]);
             }
             {
-                const int key = warp * 16 + (mi & 1) * 8 + mr;
+                const int key = sub * 16 + (mi & 1) * 8 + mr;
                 const uint32_t vb = smem_u32(vt) + key * 128;
 #pragma unroll
                 for (int c = 0; c < DP / 8; c += 2) {
@@ -544,7 +568,7 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[st]);
         }
-        // the four warps' sums, 16 rows at a time
+        // the warps' sums, 16 rows at a time
 #pragma unroll
         for (int u = 0; u < MT; ++u) {
 #pragma unroll
@@ -562,9 +586,9 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
                 *reinterpret_cast<float2*>(mw + gid * L::LO + 8 * c + 2 * tid) = make_float2(o[u][c][0], o[u][c][1]);
                 *reinterpret_cast<float2*>(mw + (gid + 8) * L::LO + 8 * c + 2 * tid) = make_float2(o[u][c][2], o[u][c][3]);
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (ok) finish_piece<T>(g, pc, merge, 4, 16 * L::LO, L::LO, m_s, l_s, 16 * u, 16, threadIdx.x, 128);
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * DM_WARPS) : "memory");
+            if (ok) finish_piece<T>(g, pc, merge, DM_WARPS, 16 * L::LO, L::LO, m_s, l_s, 16 * u, 16, threadIdx.x, 32 * DM_WARPS);
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * DM_WARPS) : "memory");
         }
     }
 }
@@ -759,22 +783,6 @@ struct DecPlan {
     }
 };
 
-// Launches after `first`, whose blocks let the next kernel's start early.
-template <typename F, typename... A>
-cudaError_t launch_after(F* kernel, unsigned grid, int threads, int smem, cudaStream_t s, A... args) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <typename T, int DP, int MT>
 tl_status launch_mma(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
@@ -836,7 +844,7 @@ tl_status launch_attn_few(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s
     g.spans = nullptr;
     g.err = c->d_flags + 8;
     // no more blocks than tiles there can be
-    const int64_t units = (int64_t)a.b * a.hkv * g.row_blocks;
+    const int64_t units = (int64_t)a.b * a.hkv * g.row_blocks, rows = (int64_t)a.nq * (a.hq / a.hkv);
     g.blocks = (int)std::min<int64_t>(few_blocks(a), units * ((a.nk + DT - 1) / DT));
     cudaEvent_t ev[2];
     if (a.k_doc) {
@@ -854,9 +862,9 @@ tl_status launch_attn_few(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s
     launch_begin_on(c, s, "attention_decode_join", 0, 0, ev);
     cudaError_t e;
     switch (a.dtype) {
-    case TL_TYPE_F32: e = launch_after(k_decode_join<float>, (unsigned)units, JOIN_THREADS, 0, s, g); break;
-    case TL_TYPE_F16: e = launch_after(k_decode_join<__half>, (unsigned)units, JOIN_THREADS, 0, s, g); break;
-    default: e = launch_after(k_decode_join<__nv_bfloat16>, (unsigned)units, JOIN_THREADS, 0, s, g);
+    case TL_TYPE_F32: e = launch_early(k_decode_join<float>, (unsigned)((int64_t)a.b * a.hkv * rows), JOIN_THREADS, 0, s, g); break;
+    case TL_TYPE_F16: e = launch_early(k_decode_join<__half>, (unsigned)((int64_t)a.b * a.hkv * rows), JOIN_THREADS, 0, s, g); break;
+    default: e = launch_early(k_decode_join<__nv_bfloat16>, (unsigned)((int64_t)a.b * a.hkv * rows), JOIN_THREADS, 0, s, g);
     }
     TL_CK(c, e);
     return launch_end_on(c, s, ev);

@@ -8,6 +8,7 @@ fallback: without the built library or a GPU, construction raises.
 """
 import ctypes as C
 import struct
+from operator import methodcaller
 
 import numpy as np
 
@@ -16,9 +17,11 @@ from . import abi
 
 # tl_array: data, dtype, rank, dims[4], strides[4]
 _ARRAY = struct.Struct("=Qii4q4q")
+_LIST = np.dtype([("data", "u8"), ("dtype", "i4"), ("rank", "i4"), ("dims", "i8", 4), ("strides", "i8", 4)])
 _TYPES = {"torch.float32": abi.TL_TYPE_F32, "torch.float16": abi.TL_TYPE_F16, "torch.bfloat16": abi.TL_TYPE_BF16,
           "float32": abi.TL_TYPE_F32, "float16": abi.TL_TYPE_F16, "bfloat16": abi.TL_TYPE_BF16}
 _type_of = {}          # dtype object -> TL_TYPE_*
+_DATA, _NUMEL, _DEVICE, _IS_CONTIGUOUS = (methodcaller(n) for n in ("data_ptr", "numel", "get_device", "is_contiguous"))
 _ATTENTION_AT = {n: getattr(abi.Attention, n).offset for n, _ in abi.Attention._fields_}
 _ATTENTION_TAIL = struct.Struct("=QffiiQQQQQQQqQ")   # lse .. stream
 
@@ -171,8 +174,8 @@ class Context:
         return buf.value.decode()
 
     # ------------------------------------------------------------------ array operators
-    # Arrays are device tensors (torch's, or any object with data_ptr(), dtype,
-    # shape, stride() and device), or names of this context's tensors, which
+    # Arrays are device tensors (torch's, or any object with their data_ptr(), dtype,
+    # shape, stride(), get_device(), numel() and is_contiguous()), or names of this context's tensors, which
     # stand for their fp32 storage.  stream: a cudaStream_t handle (torch's
     # current stream: torch.cuda.current_stream().cuda_stream), or None for the
     # context's own stream, on which its programs run.  Device tensors that
@@ -183,19 +186,22 @@ class Context:
             a = abi.Array()
             self.check(self.lib.tl_tensor_array(self._lookup(x), 1 if write else 0, C.byref(a)), f"{what} {x}")
             return a.data or 0, a.dtype, tuple(a.dims[:a.rank]), tuple(a.strides[:a.rank])
-        dt = x.dtype
-        t = _type_of.get(dt)
+        t = _type_of.get(x.dtype)
         if t is None:
-            t = _type_of[dt] = _TYPES.get(str(dt), -1)
-        if t < 0:
-            raise abi.TLError(abi.TL_ERR_INVALID, f"{what}: element type {dt}, not float32, float16 or bfloat16")
+            t = self._type(x.dtype, what)
         self._on_device(x, what)
-        return x.data_ptr(), t, tuple(x.shape), x.stride()
+        return x.data_ptr(), t, x.shape, x.stride()
+
+    def _type(self, dtype, what):
+        t = _TYPES.get(str(dtype))
+        if t is None:
+            raise abi.TLError(abi.TL_ERR_INVALID, f"{what}: element type {dtype}, not float32, float16 or bfloat16")
+        _type_of[dtype] = t
+        return t
 
     def _on_device(self, x, what):
-        d = x.device
-        if d.type != "cuda" or (d.index or 0) != self.device:
-            raise abi.TLError(abi.TL_ERR_INVALID, f"{what} is on {d}, the context on cuda:{self.device}")
+        if x.get_device() != self.device:
+            raise abi.TLError(abi.TL_ERR_INVALID, f"{what} is on {x.device}, the context on cuda:{self.device}")
 
     def _heads(self, buf, field, x, what, write=False):
         """Packs [heads and positions] of rank 2 to 4 as [batch, heads, positions, head size]."""
@@ -204,7 +210,7 @@ class Context:
         if r != 4:
             if r < 2 or r > 4:
                 raise abi.TLError(abi.TL_ERR_INVALID, f"attention: {what} has rank {r}, not 2 to 4")
-            shape, strides = (1,) * (4 - r) + shape, (0,) * (4 - r) + tuple(strides)
+            shape, strides = (1,) * (4 - r) + tuple(shape), (0,) * (4 - r) + tuple(strides)
         _ARRAY.pack_into(buf, _ATTENTION_AT[field], p, t, 4, *shape, *strides)
         return shape
 
@@ -221,6 +227,8 @@ class Context:
             if str(x.dtype).rpartition(".")[2] != kind or not x.is_contiguous():
                 raise abi.TLError(abi.TL_ERR_INVALID, f"{what} is not a contiguous array of {kind}")
             p, have = x.data_ptr(), tuple(x.shape)
+        if have == shape:
+            return p
         n = 1
         for k in shape:
             n *= k
@@ -300,28 +308,36 @@ class Context:
         return n
 
     def _list(self, arrays, what, write):
-        buf = bytearray(_ARRAY.size * len(arrays))
-        at = 0
-        for x in arrays:
+        """Packs arrays as tl_array (a contiguous one as its elements in a row)."""
+        out = np.zeros(len(arrays), _LIST)
+        if not any(isinstance(x, str) for x in arrays) and all(map(_IS_CONTIGUOUS, arrays)):
+            # a column at a time: lists are long
+            for d in set(map(_DEVICE, arrays)) - {self.device}:
+                raise abi.TLError(abi.TL_ERR_INVALID, f"{what} on device {d}, the context on cuda:{self.device}")
+            types = [x.dtype for x in arrays]
+            for t in set(types) - _type_of.keys():
+                self._type(t, what)
+            n = len(arrays)
+            out["data"] = np.fromiter(map(_DATA, arrays), np.uint64, n)
+            out["dtype"] = [_type_of[t] for t in types]
+            out["rank"] = 1
+            out["dims"][:, 0] = np.fromiter(map(_NUMEL, arrays), np.int64, n)
+            out["strides"][:, 0] = 1
+            return out
+        for a, x in zip(out, arrays):
             p, t, shape, strides = self._view(x, what, write)
             r = len(shape)
             if r > abi.TL_ARRAY_RANK:
                 if not x.is_contiguous():
                     raise abi.TLError(abi.TL_ERR_INVALID, f"{what}: rank {r} and not contiguous")
                 shape, strides, r = (x.numel(),), (1,), 1
-            pad = (0,) * (4 - r)
-            _ARRAY.pack_into(buf, at, p, t, r, *shape, *pad, *strides, *pad)
-            at += _ARRAY.size
-        return buf
+            a["data"], a["dtype"], a["rank"], a["dims"][:r], a["strides"][:r] = p, t, r, shape, strides
+        return out
 
     def _clip_lists(self, grads, out):
         if out is not None and len(out) != len(grads):
             raise abi.TLError(abi.TL_ERR_INVALID, f"clip: {len(out)} outputs for {len(grads)} gradients")
-
-        def at(arrays, what, write):
-            buf = self._list(arrays, what, write) or bytearray(1)
-            return (C.c_char * len(buf)).from_buffer(buf)
-        return at(grads, "gradient", out is None), None if out is None else at(out, "output", True)
+        return self._list(grads, "gradient", out is None), None if out is None else self._list(out, "output", True)
 
     def clip_gradients(self, grads, max_norm, out=None, norm=None, workspace=None, stream=None):
         """Scales the arrays so that their global norm is at most max_norm (tl_clip_gradients).
@@ -331,13 +347,14 @@ class Context:
         """
         a, o = self._clip_lists(grads, out)
         at = self._plain(norm, "norm", "float32", ())
-        self.check(self.lib.tl_clip_gradients(self.h, a, o, len(grads), max_norm, at, *self._room(workspace),
-                                              self._stream(stream)), "clip_gradients")
+        self.check(self.lib.tl_clip_gradients(self.h, a.ctypes.data, o if o is None else o.ctypes.data, len(grads), max_norm,
+                                              at, *self._room(workspace), self._stream(stream)), "clip_gradients")
         return grads if out is None else out
 
     def clip_workspace(self, grads, max_norm, out=None):
         """Bytes of workspace of a clip_gradients call."""
-        n = self.lib.tl_clip_workspace(self.h, *self._clip_lists(grads, out), len(grads), max_norm)
+        a, o = self._clip_lists(grads, out)
+        n = self.lib.tl_clip_workspace(self.h, a.ctypes.data, o if o is None else o.ctypes.data, len(grads), max_norm)
         self.check(max(0, -n), "clip_workspace")
         return n
 
