@@ -460,15 +460,19 @@ tl_status tl_tensor_array(tl_tensor* t, int32_t write, tl_array* out);
  * A query that sees no key gives o = 0 and lse = -inf, and takes and gives no
  * gradient.  What k and v hold at and after kv_len[b] and at keys of a negative
  * document, and q and dout at queries of a negative document, does not matter,
- * not even infinities or NaN; elsewhere a value that is not finite reaches the
- * results as it does in the formulas (0 times infinity included).
+ * not even infinities or NaN; elsewhere a value that is not finite reaches
+ * every result it would reach in the formulas (0 times infinity included), and
+ * may reach others of the same tile of queries or keys.
  *
  * Arrays of rank 4, [batch, heads, positions, head size], of one type, head
  * size 1..256, any strides (k and v may have strides of 0; arrays that are
- * written may not overlap themselves, one another or an input).  fp32 is
- * computed in fp32; 16-bit types take their products from 16-bit operands
- * (scores' exponentials and dx rounded to them) with 32-bit sums, the softmax
- * and its statistics in 32 bits.
+ * written may not overlap themselves, one another or an input).  Sums, the
+ * softmax and its statistics are in 32 bits.  16-bit types take their products
+ * from 16-bit operands (exponentials, and dx of the backward pass, rounded to
+ * them).  fp32 arrays are computed in fp32, those of head size up to 64 with 22
+ * bits of each operand of a product, or 2^-39 of the largest of its kind in
+ * the heads that share a key head where that is more; a value that is not finite
+ * then makes the results that depend on it NaN.
  * The device arrays slopes [Hq] fp32 (constants: they get no gradient),
  * prefix_len, kv_len, q_start [batch] int32, q_doc [batch, Nq] and
  * k_doc [batch, Nk] int32 are contiguous.  kv_len NULL: all Nk keys; its values

@@ -1,5 +1,5 @@
 // Device pieces shared by the tensor-core attention kernels (16-bit operands,
-// head size up to 128).
+// head size up to 128; fp32 arrays of head size up to 64 as pairs of fp16).
 //
 // Operand tiles are 128 rows of one head in shared memory as one or two
 // chunks of 64 columns (16 KB each, 128-byte swizzle), which TMA writes from a
@@ -24,6 +24,46 @@ constexpr float kLn2 = 0.6931471805599453f;
 // below 2^15.
 template <typename T> struct Lift { static constexpr float log2 = 0.f; };
 template <> struct Lift<__half> { static constexpr float log2 = 6.f; };
+
+// ---------------------------------------------------------------- packed fp32
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2(float lo, float hi) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(f2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+template <typename T> __device__ __forceinline__ uint32_t pack16(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <> __device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
 
 // ---------------------------------------------------------------- tcgen05
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -105,6 +145,101 @@ __device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a, uint32_t b, uin
         umma_f16_ts(d, a + 8 * k, umma_desc(b + k * 2048, CHUNK_BYTES, 1024, kLayoutSW128), idesc, accumulate | (k > 0));
 }
 
+// The same with operands in two parts (x = hi + lo, see SplitPlan): chunk 0 of a
+// tile holds hi, chunk 1 lo.  lo hi + hi lo + hi hi; lo lo, 2^-22 of the
+// product, is left out.  The small products go first: the tensor cores cut
+// their fp32 sums (2^-23 of the sum a step), so the large sum should see few
+// steps.
+template <typename T>
+__device__ __forceinline__ void mma_rows_split(uint32_t d, uint32_t a, uint32_t b, int ksteps) {
+    constexpr uint32_t idesc = f16_idesc<T>(TILE, false);
+#pragma unroll
+    for (int part = 0; part < 3; ++part) {
+        const uint32_t pa = part == 0 ? CHUNK_BYTES : 0, pb = part == 1 ? CHUNK_BYTES : 0;
+        for (int k = 0; k < ksteps; ++k)
+            umma_f16_ss(d, umma_desc(a + pa + k * 32, 16, 1024, kLayoutSW128), umma_desc(b + pb + k * 32, 16, 1024, kLayoutSW128),
+                        idesc, part > 0 || k > 0);
+    }
+}
+// D = A B anew (the caller adds the tiles up in fp32): A's parts in TMEM at
+// acol(part, k), k steps of 16 rows of the tile.
+template <typename T, typename F>
+__device__ __forceinline__ void mma_cols_split(uint32_t d, uint32_t b, uint32_t idesc, F acol) {
+#pragma unroll
+    for (int part = 0; part < 3; ++part)
+#pragma unroll
+        for (int k = 0; k < TILE / 16; ++k)
+            umma_f16_ts(d, acol(part == 0 ? 1 : 0, k),
+                        umma_desc(b + (part == 1 ? CHUNK_BYTES : 0) + k * 2048, CHUNK_BYTES, 1024, kLayoutSW128), idesc,
+                        part > 0 || k > 0);
+}
+// hi and lo of a pair of values as fp16 pairs
+__device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t& lo) {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(b), "f"(a));
+    const __half2 h = *reinterpret_cast<const __half2*>(&hi);
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(b - __high2float(h)), "f"(a - __low2float(h)));
+}
+// N TMEM columns at acc = columns at `from` + (fresh: 0, else what is there)
+template <int N>
+__device__ __forceinline__ void tmem_add(uint32_t acc, uint32_t from, bool fresh) {
+#pragma unroll 1
+    for (int k = 0; k < N; k += 32) {
+        uint32_t x[32], y[32];
+        tmem_ld32(from + k, x);
+        if (!fresh) tmem_ld32(acc + k, y);
+        tmem_wait_ld();
+        if (!fresh)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) + __uint_as_float(y[i]));
+        tmem_st32(acc + k, x);
+    }
+}
+
+// A row of DP fp32 sums in TMEM, scaled, as values of an array: 16-bit rows
+// are 16-byte aligned (tc_array), fp32 ones may lie anyhow.  any: there are sums
+// (else zeros); live: the columns may be read (the same for the whole warp).
+template <typename U, int DP>
+__device__ __forceinline__ void store_row(const HeadsView& v, int b, int h, int64_t row, bool on, int d, uint32_t taddr, bool any,
+                                          bool live, float mul) {
+    U* p = static_cast<U*>(v.p) + b * v.sb + h * v.sh + row * v.ss;
+    const bool wide = std::is_same<U, float>::value && v.sd == 1 && d % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+    for (int k = 0; k < DP / 32; ++k) {
+        uint32_t o[32];
+        if (live) {
+            tmem_ld32(taddr + 32 * k, o);
+            tmem_wait_ld();
+        }
+        if (!on) continue;
+        if constexpr (std::is_same<U, float>::value) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int c = 32 * k + 4 * q;
+                if (c >= d) break;
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = any ? __uint_as_float(o[4 * q + e]) * mul : 0.f;
+                if (wide) {
+                    *reinterpret_cast<float4*>(p + c) = make_float4(w[0], w[1], w[2], w[3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < d) p[(c + e) * v.sd] = w[e];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (32 * k + 8 * q >= d) break;
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    w[e] = any ? pack16<U>(__uint_as_float(o[8 * q + 2 * e]) * mul, __uint_as_float(o[8 * q + 2 * e + 1]) * mul) : 0u;
+                *reinterpret_cast<uint4*>(p + 32 * k + 8 * q) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+}
+
 // ---------------------------------------------------------------- TMA
 // One head's rows in a 4-D map; strides of 0 and dims of 1 take coordinate 0.
 struct HeadMap {
@@ -120,54 +255,22 @@ __device__ __forceinline__ void tma_tile(uint32_t dst, const HeadMap& m, uint64_
             : "memory");
 }
 
-// ---------------------------------------------------------------- packed fp32
-typedef unsigned long long f2;
-__device__ __forceinline__ f2 pack2(float lo, float hi) {
-    f2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ void unpack2(f2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-    f2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-    f2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ f2 add2(f2 a, f2 b) {
-    f2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-template <typename T> __device__ __forceinline__ uint32_t pack16(float lo, float hi);
-template <> __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-template <> __device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
 // ---------------------------------------------------------------- capped scores
-// softcap tanh(x / softcap) for |x| <= softcap as x P((x / softcap)^2): P is
-// the polynomial of degree 4 that has the least largest relative error for
-// tanh(u) / u on u^2 in [0, 1] (a linear programme over a Chebyshev grid
-// gives it): 6.9e-6, far below the rounding of a 16-bit probability.  Tiles
-// that hold a larger score take tanh u = 1 - 2 / (1 + e^2u).
-constexpr float kTanh0 = 0.999993085861206f, kTanh1 = -0.3329806625843048f, kTanh2 = 0.13036811351776123f,
-                kTanh3 = -0.04481755569577217f, kTanh4 = 0.009036424569785595f;
+// softcap tanh(x / softcap) as x P((x / softcap)^2), where P has the least
+// largest relative error for tanh(u) / u over the range (a linear programme
+// over a Chebyshev grid gives it).  16-bit probabilities: |u| <= 1, degree 4,
+// 6.9e-6, far below the rounding of p.  Fp32: |u| <= 0.625, degree 5, 3.9e-9, below
+// the rounding of fp32.  Tiles that hold a larger score take tanh u =
+// 1 - 2 / (1 + e^2u) (fp32: for those scores alone; there 1.2e-7 off is
+// relative to more than 0.55).
+template <bool FINE>
+__device__ __forceinline__ constexpr float tanh_coef(int i) {
+    if (FINE)
+        return i == 0 ? 1.0f : i == 1 ? -0.3333325982093811f : i == 2 ? 0.13331125676631927f : i == 3 ? -0.053720925003290176f
+               : i == 4 ? 0.020590508356690407f : -0.00565946102142334f;
+    return i == 0 ? 0.999993085861206f : i == 1 ? -0.3329806625843048f : i == 2 ? 0.13036811351776123f
+           : i == 3 ? -0.04481755569577217f : 0.009036424569785595f;
+}
 
 struct CapCoef {
     float limit;       // largest |q.k| of the polynomial
@@ -176,9 +279,10 @@ struct CapCoef {
     float wide;        // 2 log2(e) scale / softcap: 2u in base 2
     float top;         // softcap log2 e
 };
+template <bool FINE>
 __device__ __forceinline__ CapCoef cap_coef(float scale, float cap) {
     CapCoef c;
-    c.limit = cap / scale;
+    c.limit = (FINE ? 0.625f : 1.f) * (cap / scale);
     c.k2 = (scale / cap) * (scale / cap);
     c.mul = scale * kLog2e;
     c.wide = 2.f * kLog2e * scale / cap;
@@ -187,12 +291,46 @@ __device__ __forceinline__ CapCoef cap_coef(float scale, float cap) {
 }
 __device__ __forceinline__ float wide_tanh(float x, float wide) { return 1.f - __fdividef(2.f, 1.f + ex2(x * wide)); }
 // tanh(u) / u of a pair of scores within the limit
+template <bool FINE>
 __device__ __forceinline__ f2 tanh_ratio(f2 x, f2 k2) {
+    constexpr int N = FINE ? 5 : 4;
     const f2 z = mul2(mul2(x, x), k2);
-    f2 r = fma2(z, pack2(kTanh4, kTanh4), pack2(kTanh3, kTanh3));
-    r = fma2(r, z, pack2(kTanh2, kTanh2));
-    r = fma2(r, z, pack2(kTanh1, kTanh1));
-    return fma2(r, z, pack2(kTanh0, kTanh0));
+    f2 r = pack2(tanh_coef<FINE>(N), tanh_coef<FINE>(N));
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) r = fma2(r, z, pack2(tanh_coef<FINE>(i), tanh_coef<FINE>(i)));
+    return r;
+}
+// The largest |score| of a row.
+template <int N>
+__device__ __forceinline__ float largest(const f2 (&x)[N]) {
+    float big = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float lo, hi;
+        unpack2(x[i], lo, hi);
+        big = fmaxf(big, fmaxf(fabsf(lo), fabsf(hi)));
+    }
+    return big;
+}
+// softcap tanh(x / softcap) in base 2 of a pair, in a tile with scores past
+// the limit; *t: the tanh.
+template <bool FINE>
+__device__ __forceinline__ f2 wide_score(f2 x, const CapCoef& cap, f2* t) {
+    float lo, hi;
+    unpack2(x, lo, hi);
+    f2 y = pack2(cap.top * wide_tanh(lo, cap.wide), cap.top * wide_tanh(hi, cap.wide));
+    *t = pack2(wide_tanh(lo, cap.wide), wide_tanh(hi, cap.wide));
+    if (FINE) {
+        float a, b, c, d, e, f;
+        const f2 xr = mul2(x, tanh_ratio<true>(x, pack2(cap.k2, cap.k2)));
+        unpack2(mul2(xr, pack2(cap.mul, cap.mul)), a, b);
+        unpack2(mul2(xr, pack2(sqrtf(cap.k2), sqrtf(cap.k2))), c, d);
+        unpack2(*t, e, f);
+        *t = pack2(fabsf(lo) <= cap.limit ? c : e, fabsf(hi) <= cap.limit ? d : f);
+        unpack2(y, e, f);
+        y = pack2(fabsf(lo) <= cap.limit ? a : e, fabsf(hi) <= cap.limit ? b : f);
+    }
+    return y;
 }
 
 // ---------------------------------------------------------------- documents
@@ -289,6 +427,37 @@ bool make_head_map(HeadMap* m, const HeadsView& v, int dtype, int b, int h, int6
 // the arrays a tensor-core kernel takes: 16-bit, head size contiguous, 16-byte
 // aligned rows
 bool tc_array(const HeadsView& v, int b, int h, int64_t n);
+// fp32 arrays on the tensor cores (k_attention_split.cu).  A value times a
+// power of two of its key head's group (the largest of these heads then lies
+// in 2^14 .. 2^15) is hi + lo, two fp16 numbers of 11 bits: 22 bits of it, or 2^-25
+// where that is more, which is 2^-39 of the largest.  One array:
+// [b, h, n, 128] fp16, columns 0..63 hi, 64..127 lo, zeros past the head size and in
+// rows that must not count.
+constexpr int kSplitMaxHead = 64;
+struct SplitArray {
+    HeadsView v;
+    int h, n;
+    bool keys;          // rows count below kv_len and in documents of k_doc (else of q_doc)
+    int norm;           // largest row norm^2 into norms[2 * (b * hkv + key head) + norm]; -1: none
+    __half* out;
+    uint32_t* top;      // [b, hkv] largest |x| of the group's heads as bits
+};
+struct SplitPlan {
+    size_t top, norms, data[4], bytes;   // of q, k, v, dout (backward)
+    SplitPlan(const AttnCall& a, bool backward);
+};
+// queues the splitting; maps: q, k, v, dout
+tl_status launch_split(tl_ctx* c, const AttnCall& a, bool backward, uint8_t* ws, HeadMap* maps, cudaStream_t s);
+// the power of two of a group, from its largest value
+__device__ __forceinline__ int split_exp(const uint32_t* top, int group) {
+    const float m = __uint_as_float(top[group]);
+    if (!(m > 0.f) || m > 3.4e38f) return 0;
+    return min(max(14 - ilogbf(m), -60), 60);
+}
+struct SplitTops {
+    const uint32_t *q, *k, *v, *dout;    // null: operands are the arrays themselves
+};
+
 tl_status launch_doc_ranges(tl_ctx* c, const int32_t* doc, int b, int n, DocRange* out, cudaStream_t s);
 
 }  // namespace tl

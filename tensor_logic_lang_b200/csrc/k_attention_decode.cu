@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
         return;
     }
 
-    const CapCoef cap = cap_coef(a.scale, a.cap > 0.f ? a.cap : 1.f);
+    const CapCoef cap = cap_coef<false>(a.scale, a.cap > 0.f ? a.cap : 1.f);
     const int gid = lane >> 2, tid = lane & 3, mi = lane >> 3, mr = lane & 7;
     const int ksteps = (a.d + 15) / 16;
     T* qs = reinterpret_cast<T*>(smem + L::Q);
@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(DA_THREADS) k_decode_any(const __grid_constant
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     PieceWalk walk = block_pieces<DA_THREADS / 32>(g, red, found);
-    const CapCoef cap = cap_coef(a.scale == 0.f ? 1.f : a.scale, a.cap > 0.f ? a.cap : 1.f);
+    const CapCoef cap = cap_coef<false>(a.scale == 0.f ? 1.f : a.scale, a.cap > 0.f ? a.cap : 1.f);
     const int group = a.hq / a.hkv;
     constexpr int NC = DP >= 128 ? DP / 128 : 1, LANES = DP >= 128 ? 32 : DP / 4;
     Piece pc;
@@ -764,7 +764,7 @@ __global__ void __launch_bounds__(DA_THREADS) k_decode_any(const __grid_constant
     }
 }
 
-bool few_takes_mma(const AttnCall& a) { return attn_tc_takes(a); }
+bool few_takes_mma(const AttnCall& a) { return a.dtype != TL_TYPE_F32 && attn_tc_takes(a); }
 int few_rows(const AttnCall& a) {
     const int64_t rows = (int64_t)a.nq * (a.hq / a.hkv);
     if (few_takes_mma(a)) return rows <= 16 ? 16 : 32;

@@ -1,0 +1,131 @@
+// fp32 arrays as pairs of fp16 for the tensor-core attention kernels: the
+// largest value of every group of heads, then hi and lo of every value (attn_tc.h,
+// SplitArray).  HBM-bound: the arrays are read twice (the second time mostly
+// from the L2 cache) and their 4 bytes a value written once.
+//
+// Three fp16 products of 11-bit parts give 22 bits; TF32 would take the same
+// three at half the rate, and fp32 on the CUDA cores runs at a tenth of it.
+#include <algorithm>
+
+#include "attn_tc.h"
+
+namespace tl {
+namespace {
+
+constexpr int SP_ROWS = 64;   // of a block of 8 warps
+
+struct SplitArgs {
+    AttnCall a;
+    SplitArray arr[4];
+    uint32_t* norms;
+};
+
+__device__ __forceinline__ bool row_counts(const AttnCall& a, const SplitArray& x, int b, int64_t r) {
+    if (r >= x.n) return false;
+    if (!x.keys) return !a.q_doc || a.q_doc[(int64_t)b * a.nq + r] >= 0;
+    const int kv = a.kv_len ? min(max(a.kv_len[b], 0), a.nk) : a.nk;
+    return r < kv && (!a.k_doc || a.k_doc[(int64_t)b * a.nk + r] >= 0);
+}
+
+// A warp takes 8 rows, a lane columns 2 lane and 2 lane + 1.
+template <bool WRITE>
+__global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs g) {
+    const AttnCall& a = g.a;
+    const SplitArray& x = g.arr[blockIdx.y];
+    const int blocks = (x.n + SP_ROWS - 1) / SP_ROWS;
+    if (blockIdx.x >= (unsigned)(blocks * x.h) * a.b) return;
+    const int bh = blockIdx.x / blocks, b = bh / x.h, h = bh % x.h;
+    const int group = b * a.hkv + h / (x.h / a.hkv);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, c = 2 * lane;
+    const int64_t r0 = (int64_t)(blockIdx.x % blocks) * SP_ROWS + warp * 8;
+    const float* p = static_cast<const float*>(x.v.p) + b * x.v.sb + h * x.v.sh;
+    float u[8], w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const bool on = row_counts(a, x, b, r0 + k);
+        u[k] = on && c < a.d ? p[(r0 + k) * x.v.ss + c * x.v.sd] : 0.f;
+        w[k] = on && c + 1 < a.d ? p[(r0 + k) * x.v.ss + (c + 1) * x.v.sd] : 0.f;
+    }
+    if (WRITE) {
+        const float up = exp2f((float)split_exp(x.top, group));
+        __half* out = x.out + ((int64_t)bh * x.n + r0) * 128 + c;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (r0 + k >= x.n) break;
+            uint32_t hi, lo;
+            split16(u[k] * up, w[k] * up, hi, lo);
+            *reinterpret_cast<uint32_t*>(out + k * 128) = hi;
+            *reinterpret_cast<uint32_t*>(out + k * 128 + 64) = lo;
+        }
+    } else {
+        float top = 0.f, norm = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            top = fmaxf(top, fmaxf(fabsf(u[k]), fabsf(w[k])));
+            float n2 = fmaf(u[k], u[k], w[k] * w[k]);
+            if (x.norm >= 0) {
+#pragma unroll
+                for (int o = 16; o; o >>= 1) n2 += __shfl_xor_sync(0xffffffffu, n2, o);
+                norm = fmaxf(norm, n2);
+            }
+        }
+        // non-negative floats order like their bits; a maximum does not depend on the order
+        const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+        if (lane == 0) {
+            atomicMax(&x.top[group], m);
+            if (x.norm >= 0) atomicMax(&g.norms[2 * group + x.norm], __float_as_uint(norm));
+        }
+    }
+}
+
+}  // namespace
+
+SplitPlan::SplitPlan(const AttnCall& a, bool backward) {
+    bytes = 0;
+    auto take = [&](size_t n) { const size_t at = bytes; bytes += (n + 255) / 256 * 256; return at; };
+    // the words that start at zero lie together
+    const size_t groups = (size_t)a.b * a.hkv;
+    top = take(groups * (4 * 4 + 8));
+    norms = top + groups * 4 * 4;
+    const size_t q = (size_t)a.b * a.hq * a.nq * 256, k = (size_t)a.b * a.hkv * a.nk * 256;
+    data[0] = take(q);
+    data[1] = take(k);
+    data[2] = take(k);
+    data[3] = take(backward ? q : 0);
+}
+
+tl_status launch_split(tl_ctx* c, const AttnCall& a, bool backward, uint8_t* ws, HeadMap* maps, cudaStream_t s) {
+    const SplitPlan plan(a, backward);
+    SplitArgs g;
+    g.a = a;
+    uint32_t* top = reinterpret_cast<uint32_t*>(ws + plan.top);
+    g.norms = reinterpret_cast<uint32_t*>(ws + plan.norms);
+    const int count = backward ? 4 : 3;
+    const HeadsView* views[4] = {&a.q, &a.k, &a.v, &a.dout};
+    int64_t grid = 0;
+    for (int i = 0; i < count; ++i) {
+        SplitArray& x = g.arr[i];
+        x.keys = i == 1 || i == 2;
+        x.v = *views[i];
+        x.h = x.keys ? a.hkv : a.hq;
+        x.n = x.keys ? a.nk : a.nq;
+        x.norm = !backward ? -1 : i == 3 ? 0 : i == 2 ? 1 : -1;
+        x.out = reinterpret_cast<__half*>(ws + plan.data[i]);
+        x.top = top;
+        top += (size_t)a.b * a.hkv;
+        grid = std::max<int64_t>(grid, (int64_t)a.b * x.h * ((x.n + SP_ROWS - 1) / SP_ROWS));
+        const HeadsView flat = {x.out, (int64_t)x.h * x.n * 128, (int64_t)x.n * 128, 128, 1};
+        if (!make_head_map(&maps[i], flat, TL_TYPE_F16, a.b, x.h, x.n, 128)) return fail(c, TL_ERR_CUDA, "attention: tensor maps");
+    }
+    TL_CK(c, cudaMemsetAsync(ws + plan.top, 0, (size_t)a.b * a.hkv * (4 * 4 + 8), s));
+    const double bytes = (double)a.b * a.d * ((double)(backward ? 2 : 1) * a.hq * a.nq + 2.0 * a.hkv * a.nk);
+    cudaEvent_t ev[2];
+    launch_begin_on(c, s, "attention_split_top", 4 * bytes, 0, ev);
+    k_split<false><<<dim3((unsigned)grid, count), 256, 0, s>>>(g);
+    TL_TRY(launch_end_on(c, s, ev));
+    launch_begin_on(c, s, "attention_split", 8 * bytes, 0, ev);
+    k_split<true><<<dim3((unsigned)grid, count), 256, 0, s>>>(g);
+    return launch_end_on(c, s, ev);
+}
+
+}  // namespace tl

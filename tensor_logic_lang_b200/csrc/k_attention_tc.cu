@@ -1,5 +1,6 @@
 // Attention forward on the tensor cores: 16-bit operands, head size up to
-// 128, one pass over the keys with a running maximum and sum.
+// 128, or fp32 arrays of head size up to 64 as pairs of fp16 (attn_tc.h, SplitArray);
+// one pass over the keys with a running maximum and sum.
 //
 // A block owns two tiles of 128 queries that read the same keys: the same
 // rows of two heads of a group where the group has an even number of heads
@@ -19,6 +20,12 @@
 // the range), so most tiles touch O not at all.  l sums the unrounded p.
 // P is rounded to the operand type: the tensor cores take 16-bit operands;
 // each p is off by half a step, which weighs like the rounding of v.
+//
+// fp32 arrays: Q, K and V come as hi and lo, P is written as hi (over the first
+// half of S) and lo (over the second), and each product is three.  The tensor
+// cores cut their sums by 2^-23 a step, which over many keys adds up to more
+// than fp32 loses, so P V of a tile goes into columns of its own, and the row's
+// thread adds them to the sum, also in TMEM, behind S, with rounded additions.
 #include <algorithm>
 
 #include "attn_tc.h"
@@ -32,8 +39,10 @@ constexpr float kGrow = 8.f;   // rescale when the maximum grew by 2^8
 struct FwArgs {
     AttnCall a;
     const DocRange* k_ranges;   // [b, key tiles] with documents
-    int pair_heads;             // the block's tiles: heads h, h + 1 (else rows i0, i0 + 128)
+    int tiles;                  // query tiles of a block: 2, or 1 where that gives the GPU enough blocks
+    int pair_heads;             // two tiles: heads h, h + 1 (else rows i0, i0 + 128)
     int key_tiles;
+    SplitTops tops;             // fp32 arrays
     int* err;
 };
 
@@ -70,28 +79,21 @@ __global__ void __launch_bounds__(256) k_doc_ranges(const int32_t* __restrict__ 
 // score in base 2 times c (see below), with -inf where the key is not seen.
 // Returns the row's largest c-scaled score.
 //   !CAP && !BIAS: x is left as it is and c = scale log2 e; else c = 1.
-template <bool CAP, bool BIAS>
+//   FINE: the tanh to fp32
+template <bool CAP, bool BIAS, bool FINE>
 __device__ __forceinline__ float score_row(f2 (&x)[TILE / 2], float c1, const CapCoef& cap, float slope2, int p, int j0,
                                            bool masked, const uint32_t (&bits)[4]) {
     if (CAP) {
-        float big = 0.f;
-#pragma unroll
-        for (int i = 0; i < TILE / 2; ++i) {
-            float lo, hi;
-            unpack2(x[i], lo, hi);
-            big = fmaxf(big, fmaxf(fabsf(lo), fabsf(hi)));
-        }
-        if (__any_sync(0xffffffffu, !(big <= cap.limit))) {
+        if (__any_sync(0xffffffffu, !(largest(x) <= cap.limit))) {
 #pragma unroll
             for (int i = 0; i < TILE / 2; ++i) {
-                float lo, hi;
-                unpack2(x[i], lo, hi);
-                x[i] = pack2(cap.top * wide_tanh(lo, cap.wide), cap.top * wide_tanh(hi, cap.wide));
+                f2 t;
+                x[i] = wide_score<FINE>(x[i], cap, &t);
             }
         } else {
             const f2 k2 = pack2(cap.k2, cap.k2), mul = pack2(cap.mul, cap.mul);
 #pragma unroll
-            for (int i = 0; i < TILE / 2; ++i) x[i] = mul2(mul2(x[i], mul), tanh_ratio(x[i], k2));
+            for (int i = 0; i < TILE / 2; ++i) x[i] = mul2(mul2(x[i], mul), tanh_ratio<FINE>(x[i], k2));
         }
     }
     if (BIAS) {
@@ -136,11 +138,15 @@ __device__ __forceinline__ float score_row(f2 (&x)[TILE / 2], float c1, const Ca
     return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
 
-template <typename T, int DP, bool CAP, bool BIAS>
+// T: operands, U: the arrays' type (float: split operands, DP = 128 columns of
+// hi and lo)
+template <typename T, typename U, int DP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(FW_THREADS, 1)
     k_attn_tc(const __grid_constant__ HeadMap mq, const __grid_constant__ HeadMap mk, const __grid_constant__ HeadMap mv,
               const __grid_constant__ FwArgs g) {
     using L = FwSmem<DP>;
+    constexpr bool SPLIT = !std::is_same<T, U>::value;
+    constexpr int DO = SPLIT ? 64 : DP;   // columns of O
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::BAR);
@@ -155,7 +161,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     // of a causal call, go first
     const int group = a.hq / a.hkv;
     const int units = g.pair_heads ? a.hq / 2 : a.hq;
-    const int span = g.pair_heads ? TILE : 2 * TILE;
+    const int span = g.pair_heads ? TILE : g.tiles * TILE;
     const int row_blocks = (a.nq + span - 1) / span;
     const unsigned per_row = (unsigned)units * a.b;
     const int rb = row_blocks - 1 - (int)(blockIdx.x / per_row);
@@ -216,8 +222,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             int kt = walk.next(&masked);
             int n = 0;   // ring entries filled
             if (kt >= 0 && lane == 0) {
-                mbar_expect_tx(q_full, 2 * L::TILE_B);
-                for (int t = 0; t < 2; ++t)
+                mbar_expect_tx(q_full, g.tiles * L::TILE_B);
+                for (int t = 0; t < g.tiles; ++t)
                     tma_tile(smem_u32(smem + L::Q + t * L::TILE_B), mq, q_full, L::CH, i0 + (g.pair_heads ? 0 : t * TILE),
                              h0 + (g.pair_heads ? t : 0), b);
             }
@@ -247,8 +253,9 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             };
             auto scores = [&](int t, int stage) {
                 if (ok && lane == 0) {
-                    mma_rows<T>(tmem + t * TILE, smem_u32(smem + L::Q + t * L::TILE_B),
-                                smem_u32(smem + L::KV + stage * L::TILE_B), ksteps);
+                    const uint32_t sq = smem_u32(smem + L::Q + t * L::TILE_B), sk = smem_u32(smem + L::KV + stage * L::TILE_B);
+                    if (SPLIT) mma_rows_split<T>(tmem + t * TILE, sq, sk, ksteps);
+                    else mma_rows<T>(tmem + t * TILE, sq, sk, ksteps);
                     umma_commit(&s_full[t]);
                 }
                 __syncwarp();
@@ -256,8 +263,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             if (kt >= 0) {
                 wait_full(q_full, 0, 1);
                 wait_full(full, n, FW_STAGES);
-                scores(0, n % FW_STAGES);
-                scores(1, n % FW_STAGES);
+                for (int t = 0; t < g.tiles; ++t) scores(t, n % FW_STAGES);
                 if (ok && lane == 0) umma_commit(&empty[n % FW_STAGES]);
                 ++n;
             }
@@ -266,7 +272,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 wait_full(full, n, FW_STAGES);
                 ++n;
                 // rows of V that must not count: 0 probability times what they hold could be NaN
-                if (ok && ((kd && masked) || (mask.kv < a.nk && (kt + 1) * TILE > mask.kv))) {
+                if (!SPLIT && ok && ((kd && masked) || (mask.kv < a.nk && (kt + 1) * TILE > mask.kv))) {
                     clear_rows(smem + L::KV + vs * L::TILE_B, L::CH, [&](int r) {
                         const int j = kt * TILE + r;
                         return j >= mask.kv || (kd && kd[j] < 0);
@@ -276,13 +282,16 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 }
                 bool next_masked;
                 const int next = walk.next(&next_masked);
-                for (int t = 0; t < 2; ++t) {
+                for (int t = 0; t < g.tiles; ++t) {
                     ok = ok && mbar_wait(&p_full[t], it & 1, g.err);
                     ok = __all_sync(0xffffffffu, ok);
                     tc_fence_after();
                     if (ok && lane == 0) {
-                        mma_cols<T>(tmem + 2 * TILE + t * DP, tmem + t * TILE, smem_u32(smem + L::KV + vs * L::TILE_B), idesc_o,
-                                    it > 0);
+                        const uint32_t to = tmem + 2 * TILE + t * DO, sv = smem_u32(smem + L::KV + vs * L::TILE_B);
+                        if (SPLIT)
+                            mma_cols_split<T>(to, sv, idesc_o, [&](int part, int k) { return tmem + t * TILE + part * 64 + 8 * k; });
+                        else
+                            mma_cols<T>(to, tmem + t * TILE, sv, idesc_o, it > 0);
                         if (next < 0) umma_commit(&o_done[t]);
                     }
                     __syncwarp();
@@ -301,16 +310,20 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 masked = next_masked;
             }
         }
-    } else {
+    } else if (warp / 4 < g.tiles) {
         // ---------------------------------------------------- a row per thread
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int t = warp / 4, r = threadIdx.x % TILE;
         const int i = i0 + r + (g.pair_heads ? 0 : t * TILE), h = h0 + (g.pair_heads ? t : 0);
         const int p = mask.p0 + i, limit = mask.key_end(i, 1);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + t * TILE + lanes, to = tmem + 2 * TILE + t * DP + lanes;
-        const float c1 = a.scale * kLog2e, c = CAP || BIAS ? 1.f : c1;
-        const CapCoef cap = cap_coef(a.scale, CAP ? a.cap : 1.f);
+        const uint32_t ts = tmem + t * TILE + lanes, to = tmem + 2 * TILE + t * DO + lanes;
+        const uint32_t acc = SPLIT ? tmem + 3 * TILE + t * DO + lanes : to;   // the sum over the tiles
+        // split operands carry powers of two of their heads
+        const int e_qk = SPLIT ? split_exp(g.tops.q, b * a.hkv + kvh) + split_exp(g.tops.k, b * a.hkv + kvh) : 0;
+        const float scale = SPLIT ? a.scale * exp2f((float)-e_qk) : a.scale;
+        const float c1 = scale * kLog2e, c = CAP || BIAS ? 1.f : c1;
+        const CapCoef cap = cap_coef<SPLIT>(scale, CAP ? a.cap : 1.f);
         const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
         const int doc = qd && i < a.nq ? qd[i] : -1;
         float m = -INFINITY, l = 0.f;
@@ -337,6 +350,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             ok = ok && mbar_wait(&s_full[t], it & 1, g.err);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc_fence_after();
+            if (SPLIT && it > 0) tmem_add<DO>(acc, to, it == 1);   // P V of the tile before, done before this S
             f2 x[TILE / 2];
             {
                 uint32_t raw[TILE];
@@ -346,7 +360,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
 #pragma unroll
                 for (int k = 0; k < TILE / 2; ++k) x[k] = pack2(__uint_as_float(raw[2 * k]), __uint_as_float(raw[2 * k + 1]));
             }
-            const float top = c * score_row<CAP, BIAS>(x, c1, cap, slope2, p, j0, masked, bits);
+            const float top = c * score_row<CAP, BIAS, SPLIT>(x, c1, cap, slope2, p, j0, masked, bits);
             // a new reference maximum, for the first seen key of a row or a large step
             if (__any_sync(0xffffffffu, top > m + kGrow || (m == -INFINITY && top > m))) {
                 const float nm = fmaxf(m, top);
@@ -354,10 +368,11 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 l *= by;
                 m = nm;
                 if (it > 0) {
+                    if (SPLIT) tmem_wait_st();
                     const f2 by2 = pack2(by, by);
-                    for (int k = 0; k < DP / 32; ++k) {
+                    for (int k = 0; k < DO / 32; ++k) {
                         uint32_t o[32];
-                        tmem_ld32(to + 32 * k, o);
+                        tmem_ld32(acc + 32 * k, o);
                         tmem_wait_ld();
 #pragma unroll
                         for (int q = 0; q < 16; ++q) {
@@ -366,7 +381,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                             o[2 * q] = __float_as_uint(lo);
                             o[2 * q + 1] = __float_as_uint(hi);
                         }
-                        tmem_st32(to + 32 * k, o);
+                        tmem_st32(acc + 32 * k, o);
                     }
                 }
             }
@@ -376,7 +391,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             f2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                uint32_t out[16];
+                uint32_t out[16], low[SPLIT ? 16 : 1];
 #pragma unroll
                 for (int q = 0; q < 16; ++q) {
                     float lo, hi;
@@ -384,9 +399,11 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                     lo = ex2(lo);
                     hi = ex2(hi);
                     sum[q & 1] = add2(sum[q & 1], pack2(lo, hi));
-                    out[q] = pack16<T>(lo, hi);
+                    if (SPLIT) split16(lo, hi, out[q], low[SPLIT ? q : 0]);
+                    else out[q] = pack16<T>(lo, hi);
                 }
                 tmem_st16(ts + 16 * k, out);
+                if (SPLIT) tmem_st16(ts + 64 + 16 * k, low);
             }
             {
                 float lo, hi;
@@ -404,27 +421,14 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             tc_fence_after();
         }
         const bool none = it == 0 || l == 0.f;   // no key seen
-        const float inv = none ? 0.f : 1.f / l;
+        float inv = none ? 0.f : 1.f / l;
+        if (ok && SPLIT && it > 0) {
+            tmem_add<DO>(acc, to, it == 1);
+            tmem_wait_st();
+            inv *= exp2f((float)-split_exp(g.tops.v, b * a.hkv + kvh));
+        }
         if (ok) {
-            T* row = static_cast<T*>(a.o.p) + b * a.o.sb + h * a.o.sh + i * a.o.ss;
-            for (int k = 0; k < DP / 32; ++k) {
-                uint32_t o[32];
-                if (it > 0) {
-                    tmem_ld32(to + 32 * k, o);
-                    tmem_wait_ld();
-                }
-                if (i < a.nq)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        if (32 * k + 8 * q >= a.d) break;
-                        uint32_t v[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            v[e] = none ? 0u : pack16<T>(__uint_as_float(o[8 * q + 2 * e]) * inv,
-                                                         __uint_as_float(o[8 * q + 2 * e + 1]) * inv);
-                        *reinterpret_cast<uint4*>(row + 32 * k + 8 * q) = make_uint4(v[0], v[1], v[2], v[3]);
-                    }
-            }
+            store_row<U, DO>(a.o, b, h, i, i < a.nq, a.d, acc, !none, it > 0, inv);
             if (a.lse && i < a.nq)
                 a.lse[((int64_t)b * a.hq + h) * a.nq + i] = none ? -INFINITY : (m - Lift<T>::log2) * kLn2 + logf(l);
         }
@@ -437,18 +441,25 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     }
 }
 
-template <typename T, int DP, bool CAP, bool BIAS>
-tl_status launch(tl_ctx* c, const HeadMap& mq, const HeadMap& mk, const HeadMap& mv, const FwArgs& g, cudaStream_t s) {
+template <typename T, typename U, int DP, bool CAP, bool BIAS>
+tl_status launch(tl_ctx* c, const HeadMap* m, const FwArgs& g, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     constexpr int smem = FwSmem<DP>::BYTES;
-    TL_TRY(kernel_smem(c, k_attn_tc<T, DP, CAP, BIAS>, smem, done));
+    TL_TRY(kernel_smem(c, k_attn_tc<T, U, DP, CAP, BIAS>, smem, done));
     const AttnCall& a = g.a;
-    const int span = g.pair_heads ? TILE : 2 * TILE;
+    const int span = g.pair_heads ? TILE : g.tiles * TILE;
     const int64_t grid = (int64_t)a.b * (g.pair_heads ? a.hq / 2 : a.hq) * ((a.nq + span - 1) / span);
     cudaEvent_t ev[2];
     launch_begin_on(c, s, "attention_tc", 0, 4.0 * a.d * attn_pairs(a), ev);
-    k_attn_tc<T, DP, CAP, BIAS><<<(unsigned)grid, FW_THREADS, smem, s>>>(mq, mk, mv, g);
+    k_attn_tc<T, U, DP, CAP, BIAS><<<(unsigned)grid, FW_THREADS, smem, s>>>(m[0], m[1], m[2], g);
     return launch_end_on(c, s, ev);
+}
+
+template <typename T, typename U, int DP>
+tl_status launch_scores(tl_ctx* c, const HeadMap* m, const FwArgs& g, cudaStream_t s) {
+    const bool bias = g.a.slopes != nullptr;
+    if (g.a.cap > 0.f) return bias ? launch<T, U, DP, true, true>(c, m, g, s) : launch<T, U, DP, true, false>(c, m, g, s);
+    return bias ? launch<T, U, DP, false, true>(c, m, g, s) : launch<T, U, DP, false, false>(c, m, g, s);
 }
 
 }  // namespace
@@ -459,10 +470,12 @@ bool tc_array(const HeadsView& v, int b, int h, int64_t n) {
 }
 
 bool attn_tc_takes(const AttnCall& a) {
-    // positions within an int32 tile coordinate; a scale that keeps the order of
-    // the scores (the row maximum is taken before scaling)
-    return a.dtype != TL_TYPE_F32 && a.d % 8 == 0 && a.d <= 128 && a.scale > 0.f && tc_array(a.q, a.b, a.hq, a.nq) &&
-           tc_array(a.k, a.b, a.hkv, a.nk) && tc_array(a.v, a.b, a.hkv, a.nk) && tc_array(a.o, a.b, a.hq, a.nq) && a.nk > 0;
+    // a scale that keeps the order of the scores (the row maximum is taken
+    // before scaling)
+    if (a.nk == 0 || !(a.scale > 0.f)) return false;
+    if (a.dtype == TL_TYPE_F32) return a.d <= kSplitMaxHead;   // its operands are copies, the arrays may lie anyhow
+    return a.d % 8 == 0 && a.d <= 128 && tc_array(a.q, a.b, a.hq, a.nq) && tc_array(a.k, a.b, a.hkv, a.nk) &&
+           tc_array(a.v, a.b, a.hkv, a.nk) && tc_array(a.o, a.b, a.hq, a.nq);
 }
 
 bool make_head_map(HeadMap* m, const HeadsView& v, int dtype, int b, int h, int64_t n, int d, int box_rows) {
@@ -489,9 +502,12 @@ bool make_head_map(HeadMap* m, const HeadsView& v, int dtype, int b, int h, int6
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// documents: the ranges of the key tiles
+// documents: the ranges of the key tiles; fp32: the split operands
+static size_t ranges_bytes(const AttnCall& a) {
+    return a.k_doc ? ((size_t)a.b * ((a.nk + TILE - 1) / TILE) * sizeof(DocRange) + 255) / 256 * 256 : 0;
+}
 size_t attn_tc_workspace(const AttnCall& a) {
-    return a.k_doc ? (size_t)a.b * ((a.nk + TILE - 1) / TILE) * sizeof(DocRange) : 0;
+    return ranges_bytes(a) + (a.dtype == TL_TYPE_F32 ? SplitPlan(a, false).bytes : 0);
 }
 
 tl_status launch_doc_ranges(tl_ctx* c, const int32_t* doc, int b, int n, DocRange* out, cudaStream_t s) {
@@ -507,23 +523,31 @@ tl_status launch_attn_tc(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s)
     FwArgs g;
     g.a = a;
     g.k_ranges = static_cast<DocRange*>(ws);
-    g.pair_heads = a.hq / a.hkv % 2 == 0;
+    // one tile a block while that fills no more than the GPU's SMs at once
+    g.tiles = (int64_t)a.b * a.hq * ((a.nq + TILE - 1) / TILE) <= c->sm_count ? 1 : 2;
+    g.pair_heads = g.tiles == 2 && a.hq / a.hkv % 2 == 0;
     g.key_tiles = (a.nk + TILE - 1) / TILE;
     g.err = c->d_flags + 8;
-    HeadMap mq, mk, mv;
-    if (!make_head_map(&mq, a.q, a.dtype, a.b, a.hq, a.nq, a.d) || !make_head_map(&mk, a.k, a.dtype, a.b, a.hkv, a.nk, a.d) ||
-        !make_head_map(&mv, a.v, a.dtype, a.b, a.hkv, a.nk, a.d))
-        return fail(c, TL_ERR_CUDA, "attention: tensor maps");
     if (a.k_doc) TL_TRY(launch_doc_ranges(c, a.k_doc, a.b, a.nk, static_cast<DocRange*>(ws), s));
     c->flags_armed = true;
-#define TL_ATTN(T, DP)                                                                     \
-    (a.cap > 0.f ? (a.slopes ? launch<T, DP, true, true>(c, mq, mk, mv, g, s)              \
-                             : launch<T, DP, true, false>(c, mq, mk, mv, g, s))            \
-                 : (a.slopes ? launch<T, DP, false, true>(c, mq, mk, mv, g, s)             \
-                             : launch<T, DP, false, false>(c, mq, mk, mv, g, s)))
-    if (a.dtype == TL_TYPE_F16) return a.d <= 64 ? TL_ATTN(__half, 64) : TL_ATTN(__half, 128);
-    return a.d <= 64 ? TL_ATTN(__nv_bfloat16, 64) : TL_ATTN(__nv_bfloat16, 128);
-#undef TL_ATTN
+    HeadMap m[4];
+    if (a.dtype == TL_TYPE_F32) {
+        uint8_t* w = static_cast<uint8_t*>(ws) + ranges_bytes(a);
+        TL_TRY(launch_split(c, a, false, w, m, s));
+        g.tops.q = reinterpret_cast<const uint32_t*>(w + SplitPlan(a, false).top);
+        g.tops.k = g.tops.q + (size_t)a.b * a.hkv;
+        g.tops.v = g.tops.k + (size_t)a.b * a.hkv;
+        g.tops.dout = nullptr;
+        return launch_scores<__half, float, 128>(c, m, g, s);
+    }
+    g.tops = {nullptr, nullptr, nullptr, nullptr};
+    if (!make_head_map(&m[0], a.q, a.dtype, a.b, a.hq, a.nq, a.d) || !make_head_map(&m[1], a.k, a.dtype, a.b, a.hkv, a.nk, a.d) ||
+        !make_head_map(&m[2], a.v, a.dtype, a.b, a.hkv, a.nk, a.d))
+        return fail(c, TL_ERR_CUDA, "attention: tensor maps");
+    if (a.dtype == TL_TYPE_F16)
+        return a.d <= 64 ? launch_scores<__half, __half, 64>(c, m, g, s) : launch_scores<__half, __half, 128>(c, m, g, s);
+    return a.d <= 64 ? launch_scores<__nv_bfloat16, __nv_bfloat16, 64>(c, m, g, s)
+                     : launch_scores<__nv_bfloat16, __nv_bfloat16, 128>(c, m, g, s);
 }
 
 }  // namespace tl

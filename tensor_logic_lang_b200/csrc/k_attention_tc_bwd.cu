@@ -1,10 +1,12 @@
 // Attention backward on the tensor cores: 16-bit operands, head size up to
-// 128.  With p = exp(s - lse), dp = dout v^T, D = dout . o by row,
+// 128, or fp32 arrays of head size up to 64 as pairs of fp16 (attn_tc.h,
+// SplitArray).  With p = exp(s - lse), dp = dout v^T, D = dout . o by row,
 //   dx = p (dp - D) (1 - tanh^2),  dq = scale dx k,  dk = scale dx^T q,  dv = p^T dout
 // the scores are taken again from q and k (S is never stored), twice:
 //
 //   k_attn_prep    by tile of 128 queries: log2(e) lse and D, ready for the
-//                  kernels below; the largest row norms of dout and v (fp16)
+//                  kernels below; the largest row norms of dout and v (fp16;
+//                  fp32 arrays: k_attn_prep_f32, norms with the splitting)
 //   k_attn_tc_dkv  a block per (key tile, head): dk and dv stay in TMEM while
 //                  the query tiles pass; the heads of a group form a cluster
 //                  and add their sums through distributed shared memory in a
@@ -24,6 +26,9 @@
 // at 2^-24, so p is written 2^14 larger, and dx times the power of two that
 // puts its bound, 2 max|dout_i| max|v_j| (norms; |dp| and |D| are at most half
 // of it), at 2^15: neither can overflow, and small gradients keep their bits.
+// fp32 arrays: p and dx are written as hi and lo, each product is three, and
+// the sums over the tiles are added by the rows' threads (the tensor cores cut
+// theirs, see k_attention_tc.cu).
 #include <algorithm>
 
 #include "attn_tc.h"
@@ -40,8 +45,9 @@ template <> struct PLift<__half> { static constexpr float log2 = 14.f, back = 1.
 struct BwArgs {
     AttnCall a;
     const float* stats;          // [b, hq, query tiles][2][128]
-    const uint32_t* norms;       // fp16: [b, hkv][2] largest |dout_i|^2, |v_j|^2 as bits
+    const uint32_t* norms;       // fp16, fp32: [b, hkv][2] largest |dout_i|^2, |v_j|^2 as bits
     const DocRange *q_ranges, *k_ranges;
+    SplitTops tops;              // fp32 arrays
     int q_tiles, k_tiles, cluster;
     int* err;
 };
@@ -150,6 +156,37 @@ __global__ void __launch_bounds__(256)
     }
 }
 
+// The statistics of fp32 arrays of any layout: a warp takes 8 rows, a lane
+// columns 2 lane and 2 lane + 1 (head size up to 64).
+__global__ void __launch_bounds__(256) k_attn_prep_f32(const __grid_constant__ AttnCall a, float* __restrict__ stats, int q_tiles) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, c = 2 * lane;
+    const int64_t blk = blockIdx.x / 2;   // half a tile a block
+    const int qt = (int)(blk % q_tiles), h = (int)(blk / q_tiles % a.hq), b = (int)(blk / q_tiles / a.hq);
+    const int r0 = (blockIdx.x % 2) * 64 + warp * 8;
+    const float* x = static_cast<const float*>(a.dout.p) + b * a.dout.sb + h * a.dout.sh;
+    const float* y = static_cast<const float*>(a.o.p) + b * a.o.sb + h * a.o.sh;
+    float dot[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int64_t i = qt * TILE + r0 + k;
+        const bool on = i < a.nq && (!a.q_doc || a.q_doc[(int64_t)b * a.nq + i] >= 0);
+        dot[k] = on && c < a.d ? x[i * a.dout.ss + c * a.dout.sd] * y[i * a.o.ss + c * a.o.sd] : 0.f;
+        if (on && c + 1 < a.d) dot[k] = fmaf(x[i * a.dout.ss + (c + 1) * a.dout.sd], y[i * a.o.ss + (c + 1) * a.o.sd], dot[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+#pragma unroll
+        for (int w = 16; w; w >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], w);
+        const int64_t i = qt * TILE + r0 + k;
+        if (lane == 0) {
+            const bool on = i < a.nq && (!a.q_doc || a.q_doc[(int64_t)b * a.nq + i] >= 0);
+            const float lse = on ? a.lse[((int64_t)b * a.hq + h) * a.nq + i] : -INFINITY;
+            stats[blk * 2 * TILE + r0 + k] = lse == -INFINITY ? -INFINITY : PLift<__half>::log2 - lse * kLog2e;
+            stats[blk * 2 * TILE + TILE + r0 + k] = -dot[k];
+        }
+    }
+}
+
 // The power of two that dx is written with (see the top of the file).
 template <typename T>
 __device__ __forceinline__ float dx_lift(const BwArgs& g, int b, int kvh) {
@@ -164,34 +201,25 @@ __device__ __forceinline__ float dx_lift(const BwArgs& g, int b, int kvh) {
 // 64 scores q.k of a row -> p in base 2 (16-bit pairs) and p (1 - tanh^2).
 // off: position of column 0 relative to the row's (|off + c| is the distance);
 // nl(i): minus log2(e) lse of the columns 2i, 2i + 1.
-template <typename T, bool CAP, bool BIAS, typename NL>
-__device__ __forceinline__ void grad_row(f2 (&x)[32], uint32_t (&p16)[32], float c1, const CapCoef& cap, float slope2, int off,
+// SPLIT: p16 and low take hi and lo, and the tanh is good to fp32.
+template <typename T, bool CAP, bool BIAS, bool SPLIT, typename NL>
+__device__ __forceinline__ void grad_row(f2 (&x)[32], uint32_t (&p16)[32], uint32_t (&low)[32], float c1, const CapCoef& cap, float slope2, int off,
                                          bool masked, uint32_t bits0, uint32_t bits1, NL nl) {
     f2 bend[CAP ? 32 : 1];
     if (CAP) {
-        float big = 0.f;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            float lo, hi;
-            unpack2(x[i], lo, hi);
-            big = fmaxf(big, fmaxf(fabsf(lo), fabsf(hi)));
-        }
         const f2 one = pack2(1.f, 1.f);
-        if (__any_sync(0xffffffffu, !(big <= cap.limit))) {
+        if (__any_sync(0xffffffffu, !(largest(x) <= cap.limit))) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-                float lo, hi;
-                unpack2(x[i], lo, hi);
-                lo = wide_tanh(lo, cap.wide);
-                hi = wide_tanh(hi, cap.wide);
-                bend[i] = fma2(pack2(-lo, -hi), pack2(lo, hi), one);
-                x[i] = pack2(cap.top * lo, cap.top * hi);
+                f2 t;
+                x[i] = wide_score<SPLIT>(x[i], cap, &t);
+                bend[i] = fma2(mul2(t, pack2(-1.f, -1.f)), t, one);
             }
         } else {
             const f2 k2 = pack2(cap.k2, cap.k2), mul = pack2(cap.mul, cap.mul), neg = pack2(-cap.k2, -cap.k2);
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-                const f2 r = tanh_ratio(x[i], k2), xr = mul2(x[i], r);
+                const f2 r = tanh_ratio<SPLIT>(x[i], k2), xr = mul2(x[i], r);
                 bend[i] = fma2(mul2(xr, neg), xr, one);
                 x[i] = mul2(xr, mul);
             }
@@ -223,15 +251,17 @@ __device__ __forceinline__ void grad_row(f2 (&x)[32], uint32_t (&p16)[32], float
         }
         lo = ex2(lo);
         hi = ex2(hi);
-        p16[i] = pack16<T>(lo, hi);
+        if (SPLIT) split16(lo, hi, p16[i], low[i]);
+        else p16[i] = pack16<T>(lo, hi);
         x[i] = pack2(lo, hi);
         if (CAP) x[i] = mul2(x[i], bend[i]);
     }
 }
 
 // dx = pb (dp - D), zero where the key is not seen (there dp may be anything)
-template <typename T, typename ND>
-__device__ __forceinline__ void grad_dx(const f2 (&pb)[32], const uint32_t (&dp)[64], uint32_t (&out)[32], float lift, bool masked,
+template <typename T, bool SPLIT, typename ND>
+__device__ __forceinline__ void grad_dx(const f2 (&pb)[32], const uint32_t (&dp)[64], uint32_t (&out)[32], uint32_t (&low)[32],
+                                        float lift, bool masked,
                                         uint32_t bits0, uint32_t bits1, ND nd) {
     const f2 up = pack2(lift, lift);
 #pragma unroll
@@ -244,7 +274,8 @@ __device__ __forceinline__ void grad_dx(const f2 (&pb)[32], const uint32_t (&dp)
             lo = (w >> (2 * i % 32)) & 1 ? lo : 0.f;
             hi = (w >> (2 * i % 32 + 1)) & 1 ? hi : 0.f;
         }
-        out[i] = pack16<T>(lo, hi);
+        if (SPLIT) split16(lo, hi, out[i], low[i]);
+        else out[i] = pack16<T>(lo, hi);
     }
 }
 
@@ -270,27 +301,10 @@ __device__ __forceinline__ void mma_halves(uint32_t d, uint32_t a, uint32_t b, u
                     accumulate | (k > 0));
 }
 
-// A row of DP fp32 sums in TMEM, scaled, as 16-bit values of an array.
-template <typename T, int DP>
-__device__ __forceinline__ void store_row(const HeadsView& v, int b, int h, int64_t row, bool on, int d, uint32_t taddr, bool any, float mul) {
-    T* p = static_cast<T*>(v.p) + b * v.sb + h * v.sh + row * v.ss;
-    for (int k = 0; k < DP / 32; ++k) {
-        uint32_t o[32];
-        if (any) {
-            tmem_ld32(taddr + 32 * k, o);
-            tmem_wait_ld();
-        }
-        if (on)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                if (32 * k + 8 * q >= d) break;
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    w[e] = any ? pack16<T>(__uint_as_float(o[8 * q + 2 * e]) * mul, __uint_as_float(o[8 * q + 2 * e + 1]) * mul) : 0u;
-                *reinterpret_cast<uint4*>(p + 32 * k + 8 * q) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-    }
+// D = A B anew for split operands: in each half's 64 TMEM columns 32 of hi, 32 of lo
+template <typename T>
+__device__ __forceinline__ void mma_halves_split(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+    mma_cols_split<T>(d, b, idesc, [&](int part, int k) { return a + (k / 4) * 64 + part * 32 + (k % 4) * 8; });
 }
 
 // What the two gradient kernels share: barriers, TMEM, the documents of the block's rows.
@@ -362,13 +376,28 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, bool o
     return ok;
 }
 
+// The powers of two that split operands carry.
+struct SplitExps {
+    int q, k, v, dout;
+};
+template <bool SPLIT>
+__device__ __forceinline__ SplitExps split_exps(const BwArgs& g, int b, int kvh) {
+    const int i = b * g.a.hkv + kvh;
+    if (!SPLIT) return {0, 0, 0, 0};
+    return {split_exp(g.tops.q, i), split_exp(g.tops.k, i), split_exp(g.tops.v, i), split_exp(g.tops.dout, i)};
+}
+
 // ---------------------------------------------------------------- dk, dv
-// TMEM: S^T (P^T) 0..127, dp^T (dx^T) 128..255, dv, dk (DP columns each).
-template <typename T, int DP, bool CAP, bool BIAS>
+// TMEM: S^T (P^T) 0..127, dp^T (dx^T) 128..255, dv, dk (DO columns each; split
+// operands: their sums over the tiles behind them).
+// T: operands, U: the arrays' type (float: split operands).
+template <typename T, typename U, int DP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(BW_THREADS, 1)
     k_attn_tc_dkv(const __grid_constant__ HeadMap mq, const __grid_constant__ HeadMap mk, const __grid_constant__ HeadMap mv,
                   const __grid_constant__ HeadMap mdo, const __grid_constant__ BwArgs g) {
     using L = BwSmem<DP>;
+    constexpr bool SPLIT = !std::is_same<T, U>::value;
+    constexpr int DO = SPLIT ? 64 : DP;   // columns of a result
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const AttnCall& a = g.a;
@@ -385,7 +414,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     BwBlock bb(smem + L::BAR, smem + L::DOCS);
     DocRange mine;
     const uint32_t tmem = bb.setup(kd ? kd + j0 : nullptr, min(TILE, a.nk - j0), &mine);
-    const uint32_t t_s = tmem, t_dp = tmem + TILE, t_dv = tmem + 2 * TILE, t_dk = tmem + 2 * TILE + DP;
+    const uint32_t t_s = tmem, t_dp = tmem + TILE, t_dv = tmem + 2 * TILE, t_dk = tmem + 2 * TILE + DO;
+    const uint32_t t_dva = tmem + 3 * TILE, t_dka = t_dva + 64;   // split operands: the sums over the tiles
 
     // query tiles that see some of the keys; from `clear` on they see all of them
     int begin = 0, end = g.q_tiles, clear = 0;
@@ -446,9 +476,17 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             const int ksteps = (a.d + 15) / 16;
             const uint32_t idesc = f16_idesc<T>(16 * ksteps, true);
             const uint32_t sk = smem_u32(smem + L::FIX), sv = sk + L::TILE_B;
+            auto rows = [&](uint32_t d, uint32_t x, uint32_t y) {
+                if (SPLIT) mma_rows_split<T>(d, x, y, ksteps);
+                else mma_rows<T>(d, x, y, ksteps);
+            };
+            auto halves = [&](uint32_t d, uint32_t x, uint32_t y, bool more) {
+                if (SPLIT) mma_halves_split<T>(d, x, y, idesc);
+                else mma_halves<T>(d, x, y, idesc, more);
+            };
             // query rows of negative documents: 0 times what they hold could be NaN
             auto clean = [&](int s) {
-                if (!qd || !masked) return;
+                if (SPLIT || !qd || !masked) return;
                 auto bad = [&](int r) { const int i = qt * TILE + r; return i < a.nq && qd[i] < 0; };
                 clear_rows(smem + L::RING + s * 2 * L::TILE_B, L::CH, bad);
                 clear_rows(smem + L::RING + s * 2 * L::TILE_B + L::TILE_B, L::CH, bad);
@@ -462,9 +500,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 if (ok) clean(0);
                 const uint32_t sq = smem_u32(smem + L::RING);
                 if (ok && lane == 0) {
-                    mma_rows<T>(t_s, sk, sq, ksteps);
+                    rows(t_s, sk, sq);
                     umma_commit(&bb.s_full[0]);
-                    mma_rows<T>(t_dp, sv, sq + L::TILE_B, ksteps);
+                    rows(t_dp, sv, sq + L::TILE_B);
                     umma_commit(bb.dp_full);
                 }
                 __syncwarp();
@@ -474,24 +512,24 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 const uint32_t sq = smem_u32(smem + L::RING + s * 2 * L::TILE_B);
                 const uint32_t sq1 = smem_u32(smem + L::RING + s1 * 2 * L::TILE_B);
                 ok = warp_wait(bb.p_full, n & 1, ok, g.err);
-                if (ok && lane == 0) mma_halves<T>(t_dv, t_s, sq + L::TILE_B, idesc, n > 0);
+                if (ok && lane == 0) halves(t_dv, t_s, sq + L::TILE_B, n > 0);
                 __syncwarp();
                 next();
                 if (qt >= 0) {
                     ok = warp_wait(&bb.full[s1], ((n + 1) / BW_STAGES) & 1, ok, g.err);
                     if (ok) clean(s1);
                     if (ok && lane == 0) {
-                        mma_rows<T>(t_s, sk, sq1, ksteps);
+                        rows(t_s, sk, sq1);
                         umma_commit(&bb.s_full[0]);
                     }
                     __syncwarp();
                 }
                 ok = warp_wait(bb.dx_full, n & 1, ok, g.err);
                 if (ok && lane == 0) {
-                    mma_halves<T>(t_dk, t_dp, sq, idesc, n > 0);
+                    halves(t_dk, t_dp, sq, n > 0);
                     umma_commit(&bb.empty[s]);
                     if (qt >= 0) {
-                        mma_rows<T>(t_dp, sv, sq1 + L::TILE_B, ksteps);
+                        rows(t_dp, sv, sq1 + L::TILE_B);
                         umma_commit(bb.dp_full);
                     } else {
                         umma_commit(bb.done);
@@ -506,9 +544,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int wg = warp / 4, r = threadIdx.x % TILE, j = j0 + r;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const float c1 = a.scale * kLog2e;
-        const CapCoef cap = cap_coef(a.scale, CAP ? a.cap : 1.f);
+        const SplitExps ex = split_exps<SPLIT>(g, b, kvh);
+        const float scale = SPLIT ? a.scale * exp2f((float)-(ex.q + ex.k)) : a.scale, c1 = scale * kLog2e;
+        const CapCoef cap = cap_coef<SPLIT>(scale, CAP ? a.cap : 1.f);
         const float lift = dx_lift<T>(g, b, kvh), up = lift * PLift<T>::back;
+        const float up_dp = SPLIT ? up * exp2f((float)-(ex.dout + ex.v)) : up;   // dp carries the powers of dout and v
         const int doc = kd && j < a.nk ? kd[j] : -1;
         int n = 0;
         for (; qt >= 0 && ok; next(), ++n) {
@@ -536,11 +576,14 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             if (!ok) break;
             f2 x[32];
             {
+                // dv of the tile before, done before this S
+                if (SPLIT && wg == 0 && n > 0) tmem_add<DO>(t_dva + lanes, t_dv + lanes, n == 1);
                 load64(t_s + lanes + wg * 64, x);
-                uint32_t p16[32];
-                grad_row<T, CAP, BIAS>(x, p16, c1, cap, slope2, mask.p0 + i0 - j, masked, bits0, bits1,
+                uint32_t p16[32], low[32];
+                grad_row<T, CAP, BIAS, SPLIT>(x, p16, low, c1, cap, slope2, mask.p0 + i0 - j, masked, bits0, bits1,
                                        [&](int i) { return *reinterpret_cast<const f2*>(st + 2 * i); });
                 tmem_st32(t_s + lanes + wg * 64, p16);
+                if (SPLIT) tmem_st32(t_s + lanes + wg * 64 + 32, low);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -548,27 +591,39 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             ok = warp_wait(bb.dp_full, n & 1, ok, g.err);
             if (!ok) break;
             {
-                uint32_t dp[64], dx[32];
+                // dk of the tile before, done before this dp
+                if (SPLIT && wg == 1 && n > 0) tmem_add<DO>(t_dka + lanes, t_dk + lanes, n == 1);
+                uint32_t dp[64], dx[32], low[32];
                 load64(t_dp + lanes + wg * 64, dp);
                 const f2 up2 = pack2(up, up);
-                grad_dx<T>(x, dp, dx, up, masked, bits0, bits1, [&](int i) {
+                grad_dx<T, SPLIT>(x, dp, dx, low, up_dp, masked, bits0, bits1, [&](int i) {
                     const f2 d = *reinterpret_cast<const f2*>(st + TILE + 2 * i);
                     return PLift<T>::log2 == 0.f ? d : mul2(d, up2);
                 });
                 tmem_st32(t_dp + lanes + wg * 64, dx);
+                if (SPLIT) tmem_st32(t_dp + lanes + wg * 64 + 32, low);
             }
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(bb.dx_full);
         }
         if (any) ok = warp_wait(bb.done, 0, ok, g.err);
-        const uint32_t mine_at = (wg ? t_dk : t_dv) + lanes;
-        const float mul = wg ? a.scale / lift : PLift<T>::back;
+        uint32_t mine_at = (wg ? t_dk : t_dv) + lanes;
+        float mul = wg ? a.scale / lift : PLift<T>::back;
+        if (SPLIT) {
+            const uint32_t acc = (wg ? t_dka : t_dva) + lanes;
+            if (any && ok) {
+                tmem_add<DO>(acc, mine_at, n == 1);
+                tmem_wait_st();
+            }
+            mine_at = acc;
+            mul *= exp2f((float)-(wg ? ex.q : ex.dout));
+        }
         if (g.cluster == 1) {
-            if (ok) store_row<T, DP>(wg ? a.dk : a.dv, b, kvh, j, j < a.nk, a.d, mine_at, any, mul);
+            if (ok) store_row<U, DO>(wg ? a.dk : a.dv, b, kvh, j, j < a.nk, a.d, mine_at, any, any, mul);
         } else if (any && ok) {
             float* row = reinterpret_cast<float*>(smem) + (wg * TILE + r) * L::SUM_LD;
-            for (int k = 0; k < DP / 32; ++k) {
+            for (int k = 0; k < DO / 32; ++k) {
                 uint32_t o[32];
                 tmem_ld32(mine_at + 32 * k, o);
                 tmem_wait_ld();
@@ -587,7 +642,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         if (warp < 8) {
             const int share = TILE / g.cluster, r0 = rank * share;
             const uint32_t sums = smem_u32(smem);
-            constexpr int V = DP / 4;
+            constexpr int V = DO / 4;
             for (int e = threadIdx.x; e < 2 * share * V; e += 2 * TILE) {
                 const int c = e % V, r = r0 + e / V % share, wg = e / V / share;
                 if (j0 + r >= a.nk || 4 * c >= a.d) continue;
@@ -605,8 +660,14 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                         s[0] += x; s[1] += y; s[2] += z; s[3] += w;
                     }
                 const HeadsView& v = wg ? a.dk : a.dv;
-                T* p = static_cast<T*>(v.p) + b * v.sb + kvh * v.sh + (int64_t)(j0 + r) * v.ss + 4 * c;
-                *reinterpret_cast<uint2*>(p) = make_uint2(pack16<T>(s[0], s[1]), pack16<T>(s[2], s[3]));
+                U* p = static_cast<U*>(v.p) + b * v.sb + kvh * v.sh + (int64_t)(j0 + r) * v.ss;
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (4 * c + k < a.d) p[(4 * c + k) * v.sd] = s[k];
+                } else {
+                    *reinterpret_cast<uint2*>(p + 4 * c) = make_uint2(pack16<T>(s[0], s[1]), pack16<T>(s[2], s[3]));
+                }
             }
         }
         __syncwarp();
@@ -618,11 +679,13 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 
 // ---------------------------------------------------------------- dq
 // TMEM: S of two tiles 0..255, dp (dx) 256..383, dq 384..511.
-template <typename T, int DP, bool CAP, bool BIAS>
+template <typename T, typename U, int DP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(BW_THREADS, 1)
     k_attn_tc_dq(const __grid_constant__ HeadMap mq, const __grid_constant__ HeadMap mk, const __grid_constant__ HeadMap mv,
                  const __grid_constant__ HeadMap mdo, const __grid_constant__ BwArgs g) {
     using L = BwSmem<DP>;
+    constexpr bool SPLIT = !std::is_same<T, U>::value;
+    constexpr int DO = SPLIT ? 64 : DP;   // columns of a result
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const AttnCall& a = g.a;
@@ -638,6 +701,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     DocRange mine;
     const uint32_t tmem = bb.setup(qd ? qd + i0 : nullptr, rows, &mine);
     const uint32_t t_dp = tmem + 2 * TILE, t_dq = tmem + 3 * TILE;
+    const uint32_t t_dqa = t_dq + 64;   // split operands: the sum over the tiles
     TileWalk walk;
     walk.start(0, (max(mask.key_end(i0, rows), 0) + TILE - 1) / TILE, 0, max(mask.key_end(i0, 1), 0) / TILE,
                kd ? g.k_ranges + (int64_t)b * g.k_tiles : nullptr, mine);
@@ -673,9 +737,17 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             const int ksteps = (a.d + 15) / 16;
             const uint32_t idesc = f16_idesc<T>(16 * ksteps, true);
             const uint32_t sq = smem_u32(smem + L::FIX), sdo = sq + L::TILE_B;
+            auto rows = [&](uint32_t d, uint32_t x, uint32_t y) {
+                if (SPLIT) mma_rows_split<T>(d, x, y, ksteps);
+                else mma_rows<T>(d, x, y, ksteps);
+            };
+            auto halves = [&](uint32_t d, uint32_t x, uint32_t y, bool more) {
+                if (SPLIT) mma_halves_split<T>(d, x, y, idesc);
+                else mma_halves<T>(d, x, y, idesc, more);
+            };
             // keys that must not count: 0 times what they hold could be NaN
             auto clean = [&](int s) {
-                if (!((kd && masked) || (mask.kv < a.nk && (kt + 1) * TILE > mask.kv))) return;
+                if (SPLIT || !((kd && masked) || (mask.kv < a.nk && (kt + 1) * TILE > mask.kv))) return;
                 clear_rows(smem + L::RING + s * 2 * L::TILE_B, L::CH, [&](int r) {
                     const int j = kt * TILE + r;
                     return j >= mask.kv || (kd && kd[j] < 0);
@@ -690,9 +762,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 if (ok) clean(0);
                 const uint32_t sk = smem_u32(smem + L::RING);
                 if (ok && lane == 0) {
-                    mma_rows<T>(tmem, sq, sk, ksteps);
+                    rows(tmem, sq, sk);
                     umma_commit(&bb.s_full[0]);
-                    mma_rows<T>(t_dp, sdo, sk + L::TILE_B, ksteps);
+                    rows(t_dp, sdo, sk + L::TILE_B);
                     umma_commit(bb.dp_full);
                 }
                 __syncwarp();
@@ -707,17 +779,17 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                     if (ok) clean(s1);
                     // the scores before last have been read: their dx came before
                     if (ok && lane == 0) {
-                        mma_rows<T>(tmem + ((n + 1) & 1) * TILE, sq, sk1, ksteps);
+                        rows(tmem + ((n + 1) & 1) * TILE, sq, sk1);
                         umma_commit(&bb.s_full[(n + 1) & 1]);
                     }
                     __syncwarp();
                 }
                 ok = warp_wait(bb.dx_full, n & 1, ok, g.err);
                 if (ok && lane == 0) {
-                    mma_halves<T>(t_dq, t_dp, sk, idesc, n > 0);
+                    halves(t_dq, t_dp, sk, n > 0);
                     umma_commit(&bb.empty[s]);
                     if (kt >= 0) {
-                        mma_rows<T>(t_dp, sdo, sk1 + L::TILE_B, ksteps);
+                        rows(t_dp, sdo, sk1 + L::TILE_B);
                         umma_commit(bb.dp_full);
                     } else {
                         umma_commit(bb.done);
@@ -732,10 +804,12 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int wg = warp / 4, r = threadIdx.x % TILE, i = i0 + r;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const float c1 = a.scale * kLog2e;
-        const CapCoef cap = cap_coef(a.scale, CAP ? a.cap : 1.f);
+        const SplitExps ex = split_exps<SPLIT>(g, b, kvh);
+        const float scale = SPLIT ? a.scale * exp2f((float)-(ex.q + ex.k)) : a.scale, c1 = scale * kLog2e;
+        const CapCoef cap = cap_coef<SPLIT>(scale, CAP ? a.cap : 1.f);
         const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
         const float lift = dx_lift<T>(g, b, kvh), up = lift * PLift<T>::back;
+        const float up_dp = SPLIT ? up * exp2f((float)-(ex.dout + ex.v)) : up;   // dp carries the powers of dout and v
         const float* st = g.stats + (((int64_t)b * a.hq + h) * g.q_tiles + qt) * 2 * TILE;
         const float nl = st[r], nd = st[TILE + r] * up;
         const f2 nl2 = pack2(nl, nl), nd2 = pack2(nd, nd);
@@ -761,17 +835,20 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             f2 x[32];
             load64(tmem + (n & 1) * TILE + lanes + wg * 64, x);
             {
-                uint32_t unused[32];
-                grad_row<T, CAP, BIAS>(x, unused, c1, cap, slope2, jw - (mask.p0 + i), masked, bits0, bits1,
+                uint32_t unused[32], low[32];
+                grad_row<T, CAP, BIAS, SPLIT>(x, unused, low, c1, cap, slope2, jw - (mask.p0 + i), masked, bits0, bits1,
                                        [&](int) { return nl2; });
             }
             ok = warp_wait(bb.dp_full, n & 1, ok, g.err);
             if (!ok) break;
             {
-                uint32_t dp[64], dx[32];
+                // dq of the tile before, done before this dp: 32 columns a warpgroup
+                if (SPLIT && n > 0) tmem_add<DO / 2>(t_dqa + lanes + wg * (DO / 2), t_dq + lanes + wg * (DO / 2), n == 1);
+                uint32_t dp[64], dx[32], low[32];
                 load64(t_dp + lanes + wg * 64, dp);
-                grad_dx<T>(x, dp, dx, up, masked, bits0, bits1, [&](int) { return nd2; });
+                grad_dx<T, SPLIT>(x, dp, dx, low, up_dp, masked, bits0, bits1, [&](int) { return nd2; });
                 tmem_st32(t_dp + lanes + wg * 64, dx);
+                if (SPLIT) tmem_st32(t_dp + lanes + wg * 64 + 32, low);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -780,10 +857,20 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         if (any) ok = warp_wait(bb.done, 0, ok, g.err);
         // each warpgroup writes half of the columns
         if (ok) {
-            constexpr int HALF = DP / 2;
+            constexpr int HALF = DO / 2;
+            uint32_t at = t_dq + lanes + wg * HALF;
+            float mul = a.scale / lift;
+            if (SPLIT) {
+                if (any) {
+                    tmem_add<HALF>(t_dqa + lanes + wg * HALF, at, n == 1);
+                    tmem_wait_st();
+                }
+                at = t_dqa + lanes + wg * HALF;
+                mul *= exp2f((float)-ex.k);
+            }
             HeadsView v = a.dq;
-            v.p = static_cast<T*>(v.p) + wg * HALF;
-            store_row<T, HALF>(v, b, h, i, i < a.nq, a.d - wg * HALF, t_dq + lanes + wg * HALF, any, a.scale / lift);
+            v.p = static_cast<U*>(v.p) + wg * HALF * v.sd;
+            store_row<U, HALF>(v, b, h, i, i < a.nq, a.d - wg * HALF, at, any, any, mul);
         }
     }
     bb.finish(tmem);
@@ -791,7 +878,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 
 struct BwPlan {
     int q_tiles, k_tiles;
-    size_t stats, norms, q_ranges, k_ranges, bytes;
+    size_t stats, norms, q_ranges, k_ranges, split, bytes;
     explicit BwPlan(const AttnCall& a) {
         q_tiles = (a.nq + TILE - 1) / TILE;
         k_tiles = (a.nk + TILE - 1) / TILE;
@@ -801,15 +888,16 @@ struct BwPlan {
         norms = take(a.dtype == TL_TYPE_F16 ? (size_t)a.b * a.hkv * 8 : 0);
         q_ranges = take(a.q_doc ? (size_t)a.b * q_tiles * sizeof(DocRange) : 0);
         k_ranges = take(a.q_doc ? (size_t)a.b * k_tiles * sizeof(DocRange) : 0);
+        split = take(a.dtype == TL_TYPE_F32 ? SplitPlan(a, true).bytes : 0);
     }
 };
 
-template <typename T, int DP, bool CAP, bool BIAS>
-tl_status launch(tl_ctx* c, const HeadMap& mq, const HeadMap& mk, const HeadMap& mv, const HeadMap& mdo, const BwArgs& g, cudaStream_t s) {
+template <typename T, typename U, int DP, bool CAP, bool BIAS>
+tl_status launch(tl_ctx* c, const HeadMap* m, const BwArgs& g, cudaStream_t s) {
     static std::atomic<uint64_t> done_kv{0}, done_q{0};
     constexpr int smem = BwSmem<DP>::BYTES;
-    TL_TRY(kernel_smem(c, k_attn_tc_dkv<T, DP, CAP, BIAS>, smem, done_kv));
-    TL_TRY(kernel_smem(c, k_attn_tc_dq<T, DP, CAP, BIAS>, smem, done_q));
+    TL_TRY(kernel_smem(c, k_attn_tc_dkv<T, U, DP, CAP, BIAS>, smem, done_kv));
+    TL_TRY(kernel_smem(c, k_attn_tc_dq<T, U, DP, CAP, BIAS>, smem, done_q));
     const AttnCall& a = g.a;
     cudaEvent_t ev[2];
     cudaLaunchConfig_t cfg = {};
@@ -824,17 +912,26 @@ tl_status launch(tl_ctx* c, const HeadMap& mq, const HeadMap& mk, const HeadMap&
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     launch_begin_on(c, s, "attention_tc_dkv", 0, 8.0 * a.d * attn_pairs(a), ev);
-    TL_CK(c, cudaLaunchKernelEx(&cfg, k_attn_tc_dkv<T, DP, CAP, BIAS>, mq, mk, mv, mdo, g));
+    TL_CK(c, cudaLaunchKernelEx(&cfg, k_attn_tc_dkv<T, U, DP, CAP, BIAS>, m[0], m[1], m[2], m[3], g));
     TL_TRY(launch_end_on(c, s, ev));
     launch_begin_on(c, s, "attention_tc_dq", 0, 6.0 * a.d * attn_pairs(a), ev);
-    k_attn_tc_dq<T, DP, CAP, BIAS><<<(unsigned)((int64_t)g.q_tiles * a.b * a.hq), BW_THREADS, smem, s>>>(mq, mk, mv, mdo, g);
+    k_attn_tc_dq<T, U, DP, CAP, BIAS><<<(unsigned)((int64_t)g.q_tiles * a.b * a.hq), BW_THREADS, smem, s>>>(m[0], m[1], m[2], m[3], g);
     return launch_end_on(c, s, ev);
+}
+
+template <typename T, typename U, int DP>
+tl_status launch_scores(tl_ctx* c, const HeadMap* m, const BwArgs& g, cudaStream_t s) {
+    const bool bias = g.a.slopes != nullptr;
+    if (g.a.cap > 0.f) return bias ? launch<T, U, DP, true, true>(c, m, g, s) : launch<T, U, DP, true, false>(c, m, g, s);
+    return bias ? launch<T, U, DP, false, true>(c, m, g, s) : launch<T, U, DP, false, false>(c, m, g, s);
 }
 
 }  // namespace
 
 bool attn_tc_backward_takes(const AttnCall& a) {
-    return attn_tc_takes(a) && a.nq > 0 && tc_array(a.dout, a.b, a.hq, a.nq) && tc_array(a.dq, a.b, a.hq, a.nq) &&
+    if (!attn_tc_takes(a) || a.nq == 0) return false;
+    if (a.dtype == TL_TYPE_F32) return true;
+    return tc_array(a.dout, a.b, a.hq, a.nq) && tc_array(a.dq, a.b, a.hq, a.nq) &&
            tc_array(a.dk, a.b, a.hkv, a.nk) && tc_array(a.dv, a.b, a.hkv, a.nk);
 }
 
@@ -856,31 +953,43 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
     const int group = a.hq / a.hkv;
     g.cluster = group % 8 == 0 ? 8 : group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
     g.err = c->d_flags + 8;
-    HeadMap mq, mk, mv, mdo;
-    if (!make_head_map(&mq, a.q, a.dtype, a.b, a.hq, a.nq, a.d) || !make_head_map(&mk, a.k, a.dtype, a.b, a.hkv, a.nk, a.d) ||
-        !make_head_map(&mv, a.v, a.dtype, a.b, a.hkv, a.nk, a.d) || !make_head_map(&mdo, a.dout, a.dtype, a.b, a.hq, a.nq, a.d))
-        return fail(c, TL_ERR_CUDA, "attention: tensor maps");
     c->flags_armed = true;
-    if (norms) TL_CK(c, cudaMemsetAsync(norms, 0, (size_t)a.b * a.hkv * 8, s));
     if (a.q_doc) {
         TL_TRY(launch_doc_ranges(c, a.q_doc, a.b, a.nq, reinterpret_cast<DocRange*>(w + plan.q_ranges), s));
         TL_TRY(launch_doc_ranges(c, a.k_doc, a.b, a.nk, reinterpret_cast<DocRange*>(w + plan.k_ranges), s));
     }
-    const int64_t blocks = (int64_t)a.b * a.hq * plan.q_tiles + (norms ? (int64_t)a.b * a.hkv * plan.k_tiles : 0);
+    HeadMap m[4];
     const double rows = (double)a.b * a.hq * a.nq;
+    const int64_t tiles = (int64_t)a.b * a.hq * plan.q_tiles;
     cudaEvent_t ev[2];
+    if (a.dtype == TL_TYPE_F32) {
+        uint8_t* sw = w + plan.split;
+        const SplitPlan sp(a, true);
+        TL_TRY(launch_split(c, a, true, sw, m, s));
+        g.norms = reinterpret_cast<const uint32_t*>(sw + sp.norms);
+        g.tops.q = reinterpret_cast<const uint32_t*>(sw + sp.top);
+        g.tops.k = g.tops.q + (size_t)a.b * a.hkv;
+        g.tops.v = g.tops.k + (size_t)a.b * a.hkv;
+        g.tops.dout = g.tops.v + (size_t)a.b * a.hkv;
+        launch_begin_on(c, s, "attention_prep", 8.0 * rows * a.d, 2.0 * rows * a.d, ev);
+        k_attn_prep_f32<<<(unsigned)(2 * tiles), 256, 0, s>>>(a, stats, plan.q_tiles);
+        TL_TRY(launch_end_on(c, s, ev));
+        return launch_scores<__half, float, 128>(c, m, g, s);
+    }
+    g.tops = {nullptr, nullptr, nullptr, nullptr};
+    if (!make_head_map(&m[0], a.q, a.dtype, a.b, a.hq, a.nq, a.d) || !make_head_map(&m[1], a.k, a.dtype, a.b, a.hkv, a.nk, a.d) ||
+        !make_head_map(&m[2], a.v, a.dtype, a.b, a.hkv, a.nk, a.d) || !make_head_map(&m[3], a.dout, a.dtype, a.b, a.hq, a.nq, a.d))
+        return fail(c, TL_ERR_CUDA, "attention: tensor maps");
+    if (norms) TL_CK(c, cudaMemsetAsync(norms, 0, (size_t)a.b * a.hkv * 8, s));
+    const int64_t blocks = tiles + (norms ? (int64_t)a.b * a.hkv * plan.k_tiles : 0);
     launch_begin_on(c, s, "attention_prep", 4.0 * rows * a.d, 2.0 * rows * a.d, ev);
     if (a.dtype == TL_TYPE_F16) k_attn_prep<__half><<<(unsigned)blocks, 256, 0, s>>>(a, stats, norms, plan.q_tiles, plan.k_tiles);
     else k_attn_prep<__nv_bfloat16><<<(unsigned)blocks, 256, 0, s>>>(a, stats, norms, plan.q_tiles, plan.k_tiles);
     TL_TRY(launch_end_on(c, s, ev));
-#define TL_ATTN(T, DP)                                                                  \
-    (a.cap > 0.f ? (a.slopes ? launch<T, DP, true, true>(c, mq, mk, mv, mdo, g, s)      \
-                             : launch<T, DP, true, false>(c, mq, mk, mv, mdo, g, s))    \
-                 : (a.slopes ? launch<T, DP, false, true>(c, mq, mk, mv, mdo, g, s)     \
-                             : launch<T, DP, false, false>(c, mq, mk, mv, mdo, g, s)))
-    if (a.dtype == TL_TYPE_F16) return a.d <= 64 ? TL_ATTN(__half, 64) : TL_ATTN(__half, 128);
-    return a.d <= 64 ? TL_ATTN(__nv_bfloat16, 64) : TL_ATTN(__nv_bfloat16, 128);
-#undef TL_ATTN
+    if (a.dtype == TL_TYPE_F16)
+        return a.d <= 64 ? launch_scores<__half, __half, 64>(c, m, g, s) : launch_scores<__half, __half, 128>(c, m, g, s);
+    return a.d <= 64 ? launch_scores<__nv_bfloat16, __nv_bfloat16, 64>(c, m, g, s)
+                     : launch_scores<__nv_bfloat16, __nv_bfloat16, 128>(c, m, g, s);
 }
 
 }  // namespace tl

@@ -14,6 +14,15 @@ and gives each result with a bound for every element:
 and in every type a slack g relative to the sizes of the terms for the 32-bit
 arithmetic: scores that are off by s 2^-24 times a few, the exponential and
 the tanh (g = 2^-12 beside 16-bit roundings, 2^-16 in fp32).
+
+fp32 arrays of head size up to 64 go through the tensor cores as pairs of fp16
+numbers, hi + lo: a value x below 2^15 keeps 22 bits, or 2^-25 where that is
+more (fp16 ends at 2^-24, half a step of it).  In the backward pass p goes in as
+2^14 p, so it is off by up to 2^-25 / 2^14 = 2^-39; dx / scale goes in times the
+power of two L that puts B = 2 max|dout_i| max|v_j| (norms, over the heads of
+a group) between 2^14 and 2^15, L >= 2^14 / B, so it is off by up to
+2^-25 / L <= 2^-39 B.  Both are absolute, for every pair that is seen (tiny):
+they count where a key's every p is that small.
 """
 import math
 
@@ -89,10 +98,17 @@ def reference(q, k, v, dout=None, *, scale=None, softcap=0.0, slopes=None, causa
     def grouped(y):
         return y.view(b, hkv, group, nk, d).sum(2)
 
+    off_p = torch.zeros_like(p)
+    if q.dtype == torch.float32:
+        def top(y, heads):
+            return y.norm(dim=-1).amax(-1).view(b, hkv, heads).amax(-1).repeat_interleave(group, 1)
+        both = 2.0 * top(DO, group) * top(V, group) if nq and nk else torch.zeros((b, hq), device=dev)
+        off = off + seen * 2.0 ** -39 * both.view(b, hq, 1, 1) * scale
+        off_p = seen * 2.0 ** -39
     dq, dk, dv = dx @ K, grouped(dx.transpose(-1, -2) @ Q), grouped(p.transpose(-1, -2) @ DO)
     res["dq"] = (dq, h * dq.abs() + off @ K.abs() + tiny)
     res["dk"] = (dk, h * dk.abs() + grouped(off.transpose(-1, -2) @ Q.abs()) + tiny)
-    res["dv"] = (dv, h * dv.abs() + grouped(((h + g * big) * p).transpose(-1, -2) @ DO.abs()) + tiny)
+    res["dv"] = (dv, h * dv.abs() + grouped(((h + g * big) * p + off_p).transpose(-1, -2) @ DO.abs()) + tiny)
     return res
 
 
