@@ -66,6 +66,15 @@ template <> __device__ __forceinline__ uint32_t pack16<__half>(float lo, float h
 }
 
 // ---------------------------------------------------------------- tcgen05
+// One lane of a converged warp.  ptxas knows that the branch it guards has one
+// thread and keeps descriptors in uniform registers there (a branch on the lane
+// number costs about 90 cycles an MMA, more than the MMA).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p)::"memory");
+    return p != 0;
+}
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -103,6 +112,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
 // Instruction descriptor of kind::f16: fp32 sums, A and B of one 16-bit type,
 // A K-major, M = 128.
 template <typename T>
@@ -111,40 +129,48 @@ __device__ __forceinline__ constexpr uint32_t f16_idesc(int n, bool b_mn) {
     return (1u << 4) | (t << 7) | (t << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(TILE >> 4) << 24);
 }
-__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// The MMA warp shares its scheduler with the warps that compute, so every
+// instruction it needs beside tcgen05.mma delays the tensor cores: descriptors
+// differ only in the address field of their low word (16-byte units, below
+// 2^14, no carry), and each MMA costs one addition to it.  (In a cluster a
+// shared address carries the block's rank above these bits.)
+constexpr uint32_t kDescRows = 1024 >> 4;   // high word without the version and the swizzle: 8 rows (SBO)
+constexpr uint32_t kDescHigh = kDescRows | (1u << 14) | (2u << 29);   // version 1, 128-byte swizzle
+__device__ __forceinline__ uint32_t desc_rows(uint32_t saddr) { return ((saddr >> 4) & 0x3FFF) | (1u << 16); }   // K-major (LBO unused)
+__device__ __forceinline__ uint32_t desc_cols(uint32_t saddr) { return ((saddr >> 4) & 0x3FFF) | ((CHUNK_BYTES >> 4) << 16); }   // MN-major: LBO to the next 64 columns
+template <bool ACC>
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+        "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
+        "mov.b64 x, {%1, %4};\n\tmov.b64 y, {%2, %4};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "n"(kDescHigh), "n"(ACC ? 1 : 0));
 }
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+        "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\t"
+        "mov.b64 y, {%2, %4};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "n"(kDescHigh), "r"(accumulate));
 }
 
-// D[128 x 128] = A B^T over the head size (ksteps of 16), both K-major tiles.
-template <typename T>
+// D[128 x 128] = A B^T over the head size (ksteps of 16, at most N), both
+// K-major tiles.  N steps, all of them of the largest head size, are unrolled.
+template <typename T, int N>
 __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, int ksteps) {
     constexpr uint32_t idesc = f16_idesc<T>(TILE, false);
-    for (int k = 0; k < ksteps; ++k) {
-        const uint32_t at = (k >> 2) * CHUNK_BYTES + (k & 3) * 32;
-        umma_f16_ss(d, umma_desc(a + at, 16, 1024, kLayoutSW128), umma_desc(b + at, 16, 1024, kLayoutSW128), idesc,
-                    k > 0);
+    const uint32_t da = desc_rows(a), db = desc_rows(b);
+    auto at = [](int k) { return (uint32_t)((k / 4) * (CHUNK_BYTES >> 4) + (k % 4) * 2); };
+    umma_f16_ss<false>(d, da, db, idesc);
+    if (ksteps == N) {
+#pragma unroll
+        for (int k = 1; k < N; ++k) umma_f16_ss<true>(d, da + at(k), db + at(k), idesc);
+    } else {
+        for (int k = 1; k < ksteps; ++k) umma_f16_ss<true>(d, da + at(k), db + at(k), idesc);
     }
 }
-// D[128 x n] (+)= A B: A 128 x 128 16-bit in TMEM (two columns of it to a TMEM
-// column), B the tile's 128 rows as contracted index.
-template <typename T>
-__device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
-#pragma unroll
-    for (int k = 0; k < TILE / 16; ++k)
-        umma_f16_ts(d, a + 8 * k, umma_desc(b + k * 2048, CHUNK_BYTES, 1024, kLayoutSW128), idesc, accumulate | (k > 0));
-}
-
 // The same with operands in two parts (x = hi + lo, see SplitPlan): chunk 0 of a
 // tile holds hi, chunk 1 lo.  lo hi + hi lo + hi hi; lo lo, 2^-22 of the
 // product, is left out.  The small products go first: the tensor cores cut
@@ -152,26 +178,53 @@ __device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a, uint32_t b, uin
 // steps.
 template <typename T>
 __device__ __forceinline__ void mma_rows_split(uint32_t d, uint32_t a, uint32_t b, int ksteps) {
-    constexpr uint32_t idesc = f16_idesc<T>(TILE, false);
+    constexpr uint32_t idesc = f16_idesc<T>(TILE, false), low = CHUNK_BYTES >> 4;
+    const uint32_t da = desc_rows(a), db = desc_rows(b);
+    umma_f16_ss<false>(d, da + low, db, idesc);
+    if (ksteps == 4) {
 #pragma unroll
-    for (int part = 0; part < 3; ++part) {
-        const uint32_t pa = part == 0 ? CHUNK_BYTES : 0, pb = part == 1 ? CHUNK_BYTES : 0;
-        for (int k = 0; k < ksteps; ++k)
-            umma_f16_ss(d, umma_desc(a + pa + k * 32, 16, 1024, kLayoutSW128), umma_desc(b + pb + k * 32, 16, 1024, kLayoutSW128),
-                        idesc, part > 0 || k > 0);
+        for (int k = 1; k < 4; ++k) umma_f16_ss<true>(d, da + low + 2 * k, db + 2 * k, idesc);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_f16_ss<true>(d, da + 2 * k, db + low + 2 * k, idesc);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_f16_ss<true>(d, da + 2 * k, db + 2 * k, idesc);
+    } else {
+        for (int k = 1; k < ksteps; ++k) umma_f16_ss<true>(d, da + low + 2 * k, db + 2 * k, idesc);
+        for (int k = 0; k < ksteps; ++k) umma_f16_ss<true>(d, da + 2 * k, db + low + 2 * k, idesc);
+        for (int k = 0; k < ksteps; ++k) umma_f16_ss<true>(d, da + 2 * k, db + 2 * k, idesc);
     }
 }
-// D = A B anew (the caller adds the tiles up in fp32): A's parts in TMEM at
-// acol(part, k), k steps of 16 rows of the tile.
-template <typename T, typename F>
-__device__ __forceinline__ void mma_cols_split(uint32_t d, uint32_t b, uint32_t idesc, F acol) {
+// D[128 x n] (+)= A B: A 128 x 128 16-bit in TMEM, in two halves of 64 columns
+// (32 TMEM columns each, 64 apart: each over the fp32 scores it comes from), B
+// the tile's 128 rows as contracted index.
+__device__ __forceinline__ void mma_halves(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    const uint32_t db = desc_cols(b);
+    umma_f16_ts(d, a, db, idesc, accumulate);
+#pragma unroll
+    for (int k = 1; k < TILE / 16; ++k) umma_f16_ts(d, a + (k / 4) * 64 + (k % 4) * 8, db + k * (2048 >> 4), idesc, 1);
+}
+// D = A B anew for split operands (the caller adds the tiles up in fp32): in
+// each half's 64 TMEM columns 32 of hi, 32 of lo.
+__device__ __forceinline__ void mma_halves_split(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+    const uint32_t db = desc_cols(b);
 #pragma unroll
     for (int part = 0; part < 3; ++part)
 #pragma unroll
         for (int k = 0; k < TILE / 16; ++k)
-            umma_f16_ts(d, acol(part == 0 ? 1 : 0, k),
-                        umma_desc(b + (part == 1 ? CHUNK_BYTES : 0) + k * 2048, CHUNK_BYTES, 1024, kLayoutSW128), idesc,
-                        part > 0 || k > 0);
+            umma_f16_ts(d, a + (k / 4) * 64 + (part == 0 ? 32 : 0) + (k % 4) * 8,
+                        db + (part == 1 ? CHUNK_BYTES >> 4 : 0) + k * (2048 >> 4), idesc, part > 0 || k > 0);
+}
+// 64 columns of the warp's lanes
+__device__ __forceinline__ void load64(uint32_t taddr, uint32_t (&raw)[64]) {
+    tmem_ld32(taddr, raw);
+    tmem_ld32(taddr + 32, raw + 32);
+    tmem_wait_ld();
+}
+__device__ __forceinline__ void load64(uint32_t taddr, f2 (&x)[32]) {
+    uint32_t raw[64];
+    load64(taddr, raw);
+#pragma unroll
+    for (int k = 0; k < 32; ++k) x[k] = pack2(__uint_as_float(raw[2 * k]), __uint_as_float(raw[2 * k + 1]));
 }
 // hi and lo of a pair of values as fp16 pairs
 __device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t& lo) {
@@ -258,8 +311,8 @@ __device__ __forceinline__ void tma_tile(uint32_t dst, const HeadMap& m, uint64_
 // ---------------------------------------------------------------- capped scores
 // softcap tanh(x / softcap) as x P((x / softcap)^2), where P has the least
 // largest relative error for tanh(u) / u over the range (a linear programme
-// over a Chebyshev grid gives it).  16-bit probabilities: |u| <= 1, degree 4,
-// 6.9e-6, far below the rounding of p.  Fp32: |u| <= 0.625, degree 5, 3.9e-9, below
+// over a Chebyshev grid gives it).  16-bit probabilities: |u| <= 0.75, degree 3,
+// 1.1e-5, far below the rounding of p.  Fp32: |u| <= 0.625, degree 5, 3.9e-9, below
 // the rounding of fp32.  Tiles that hold a larger score take tanh u =
 // 1 - 2 / (1 + e^2u) (fp32: for those scores alone; there 1.2e-7 off is
 // relative to more than 0.55).
@@ -268,38 +321,43 @@ __device__ __forceinline__ constexpr float tanh_coef(int i) {
     if (FINE)
         return i == 0 ? 1.0f : i == 1 ? -0.3333325982093811f : i == 2 ? 0.13331125676631927f : i == 3 ? -0.053720925003290176f
                : i == 4 ? 0.020590508356690407f : -0.00565946102142334f;
-    return i == 0 ? 0.999993085861206f : i == 1 ? -0.3329806625843048f : i == 2 ? 0.13036811351776123f
-           : i == 3 ? -0.04481755569577217f : 0.009036424569785595f;
+    return i == 0 ? 0.9999889731407166f : i == 1 ? -0.33269670605659485f : i == 2 ? 0.12742698192596436f : -0.035452794283628464f;
 }
 
+template <bool FINE>
 struct CapCoef {
+    static constexpr int N = FINE ? 5 : 3;
     float limit;       // largest |q.k| of the polynomial
-    float k2;          // (scale / softcap)^2
-    float mul;         // scale log2 e
+    float k2;          // (scale / softcap)^2; fp32
+    float mul;         // scale log2 e; fp32
     float wide;        // 2 log2(e) scale / softcap: 2u in base 2
     float top;         // softcap log2 e
-};
-template <bool FINE>
-__device__ __forceinline__ CapCoef cap_coef(float scale, float cap) {
-    CapCoef c;
-    c.limit = (FINE ? 0.625f : 1.f) * (cap / scale);
-    c.k2 = (scale / cap) * (scale / cap);
-    c.mul = scale * kLog2e;
-    c.wide = 2.f * kLog2e * scale / cap;
-    c.top = cap * kLog2e;
-    return c;
-}
-__device__ __forceinline__ float wide_tanh(float x, float wide) { return 1.f - __fdividef(2.f, 1.f + ex2(x * wide)); }
-// tanh(u) / u of a pair of scores within the limit
-template <bool FINE>
-__device__ __forceinline__ f2 tanh_ratio(f2 x, f2 k2) {
-    constexpr int N = FINE ? 5 : 4;
-    const f2 z = mul2(mul2(x, x), k2);
-    f2 r = pack2(tanh_coef<FINE>(N), tanh_coef<FINE>(N));
+    float c[N + 1];    // 16-bit: P's coefficients times scale log2(e) k2^i
+    __device__ __forceinline__ CapCoef(float scale, float cap) {
+        limit = (FINE ? 0.625f : 0.75f) * (cap / scale);
+        k2 = (scale / cap) * (scale / cap);
+        mul = scale * kLog2e;
+        wide = 2.f * kLog2e * scale / cap;
+        top = cap * kLog2e;
+        float f = FINE ? 1.f : mul;
 #pragma unroll
-    for (int i = N - 1; i >= 0; --i) r = fma2(r, z, pack2(tanh_coef<FINE>(i), tanh_coef<FINE>(i)));
-    return r;
-}
+        for (int i = 0; i <= N; ++i) {
+            c[i] = tanh_coef<FINE>(i) * f;
+            if (!FINE) f *= k2;
+        }
+        if (!(fabsf(c[N]) < 3e38f)) limit = -1.f;   // out of range: never the polynomial
+    }
+    // score / x in base 2 of a pair within the limit
+    __device__ __forceinline__ f2 ratio(f2 x) const {
+        f2 z = mul2(x, x);
+        if (FINE) z = mul2(z, pack2(k2, k2));
+        f2 r = pack2(c[N], c[N]);
+#pragma unroll
+        for (int i = N - 1; i >= 0; --i) r = fma2(r, z, pack2(c[i], c[i]));
+        return FINE ? mul2(r, pack2(mul, mul)) : r;
+    }
+};
+__device__ __forceinline__ float wide_tanh(float x, float wide) { return 1.f - __fdividef(2.f, 1.f + ex2(x * wide)); }
 // The largest |score| of a row.
 template <int N>
 __device__ __forceinline__ float largest(const f2 (&x)[N]) {
@@ -312,25 +370,19 @@ __device__ __forceinline__ float largest(const f2 (&x)[N]) {
     }
     return big;
 }
-// softcap tanh(x / softcap) in base 2 of a pair, in a tile with scores past
-// the limit; *t: the tanh.
+// The score in base 2 of a pair in a tile with scores past the limit.
 template <bool FINE>
-__device__ __forceinline__ f2 wide_score(f2 x, const CapCoef& cap, f2* t) {
+__device__ __forceinline__ f2 wide_score(f2 x, const CapCoef<FINE>& cap) {
     float lo, hi;
     unpack2(x, lo, hi);
-    f2 y = pack2(cap.top * wide_tanh(lo, cap.wide), cap.top * wide_tanh(hi, cap.wide));
-    *t = pack2(wide_tanh(lo, cap.wide), wide_tanh(hi, cap.wide));
+    float y = cap.top * wide_tanh(lo, cap.wide), z = cap.top * wide_tanh(hi, cap.wide);
     if (FINE) {
-        float a, b, c, d, e, f;
-        const f2 xr = mul2(x, tanh_ratio<true>(x, pack2(cap.k2, cap.k2)));
-        unpack2(mul2(xr, pack2(cap.mul, cap.mul)), a, b);
-        unpack2(mul2(xr, pack2(sqrtf(cap.k2), sqrtf(cap.k2))), c, d);
-        unpack2(*t, e, f);
-        *t = pack2(fabsf(lo) <= cap.limit ? c : e, fabsf(hi) <= cap.limit ? d : f);
-        unpack2(y, e, f);
-        y = pack2(fabsf(lo) <= cap.limit ? a : e, fabsf(hi) <= cap.limit ? b : f);
+        float a, b;
+        unpack2(mul2(x, cap.ratio(x)), a, b);
+        y = fabsf(lo) <= cap.limit ? a : y;
+        z = fabsf(hi) <= cap.limit ? b : z;
     }
-    return y;
+    return pack2(y, z);
 }
 
 // ---------------------------------------------------------------- documents
@@ -384,26 +436,25 @@ struct TileWalk {
     }
 };
 
-// Bits of the 128 other positions whose document is `doc`, lane by lane: the
-// lane holds the documents of positions lane, 32 + lane, ... in other[4] and
+// Bits of the 64 other positions whose document is `doc`, lane by lane: the
+// lane holds the documents of positions lane and 32 + lane in other[2] and
 // wants its own row's doc.  The distinct documents of a warp's rows are few
-// (one ballot each).
-__device__ __forceinline__ void doc_bits(const int (&other)[4], int doc, uint32_t (&bits)[4]) {
+// (two ballots each).
+__device__ __forceinline__ void doc_bits(const int (&other)[2], int doc, uint32_t (&bits)[2]) {
     uint32_t left = 0xffffffffu;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) bits[w] = 0;
+    bits[0] = bits[1] = 0;
     while (left) {
         const int d = __shfl_sync(0xffffffffu, doc, __ffs(left) - 1);
         const bool mine = doc == d;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < 2; ++w) {
             const uint32_t m = __ballot_sync(0xffffffffu, other[w] == d && d >= 0);
             if (mine) bits[w] = m;
         }
         left &= ~__ballot_sync(0xffffffffu, mine);
     }
 }
-// the low n bits of word w of a 128-bit row
+// the low n bits of word w of a row
 __device__ __forceinline__ uint32_t low_bits(int n, int w) {
     const int k = n - 32 * w;
     return k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1;

@@ -224,7 +224,7 @@ struct DecRow {
         slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
     }
     // q.k -> score in base 2, -inf when not seen
-    __device__ __forceinline__ float score(float x, int j, int jdoc, const AttnCall& a, const CapCoef& cap) const {
+    __device__ __forceinline__ float score(float x, int j, int jdoc, const AttnCall& a, const CapCoef<false>& cap) const {
         float y = a.cap > 0.f ? cap.top * wide_tanh(x, cap.wide) : x * cap.mul;
         y -= slope2 * fabsf((float)(p - j));
         return j < limit && (!a.k_doc || (doc >= 0 && jdoc == doc)) ? y : -INFINITY;
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
         return;
     }
 
-    const CapCoef cap = cap_coef<false>(a.scale, a.cap > 0.f ? a.cap : 1.f);
+    const CapCoef<false> cap(a.scale, a.cap > 0.f ? a.cap : 1.f);
     const int gid = lane >> 2, tid = lane & 3, mi = lane >> 3, mr = lane & 7;
     const int ksteps = (a.d + 15) / 16;
     T* qs = reinterpret_cast<T*>(smem + L::Q);
@@ -619,7 +619,6 @@ __global__ void __launch_bounds__(DA_THREADS) k_decode_any(const __grid_constant
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     PieceWalk walk = block_pieces<DA_THREADS / 32>(g, red, found);
-    const CapCoef cap = cap_coef<false>(a.scale == 0.f ? 1.f : a.scale, a.cap > 0.f ? a.cap : 1.f);
     const int group = a.hq / a.hkv;
     constexpr int NC = DP >= 128 ? DP / 128 : 1, LANES = DP >= 128 ? 32 : DP / 4;
     Piece pc;

@@ -6,12 +6,13 @@
 // rows of two heads of a group where the group has an even number of heads
 // (each causal tile then needs exactly the keys the block loads), else
 // neighbouring rows of one head.  Warps:
-//   0-3, 4-7  one query row per thread of tile 0, 1: scores out of TMEM,
-//             softmax statistics, probabilities (16-bit) back into TMEM over
-//             the scores
-//   8         tensor cores: S = Q K^T (SMEM x SMEM), O += P V (TMEM x SMEM)
-//   9         TMA: Q once, then K and V tiles through a ring of four
-// TMEM: S0 S1 (128 columns each, P over their first half), O0 O1.  While one
+//   0-7, 8-15  tile 0, 1: a thread has 64 of a query's 128 scores: scores out
+//              of TMEM, softmax statistics (the two halves of a row agree on
+//              its maximum through shared memory), probabilities (16-bit) back
+//              into TMEM over the scores
+//   16         tensor cores: S = Q K^T (SMEM x SMEM), O += P V (TMEM x SMEM)
+//   17         TMA: Q once, then K and V tiles through a ring of four
+// TMEM: S0 S1 (128 columns each, P over the first half of each 64), O0 O1.  While one
 // tile's softmax runs, the other tile's products do; S of the next keys is
 // issued right behind P V of these, which orders it after P is read.
 //
@@ -33,7 +34,14 @@
 namespace tl {
 namespace {
 
-constexpr int FW_THREADS = 384, FW_STAGES = 4;
+constexpr int FW_SOFTMAX = 512, FW_THREADS = FW_SOFTMAX + 64, FW_STAGES = 4;
+constexpr int FW_MMA = FW_SOFTMAX / 32, FW_TMA = FW_MMA + 1;   // warps
+// Capped scores lie in +-top (base 2), so bf16, which has the range of fp32,
+// needs no maximum: with the reference top - 20 every p lies in 2^(20 - 2 top)
+// .. 2^20, above 2^-125 up to top = 72.5 (softcap 50.2).  No maxima, no agreeing
+// on them, no rescaling.
+constexpr float kFixTop = 72.5f;
+__device__ __forceinline__ float fixed_top(float top) { return top - 20.f; }
 constexpr float kGrow = 8.f;   // rescale when the maximum grew by 2^8
 
 struct FwArgs {
@@ -49,8 +57,8 @@ struct FwArgs {
 template <int DP>
 struct FwSmem {
     static constexpr int CH = DP / 64, TILE_B = CH * CHUNK_BYTES;
-    static constexpr int Q = 0, KV = 2 * TILE_B, BAR = KV + FW_STAGES * TILE_B, DOCS = BAR + 256,
-                         BYTES = DOCS + 64 + 1024;
+    static constexpr int Q = 0, KV = 2 * TILE_B, BAR = KV + FW_STAGES * TILE_B, DOCS = BAR + 256, ROWS = DOCS + 64,
+                         BYTES = ROWS + 2 * 2 * 2 * TILE * 4 + 1024;   // ROWS: [parity][tile][half][row]
 };
 
 // the smallest / largest document of each tile of 128 keys (queries), a warp per tile
@@ -75,43 +83,39 @@ __global__ void __launch_bounds__(256) k_doc_ranges(const int32_t* __restrict__ 
     if (lane == 0) out[t] = r;
 }
 
-// One tile of scores of this thread's row: x (q.k) in registers becomes the
+// 64 scores of this thread's row: x (q.k) in registers becomes the
 // score in base 2 times c (see below), with -inf where the key is not seen.
 // Returns the row's largest c-scaled score.
 //   !CAP && !BIAS: x is left as it is and c = scale log2 e; else c = 1.
-//   FINE: the tanh to fp32
-template <bool CAP, bool BIAS, bool FINE>
-__device__ __forceinline__ float score_row(f2 (&x)[TILE / 2], float c1, const CapCoef& cap, float slope2, int p, int j0,
-                                           bool masked, const uint32_t (&bits)[4]) {
+//   FINE: the tanh to fp32; FIX: shift is added and no maximum taken
+template <bool CAP, bool BIAS, bool FINE, bool FIX>
+__device__ __forceinline__ float score_row(f2 (&x)[32], float c1, const CapCoef<FINE>& cap, f2 shift, float slope2, int p, int j0,
+                                           bool masked, uint32_t bits0, uint32_t bits1) {
     if (CAP) {
         if (__any_sync(0xffffffffu, !(largest(x) <= cap.limit))) {
 #pragma unroll
-            for (int i = 0; i < TILE / 2; ++i) {
-                f2 t;
-                x[i] = wide_score<FINE>(x[i], cap, &t);
-            }
+            for (int i = 0; i < 32; ++i) x[i] = FIX ? add2(wide_score<FINE>(x[i], cap), shift) : wide_score<FINE>(x[i], cap);
         } else {
-            const f2 k2 = pack2(cap.k2, cap.k2), mul = pack2(cap.mul, cap.mul);
 #pragma unroll
-            for (int i = 0; i < TILE / 2; ++i) x[i] = mul2(mul2(x[i], mul), tanh_ratio<FINE>(x[i], k2));
+            for (int i = 0; i < 32; ++i) x[i] = FIX ? fma2(x[i], cap.ratio(x[i]), shift) : mul2(x[i], cap.ratio(x[i]));
         }
     }
     if (BIAS) {
         // -slope |p - j| is linear in j on either side of p
-        const bool before = __all_sync(0xffffffffu, j0 + TILE - 1 <= p), after = __all_sync(0xffffffffu, j0 >= p);
+        const bool before = __all_sync(0xffffffffu, j0 + 63 <= p), after = __all_sync(0xffffffffu, j0 >= p);
         const f2 c = CAP ? pack2(1.f, 1.f) : pack2(c1, c1);
         if (before || after) {
             const float k = before ? slope2 : -slope2, kb = k * (float)(j0 - p);
             const f2 kk = pack2(k, k), base = pack2(kb, kb);
 #pragma unroll
-            for (int i = 0; i < TILE / 2; ++i) {
+            for (int i = 0; i < 32; ++i) {
                 const f2 bias = fma2(kk, pack2((float)(2 * i), (float)(2 * i + 1)), base);
                 x[i] = CAP ? add2(x[i], bias) : fma2(x[i], c, bias);
             }
         } else {
             const float at = (float)(j0 - p);
 #pragma unroll
-            for (int i = 0; i < TILE / 2; ++i) {
+            for (int i = 0; i < 32; ++i) {
                 const f2 bias = pack2(-slope2 * fabsf(at + (float)(2 * i)), -slope2 * fabsf(at + (float)(2 * i + 1)));
                 x[i] = CAP ? add2(x[i], bias) : fma2(x[i], c, bias);
             }
@@ -119,18 +123,19 @@ __device__ __forceinline__ float score_row(f2 (&x)[TILE / 2], float c1, const Ca
     }
     if (masked) {
 #pragma unroll
-        for (int i = 0; i < TILE / 2; ++i) {
+        for (int i = 0; i < 32; ++i) {
             float lo, hi;
             unpack2(x[i], lo, hi);
-            const uint32_t w = bits[i / 16];
+            const uint32_t w = i < 16 ? bits0 : bits1;
             lo = (w >> (2 * i % 32)) & 1 ? lo : -INFINITY;
             hi = (w >> (2 * i % 32 + 1)) & 1 ? hi : -INFINITY;
             x[i] = pack2(lo, hi);
         }
     }
+    if (FIX) return 0.f;
     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int i = 0; i < TILE / 2; ++i) {
+    for (int i = 0; i < 32; ++i) {
         float lo, hi;
         unpack2(x[i], lo, hi);
         top[i % 4] = fmaxf(top[i % 4], fmaxf(lo, hi));
@@ -139,8 +144,8 @@ __device__ __forceinline__ float score_row(f2 (&x)[TILE / 2], float c1, const Ca
 }
 
 // T: operands, U: the arrays' type (float: split operands, DP = 128 columns of
-// hi and lo)
-template <typename T, typename U, int DP, bool CAP, bool BIAS>
+// hi and lo).  FIX: see fixed_top.
+template <typename T, typename U, int DP, bool CAP, bool BIAS, bool FIX>
 __global__ void __launch_bounds__(FW_THREADS, 1)
     k_attn_tc(const __grid_constant__ HeadMap mq, const __grid_constant__ HeadMap mk, const __grid_constant__ HeadMap mv,
               const __grid_constant__ FwArgs g) {
@@ -175,15 +180,15 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
         for (int s = 0; s < FW_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&p_full[t], TILE); mbar_init(&o_done[t], 1); }
+        for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 2 * TILE); mbar_init(&o_done[t], 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         docs[0] = 0x7fffffff; docs[1] = -1; docs[2] = 0;
     }
-    if (warp == 8) {
+    if (warp == FW_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    if (warp == 9 && lane == 0) {
+    if (warp == FW_TMA && lane == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mq.map)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mk.map)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mv.map)) : "memory");
@@ -215,9 +220,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     }
     bool masked, ok = true;
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 9) {
+    if (warp >= FW_MMA) {
+        if (warp == FW_TMA) {
             // ------------------------------------------------ TMA
             int kt = walk.next(&masked);
             int n = 0;   // ring entries filled
@@ -240,7 +244,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             }
             if (!ok)   // copies in flight land before the block ends
                 for (int e = max(0, n - FW_STAGES); e < n - 1; ++e) mbar_wait(&full[e % FW_STAGES], (e / FW_STAGES) & 1, g.err);
-        } else if (warp == 8) {
+        } else if (warp == FW_MMA) {
             // ------------------------------------------------ tensor cores
             const int ksteps = (a.d + 15) / 16;
             const uint32_t idesc_o = f16_idesc<T>(16 * ksteps, true);
@@ -252,10 +256,10 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 tc_fence_after();
             };
             auto scores = [&](int t, int stage) {
-                if (ok && lane == 0) {
+                if (ok && elect_one()) {
                     const uint32_t sq = smem_u32(smem + L::Q + t * L::TILE_B), sk = smem_u32(smem + L::KV + stage * L::TILE_B);
                     if (SPLIT) mma_rows_split<T>(tmem + t * TILE, sq, sk, ksteps);
-                    else mma_rows<T>(tmem + t * TILE, sq, sk, ksteps);
+                    else mma_rows<T, DP / 16>(tmem + t * TILE, sq, sk, ksteps);
                     umma_commit(&s_full[t]);
                 }
                 __syncwarp();
@@ -264,7 +268,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 wait_full(q_full, 0, 1);
                 wait_full(full, n, FW_STAGES);
                 for (int t = 0; t < g.tiles; ++t) scores(t, n % FW_STAGES);
-                if (ok && lane == 0) umma_commit(&empty[n % FW_STAGES]);
+                if (ok && elect_one()) umma_commit(&empty[n % FW_STAGES]);
                 ++n;
             }
             for (int it = 0; kt >= 0 && ok; ++it) {
@@ -282,25 +286,23 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 }
                 bool next_masked;
                 const int next = walk.next(&next_masked);
+                if (next >= 0) wait_full(full, n, FW_STAGES);   // the next keys: nothing waits between P V and S
                 for (int t = 0; t < g.tiles; ++t) {
                     ok = ok && mbar_wait(&p_full[t], it & 1, g.err);
                     ok = __all_sync(0xffffffffu, ok);
                     tc_fence_after();
-                    if (ok && lane == 0) {
+                    if (ok && elect_one()) {
                         const uint32_t to = tmem + 2 * TILE + t * DO, sv = smem_u32(smem + L::KV + vs * L::TILE_B);
-                        if (SPLIT)
-                            mma_cols_split<T>(to, sv, idesc_o, [&](int part, int k) { return tmem + t * TILE + part * 64 + 8 * k; });
-                        else
-                            mma_cols<T>(to, tmem + t * TILE, sv, idesc_o, it > 0);
+                        if (SPLIT) mma_halves_split(to, tmem + t * TILE, sv, idesc_o);
+                        else mma_halves(to, tmem + t * TILE, sv, idesc_o, it > 0);
                         if (next < 0) umma_commit(&o_done[t]);
                     }
                     __syncwarp();
                     if (next >= 0) {
-                        if (t == 0) wait_full(full, n, FW_STAGES);
                         scores(t, n % FW_STAGES);
                     }
                 }
-                if (ok && lane == 0) {
+                if (ok && elect_one()) {
                     umma_commit(&empty[vs]);
                     if (next >= 0) umma_commit(&empty[n % FW_STAGES]);
                 }
@@ -310,78 +312,78 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 masked = next_masked;
             }
         }
-    } else if (warp / 4 < g.tiles) {
-        // ---------------------------------------------------- a row per thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-        const int t = warp / 4, r = threadIdx.x % TILE;
+    } else if (warp / 8 < g.tiles) {
+        // ---------------------------------------------------- half a row per thread
+        const int t = warp / 8, half = warp / 4 % 2, r = threadIdx.x % TILE;
         const int i = i0 + r + (g.pair_heads ? 0 : t * TILE), h = h0 + (g.pair_heads ? t : 0);
         const int p = mask.p0 + i, limit = mask.key_end(i, 1);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + t * TILE + lanes, to = tmem + 2 * TILE + t * DO + lanes;
-        const uint32_t acc = SPLIT ? tmem + 3 * TILE + t * DO + lanes : to;   // the sum over the tiles
+        constexpr int DH = DO / 2;            // this thread's columns of O
+        const uint32_t ts = tmem + t * TILE + half * 64 + lanes, to = tmem + 2 * TILE + t * DO + half * DH + lanes;
+        const uint32_t acc = SPLIT ? to + TILE : to;   // the sum over the tiles
+        float* rows_at = reinterpret_cast<float*>(smem + L::ROWS) + t * 2 * TILE + r;   // [parity][tile][half][row]
         // split operands carry powers of two of their heads
         const int e_qk = SPLIT ? split_exp(g.tops.q, b * a.hkv + kvh) + split_exp(g.tops.k, b * a.hkv + kvh) : 0;
         const float scale = SPLIT ? a.scale * exp2f((float)-e_qk) : a.scale;
         const float c1 = scale * kLog2e, c = CAP || BIAS ? 1.f : c1;
-        const CapCoef cap = cap_coef<SPLIT>(scale, CAP ? a.cap : 1.f);
+        const CapCoef<SPLIT> cap(scale, CAP ? a.cap : 1.f);
+        const float fix = fixed_top(cap.top);
+        const f2 shift = pack2(-fix, -fix);
         const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
         const int doc = qd && i < a.nq ? qd[i] : -1;
         float m = -INFINITY, l = 0.f;
         int it = 0;
         for (int kt = walk.next(&masked); kt >= 0; kt = walk.next(&masked), ++it) {
-            const int j0 = kt * TILE;
-            uint32_t bits[4];
+            const int j0 = kt * TILE + half * 64;
+            uint32_t bits0 = 0xffffffffu, bits1 = 0xffffffffu;
             if (masked) {
+                bits0 = low_bits(limit - j0, 0);
+                bits1 = low_bits(limit - j0, 1);
                 if (kd) {
-                    int other[4];
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const int j = j0 + 32 * w + lane;
-                        other[w] = j < a.nk ? __ldg(kd + j) : -1;
-                    }
-                    doc_bits(other, doc, bits);
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) bits[w] &= low_bits(limit - j0, w);
-                } else {
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) bits[w] = low_bits(limit - j0, w);
+                    const int other[2] = {j0 + lane < a.nk ? __ldg(kd + j0 + lane) : -1,
+                                          j0 + 32 + lane < a.nk ? __ldg(kd + j0 + 32 + lane) : -1};
+                    uint32_t same[2];
+                    doc_bits(other, doc, same);
+                    bits0 &= same[0];
+                    bits1 &= same[1];
                 }
             }
             ok = ok && mbar_wait(&s_full[t], it & 1, g.err);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc_fence_after();
-            if (SPLIT && it > 0) tmem_add<DO>(acc, to, it == 1);   // P V of the tile before, done before this S
-            f2 x[TILE / 2];
-            {
-                uint32_t raw[TILE];
+            if (SPLIT && it > 0) tmem_add<DH>(acc, to, it == 1);   // P V of the tile before, done before this S
+            f2 x[32];
+            load64(ts, x);
+            float top = c * score_row<CAP, BIAS, SPLIT, FIX>(x, c1, cap, shift, slope2, p, j0, masked, bits0, bits1);
+            if (!FIX) {
+                // the row's other half
+                float* mine_at = rows_at + (it & 1) * 4 * TILE;
+                mine_at[half * TILE] = top;
+                asm volatile("bar.sync %0, 256;" ::"r"(1 + t) : "memory");
+                top = fmaxf(top, mine_at[(1 - half) * TILE]);
+                // a new reference maximum, for the first seen key of a row or a large step
+                if (__any_sync(0xffffffffu, top > m + kGrow || (m == -INFINITY && top > m))) {
+                    const float nm = fmaxf(m, top);
+                    const float by = nm == -INFINITY ? 1.f : ex2(m - nm);
+                    l *= by;
+                    m = nm;
+                    if (it > 0) {
+                        if (SPLIT) tmem_wait_st();
+                        const f2 by2 = pack2(by, by);
+#pragma unroll 1
+                        for (int k = 0; k < DH / 16; ++k) {
+                            uint32_t o[16];
+                            tmem_ld16(acc + 16 * k, o);
+                            tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < 4; ++k) tmem_ld32(ts + 32 * k, raw + 32 * k);
-                tmem_wait_ld();
-#pragma unroll
-                for (int k = 0; k < TILE / 2; ++k) x[k] = pack2(__uint_as_float(raw[2 * k]), __uint_as_float(raw[2 * k + 1]));
-            }
-            const float top = c * score_row<CAP, BIAS, SPLIT>(x, c1, cap, slope2, p, j0, masked, bits);
-            // a new reference maximum, for the first seen key of a row or a large step
-            if (__any_sync(0xffffffffu, top > m + kGrow || (m == -INFINITY && top > m))) {
-                const float nm = fmaxf(m, top);
-                const float by = nm == -INFINITY ? 1.f : ex2(m - nm);
-                l *= by;
-                m = nm;
-                if (it > 0) {
-                    if (SPLIT) tmem_wait_st();
-                    const f2 by2 = pack2(by, by);
-                    for (int k = 0; k < DO / 32; ++k) {
-                        uint32_t o[32];
-                        tmem_ld32(acc + 32 * k, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) {
-                            float lo, hi;
-                            unpack2(mul2(pack2(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1])), by2), lo, hi);
-                            o[2 * q] = __float_as_uint(lo);
-                            o[2 * q + 1] = __float_as_uint(hi);
+                            for (int q = 0; q < 8; ++q) {
+                                float lo, hi;
+                                unpack2(mul2(pack2(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1])), by2), lo, hi);
+                                o[2 * q] = __float_as_uint(lo);
+                                o[2 * q + 1] = __float_as_uint(hi);
+                            }
+                            tmem_st16(acc + 16 * k, o);
                         }
-                        tmem_st32(acc + 32 * k, o);
                     }
                 }
             }
@@ -390,12 +392,12 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             const f2 c2 = pack2(c, c), ref2 = pack2(-ref, -ref);
             f2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 2; ++k) {
                 uint32_t out[16], low[SPLIT ? 16 : 1];
 #pragma unroll
                 for (int q = 0; q < 16; ++q) {
                     float lo, hi;
-                    unpack2(CAP || BIAS ? add2(x[16 * k + q], ref2) : fma2(x[16 * k + q], c2, ref2), lo, hi);
+                    unpack2(FIX ? x[16 * k + q] : CAP || BIAS ? add2(x[16 * k + q], ref2) : fma2(x[16 * k + q], c2, ref2), lo, hi);
                     lo = ex2(lo);
                     hi = ex2(hi);
                     sum[q & 1] = add2(sum[q & 1], pack2(lo, hi));
@@ -403,7 +405,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                     else out[q] = pack16<T>(lo, hi);
                 }
                 tmem_st16(ts + 16 * k, out);
-                if (SPLIT) tmem_st16(ts + 64 + 16 * k, low);
+                if (SPLIT) tmem_st16(ts + 32 + 16 * k, low);
             }
             {
                 float lo, hi;
@@ -420,44 +422,52 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
         }
+        float* mine_at = rows_at + (it & 1) * 4 * TILE;
+        mine_at[half * TILE] = l;
+        asm volatile("bar.sync %0, 256;" ::"r"(1 + t) : "memory");
+        l += mine_at[(1 - half) * TILE];
         const bool none = it == 0 || l == 0.f;   // no key seen
         float inv = none ? 0.f : 1.f / l;
         if (ok && SPLIT && it > 0) {
-            tmem_add<DO>(acc, to, it == 1);
+            tmem_add<DH>(acc, to, it == 1);
             tmem_wait_st();
             inv *= exp2f((float)-split_exp(g.tops.v, b * a.hkv + kvh));
         }
         if (ok) {
-            store_row<U, DO>(a.o, b, h, i, i < a.nq, a.d, acc, !none, it > 0, inv);
-            if (a.lse && i < a.nq)
-                a.lse[((int64_t)b * a.hq + h) * a.nq + i] = none ? -INFINITY : (m - Lift<T>::log2) * kLn2 + logf(l);
+            HeadsView o = a.o;
+            o.p = static_cast<U*>(o.p) + half * DH * o.sd;
+            store_row<U, DH>(o, b, h, i, i < a.nq, a.d - half * DH, acc, !none, it > 0, inv);
+            if (a.lse && i < a.nq && half == 0)
+                a.lse[((int64_t)b * a.hq + h) * a.nq + i] = none ? -INFINITY : (FIX ? fix : m - Lift<T>::log2) * kLn2 + logf(l);
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == FW_MMA) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
     }
 }
 
-template <typename T, typename U, int DP, bool CAP, bool BIAS>
+template <typename T, typename U, int DP, bool CAP, bool BIAS, bool FIX = false>
 tl_status launch(tl_ctx* c, const HeadMap* m, const FwArgs& g, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     constexpr int smem = FwSmem<DP>::BYTES;
-    TL_TRY(kernel_smem(c, k_attn_tc<T, U, DP, CAP, BIAS>, smem, done));
+    TL_TRY(kernel_smem(c, k_attn_tc<T, U, DP, CAP, BIAS, FIX>, smem, done));
     const AttnCall& a = g.a;
     const int span = g.pair_heads ? TILE : g.tiles * TILE;
     const int64_t grid = (int64_t)a.b * (g.pair_heads ? a.hq / 2 : a.hq) * ((a.nq + span - 1) / span);
     cudaEvent_t ev[2];
     launch_begin_on(c, s, "attention_tc", 0, 4.0 * a.d * attn_pairs(a), ev);
-    k_attn_tc<T, U, DP, CAP, BIAS><<<(unsigned)grid, FW_THREADS, smem, s>>>(m[0], m[1], m[2], g);
+    k_attn_tc<T, U, DP, CAP, BIAS, FIX><<<(unsigned)grid, FW_THREADS, smem, s>>>(m[0], m[1], m[2], g);
     return launch_end_on(c, s, ev);
 }
 
 template <typename T, typename U, int DP>
 tl_status launch_scores(tl_ctx* c, const HeadMap* m, const FwArgs& g, cudaStream_t s) {
     const bool bias = g.a.slopes != nullptr;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        if (g.a.cap > 0.f && !bias && g.a.cap * kLog2e <= kFixTop) return launch<T, U, DP, true, false, true>(c, m, g, s);
     if (g.a.cap > 0.f) return bias ? launch<T, U, DP, true, true>(c, m, g, s) : launch<T, U, DP, true, false>(c, m, g, s);
     return bias ? launch<T, U, DP, false, true>(c, m, g, s) : launch<T, U, DP, false, false>(c, m, g, s);
 }

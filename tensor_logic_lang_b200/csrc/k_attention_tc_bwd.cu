@@ -203,27 +203,21 @@ __device__ __forceinline__ float dx_lift(const BwArgs& g, int b, int kvh) {
 // nl(i): minus log2(e) lse of the columns 2i, 2i + 1.
 // SPLIT: p16 and low take hi and lo, and the tanh is good to fp32.
 template <typename T, bool CAP, bool BIAS, bool SPLIT, typename NL>
-__device__ __forceinline__ void grad_row(f2 (&x)[32], uint32_t (&p16)[32], uint32_t (&low)[32], float c1, const CapCoef& cap, float slope2, int off,
+__device__ __forceinline__ void grad_row(f2 (&x)[32], uint32_t (&p16)[32], uint32_t (&low)[32], float c1, const CapCoef<SPLIT>& cap, float slope2, int off,
                                          bool masked, uint32_t bits0, uint32_t bits1, NL nl) {
     f2 bend[CAP ? 32 : 1];
     if (CAP) {
-        const f2 one = pack2(1.f, 1.f);
         if (__any_sync(0xffffffffu, !(largest(x) <= cap.limit))) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                f2 t;
-                x[i] = wide_score<SPLIT>(x[i], cap, &t);
-                bend[i] = fma2(mul2(t, pack2(-1.f, -1.f)), t, one);
-            }
+            for (int i = 0; i < 32; ++i) x[i] = wide_score<SPLIT>(x[i], cap);
         } else {
-            const f2 k2 = pack2(cap.k2, cap.k2), mul = pack2(cap.mul, cap.mul), neg = pack2(-cap.k2, -cap.k2);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const f2 r = tanh_ratio<SPLIT>(x[i], k2), xr = mul2(x[i], r);
-                bend[i] = fma2(mul2(xr, neg), xr, one);
-                x[i] = mul2(xr, mul);
-            }
+            for (int i = 0; i < 32; ++i) x[i] = mul2(x[i], cap.ratio(x[i]));
         }
+        // 1 - tanh^2, the tanh from the score
+        const float inv = -1.f / (cap.top * cap.top);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) bend[i] = fma2(mul2(x[i], pack2(inv, inv)), x[i], pack2(1.f, 1.f));
     }
     const f2 c = CAP ? pack2(1.f, 1.f) : pack2(c1, c1);
     if (BIAS) {
@@ -277,34 +271,6 @@ __device__ __forceinline__ void grad_dx(const f2 (&pb)[32], const uint32_t (&dp)
         if (SPLIT) split16(lo, hi, out[i], low[i]);
         else out[i] = pack16<T>(lo, hi);
     }
-}
-
-__device__ __forceinline__ void load64(uint32_t taddr, uint32_t (&raw)[64]) {
-    tmem_ld32(taddr, raw);
-    tmem_ld32(taddr + 32, raw + 32);
-    tmem_wait_ld();
-}
-__device__ __forceinline__ void load64(uint32_t taddr, f2 (&x)[32]) {
-    uint32_t raw[64];
-    load64(taddr, raw);
-#pragma unroll
-    for (int k = 0; k < 32; ++k) x[k] = pack2(__uint_as_float(raw[2 * k]), __uint_as_float(raw[2 * k + 1]));
-}
-
-// D[128 x n] (+)= A B as mma_cols, A in two halves of 64 columns of the
-// contracted index, 32 TMEM columns each, 64 columns apart
-template <typename T>
-__device__ __forceinline__ void mma_halves(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
-#pragma unroll
-    for (int k = 0; k < TILE / 16; ++k)
-        umma_f16_ts(d, a + (k / 4) * 64 + (k % 4) * 8, umma_desc(b + k * 2048, CHUNK_BYTES, 1024, kLayoutSW128), idesc,
-                    accumulate | (k > 0));
-}
-
-// D = A B anew for split operands: in each half's 64 TMEM columns 32 of hi, 32 of lo
-template <typename T>
-__device__ __forceinline__ void mma_halves_split(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
-    mma_cols_split<T>(d, b, idesc, [&](int part, int k) { return a + (k / 4) * 64 + part * 32 + (k % 4) * 8; });
 }
 
 // What the two gradient kernels share: barriers, TMEM, the documents of the block's rows.
@@ -478,11 +444,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             const uint32_t sk = smem_u32(smem + L::FIX), sv = sk + L::TILE_B;
             auto rows = [&](uint32_t d, uint32_t x, uint32_t y) {
                 if (SPLIT) mma_rows_split<T>(d, x, y, ksteps);
-                else mma_rows<T>(d, x, y, ksteps);
+                else mma_rows<T, DP / 16>(d, x, y, ksteps);
             };
             auto halves = [&](uint32_t d, uint32_t x, uint32_t y, bool more) {
-                if (SPLIT) mma_halves_split<T>(d, x, y, idesc);
-                else mma_halves<T>(d, x, y, idesc, more);
+                if (SPLIT) mma_halves_split(d, x, y, idesc);
+                else mma_halves(d, x, y, idesc, more);
             };
             // query rows of negative documents: 0 times what they hold could be NaN
             auto clean = [&](int s) {
@@ -499,7 +465,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 ok = warp_wait(&bb.full[0], 0, ok, g.err);
                 if (ok) clean(0);
                 const uint32_t sq = smem_u32(smem + L::RING);
-                if (ok && lane == 0) {
+                if (ok && elect_one()) {
                     rows(t_s, sk, sq);
                     umma_commit(&bb.s_full[0]);
                     rows(t_dp, sv, sq + L::TILE_B);
@@ -512,20 +478,20 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 const uint32_t sq = smem_u32(smem + L::RING + s * 2 * L::TILE_B);
                 const uint32_t sq1 = smem_u32(smem + L::RING + s1 * 2 * L::TILE_B);
                 ok = warp_wait(bb.p_full, n & 1, ok, g.err);
-                if (ok && lane == 0) halves(t_dv, t_s, sq + L::TILE_B, n > 0);
+                if (ok && elect_one()) halves(t_dv, t_s, sq + L::TILE_B, n > 0);
                 __syncwarp();
                 next();
                 if (qt >= 0) {
                     ok = warp_wait(&bb.full[s1], ((n + 1) / BW_STAGES) & 1, ok, g.err);
                     if (ok) clean(s1);
-                    if (ok && lane == 0) {
+                    if (ok && elect_one()) {
                         rows(t_s, sk, sq1);
                         umma_commit(&bb.s_full[0]);
                     }
                     __syncwarp();
                 }
                 ok = warp_wait(bb.dx_full, n & 1, ok, g.err);
-                if (ok && lane == 0) {
+                if (ok && elect_one()) {
                     halves(t_dk, t_dp, sq, n > 0);
                     umma_commit(&bb.empty[s]);
                     if (qt >= 0) {
@@ -546,7 +512,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const SplitExps ex = split_exps<SPLIT>(g, b, kvh);
         const float scale = SPLIT ? a.scale * exp2f((float)-(ex.q + ex.k)) : a.scale, c1 = scale * kLog2e;
-        const CapCoef cap = cap_coef<SPLIT>(scale, CAP ? a.cap : 1.f);
+        const CapCoef<SPLIT> cap(scale, CAP ? a.cap : 1.f);
         const float lift = dx_lift<T>(g, b, kvh), up = lift * PLift<T>::back;
         const float up_dp = SPLIT ? up * exp2f((float)-(ex.dout + ex.v)) : up;   // dp carries the powers of dout and v
         const int doc = kd && j < a.nk ? kd[j] : -1;
@@ -561,9 +527,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 bits0 = ~low_bits(from, 0);
                 bits1 = ~low_bits(from, 1);
                 if (qd) {
-                    const int other[4] = {i0 + lane < a.nq ? __ldg(qd + i0 + lane) : -1,
-                                          i0 + 32 + lane < a.nq ? __ldg(qd + i0 + 32 + lane) : -1, -1, -1};
-                    uint32_t same[4];
+                    const int other[2] = {i0 + lane < a.nq ? __ldg(qd + i0 + lane) : -1,
+                                          i0 + 32 + lane < a.nq ? __ldg(qd + i0 + 32 + lane) : -1};
+                    uint32_t same[2];
                     doc_bits(other, doc, same);
                     bits0 &= same[0];
                     bits1 &= same[1];
@@ -739,11 +705,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             const uint32_t sq = smem_u32(smem + L::FIX), sdo = sq + L::TILE_B;
             auto rows = [&](uint32_t d, uint32_t x, uint32_t y) {
                 if (SPLIT) mma_rows_split<T>(d, x, y, ksteps);
-                else mma_rows<T>(d, x, y, ksteps);
+                else mma_rows<T, DP / 16>(d, x, y, ksteps);
             };
             auto halves = [&](uint32_t d, uint32_t x, uint32_t y, bool more) {
-                if (SPLIT) mma_halves_split<T>(d, x, y, idesc);
-                else mma_halves<T>(d, x, y, idesc, more);
+                if (SPLIT) mma_halves_split(d, x, y, idesc);
+                else mma_halves(d, x, y, idesc, more);
             };
             // keys that must not count: 0 times what they hold could be NaN
             auto clean = [&](int s) {
@@ -761,7 +727,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 ok = warp_wait(&bb.full[0], 0, ok, g.err);
                 if (ok) clean(0);
                 const uint32_t sk = smem_u32(smem + L::RING);
-                if (ok && lane == 0) {
+                if (ok && elect_one()) {
                     rows(tmem, sq, sk);
                     umma_commit(&bb.s_full[0]);
                     rows(t_dp, sdo, sk + L::TILE_B);
@@ -778,14 +744,14 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                     ok = warp_wait(&bb.full[s1], ((n + 1) / BW_STAGES) & 1, ok, g.err);
                     if (ok) clean(s1);
                     // the scores before last have been read: their dx came before
-                    if (ok && lane == 0) {
+                    if (ok && elect_one()) {
                         rows(tmem + ((n + 1) & 1) * TILE, sq, sk1);
                         umma_commit(&bb.s_full[(n + 1) & 1]);
                     }
                     __syncwarp();
                 }
                 ok = warp_wait(bb.dx_full, n & 1, ok, g.err);
-                if (ok && lane == 0) {
+                if (ok && elect_one()) {
                     halves(t_dq, t_dp, sk, n > 0);
                     umma_commit(&bb.empty[s]);
                     if (kt >= 0) {
@@ -806,7 +772,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const SplitExps ex = split_exps<SPLIT>(g, b, kvh);
         const float scale = SPLIT ? a.scale * exp2f((float)-(ex.q + ex.k)) : a.scale, c1 = scale * kLog2e;
-        const CapCoef cap = cap_coef<SPLIT>(scale, CAP ? a.cap : 1.f);
+        const CapCoef<SPLIT> cap(scale, CAP ? a.cap : 1.f);
         const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
         const float lift = dx_lift<T>(g, b, kvh), up = lift * PLift<T>::back;
         const float up_dp = SPLIT ? up * exp2f((float)-(ex.dout + ex.v)) : up;   // dp carries the powers of dout and v
@@ -822,9 +788,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 bits0 = low_bits(limit - jw, 0);
                 bits1 = low_bits(limit - jw, 1);
                 if (kd) {
-                    const int other[4] = {jw + lane < a.nk ? __ldg(kd + jw + lane) : -1,
-                                          jw + 32 + lane < a.nk ? __ldg(kd + jw + 32 + lane) : -1, -1, -1};
-                    uint32_t same[4];
+                    const int other[2] = {jw + lane < a.nk ? __ldg(kd + jw + lane) : -1,
+                                          jw + 32 + lane < a.nk ? __ldg(kd + jw + 32 + lane) : -1};
+                    uint32_t same[2];
                     doc_bits(other, doc, same);
                     bits0 &= same[0];
                     bits1 &= same[1];
