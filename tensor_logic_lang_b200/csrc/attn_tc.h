@@ -194,37 +194,43 @@ __device__ __forceinline__ void mma_rows_split(uint32_t d, uint32_t a, uint32_t 
         for (int k = 0; k < ksteps; ++k) umma_f16_ss<true>(d, da + 2 * k, db + 2 * k, idesc);
     }
 }
-// D[128 x n] (+)= A B: A 128 x 128 16-bit in TMEM, in two halves of 64 columns
-// (32 TMEM columns each, 64 apart: each over the fp32 scores it comes from), B
-// the tile's 128 rows as contracted index.
-__device__ __forceinline__ void mma_halves(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+// D[128 x n] (+)= A B: A 128 x 128 16-bit in TMEM, in parts of W columns (W / 2
+// TMEM columns each, W apart: each over the fp32 scores it comes from), B the
+// tile's 128 rows as contracted index.
+template <int W>
+__device__ __forceinline__ constexpr uint32_t part_col(int k) { return (16 * k / W) * W + (16 * k % W) / 2; }
+template <int W>
+__device__ __forceinline__ void mma_parts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     const uint32_t db = desc_cols(b);
     umma_f16_ts(d, a, db, idesc, accumulate);
 #pragma unroll
-    for (int k = 1; k < TILE / 16; ++k) umma_f16_ts(d, a + (k / 4) * 64 + (k % 4) * 8, db + k * (2048 >> 4), idesc, 1);
+    for (int k = 1; k < TILE / 16; ++k) umma_f16_ts(d, a + part_col<W>(k), db + k * (2048 >> 4), idesc, 1);
 }
 // D = A B anew for split operands (the caller adds the tiles up in fp32): in
-// each half's 64 TMEM columns 32 of hi, 32 of lo.
-__device__ __forceinline__ void mma_halves_split(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+// each part's W TMEM columns W / 2 of hi, W / 2 of lo.
+template <int W>
+__device__ __forceinline__ void mma_parts_split(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
     const uint32_t db = desc_cols(b);
 #pragma unroll
     for (int part = 0; part < 3; ++part)
 #pragma unroll
         for (int k = 0; k < TILE / 16; ++k)
-            umma_f16_ts(d, a + (k / 4) * 64 + (part == 0 ? 32 : 0) + (k % 4) * 8,
-                        db + (part == 1 ? CHUNK_BYTES >> 4 : 0) + k * (2048 >> 4), idesc, part > 0 || k > 0);
+            umma_f16_ts(d, a + part_col<W>(k) + (part == 0 ? W / 2 : 0), db + (part == 1 ? CHUNK_BYTES >> 4 : 0) + k * (2048 >> 4), idesc,
+                        part > 0 || k > 0);
 }
-// 64 columns of the warp's lanes
-__device__ __forceinline__ void load64(uint32_t taddr, uint32_t (&raw)[64]) {
-    tmem_ld32(taddr, raw);
-    tmem_ld32(taddr + 32, raw + 32);
+// N columns of the warp's lanes
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&raw)[N]) {
+#pragma unroll
+    for (int k = 0; k < N / 32; ++k) tmem_ld32(taddr + 32 * k, raw + 32 * k);
     tmem_wait_ld();
 }
-__device__ __forceinline__ void load64(uint32_t taddr, f2 (&x)[32]) {
-    uint32_t raw[64];
-    load64(taddr, raw);
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, f2 (&x)[N]) {
+    uint32_t raw[2 * N];
+    tmem_load(taddr, raw);
 #pragma unroll
-    for (int k = 0; k < 32; ++k) x[k] = pack2(__uint_as_float(raw[2 * k]), __uint_as_float(raw[2 * k + 1]));
+    for (int k = 0; k < N; ++k) x[k] = pack2(__uint_as_float(raw[2 * k]), __uint_as_float(raw[2 * k + 1]));
 }
 // hi and lo of a pair of values as fp16 pairs
 __device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t& lo) {
@@ -236,15 +242,15 @@ __device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t
 template <int N>
 __device__ __forceinline__ void tmem_add(uint32_t acc, uint32_t from, bool fresh) {
 #pragma unroll 1
-    for (int k = 0; k < N; k += 32) {
-        uint32_t x[32], y[32];
-        tmem_ld32(from + k, x);
-        if (!fresh) tmem_ld32(acc + k, y);
+    for (int k = 0; k < N; k += 16) {
+        uint32_t x[16], y[16];
+        tmem_ld16(from + k, x);
+        if (!fresh) tmem_ld16(acc + k, y);
         tmem_wait_ld();
         if (!fresh)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) + __uint_as_float(y[i]));
-        tmem_st32(acc + k, x);
+            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) + __uint_as_float(y[i]));
+        tmem_st16(acc + k, x);
     }
 }
 
@@ -256,17 +262,17 @@ __device__ __forceinline__ void store_row(const HeadsView& v, int b, int h, int6
                                           bool live, float mul) {
     U* p = static_cast<U*>(v.p) + b * v.sb + h * v.sh + row * v.ss;
     const bool wide = std::is_same<U, float>::value && v.sd == 1 && d % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
-    for (int k = 0; k < DP / 32; ++k) {
-        uint32_t o[32];
+    for (int k = 0; k < DP / 16; ++k) {
+        uint32_t o[16];
         if (live) {
-            tmem_ld32(taddr + 32 * k, o);
+            tmem_ld16(taddr + 16 * k, o);
             tmem_wait_ld();
         }
         if (!on) continue;
         if constexpr (std::is_same<U, float>::value) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const int c = 32 * k + 4 * q;
+            for (int q = 0; q < 4; ++q) {
+                const int c = 16 * k + 4 * q;
                 if (c >= d) break;
                 float w[4];
 #pragma unroll
@@ -281,13 +287,13 @@ __device__ __forceinline__ void store_row(const HeadsView& v, int b, int h, int6
             }
         } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                if (32 * k + 8 * q >= d) break;
+            for (int q = 0; q < 2; ++q) {
+                if (16 * k + 8 * q >= d) break;
                 uint32_t w[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     w[e] = any ? pack16<U>(__uint_as_float(o[8 * q + 2 * e]) * mul, __uint_as_float(o[8 * q + 2 * e + 1]) * mul) : 0u;
-                *reinterpret_cast<uint4*>(p + 32 * k + 8 * q) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(p + 16 * k + 8 * q) = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
     }
@@ -436,18 +442,20 @@ struct TileWalk {
     }
 };
 
-// Bits of the 64 other positions whose document is `doc`, lane by lane: the
-// lane holds the documents of positions lane and 32 + lane in other[2] and
-// wants its own row's doc.  The distinct documents of a warp's rows are few
-// (two ballots each).
-__device__ __forceinline__ void doc_bits(const int (&other)[2], int doc, uint32_t (&bits)[2]) {
+// Bits of 32 W other positions whose document is `doc`, lane by lane: the lane
+// holds the documents of positions lane, 32 + lane, ... in other[W] and wants
+// its own row's doc.  The distinct documents of a warp's rows are few (W
+// ballots each).
+template <int W>
+__device__ __forceinline__ void doc_bits(const int (&other)[W], int doc, uint32_t (&bits)[W]) {
     uint32_t left = 0xffffffffu;
-    bits[0] = bits[1] = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) bits[w] = 0;
     while (left) {
         const int d = __shfl_sync(0xffffffffu, doc, __ffs(left) - 1);
         const bool mine = doc == d;
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
+        for (int w = 0; w < W; ++w) {
             const uint32_t m = __ballot_sync(0xffffffffu, other[w] == d && d >= 0);
             if (mine) bits[w] = m;
         }

@@ -293,8 +293,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                     tc_fence_after();
                     if (ok && elect_one()) {
                         const uint32_t to = tmem + 2 * TILE + t * DO, sv = smem_u32(smem + L::KV + vs * L::TILE_B);
-                        if (SPLIT) mma_halves_split(to, tmem + t * TILE, sv, idesc_o);
-                        else mma_halves(to, tmem + t * TILE, sv, idesc_o, it > 0);
+                        if (SPLIT) mma_parts_split<64>(to, tmem + t * TILE, sv, idesc_o);
+                        else mma_parts<64>(to, tmem + t * TILE, sv, idesc_o, it > 0);
                         if (next < 0) umma_commit(&o_done[t]);
                     }
                     __syncwarp();
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             tc_fence_after();
             if (SPLIT && it > 0) tmem_add<DH>(acc, to, it == 1);   // P V of the tile before, done before this S
             f2 x[32];
-            load64(ts, x);
+            tmem_load(ts, x);
             float top = c * score_row<CAP, BIAS, SPLIT, FIX>(x, c1, cap, shift, slope2, p, j0, masked, bits0, bits1);
             if (!FIX) {
                 // the row's other half

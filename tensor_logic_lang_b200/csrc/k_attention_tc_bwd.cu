@@ -16,9 +16,9 @@
 //
 // Seven products where one kernel for all three would need five, but no
 // atomics on dq: the results do not depend on the order of the blocks, and
-// there is no fp32 copy of dq in memory.  Two warpgroups take 64 columns of
+// there is no fp32 copy of dq in memory.  Four warpgroups take 32 columns of
 // the 128 x 128 scores each; P (dx) goes back to TMEM as a 16-bit operand over
-// the half of S (dp) its warpgroup has read.  While the exponentials of one
+// the part of S (dp) its warpgroup has read.  While the exponentials of one
 // tile run, the products of the tile before and the scores of the next do.
 //
 // 16-bit roundings: p and dx as operands of the last products (tensor cores
@@ -36,7 +36,9 @@
 namespace tl {
 namespace {
 
-constexpr int BW_THREADS = 384, BW_STAGES = 2;
+constexpr int BW_COMPUTE = 512, BW_THREADS = BW_COMPUTE + 64, BW_STAGES = 2;
+constexpr int BW_MMA = BW_COMPUTE / 32, BW_TMA = BW_MMA + 1;   // warps
+constexpr int BW_COLS = 32;   // scores of a thread
 constexpr int STAT_BYTES = 2 * TILE * 4;   // of a query tile: -log2(e) lse (+ lift), -D
 
 template <typename T> struct PLift { static constexpr float log2 = 0.f, back = 1.f; };
@@ -198,50 +200,49 @@ __device__ __forceinline__ float dx_lift(const BwArgs& g, int b, int kvh) {
 }
 
 // ---------------------------------------------------------------- elements
-// 64 scores q.k of a row -> p in base 2 (16-bit pairs) and p (1 - tanh^2).
+// 32 scores q.k of a row -> p in base 2 (16-bit pairs) and p (1 - tanh^2).
 // off: position of column 0 relative to the row's (|off + c| is the distance);
 // nl(i): minus log2(e) lse of the columns 2i, 2i + 1.
 // SPLIT: p16 and low take hi and lo, and the tanh is good to fp32.
 template <typename T, bool CAP, bool BIAS, bool SPLIT, typename NL>
-__device__ __forceinline__ void grad_row(f2 (&x)[32], uint32_t (&p16)[32], uint32_t (&low)[32], float c1, const CapCoef<SPLIT>& cap, float slope2, int off,
-                                         bool masked, uint32_t bits0, uint32_t bits1, NL nl) {
-    f2 bend[CAP ? 32 : 1];
+__device__ __forceinline__ void grad_row(f2 (&x)[16], uint32_t (&p16)[16], uint32_t (&low)[16], float c1, const CapCoef<SPLIT>& cap, float slope2, int off,
+                                         bool masked, uint32_t bits, NL nl) {
+    f2 bend[CAP ? 16 : 1];
     if (CAP) {
         if (__any_sync(0xffffffffu, !(largest(x) <= cap.limit))) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = wide_score<SPLIT>(x[i], cap);
+            for (int i = 0; i < 16; ++i) x[i] = wide_score<SPLIT>(x[i], cap);
         } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = mul2(x[i], cap.ratio(x[i]));
+            for (int i = 0; i < 16; ++i) x[i] = mul2(x[i], cap.ratio(x[i]));
         }
         // 1 - tanh^2, the tanh from the score
         const float inv = -1.f / (cap.top * cap.top);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) bend[i] = fma2(mul2(x[i], pack2(inv, inv)), x[i], pack2(1.f, 1.f));
+        for (int i = 0; i < 16; ++i) bend[i] = fma2(mul2(x[i], pack2(inv, inv)), x[i], pack2(1.f, 1.f));
     }
     const f2 c = CAP ? pack2(1.f, 1.f) : pack2(c1, c1);
     if (BIAS) {
-        const bool after = __all_sync(0xffffffffu, off >= 0), before = __all_sync(0xffffffffu, off + 63 <= 0);
+        const bool after = __all_sync(0xffffffffu, off >= 0), before = __all_sync(0xffffffffu, off + 31 <= 0);
         if (after || before) {
             const float k = after ? -slope2 : slope2, kb = k * (float)off;
             const f2 kk = pack2(k, k), base = pack2(kb, kb);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = fma2(x[i], c, fma2(kk, pack2((float)(2 * i), (float)(2 * i + 1)), base));
+            for (int i = 0; i < 16; ++i) x[i] = fma2(x[i], c, fma2(kk, pack2((float)(2 * i), (float)(2 * i + 1)), base));
         } else {
             const float at = (float)off;
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
+            for (int i = 0; i < 16; ++i)
                 x[i] = fma2(x[i], c, pack2(-slope2 * fabsf(at + (float)(2 * i)), -slope2 * fabsf(at + (float)(2 * i + 1))));
         }
     }
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < 16; ++i) {
         float lo, hi;
         unpack2(CAP || BIAS ? add2(x[i], nl(i)) : fma2(x[i], c, nl(i)), lo, hi);
         if (masked) {
-            const uint32_t w = i < 16 ? bits0 : bits1;
-            lo = (w >> (2 * i % 32)) & 1 ? lo : -INFINITY;
-            hi = (w >> (2 * i % 32 + 1)) & 1 ? hi : -INFINITY;
+            lo = (bits >> (2 * i)) & 1 ? lo : -INFINITY;
+            hi = (bits >> (2 * i + 1)) & 1 ? hi : -INFINITY;
         }
         lo = ex2(lo);
         hi = ex2(hi);
@@ -254,19 +255,18 @@ __device__ __forceinline__ void grad_row(f2 (&x)[32], uint32_t (&p16)[32], uint3
 
 // dx = pb (dp - D), zero where the key is not seen (there dp may be anything)
 template <typename T, bool SPLIT, typename ND>
-__device__ __forceinline__ void grad_dx(const f2 (&pb)[32], const uint32_t (&dp)[64], uint32_t (&out)[32], uint32_t (&low)[32],
+__device__ __forceinline__ void grad_dx(const f2 (&pb)[16], const uint32_t (&dp)[32], uint32_t (&out)[16], uint32_t (&low)[16],
                                         float lift, bool masked,
-                                        uint32_t bits0, uint32_t bits1, ND nd) {
+                                        uint32_t bits, ND nd) {
     const f2 up = pack2(lift, lift);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < 16; ++i) {
         const f2 d2 = pack2(__uint_as_float(dp[2 * i]), __uint_as_float(dp[2 * i + 1]));
         float lo, hi;
         unpack2(mul2(pb[i], PLift<T>::log2 == 0.f ? add2(d2, nd(i)) : fma2(d2, up, nd(i))), lo, hi);
         if (masked) {
-            const uint32_t w = i < 16 ? bits0 : bits1;
-            lo = (w >> (2 * i % 32)) & 1 ? lo : 0.f;
-            hi = (w >> (2 * i % 32 + 1)) & 1 ? hi : 0.f;
+            lo = (bits >> (2 * i)) & 1 ? lo : 0.f;
+            hi = (bits >> (2 * i + 1)) & 1 ? hi : 0.f;
         }
         if (SPLIT) split16(lo, hi, out[i], low[i]);
         else out[i] = pack16<T>(lo, hi);
@@ -298,11 +298,11 @@ struct BwBlock {
             mbar_init(fix, 1);
             for (int s = 0; s < BW_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
             mbar_init(&s_full[0], 1); mbar_init(&s_full[1], 1);
-            mbar_init(p_full, 2 * TILE); mbar_init(dp_full, 1); mbar_init(dx_full, 2 * TILE); mbar_init(done, 1);
+            mbar_init(p_full, BW_COMPUTE); mbar_init(dp_full, 1); mbar_init(dx_full, BW_COMPUTE); mbar_init(done, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             docs[0] = 0x7fffffff; docs[1] = -1; docs[2] = 0;
         }
-        if (warp == 8) {
+        if (warp == BW_MMA) {
             asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         }
@@ -328,7 +328,7 @@ struct BwBlock {
     __device__ __forceinline__ void finish(uint32_t tmem) {
         tc_fence_before();
         __syncthreads();
-        if (threadIdx.x / 32 == 8) {
+        if (threadIdx.x / 32 == BW_MMA) {
             tc_fence_after();
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
         }
@@ -409,9 +409,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     next();
     const bool any = qt >= 0;   // the same for every head
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 9) {
+    if (warp >= BW_MMA) {
+        if (warp == BW_TMA) {
             // ------------------------------------------------ TMA
             if (any && lane == 0) {
                 mbar_expect_tx(bb.fix, 2 * L::TILE_B);
@@ -437,7 +436,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             if (!ok)   // copies in flight land before the block ends
                 for (int e = max(0, n - 1 - BW_STAGES); e < n - 1; ++e)
                     mbar_wait(&bb.full[e % BW_STAGES], (e / BW_STAGES) & 1, g.err);
-        } else if (warp == 8) {
+        } else {
             // ------------------------------------------------ tensor cores
             const int ksteps = (a.d + 15) / 16;
             const uint32_t idesc = f16_idesc<T>(16 * ksteps, true);
@@ -446,9 +445,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 if (SPLIT) mma_rows_split<T>(d, x, y, ksteps);
                 else mma_rows<T, DP / 16>(d, x, y, ksteps);
             };
-            auto halves = [&](uint32_t d, uint32_t x, uint32_t y, bool more) {
-                if (SPLIT) mma_halves_split(d, x, y, idesc);
-                else mma_halves(d, x, y, idesc, more);
+            auto parts = [&](uint32_t d, uint32_t x, uint32_t y, bool more) {
+                if (SPLIT) mma_parts_split<BW_COLS>(d, x, y, idesc);
+                else mma_parts<BW_COLS>(d, x, y, idesc, more);
             };
             // query rows of negative documents: 0 times what they hold could be NaN
             auto clean = [&](int s) {
@@ -478,7 +477,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 const uint32_t sq = smem_u32(smem + L::RING + s * 2 * L::TILE_B);
                 const uint32_t sq1 = smem_u32(smem + L::RING + s1 * 2 * L::TILE_B);
                 ok = warp_wait(bb.p_full, n & 1, ok, g.err);
-                if (ok && elect_one()) halves(t_dv, t_s, sq + L::TILE_B, n > 0);
+                if (ok && elect_one()) parts(t_dv, t_s, sq + L::TILE_B, n > 0);
                 __syncwarp();
                 next();
                 if (qt >= 0) {
@@ -492,7 +491,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 }
                 ok = warp_wait(bb.dx_full, n & 1, ok, g.err);
                 if (ok && elect_one()) {
-                    halves(t_dk, t_dp, sq, n > 0);
+                    parts(t_dk, t_dp, sq, n > 0);
                     umma_commit(&bb.empty[s]);
                     if (qt >= 0) {
                         rows(t_dp, sv, sq1 + L::TILE_B);
@@ -506,9 +505,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             }
         }
     } else {
-        // ---------------------------------------------------- a key per thread, 64 queries
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        // ---------------------------------------------------- 32 queries of a key per thread
         const int wg = warp / 4, r = threadIdx.x % TILE, j = j0 + r;
+        // at the end: dv (dk) and half of its columns
+        constexpr int DH = DO / 2;
+        const int which = wg / 2, col0 = wg % 2 * DH;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const SplitExps ex = split_exps<SPLIT>(g, b, kvh);
         const float scale = SPLIT ? a.scale * exp2f((float)-(ex.q + ex.k)) : a.scale, c1 = scale * kLog2e;
@@ -518,38 +519,35 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         const int doc = kd && j < a.nk ? kd[j] : -1;
         int n = 0;
         for (; qt >= 0 && ok; next(), ++n) {
-            const int i0 = qt * TILE + wg * 64;
-            uint32_t bits0 = 0xffffffffu, bits1 = 0xffffffffu;
+            const int i0 = qt * TILE + wg * BW_COLS;
+            uint32_t bits = 0xffffffffu;
             if (masked) {
                 // queries from `from` on see the key
                 int from = mask.causal && j >= mask.prefix ? j - mask.p0 - i0 : 0;
-                if (j >= mask.kv) from = 64;
-                bits0 = ~low_bits(from, 0);
-                bits1 = ~low_bits(from, 1);
+                if (j >= mask.kv) from = BW_COLS;
+                bits = ~low_bits(from, 0);
                 if (qd) {
-                    const int other[2] = {i0 + lane < a.nq ? __ldg(qd + i0 + lane) : -1,
-                                          i0 + 32 + lane < a.nq ? __ldg(qd + i0 + 32 + lane) : -1};
-                    uint32_t same[2];
+                    const int other[1] = {i0 + lane < a.nq ? __ldg(qd + i0 + lane) : -1};
+                    uint32_t same[1];
                     doc_bits(other, doc, same);
-                    bits0 &= same[0];
-                    bits1 &= same[1];
+                    bits &= same[0];
                 }
             }
             const float slope2 = BIAS ? __ldg(a.slopes + h) * kLog2e : 0.f;
-            const float* st = reinterpret_cast<const float*>(smem + L::STAT + (n % BW_STAGES) * STAT_BYTES) + wg * 64;
+            const float* st = reinterpret_cast<const float*>(smem + L::STAT + (n % BW_STAGES) * STAT_BYTES) + wg * BW_COLS;
             ok = warp_wait(&bb.full[n % BW_STAGES], (n / BW_STAGES) & 1, ok, g.err);   // the statistics
             ok = warp_wait(&bb.s_full[0], n & 1, ok, g.err);
             if (!ok) break;
-            f2 x[32];
+            f2 x[16];
             {
                 // dv of the tile before, done before this S
-                if (SPLIT && wg == 0 && n > 0) tmem_add<DO>(t_dva + lanes, t_dv + lanes, n == 1);
-                load64(t_s + lanes + wg * 64, x);
-                uint32_t p16[32], low[32];
-                grad_row<T, CAP, BIAS, SPLIT>(x, p16, low, c1, cap, slope2, mask.p0 + i0 - j, masked, bits0, bits1,
+                if (SPLIT && which == 0 && n > 0) tmem_add<DH>(t_dva + lanes + col0, t_dv + lanes + col0, n == 1);
+                tmem_load(t_s + lanes + wg * BW_COLS, x);
+                uint32_t p16[16], low[16];
+                grad_row<T, CAP, BIAS, SPLIT>(x, p16, low, c1, cap, slope2, mask.p0 + i0 - j, masked, bits,
                                        [&](int i) { return *reinterpret_cast<const f2*>(st + 2 * i); });
-                tmem_st32(t_s + lanes + wg * 64, p16);
-                if (SPLIT) tmem_st32(t_s + lanes + wg * 64 + 32, low);
+                tmem_st16(t_s + lanes + wg * BW_COLS, p16);
+                if (SPLIT) tmem_st16(t_s + lanes + wg * BW_COLS + 16, low);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -558,44 +556,46 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             if (!ok) break;
             {
                 // dk of the tile before, done before this dp
-                if (SPLIT && wg == 1 && n > 0) tmem_add<DO>(t_dka + lanes, t_dk + lanes, n == 1);
-                uint32_t dp[64], dx[32], low[32];
-                load64(t_dp + lanes + wg * 64, dp);
+                if (SPLIT && which == 1 && n > 0) tmem_add<DH>(t_dka + lanes + col0, t_dk + lanes + col0, n == 1);
+                uint32_t dp[32], dx[16], low[16];
+                tmem_load(t_dp + lanes + wg * BW_COLS, dp);
                 const f2 up2 = pack2(up, up);
-                grad_dx<T, SPLIT>(x, dp, dx, low, up_dp, masked, bits0, bits1, [&](int i) {
+                grad_dx<T, SPLIT>(x, dp, dx, low, up_dp, masked, bits, [&](int i) {
                     const f2 d = *reinterpret_cast<const f2*>(st + TILE + 2 * i);
                     return PLift<T>::log2 == 0.f ? d : mul2(d, up2);
                 });
-                tmem_st32(t_dp + lanes + wg * 64, dx);
-                if (SPLIT) tmem_st32(t_dp + lanes + wg * 64 + 32, low);
+                tmem_st16(t_dp + lanes + wg * BW_COLS, dx);
+                if (SPLIT) tmem_st16(t_dp + lanes + wg * BW_COLS + 16, low);
             }
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(bb.dx_full);
         }
         if (any) ok = warp_wait(bb.done, 0, ok, g.err);
-        uint32_t mine_at = (wg ? t_dk : t_dv) + lanes;
-        float mul = wg ? a.scale / lift : PLift<T>::back;
+        uint32_t mine_at = (which ? t_dk : t_dv) + lanes + col0;
+        float mul = which ? a.scale / lift : PLift<T>::back;
         if (SPLIT) {
-            const uint32_t acc = (wg ? t_dka : t_dva) + lanes;
+            const uint32_t acc = (which ? t_dka : t_dva) + lanes + col0;
             if (any && ok) {
-                tmem_add<DO>(acc, mine_at, n == 1);
+                tmem_add<DH>(acc, mine_at, n == 1);
                 tmem_wait_st();
             }
             mine_at = acc;
-            mul *= exp2f((float)-(wg ? ex.q : ex.dout));
+            mul *= exp2f((float)-(which ? ex.q : ex.dout));
         }
         if (g.cluster == 1) {
-            if (ok) store_row<U, DO>(wg ? a.dk : a.dv, b, kvh, j, j < a.nk, a.d, mine_at, any, any, mul);
+            HeadsView v = which ? a.dk : a.dv;
+            v.p = static_cast<U*>(v.p) + col0 * v.sd;
+            if (ok) store_row<U, DH>(v, b, kvh, j, j < a.nk, a.d - col0, mine_at, any, any, mul);
         } else if (any && ok) {
-            float* row = reinterpret_cast<float*>(smem) + (wg * TILE + r) * L::SUM_LD;
-            for (int k = 0; k < DO / 32; ++k) {
-                uint32_t o[32];
-                tmem_ld32(mine_at + 32 * k, o);
+            float* row = reinterpret_cast<float*>(smem) + (which * TILE + r) * L::SUM_LD + col0;
+            for (int k = 0; k < DH / 16; ++k) {
+                uint32_t o[16];
+                tmem_ld16(mine_at + 16 * k, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    *reinterpret_cast<float4*>(row + 32 * k + 4 * q) =
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<float4*>(row + 16 * k + 4 * q) =
                         make_float4(__uint_as_float(o[4 * q]) * mul, __uint_as_float(o[4 * q + 1]) * mul,
                                     __uint_as_float(o[4 * q + 2]) * mul, __uint_as_float(o[4 * q + 3]) * mul);
             }
@@ -605,11 +605,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     if (g.cluster > 1) {
         // each block adds its share of the rows over the cluster, in the order of the heads
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-        if (warp < 8) {
+        if (warp < BW_MMA) {
             const int share = TILE / g.cluster, r0 = rank * share;
             const uint32_t sums = smem_u32(smem);
             constexpr int V = DO / 4;
-            for (int e = threadIdx.x; e < 2 * share * V; e += 2 * TILE) {
+            for (int e = threadIdx.x; e < 2 * share * V; e += BW_COMPUTE) {
                 const int c = e % V, r = r0 + e / V % share, wg = e / V / share;
                 if (j0 + r >= a.nk || 4 * c >= a.d) continue;
                 float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -675,9 +675,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     int kt = walk.next(&masked);
     const bool any = kt >= 0;
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 9) {
+    if (warp >= BW_MMA) {
+        if (warp == BW_TMA) {
             // ------------------------------------------------ TMA
             if (any && lane == 0) {
                 mbar_expect_tx(bb.fix, 2 * L::TILE_B);
@@ -698,7 +697,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             if (!ok)
                 for (int e = max(0, n - 1 - BW_STAGES); e < n - 1; ++e)
                     mbar_wait(&bb.full[e % BW_STAGES], (e / BW_STAGES) & 1, g.err);
-        } else if (warp == 8) {
+        } else {
             // ------------------------------------------------ tensor cores
             const int ksteps = (a.d + 15) / 16;
             const uint32_t idesc = f16_idesc<T>(16 * ksteps, true);
@@ -707,9 +706,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 if (SPLIT) mma_rows_split<T>(d, x, y, ksteps);
                 else mma_rows<T, DP / 16>(d, x, y, ksteps);
             };
-            auto halves = [&](uint32_t d, uint32_t x, uint32_t y, bool more) {
-                if (SPLIT) mma_halves_split(d, x, y, idesc);
-                else mma_halves(d, x, y, idesc, more);
+            auto parts = [&](uint32_t d, uint32_t x, uint32_t y, bool more) {
+                if (SPLIT) mma_parts_split<BW_COLS>(d, x, y, idesc);
+                else mma_parts<BW_COLS>(d, x, y, idesc, more);
             };
             // keys that must not count: 0 times what they hold could be NaN
             auto clean = [&](int s) {
@@ -752,7 +751,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 }
                 ok = warp_wait(bb.dx_full, n & 1, ok, g.err);
                 if (ok && elect_one()) {
-                    halves(t_dq, t_dp, sk, n > 0);
+                    parts(t_dq, t_dp, sk, n > 0);
                     umma_commit(&bb.empty[s]);
                     if (kt >= 0) {
                         rows(t_dp, sdo, sk1 + L::TILE_B);
@@ -766,8 +765,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             }
         }
     } else {
-        // ---------------------------------------------------- a query per thread, 64 keys
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        // ---------------------------------------------------- 32 keys of a query per thread
         const int wg = warp / 4, r = threadIdx.x % TILE, i = i0 + r;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const SplitExps ex = split_exps<SPLIT>(g, b, kvh);
@@ -782,61 +780,58 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         const int doc = qd && i < a.nq ? qd[i] : -1, limit = mask.key_end(i, 1);
         int n = 0;
         for (; kt >= 0 && ok; kt = walk.next(&masked), ++n) {
-            const int jw = kt * TILE + wg * 64;
-            uint32_t bits0 = 0xffffffffu, bits1 = 0xffffffffu;
+            const int jw = kt * TILE + wg * BW_COLS;
+            uint32_t bits = 0xffffffffu;
             if (masked) {
-                bits0 = low_bits(limit - jw, 0);
-                bits1 = low_bits(limit - jw, 1);
+                bits = low_bits(limit - jw, 0);
                 if (kd) {
-                    const int other[2] = {jw + lane < a.nk ? __ldg(kd + jw + lane) : -1,
-                                          jw + 32 + lane < a.nk ? __ldg(kd + jw + 32 + lane) : -1};
-                    uint32_t same[2];
+                    const int other[1] = {jw + lane < a.nk ? __ldg(kd + jw + lane) : -1};
+                    uint32_t same[1];
                     doc_bits(other, doc, same);
-                    bits0 &= same[0];
-                    bits1 &= same[1];
+                    bits &= same[0];
                 }
             }
             ok = warp_wait(&bb.s_full[n & 1], (n / 2) & 1, ok, g.err);
             if (!ok) break;
-            f2 x[32];
-            load64(tmem + (n & 1) * TILE + lanes + wg * 64, x);
+            f2 x[16];
+            tmem_load(tmem + (n & 1) * TILE + lanes + wg * BW_COLS, x);
             {
-                uint32_t unused[32], low[32];
-                grad_row<T, CAP, BIAS, SPLIT>(x, unused, low, c1, cap, slope2, jw - (mask.p0 + i), masked, bits0, bits1,
+                uint32_t unused[16], low[16];
+                grad_row<T, CAP, BIAS, SPLIT>(x, unused, low, c1, cap, slope2, jw - (mask.p0 + i), masked, bits,
                                        [&](int) { return nl2; });
             }
             ok = warp_wait(bb.dp_full, n & 1, ok, g.err);
             if (!ok) break;
             {
-                // dq of the tile before, done before this dp: 32 columns a warpgroup
-                if (SPLIT && n > 0) tmem_add<DO / 2>(t_dqa + lanes + wg * (DO / 2), t_dq + lanes + wg * (DO / 2), n == 1);
-                uint32_t dp[64], dx[32], low[32];
-                load64(t_dp + lanes + wg * 64, dp);
-                grad_dx<T, SPLIT>(x, dp, dx, low, up_dp, masked, bits0, bits1, [&](int) { return nd2; });
-                tmem_st32(t_dp + lanes + wg * 64, dx);
-                if (SPLIT) tmem_st32(t_dp + lanes + wg * 64 + 32, low);
+                // dq of the tile before, done before this dp
+                if (SPLIT && n > 0) tmem_add<DO / 4>(t_dqa + lanes + wg * (DO / 4), t_dq + lanes + wg * (DO / 4), n == 1);
+                uint32_t dp[32], dx[16], low[16];
+                tmem_load(t_dp + lanes + wg * BW_COLS, dp);
+                grad_dx<T, SPLIT>(x, dp, dx, low, up_dp, masked, bits, [&](int) { return nd2; });
+                tmem_st16(t_dp + lanes + wg * BW_COLS, dx);
+                if (SPLIT) tmem_st16(t_dp + lanes + wg * BW_COLS + 16, low);
             }
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(bb.dx_full);
         }
         if (any) ok = warp_wait(bb.done, 0, ok, g.err);
-        // each warpgroup writes half of the columns
+        // each warpgroup writes a quarter of the columns
         if (ok) {
-            constexpr int HALF = DO / 2;
-            uint32_t at = t_dq + lanes + wg * HALF;
+            constexpr int PART = DO / 4;
+            uint32_t at = t_dq + lanes + wg * PART;
             float mul = a.scale / lift;
             if (SPLIT) {
                 if (any) {
-                    tmem_add<HALF>(t_dqa + lanes + wg * HALF, at, n == 1);
+                    tmem_add<PART>(t_dqa + lanes + wg * PART, at, n == 1);
                     tmem_wait_st();
                 }
-                at = t_dqa + lanes + wg * HALF;
+                at = t_dqa + lanes + wg * PART;
                 mul *= exp2f((float)-ex.k);
             }
             HeadsView v = a.dq;
-            v.p = static_cast<U*>(v.p) + wg * HALF * v.sd;
-            store_row<U, HALF>(v, b, h, i, i < a.nq, a.d - wg * HALF, at, any, any, mul);
+            v.p = static_cast<U*>(v.p) + wg * PART * v.sd;
+            store_row<U, PART>(v, b, h, i, i < a.nq, a.d - wg * PART, at, any, any, mul);
         }
     }
     bb.finish(tmem);
