@@ -92,6 +92,23 @@ cudaError_t launch_early(void (*kernel)(P...), unsigned grid, int threads, int s
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// A launch in clusters of `cluster` blocks along x.
+template <typename... P, typename... A>
+cudaError_t launch_cluster(void (*kernel)(P...), unsigned grid, int cluster, int threads, int smem, cudaStream_t s, const A&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 inline size_t type_size(int dtype) { return dtype == TL_TYPE_F32 ? 4 : 2; }
 
 // algorithmic work of a call for the profile: every pair of a query and a key

@@ -3,17 +3,19 @@
 //
 // The queries of a group's heads that read one key head are the rows of a
 // unit (16 or 32 of them; more rows make more units).  A unit's keys are cut
-// into tiles of 64, the tiles of all units form one line, and each block takes
+// into tiles (of 64, or 128 of head sizes up to 64), the tiles of all units form one line, and each block takes
 // an equal piece of it, whatever the sequences' lengths: all blocks run at
 // once and end together.  A piece that covers a unit whole writes its output;
 // the pieces of a unit that lies over several blocks leave their sums,
 // maxima and unnormalised outputs in the workspace (at most two a block), and
-// k_decode_join adds them in the order of the keys.
+// k_decode_join adds them in the order of the keys.  Where a call has few units
+// and short caches, a cluster of 8 blocks shares each unit instead and joins its
+// pieces through distributed shared memory: one launch, no line to divide.
 //
 //   k_decode_mma   16-bit types with aligned rows and head sizes up to 128: TMA
 //                  tiles (128-byte swizzle) through a ring; each of four
-//                  warps takes 16 keys of a tile for all rows (two sets of
-//                  four take the tiles in turn), with mma.sync.m16n8k16 (at a few rows a key the tensor work is a
+//                  warps takes a quarter of a tile's keys for all rows (two
+//                  sets of four take the tiles in turn), with mma.sync.m16n8k16 (at a few rows a key the tensor work is a
 //                  fraction of the time the key's bytes take)
 //   k_decode_any   any type, stride and head size: tiles as fp32 in shared
 //                  memory, FFMA
@@ -24,12 +26,13 @@
 namespace tl {
 namespace {
 
-constexpr int DT = 64;                // keys of a tile
 constexpr int JOIN_THREADS = 128;
 
 struct DecArgs {
     AttnCall a;
-    int rows;          // of a unit: 16 or 32
+    int tile;          // keys of a tile
+    int cluster;       // blocks that share a unit, or 1: the blocks share the line
+    int rows;          // of a unit
     int row_blocks;    // units of a key head
     int blocks;        // of the kernel that reads the cache
     const int2* spans; // [b] with documents: the first and one past the last key that may be seen
@@ -46,7 +49,7 @@ __device__ __forceinline__ int2 seq_tiles(const DecArgs& g, int b) {
         end = min(s.y, end);
     }
     if (end <= begin) return make_int2(0, 0);
-    return make_int2(begin / DT, (end + DT - 1) / DT);
+    return make_int2(begin / g.tile, (end + g.tile - 1) / g.tile);
 }
 
 // Sum over the block; every thread gets it.  NW warps, red[NW] words.
@@ -167,6 +170,19 @@ struct PieceWalk {
     int64_t left;      // tiles left for this block
     bool first;
     __device__ __forceinline__ bool next(const DecArgs& g, Piece* p) {
+        if (g.cluster > 1) {   // the block's share of its cluster's unit, which may be empty
+            if (!first) return false;
+            first = false;
+            const int unit = blockIdx.x / g.cluster, rank = blockIdx.x % g.cluster, n = at.span.y - at.span.x;
+            p->b = at.b;
+            p->kvh = unit / g.row_blocks % g.a.hkv;
+            p->rb = unit % g.row_blocks;
+            p->t0 = at.span.x + n * rank / g.cluster;
+            p->t1 = at.span.x + n * (rank + 1) / g.cluster;
+            p->whole = false;
+            p->slot = 0;
+            return true;
+        }
         if (left <= 0) return false;
         const int units = g.a.hkv * g.row_blocks;
         while (at.tile >= at.span.y || at.span.x >= at.span.y) {   // the next unit with tiles
@@ -198,7 +214,12 @@ template <int NW>
 __device__ __forceinline__ PieceWalk block_pieces(const DecArgs& g, int64_t* red, int64_t* found) {
     PieceWalk w;
     w.first = true;
-    w.at = find_place<NW>(g, &w.left, red, found);
+    if (g.cluster > 1) {
+        w.at.b = blockIdx.x / g.cluster / (g.a.hkv * g.row_blocks);
+        w.at.span = seq_tiles(g, w.at.b);
+    } else {
+        w.at = find_place<NW>(g, &w.left, red, found);
+    }
     return w;
 }
 
@@ -232,10 +253,10 @@ struct DecRow {
 };
 
 // The end of a piece: `warps` sums of o (rows x ld fp32 each), m, l in shared
-// memory -> the output, or the block's part.
+// memory -> the output, or the block's part (in a cluster: `shared`).
 template <typename T>
 __device__ __forceinline__ void finish_piece(const DecArgs& g, const Piece& pc, const float* o, int warps, int wstride, int ld,
-                                             const float* m, const float* l, int row0, int rows, int thread, int threads) {
+                                             const float* m, const float* l, int row0, int rows, int thread, int threads, float* shared) {
     const AttnCall& a = g.a;
     const int d2 = a.d + 2, used = min(rows, a.nq * (a.hq / a.hkv) - pc.rb * g.rows - row0);
     for (int e = thread; e < used * a.d; e += threads) {
@@ -257,11 +278,53 @@ __device__ __forceinline__ void finish_piece(const DecArgs& g, const Piece& pc, 
             if (a.lse && c == 0)
                 a.lse[((int64_t)pc.b * a.hq + h) * a.nq + i] = none ? -INFINITY : top * kLn2 + logf(sum);
         } else {
-            float* part = g.part + ((size_t)(blockIdx.x * 2 + pc.slot) * g.rows + row0 + r) * d2;
+            float* part = (g.cluster > 1 ? shared : g.part + (size_t)(blockIdx.x * 2 + pc.slot) * g.rows * d2) + (row0 + r) * d2;
             part[c] = out;
             if (c == 0) { part[a.d] = top; part[a.d + 1] = sum; }
         }
     }
+}
+
+// The pieces of a cluster's unit, each in its block's `shared`, joined in the
+// order of the keys: the blocks take rows x columns in turn.
+template <typename T>
+__device__ __forceinline__ void join_cluster(const DecArgs& g, const Piece& pc, const float* shared, int threads) {
+    const AttnCall& a = g.a;
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const int rank = blockIdx.x % g.cluster, d2 = a.d + 2;
+    const int used = min(g.rows, a.nq * (a.hq / a.hkv) - pc.rb * g.rows);
+    for (int e = rank * threads + threadIdx.x; threadIdx.x < threads && e < used * a.d; e += threads * g.cluster) {
+        const int r = e / a.d, c = e % a.d;
+        float o[8], m[8], l[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            uint32_t at;
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(shared + r * d2)), "r"(min(q, g.cluster - 1)));
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o[q]) : "r"(at + 4 * c));
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(m[q]) : "r"(at + 4 * a.d));
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(l[q]) : "r"(at + 4 * a.d + 4));
+        }
+        float top = -INFINITY, sum = 0.f, out = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (q < g.cluster) top = fmaxf(top, m[q]);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (q < g.cluster) {
+                const float by = top == -INFINITY ? 0.f : ex2(m[q] - top);
+                sum = fmaf(by, l[q], sum);
+                out = fmaf(by, o[q], out);
+            }
+        int i, h;
+        unit_row(a, pc.kvh, pc.rb * g.rows + r, &i, &h);
+        const bool none = sum == 0.f;
+        static_cast<T*>(a.o.p)[pc.b * a.o.sb + h * a.o.sh + i * a.o.ss + c * a.o.sd] = from_f32<T>(none ? 0.f : out / sum);
+        if (a.lse && c == 0) a.lse[((int64_t)pc.b * a.hq + h) * a.nq + i] = none ? -INFINITY : top * kLn2 + logf(sum);
+    }
+    __syncwarp();
+    // a block's part stays until the others have read it
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // A block a row: rows of units that lie over several blocks, and of sequences
@@ -273,8 +336,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_decode_join(const __grid_const
     const int rows = a.nq * (a.hq / a.hkv), units = a.hkv * g.row_blocks;
     const int row = blockIdx.x % rows, kvh = blockIdx.x / rows % a.hkv, b = blockIdx.x / rows / a.hkv;
     const int unit = kvh * g.row_blocks + row / g.rows, r = row % g.rows;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    int64_t all;
+    int64_t all;   // from the lengths, which were there before the kernel that reads the cache
     const int64_t before = tiles_before<JOIN_THREADS / 32>(g, b, &all, red) * units;
     all *= units;
     const int2 span = seq_tiles(g, b);
@@ -283,6 +345,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_decode_join(const __grid_const
     const int64_t u0 = before + (int64_t)unit * n, u1 = u0 + n;
     const int first = (int)(u0 / per), last = n ? (int)((u1 - 1) / per) : first;
     if (n && first == last) return;   // one block wrote it
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     int i, h;
     unit_row(a, kvh, row, &i, &h);
     // a block's second piece is the one that starts inside it
@@ -337,10 +400,11 @@ constexpr int DM_THREADS = 32 * (DM_WARPS + 1);      // and one warp of TMA
 
 template <int DP, int MT>
 struct DmSmem {
-    static constexpr int CH = DP / 64, CHUNK = DT * 128, TILE_B = CH * CHUNK, STAGES = DP == 64 ? 8 : 4;
+    static constexpr int KW = DP == 64 ? 32 : 16, DT = 4 * KW;   // keys of a warp, of a tile
+    static constexpr int CH = DP / 64, CHUNK = DT * 128, TILE_B = CH * CHUNK, STAGES = 4;
     static constexpr int LQ = DP + 8;   // 16-bit query rows, padded by 16 bytes
     static constexpr int KV = 0, Q = STAGES * 2 * TILE_B, MERGE = Q + 16 * MT * LQ * 2, LO = DP + 4,
-                         STAT = MERGE + DM_WARPS * 16 * LO * 4, BAR = STAT + 2 * DM_WARPS * 16 * 4, BYTES = BAR + 256 + 1024;
+                         STAT = MERGE + DM_WARPS * 16 * LO * 4, PART = STAT + 2 * DM_WARPS * 16 * 4, BAR = PART + 16 * MT * (DP + 2) * 4, BYTES = BAR + 256 + 1024;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t at, uint32_t* r) {
@@ -403,7 +467,7 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
                             asm volatile(
                                 "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, "
                                 "%6}], [%2];" ::"r"(smem_u32(smem + L::KV + (2 * s + w) * L::TILE_B + c * L::CHUNK)),
-                                "l"(reinterpret_cast<uint64_t>(&m.map)), "r"(smem_u32(&full[s])), "r"(64 * c), "r"(t * DT),
+                                "l"(reinterpret_cast<uint64_t>(&m.map)), "r"(smem_u32(&full[s])), "r"(64 * c), "r"(t * L::DT),
                                 "r"(pc.kvh * m.mh), "r"(pc.b * m.mb)
                                 : "memory");
                         }
@@ -412,6 +476,7 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
             }
         if (!ok)
             for (int e = max(0, n - 1 - L::STAGES); e < n - 1; ++e) mbar_wait(&full[e % L::STAGES], (e / L::STAGES) & 1, g.err);
+        if (g.cluster > 1) join_cluster<T>(g, pc, reinterpret_cast<float*>(smem + L::PART), 32 * DM_WARPS);
         return;
     }
 
@@ -455,56 +520,62 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
                 for (int e = 0; e < 4; ++e) o[u][c][e] = 0.f;
         for (int t = pc.t0; t < pc.t1 && ok; ++t, ++n) {
             if (n % DM_SETS != set) continue;
-            const int st = n % L::STAGES, j0 = t * DT + sub * 16;
+            constexpr int KW = L::KW, NK = KW / 8;   // tiles of 8 keys of a warp
+            const int st = n % L::STAGES, j0 = t * L::DT + sub * KW;
             ok = mbar_wait(&full[st], (n / L::STAGES) & 1, g.err);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             uint8_t* kt = smem + L::KV + 2 * st * L::TILE_B;
             uint8_t* vt = kt + L::TILE_B;
             // keys whose values must not count: 0 times what they hold could be NaN
-            const int jl = j0 + (lane & 15);
+            const int jl = j0 + lane % KW;
             const int jdoc = kd && jl < a.nk ? __ldg(kd + jl) : -1;
             const bool bad = jl >= mask.kv || (kd && jdoc < 0);
             const bool dirty = __any_sync(0xffffffffu, bad);
             if (dirty) {
-                if (bad && lane < 16)
+                if (bad && lane < KW)
                     for (int c = 0; c < L::CH; ++c)
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
-                            *reinterpret_cast<uint4*>(vt + c * L::CHUNK + (sub * 16 + lane) * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(vt + c * L::CHUNK + (sub * KW + lane) * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
                 __syncwarp();
             }
-            // scores of 16 keys: two tiles of 8 columns
-            float s[MT][2][4];
+            // scores of the warp's keys, 8 to a tile
+            float s[MT][NK][4];
 #pragma unroll
             for (int u = 0; u < MT; ++u)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s[u][e / 4][e % 4] = 0.f;
+                for (int e = 0; e < 4 * NK; ++e) s[u][e / 4][e % 4] = 0.f;
             {
-                const int key = sub * 16 + (mi >> 1) * 8 + mr;
+                const int key = sub * KW + (mi >> 1) * 8 + mr;
                 const uint32_t kb = smem_u32(kt) + key * 128;
                 const uint32_t qb = smem_u32(qs) + ((mi & 1) * 8 + mr) * (L::LQ * 2) + (mi >> 1) * 16;
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
                     if (k >= ksteps) break;
                     const int c16 = 2 * (k % 4) + (mi & 1);
-                    uint32_t kf[4];
-                    ldsm4(kb + (k / 4) * L::CHUNK + ((c16 ^ (key & 7)) << 4), kf);
+                    uint32_t kf[NK / 2][4];
+#pragma unroll
+                    for (int x = 0; x < NK / 2; ++x)
+                        ldsm4(kb + x * 16 * 128 + (k / 4) * L::CHUNK + ((c16 ^ (key & 7)) << 4), kf[x]);
 #pragma unroll
                     for (int u = 0; u < MT; ++u) {
                         uint32_t qf[4];
                         ldsm4(qb + u * 16 * L::LQ * 2 + k * 32, qf);
-                        mma16816<T>(s[u][0], qf, kf[0], kf[1]);
-                        mma16816<T>(s[u][1], qf, kf[2], kf[3]);
+#pragma unroll
+                        for (int x = 0; x < NK / 2; ++x) {
+                            mma16816<T>(s[u][2 * x], qf, kf[x][0], kf[x][1]);
+                            mma16816<T>(s[u][2 * x + 1], qf, kf[x][2], kf[x][3]);
+                        }
                     }
                 }
             }
-            uint32_t p[MT][4];
+            uint32_t p[MT][NK / 2][4];
 #pragma unroll
             for (int u = 0; u < MT; ++u) {
                 float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
+                for (int x = 0; x < NK; ++x)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int col = 8 * x + 2 * tid + (e & 1);
@@ -534,33 +605,35 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
                         }
                     }
                 }
-                float pr[2][4];
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
+                for (int x = 0; x < NK; ++x) {
+                    float pr[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float ref = (m[u][e >> 1] == -INFINITY ? 0.f : m[u][e >> 1]) - Lift<T>::log2;
-                        pr[x][e] = ex2(s[u][x][e] - ref);
-                        l[u][e >> 1] += pr[x][e];
+                        pr[e] = ex2(s[u][x][e] - ref);
+                        l[u][e >> 1] += pr[e];
                     }
-                p[u][0] = pack16<T>(pr[0][0], pr[0][1]);
-                p[u][1] = pack16<T>(pr[0][2], pr[0][3]);
-                p[u][2] = pack16<T>(pr[1][0], pr[1][1]);
-                p[u][3] = pack16<T>(pr[1][2], pr[1][3]);
+                    p[u][x / 2][2 * (x % 2)] = pack16<T>(pr[0], pr[1]);
+                    p[u][x / 2][2 * (x % 2) + 1] = pack16<T>(pr[2], pr[3]);
+                }
             }
             {
-                const int key = sub * 16 + (mi & 1) * 8 + mr;
+                const int key = sub * KW + (mi & 1) * 8 + mr;
                 const uint32_t vb = smem_u32(vt) + key * 128;
 #pragma unroll
                 for (int c = 0; c < DP / 8; c += 2) {
                     if (8 * c >= a.d) break;
                     const int c16 = c % 8 + (mi >> 1);
-                    uint32_t vf[4];
-                    ldsm4t(vb + (c / 8) * L::CHUNK + ((c16 ^ (key & 7)) << 4), vf);
 #pragma unroll
-                    for (int u = 0; u < MT; ++u) {
-                        mma16816<T>(o[u][c], p[u], vf[0], vf[1]);
-                        mma16816<T>(o[u][c + 1], p[u], vf[2], vf[3]);
+                    for (int x = 0; x < NK / 2; ++x) {
+                        uint32_t vf[4];
+                        ldsm4t(vb + x * 16 * 128 + (c / 8) * L::CHUNK + ((c16 ^ (key & 7)) << 4), vf);
+#pragma unroll
+                        for (int u = 0; u < MT; ++u) {
+                            mma16816<T>(o[u][c], p[u][x], vf[0], vf[1]);
+                            mma16816<T>(o[u][c + 1], p[u][x], vf[2], vf[3]);
+                        }
                     }
                 }
             }
@@ -587,31 +660,33 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
                 *reinterpret_cast<float2*>(mw + (gid + 8) * L::LO + 8 * c + 2 * tid) = make_float2(o[u][c][2], o[u][c][3]);
             }
             asm volatile("bar.sync 1, %0;" ::"n"(32 * DM_WARPS) : "memory");
-            if (ok) finish_piece<T>(g, pc, merge, DM_WARPS, 16 * L::LO, L::LO, m_s, l_s, 16 * u, 16, threadIdx.x, 32 * DM_WARPS);
+            if (ok) finish_piece<T>(g, pc, merge, DM_WARPS, 16 * L::LO, L::LO, m_s, l_s, 16 * u, 16, threadIdx.x, 32 * DM_WARPS,
+                                    reinterpret_cast<float*>(smem + L::PART));
             asm volatile("bar.sync 1, %0;" ::"n"(32 * DM_WARPS) : "memory");
         }
     }
+    if (g.cluster > 1) join_cluster<T>(g, pc, reinterpret_cast<float*>(smem + L::PART), 32 * DM_WARPS);
 }
 
 // ---------------------------------------------------------------- any type
-constexpr int DA_THREADS = 256;
+constexpr int DA_THREADS = 256, DA_T = 64;   // threads, keys of a tile
 
 template <int DP, int RB>
 struct DaSmem {
     static constexpr int LD = DP + 16;   // rows half of the banks apart
-    static constexpr int K = 0, V = K + DT * LD * 4, Q = V + DT * LD * 4, P = Q + RB * DP * 4, STAT = P + DT * RB * 4,
+    static constexpr int K = 0, V = K + DA_T * LD * 4, Q = V + DA_T * LD * 4, P = Q + RB * DP * 4, STAT = P + DA_T * RB * 4,
                          BYTES = STAT + 3 * RB * 4;
-    static_assert(8 * RB * DP <= 2 * DT * LD, "the warps' sums lie over the tiles");
+    static_assert(8 * RB * DP <= 2 * DA_T * LD, "the warps' sums lie over the tiles");
 };
 
 // Scores: four threads a key, each a quarter of its columns for all rows.
 // Sums: warp w takes keys w, w + 8, ... of the tile, a lane 4 columns of every
 // 128, for all rows.
-template <typename T, int DP, int RB>
+template <typename T, int DP, int RB, bool VEC>
 __global__ void __launch_bounds__(DA_THREADS) k_decode_any(const __grid_constant__ DecArgs g) {
     using L = DaSmem<DP, RB>;
     extern __shared__ __align__(16) uint8_t smem[];
-    float *K = reinterpret_cast<float*>(smem + L::K), *V = reinterpret_cast<float*>(smem + L::V);
+    float *K = reinterpret_cast<float*>(smem + L::K), *V_ = reinterpret_cast<float*>(smem + L::V);
     float *Q = reinterpret_cast<float*>(smem + L::Q), *P = reinterpret_cast<float*>(smem + L::P);
     float *m_s = reinterpret_cast<float*>(smem + L::STAT), *l_s = m_s + RB, *by_s = l_s + RB;
     __shared__ int64_t red[DA_THREADS / 32], found[2];
@@ -637,6 +712,9 @@ __global__ void __launch_bounds__(DA_THREADS) k_decode_any(const __grid_constant
             Q[r * DP + c] = v;
         }
         if (threadIdx.x < RB) { m_s[threadIdx.x] = -INFINITY; l_s[threadIdx.x] = 0.f; }
+        DecRow rows[RB / 4];   // of the scores this thread writes: rows threadIdx.x % 4, + 4, ...
+#pragma unroll
+        for (int r = 0; r < RB / 4; ++r) rows[r].set(a, mask, pc.b, pc.kvh, pc.rb * g.rows + 4 * r + threadIdx.x % 4);
         float o[RB][NC][4];
 #pragma unroll
         for (int r = 0; r < RB; ++r)
@@ -646,18 +724,51 @@ __global__ void __launch_bounds__(DA_THREADS) k_decode_any(const __grid_constant
                 for (int e = 0; e < 4; ++e) o[r][c][e] = 0.f;
         const T* kp = static_cast<const T*>(a.k.p) + pc.b * a.k.sb + pc.kvh * a.k.sh;
         const T* vp = static_cast<const T*>(a.v.p) + pc.b * a.v.sb + pc.kvh * a.v.sh;
+        // 16-byte vectors of the tile after this one are in registers while this
+        // one is used (VEC: rows and head size allow them)
+        constexpr int V = 16 / sizeof(T), NV = DA_T * DP / V / DA_THREADS;
+        uint4 kr[VEC ? NV : 1], vr[VEC ? NV : 1];
+        auto fetch = [&](int t) {
+            if constexpr (VEC) {
+#pragma unroll
+                for (int e = 0; e < NV; ++e) {
+                    const int at = threadIdx.x + e * DA_THREADS, r = at / (DP / V), c = at % (DP / V) * V;
+                    const int64_t j = (int64_t)t * DA_T + r;
+                    const bool on = t < pc.t1 && j < mask.kv && c < a.d && (!kd || kd[j] >= 0);
+                    kr[e] = on ? *reinterpret_cast<const uint4*>(kp + j * a.k.ss + c) : make_uint4(0, 0, 0, 0);
+                    vr[e] = on ? *reinterpret_cast<const uint4*>(vp + j * a.v.ss + c) : make_uint4(0, 0, 0, 0);
+                }
+            }
+        };
+        fetch(pc.t0);
         for (int t = pc.t0; t < pc.t1; ++t) {
-            const int j0 = t * DT;
+            const int j0 = t * DA_T;
             __syncthreads();
+            if constexpr (VEC) {
+#pragma unroll
+                for (int e = 0; e < NV; ++e) {
+                    const int at = threadIdx.x + e * DA_THREADS, r = at / (DP / V), c = at % (DP / V) * V;
+                    const T *ke = reinterpret_cast<const T*>(&kr[e]), *ve = reinterpret_cast<const T*>(&vr[e]);
+#pragma unroll
+                    for (int f = 0; f < V; f += 4) {
+                        *reinterpret_cast<float4*>(K + r * L::LD + c + f) =
+                            make_float4(to_f32(ke[f]), to_f32(ke[f + 1]), to_f32(ke[f + 2]), to_f32(ke[f + 3]));
+                        *reinterpret_cast<float4*>(V_ + r * L::LD + c + f) =
+                            make_float4(to_f32(ve[f]), to_f32(ve[f + 1]), to_f32(ve[f + 2]), to_f32(ve[f + 3]));
+                    }
+                }
+            } else {
 #pragma unroll 4
-            for (int e = threadIdx.x; e < DT * DP; e += DA_THREADS) {
-                const int r = e / DP, c = e % DP;
-                const int64_t j = j0 + r;
-                const bool on = j < mask.kv && c < a.d && (!kd || kd[j] >= 0);
-                K[r * L::LD + c] = on ? to_f32(kp[j * a.k.ss + c * a.k.sd]) : 0.f;
-                V[r * L::LD + c] = on ? to_f32(vp[j * a.v.ss + c * a.v.sd]) : 0.f;
+                for (int e = threadIdx.x; e < DA_T * DP; e += DA_THREADS) {
+                    const int r = e / DP, c = e % DP;
+                    const int64_t j = j0 + r;
+                    const bool on = j < mask.kv && c < a.d && (!kd || kd[j] >= 0);
+                    K[r * L::LD + c] = on ? to_f32(kp[j * a.k.ss + c * a.k.sd]) : 0.f;
+                    V_[r * L::LD + c] = on ? to_f32(vp[j * a.v.ss + c * a.v.sd]) : 0.f;
+                }
             }
             __syncthreads();
+            fetch(t + 1);
             {
                 const int key = threadIdx.x / 4, part = threadIdx.x % 4;
                 float s[RB];
@@ -681,8 +792,7 @@ __global__ void __launch_bounds__(DA_THREADS) k_decode_any(const __grid_constant
 #pragma unroll
                 for (int r = 0; r < RB; ++r)
                     if (r % 4 == part) {
-                        DecRow row;
-                        row.set(a, mask, pc.b, pc.kvh, pc.rb * g.rows + r);
+                        const DecRow& row = rows[r / 4];
                         float x = s[r];
                         float y = a.cap > 0.f ? a.cap * kLog2e * tanhf(x * (a.scale / a.cap)) : x * (a.scale * kLog2e);
                         y -= row.slope2 * fabsf((float)(row.p - j));
@@ -723,10 +833,10 @@ __global__ void __launch_bounds__(DA_THREADS) k_decode_any(const __grid_constant
                             for (int e = 0; e < 4; ++e) o[r][c][e] *= by;
                 }
 #pragma unroll 2
-                for (int key = warp; key < DT; key += DA_THREADS / 32) {
+                for (int key = warp; key < DA_T; key += DA_THREADS / 32) {
                     float4 v[NC];
 #pragma unroll
-                    for (int c = 0; c < NC; ++c) v[c] = *reinterpret_cast<const float4*>(V + key * L::LD + 128 * c + 4 * lane);
+                    for (int c = 0; c < NC; ++c) v[c] = *reinterpret_cast<const float4*>(V_ + key * L::LD + 128 * c + 4 * lane);
 #pragma unroll
                     for (int r = 0; r < RB; ++r) {
                         const float p = P[key * RB + r];
@@ -759,7 +869,9 @@ __global__ void __launch_bounds__(DA_THREADS) k_decode_any(const __grid_constant
             Q[e] = s;
         }
         __syncthreads();
-        finish_piece<T>(g, pc, Q, 1, 0, DP, m_s, l_s, 0, RB, threadIdx.x, DA_THREADS);
+        finish_piece<T>(g, pc, Q, 1, 0, DP, m_s, l_s, 0, RB, threadIdx.x, DA_THREADS, K);
+        __syncthreads();
+        if (g.cluster > 1) join_cluster<T>(g, pc, K, DA_THREADS);
     }
 }
 
@@ -789,20 +901,34 @@ tl_status launch_mma(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
     TL_TRY(kernel_smem(c, k_decode_mma<T, DP, MT>, smem, done));
     const AttnCall& a = g.a;
     HeadMap mk, mv;
-    if (!make_head_map(&mk, a.k, a.dtype, a.b, a.hkv, a.nk, a.d, DT) || !make_head_map(&mv, a.v, a.dtype, a.b, a.hkv, a.nk, a.d, DT))
+    if (!make_head_map(&mk, a.k, a.dtype, a.b, a.hkv, a.nk, a.d, DmSmem<DP, MT>::DT) ||
+        !make_head_map(&mv, a.v, a.dtype, a.b, a.hkv, a.nk, a.d, DmSmem<DP, MT>::DT))
         return fail(c, TL_ERR_CUDA, "attention: tensor maps");
     c->flags_armed = true;
-    k_decode_mma<T, DP, MT><<<g.blocks, DM_THREADS, smem, s>>>(mk, mv, g);
+    TL_CK(c, launch_cluster(k_decode_mma<T, DP, MT>, g.blocks, g.cluster, DM_THREADS, smem, s, mk, mv, g));
+    return TL_OK;
+}
+
+template <typename T, int DP, int RB, bool VEC>
+tl_status launch_any_as(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    constexpr int smem = DaSmem<DP, RB>::BYTES;
+    TL_TRY(kernel_smem(c, k_decode_any<T, DP, RB, VEC>, smem, done));
+    TL_CK(c, launch_cluster(k_decode_any<T, DP, RB, VEC>, g.blocks, g.cluster, DA_THREADS, smem, s, g));
     return TL_OK;
 }
 
 template <typename T, int DP, int RB>
 tl_status launch_any(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
-    static std::atomic<uint64_t> done{0};
-    constexpr int smem = DaSmem<DP, RB>::BYTES;
-    TL_TRY(kernel_smem(c, k_decode_any<T, DP, RB>, smem, done));
-    k_decode_any<T, DP, RB><<<g.blocks, DA_THREADS, smem, s>>>(g);
-    return TL_OK;
+    // rows of whole 16-byte vectors
+    const AttnCall& a = g.a;
+    const int64_t n = 16 / sizeof(T);
+    auto fits = [&](const HeadsView& v) {
+        return v.sd == 1 && reinterpret_cast<uintptr_t>(v.p) % 16 == 0 && (a.nk <= 1 || v.ss % n == 0) && (a.hkv <= 1 || v.sh % n == 0) &&
+               (a.b <= 1 || v.sb % n == 0);
+    };
+    if (a.d % n == 0 && fits(a.k) && fits(a.v)) return launch_any_as<T, DP, RB, true>(c, g, s);
+    return launch_any_as<T, DP, RB, false>(c, g, s);
 }
 
 template <typename T>
@@ -844,7 +970,11 @@ tl_status launch_attn_few(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s
     g.err = c->d_flags + 8;
     // no more blocks than tiles there can be
     const int64_t units = (int64_t)a.b * a.hkv * g.row_blocks, rows = (int64_t)a.nq * (a.hq / a.hkv);
-    g.blocks = (int)std::min<int64_t>(few_blocks(a), units * ((a.nk + DT - 1) / DT));
+    g.tile = few_takes_mma(a) && a.d <= 64 ? 128 : 64;
+    const int64_t tiles = (a.nk + g.tile - 1) / g.tile;
+    // a cluster a unit while all of them run at once and a block has few tiles
+    g.cluster = units * 8 <= kSms && tiles <= 32 ? 8 : 1;
+    g.blocks = g.cluster > 1 ? (int)units * g.cluster : (int)std::min<int64_t>(few_blocks(a), units * tiles);
     cudaEvent_t ev[2];
     if (a.k_doc) {
         int2* spans = reinterpret_cast<int2*>(w + plan.spans);
@@ -858,6 +988,7 @@ tl_status launch_attn_few(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s
     case TL_TYPE_F16: TL_TRY(launch_type<__half>(c, g, s)); break;
     default: TL_TRY(launch_type<__nv_bfloat16>(c, g, s));
     }
+    if (g.cluster > 1) return TL_OK;
     launch_begin_on(c, s, "attention_decode_join", 0, 0, ev);
     cudaError_t e;
     switch (a.dtype) {

@@ -861,19 +861,9 @@ tl_status launch(tl_ctx* c, const HeadMap* m, const BwArgs& g, cudaStream_t s) {
     TL_TRY(kernel_smem(c, k_attn_tc_dq<T, U, DP, CAP, BIAS>, smem, done_q));
     const AttnCall& a = g.a;
     cudaEvent_t ev[2];
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = g.cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)((int64_t)g.k_tiles * a.b * a.hkv * g.cluster));
-    cfg.blockDim = dim3(BW_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
     launch_begin_on(c, s, "attention_tc_dkv", 0, 8.0 * a.d * attn_pairs(a), ev);
-    TL_CK(c, cudaLaunchKernelEx(&cfg, k_attn_tc_dkv<T, U, DP, CAP, BIAS>, m[0], m[1], m[2], m[3], g));
+    TL_CK(c, launch_cluster(k_attn_tc_dkv<T, U, DP, CAP, BIAS>, (unsigned)((int64_t)g.k_tiles * a.b * a.hkv * g.cluster), g.cluster,
+                            BW_THREADS, smem, s, m[0], m[1], m[2], m[3], g));
     TL_TRY(launch_end_on(c, s, ev));
     launch_begin_on(c, s, "attention_tc_dq", 0, 6.0 * a.d * attn_pairs(a), ev);
     k_attn_tc_dq<T, U, DP, CAP, BIAS><<<(unsigned)((int64_t)g.q_tiles * a.b * a.hq), BW_THREADS, smem, s>>>(m[0], m[1], m[2], m[3], g);
