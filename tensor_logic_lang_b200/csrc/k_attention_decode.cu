@@ -14,8 +14,8 @@
 //
 //   k_decode_mma   16-bit types with aligned rows and head sizes up to 128: TMA
 //                  tiles (128-byte swizzle) through a ring; each of four
-//                  warps takes a quarter of a tile's keys for all rows (two
-//                  sets of four take the tiles in turn), with mma.sync.m16n8k16 (at a few rows a key the tensor work is a
+//                  warps takes a quarter of a tile's keys for all rows, with
+//                  mma.sync.m16n8k16 (at a few rows a key the tensor work is a
 //                  fraction of the time the key's bytes take)
 //   k_decode_any   any type, stride and head size: tiles as fp32 in shared
 //                  memory, FFMA
@@ -27,6 +27,7 @@ namespace tl {
 namespace {
 
 constexpr int JOIN_THREADS = 128;
+constexpr int kSms = 148;
 
 struct DecArgs {
     AttnCall a;
@@ -332,6 +333,7 @@ __device__ __forceinline__ void join_cluster(const DecArgs& g, const Piece& pc, 
 template <typename T>
 __global__ void __launch_bounds__(JOIN_THREADS) k_decode_join(const __grid_constant__ DecArgs g) {
     __shared__ int64_t red[JOIN_THREADS / 32];
+    __shared__ float weight[2 * kSms], sums[2 * kSms], tops[JOIN_THREADS / 32];   // of at most every block
     const AttnCall& a = g.a;
     const int rows = a.nq * (a.hq / a.hkv), units = a.hkv * g.row_blocks;
     const int row = blockIdx.x % rows, kvh = blockIdx.x / rows % a.hkv, b = blockIdx.x / rows / a.hkv;
@@ -350,18 +352,30 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_decode_join(const __grid_const
     unit_row(a, kvh, row, &i, &h);
     // a block's second piece is the one that starts inside it
     auto part = [&](int q) { return g.part + ((size_t)(q * 2 + ((int64_t)q * per < u0 ? 1 : 0)) * g.rows + r) * d2; };
+    // the parts' maxima and sums, a thread a part; weights for the columns
+    const int parts = n ? last - first + 1 : 0;
+    float top = -INFINITY;
+    for (int q = threadIdx.x; q < parts; q += JOIN_THREADS) {
+        const float* p = part(first + q);
+        weight[q] = p[a.d];
+        sums[q] = p[a.d + 1];
+        top = fmaxf(top, weight[q]);
+    }
+#pragma unroll
+    for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < JOIN_THREADS / 32; ++w) top = fmaxf(top, tops[w]);
+    for (int q = threadIdx.x; q < parts; q += JOIN_THREADS) weight[q] = top == -INFINITY ? 0.f : ex2(weight[q] - top);
+    __syncthreads();
     for (int c = threadIdx.x; c < a.d; c += JOIN_THREADS) {
-        float top = -INFINITY, sum = 0.f, out = 0.f;
-        if (n) {
-#pragma unroll 4
-            for (int q = first; q <= last; ++q) top = fmaxf(top, part(q)[a.d]);
-#pragma unroll 4
-            for (int q = first; q <= last; ++q) {
-                const float* p = part(q);
-                const float by = top == -INFINITY ? 0.f : ex2(p[a.d] - top);
-                sum = fmaf(by, p[a.d + 1], sum);
-                out = fmaf(by, p[c], out);
-            }
+        float sum = 0.f, out = 0.f;
+#pragma unroll 8
+        for (int q = 0; q < parts; ++q) {
+            sum = fmaf(weight[q], sums[q], sum);
+            out = fmaf(weight[q], part(first + q)[c], out);
         }
         const bool none = sum == 0.f;
         static_cast<T*>(a.o.p)[b * a.o.sb + h * a.o.sh + i * a.o.ss + c * a.o.sd] = from_f32<T>(none ? 0.f : out / sum);
@@ -395,16 +409,16 @@ __global__ void __launch_bounds__(256) k_doc_spans(const __grid_constant__ AttnC
 }
 
 // ---------------------------------------------------------------- tensor cores
-constexpr int DM_SETS = 2, DM_WARPS = 4 * DM_SETS;   // sets of four warps take the tiles in turn
-constexpr int DM_THREADS = 32 * (DM_WARPS + 1);      // and one warp of TMA
 
 template <int DP, int MT>
 struct DmSmem {
     static constexpr int KW = DP == 64 ? 32 : 16, DT = 4 * KW;   // keys of a warp, of a tile
-    static constexpr int CH = DP / 64, CHUNK = DT * 128, TILE_B = CH * CHUNK, STAGES = 4;
+    // sets of four warps take the tiles in turn; one warp of TMA
+    static constexpr int SETS = MT, WARPS = 4 * SETS, THREADS = 32 * (WARPS + 1), PER_SM = MT == 1 ? 2 : 1;
+    static constexpr int CH = DP / 64, CHUNK = DT * 128, TILE_B = CH * CHUNK, STAGES = 2 * SETS;
     static constexpr int LQ = DP + 8;   // 16-bit query rows, padded by 16 bytes
     static constexpr int KV = 0, Q = STAGES * 2 * TILE_B, MERGE = Q + 16 * MT * LQ * 2, LO = DP + 4,
-                         STAT = MERGE + DM_WARPS * 16 * LO * 4, PART = STAT + 2 * DM_WARPS * 16 * 4, BAR = PART + 16 * MT * (DP + 2) * 4, BYTES = BAR + 256 + 1024;
+                         STAT = MERGE + WARPS * 16 * LO * 4, PART = STAT + 2 * WARPS * 16 * 4, BAR = PART + 16 * MT * (DP + 2) * 4, BYTES = BAR + 256 + 1024;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t at, uint32_t* r) {
@@ -433,14 +447,14 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
 
 // MT: tiles of 16 rows of a unit
 template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(DM_THREADS, 1)
+__global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_SM)
     k_decode_mma(const __grid_constant__ HeadMap mk, const __grid_constant__ HeadMap mv, const __grid_constant__ DecArgs g) {
     using L = DmSmem<DP, MT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR);
     uint64_t* empty = full + L::STAGES;
-    __shared__ int64_t red[DM_THREADS / 32], found[2];
+    __shared__ int64_t red[L::THREADS / 32], found[2];
     const AttnCall& a = g.a;
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -448,12 +462,12 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
         for (int s = 0; s < L::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 4); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    PieceWalk walk = block_pieces<DM_THREADS / 32>(g, red, found);
+    PieceWalk walk = block_pieces<L::THREADS / 32>(g, red, found);
     __syncthreads();
     Piece pc;
     int n = 0;
     bool ok = true;
-    if (warp == DM_WARPS) {
+    if (warp == L::WARPS) {
         while (ok && walk.next(g, &pc))
             for (int t = pc.t0; t < pc.t1 && ok; ++t, ++n) {
                 const int s = n % L::STAGES;
@@ -476,7 +490,7 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
             }
         if (!ok)
             for (int e = max(0, n - 1 - L::STAGES); e < n - 1; ++e) mbar_wait(&full[e % L::STAGES], (e / L::STAGES) & 1, g.err);
-        if (g.cluster > 1) join_cluster<T>(g, pc, reinterpret_cast<float*>(smem + L::PART), 32 * DM_WARPS);
+        if (g.cluster > 1) join_cluster<T>(g, pc, reinterpret_cast<float*>(smem + L::PART), 32 * L::WARPS);
         return;
     }
 
@@ -485,13 +499,13 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
     const int ksteps = (a.d + 15) / 16;
     T* qs = reinterpret_cast<T*>(smem + L::Q);
     float* merge = reinterpret_cast<float*>(smem + L::MERGE);
-    float *m_s = reinterpret_cast<float*>(smem + L::STAT), *l_s = m_s + DM_WARPS * 16;
+    float *m_s = reinterpret_cast<float*>(smem + L::STAT), *l_s = m_s + L::WARPS * 16;
     const int set = warp / 4, sub = warp % 4;
     while (walk.next(g, &pc)) {
         const SeqMask mask(a, pc.b);
         const int32_t* kd = a.k_doc ? a.k_doc + (int64_t)pc.b * a.nk : nullptr;
         // the unit's query rows (zeros past the last one and past the head size)
-        for (int e = threadIdx.x; e < 16 * MT * DP / 8; e += 32 * DM_WARPS) {
+        for (int e = threadIdx.x; e < 16 * MT * DP / 8; e += 32 * L::WARPS) {
             const int r = e / (DP / 8), c = e % (DP / 8) * 8, row = pc.rb * g.rows + r;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (row < a.nq * (a.hq / a.hkv) && c < a.d) {
@@ -501,7 +515,7 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
             }
             *reinterpret_cast<uint4*>(qs + r * L::LQ + c) = v;
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * DM_WARPS) : "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * L::WARPS) : "memory");
         DecRow row[MT][2];
         float m[MT][2], l[MT][2], o[MT][DP / 8][4];
 #pragma unroll
@@ -519,7 +533,7 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[u][c][e] = 0.f;
         for (int t = pc.t0; t < pc.t1 && ok; ++t, ++n) {
-            if (n % DM_SETS != set) continue;
+            if (n % L::SETS != set) continue;
             constexpr int KW = L::KW, NK = KW / 8;   // tiles of 8 keys of a warp
             const int st = n % L::STAGES, j0 = t * L::DT + sub * KW;
             ok = mbar_wait(&full[st], (n / L::STAGES) & 1, g.err);
@@ -659,13 +673,13 @@ __global__ void __launch_bounds__(DM_THREADS, 1)
                 *reinterpret_cast<float2*>(mw + gid * L::LO + 8 * c + 2 * tid) = make_float2(o[u][c][0], o[u][c][1]);
                 *reinterpret_cast<float2*>(mw + (gid + 8) * L::LO + 8 * c + 2 * tid) = make_float2(o[u][c][2], o[u][c][3]);
             }
-            asm volatile("bar.sync 1, %0;" ::"n"(32 * DM_WARPS) : "memory");
-            if (ok) finish_piece<T>(g, pc, merge, DM_WARPS, 16 * L::LO, L::LO, m_s, l_s, 16 * u, 16, threadIdx.x, 32 * DM_WARPS,
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * L::WARPS) : "memory");
+            if (ok) finish_piece<T>(g, pc, merge, L::WARPS, 16 * L::LO, L::LO, m_s, l_s, 16 * u, 16, threadIdx.x, 32 * L::WARPS,
                                     reinterpret_cast<float*>(smem + L::PART));
-            asm volatile("bar.sync 1, %0;" ::"n"(32 * DM_WARPS) : "memory");
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * L::WARPS) : "memory");
         }
     }
-    if (g.cluster > 1) join_cluster<T>(g, pc, reinterpret_cast<float*>(smem + L::PART), 32 * DM_WARPS);
+    if (g.cluster > 1) join_cluster<T>(g, pc, reinterpret_cast<float*>(smem + L::PART), 32 * L::WARPS);
 }
 
 // ---------------------------------------------------------------- any type
@@ -881,8 +895,7 @@ int few_rows(const AttnCall& a) {
     if (few_takes_mma(a)) return rows <= 16 ? 16 : 32;
     return rows <= 4 ? 4 : 16;
 }
-constexpr int kSms = 148;
-int few_blocks(const AttnCall& a) { return few_takes_mma(a) || a.d > 128 ? kSms : 2 * kSms; }
+int few_blocks(const AttnCall& a) { return (few_takes_mma(a) ? few_rows(a) > 16 : a.d > 128) ? kSms : 2 * kSms; }
 
 struct DecPlan {
     size_t part, spans, bytes;
@@ -905,7 +918,7 @@ tl_status launch_mma(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
         !make_head_map(&mv, a.v, a.dtype, a.b, a.hkv, a.nk, a.d, DmSmem<DP, MT>::DT))
         return fail(c, TL_ERR_CUDA, "attention: tensor maps");
     c->flags_armed = true;
-    TL_CK(c, launch_cluster(k_decode_mma<T, DP, MT>, g.blocks, g.cluster, DM_THREADS, smem, s, mk, mv, g));
+    TL_CK(c, launch_cluster(k_decode_mma<T, DP, MT>, g.blocks, g.cluster, DmSmem<DP, MT>::THREADS, smem, s, mk, mv, g));
     return TL_OK;
 }
 
