@@ -46,10 +46,12 @@ R entry(tl_ctx* c, R oom, F f) {
 // *capturing: the stream is in capture, where a stream's device may not be
 // asked for (a launch on a stream of another device fails by itself).
 tl_status check_stream(tl_ctx* c, cudaStream_t s, bool* capturing) {
+    *capturing = false;
+    if (!s || s == cudaStreamLegacy) return TL_OK;   // the current device's, never in capture
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     TL_CK(c, cudaStreamIsCapturing(s, &cap));
     *capturing = cap != cudaStreamCaptureStatusNone;
-    if (*capturing || !s || s == cudaStreamLegacy || s == cudaStreamPerThread) return TL_OK;   // the current device's
+    if (*capturing || s == cudaStreamPerThread) return TL_OK;
     int dev = -1;
     TL_CK(c, cudaStreamGetDevice(s, &dev));
     if (dev != c->device) return fail(c, TL_ERR_INVALID, "the stream belongs to device %d, the context to %d", dev, c->device);

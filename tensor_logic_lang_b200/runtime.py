@@ -22,8 +22,10 @@ _TYPES = {"torch.float32": abi.TL_TYPE_F32, "torch.float16": abi.TL_TYPE_F16, "t
           "float32": abi.TL_TYPE_F32, "float16": abi.TL_TYPE_F16, "bfloat16": abi.TL_TYPE_BF16}
 _type_of = {}          # dtype object -> TL_TYPE_*
 _DATA, _NUMEL, _DEVICE, _IS_CONTIGUOUS = (methodcaller(n) for n in ("data_ptr", "numel", "get_device", "is_contiguous"))
-_ATTENTION_AT = {n: getattr(abi.Attention, n).offset for n, _ in abi.Attention._fields_}
-_ATTENTION_TAIL = struct.Struct("=QffiiQQQQQQQqQ")   # lse .. stream
+# tl_attention: eight tl_array, then lse .. stream
+_ATTENTION = struct.Struct("=" + "Qii4q4q" * 8 + "QffiiQQQQQQQqQ")
+_NO_GRADS = (0,) * (11 * 4)
+_PAD = [(0,) * (abi.TL_ARRAY_RANK - r) for r in range(abi.TL_ARRAY_RANK + 1)]
 
 
 class Context:
@@ -203,21 +205,18 @@ class Context:
         if x.get_device() != self.device:
             raise abi.TLError(abi.TL_ERR_INVALID, f"{what} is on {x.device}, the context on cuda:{self.device}")
 
-    def _heads(self, buf, field, x, what, write=False):
-        """Packs [heads and positions] of rank 2 to 4 as [batch, heads, positions, head size]."""
+    def _heads(self, x, what, write=False):
+        """The fields of an array of rank 2 to 4 as [batch, heads, positions, head size]."""
         p, t, shape, strides = self._view(x, what, write)
         r = len(shape)
         if r != 4:
             if r < 2 or r > 4:
                 raise abi.TLError(abi.TL_ERR_INVALID, f"attention: {what} has rank {r}, not 2 to 4")
             shape, strides = (1,) * (4 - r) + tuple(shape), (0,) * (4 - r) + tuple(strides)
-        _ARRAY.pack_into(buf, _ATTENTION_AT[field], p, t, 4, *shape, *strides)
-        return shape
+        return (p, t, 4, *shape, *strides)
 
     def _plain(self, x, what, kind, shape):
-        """Address of a contiguous device array of one type and shape (0 for None)."""
-        if x is None:
-            return 0
+        """Address of a contiguous device array of one type and shape."""
         if isinstance(x, str):
             if kind != "float32":
                 raise abi.TLError(abi.TL_ERR_INVALID, f"{what} is an array of {kind}, not a tensor's name")
@@ -252,26 +251,24 @@ class Context:
 
     def _attention(self, q, k, v, out, lse, grads, scale, softcap, slopes, causal, prefix_len, q_doc, k_doc, kv_len,
                    q_start, workspace, stream, writes_out):
-        buf = bytearray(C.sizeof(abi.Attention))
-        b, hq, nq, d = self._heads(buf, "q", q, "q")
-        nk = self._heads(buf, "k", k, "k")[2]
-        self._heads(buf, "v", v, "v")
-        self._heads(buf, "o", out, "out", writes_out)
+        qa, ka, va, oa = self._heads(q, "q"), self._heads(k, "k"), self._heads(v, "v"), self._heads(out, "out", writes_out)
+        b, hq, nq, d = qa[3:7]
+        nk = ka[5]
+        ga = _NO_GRADS
         if grads:
-            for f, x in zip(("dout", "dq", "dk", "dv"), grads):
-                self._heads(buf, f, x, f, f != "dout")
-        room = self._room(workspace)
-        one = (b,)
+            ga = sum((self._heads(x, n, n != "dout") for x, n in zip(grads, ("dout", "dq", "dk", "dv"))), ())
         if scale is None:
             scale = d ** -0.5 if d else 1.0
-        _ATTENTION_TAIL.pack_into(
-            buf, _ATTENTION_AT["lse"], self._plain(lse, "lse", "float32", (b, hq, nq)),
-            scale, softcap, 1 if causal else 0, 0,
-            self._plain(slopes, "slopes", "float32", (hq,)), self._plain(prefix_len, "prefix_len", "int32", one),
-            self._plain(q_doc, "q_doc", "int32", (b, nq)), self._plain(k_doc, "k_doc", "int32", (b, nk)),
-            self._plain(kv_len, "kv_len", "int32", one), self._plain(q_start, "q_start", "int32", one),
-            *room, self._stream(stream))
-        return (C.c_char * len(buf)).from_buffer(buf)
+        ws, room = self._room(workspace)
+        plain, one = self._plain, (b,)
+        return _ATTENTION.pack(
+            *qa, *ka, *va, *oa, *ga, lse is not None and plain(lse, "lse", "float32", (b, hq, nq)), scale, softcap,
+            1 if causal else 0, 0, slopes is not None and plain(slopes, "slopes", "float32", (hq,)),
+            prefix_len is not None and plain(prefix_len, "prefix_len", "int32", one),
+            q_doc is not None and plain(q_doc, "q_doc", "int32", (b, nq)),
+            k_doc is not None and plain(k_doc, "k_doc", "int32", (b, nk)),
+            kv_len is not None and plain(kv_len, "kv_len", "int32", one),
+            q_start is not None and plain(q_start, "q_start", "int32", one), ws, room, self._stream(stream))
 
     def attention(self, q, k, v, out, lse=None, *, scale=None, softcap=0.0, slopes=None, causal=False, prefix_len=None,
                   q_doc=None, k_doc=None, kv_len=None, q_start=None, workspace=None, stream=None):
@@ -309,30 +306,31 @@ class Context:
 
     def _list(self, arrays, what, write):
         """Packs arrays as tl_array (a contiguous one as its elements in a row)."""
-        out = np.zeros(len(arrays), _LIST)
-        if not any(isinstance(x, str) for x in arrays) and all(map(_IS_CONTIGUOUS, arrays)):
-            # a column at a time: lists are long
+        n = len(arrays)
+        if n > 16 and not any(isinstance(x, str) for x in arrays) and all(map(_IS_CONTIGUOUS, arrays)):
+            # long lists a column at a time
             for d in set(map(_DEVICE, arrays)) - {self.device}:
                 raise abi.TLError(abi.TL_ERR_INVALID, f"{what} on device {d}, the context on cuda:{self.device}")
             types = [x.dtype for x in arrays]
             for t in set(types) - _type_of.keys():
                 self._type(t, what)
-            n = len(arrays)
+            out = np.zeros(n, _LIST)
             out["data"] = np.fromiter(map(_DATA, arrays), np.uint64, n)
             out["dtype"] = [_type_of[t] for t in types]
             out["rank"] = 1
             out["dims"][:, 0] = np.fromiter(map(_NUMEL, arrays), np.int64, n)
             out["strides"][:, 0] = 1
-            return out
-        for a, x in zip(out, arrays):
+            return out.tobytes()
+        parts = []
+        for x in arrays:
             p, t, shape, strides = self._view(x, what, write)
             r = len(shape)
             if r > abi.TL_ARRAY_RANK:
                 if not x.is_contiguous():
                     raise abi.TLError(abi.TL_ERR_INVALID, f"{what}: rank {r} and not contiguous")
                 shape, strides, r = (x.numel(),), (1,), 1
-            a["data"], a["dtype"], a["rank"], a["dims"][:r], a["strides"][:r] = p, t, r, shape, strides
-        return out
+            parts.append(_ARRAY.pack(p, t, r, *shape, *_PAD[r], *strides, *_PAD[r]))
+        return b"".join(parts)
 
     def _clip_lists(self, grads, out):
         if out is not None and len(out) != len(grads):
@@ -346,15 +344,15 @@ class Context:
         receives the norm before the scaling.  Nothing is copied to the host.
         """
         a, o = self._clip_lists(grads, out)
-        at = self._plain(norm, "norm", "float32", ())
-        self.check(self.lib.tl_clip_gradients(self.h, a.ctypes.data, o if o is None else o.ctypes.data, len(grads), max_norm,
+        at = None if norm is None else self._plain(norm, "norm", "float32", ())
+        self.check(self.lib.tl_clip_gradients(self.h, a, o, len(grads), max_norm,
                                               at, *self._room(workspace), self._stream(stream)), "clip_gradients")
         return grads if out is None else out
 
     def clip_workspace(self, grads, max_norm, out=None):
         """Bytes of workspace of a clip_gradients call."""
         a, o = self._clip_lists(grads, out)
-        n = self.lib.tl_clip_workspace(self.h, a.ctypes.data, o if o is None else o.ctypes.data, len(grads), max_norm)
+        n = self.lib.tl_clip_workspace(self.h, a, o, len(grads), max_norm)
         self.check(max(0, -n), "clip_workspace")
         return n
 
