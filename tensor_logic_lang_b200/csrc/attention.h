@@ -74,40 +74,36 @@ tl_status kernel_smem(tl_ctx* c, F* kernel, int bytes, std::atomic<uint64_t>& do
     return TL_OK;
 }
 
-// A launch whose blocks may start when every block of the kernel before it in
-// the stream has said griddepcontrol.launch_dependents; they wait for its
-// results with griddepcontrol.wait.
+// A launch in clusters of `cluster` blocks along x.  early: its blocks may start
+// when every block of the kernel before it in the stream has said
+// griddepcontrol.launch_dependents or ended; they wait for its results with
+// griddepcontrol.wait.
 template <typename... P, typename... A>
-cudaError_t launch_early(void (*kernel)(P...), unsigned grid, int threads, int smem, cudaStream_t s, const A&... args) {
+cudaError_t launch_with(void (*kernel)(P...), dim3 grid, int cluster, int threads, int smem, bool early, cudaStream_t s, const A&... args) {
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(grid);
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (early) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
-
-// A launch in clusters of `cluster` blocks along x.
-template <typename... P, typename... A>
-cudaError_t launch_cluster(void (*kernel)(P...), unsigned grid, int cluster, int threads, int smem, cudaStream_t s, const A&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 inline size_t type_size(int dtype) { return dtype == TL_TYPE_F32 ? 4 : 2; }
 

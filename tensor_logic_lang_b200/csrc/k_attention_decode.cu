@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_decode_join(const __grid_const
     const int64_t u0 = before + (int64_t)unit * n, u1 = u0 + n;
     const int first = (int)(u0 / per), last = n ? (int)((u1 - 1) / per) : first;
     if (n && first == last) return;   // one block wrote it
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    wait_for_previous();
     int i, h;
     unit_row(a, kvh, row, &i, &h);
     // a block's second piece is the one that starts inside it
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
     __shared__ int64_t red[L::THREADS / 32], found[2];
     const AttnCall& a = g.a;
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    let_next_start();
     if (threadIdx.x == 0) {
         for (int s = 0; s < L::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 4); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(DA_THREADS) k_decode_any(const __grid_constant
     __shared__ int64_t red[DA_THREADS / 32], found[2];
     const AttnCall& a = g.a;
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    let_next_start();
     PieceWalk walk = block_pieces<DA_THREADS / 32>(g, red, found);
     const int group = a.hq / a.hkv;
     constexpr int NC = DP >= 128 ? DP / 128 : 1, LANES = DP >= 128 ? 32 : DP / 4;
@@ -918,7 +918,7 @@ tl_status launch_mma(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
         !make_head_map(&mv, a.v, a.dtype, a.b, a.hkv, a.nk, a.d, DmSmem<DP, MT>::DT))
         return fail(c, TL_ERR_CUDA, "attention: tensor maps");
     c->flags_armed = true;
-    TL_CK(c, launch_cluster(k_decode_mma<T, DP, MT>, g.blocks, g.cluster, DmSmem<DP, MT>::THREADS, smem, s, mk, mv, g));
+    TL_CK(c, launch_with(k_decode_mma<T, DP, MT>, dim3(g.blocks), g.cluster, DmSmem<DP, MT>::THREADS, smem, false, s, mk, mv, g));
     return TL_OK;
 }
 
@@ -927,7 +927,7 @@ tl_status launch_any_as(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     constexpr int smem = DaSmem<DP, RB>::BYTES;
     TL_TRY(kernel_smem(c, k_decode_any<T, DP, RB, VEC>, smem, done));
-    TL_CK(c, launch_cluster(k_decode_any<T, DP, RB, VEC>, g.blocks, g.cluster, DA_THREADS, smem, s, g));
+    TL_CK(c, launch_with(k_decode_any<T, DP, RB, VEC>, dim3(g.blocks), g.cluster, DA_THREADS, smem, false, s, g));
     return TL_OK;
 }
 
@@ -1005,9 +1005,9 @@ tl_status launch_attn_few(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s
     launch_begin_on(c, s, "attention_decode_join", 0, 0, ev);
     cudaError_t e;
     switch (a.dtype) {
-    case TL_TYPE_F32: e = launch_early(k_decode_join<float>, (unsigned)((int64_t)a.b * a.hkv * rows), JOIN_THREADS, 0, s, g); break;
-    case TL_TYPE_F16: e = launch_early(k_decode_join<__half>, (unsigned)((int64_t)a.b * a.hkv * rows), JOIN_THREADS, 0, s, g); break;
-    default: e = launch_early(k_decode_join<__nv_bfloat16>, (unsigned)((int64_t)a.b * a.hkv * rows), JOIN_THREADS, 0, s, g);
+    case TL_TYPE_F32: e = launch_with(k_decode_join<float>, dim3((unsigned)((int64_t)a.b * a.hkv * rows)), 1, JOIN_THREADS, 0, true, s, g); break;
+    case TL_TYPE_F16: e = launch_with(k_decode_join<__half>, dim3((unsigned)((int64_t)a.b * a.hkv * rows)), 1, JOIN_THREADS, 0, true, s, g); break;
+    default: e = launch_with(k_decode_join<__nv_bfloat16>, dim3((unsigned)((int64_t)a.b * a.hkv * rows)), 1, JOIN_THREADS, 0, true, s, g);
     }
     TL_CK(c, e);
     return launch_end_on(c, s, ev);

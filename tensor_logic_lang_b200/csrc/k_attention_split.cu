@@ -30,6 +30,8 @@ __device__ __forceinline__ bool row_counts(const AttnCall& a, const SplitArray& 
 // A warp takes 8 rows, a lane columns 2 lane and 2 lane + 1.
 template <bool WRITE>
 __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs g) {
+    let_next_start();
+    if (WRITE) wait_for_previous();   // the largest values
     const AttnCall& a = g.a;
     const SplitArray& x = g.arr[blockIdx.y];
     const int blocks = (x.n + SP_ROWS - 1) / SP_ROWS;
@@ -124,7 +126,7 @@ tl_status launch_split(tl_ctx* c, const AttnCall& a, bool backward, uint8_t* ws,
     k_split<false><<<dim3((unsigned)grid, count), 256, 0, s>>>(g);
     TL_TRY(launch_end_on(c, s, ev));
     launch_begin_on(c, s, "attention_split", 8 * bytes, 0, ev);
-    k_split<true><<<dim3((unsigned)grid, count), 256, 0, s>>>(g);
+    TL_CK(c, launch_with(k_split<true>, dim3((unsigned)grid, count), 1, 256, 0, true, s, g));
     return launch_end_on(c, s, ev);
 }
 

@@ -64,6 +64,7 @@ struct FwSmem {
 // the smallest / largest document of each tile of 128 keys (queries), a warp per tile
 __global__ void __launch_bounds__(256) k_doc_ranges(const int32_t* __restrict__ doc, int n, int tiles, int64_t total,
                                                     DocRange* __restrict__ out) {
+    let_next_start();
     const int lane = threadIdx.x & 31;
     const int64_t t = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
     if (t >= total) return;
@@ -197,6 +198,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    wait_for_previous();   // the documents' ranges, the split operands
     DocRange mine = no_docs();
     if (qd) {
         const int r = threadIdx.x;
@@ -459,7 +461,9 @@ tl_status launch(tl_ctx* c, const HeadMap* m, const FwArgs& g, cudaStream_t s) {
     const int64_t grid = (int64_t)a.b * (g.pair_heads ? a.hq / 2 : a.hq) * ((a.nq + span - 1) / span);
     cudaEvent_t ev[2];
     launch_begin_on(c, s, "attention_tc", 0, 4.0 * a.d * attn_pairs(a), ev);
-    k_attn_tc<T, U, DP, CAP, BIAS, FIX><<<(unsigned)grid, FW_THREADS, smem, s>>>(m[0], m[1], m[2], g);
+    // early behind a kernel of this call
+    TL_CK(c, launch_with(k_attn_tc<T, U, DP, CAP, BIAS, FIX>, dim3((unsigned)grid), 1, FW_THREADS, smem, !std::is_same<T, U>::value || a.k_doc != nullptr, s,
+                         m[0], m[1], m[2], g));
     return launch_end_on(c, s, ev);
 }
 

@@ -79,37 +79,42 @@ __device__ __forceinline__ void dot8(const uint4& x, const uint4& y, float& xy, 
     }
 }
 
-// Blocks of a tile of 128 rows, 16 lanes a row, 8 rows of a half warp in
-// flight: first the query tiles, then (fp16) the key tiles' norms of v.
+// Blocks of half a tile, 16 lanes a row, 4 rows of a half warp in flight:
+// first the query tiles, then (fp16) the key tiles' norms of v.
 template <typename T>
 __global__ void __launch_bounds__(256)
     k_attn_prep(const __grid_constant__ AttnCall a, float* __restrict__ stats, uint32_t* __restrict__ norms, int q_tiles, int k_tiles) {
+    let_next_start();
+    constexpr int R = 4;
     const int half = threadIdx.x / 16, sub = threadIdx.x % 16, c0 = sub * 8;
-    int64_t blk = blockIdx.x;
+    int64_t blk = blockIdx.x / 2;
+    const int r0 = blockIdx.x % 2 * (TILE / 2) + half * R;
     const int64_t n_q = (int64_t)a.b * a.hq * q_tiles;
     float top = 0.f;
     const bool keys = blk >= n_q;
     int group_of;
+    uint4 x[R], y[R];
     if (!keys) {
-        const int qt = (int)(blk % q_tiles);
+        const int i0 = (int)(blk % q_tiles) * TILE + r0;
         const int h = (int)(blk / q_tiles % a.hq), b = (int)(blk / q_tiles / a.hq);
         group_of = b * a.hkv + h / (a.hq / a.hkv);
         const T* dout = static_cast<const T*>(a.dout.p) + b * a.dout.sb + h * a.dout.sh + c0;
         const T* o = static_cast<const T*>(a.o.p) + b * a.o.sb + h * a.o.sh + c0;
-        uint4 x[8], y[8];
-        bool on[8];
+        float lse = -INFINITY;   // of row sub, of the first R lanes
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int i = qt * TILE + half * 8 + k;
-            on[k] = i < a.nq && (!a.q_doc || a.q_doc[(int64_t)b * a.nq + i] >= 0);
+        for (int k = 0; k < R; ++k) {
+            const int64_t i = i0 + k;
+            const bool on = i < a.nq && (!a.q_doc || a.q_doc[(int64_t)b * a.nq + i] >= 0);
             x[k] = y[k] = make_uint4(0, 0, 0, 0);
-            if (on[k] && c0 < a.d) {
+            if (on && c0 < a.d) {
                 x[k] = *reinterpret_cast<const uint4*>(dout + i * a.dout.ss);
                 y[k] = *reinterpret_cast<const uint4*>(o + i * a.o.ss);
             }
+            if (on && sub == k) lse = a.lse[((int64_t)b * a.hq + h) * a.nq + i];
         }
+        float mine = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < R; ++k) {
             float xy = 0.f, xx = 0.f;
             dot8<T>(x[k], y[k], xy, xx);
 #pragma unroll
@@ -118,32 +123,30 @@ __global__ void __launch_bounds__(256)
                 xx += __shfl_xor_sync(0xffffffffu, xx, w);
             }
             top = fmaxf(top, xx);
-            if (sub == 0) {
-                const int r = half * 8 + k, i = qt * TILE + r;
-                float* st = stats + blk * 2 * TILE;
-                const float lse = on[k] ? a.lse[((int64_t)b * a.hq + h) * a.nq + i] : -INFINITY;
-                // a row that sees nothing has p = 2^-inf = 0 everywhere
-                st[r] = lse == -INFINITY ? -INFINITY : PLift<T>::log2 - lse * kLog2e;
-                st[TILE + r] = -xy;
-            }
+            if (sub == k) mine = xy;
+        }
+        if (sub < R) {
+            float* st = stats + blk * 2 * TILE + r0 + sub;
+            // a row that sees nothing has p = 2^-inf = 0 everywhere
+            st[0] = lse == -INFINITY ? -INFINITY : PLift<T>::log2 - lse * kLog2e;
+            st[TILE] = -mine;
         }
     } else {
         blk -= n_q;
-        const int kt = (int)(blk % k_tiles);
+        const int64_t j0 = (blk % k_tiles) * TILE + r0;
         const int h = (int)(blk / k_tiles % a.hkv), b = (int)(blk / k_tiles / a.hkv);
         group_of = b * a.hkv + h;
         const int kv = a.kv_len ? min(max(a.kv_len[b], 0), a.nk) : a.nk;
         const T* v = static_cast<const T*>(a.v.p) + b * a.v.sb + h * a.v.sh + c0;
-        uint4 x[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int j = kt * TILE + half * 8 + k;
+        for (int k = 0; k < R; ++k) {
+            const int64_t j = j0 + k;
             x[k] = make_uint4(0, 0, 0, 0);
             if (j < kv && (!a.k_doc || a.k_doc[(int64_t)b * a.nk + j] >= 0) && c0 < a.d)
                 x[k] = *reinterpret_cast<const uint4*>(v + j * a.v.ss);
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < R; ++k) {
             float xy = 0.f, xx = 0.f;
             dot8<T>(x[k], x[k], xy, xx);
 #pragma unroll
@@ -161,6 +164,8 @@ __global__ void __launch_bounds__(256)
 // The statistics of fp32 arrays of any layout: a warp takes 8 rows, a lane
 // columns 2 lane and 2 lane + 1 (head size up to 64).
 __global__ void __launch_bounds__(256) k_attn_prep_f32(const __grid_constant__ AttnCall a, float* __restrict__ stats, int q_tiles) {
+    let_next_start();
+    wait_for_previous();   // the split operands, which the kernel behind this one reads
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, c = 2 * lane;
     const int64_t blk = blockIdx.x / 2;   // half a tile a block
     const int qt = (int)(blk % q_tiles), h = (int)(blk / q_tiles % a.hq), b = (int)(blk / q_tiles / a.hq);
@@ -292,7 +297,7 @@ struct BwBlock {
         docs = reinterpret_cast<int*>(docs_at);
     }
     // returns the TMEM base; `doc`: documents of the block's rows, or null
-    __device__ __forceinline__ uint32_t setup(const int32_t* doc, int rows, DocRange* mine) {
+    __device__ __forceinline__ uint32_t setup(const int32_t* doc, int rows, DocRange* mine, bool wait) {
         const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
         if (threadIdx.x == 0) {
             mbar_init(fix, 1);
@@ -309,6 +314,7 @@ struct BwBlock {
         tc_fence_before();
         __syncthreads();
         tc_fence_after();
+        if (wait) wait_for_previous();   // the statistics, the documents' ranges, the split operands
         *mine = no_docs();
         if (doc) {
             const int r = threadIdx.x;
@@ -379,7 +385,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     const int32_t* kd = a.k_doc ? a.k_doc + (int64_t)b * a.nk : nullptr;
     BwBlock bb(smem + L::BAR, smem + L::DOCS);
     DocRange mine;
-    const uint32_t tmem = bb.setup(kd ? kd + j0 : nullptr, min(TILE, a.nk - j0), &mine);
+    const uint32_t tmem = bb.setup(kd ? kd + j0 : nullptr, min(TILE, a.nk - j0), &mine, true);
+    // the dq kernel may start on the SMs that this one leaves: what it reads is there
+    let_next_start();
     const uint32_t t_s = tmem, t_dp = tmem + TILE, t_dv = tmem + 2 * TILE, t_dk = tmem + 2 * TILE + DO;
     const uint32_t t_dva = tmem + 3 * TILE, t_dka = t_dva + 64;   // split operands: the sums over the tiles
 
@@ -665,7 +673,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     const int32_t* kd = a.k_doc ? a.k_doc + (int64_t)b * a.nk : nullptr;
     BwBlock bb(smem + L::BAR, smem + L::DOCS);
     DocRange mine;
-    const uint32_t tmem = bb.setup(qd ? qd + i0 : nullptr, rows, &mine);
+    const uint32_t tmem = bb.setup(qd ? qd + i0 : nullptr, rows, &mine, false);
     const uint32_t t_dp = tmem + 2 * TILE, t_dq = tmem + 3 * TILE;
     const uint32_t t_dqa = t_dq + 64;   // split operands: the sum over the tiles
     TileWalk walk;
@@ -834,6 +842,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             store_row<U, PART>(v, b, h, i, i < a.nq, a.d - wg * PART, at, any, any, mul);
         }
     }
+    wait_for_previous();   // the dk, dv kernel, which this one did not need, so that its end is the call's
     bb.finish(tmem);
 }
 
@@ -862,11 +871,12 @@ tl_status launch(tl_ctx* c, const HeadMap* m, const BwArgs& g, cudaStream_t s) {
     const AttnCall& a = g.a;
     cudaEvent_t ev[2];
     launch_begin_on(c, s, "attention_tc_dkv", 0, 8.0 * a.d * attn_pairs(a), ev);
-    TL_CK(c, launch_cluster(k_attn_tc_dkv<T, U, DP, CAP, BIAS>, (unsigned)((int64_t)g.k_tiles * a.b * a.hkv * g.cluster), g.cluster,
-                            BW_THREADS, smem, s, m[0], m[1], m[2], m[3], g));
+    TL_CK(c, launch_with(k_attn_tc_dkv<T, U, DP, CAP, BIAS>, dim3((unsigned)((int64_t)g.k_tiles * a.b * a.hkv * g.cluster)), g.cluster,
+                         BW_THREADS, smem, true, s, m[0], m[1], m[2], m[3], g));
     TL_TRY(launch_end_on(c, s, ev));
     launch_begin_on(c, s, "attention_tc_dq", 0, 6.0 * a.d * attn_pairs(a), ev);
-    k_attn_tc_dq<T, U, DP, CAP, BIAS><<<(unsigned)((int64_t)g.q_tiles * a.b * a.hq), BW_THREADS, smem, s>>>(m[0], m[1], m[2], m[3], g);
+    TL_CK(c, launch_with(k_attn_tc_dq<T, U, DP, CAP, BIAS>, dim3((unsigned)((int64_t)g.q_tiles * a.b * a.hq)), 1, BW_THREADS, smem, true, s,
+                         m[0], m[1], m[2], m[3], g));
     return launch_end_on(c, s, ev);
 }
 
@@ -902,7 +912,13 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
     g.q_tiles = plan.q_tiles;
     g.k_tiles = plan.k_tiles;
     const int group = a.hq / a.hkv;
-    g.cluster = group % 8 == 0 ? 8 : group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+    // clusters of two, larger ones only where that gives the GPU its blocks: a
+    // cluster waits for as many free SMs of one GPC (2 x 2048 x 16 heads over 4:
+    // clusters of 1, 2, 4 took 185, 109, 138 us; 8 x 512 x 16 over 2: 74, 45, 68)
+    g.cluster = group % 2 ? 1 : 2;
+    while (g.cluster > 1 && g.cluster < 8 && group % (2 * g.cluster) == 0 &&
+           (int64_t)plan.k_tiles * a.b * a.hkv * g.cluster < c->sm_count * 2 / 3)
+        g.cluster *= 2;
     g.err = c->d_flags + 8;
     c->flags_armed = true;
     if (a.q_doc) {
@@ -923,7 +939,7 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
         g.tops.v = g.tops.k + (size_t)a.b * a.hkv;
         g.tops.dout = g.tops.v + (size_t)a.b * a.hkv;
         launch_begin_on(c, s, "attention_prep", 8.0 * rows * a.d, 2.0 * rows * a.d, ev);
-        k_attn_prep_f32<<<(unsigned)(2 * tiles), 256, 0, s>>>(a, stats, plan.q_tiles);
+        TL_CK(c, launch_with(k_attn_prep_f32, dim3((unsigned)(2 * tiles)), 1, 256, 0, true, s, a, stats, plan.q_tiles));
         TL_TRY(launch_end_on(c, s, ev));
         return launch_scores<__half, float, 128>(c, m, g, s);
     }
@@ -934,8 +950,8 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
     if (norms) TL_CK(c, cudaMemsetAsync(norms, 0, (size_t)a.b * a.hkv * 8, s));
     const int64_t blocks = tiles + (norms ? (int64_t)a.b * a.hkv * plan.k_tiles : 0);
     launch_begin_on(c, s, "attention_prep", 4.0 * rows * a.d, 2.0 * rows * a.d, ev);
-    if (a.dtype == TL_TYPE_F16) k_attn_prep<__half><<<(unsigned)blocks, 256, 0, s>>>(a, stats, norms, plan.q_tiles, plan.k_tiles);
-    else k_attn_prep<__nv_bfloat16><<<(unsigned)blocks, 256, 0, s>>>(a, stats, norms, plan.q_tiles, plan.k_tiles);
+    if (a.dtype == TL_TYPE_F16) k_attn_prep<__half><<<(unsigned)(2 * blocks), 256, 0, s>>>(a, stats, norms, plan.q_tiles, plan.k_tiles);
+    else k_attn_prep<__nv_bfloat16><<<(unsigned)(2 * blocks), 256, 0, s>>>(a, stats, norms, plan.q_tiles, plan.k_tiles);
     TL_TRY(launch_end_on(c, s, ev));
     if (a.dtype == TL_TYPE_F16)
         return a.d <= 64 ? launch_scores<__half, __half, 64>(c, m, g, s) : launch_scores<__half, __half, 128>(c, m, g, s);

@@ -167,7 +167,7 @@ __device__ __forceinline__ double chunk_squares(const T* p, int64_t n) {
 template <int CAP>
 __global__ void __launch_bounds__(CL_THREADS) k_clip_norm(const __grid_constant__ ClipList<CAP> list, double* __restrict__ part) {
     __shared__ double red[CL_THREADS / 32];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    let_next_start();
     __shared__ __align__(16) Index<CAP> index;
     index.fill(list);
     double s = 0;
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(CL_THREADS)
     __shared__ double red[CL_THREADS / 32];
     __shared__ __align__(16) Index<CAP> index;
     index.fill(list);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    wait_for_previous();
     double s = 0;
     for (int i = threadIdx.x; i < n_part; i += CL_THREADS) s += part[i];
     const double norm = sqrt(block_sum(s, red));
@@ -320,7 +320,7 @@ tl_status clip(tl_ctx* c, const std::vector<ClipItem>& items, double max_norm, f
         if (lists[i].chunks > CL_MAX_BLOCKS) grid[i] = (grid[i] + 1) / 2;
         launch_begin_on(c, s, "clip_scale", (bytes + wrote) / lists.size(), 0, ev);
         if (lists.size() == 1) {
-            TL_CK(c, launch_early(k_clip_scale<CAP>, grid[i], CL_THREADS, 0, s, lists[i], static_cast<const double*>(part), n_part,
+            TL_CK(c, launch_with(k_clip_scale<CAP>, dim3(grid[i]), 1, CL_THREADS, 0, true, s, lists[i], static_cast<const double*>(part), n_part,
                                   max_norm, norm));
         } else {
             k_clip_scale<CAP><<<grid[i], CL_THREADS, 0, s>>>(lists[i], part, n_part, max_norm, i == 0 ? norm : nullptr);
