@@ -117,8 +117,7 @@ size_t attn_general_workspace(const AttnCall& a, bool backward);
 tl_status launch_attn_general(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s);
 tl_status launch_attn_general_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s);
 
-// k_attention_tc.cu: 16-bit types with aligned rows, head size up to 128; fp32
-// of head size up to 64
+// k_attention_tc.cu: 16-bit types with aligned rows, and fp32, of head size up to 128
 bool attn_tc_takes(const AttnCall& a);
 size_t attn_tc_workspace(const AttnCall& a);
 tl_status launch_attn_tc(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s);

@@ -176,11 +176,12 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, int
 // product, is left out.  The small products go first: the tensor cores cut
 // their fp32 sums (2^-23 of the sum a step), so the large sum should see few
 // steps.
-template <typename T>
+// MORE: added to D.
+template <typename T, bool MORE = false>
 __device__ __forceinline__ void mma_rows_split(uint32_t d, uint32_t a, uint32_t b, int ksteps) {
     constexpr uint32_t idesc = f16_idesc<T>(TILE, false), low = CHUNK_BYTES >> 4;
     const uint32_t da = desc_rows(a), db = desc_rows(b);
-    umma_f16_ss<false>(d, da + low, db, idesc);
+    umma_f16_ss<MORE>(d, da + low, db, idesc);
     if (ksteps == 4) {
 #pragma unroll
         for (int k = 1; k < 4; ++k) umma_f16_ss<true>(d, da + low + 2 * k, db + 2 * k, idesc);
@@ -206,17 +207,17 @@ __device__ __forceinline__ void mma_parts(uint32_t d, uint32_t a, uint32_t b, ui
 #pragma unroll
     for (int k = 1; k < TILE / 16; ++k) umma_f16_ts(d, a + part_col<W>(k), db + k * (2048 >> 4), idesc, 1);
 }
-// D = A B anew for split operands (the caller adds the tiles up in fp32): in
-// each part's W TMEM columns W / 2 of hi, W / 2 of lo.
+// The same for split operands (the caller adds the tiles up in fp32): in each
+// part's W TMEM columns W / 2 of hi, W / 2 of lo.
 template <int W>
-__device__ __forceinline__ void mma_parts_split(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+__device__ __forceinline__ void mma_parts_split(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     const uint32_t db = desc_cols(b);
 #pragma unroll
     for (int part = 0; part < 3; ++part)
 #pragma unroll
         for (int k = 0; k < TILE / 16; ++k)
             umma_f16_ts(d, a + part_col<W>(k) + (part == 0 ? W / 2 : 0), db + (part == 1 ? CHUNK_BYTES >> 4 : 0) + k * (2048 >> 4), idesc,
-                        part > 0 || k > 0);
+                        part > 0 || k > 0 ? 1u : accumulate);
 }
 // N columns of the warp's lanes
 template <int N>
@@ -305,12 +306,12 @@ struct HeadMap {
     CUtensorMap map;
     int mh, mb;   // 1, or 0 where every head (sequence) is the same memory
 };
-__device__ __forceinline__ void tma_tile(uint32_t dst, const HeadMap& m, uint64_t* bar, int chunks, int row, int h, int b) {
+__device__ __forceinline__ void tma_tile(uint32_t dst, const HeadMap& m, uint64_t* bar, int chunks, int row, int h, int b, int first = 0) {
     for (int c = 0; c < chunks; ++c)
         asm volatile(
             "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
             ::"r"(dst + c * CHUNK_BYTES),
-            "l"(reinterpret_cast<uint64_t>(&m.map)), "r"(smem_u32(bar)), "r"(64 * c), "r"(row), "r"(h * m.mh), "r"(b * m.mb)
+            "l"(reinterpret_cast<uint64_t>(&m.map)), "r"(smem_u32(bar)), "r"(64 * (first + c)), "r"(row), "r"(h * m.mh), "r"(b * m.mb)
             : "memory");
 }
 
@@ -491,8 +492,10 @@ bool tc_array(const HeadsView& v, int b, int h, int64_t n);
 // in 2^14 .. 2^15) is hi + lo, two fp16 numbers of 11 bits: 22 bits of it, or 2^-25
 // where that is more, which is 2^-39 of the largest.  One array:
 // [b, h, n, 128] fp16, columns 0..63 hi, 64..127 lo, zeros past the head size and in
-// rows that must not count.
-constexpr int kSplitMaxHead = 64;
+// rows that must not count; head sizes above 64 have two such halves behind one
+// another, [b, h, n, 256].
+constexpr int kSplitMaxHead = 128;
+inline int split_width(int d) { return d <= 64 ? 128 : 256; }
 struct SplitArray {
     HeadsView v;
     int h, n;

@@ -27,8 +27,8 @@ __device__ __forceinline__ bool row_counts(const AttnCall& a, const SplitArray& 
     return r < kv && (!a.k_doc || a.k_doc[(int64_t)b * a.nk + r] >= 0);
 }
 
-// A warp takes 8 rows, a lane columns 2 lane and 2 lane + 1.
-template <bool WRITE>
+// A warp takes 8 rows, a lane columns 2 lane and 2 lane + 1 of every 64.
+template <bool WRITE, int HALVES>
 __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs g) {
     let_next_start();
     if (WRITE) wait_for_previous();   // the largest values
@@ -41,30 +41,41 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, c = 2 * lane;
     const int64_t r0 = (int64_t)(blockIdx.x % blocks) * SP_ROWS + warp * 8;
     const float* p = static_cast<const float*>(x.v.p) + b * x.v.sb + h * x.v.sh;
-    float u[8], w[8];
+    float u[8][HALVES], w[8][HALVES];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         const bool on = row_counts(a, x, b, r0 + k);
-        u[k] = on && c < a.d ? p[(r0 + k) * x.v.ss + c * x.v.sd] : 0.f;
-        w[k] = on && c + 1 < a.d ? p[(r0 + k) * x.v.ss + (c + 1) * x.v.sd] : 0.f;
+#pragma unroll
+        for (int f = 0; f < HALVES; ++f) {
+            const int col = c + 64 * f;
+            u[k][f] = on && col < a.d ? p[(r0 + k) * x.v.ss + col * x.v.sd] : 0.f;
+            w[k][f] = on && col + 1 < a.d ? p[(r0 + k) * x.v.ss + (col + 1) * x.v.sd] : 0.f;
+        }
     }
     if (WRITE) {
         const float up = exp2f((float)split_exp(x.top, group));
-        __half* out = x.out + ((int64_t)bh * x.n + r0) * 128 + c;
+        __half* out = x.out + ((int64_t)bh * x.n + r0) * (128 * HALVES) + c;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             if (r0 + k >= x.n) break;
-            uint32_t hi, lo;
-            split16(u[k] * up, w[k] * up, hi, lo);
-            *reinterpret_cast<uint32_t*>(out + k * 128) = hi;
-            *reinterpret_cast<uint32_t*>(out + k * 128 + 64) = lo;
+#pragma unroll
+            for (int f = 0; f < HALVES; ++f) {
+                uint32_t hi, lo;
+                split16(u[k][f] * up, w[k][f] * up, hi, lo);
+                *reinterpret_cast<uint32_t*>(out + (k * HALVES + f) * 128) = hi;
+                *reinterpret_cast<uint32_t*>(out + (k * HALVES + f) * 128 + 64) = lo;
+            }
         }
     } else {
         float top = 0.f, norm = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            top = fmaxf(top, fmaxf(fabsf(u[k]), fabsf(w[k])));
-            float n2 = fmaf(u[k], u[k], w[k] * w[k]);
+            float n2 = 0.f;
+#pragma unroll
+            for (int f = 0; f < HALVES; ++f) {
+                top = fmaxf(top, fmaxf(fabsf(u[k][f]), fabsf(w[k][f])));
+                n2 = fmaf(u[k][f], u[k][f], fmaf(w[k][f], w[k][f], n2));
+            }
             if (x.norm >= 0) {
 #pragma unroll
                 for (int o = 16; o; o >>= 1) n2 += __shfl_xor_sync(0xffffffffu, n2, o);
@@ -89,7 +100,7 @@ SplitPlan::SplitPlan(const AttnCall& a, bool backward) {
     const size_t groups = (size_t)a.b * a.hkv;
     top = take(groups * (4 * 4 + 8));
     norms = top + groups * 4 * 4;
-    const size_t q = (size_t)a.b * a.hq * a.nq * 256, k = (size_t)a.b * a.hkv * a.nk * 256;
+    const size_t row = 2 * (size_t)split_width(a.d), q = row * a.b * a.hq * a.nq, k = row * a.b * a.hkv * a.nk;
     data[0] = take(q);
     data[1] = take(k);
     data[2] = take(k);
@@ -116,17 +127,19 @@ tl_status launch_split(tl_ctx* c, const AttnCall& a, bool backward, uint8_t* ws,
         x.top = top;
         top += (size_t)a.b * a.hkv;
         grid = std::max<int64_t>(grid, (int64_t)a.b * x.h * ((x.n + SP_ROWS - 1) / SP_ROWS));
-        const HeadsView flat = {x.out, (int64_t)x.h * x.n * 128, (int64_t)x.n * 128, 128, 1};
-        if (!make_head_map(&maps[i], flat, TL_TYPE_F16, a.b, x.h, x.n, 128)) return fail(c, TL_ERR_CUDA, "attention: tensor maps");
+        const int64_t w = split_width(a.d);
+        const HeadsView flat = {x.out, x.h * x.n * w, x.n * w, w, 1};
+        if (!make_head_map(&maps[i], flat, TL_TYPE_F16, a.b, x.h, x.n, (int)w)) return fail(c, TL_ERR_CUDA, "attention: tensor maps");
     }
     TL_CK(c, cudaMemsetAsync(ws + plan.top, 0, (size_t)a.b * a.hkv * (4 * 4 + 8), s));
     const double bytes = (double)a.b * a.d * ((double)(backward ? 2 : 1) * a.hq * a.nq + 2.0 * a.hkv * a.nk);
     cudaEvent_t ev[2];
     launch_begin_on(c, s, "attention_split_top", 4 * bytes, 0, ev);
-    k_split<false><<<dim3((unsigned)grid, count), 256, 0, s>>>(g);
+    const bool wide = a.d > 64;
+    TL_CK(c, launch_with(wide ? k_split<false, 2> : k_split<false, 1>, dim3((unsigned)grid, count), 1, 256, 0, false, s, g));
     TL_TRY(launch_end_on(c, s, ev));
     launch_begin_on(c, s, "attention_split", 8 * bytes, 0, ev);
-    TL_CK(c, launch_with(k_split<true>, dim3((unsigned)grid, count), 1, 256, 0, true, s, g));
+    TL_CK(c, launch_with(wide ? k_split<true, 2> : k_split<true, 1>, dim3((unsigned)grid, count), 1, 256, 0, true, s, g));
     return launch_end_on(c, s, ev);
 }
 

@@ -144,15 +144,16 @@ __device__ __forceinline__ float score_row(f2 (&x)[32], float c1, const CapCoef<
     return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
 
-// T: operands, U: the arrays' type (float: split operands, DP = 128 columns of
-// hi and lo).  FIX: see fixed_top.
+// T: operands, U: the arrays' type (float: split operands, DP = 128 or 256 columns
+// of hi and lo).  FIX: see fixed_top.
 template <typename T, typename U, int DP, bool CAP, bool BIAS, bool FIX>
 __global__ void __launch_bounds__(FW_THREADS, 1)
     k_attn_tc(const __grid_constant__ HeadMap mq, const __grid_constant__ HeadMap mk, const __grid_constant__ HeadMap mv,
               const __grid_constant__ FwArgs g) {
-    using L = FwSmem<DP>;
     constexpr bool SPLIT = !std::is_same<T, U>::value;
-    constexpr int DO = SPLIT ? 64 : DP;   // columns of O
+    constexpr int HALVES = DP > 128 ? 2 : 1;   // split operands of more than 64 columns: a tile is two, one behind the other
+    using L = FwSmem<DP / HALVES>;
+    constexpr int DO = SPLIT ? DP / 2 : DP;    // columns of O
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::BAR);
@@ -228,19 +229,21 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             int kt = walk.next(&masked);
             int n = 0;   // ring entries filled
             if (kt >= 0 && lane == 0) {
-                mbar_expect_tx(q_full, g.tiles * L::TILE_B);
+                mbar_expect_tx(q_full, g.tiles * HALVES * L::TILE_B);
                 for (int t = 0; t < g.tiles; ++t)
-                    tma_tile(smem_u32(smem + L::Q + t * L::TILE_B), mq, q_full, L::CH, i0 + (g.pair_heads ? 0 : t * TILE),
-                             h0 + (g.pair_heads ? t : 0), b);
+                    for (int f = 0; f < HALVES; ++f)
+                        tma_tile(smem_u32(smem + L::Q + (t * HALVES + f) * L::TILE_B), mq, q_full, L::CH,
+                                 i0 + (g.pair_heads ? 0 : t * TILE), h0 + (g.pair_heads ? t : 0), b, f * L::CH);
             }
             for (; kt >= 0 && ok; kt = walk.next(&masked)) {
-                for (int w = 0; w < 2 && ok; ++w, ++n) {
+                for (int w = 0; w < 2 * HALVES && ok; ++w, ++n) {
                     const int s = n % FW_STAGES;
                     ok = n < FW_STAGES || mbar_wait(&empty[s], ((n / FW_STAGES) & 1) ^ 1, g.err);
                     ok = __all_sync(0xffffffffu, ok);
                     if (ok && lane == 0) {
                         mbar_expect_tx(&full[s], L::TILE_B);
-                        tma_tile(smem_u32(smem + L::KV + s * L::TILE_B), w ? mv : mk, &full[s], L::CH, kt * TILE, kvh, b);
+                        tma_tile(smem_u32(smem + L::KV + s * L::TILE_B), w / HALVES ? mv : mk, &full[s], L::CH, kt * TILE, kvh, b,
+                                 w % HALVES * L::CH);
                     }
                 }
             }
@@ -257,29 +260,43 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 ok = __all_sync(0xffffffffu, ok);
                 tc_fence_after();
             };
-            auto scores = [&](int t, int stage) {
+            // the ring entry e's tile
+            auto entry = [&](int e) { return smem_u32(smem + L::KV + e % FW_STAGES * L::TILE_B); };
+            auto scores = [&](int t, int e) {
                 if (ok && elect_one()) {
-                    const uint32_t sq = smem_u32(smem + L::Q + t * L::TILE_B), sk = smem_u32(smem + L::KV + stage * L::TILE_B);
-                    if (SPLIT) mma_rows_split<T>(tmem + t * TILE, sq, sk, ksteps);
-                    else mma_rows<T, DP / 16>(tmem + t * TILE, sq, sk, ksteps);
+                    const uint32_t sq = smem_u32(smem + L::Q + t * HALVES * L::TILE_B);
+                    if (HALVES == 2) {
+                        mma_rows_split<T>(tmem + t * TILE, sq, entry(e), 4);
+                        mma_rows_split<T, true>(tmem + t * TILE, sq + L::TILE_B, entry(e + 1), ksteps - 4);
+                    } else if (SPLIT) {
+                        mma_rows_split<T>(tmem + t * TILE, sq, entry(e), ksteps);
+                    } else {
+                        mma_rows<T, DP / 16>(tmem + t * TILE, sq, entry(e), ksteps);
+                    }
                     umma_commit(&s_full[t]);
                 }
                 __syncwarp();
             };
+            auto free_entries = [&](int e) {   // by one lane
+                for (int f = 0; f < HALVES; ++f) umma_commit(&empty[(e + f) % FW_STAGES]);
+            };
+            auto wait_entries = [&](int e) {
+                for (int f = 0; f < HALVES; ++f) wait_full(full, e + f, FW_STAGES);
+            };
             if (kt >= 0) {
                 wait_full(q_full, 0, 1);
-                wait_full(full, n, FW_STAGES);
-                for (int t = 0; t < g.tiles; ++t) scores(t, n % FW_STAGES);
-                if (ok && elect_one()) umma_commit(&empty[n % FW_STAGES]);
-                ++n;
+                wait_entries(n);
+                for (int t = 0; t < g.tiles; ++t) scores(t, n);
+                if (ok && elect_one()) free_entries(n);
+                n += HALVES;
             }
             for (int it = 0; kt >= 0 && ok; ++it) {
-                const int vs = n % FW_STAGES;
-                wait_full(full, n, FW_STAGES);
-                ++n;
+                const int vs = n;   // V's entries
+                wait_entries(n);
+                n += HALVES;
                 // rows of V that must not count: 0 probability times what they hold could be NaN
                 if (!SPLIT && ok && ((kd && masked) || (mask.kv < a.nk && (kt + 1) * TILE > mask.kv))) {
-                    clear_rows(smem + L::KV + vs * L::TILE_B, L::CH, [&](int r) {
+                    clear_rows(smem + L::KV + vs % FW_STAGES * L::TILE_B, L::CH, [&](int r) {
                         const int j = kt * TILE + r;
                         return j >= mask.kv || (kd && kd[j] < 0);
                     });
@@ -288,28 +305,32 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 }
                 bool next_masked;
                 const int next = walk.next(&next_masked);
-                if (next >= 0) wait_full(full, n, FW_STAGES);   // the next keys: nothing waits between P V and S
+                if (next >= 0) wait_entries(n);   // the next keys: nothing waits between P V and S
                 for (int t = 0; t < g.tiles; ++t) {
                     ok = ok && mbar_wait(&p_full[t], it & 1, g.err);
                     ok = __all_sync(0xffffffffu, ok);
                     tc_fence_after();
                     if (ok && elect_one()) {
-                        const uint32_t to = tmem + 2 * TILE + t * DO, sv = smem_u32(smem + L::KV + vs * L::TILE_B);
-                        if (SPLIT) mma_parts_split<64>(to, tmem + t * TILE, sv, idesc_o);
-                        else mma_parts<64>(to, tmem + t * TILE, sv, idesc_o, it > 0);
+                        const uint32_t to = tmem + 2 * TILE + t * DO, tp = tmem + t * TILE;
+                        if (HALVES == 2) {
+                            mma_parts_split<64>(to, tp, entry(vs), f16_idesc<T>(64, true), 0);
+                            mma_parts_split<64>(to + 64, tp, entry(vs + 1), f16_idesc<T>(16 * (ksteps - 4), true), 0);
+                        } else if (SPLIT) {
+                            mma_parts_split<64>(to, tp, entry(vs), idesc_o, 0);
+                        } else {
+                            mma_parts<64>(to, tp, entry(vs), idesc_o, it > 0);
+                        }
                         if (next < 0) umma_commit(&o_done[t]);
                     }
                     __syncwarp();
-                    if (next >= 0) {
-                        scores(t, n % FW_STAGES);
-                    }
+                    if (next >= 0) scores(t, n);
                 }
                 if (ok && elect_one()) {
-                    umma_commit(&empty[vs]);
-                    if (next >= 0) umma_commit(&empty[n % FW_STAGES]);
+                    free_entries(vs);
+                    if (next >= 0) free_entries(n);
                 }
                 __syncwarp();
-                if (next >= 0) ++n;
+                if (next >= 0) n += HALVES;
                 kt = next;
                 masked = next_masked;
             }
@@ -454,7 +475,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
 template <typename T, typename U, int DP, bool CAP, bool BIAS, bool FIX = false>
 tl_status launch(tl_ctx* c, const HeadMap* m, const FwArgs& g, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
-    constexpr int smem = FwSmem<DP>::BYTES;
+    constexpr int smem = FwSmem<(DP > 128 ? 128 : DP)>::BYTES;
     TL_TRY(kernel_smem(c, k_attn_tc<T, U, DP, CAP, BIAS, FIX>, smem, done));
     const AttnCall& a = g.a;
     const int span = g.pair_heads ? TILE : g.tiles * TILE;
@@ -552,6 +573,11 @@ tl_status launch_attn_tc(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s)
         g.tops.k = g.tops.q + (size_t)a.b * a.hkv;
         g.tops.v = g.tops.k + (size_t)a.b * a.hkv;
         g.tops.dout = nullptr;
+        if (a.d > 64) {   // a query tile and its sums take what two of the smaller head size do
+            g.tiles = 1;
+            g.pair_heads = 0;
+            return launch_scores<__half, float, 256>(c, m, g, s);
+        }
         return launch_scores<__half, float, 128>(c, m, g, s);
     }
     g.tops = {nullptr, nullptr, nullptr, nullptr};

@@ -1,6 +1,5 @@
 // Attention backward on the tensor cores: 16-bit operands, head size up to
-// 128, or fp32 arrays of head size up to 64 as pairs of fp16 (attn_tc.h,
-// SplitArray).  With p = exp(s - lse), dp = dout v^T, D = dout . o by row,
+// 128, or fp32 arrays as pairs of fp16 (attn_tc.h, SplitArray).  With p = exp(s - lse), dp = dout v^T, D = dout . o by row,
 //   dx = p (dp - D) (1 - tanh^2),  dq = scale dx k,  dk = scale dx^T q,  dv = p^T dout
 // the scores are taken again from q and k (S is never stored), twice:
 //
@@ -28,7 +27,11 @@
 // of it), at 2^15: neither can overflow, and small gradients keep their bits.
 // fp32 arrays: p and dx are written as hi and lo, each product is three, and
 // the sums over the tiles are added by the rows' threads (the tensor cores cut
-// theirs, see k_attention_tc.cu).
+// theirs, see k_attention_tc.cu).  Of head sizes above 64 (WIDE) the resident
+// operands fill shared memory but for two tiles of 64 columns, so the passing
+// ones come in halves, each as often as a product needs it (twice, from the L2
+// cache), and dk and dv, which leave no room for sums in TMEM, are added to
+// the outputs every 4 tiles.
 #include <algorithm>
 
 #include "attn_tc.h"
@@ -56,13 +59,15 @@ struct BwArgs {
 
 template <int DP>
 struct BwSmem {
-    static constexpr int CH = DP / 64, TILE_B = CH * CHUNK_BYTES;
-    // two resident tiles, stages of two tiles and the statistics
-    static constexpr int FIX = 0, RING = 2 * TILE_B, STAT = RING + BW_STAGES * 2 * TILE_B, BAR = STAT + BW_STAGES * STAT_BYTES,
+    static constexpr bool WIDE = DP > 128;   // halves of 64 columns, hi and lo
+    static constexpr int CH = WIDE ? 2 : DP / 64, TILE_B = CH * CHUNK_BYTES;
+    // two resident tiles, stages of two tiles and the statistics; WIDE: four
+    // resident halves, a ring of two
+    static constexpr int FIX = 0, RING = (WIDE ? 4 : 2) * TILE_B, STAT = 6 * TILE_B, BAR = STAT + BW_STAGES * STAT_BYTES,
                          DOCS = BAR + 256, BYTES = DOCS + 64 + 1024;
     // the cluster's sums: dv and dk as fp32 rows padded by 16 bytes, over the tiles
     static constexpr int SUM_LD = DP + 4;
-    static_assert(2 * TILE * SUM_LD * 4 <= STAT, "the sums lie over the tiles");
+    static_assert(WIDE || 2 * TILE * SUM_LD * 4 <= STAT, "the sums lie over the tiles");
 };
 
 // ---------------------------------------------------------------- preparation
@@ -162,7 +167,7 @@ __global__ void __launch_bounds__(256)
 }
 
 // The statistics of fp32 arrays of any layout: a warp takes 8 rows, a lane
-// columns 2 lane and 2 lane + 1 (head size up to 64).
+// columns 2 lane and 2 lane + 1 of every 64.
 __global__ void __launch_bounds__(256) k_attn_prep_f32(const __grid_constant__ AttnCall a, float* __restrict__ stats, int q_tiles) {
     let_next_start();
     wait_for_previous();   // the split operands, which the kernel behind this one reads
@@ -177,8 +182,11 @@ __global__ void __launch_bounds__(256) k_attn_prep_f32(const __grid_constant__ A
     for (int k = 0; k < 8; ++k) {
         const int64_t i = qt * TILE + r0 + k;
         const bool on = i < a.nq && (!a.q_doc || a.q_doc[(int64_t)b * a.nq + i] >= 0);
-        dot[k] = on && c < a.d ? x[i * a.dout.ss + c * a.dout.sd] * y[i * a.o.ss + c * a.o.sd] : 0.f;
-        if (on && c + 1 < a.d) dot[k] = fmaf(x[i * a.dout.ss + (c + 1) * a.dout.sd], y[i * a.o.ss + (c + 1) * a.o.sd], dot[k]);
+        dot[k] = 0.f;
+        for (int e = c; on && e < a.d; e += 64) {
+            dot[k] = fmaf(x[i * a.dout.ss + e * a.dout.sd], y[i * a.o.ss + e * a.o.sd], dot[k]);
+            if (e + 1 < a.d) dot[k] = fmaf(x[i * a.dout.ss + (e + 1) * a.dout.sd], y[i * a.o.ss + (e + 1) * a.o.sd], dot[k]);
+        }
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -280,7 +288,7 @@ __device__ __forceinline__ void grad_dx(const f2 (&pb)[16], const uint32_t (&dp)
 
 // What the two gradient kernels share: barriers, TMEM, the documents of the block's rows.
 struct BwBlock {
-    uint64_t *fix, *full, *empty, *s_full, *p_full, *dp_full, *dx_full, *done;
+    uint64_t *fix, *full, *empty, *s_full, *p_full, *dp_full, *dx_full, *done, *stat_full;
     uint32_t* tmem_slot;
     int* docs;
     __device__ __forceinline__ BwBlock(uint8_t* bars, uint8_t* docs_at) {
@@ -293,6 +301,7 @@ struct BwBlock {
         dp_full = p_full + 1;
         dx_full = dp_full + 1;
         done = dx_full + 1;
+        stat_full = done + 1;         // two; WIDE
         tmem_slot = reinterpret_cast<uint32_t*>(bar + 24);
         docs = reinterpret_cast<int*>(docs_at);
     }
@@ -303,6 +312,7 @@ struct BwBlock {
             mbar_init(fix, 1);
             for (int s = 0; s < BW_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
             mbar_init(&s_full[0], 1); mbar_init(&s_full[1], 1);
+            mbar_init(&stat_full[0], 1); mbar_init(&stat_full[1], 1);
             mbar_init(p_full, BW_COMPUTE); mbar_init(dp_full, 1); mbar_init(dx_full, BW_COMPUTE); mbar_init(done, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             docs[0] = 0x7fffffff; docs[1] = -1; docs[2] = 0;
@@ -348,6 +358,88 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, bool o
     return ok;
 }
 
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
+                 "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// WIDE: the ring of two halves (64 columns, hi and lo) that pass, entry by entry
+// in the same order for the warp that loads and the one that multiplies.
+constexpr int WIDE_FLUSH = 4;   // tiles whose dk and dv the tensor cores add
+struct HalfRing {
+    static constexpr int HALF = 2 * CHUNK_BYTES;
+    const BwBlock& bb;
+    uint8_t* at;
+    int* err;
+    int e = 0;
+    __device__ __forceinline__ HalfRing(const BwBlock& b, uint8_t* ring, int* er) : bb(b), at(ring), err(er) {}
+    // both halves of a tile of rows
+    __device__ __forceinline__ void load2(const HeadMap& m, int tile, int h, int b, bool& ok) {
+        for (int f = 0; f < 2; ++f) {
+            const int s = e % 2;
+            if (e >= 2) ok = warp_wait(&bb.empty[s], ((e / 2) & 1) ^ 1, ok, err);
+            if (!ok) return;
+            if (elect_one()) {
+                mbar_expect_tx(&bb.full[s], HALF);
+                tma_tile(smem_u32(at + s * HALF), m, &bb.full[s], 2, tile * TILE, h, b, 2 * f);
+            }
+            __syncwarp();
+            ++e;
+        }
+    }
+    // copies in flight land before the block ends
+    __device__ __forceinline__ void drain(bool ok) {
+        if (!ok)
+            for (int i = max(0, e - 2); i < e; ++i) mbar_wait(&bb.full[i % 2], (i / 2) & 1, err);
+    }
+    // D = X Y^T over both halves: X resident, Y passes
+    template <typename T>
+    __device__ __forceinline__ void rows2(uint32_t d, uint32_t x, int ksteps, uint64_t* done, bool& ok) {
+        for (int f = 0; f < 2; ++f, ++e) {
+            const int s = e % 2;
+            ok = warp_wait(&bb.full[s], (e / 2) & 1, ok, err);
+            if (ok && elect_one()) {
+                if (f == 0) mma_rows_split<T>(d, x, smem_u32(at + s * HALF), 4);
+                else mma_rows_split<T, true>(d, x + HALF, smem_u32(at + s * HALF), ksteps - 4);
+                umma_commit(&bb.empty[s]);
+                if (f == 1) umma_commit(done);
+            }
+            __syncwarp();
+        }
+    }
+    // columns 0..63 and 64.. of D (+)= A Y: Y passes
+    template <typename T>
+    __device__ __forceinline__ void parts2(uint32_t d, uint32_t a, int ksteps, bool more, bool& ok) {
+        for (int f = 0; f < 2; ++f, ++e) {
+            const int s = e % 2;
+            ok = warp_wait(&bb.full[s], (e / 2) & 1, ok, err);
+            if (ok && elect_one()) {
+                mma_parts_split<BW_COLS>(d + 64 * f, a, smem_u32(at + s * HALF), f16_idesc<T>(f ? 16 * (ksteps - 4) : 64, true), more);
+                umma_commit(&bb.empty[s]);
+            }
+            __syncwarp();
+        }
+    }
+};
+// A row's columns col0 .. col0 + N - 1 of an fp32 output (+)= N TMEM columns times mul.
+template <int N>
+__device__ __forceinline__ void add_row(const HeadsView& v, int b, int h, int64_t row, int col0, bool on, int d, uint32_t taddr, float mul,
+                                        bool fresh) {
+    float* p = static_cast<float*>(v.p) + b * v.sb + h * v.sh + row * v.ss;
+    for (int k = 0; k < N; k += 16) {
+        uint32_t o[16];
+        tmem_ld16(taddr + k, o);
+        tmem_wait_ld();
+        if (on)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                const int c = col0 + k + q;
+                if (c < d) p[c * v.sd] = __uint_as_float(o[q]) * mul + (fresh ? 0.f : p[c * v.sd]);
+            }
+    }
+}
+
 // The powers of two that split operands carry.
 struct SplitExps {
     int q, k, v, dout;
@@ -369,7 +461,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                   const __grid_constant__ HeadMap mdo, const __grid_constant__ BwArgs g) {
     using L = BwSmem<DP>;
     constexpr bool SPLIT = !std::is_same<T, U>::value;
-    constexpr int DO = SPLIT ? 64 : DP;   // columns of a result
+    constexpr bool WIDE = L::WIDE;
+    constexpr int DO = SPLIT ? DP / 2 : DP;   // columns of a result
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const AttnCall& a = g.a;
@@ -421,12 +514,47 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         if (warp == BW_TMA) {
             // ------------------------------------------------ TMA
             if (any && lane == 0) {
-                mbar_expect_tx(bb.fix, 2 * L::TILE_B);
-                tma_tile(smem_u32(smem + L::FIX), mk, bb.fix, L::CH, j0, kvh, b);
-                tma_tile(smem_u32(smem + L::FIX + L::TILE_B), mv, bb.fix, L::CH, j0, kvh, b);
+                mbar_expect_tx(bb.fix, L::RING);
+                for (int f = 0; f < (WIDE ? 2 : 1); ++f) {
+                    tma_tile(smem_u32(smem + L::FIX + f * L::TILE_B), mk, bb.fix, L::CH, j0, kvh, b, 2 * f);
+                    tma_tile(smem_u32(smem + L::FIX + L::RING / 2 + f * L::TILE_B), mv, bb.fix, L::CH, j0, kvh, b, 2 * f);
+                }
             }
             int n = 0;
-            for (; qt >= 0 && ok; next(), ++n) {
+            if (WIDE) {
+                // Q and dout halves in the order in which the products take them: of
+                // tile n, n's S and dp, then dv of n, S of n + 1, dk of n, dp of n + 1
+                HalfRing ring(bb, smem + L::RING, g.err);
+                int n_qt = qt, n_h = h;
+                auto stats_of = [&]() {
+                    if (!elect_one()) return;
+                    mbar_expect_tx(&bb.stat_full[n & 1], STAT_BYTES);
+                    bulk_load(smem + L::STAT + (n & 1) * STAT_BYTES, g.stats + (((int64_t)b * a.hq + n_h) * g.q_tiles + n_qt) * 2 * TILE,
+                              STAT_BYTES, &bb.stat_full[n & 1]);
+                };
+                if (n_qt >= 0) {
+                    stats_of();
+                    ring.load2(mq, n_qt, n_h, b, ok);
+                    ring.load2(mdo, n_qt, n_h, b, ok);
+                }
+                while (n_qt >= 0 && ok) {
+                    const int p_qt = n_qt, p_h = n_h;
+                    ring.load2(mdo, p_qt, p_h, b, ok);
+                    next();
+                    n_qt = qt;
+                    n_h = h;
+                    ++n;
+                    if (n_qt >= 0) {
+                        ring.load2(mq, n_qt, n_h, b, ok);
+                        if (ok) stats_of();   // over those of n - 2: the ring is past dk of n - 2
+                        __syncwarp();
+                    }
+                    ring.load2(mq, p_qt, p_h, b, ok);
+                    if (n_qt >= 0) ring.load2(mdo, n_qt, n_h, b, ok);
+                }
+                ring.drain(ok);
+            }
+            for (; !WIDE && qt >= 0 && ok; next(), ++n) {
                 const int s = n % BW_STAGES;
                 if (n >= BW_STAGES) ok = warp_wait(&bb.empty[s], ((n / BW_STAGES) & 1) ^ 1, ok, g.err);
                 if (ok && lane == 0) {
@@ -435,26 +563,23 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                     tma_tile(at, mq, &bb.full[s], L::CH, qt * TILE, h, b);
                     tma_tile(at + L::TILE_B, mdo, &bb.full[s], L::CH, qt * TILE, h, b);
                     const float* st = g.stats + (((int64_t)b * a.hq + h) * g.q_tiles + qt) * 2 * TILE;
-                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                                     smem_u32(smem + L::STAT + s * STAT_BYTES)),
-                                 "l"(st), "r"(STAT_BYTES), "r"(smem_u32(&bb.full[s]))
-                                 : "memory");
+                    bulk_load(smem + L::STAT + s * STAT_BYTES, st, STAT_BYTES, &bb.full[s]);
                 }
             }
-            if (!ok)   // copies in flight land before the block ends
+            if (!WIDE && !ok)   // copies in flight land before the block ends
                 for (int e = max(0, n - 1 - BW_STAGES); e < n - 1; ++e)
                     mbar_wait(&bb.full[e % BW_STAGES], (e / BW_STAGES) & 1, g.err);
         } else {
             // ------------------------------------------------ tensor cores
             const int ksteps = (a.d + 15) / 16;
             const uint32_t idesc = f16_idesc<T>(16 * ksteps, true);
-            const uint32_t sk = smem_u32(smem + L::FIX), sv = sk + L::TILE_B;
+            const uint32_t sk = smem_u32(smem + L::FIX), sv = sk + L::RING / 2;
             auto rows = [&](uint32_t d, uint32_t x, uint32_t y) {
                 if (SPLIT) mma_rows_split<T>(d, x, y, ksteps);
                 else mma_rows<T, DP / 16>(d, x, y, ksteps);
             };
             auto parts = [&](uint32_t d, uint32_t x, uint32_t y, bool more) {
-                if (SPLIT) mma_parts_split<BW_COLS>(d, x, y, idesc);
+                if (SPLIT) mma_parts_split<BW_COLS>(d, x, y, idesc, 0);
                 else mma_parts<BW_COLS>(d, x, y, idesc, more);
             };
             // query rows of negative documents: 0 times what they hold could be NaN
@@ -467,7 +592,25 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 __syncwarp();
             };
             int n = 0;
-            if (any) {
+            if (WIDE && any) {
+                HalfRing ring(bb, smem + L::RING, g.err);
+                ok = warp_wait(bb.fix, 0, ok, g.err);
+                ring.rows2<T>(t_s, sk, ksteps, &bb.s_full[0], ok);
+                ring.rows2<T>(t_dp, sv, ksteps, bb.dp_full, ok);
+                while (qt >= 0 && ok) {
+                    ok = warp_wait(bb.p_full, n & 1, ok, g.err);
+                    ring.parts2<T>(t_dv, t_s, ksteps, n % WIDE_FLUSH != 0, ok);
+                    next();
+                    if (qt >= 0) ring.rows2<T>(t_s, sk, ksteps, &bb.s_full[0], ok);
+                    ok = warp_wait(bb.dx_full, n & 1, ok, g.err);
+                    ring.parts2<T>(t_dk, t_dp, ksteps, n % WIDE_FLUSH != 0, ok);
+                    if (qt >= 0) ring.rows2<T>(t_dp, sv, ksteps, bb.dp_full, ok);
+                    else if (ok && elect_one()) umma_commit(bb.done);
+                    __syncwarp();
+                    ++n;
+                }
+            }
+            if (!WIDE && any) {
                 ok = warp_wait(bb.fix, 0, ok, g.err);
                 ok = warp_wait(&bb.full[0], 0, ok, g.err);
                 if (ok) clean(0);
@@ -480,7 +623,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 }
                 __syncwarp();
             }
-            while (qt >= 0 && ok) {
+            while (!WIDE && qt >= 0 && ok) {
                 const int s = n % BW_STAGES, s1 = (n + 1) % BW_STAGES;
                 const uint32_t sq = smem_u32(smem + L::RING + s * 2 * L::TILE_B);
                 const uint32_t sq1 = smem_u32(smem + L::RING + s1 * 2 * L::TILE_B);
@@ -525,6 +668,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         const float lift = dx_lift<T>(g, b, kvh), up = lift * PLift<T>::back;
         const float up_dp = SPLIT ? up * exp2f((float)-(ex.dout + ex.v)) : up;   // dp carries the powers of dout and v
         const int doc = kd && j < a.nk ? kd[j] : -1;
+        const float mul = (which ? a.scale / lift : PLift<T>::back) * (SPLIT ? exp2f((float)-(which ? ex.q : ex.dout)) : 1.f);
         int n = 0;
         for (; qt >= 0 && ok; next(), ++n) {
             const int i0 = qt * TILE + wg * BW_COLS;
@@ -543,13 +687,19 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             }
             const float slope2 = BIAS ? __ldg(a.slopes + h) * kLog2e : 0.f;
             const float* st = reinterpret_cast<const float*>(smem + L::STAT + (n % BW_STAGES) * STAT_BYTES) + wg * BW_COLS;
-            ok = warp_wait(&bb.full[n % BW_STAGES], (n / BW_STAGES) & 1, ok, g.err);   // the statistics
+            uint64_t* landed = WIDE ? &bb.stat_full[n & 1] : &bb.full[n % BW_STAGES];   // the statistics
+            ok = warp_wait(landed, (n / 2) & 1, ok, g.err);
             ok = warp_wait(&bb.s_full[0], n & 1, ok, g.err);
             if (!ok) break;
             f2 x[16];
             {
                 // dv of the tile before, done before this S
-                if (SPLIT && which == 0 && n > 0) tmem_add<DH>(t_dva + lanes + col0, t_dv + lanes + col0, n == 1);
+                if (WIDE) {
+                    if (which == 0 && n > 0 && n % WIDE_FLUSH == 0)
+                        add_row<DH>(a.dv, b, kvh, j, col0, j < a.nk, a.d, t_dv + lanes + col0, mul, n == WIDE_FLUSH);
+                } else if (SPLIT && which == 0 && n > 0) {
+                    tmem_add<DH>(t_dva + lanes + col0, t_dv + lanes + col0, n == 1);
+                }
                 tmem_load(t_s + lanes + wg * BW_COLS, x);
                 uint32_t p16[16], low[16];
                 grad_row<T, CAP, BIAS, SPLIT>(x, p16, low, c1, cap, slope2, mask.p0 + i0 - j, masked, bits,
@@ -564,7 +714,12 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             if (!ok) break;
             {
                 // dk of the tile before, done before this dp
-                if (SPLIT && which == 1 && n > 0) tmem_add<DH>(t_dka + lanes + col0, t_dk + lanes + col0, n == 1);
+                if (WIDE) {
+                    if (which == 1 && n > 0 && n % WIDE_FLUSH == 0)
+                        add_row<DH>(a.dk, b, kvh, j, col0, j < a.nk, a.d, t_dk + lanes + col0, mul, n == WIDE_FLUSH);
+                } else if (SPLIT && which == 1 && n > 0) {
+                    tmem_add<DH>(t_dka + lanes + col0, t_dk + lanes + col0, n == 1);
+                }
                 uint32_t dp[32], dx[16], low[16];
                 tmem_load(t_dp + lanes + wg * BW_COLS, dp);
                 const f2 up2 = pack2(up, up);
@@ -581,17 +736,17 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         }
         if (any) ok = warp_wait(bb.done, 0, ok, g.err);
         uint32_t mine_at = (which ? t_dk : t_dv) + lanes + col0;
-        float mul = which ? a.scale / lift : PLift<T>::back;
-        if (SPLIT) {
+        if (SPLIT && !WIDE) {
             const uint32_t acc = (which ? t_dka : t_dva) + lanes + col0;
             if (any && ok) {
                 tmem_add<DH>(acc, mine_at, n == 1);
                 tmem_wait_st();
             }
             mine_at = acc;
-            mul *= exp2f((float)-(which ? ex.q : ex.dout));
         }
-        if (g.cluster == 1) {
+        if (WIDE && any) {
+            if (ok) add_row<DH>(which ? a.dk : a.dv, b, kvh, j, col0, j < a.nk, a.d, mine_at, mul, n <= WIDE_FLUSH);
+        } else if (g.cluster == 1) {
             HeadsView v = which ? a.dk : a.dv;
             v.p = static_cast<U*>(v.p) + col0 * v.sd;
             if (ok) store_row<U, DH>(v, b, kvh, j, j < a.nk, a.d - col0, mine_at, any, any, mul);
@@ -652,14 +807,16 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 }
 
 // ---------------------------------------------------------------- dq
-// TMEM: S of two tiles 0..255, dp (dx) 256..383, dq 384..511.
+// TMEM: S of two tiles 0..255, dp (dx) 256..383, dq 384..511 (WIDE: S of one
+// tile, dp, dq, its sum).
 template <typename T, typename U, int DP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(BW_THREADS, 1)
     k_attn_tc_dq(const __grid_constant__ HeadMap mq, const __grid_constant__ HeadMap mk, const __grid_constant__ HeadMap mv,
                  const __grid_constant__ HeadMap mdo, const __grid_constant__ BwArgs g) {
     using L = BwSmem<DP>;
     constexpr bool SPLIT = !std::is_same<T, U>::value;
-    constexpr int DO = SPLIT ? 64 : DP;   // columns of a result
+    constexpr bool WIDE = L::WIDE;
+    constexpr int DO = SPLIT ? DP / 2 : DP;   // columns of a result
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const AttnCall& a = g.a;
@@ -674,8 +831,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     BwBlock bb(smem + L::BAR, smem + L::DOCS);
     DocRange mine;
     const uint32_t tmem = bb.setup(qd ? qd + i0 : nullptr, rows, &mine, false);
-    const uint32_t t_dp = tmem + 2 * TILE, t_dq = tmem + 3 * TILE;
-    const uint32_t t_dqa = t_dq + 64;   // split operands: the sum over the tiles
+    const uint32_t t_dp = tmem + (WIDE ? 1 : 2) * TILE, t_dq = t_dp + TILE;
+    const uint32_t t_dqa = t_dq + DO;   // split operands: the sum over the tiles
     TileWalk walk;
     walk.start(0, (max(mask.key_end(i0, rows), 0) + TILE - 1) / TILE, 0, max(mask.key_end(i0, 1), 0) / TILE,
                kd ? g.k_ranges + (int64_t)b * g.k_tiles : nullptr, mine);
@@ -687,12 +844,25 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         if (warp == BW_TMA) {
             // ------------------------------------------------ TMA
             if (any && lane == 0) {
-                mbar_expect_tx(bb.fix, 2 * L::TILE_B);
-                tma_tile(smem_u32(smem + L::FIX), mq, bb.fix, L::CH, i0, h, b);
-                tma_tile(smem_u32(smem + L::FIX + L::TILE_B), mdo, bb.fix, L::CH, i0, h, b);
+                mbar_expect_tx(bb.fix, L::RING);
+                for (int f = 0; f < (WIDE ? 2 : 1); ++f) {
+                    tma_tile(smem_u32(smem + L::FIX + f * L::TILE_B), mq, bb.fix, L::CH, i0, h, b, 2 * f);
+                    tma_tile(smem_u32(smem + L::FIX + L::RING / 2 + f * L::TILE_B), mdo, bb.fix, L::CH, i0, h, b, 2 * f);
+                }
             }
             int n = 0;
-            for (; kt >= 0 && ok; kt = walk.next(&masked), ++n) {
+            if (WIDE) {
+                // K and V halves in the order in which the products take them: of tile
+                // n, S and dp, then dq of n (K again), S and dp of n + 1
+                HalfRing ring(bb, smem + L::RING, g.err);
+                for (; kt >= 0 && ok; kt = walk.next(&masked)) {
+                    ring.load2(mk, kt, kvh, b, ok);
+                    if (ok) ring.load2(mv, kt, kvh, b, ok);
+                    if (ok) ring.load2(mk, kt, kvh, b, ok);
+                }
+                ring.drain(ok);
+            }
+            for (; !WIDE && kt >= 0 && ok; kt = walk.next(&masked), ++n) {
                 const int s = n % BW_STAGES;
                 if (n >= BW_STAGES) ok = warp_wait(&bb.empty[s], ((n / BW_STAGES) & 1) ^ 1, ok, g.err);
                 if (ok && lane == 0) {
@@ -702,20 +872,20 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                     tma_tile(at + L::TILE_B, mv, &bb.full[s], L::CH, kt * TILE, kvh, b);
                 }
             }
-            if (!ok)
+            if (!WIDE && !ok)
                 for (int e = max(0, n - 1 - BW_STAGES); e < n - 1; ++e)
                     mbar_wait(&bb.full[e % BW_STAGES], (e / BW_STAGES) & 1, g.err);
         } else {
             // ------------------------------------------------ tensor cores
             const int ksteps = (a.d + 15) / 16;
             const uint32_t idesc = f16_idesc<T>(16 * ksteps, true);
-            const uint32_t sq = smem_u32(smem + L::FIX), sdo = sq + L::TILE_B;
+            const uint32_t sq = smem_u32(smem + L::FIX), sdo = sq + L::RING / 2;
             auto rows = [&](uint32_t d, uint32_t x, uint32_t y) {
                 if (SPLIT) mma_rows_split<T>(d, x, y, ksteps);
                 else mma_rows<T, DP / 16>(d, x, y, ksteps);
             };
             auto parts = [&](uint32_t d, uint32_t x, uint32_t y, bool more) {
-                if (SPLIT) mma_parts_split<BW_COLS>(d, x, y, idesc);
+                if (SPLIT) mma_parts_split<BW_COLS>(d, x, y, idesc, 0);
                 else mma_parts<BW_COLS>(d, x, y, idesc, more);
             };
             // keys that must not count: 0 times what they hold could be NaN
@@ -729,7 +899,21 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 __syncwarp();
             };
             int n = 0;
-            if (any) {
+            if (WIDE && any) {
+                HalfRing ring(bb, smem + L::RING, g.err);
+                ok = warp_wait(bb.fix, 0, ok, g.err);
+                while (kt >= 0 && ok) {
+                    ring.rows2<T>(tmem, sq, ksteps, &bb.s_full[0], ok);
+                    ring.rows2<T>(t_dp, sdo, ksteps, bb.dp_full, ok);
+                    ok = warp_wait(bb.dx_full, n & 1, ok, g.err);
+                    ring.parts2<T>(t_dq, t_dp, ksteps, false, ok);
+                    ++n;
+                    kt = walk.next(&masked);
+                }
+                if (ok && elect_one()) umma_commit(bb.done);
+                __syncwarp();
+            }
+            if (!WIDE && any) {
                 ok = warp_wait(bb.fix, 0, ok, g.err);
                 ok = warp_wait(&bb.full[0], 0, ok, g.err);
                 if (ok) clean(0);
@@ -742,7 +926,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 }
                 __syncwarp();
             }
-            while (kt >= 0 && ok) {
+            while (!WIDE && kt >= 0 && ok) {
                 const int s = n % BW_STAGES, s1 = (n + 1) % BW_STAGES;
                 const uint32_t sk = smem_u32(smem + L::RING + s * 2 * L::TILE_B);
                 const uint32_t sk1 = smem_u32(smem + L::RING + s1 * 2 * L::TILE_B);
@@ -799,10 +983,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                     bits &= same[0];
                 }
             }
-            ok = warp_wait(&bb.s_full[n & 1], (n / 2) & 1, ok, g.err);
+            const int buf = WIDE ? 0 : n & 1;
+            ok = warp_wait(&bb.s_full[buf], (WIDE ? n : n / 2) & 1, ok, g.err);
             if (!ok) break;
             f2 x[16];
-            tmem_load(tmem + (n & 1) * TILE + lanes + wg * BW_COLS, x);
+            tmem_load(tmem + buf * TILE + lanes + wg * BW_COLS, x);
             {
                 uint32_t unused[16], low[16];
                 grad_row<T, CAP, BIAS, SPLIT>(x, unused, low, c1, cap, slope2, jw - (mask.p0 + i), masked, bits,
@@ -941,6 +1126,10 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
         launch_begin_on(c, s, "attention_prep", 8.0 * rows * a.d, 2.0 * rows * a.d, ev);
         TL_CK(c, launch_with(k_attn_prep_f32, dim3((unsigned)(2 * tiles)), 1, 256, 0, true, s, a, stats, plan.q_tiles));
         TL_TRY(launch_end_on(c, s, ev));
+        if (a.d > 64) {
+            g.cluster = 1;   // a block adds its heads' sums to the outputs
+            return launch_scores<__half, float, 256>(c, m, g, s);
+        }
         return launch_scores<__half, float, 128>(c, m, g, s);
     }
     g.tops = {nullptr, nullptr, nullptr, nullptr};
