@@ -54,6 +54,10 @@ struct BwArgs {
     const DocRange *q_ranges, *k_ranges;
     SplitTops tops;              // fp32 arrays
     int q_tiles, k_tiles, cluster;
+    // a block a query head instead of a key head's group: its dk and dv go to
+    // sums of its own, which k_sum_heads adds (WIDE, heads that share keys)
+    int by_head;
+    HeadsView dk, dv;
     int* err;
 };
 
@@ -469,9 +473,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     // block -> (key tile, sequence and key head, head of the group); a causal
     // call's first keys are seen by the most queries and go first
-    const int group = a.hq / a.hkv, rank = blockIdx.x % g.cluster;
-    const unsigned unit = blockIdx.x / g.cluster, bhs = (unsigned)a.b * a.hkv;
-    const int kt = (int)(unit / bhs), kvh = (int)(unit % bhs % a.hkv), b = (int)(unit % bhs / a.hkv);
+    const int heads = g.by_head ? a.hq : a.hkv, group = a.hq / a.hkv, rank = blockIdx.x % g.cluster;
+    const unsigned unit = blockIdx.x / g.cluster, bhs = (unsigned)a.b * heads;
+    const int kt = (int)(unit / bhs), out_h = (int)(unit % bhs % heads), b = (int)(unit % bhs / heads);
+    const int kvh = g.by_head ? out_h / group : out_h;
     const int j0 = kt * TILE;
     const SeqMask mask(a, b);
     const int32_t* qd = a.q_doc ? a.q_doc + (int64_t)b * a.nq : nullptr;
@@ -494,14 +499,15 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     TileWalk walk;
     bool masked, ok = true;
     // (head, query tile) pairs in order; qt < 0 after the last
-    int h = kvh * group + rank - g.cluster;
+    int h = (g.by_head ? out_h : kvh * group + rank) - g.cluster;
+    const int h_end = g.by_head ? out_h + 1 : (kvh + 1) * group;
     int qt = -1;
     auto first = [&]() { walk.start(0, 0, 0, 0, ranges, mine); };
     auto next = [&]() {
         qt = walk.next(&masked);
         while (qt < 0) {
             h += g.cluster;
-            if (h >= (kvh + 1) * group) return;
+            if (h >= h_end) return;
             walk.start(begin, end, clear, end, ranges, mine);
             qt = walk.next(&masked);
         }
@@ -696,7 +702,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 // dv of the tile before, done before this S
                 if (WIDE) {
                     if (which == 0 && n > 0 && n % WIDE_FLUSH == 0)
-                        add_row<DH>(a.dv, b, kvh, j, col0, j < a.nk, a.d, t_dv + lanes + col0, mul, n == WIDE_FLUSH);
+                        add_row<DH>(g.dv, b, out_h, j, col0, j < a.nk, a.d, t_dv + lanes + col0, mul, n == WIDE_FLUSH);
                 } else if (SPLIT && which == 0 && n > 0) {
                     tmem_add<DH>(t_dva + lanes + col0, t_dv + lanes + col0, n == 1);
                 }
@@ -716,7 +722,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 // dk of the tile before, done before this dp
                 if (WIDE) {
                     if (which == 1 && n > 0 && n % WIDE_FLUSH == 0)
-                        add_row<DH>(a.dk, b, kvh, j, col0, j < a.nk, a.d, t_dk + lanes + col0, mul, n == WIDE_FLUSH);
+                        add_row<DH>(g.dk, b, out_h, j, col0, j < a.nk, a.d, t_dk + lanes + col0, mul, n == WIDE_FLUSH);
                 } else if (SPLIT && which == 1 && n > 0) {
                     tmem_add<DH>(t_dka + lanes + col0, t_dk + lanes + col0, n == 1);
                 }
@@ -745,11 +751,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             mine_at = acc;
         }
         if (WIDE && any) {
-            if (ok) add_row<DH>(which ? a.dk : a.dv, b, kvh, j, col0, j < a.nk, a.d, mine_at, mul, n <= WIDE_FLUSH);
+            if (ok) add_row<DH>(which ? g.dk : g.dv, b, out_h, j, col0, j < a.nk, a.d, mine_at, mul, n <= WIDE_FLUSH);
         } else if (g.cluster == 1) {
-            HeadsView v = which ? a.dk : a.dv;
+            HeadsView v = which ? g.dk : g.dv;
             v.p = static_cast<U*>(v.p) + col0 * v.sd;
-            if (ok) store_row<U, DH>(v, b, kvh, j, j < a.nk, a.d - col0, mine_at, any, any, mul);
+            if (ok) store_row<U, DH>(v, b, out_h, j, j < a.nk, a.d - col0, mine_at, any, any, mul);
         } else if (any && ok) {
             float* row = reinterpret_cast<float*>(smem) + (which * TILE + r) * L::SUM_LD + col0;
             for (int k = 0; k < DH / 16; ++k) {
@@ -1031,9 +1037,27 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     bb.finish(tmem);
 }
 
+// dk and dv of a key head: the sums of its group's heads, in their order.
+__global__ void __launch_bounds__(256) k_sum_heads(const __grid_constant__ AttnCall a, const float* __restrict__ dk, const float* __restrict__ dv) {
+    const int64_t n = (int64_t)a.nk * a.d, total = (int64_t)a.b * a.hkv * n;
+    const int group = a.hq / a.hkv;
+    wait_for_previous();
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < 2 * total; e += (int64_t)gridDim.x * 256) {
+        const bool is_v = e >= total;
+        const int64_t x = is_v ? e - total : e, bh = x / n, at = x % n;
+        const float* p = (is_v ? dv : dk) + bh * group * n + at;
+        float sum = 0.f;
+        for (int q = 0; q < group; ++q) sum += p[q * n];
+        const HeadsView& v = is_v ? a.dv : a.dk;
+        static_cast<float*>(v.p)[bh / a.hkv * v.sb + bh % a.hkv * v.sh + at / a.d * v.ss + at % a.d * v.sd] = sum;
+    }
+}
+
+bool sums_by_head(const AttnCall& a) { return a.dtype == TL_TYPE_F32 && a.d > 64 && a.hq > a.hkv; }
+
 struct BwPlan {
     int q_tiles, k_tiles;
-    size_t stats, norms, q_ranges, k_ranges, split, bytes;
+    size_t stats, norms, q_ranges, k_ranges, split, sums, bytes;
     explicit BwPlan(const AttnCall& a) {
         q_tiles = (a.nq + TILE - 1) / TILE;
         k_tiles = (a.nk + TILE - 1) / TILE;
@@ -1044,6 +1068,7 @@ struct BwPlan {
         q_ranges = take(a.q_doc ? (size_t)a.b * q_tiles * sizeof(DocRange) : 0);
         k_ranges = take(a.q_doc ? (size_t)a.b * k_tiles * sizeof(DocRange) : 0);
         split = take(a.dtype == TL_TYPE_F32 ? SplitPlan(a, true).bytes : 0);
+        sums = take(sums_by_head(a) ? 2 * (size_t)a.b * a.hq * a.nk * a.d * sizeof(float) : 0);
     }
 };
 
@@ -1056,7 +1081,7 @@ tl_status launch(tl_ctx* c, const HeadMap* m, const BwArgs& g, cudaStream_t s) {
     const AttnCall& a = g.a;
     cudaEvent_t ev[2];
     launch_begin_on(c, s, "attention_tc_dkv", 0, 8.0 * a.d * attn_pairs(a), ev);
-    TL_CK(c, launch_with(k_attn_tc_dkv<T, U, DP, CAP, BIAS>, dim3((unsigned)((int64_t)g.k_tiles * a.b * a.hkv * g.cluster)), g.cluster,
+    TL_CK(c, launch_with(k_attn_tc_dkv<T, U, DP, CAP, BIAS>, dim3((unsigned)((int64_t)g.k_tiles * a.b * (g.by_head ? a.hq : a.hkv * g.cluster))), g.cluster,
                          BW_THREADS, smem, true, s, m[0], m[1], m[2], m[3], g));
     TL_TRY(launch_end_on(c, s, ev));
     launch_begin_on(c, s, "attention_tc_dq", 0, 6.0 * a.d * attn_pairs(a), ev);
@@ -1104,6 +1129,9 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
     while (g.cluster > 1 && g.cluster < 8 && group % (2 * g.cluster) == 0 &&
            (int64_t)plan.k_tiles * a.b * a.hkv * g.cluster < c->sm_count * 2 / 3)
         g.cluster *= 2;
+    g.by_head = 0;
+    g.dk = a.dk;
+    g.dv = a.dv;
     g.err = c->d_flags + 8;
     c->flags_armed = true;
     if (a.q_doc) {
@@ -1127,8 +1155,18 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
         TL_CK(c, launch_with(k_attn_prep_f32, dim3((unsigned)(2 * tiles)), 1, 256, 0, true, s, a, stats, plan.q_tiles));
         TL_TRY(launch_end_on(c, s, ev));
         if (a.d > 64) {
-            g.cluster = 1;   // a block adds its heads' sums to the outputs
-            return launch_scores<__half, float, 256>(c, m, g, s);
+            g.cluster = 1;
+            if (!sums_by_head(a)) return launch_scores<__half, float, 256>(c, m, g, s);
+            float* sums = reinterpret_cast<float*>(w + plan.sums);
+            const int64_t one = (int64_t)a.b * a.hq * a.nk * a.d;
+            g.by_head = 1;
+            g.dk = {sums, (int64_t)a.hq * a.nk * a.d, (int64_t)a.nk * a.d, a.d, 1};
+            g.dv = {sums + one, g.dk.sb, g.dk.sh, g.dk.ss, 1};
+            TL_TRY((launch_scores<__half, float, 256>(c, m, g, s)));
+            launch_begin_on(c, s, "attention_sum_heads", 4.0 * 2 * (one + one / a.hq * a.hkv), 0, ev);
+            TL_CK(c, launch_with(k_sum_heads, dim3((unsigned)std::min<int64_t>((2 * one / a.hq * a.hkv + 255) / 256, 148 * 8)), 1, 256, 0,
+                                 false, s, a, static_cast<const float*>(sums), static_cast<const float*>(sums + one)));
+            return launch_end_on(c, s, ev);
         }
         return launch_scores<__half, float, 128>(c, m, g, s);
     }
