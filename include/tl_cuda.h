@@ -469,10 +469,13 @@ tl_status tl_tensor_array(tl_tensor* t, int32_t write, tl_array* out);
  * written may not overlap themselves, one another or an input).  Sums, the
  * softmax and its statistics are in 32 bits.  16-bit types take their products
  * from 16-bit operands (exponentials, and dx of the backward pass, rounded to
- * them).  fp32 arrays are computed in fp32, those of head size up to 64 with 22
- * bits of each operand of a product, or 2^-39 of the largest of its kind in
- * the heads that share a key head where that is more; a value that is not finite
- * then makes the results that depend on it NaN.
+ * them).  fp32 arrays of head size up to 128 take 22 bits of each operand of a
+ * product, or 2^-39 of the largest of its kind in the heads that share a key
+ * head where that is more (a value that is not finite then makes the results that
+ * depend on it NaN); larger ones, and all of a TL_PREC_FP32 context, 24 bits on
+ * the CUDA cores.  The tensor cores need scale > 0 and, of 16-bit arrays, a
+ * contiguous head size that is a multiple of 8, at most 128, and 16-byte
+ * aligned rows; other calls take a general kernel, tens of times slower.
  * The device arrays slopes [Hq] fp32 (constants: they get no gradient),
  * prefix_len, kv_len, q_start [batch] int32, q_doc [batch, Nq] and
  * k_doc [batch, Nk] int32 are contiguous.  kv_len NULL: all Nk keys; its values

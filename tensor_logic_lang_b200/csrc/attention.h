@@ -24,6 +24,7 @@ struct AttnCall {
     float* lse;                   // [b, hq, nq]
     float scale, cap;
     int causal;
+    int cuda_cores;               // fp32 arrays of a TL_PREC_FP32 context: no tensor cores
     const float* slopes;
     const int32_t *prefix_len, *q_doc, *k_doc, *kv_len, *q_start;
 };

@@ -34,8 +34,8 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
     if (WRITE) wait_for_previous();   // the largest values
     const AttnCall& a = g.a;
     const SplitArray& x = g.arr[blockIdx.y];
-    const int blocks = (x.n + SP_ROWS - 1) / SP_ROWS;
-    if (blockIdx.x >= (unsigned)(blocks * x.h) * a.b) return;
+    const unsigned blocks = (x.n + SP_ROWS - 1) / SP_ROWS;
+    if (blockIdx.x >= (int64_t)blocks * x.h * a.b) return;
     const int bh = blockIdx.x / blocks, b = bh / x.h, h = bh % x.h;
     const int group = b * a.hkv + h / (x.h / a.hkv);
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, c = 2 * lane;

@@ -507,7 +507,7 @@ bool tc_array(const HeadsView& v, int b, int h, int64_t n) {
 bool attn_tc_takes(const AttnCall& a) {
     // a scale that keeps the order of the scores (the row maximum is taken
     // before scaling)
-    if (a.nk == 0 || !(a.scale > 0.f)) return false;
+    if (a.nk == 0 || !(a.scale > 0.f) || a.cuda_cores) return false;
     if (a.dtype == TL_TYPE_F32) return a.d <= kSplitMaxHead;   // its operands are copies, the arrays may lie anyhow
     return a.d % 8 == 0 && a.d <= 128 && tc_array(a.q, a.b, a.hq, a.nq) && tc_array(a.k, a.b, a.hkv, a.nk) &&
            tc_array(a.v, a.b, a.hkv, a.nk) && tc_array(a.o, a.b, a.hq, a.nq);

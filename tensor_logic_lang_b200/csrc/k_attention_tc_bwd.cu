@@ -1100,7 +1100,7 @@ tl_status launch_scores(tl_ctx* c, const HeadMap* m, const BwArgs& g, cudaStream
 }  // namespace
 
 bool attn_tc_backward_takes(const AttnCall& a) {
-    if (!attn_tc_takes(a) || a.nq == 0) return false;
+    if (!attn_tc_takes(a) || a.nq == 0 || a.hq == 0) return false;
     if (a.dtype == TL_TYPE_F32) return true;
     return tc_array(a.dout, a.b, a.hq, a.nq) && tc_array(a.dq, a.b, a.hq, a.nq) &&
            tc_array(a.dk, a.b, a.hkv, a.nk) && tc_array(a.dv, a.b, a.hkv, a.nk);

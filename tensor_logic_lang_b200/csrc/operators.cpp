@@ -191,9 +191,9 @@ tl_status check_attention(tl_ctx* c, const tl_attention& t, bool backward, AttnC
         return fail(c, TL_ERR_INVALID, "attention: %lld query heads over %lld key heads", (long long)hq, (long long)hkv);
     if (b > kMaxCount || hq > kMaxCount || nq > kMaxCount || nk > kMaxCount)
         return fail(c, TL_ERR_TOO_LARGE, "attention: more than 2^29 sequences, heads or positions");
-    // blocks are numbered in 31 bits: 16 queries or keys of a head at the least
-    if (b * hq > kMaxCount || (double)b * hq * ((std::max(nq, nk) + 15) / 16) > 2147483647.0)
-        return fail(c, TL_ERR_TOO_LARGE, "attention: batch x heads x positions above 2^35");
+    // blocks are numbered in 31 bits: one a query, or 16 keys of a head, at the least
+    if (b * hq > kMaxCount / 2 || (double)b * hq * nq > 2147483647.0 || (double)b * hq * ((nk + 15) / 16) > 2147483647.0)
+        return fail(c, TL_ERR_TOO_LARGE, "attention: batch x heads x queries above 2^31, or x keys above 2^35");
     TL_TRY(check_heads(c, t.q, "q", t, b, hq, nq, d, false));
     TL_TRY(check_heads(c, t.k, "k", t, b, hkv, nk, d, false));
     TL_TRY(check_heads(c, t.v, "v", t, b, hkv, nk, d, false));
@@ -235,6 +235,7 @@ tl_status check_attention(tl_ctx* c, const tl_attention& t, bool backward, AttnC
     a.scale = t.scale; a.cap = t.softcap; a.causal = t.causal;
     a.slopes = t.slopes; a.prefix_len = t.prefix_len; a.q_doc = t.q_doc; a.k_doc = t.k_doc;
     a.kv_len = t.kv_len; a.q_start = t.q_start;
+    a.cuda_cores = c && c->opts.precision == TL_PREC_FP32 && a.dtype == TL_TYPE_F32;
     *out = a;
     return TL_OK;
 }

@@ -178,13 +178,15 @@ class Context:
     # ------------------------------------------------------------------ array operators
     # Arrays are device tensors (torch's, or any object with their data_ptr(), dtype,
     # shape, stride(), get_device(), numel() and is_contiguous()), or names of this context's tensors, which
-    # stand for their fp32 storage.  stream: a cudaStream_t handle (torch's
+    # stand for their fp32 storage and are used on the context's own stream alone.  stream: a cudaStream_t handle (torch's
     # current stream: torch.cuda.current_stream().cuda_stream), or None for the
     # context's own stream, on which its programs run.  Device tensors that
     # another stream wrote need that stream's work done or waited for first.
     def _view(self, x, what, write=False):
         """(data, type, shape, strides) of an array argument."""
         if isinstance(x, str):
+            if self._foreign:
+                raise abi.TLError(abi.TL_ERR_INVALID, f"{what}: a tensor's storage is used on the context's own stream")
             a = abi.Array()
             self.check(self.lib.tl_tensor_array(self._lookup(x), 1 if write else 0, C.byref(a)), f"{what} {x}")
             return a.data or 0, a.dtype, tuple(a.dims[:a.rank]), tuple(a.strides[:a.rank])
@@ -239,7 +241,11 @@ class Context:
         return p
 
     def _stream(self, stream):
-        return self.lib.tl_stream(self.h) or 0 if stream is None else stream
+        own = self.lib.tl_stream(self.h) or 0
+        if stream is None:
+            stream = own
+        self._foreign = stream != own
+        return stream
 
     def _room(self, workspace):
         if workspace is None:
@@ -251,6 +257,7 @@ class Context:
 
     def _attention(self, q, k, v, out, lse, grads, scale, softcap, slopes, causal, prefix_len, q_doc, k_doc, kv_len,
                    q_start, workspace, stream, writes_out):
+        stream = self._stream(stream)
         qa, ka, va, oa = self._heads(q, "q"), self._heads(k, "k"), self._heads(v, "v"), self._heads(out, "out", writes_out)
         b, hq, nq, d = qa[3:7]
         nk = ka[5]
@@ -268,7 +275,7 @@ class Context:
             q_doc is not None and plain(q_doc, "q_doc", "int32", (b, nq)),
             k_doc is not None and plain(k_doc, "k_doc", "int32", (b, nk)),
             kv_len is not None and plain(kv_len, "kv_len", "int32", one),
-            q_start is not None and plain(q_start, "q_start", "int32", one), ws, room, self._stream(stream))
+            q_start is not None and plain(q_start, "q_start", "int32", one), ws, room, stream)
 
     def attention(self, q, k, v, out, lse=None, *, scale=None, softcap=0.0, slopes=None, causal=False, prefix_len=None,
                   q_doc=None, k_doc=None, kv_len=None, q_start=None, workspace=None, stream=None):
@@ -343,14 +350,16 @@ class Context:
         In place, or into the arrays of `out` (same dims and strides, any type).  norm: a device fp32 scalar that
         receives the norm before the scaling.  Nothing is copied to the host.
         """
+        stream = self._stream(stream)
         a, o = self._clip_lists(grads, out)
         at = None if norm is None else self._plain(norm, "norm", "float32", ())
         self.check(self.lib.tl_clip_gradients(self.h, a, o, len(grads), max_norm,
-                                              at, *self._room(workspace), self._stream(stream)), "clip_gradients")
+                                              at, *self._room(workspace), stream), "clip_gradients")
         return grads if out is None else out
 
     def clip_workspace(self, grads, max_norm, out=None):
         """Bytes of workspace of a clip_gradients call."""
+        self._stream(None)
         a, o = self._clip_lists(grads, out)
         n = self.lib.tl_clip_workspace(self.h, a, o, len(grads), max_norm)
         self.check(max(0, -n), "clip_workspace")

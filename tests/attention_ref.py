@@ -15,7 +15,15 @@ and in every type a slack g relative to the sizes of the terms for the 32-bit
 arithmetic: scores that are off by s 2^-24 times a few, the exponential and
 the tanh (g = 2^-12 beside 16-bit roundings, 2^-16 in fp32).
 
-fp32 arrays of head size up to 64 go through the tensor cores as pairs of fp16
+The tanh of a capped score is held in 32 bits: near 1 it is off by half a step,
+2^-24, elsewhere by up to 2^-21 (an exponential and a quotient of 2^-22 each),
+so 1 - tanh^2 is off by up to 2^-20 in absolute terms, which counts where it is
+small.
+
+An exponential below 2^-126, the smallest normal number of fp32 and bf16, may be
+0, and so may a dx: off by that much for every pair that is seen.
+
+fp32 arrays of head size up to 128 go through the tensor cores as pairs of fp16
 numbers, hi + lo: a value x below 2^15 keeps 22 bits, or 2^-25 where that is
 more (fp16 ends at 2^-24, half a step of it).  In the backward pass p goes in as
 2^14 p, so it is off by up to 2^-25 / 2^14 = 2^-39; dx / scale goes in times the
@@ -93,18 +101,20 @@ def reference(q, k, v, dout=None, *, scale=None, softcap=0.0, slopes=None, causa
     # every dx: its rounding, the rounding of out within D, the slack of p, dp and D
     off_D = (DO * out).abs().sum(-1, keepdim=True)
     off_dp = DO.abs() @ V.abs().transpose(-1, -2)
-    off = h * dx.abs() + p * bend.abs() * (h * off_D + g * big * ((dp - D).abs() + 2.0 ** -6 * (off_dp + off_D)))
+    off_bend = 2.0 ** -20 * scale if softcap else 0.0
+    off = h * dx.abs() + p * off_bend * (dp - D).abs() + p * bend.abs() * (h * off_D + g * big * ((dp - D).abs() + 2.0 ** -6 * (off_dp + off_D)))
 
     def grouped(y):
         return y.view(b, hkv, group, nk, d).sum(2)
 
-    off_p = torch.zeros_like(p)
+    off_p = seen * 2.0 ** -126
+    off = off + off_p * (1 + (dp - D).abs() * bend.abs())
     if q.dtype == torch.float32:
         def top(y, heads):
             return y.norm(dim=-1).amax(-1).view(b, hkv, heads).amax(-1).repeat_interleave(group, 1)
         both = 2.0 * top(DO, group) * top(V, group) if nq and nk else torch.zeros((b, hq), device=dev)
         off = off + seen * 2.0 ** -39 * both.view(b, hq, 1, 1) * scale
-        off_p = seen * 2.0 ** -39
+        off_p = off_p + seen * 2.0 ** -39
     dq, dk, dv = dx @ K, grouped(dx.transpose(-1, -2) @ Q), grouped(p.transpose(-1, -2) @ DO)
     res["dq"] = (dq, h * dq.abs() + off @ K.abs() + tiny)
     res["dk"] = (dk, h * dk.abs() + grouped(off.transpose(-1, -2) @ Q.abs()) + tiny)

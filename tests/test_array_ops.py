@@ -87,6 +87,17 @@ def test_refused_sizes(lib):
     assert need(lib, a) == -abi.TL_ERR_TOO_LARGE
 
 
+def test_refused_counts(lib):
+    # more queries than blocks can be numbered, without the memory for them
+    def wide(b, h, n):
+        return array((b, h, n, 1), (0, 0, 0, 1))
+    a = attention(b=1, hq=1, hkv=1, nq=1, nk=1, d=1)
+    a.q = wide(1 << 14, 1 << 14, 64)
+    a.k = a.v = wide(1 << 14, 1 << 14, 1)
+    a.o = array((1 << 14, 1 << 14, 64, 1), data=0x70000000)
+    assert need(lib, a) == -abi.TL_ERR_TOO_LARGE
+
+
 def test_refused_outputs(lib):
     # written arrays that overlap themselves, an input or one another
     assert need(lib, attention(o=array((2, 4, 8, 32), (0, 256, 32, 1)))) == -abi.TL_ERR_INVALID

@@ -436,6 +436,124 @@ def test_training_step_of_a_program(ctx):
         assert np.abs(ctx.tensor(n) - t * (0.5 / norm)).max() <= 1e-3 * np.abs(t).max() * 0.5 / norm
 
 
+@pytest.mark.parametrize("cap", [50.0, 50.2, 50.3, 1000.0])
+def test_cap_at_the_ends_of_the_tanh(ctx, cap):
+    # scores far past the cap on either side, for rows of all high, all low and mixed ones
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for dtype in ("bf16", "f16", "f32"):
+        for nq in (1, 150):
+            q, k, v = heads(gen, 1, 4, nq, 64, dtype), heads(gen, 1, 2, 300, 64, dtype), heads(gen, 1, 2, 300, 64, dtype)
+            q[:, 0].abs_(), q[:, 1].abs_().neg_(), k[:, 0].abs_()
+            q.mul_(40.0)
+            dout = heads(gen, 1, 4, nq, 64, dtype)
+            m = {"softcap": cap, "causal": True}
+            want = reference(q, k, v, dout, **m)
+            got = run(ctx, q, k, v, dout, m)
+            for n in want:
+                check(got[n], want[n], (dtype, nq, n))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_many_sequences(ctx, dtype):
+    # more sequences than a block has threads, most of them short or empty
+    for b, nq in ((700, 1), (300, 3), (90, 40)):
+        gen = torch.Generator(device="cuda").manual_seed(b)
+        q, k, v = heads(gen, b, 2, nq, 32, dtype), heads(gen, b, 1, 200, 32, dtype), heads(gen, b, 1, 200, 32, dtype)
+        m = {"causal": True, "kv_len": ints([(7 * i) % 230 if i % 3 else 0 for i in range(b)])}
+        got = run(ctx, q, k, v, None, m)
+        want = reference(q, k, v, **m)
+        for n in want:
+            check(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("group", [3, 8, 12, 64])
+def test_groups(ctx, group, dtype):
+    compare(ctx, 2, group, 1, 2, 700, 64, dtype, "cap causal len", seed=group)
+    compare(ctx, 1, 2 * group, 2, 140, 140, 128, dtype, "causal", seed=group)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_values_of_very_different_size(ctx, dtype):
+    # heads, and q, k, v, dout, of scales far apart: a head's results keep their digits
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    q, k, v, dout = (heads(gen, 2, 4, 200, 64, dtype) for _ in range(4))
+    for i, s in enumerate((1e-12, 1e-4, 1.0, 1e6)):
+        v[:, i].mul_(s)
+        dout[:, i].mul_(1 / s)
+    k.mul_(1e3)
+    q.mul_(1e-3)
+    m = {"causal": True}
+    want = reference(q, k, v, dout, **m)
+    got = run(ctx, q, k, v, dout, m)
+    for n in want:
+        check(got[n], want[n], n)
+
+
+def test_fp32_on_the_cuda_cores():
+    # a context of that precision keeps all 24 bits of the operands
+    from tensor_logic_lang_b200 import abi
+    from tensor_logic_lang_b200.runtime import Context
+    c = Context(device=0, precision=abi.PREC_FP32)
+    try:
+        c.profile(True)
+        compare(c, 2, 4, 2, 100, 130, 64, "f32", "cap causal")
+        names = set(c.profile_read())
+        assert "attention_general" in names and not any("tc" in n or "split" in n for n in names), names
+    finally:
+        c.close()
+
+
+def test_kernels_that_run(ctx):
+    # the kernels the rules of the entry point's documentation name
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    ctx.profile(True)
+    for dtype, nq, d, layout, want in (("bf16", 200, 64, "bhsd", "attention_tc"), ("f32", 200, 64, "bhsd", "attention_tc"),
+                                       ("f32", 200, 100, "odd", "attention_tc"), ("f16", 200, 128, "bshd", "attention_tc"),
+                                       ("bf16", 200, 100, "bhsd", "attention_general"), ("bf16", 200, 64, "odd", "attention_general"),
+                                       ("f16", 200, 192, "bhsd", "attention_general"), ("bf16", 1, 64, "bhsd", "attention_decode"),
+                                       ("f32", 3, 64, "bhsd", "attention_decode"), ("f16", 2, 100, "odd", "attention_decode")):
+        q, k, v = heads(gen, 1, 2, nq, d, dtype, layout), heads(gen, 1, 2, 300, d, dtype, layout), heads(gen, 1, 2, 300, d, dtype, layout)
+        ctx.profile_reset()
+        ctx.attention(q, k, v, like(q, "bhsd"), stream=stream())
+        assert want in ctx.profile_read(), (dtype, nq, d, layout, set(ctx.profile_read()))
+    ctx.profile(False)
+
+
+def test_offsets_past_32_bits(ctx):
+    # a cache whose last keys lie behind 2^32 bytes and 2^31 elements of it
+    n, d = (1 << 24) + 77, 128
+    k = torch.zeros((1, 1, n, d), dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros((1, 1, n, d), dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    tail = 300
+    k[:, :, -tail:] = torch.randn((1, 1, tail, d), generator=gen, device="cuda").bfloat16()
+    v[:, :, -tail:] = torch.randn((1, 1, tail, d), generator=gen, device="cuda").bfloat16()
+    for nq in (1, 130):
+        q = (torch.randn((1, 1, nq, d), generator=gen, device="cuda") * 8).bfloat16()
+        q = torch.cat([q, q], 1)
+        out, lse = like(q, "bhsd"), torch.empty((1, 2, nq), device="cuda")
+        ctx.attention(q, k, v, out, lse, causal=True, stream=stream())
+        torch.cuda.synchronize()
+        # keys of zeros have the score 0 and no value
+        want = reference(q, k[:, :, -tail:], v[:, :, -tail:], causal=True)
+        x = (q.double() @ k[:, :, -tail:].double().transpose(-1, -2)) * d ** -0.5
+        seen = torch.arange(tail, device="cuda")[None] <= torch.arange(nq, device="cuda")[:, None] + tail - nq
+        x = x.masked_fill(~seen, float("-inf"))
+        total = torch.logsumexp(torch.cat([x, torch.full((1, 2, nq, 1), float(np.log(n - tail)), device="cuda", dtype=torch.float64)], -1), -1)
+        value = torch.exp(x - total[..., None]) @ v[:, :, -tail:].double()
+        check(out, (value, want["out"][1]), "out")
+        assert ((lse.double() - total).abs() <= 1e-4 * total.abs()).all()
+
+
+def test_named_tensors_stay_on_their_stream(ctx):
+    from tensor_logic_lang_b200 import abi
+    ctx.create("Xq", (8, 16))
+    x = torch.zeros((8, 16), device="cuda")
+    with pytest.raises(abi.TLError):
+        ctx.attention("Xq", x, x, torch.empty_like(x), stream=stream())
+
+
 def test_second_device():
     if torch.cuda.device_count() < 2:
         pytest.skip("needs two GPUs")
