@@ -1,17 +1,19 @@
-// Attention forward on the tensor cores: 16-bit operands, head size up to
-// 128, or fp32 arrays of head size up to 64 as pairs of fp16 (attn_tc.h, SplitArray);
-// one pass over the keys with a running maximum and sum.
+// Attention forward on the tensor cores: 16-bit operands, or fp32 arrays as
+// pairs of fp16 (attn_tc.h, SplitArray), head size up to 128; one pass over the
+// keys with a running maximum and sum.
 //
 // A block owns two tiles of 128 queries that read the same keys: the same
 // rows of two heads of a group where the group has an even number of heads
 // (each causal tile then needs exactly the keys the block loads), else
-// neighbouring rows of one head.  Warps:
+// neighbouring rows of one head; or one tile (launch_tiles says when), and two
+// such blocks share an SM.  Warps of two tiles:
 //   0-7, 8-15  tile 0, 1: a thread has 64 of a query's 128 scores: scores out
 //              of TMEM, softmax statistics (the two halves of a row agree on
 //              its maximum through shared memory), probabilities (16-bit) back
 //              into TMEM over the scores
 //   16         tensor cores: S = Q K^T (SMEM x SMEM), O += P V (TMEM x SMEM)
-//   17         TMA: Q once, then K and V tiles through a ring of four
+//   17         TMA: Q once, then K and V tiles through a ring of four (two
+//              where two blocks share the shared memory)
 // TMEM: S0 S1 (128 columns each, P over the first half of each 64), O0 O1.  While one
 // tile's softmax runs, the other tile's products do; S of the next keys is
 // issued right behind P V of these, which orders it after P is read.
@@ -34,8 +36,6 @@
 namespace tl {
 namespace {
 
-constexpr int FW_SOFTMAX = 512, FW_THREADS = FW_SOFTMAX + 64, FW_STAGES = 4;
-constexpr int FW_MMA = FW_SOFTMAX / 32, FW_TMA = FW_MMA + 1;   // warps
 // Capped scores lie in +-top (base 2), so bf16, which has the range of fp32,
 // needs no maximum: with the reference top - 20 every p lies in 2^(20 - 2 top)
 // .. 2^20, above 2^-125 up to top = 72.5 (softcap 50.2).  No maxima, no agreeing
@@ -47,18 +47,28 @@ constexpr float kGrow = 8.f;   // rescale when the maximum grew by 2^8
 struct FwArgs {
     AttnCall a;
     const DocRange* k_ranges;   // [b, key tiles] with documents
-    int tiles;                  // query tiles of a block: 2, or 1 where that gives the GPU enough blocks
     int pair_heads;             // two tiles: heads h, h + 1 (else rows i0, i0 + 128)
     int key_tiles;
     SplitTops tops;             // fp32 arrays
     int* err;
 };
 
-template <int DP>
-struct FwSmem {
-    static constexpr int CH = DP / 64, TILE_B = CH * CHUNK_BYTES;
-    static constexpr int Q = 0, KV = 2 * TILE_B, BAR = KV + FW_STAGES * TILE_B, DOCS = BAR + 256, ROWS = DOCS + 64,
-                         BYTES = ROWS + 2 * 2 * 2 * TILE * 4 + 1024;   // ROWS: [parity][tile][half][row]
+// NT query tiles a block.  One: two blocks share an SM where TMEM and shared
+// memory allow it, with half of each.
+template <typename T, typename U, int DP, int NT>
+struct Fw {
+    static constexpr bool SPLIT = !std::is_same<T, U>::value;
+    static constexpr int HALVES = DP > 128 ? 2 : 1;   // split operands of more than 64 columns: a tile is two, one behind the other
+    static constexpr int DO = SPLIT ? DP / 2 : DP;    // columns of O
+    static constexpr int SOFTMAX = 256 * NT, THREADS = SOFTMAX + 64, MMA = SOFTMAX / 32, TMA = MMA + 1;   // threads, warps
+    static constexpr int CH = DP / HALVES / 64, TILE_B = CH * CHUNK_BYTES;
+    static constexpr int PER_SM = NT == 1 && HALVES == 1 ? 2 : 1;
+    static constexpr int STAGES = PER_SM == 2 && CH == 2 ? 2 : 4;
+    // TMEM: S of the tiles, O of the tiles, split operands: the sums over the key tiles
+    static constexpr int T_O = NT * TILE, T_ACC = T_O + NT * DO, TMEM = T_ACC + (SPLIT ? NT * DO : 0) <= 256 ? 256 : 512;
+    static_assert(T_ACC + (SPLIT ? NT * DO : 0) <= 512 && PER_SM * TMEM <= 512, "TMEM columns");
+    static constexpr int Q = 0, KV = NT * HALVES * TILE_B, BAR = KV + STAGES * TILE_B, DOCS = BAR + 256, ROWS = DOCS + 64,
+                         BYTES = ROWS + 2 * 2 * NT * TILE * 4 + 1024;   // ROWS: [parity][tile][half][row]
 };
 
 // the smallest / largest document of each tile of 128 keys (queries), a warp per tile
@@ -146,18 +156,17 @@ __device__ __forceinline__ float score_row(f2 (&x)[32], float c1, const CapCoef<
 
 // T: operands, U: the arrays' type (float: split operands, DP = 128 or 256 columns
 // of hi and lo).  FIX: see fixed_top.
-template <typename T, typename U, int DP, bool CAP, bool BIAS, bool FIX>
-__global__ void __launch_bounds__(FW_THREADS, 1)
+template <typename T, typename U, int DP, int NT, bool CAP, bool BIAS, bool FIX>
+__global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::PER_SM)
     k_attn_tc(const __grid_constant__ HeadMap mq, const __grid_constant__ HeadMap mk, const __grid_constant__ HeadMap mv,
               const __grid_constant__ FwArgs g) {
-    constexpr bool SPLIT = !std::is_same<T, U>::value;
-    constexpr int HALVES = DP > 128 ? 2 : 1;   // split operands of more than 64 columns: a tile is two, one behind the other
-    using L = FwSmem<DP / HALVES>;
-    constexpr int DO = SPLIT ? DP / 2 : DP;    // columns of O
+    using L = Fw<T, U, DP, NT>;
+    constexpr bool SPLIT = L::SPLIT;
+    constexpr int HALVES = L::HALVES, DO = L::DO;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::BAR);
-    uint64_t *q_full = bar, *full = bar + 1, *empty = full + FW_STAGES, *s_full = empty + FW_STAGES, *p_full = s_full + 2,
+    uint64_t *q_full = bar, *full = bar + 1, *empty = full + L::STAGES, *s_full = empty + L::STAGES, *p_full = s_full + 2,
              *o_done = p_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 24);
     int* docs = reinterpret_cast<int*>(smem + L::DOCS);   // lo, hi, pad of the block's rows
@@ -168,7 +177,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     // of a causal call, go first
     const int group = a.hq / a.hkv;
     const int units = g.pair_heads ? a.hq / 2 : a.hq;
-    const int span = g.pair_heads ? TILE : g.tiles * TILE;
+    const int span = g.pair_heads ? TILE : NT * TILE;
     const int row_blocks = (a.nq + span - 1) / span;
     const unsigned per_row = (unsigned)units * a.b;
     const int rb = row_blocks - 1 - (int)(blockIdx.x / per_row);
@@ -176,21 +185,21 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     const int b = u / units, h0 = (u % units) * (g.pair_heads ? 2 : 1), kvh = h0 / group;
     const int i0 = rb * span, rows = min(span, a.nq - i0);
     const SeqMask mask(a, b);
-    const int32_t* qd = a.q_doc ? a.q_doc + (int64_t)b * a.nq : nullptr;
-    const int32_t* kd = a.k_doc ? a.k_doc + (int64_t)b * a.nk : nullptr;
+    const int32_t* qd = NT == 1 && a.q_doc ? a.q_doc + (int64_t)b * a.nq : nullptr;
+    const int32_t* kd = NT == 1 && a.k_doc ? a.k_doc + (int64_t)b * a.nk : nullptr;
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
-        for (int s = 0; s < FW_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 2 * TILE); mbar_init(&o_done[t], 1); }
+        for (int s = 0; s < L::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int t = 0; t < NT; ++t) { mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 2 * TILE); mbar_init(&o_done[t], 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         docs[0] = 0x7fffffff; docs[1] = -1; docs[2] = 0;
     }
-    if (warp == FW_MMA) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
+    if (warp == L::MMA) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)L::TMEM));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    if (warp == FW_TMA && lane == 0) {
+    if (warp == L::TMA && lane == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mq.map)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mk.map)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mv.map)) : "memory");
@@ -223,22 +232,22 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     }
     bool masked, ok = true;
 
-    if (warp >= FW_MMA) {
-        if (warp == FW_TMA) {
+    if (warp >= L::MMA) {
+        if (warp == L::TMA) {
             // ------------------------------------------------ TMA
             int kt = walk.next(&masked);
             int n = 0;   // ring entries filled
             if (kt >= 0 && lane == 0) {
-                mbar_expect_tx(q_full, g.tiles * HALVES * L::TILE_B);
-                for (int t = 0; t < g.tiles; ++t)
+                mbar_expect_tx(q_full, NT * HALVES * L::TILE_B);
+                for (int t = 0; t < NT; ++t)
                     for (int f = 0; f < HALVES; ++f)
                         tma_tile(smem_u32(smem + L::Q + (t * HALVES + f) * L::TILE_B), mq, q_full, L::CH,
                                  i0 + (g.pair_heads ? 0 : t * TILE), h0 + (g.pair_heads ? t : 0), b, f * L::CH);
             }
             for (; kt >= 0 && ok; kt = walk.next(&masked)) {
                 for (int w = 0; w < 2 * HALVES && ok; ++w, ++n) {
-                    const int s = n % FW_STAGES;
-                    ok = n < FW_STAGES || mbar_wait(&empty[s], ((n / FW_STAGES) & 1) ^ 1, g.err);
+                    const int s = n % L::STAGES;
+                    ok = n < L::STAGES || mbar_wait(&empty[s], ((n / L::STAGES) & 1) ^ 1, g.err);
                     ok = __all_sync(0xffffffffu, ok);
                     if (ok && lane == 0) {
                         mbar_expect_tx(&full[s], L::TILE_B);
@@ -248,8 +257,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 }
             }
             if (!ok)   // copies in flight land before the block ends
-                for (int e = max(0, n - FW_STAGES); e < n - 1; ++e) mbar_wait(&full[e % FW_STAGES], (e / FW_STAGES) & 1, g.err);
-        } else if (warp == FW_MMA) {
+                for (int e = max(0, n - L::STAGES); e < n - 1; ++e) mbar_wait(&full[e % L::STAGES], (e / L::STAGES) & 1, g.err);
+        } else if (warp == L::MMA) {
             // ------------------------------------------------ tensor cores
             const int ksteps = (a.d + 15) / 16;
             const uint32_t idesc_o = f16_idesc<T>(16 * ksteps, true);
@@ -261,7 +270,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 tc_fence_after();
             };
             // the ring entry e's tile
-            auto entry = [&](int e) { return smem_u32(smem + L::KV + e % FW_STAGES * L::TILE_B); };
+            auto entry = [&](int e) { return smem_u32(smem + L::KV + e % L::STAGES * L::TILE_B); };
             auto scores = [&](int t, int e) {
                 if (ok && elect_one()) {
                     const uint32_t sq = smem_u32(smem + L::Q + t * HALVES * L::TILE_B);
@@ -278,15 +287,15 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 __syncwarp();
             };
             auto free_entries = [&](int e) {   // by one lane
-                for (int f = 0; f < HALVES; ++f) umma_commit(&empty[(e + f) % FW_STAGES]);
+                for (int f = 0; f < HALVES; ++f) umma_commit(&empty[(e + f) % L::STAGES]);
             };
             auto wait_entries = [&](int e) {
-                for (int f = 0; f < HALVES; ++f) wait_full(full, e + f, FW_STAGES);
+                for (int f = 0; f < HALVES; ++f) wait_full(full, e + f, L::STAGES);
             };
             if (kt >= 0) {
                 wait_full(q_full, 0, 1);
                 wait_entries(n);
-                for (int t = 0; t < g.tiles; ++t) scores(t, n);
+                for (int t = 0; t < NT; ++t) scores(t, n);
                 if (ok && elect_one()) free_entries(n);
                 n += HALVES;
             }
@@ -296,7 +305,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 n += HALVES;
                 // rows of V that must not count: 0 probability times what they hold could be NaN
                 if (!SPLIT && ok && ((kd && masked) || (mask.kv < a.nk && (kt + 1) * TILE > mask.kv))) {
-                    clear_rows(smem + L::KV + vs % FW_STAGES * L::TILE_B, L::CH, [&](int r) {
+                    clear_rows(smem + L::KV + vs % L::STAGES * L::TILE_B, L::CH, [&](int r) {
                         const int j = kt * TILE + r;
                         return j >= mask.kv || (kd && kd[j] < 0);
                     });
@@ -306,12 +315,12 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 bool next_masked;
                 const int next = walk.next(&next_masked);
                 if (next >= 0) wait_entries(n);   // the next keys: nothing waits between P V and S
-                for (int t = 0; t < g.tiles; ++t) {
+                for (int t = 0; t < NT; ++t) {
                     ok = ok && mbar_wait(&p_full[t], it & 1, g.err);
                     ok = __all_sync(0xffffffffu, ok);
                     tc_fence_after();
                     if (ok && elect_one()) {
-                        const uint32_t to = tmem + 2 * TILE + t * DO, tp = tmem + t * TILE;
+                        const uint32_t to = tmem + L::T_O + t * DO, tp = tmem + t * TILE;
                         if (HALVES == 2) {
                             mma_parts_split<64>(to, tp, entry(vs), f16_idesc<T>(64, true), 0);
                             mma_parts_split<64>(to + 64, tp, entry(vs + 1), f16_idesc<T>(16 * (ksteps - 4), true), 0);
@@ -335,15 +344,15 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                 masked = next_masked;
             }
         }
-    } else if (warp / 8 < g.tiles) {
+    } else {
         // ---------------------------------------------------- half a row per thread
         const int t = warp / 8, half = warp / 4 % 2, r = threadIdx.x % TILE;
         const int i = i0 + r + (g.pair_heads ? 0 : t * TILE), h = h0 + (g.pair_heads ? t : 0);
         const int p = mask.p0 + i, limit = mask.key_end(i, 1);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         constexpr int DH = DO / 2;            // this thread's columns of O
-        const uint32_t ts = tmem + t * TILE + half * 64 + lanes, to = tmem + 2 * TILE + t * DO + half * DH + lanes;
-        const uint32_t acc = SPLIT ? to + TILE : to;   // the sum over the tiles
+        const uint32_t ts = tmem + t * TILE + half * 64 + lanes, to = tmem + L::T_O + t * DO + half * DH + lanes;
+        const uint32_t acc = SPLIT ? to + NT * DO : to;   // the sum over the tiles
         float* rows_at = reinterpret_cast<float*>(smem + L::ROWS) + t * 2 * TILE + r;   // [parity][tile][half][row]
         // split operands carry powers of two of their heads
         const int e_qk = SPLIT ? split_exp(g.tops.q, b * a.hkv + kvh) + split_exp(g.tops.k, b * a.hkv + kvh) : 0;
@@ -380,7 +389,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             float top = c * score_row<CAP, BIAS, SPLIT, FIX>(x, c1, cap, shift, slope2, p, j0, masked, bits0, bits1);
             if (!FIX) {
                 // the row's other half
-                float* mine_at = rows_at + (it & 1) * 4 * TILE;
+                float* mine_at = rows_at + (it & 1) * 2 * NT * TILE;
                 mine_at[half * TILE] = top;
                 asm volatile("bar.sync %0, 256;" ::"r"(1 + t) : "memory");
                 top = fmaxf(top, mine_at[(1 - half) * TILE]);
@@ -445,7 +454,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
         }
-        float* mine_at = rows_at + (it & 1) * 4 * TILE;
+        float* mine_at = rows_at + (it & 1) * 2 * NT * TILE;
         mine_at[half * TILE] = l;
         asm volatile("bar.sync %0, 256;" ::"r"(1 + t) : "memory");
         l += mine_at[(1 - half) * TILE];
@@ -466,35 +475,57 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == FW_MMA) {
+    if (warp == L::MMA) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::TMEM));
     }
 }
 
-template <typename T, typename U, int DP, bool CAP, bool BIAS, bool FIX = false>
+template <typename T, typename U, int DP, int NT, bool CAP, bool BIAS, bool FIX = false>
 tl_status launch(tl_ctx* c, const HeadMap* m, const FwArgs& g, cudaStream_t s) {
+    using L = Fw<T, U, DP, NT>;
     static std::atomic<uint64_t> done{0};
-    constexpr int smem = FwSmem<(DP > 128 ? 128 : DP)>::BYTES;
-    TL_TRY(kernel_smem(c, k_attn_tc<T, U, DP, CAP, BIAS, FIX>, smem, done));
+    TL_TRY(kernel_smem(c, k_attn_tc<T, U, DP, NT, CAP, BIAS, FIX>, L::BYTES, done));
     const AttnCall& a = g.a;
-    const int span = g.pair_heads ? TILE : g.tiles * TILE;
+    const int span = g.pair_heads ? TILE : NT * TILE;
     const int64_t grid = (int64_t)a.b * (g.pair_heads ? a.hq / 2 : a.hq) * ((a.nq + span - 1) / span);
     cudaEvent_t ev[2];
     launch_begin_on(c, s, "attention_tc", 0, 4.0 * a.d * attn_pairs(a), ev);
     // early behind a kernel of this call
-    TL_CK(c, launch_with(k_attn_tc<T, U, DP, CAP, BIAS, FIX>, dim3((unsigned)grid), 1, FW_THREADS, smem, !std::is_same<T, U>::value || a.k_doc != nullptr, s,
-                         m[0], m[1], m[2], g));
+    TL_CK(c, launch_with(k_attn_tc<T, U, DP, NT, CAP, BIAS, FIX>, dim3((unsigned)grid), 1, L::THREADS, L::BYTES,
+                         L::SPLIT || a.k_doc != nullptr, s, m[0], m[1], m[2], g));
     return launch_end_on(c, s, ev);
 }
 
-template <typename T, typename U, int DP>
+template <typename T, typename U, int DP, int NT>
 tl_status launch_scores(tl_ctx* c, const HeadMap* m, const FwArgs& g, cudaStream_t s) {
     const bool bias = g.a.slopes != nullptr;
     if constexpr (std::is_same<T, __nv_bfloat16>::value)
-        if (g.a.cap > 0.f && !bias && g.a.cap * kLog2e <= kFixTop) return launch<T, U, DP, true, false, true>(c, m, g, s);
-    if (g.a.cap > 0.f) return bias ? launch<T, U, DP, true, true>(c, m, g, s) : launch<T, U, DP, true, false>(c, m, g, s);
-    return bias ? launch<T, U, DP, false, true>(c, m, g, s) : launch<T, U, DP, false, false>(c, m, g, s);
+        if (g.a.cap > 0.f && !bias && g.a.cap * kLog2e <= kFixTop) return launch<T, U, DP, NT, true, false, true>(c, m, g, s);
+    if (g.a.cap > 0.f) return bias ? launch<T, U, DP, NT, true, true>(c, m, g, s) : launch<T, U, DP, NT, true, false>(c, m, g, s);
+    return bias ? launch<T, U, DP, NT, false, true>(c, m, g, s) : launch<T, U, DP, NT, false, false>(c, m, g, s);
+}
+
+template <typename T, typename U, int DP>
+tl_status launch_tiles(tl_ctx* c, const HeadMap* m, FwArgs g, cudaStream_t s) {
+    const AttnCall& a = g.a;
+    // Two tiles a block read each key tile once for both and keep the tensor
+    // cores busier; one leaves two blocks an SM, which even out walks of
+    // different lengths.  bf16, d 128, one tile / two, us: 128 tiles of 2048
+    // keys 38 / 42; causal, 288 tiles 40 / 44, 512 tiles of 512 keys 29 / 32,
+    // of 1024 39 / 40, of 2048 58 / 52; not causal, 192 tiles 47 / 42, 512
+    // tiles 87 / 82; 512 causal tiles of 4096 keys in 16 documents 28 / 31, in 4
+    // 44 / 46, in one 95 / 81.  Lengths of documents are not known here: many
+    // (and two tiles a block have no documents).
+    const int64_t tiles = (int64_t)a.b * a.hq * ((a.nq + TILE - 1) / TILE);
+    const bool one = tiles <= c->sm_count || (a.causal && (tiles <= 2 * c->sm_count || a.nk <= 1024)) || (a.q_doc && a.k_doc);
+    g.pair_heads = 0;
+    if constexpr (DP <= 128)
+        if (!one) {
+            g.pair_heads = a.hq / a.hkv % 2 == 0;
+            return launch_scores<T, U, DP, 2>(c, m, g, s);
+        }
+    return launch_scores<T, U, DP, 1>(c, m, g, s);
 }
 
 }  // namespace
@@ -558,9 +589,6 @@ tl_status launch_attn_tc(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s)
     FwArgs g;
     g.a = a;
     g.k_ranges = static_cast<DocRange*>(ws);
-    // one tile a block while that fills no more than the GPU's SMs at once
-    g.tiles = (int64_t)a.b * a.hq * ((a.nq + TILE - 1) / TILE) <= c->sm_count ? 1 : 2;
-    g.pair_heads = g.tiles == 2 && a.hq / a.hkv % 2 == 0;
     g.key_tiles = (a.nk + TILE - 1) / TILE;
     g.err = c->d_flags + 8;
     if (a.k_doc) TL_TRY(launch_doc_ranges(c, a.k_doc, a.b, a.nk, static_cast<DocRange*>(ws), s));
@@ -573,21 +601,16 @@ tl_status launch_attn_tc(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s)
         g.tops.k = g.tops.q + (size_t)a.b * a.hkv;
         g.tops.v = g.tops.k + (size_t)a.b * a.hkv;
         g.tops.dout = nullptr;
-        if (a.d > 64) {   // a query tile and its sums take what two of the smaller head size do
-            g.tiles = 1;
-            g.pair_heads = 0;
-            return launch_scores<__half, float, 256>(c, m, g, s);
-        }
-        return launch_scores<__half, float, 128>(c, m, g, s);
+        return a.d > 64 ? launch_tiles<__half, float, 256>(c, m, g, s) : launch_tiles<__half, float, 128>(c, m, g, s);
     }
     g.tops = {nullptr, nullptr, nullptr, nullptr};
     if (!make_head_map(&m[0], a.q, a.dtype, a.b, a.hq, a.nq, a.d) || !make_head_map(&m[1], a.k, a.dtype, a.b, a.hkv, a.nk, a.d) ||
         !make_head_map(&m[2], a.v, a.dtype, a.b, a.hkv, a.nk, a.d))
         return fail(c, TL_ERR_CUDA, "attention: tensor maps");
     if (a.dtype == TL_TYPE_F16)
-        return a.d <= 64 ? launch_scores<__half, __half, 64>(c, m, g, s) : launch_scores<__half, __half, 128>(c, m, g, s);
-    return a.d <= 64 ? launch_scores<__nv_bfloat16, __nv_bfloat16, 64>(c, m, g, s)
-                     : launch_scores<__nv_bfloat16, __nv_bfloat16, 128>(c, m, g, s);
+        return a.d <= 64 ? launch_tiles<__half, __half, 64>(c, m, g, s) : launch_tiles<__half, __half, 128>(c, m, g, s);
+    return a.d <= 64 ? launch_tiles<__nv_bfloat16, __nv_bfloat16, 64>(c, m, g, s)
+                     : launch_tiles<__nv_bfloat16, __nv_bfloat16, 128>(c, m, g, s);
 }
 
 }  // namespace tl

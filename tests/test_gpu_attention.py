@@ -467,6 +467,15 @@ def test_many_sequences(ctx, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hq,hkv,nq,nk,d,names", [
+    (4, 2, 130, 70, 128, "len"), (3, 1, 260, 90, 64, "cap"), (4, 1, 130, 300, 40, "slopes len"),
+    (3, 3, 130, 1100, 64, "causal start"), (4, 2, 129, 1030, 96, "cap causal len start"), (6, 2, 200, 130, 72, "docs"),
+    (3, 1, 150, 1040, 24, "cap slopes prefix len start")])
+def test_more_tiles_than_the_gpu_holds_at_once(ctx, hq, hkv, nq, nk, d, names, dtype):
+    compare(ctx, 52, hq, hkv, nq, nk, d, dtype, names, seed=hq + nk, backward=False)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("group", [3, 8, 12, 64])
 def test_groups(ctx, group, dtype):
     compare(ctx, 2, group, 1, 2, 700, 64, dtype, "cap causal len", seed=group)
