@@ -404,6 +404,7 @@ __device__ __forceinline__ bool docs_one(const DocRange& a, const DocRange& b) {
 
 // The tiles of [begin, end) that a block has to visit, 32 at a time: ballots
 // over a lane per tile.  Every warp of a block walks the same list.
+template <bool PART = false>
 struct TileWalk {
     int base, end;
     int clear_lo, clear_hi;       // tiles within need no mask of positions
@@ -411,6 +412,7 @@ struct TileWalk {
     DocRange mine;                // documents of the block's own rows
     uint32_t active, masked;
     int lane;
+    uint32_t ours;                // PART: every `parts`-th tile, of 32 from base on
     __device__ __forceinline__ void fill() {
         const int t = base + lane;
         bool on = t < end, mk = t < clear_lo || t >= clear_hi;
@@ -421,11 +423,14 @@ struct TileWalk {
             mk = mk || !docs_one(mine, r);
         }
         active = __ballot_sync(0xffffffffu, on);
+        if (PART) active &= ours;
         masked = __ballot_sync(0xffffffffu, mk);
     }
-    __device__ __forceinline__ void start(int begin, int end_, int lo, int hi, const DocRange* r, const DocRange& m) {
+    __device__ __forceinline__ void start(int begin, int end_, int lo, int hi, const DocRange* r, const DocRange& m, int parts = 1,
+                                          int part = 0) {
         base = begin; end = end_; clear_lo = lo; clear_hi = hi; ranges = r; mine = m;
         lane = threadIdx.x & 31;
+        if (PART) ours = __ballot_sync(0xffffffffu, ((begin + lane) & (parts - 1)) == part);   // parts divides 32
         active = masked = 0;
         if (base < end) fill();
     }
@@ -442,6 +447,19 @@ struct TileWalk {
         return base + bit;
     }
 };
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// an address of this block's shared memory, in block `rank` of the cluster
+__device__ __forceinline__ uint32_t in_block(uint32_t saddr, int rank) {
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(saddr), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ void load_cluster4(uint32_t at, float (&x)[4]) {
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(at));
+}
 
 // Bits of 32 W other positions whose document is `doc`, lane by lane: the lane
 // holds the documents of positions lane, 32 + lane, ... in other[W] and wants

@@ -6,7 +6,8 @@
 // rows of two heads of a group where the group has an even number of heads
 // (each causal tile then needs exactly the keys the block loads), else
 // neighbouring rows of one head; or one tile (launch_tiles says when), and two
-// such blocks share an SM.  Warps of two tiles:
+// such blocks share an SM.  Few tiles: a cluster's blocks share the keys of one,
+// every parts-th key tile each, and add up.  Warps of two tiles:
 //   0-7, 8-15  tile 0, 1: a thread has 64 of a query's 128 scores: scores out
 //              of TMEM, softmax statistics (the two halves of a row agree on
 //              its maximum through shared memory), probabilities (16-bit) back
@@ -49,6 +50,7 @@ struct FwArgs {
     const DocRange* k_ranges;   // [b, key tiles] with documents
     int pair_heads;             // two tiles: heads h, h + 1 (else rows i0, i0 + 128)
     int key_tiles;
+    int parts;                  // one tile: blocks (a cluster) that share its keys
     SplitTops tops;             // fp32 arrays
     int* err;
 };
@@ -69,6 +71,9 @@ struct Fw {
     static_assert(T_ACC + (SPLIT ? NT * DO : 0) <= 512 && PER_SM * TMEM <= 512, "TMEM columns");
     static constexpr int Q = 0, KV = NT * HALVES * TILE_B, BAR = KV + STAGES * TILE_B, DOCS = BAR + 256, ROWS = DOCS + 64,
                          BYTES = ROWS + 2 * 2 * NT * TILE * 4 + 1024;   // ROWS: [parity][tile][half][row]
+    // shared keys, behind the walk: O as rows padded by 16 bytes, m and l of each row
+    static constexpr int OUT_ROW = DO + 4, STATS = TILE * OUT_ROW * 4;
+    static_assert(STATS + TILE * 8 <= BAR, "the rows to add fit where Q, K and V were");
 };
 
 // the smallest / largest document of each tile of 128 keys (queries), a warp per tile
@@ -154,6 +159,50 @@ __device__ __forceinline__ float score_row(f2 (&x)[32], float c1, const CapCoef<
     return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
 
+// The rows of a tile whose keys the blocks of a cluster shared: with m and l of
+// block q, w_q = 2^(m_q - max m), o = sum w_q O_q / sum w_q l_q, added in the
+// order of the blocks.  Each block stores TILE / parts rows, a warp a row.
+template <typename T, typename U, typename L, bool FIX>
+__device__ void join_parts(uint8_t* smem, const AttnCall& a, const SplitTops& tops, int parts, int part, int b, int h, int kvh, int i0) {
+    const int lane = threadIdx.x & 31, share = TILE / parts, d0 = 4 * lane;
+    const float fix = FIX ? fixed_top(CapCoef<L::SPLIT>(a.scale, a.cap).top) : 0.f;
+    const float out_scale = L::SPLIT ? exp2f((float)-split_exp(tops.v, b * a.hkv + kvh)) : 1.f;
+    for (int r = part * share + threadIdx.x / 32; r < (part + 1) * share && i0 + r < a.nq; r += L::THREADS / 32) {
+        float m = -INFINITY, l = 0.f;
+        if (lane < parts)
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m), "=f"(l) : "r"(in_block(smem_u32(smem + L::STATS) + r * 8, lane)));
+        if (l == 0.f) m = -INFINITY;
+        float top = m;
+        for (int s = 4; s; s /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s, 8));
+        const float w = l == 0.f ? 0.f : ex2(m - top);
+        float sum = 0.f, o[4] = {};
+        for (int q = 0; q < parts; ++q) {
+            const float wq = __shfl_sync(0xffffffffu, w, q);
+            sum += wq * __shfl_sync(0xffffffffu, l, q);
+            if (d0 < L::DO) {
+                float x[4];
+                load_cluster4(in_block(smem_u32(smem) + (r * L::OUT_ROW + d0) * 4, q), x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] += wq * x[e];
+            }
+        }
+        const bool none = sum == 0.f;
+        const float inv = none ? 0.f : out_scale / sum;
+        U* p = static_cast<U*>(a.o.p) + b * a.o.sb + h * a.o.sh + (int64_t)(i0 + r) * a.o.ss;
+        if constexpr (std::is_same<U, float>::value) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (d0 + e < a.d) p[(d0 + e) * a.o.sd] = none ? 0.f : o[e] * inv;
+        } else if (d0 < a.d) {   // d is a multiple of 8, the rows lie on 16 bytes
+            *reinterpret_cast<uint2*>(p + d0) =
+                none ? make_uint2(0, 0) : make_uint2(pack16<U>(o[0] * inv, o[1] * inv), pack16<U>(o[2] * inv, o[3] * inv));
+        }
+        if (a.lse && lane == 0)
+            a.lse[((int64_t)b * a.hq + h) * a.nq + i0 + r] =
+                none ? -INFINITY : (FIX ? fix : top - Lift<T>::log2) * kLn2 + logf(sum);
+    }
+}
+
 // T: operands, U: the arrays' type (float: split operands, DP = 128 or 256 columns
 // of hi and lo).  FIX: see fixed_top.
 template <typename T, typename U, int DP, int NT, bool CAP, bool BIAS, bool FIX>
@@ -180,8 +229,10 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
     const int span = g.pair_heads ? TILE : NT * TILE;
     const int row_blocks = (a.nq + span - 1) / span;
     const unsigned per_row = (unsigned)units * a.b;
-    const int rb = row_blocks - 1 - (int)(blockIdx.x / per_row);
-    const unsigned u = blockIdx.x % per_row;
+    const int parts = NT == 1 ? g.parts : 1, part = NT == 1 ? blockIdx.x % g.parts : 0;
+    const unsigned block = NT == 1 ? blockIdx.x / g.parts : blockIdx.x;
+    const int rb = row_blocks - 1 - (int)(block / per_row);
+    const unsigned u = block % per_row;
     const int b = u / units, h0 = (u % units) * (g.pair_heads ? 2 : 1), kvh = h0 / group;
     const int i0 = rb * span, rows = min(span, a.nq - i0);
     const SeqMask mask(a, b);
@@ -223,12 +274,12 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
         __syncthreads();
         mine = {docs[0], docs[1], docs[2], 0};
     }
-    TileWalk walk;
+    TileWalk<NT == 1> walk;
     {
         const int end = (max(mask.key_end(i0, rows), 0) + TILE - 1) / TILE;
         // every row sees the keys that the first one sees
         const int clear = max(mask.key_end(i0, 1), 0) / TILE;
-        walk.start(0, end, 0, clear, kd ? g.k_ranges + (int64_t)b * g.key_tiles : nullptr, mine);
+        walk.start(0, end, 0, clear, kd ? g.k_ranges + (int64_t)b * g.key_tiles : nullptr, mine, parts, part);
     }
     bool masked, ok = true;
 
@@ -465,7 +516,25 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
             tmem_wait_st();
             inv *= exp2f((float)-split_exp(g.tops.v, b * a.hkv + kvh));
         }
-        if (ok) {
+        if (NT == 1 && parts > 1) {
+            if (ok) {
+                float* to_row = reinterpret_cast<float*>(smem) + r * L::OUT_ROW + half * DH;
+                for (int k = 0; k < DH / 16; ++k) {
+                    uint32_t w[16] = {};
+                    if (it > 0) {
+                        tmem_ld16(acc + 16 * k, w);
+                        tmem_wait_ld();
+                    }
+                    if (none)
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) w[q] = 0;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        reinterpret_cast<uint4*>(to_row + 16 * k)[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+                }
+                if (half == 0) reinterpret_cast<float2*>(smem + L::STATS)[r] = make_float2(FIX ? 0.f : m, none ? 0.f : l);
+            }
+        } else if (ok) {
             HeadsView o = a.o;
             o.p = static_cast<U*>(o.p) + half * DH * o.sd;
             store_row<U, DH>(o, b, h, i, i < a.nq, a.d - half * DH, acc, !none, it > 0, inv);
@@ -479,6 +548,14 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::TMEM));
     }
+    if constexpr (NT == 1) {
+        if (parts > 1) {
+            // TMEM is given back: no block holds any while it waits for its cluster
+            cluster_sync();
+            if (ok) join_parts<T, U, L, FIX>(smem, a, g.tops, parts, part, b, h0, kvh, i0);
+            cluster_sync();   // its rows are read
+        }
+    }
 }
 
 template <typename T, typename U, int DP, int NT, bool CAP, bool BIAS, bool FIX = false>
@@ -488,11 +565,11 @@ tl_status launch(tl_ctx* c, const HeadMap* m, const FwArgs& g, cudaStream_t s) {
     TL_TRY(kernel_smem(c, k_attn_tc<T, U, DP, NT, CAP, BIAS, FIX>, L::BYTES, done));
     const AttnCall& a = g.a;
     const int span = g.pair_heads ? TILE : NT * TILE;
-    const int64_t grid = (int64_t)a.b * (g.pair_heads ? a.hq / 2 : a.hq) * ((a.nq + span - 1) / span);
+    const int64_t grid = (int64_t)a.b * (g.pair_heads ? a.hq / 2 : a.hq) * ((a.nq + span - 1) / span) * g.parts;
     cudaEvent_t ev[2];
     launch_begin_on(c, s, "attention_tc", 0, 4.0 * a.d * attn_pairs(a), ev);
     // early behind a kernel of this call
-    TL_CK(c, launch_with(k_attn_tc<T, U, DP, NT, CAP, BIAS, FIX>, dim3((unsigned)grid), 1, L::THREADS, L::BYTES,
+    TL_CK(c, launch_with(k_attn_tc<T, U, DP, NT, CAP, BIAS, FIX>, dim3((unsigned)grid), g.parts, L::THREADS, L::BYTES,
                          L::SPLIT || a.k_doc != nullptr, s, m[0], m[1], m[2], g));
     return launch_end_on(c, s, ev);
 }
@@ -508,6 +585,7 @@ tl_status launch_scores(tl_ctx* c, const HeadMap* m, const FwArgs& g, cudaStream
 
 template <typename T, typename U, int DP>
 tl_status launch_tiles(tl_ctx* c, const HeadMap* m, FwArgs g, cudaStream_t s) {
+    using L = Fw<T, U, DP, 1>;
     const AttnCall& a = g.a;
     // Two tiles a block read each key tile once for both and keep the tensor
     // cores busier; one leaves two blocks an SM, which even out walks of
@@ -520,11 +598,24 @@ tl_status launch_tiles(tl_ctx* c, const HeadMap* m, FwArgs g, cudaStream_t s) {
     const int64_t tiles = (int64_t)a.b * a.hq * ((a.nq + TILE - 1) / TILE);
     const bool one = tiles <= c->sm_count || (a.causal && (tiles <= 2 * c->sm_count || a.nk <= 1024)) || (a.q_doc && a.k_doc);
     g.pair_heads = 0;
+    g.parts = 1;
     if constexpr (DP <= 128)
         if (!one) {
             g.pair_heads = a.hq / a.hkv % 2 == 0;
             return launch_scores<T, U, DP, 2>(c, m, g, s);
         }
+    // Blocks that would leave the GPU half empty share the keys of a tile among
+    // up to eight, a cluster, which add their rows in shared memory (3 to 4 us).
+    // 1, 2, 4, 8 blocks a tile, us: bf16, d 128, 16 tiles of 32768 keys 496,
+    // 262, 137, 86, of 2048 38, 27, 19, 17; 128 tiles of 2048 38, 30; 32 tiles of 512 keys
+    // 15, 17, 15, 15, of 256 13, 15; fp32, d 64, of 512 32, 31, 26.  A tile of
+    // packed documents meets few of the keys: 64 tiles of 2048 keys in four 17,
+    // 19, 18, 18.  Where a block fills an SM (fp32, d 128, 16 tiles of 2048 keys) 82,
+    // 59, 44, 52: few clusters of eight find their SMs.
+    const int least = a.q_doc ? 32 : L::SPLIT ? 4 : 8;   // key tiles
+    while (g.key_tiles >= least && g.parts < (L::PER_SM == 1 ? 4 : 8) && tiles * g.parts * 2 <= c->sm_count * L::PER_SM &&
+           g.parts * 2 <= g.key_tiles)
+        g.parts *= 2;
     return launch_scores<T, U, DP, 1>(c, m, g, s);
 }
 

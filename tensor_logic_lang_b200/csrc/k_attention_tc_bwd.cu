@@ -53,7 +53,8 @@ struct BwArgs {
     const uint32_t* norms;       // fp16, fp32: [b, hkv][2] largest |dout_i|^2, |v_j|^2 as bits
     const DocRange *q_ranges, *k_ranges;
     SplitTops tops;              // fp32 arrays
-    int q_tiles, k_tiles, cluster;
+    int q_tiles, k_tiles;
+    int cluster, abreast, parts;   // dkv: its blocks take `abreast` heads at once, `parts` of them share a head's query tiles
     // a block a query head instead of a key head's group: its dk and dv go to
     // sums of its own, which k_sum_heads adds (WIDE, heads that share keys)
     int by_head;
@@ -496,25 +497,25 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     if (j0 >= mask.kv) end = 0;
     if (mask.kv < a.nk && j0 + TILE > mask.kv) clear = end;
     const DocRange* ranges = qd ? g.q_ranges + (int64_t)b * g.q_tiles : nullptr;
-    TileWalk walk;
+    TileWalk<true> walk;
     bool masked, ok = true;
     // (head, query tile) pairs in order; qt < 0 after the last
-    int h = (g.by_head ? out_h : kvh * group + rank) - g.cluster;
+    int h = (g.by_head ? out_h : kvh * group + rank / g.parts) - g.abreast;
     const int h_end = g.by_head ? out_h + 1 : (kvh + 1) * group;
     int qt = -1;
     auto first = [&]() { walk.start(0, 0, 0, 0, ranges, mine); };
     auto next = [&]() {
         qt = walk.next(&masked);
         while (qt < 0) {
-            h += g.cluster;
+            h += g.abreast;
             if (h >= h_end) return;
-            walk.start(begin, end, clear, end, ranges, mine);
+            walk.start(begin, end, clear, end, ranges, mine, g.parts, rank & (g.parts - 1));
             qt = walk.next(&masked);
         }
     };
     first();
     next();
-    const bool any = qt >= 0;   // the same for every head
+    const bool any = qt >= 0;
 
     if (warp >= BW_MMA) {
         if (warp == BW_TMA) {
@@ -756,12 +757,14 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             HeadsView v = which ? g.dk : g.dv;
             v.p = static_cast<U*>(v.p) + col0 * v.sd;
             if (ok) store_row<U, DH>(v, b, out_h, j, j < a.nk, a.d - col0, mine_at, any, any, mul);
-        } else if (any && ok) {
+        } else if (ok) {
             float* row = reinterpret_cast<float*>(smem) + (which * TILE + r) * L::SUM_LD + col0;
             for (int k = 0; k < DH / 16; ++k) {
-                uint32_t o[16];
-                tmem_ld16(mine_at + 16 * k, o);
-                tmem_wait_ld();
+                uint32_t o[16] = {};
+                if (any) {
+                    tmem_ld16(mine_at + 16 * k, o);
+                    tmem_wait_ld();
+                }
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                     *reinterpret_cast<float4*>(row + 16 * k + 4 * q) =
@@ -773,7 +776,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     __syncwarp();
     if (g.cluster > 1) {
         // each block adds its share of the rows over the cluster, in the order of the heads
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster_sync();
         if (warp < BW_MMA) {
             const int share = TILE / g.cluster, r0 = rank * share;
             const uint32_t sums = smem_u32(smem);
@@ -782,18 +785,12 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 const int c = e % V, r = r0 + e / V % share, wg = e / V / share;
                 if (j0 + r >= a.nk || 4 * c >= a.d) continue;
                 float s[4] = {0.f, 0.f, 0.f, 0.f};
-                if (any)
-                    for (int q = 0; q < g.cluster; ++q) {
-                        uint32_t at;
-                        float x, y, z, w;
-                        asm("mapa.shared::cluster.u32 %0, %1, %2;"
-                            : "=r"(at)
-                            : "r"(sums + ((wg * TILE + r) * L::SUM_LD + 4 * c) * 4), "r"(q));
-                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                     : "=f"(x), "=f"(y), "=f"(z), "=f"(w)
-                                     : "r"(at));
-                        s[0] += x; s[1] += y; s[2] += z; s[3] += w;
-                    }
+                for (int q = 0; q < g.cluster; ++q) {
+                    float x[4];
+                    load_cluster4(in_block(sums + ((wg * TILE + r) * L::SUM_LD + 4 * c) * 4, q), x);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[k] += x[k];
+                }
                 const HeadsView& v = wg ? a.dk : a.dv;
                 U* p = static_cast<U*>(v.p) + b * v.sb + kvh * v.sh + (int64_t)(j0 + r) * v.ss;
                 if constexpr (SPLIT) {
@@ -807,7 +804,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         }
         __syncwarp();
         // a block's sums stay until the others have read them
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster_sync();
     }
     bb.finish(tmem);
 }
@@ -839,7 +836,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     const uint32_t tmem = bb.setup(qd ? qd + i0 : nullptr, rows, &mine, false);
     const uint32_t t_dp = tmem + (WIDE ? 1 : 2) * TILE, t_dq = t_dp + TILE;
     const uint32_t t_dqa = t_dq + DO;   // split operands: the sum over the tiles
-    TileWalk walk;
+    TileWalk<> walk;
     walk.start(0, (max(mask.key_end(i0, rows), 0) + TILE - 1) / TILE, 0, max(mask.key_end(i0, 1), 0) / TILE,
                kd ? g.k_ranges + (int64_t)b * g.k_tiles : nullptr, mine);
     bool masked, ok = true;
@@ -1129,6 +1126,19 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
     while (g.cluster > 1 && g.cluster < 8 && group % (2 * g.cluster) == 0 &&
            (int64_t)plan.k_tiles * a.b * a.hkv * g.cluster < c->sm_count * 2 / 3)
         g.cluster *= 2;
+    // two blocks of the cluster for a head's query tiles where they and dq's
+    // blocks find SMs of their own (2 x 512 x 4 heads over 2: bf16 24 -> 21, fp32
+    // 57 -> 45 us; 2 x 512 x 8 heads, too many: bf16 22 -> 28); fp32 walks, twice
+    // as long a tile, gain from a causal call's shorter longest one for longer (1024
+    // x 8 heads 82 -> 61, x 16 over 4 88 -> 104).  Four never paid.
+    const int64_t kv_blocks = (int64_t)plan.k_tiles * a.b * a.hkv * g.cluster, q_blocks = (int64_t)plan.q_tiles * a.b * a.hq;
+    g.abreast = g.cluster;
+    g.parts = 1;
+    if (g.cluster <= 4 && plan.q_tiles > 1 &&
+        2 * kv_blocks + q_blocks <= (a.dtype == TL_TYPE_F32 && a.causal ? c->sm_count * 3 / 2 : c->sm_count)) {
+        g.parts = 2;
+        g.cluster *= 2;
+    }
     g.by_head = 0;
     g.dk = a.dk;
     g.dv = a.dv;
@@ -1155,7 +1165,7 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
         TL_CK(c, launch_with(k_attn_prep_f32, dim3((unsigned)(2 * tiles)), 1, 256, 0, true, s, a, stats, plan.q_tiles));
         TL_TRY(launch_end_on(c, s, ev));
         if (a.d > 64) {
-            g.cluster = 1;
+            g.cluster = g.abreast = g.parts = 1;
             if (!sums_by_head(a)) return launch_scores<__half, float, 256>(c, m, g, s);
             float* sums = reinterpret_cast<float*>(w + plan.sums);
             const int64_t one = (int64_t)a.b * a.hq * a.nk * a.d;

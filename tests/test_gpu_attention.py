@@ -476,6 +476,16 @@ def test_more_tiles_than_the_gpu_holds_at_once(ctx, hq, hkv, nq, nk, d, names, d
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("b,hq,hkv,nq,nk,d,names", [
+    (1, 1, 1, 130, 4300, 64, "len start"), (2, 2, 1, 200, 1200, 128, "cap causal start"), (5, 1, 1, 140, 1031, 40, "slopes len"),
+    (1, 2, 2, 260, 4200, 72, "docs"), (2, 1, 1, 300, 4100, 64, "ids"), (3, 2, 1, 150, 2100, 96, "cap slopes prefix len start"),
+    (4, 5, 1, 257, 700, 32, "causal start len"), (4, 1, 1, 135, 9000, 24, "causal start len")])
+def test_few_queries_many_keys(ctx, b, hq, hkv, nq, nk, d, names, dtype):
+    # blocks that share the keys of a query tile, some without any
+    compare(ctx, b, hq, hkv, nq, nk, d, dtype, names, seed=nk)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("group", [3, 8, 12, 64])
 def test_groups(ctx, group, dtype):
     compare(ctx, 2, group, 1, 2, 700, 64, dtype, "cap causal len", seed=group)
