@@ -526,8 +526,10 @@ struct SplitPlan {
     size_t top, norms, data[4], bytes;   // of q, k, v, dout (backward)
     SplitPlan(const AttnCall& a, bool backward);
 };
-// queues the splitting; maps: q, k, v, dout
-tl_status launch_split(tl_ctx* c, const AttnCall& a, bool backward, uint8_t* ws, HeadMap* maps, cudaStream_t s);
+// queues the splitting, and launch_attn_begin for the ranges; maps: q, k, v, dout;
+// stats: of the backward pass, null in a forward one
+tl_status launch_split(tl_ctx* c, const AttnCall& a, float* stats, uint8_t* ws, HeadMap* maps, DocRange* q_ranges, DocRange* k_ranges,
+                       cudaStream_t s);
 // the power of two of a group, from its largest value
 __device__ __forceinline__ int split_exp(const uint32_t* top, int group) {
     const float m = __uint_as_float(top[group]);
@@ -538,6 +540,14 @@ struct SplitTops {
     const uint32_t *q, *k, *v, *dout;    // null: operands are the arrays themselves
 };
 
-tl_status launch_doc_ranges(tl_ctx* c, const int32_t* doc, int b, int n, DocRange* out, cudaStream_t s);
+// the documents' ranges of the query and key tiles (null: not wanted), and zeros
+tl_status launch_attn_begin(tl_ctx* c, const AttnCall& a, DocRange* q_out, DocRange* k_out, uint32_t* zero, int64_t words,
+                            cudaStream_t s);
+
+// ---------------------------------------------------------------- backward
+// of a query tile: -log2(e) lse (+ lift), -D
+constexpr int STAT_BYTES = 2 * TILE * 4;
+template <typename T> struct PLift { static constexpr float log2 = 0.f, back = 1.f; };
+template <> struct PLift<__half> { static constexpr float log2 = 14.f, back = 1.f / 16384.f; };
 
 }  // namespace tl

@@ -18,6 +18,7 @@ struct SplitArgs {
     AttnCall a;
     SplitArray arr[4];
     uint32_t* norms;
+    float* stats;     // backward: [b, hq, query tiles][2][128], -log2(e) lse + lift and -D = -dout.out of each row
 };
 
 __device__ __forceinline__ bool row_counts(const AttnCall& a, const SplitArray& x, int b, int64_t r) {
@@ -34,7 +35,7 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
     if (WRITE) wait_for_previous();   // the largest values
     const AttnCall& a = g.a;
     const SplitArray& x = g.arr[blockIdx.y];
-    const unsigned blocks = (x.n + SP_ROWS - 1) / SP_ROWS;
+    const unsigned blocks = (x.n + TILE - 1) / TILE * (TILE / SP_ROWS);
     if (blockIdx.x >= (int64_t)blocks * x.h * a.b) return;
     const int bh = blockIdx.x / blocks, b = bh / x.h, h = bh % x.h;
     const int group = b * a.hkv + h / (x.h / a.hkv);
@@ -67,6 +68,34 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
             }
         }
     } else {
+        if (g.stats && blockIdx.y == 3) {
+            // dout: D of its rows, and the statistics of whole tiles
+            const float* o = static_cast<const float*>(a.o.p) + b * a.o.sb + h * a.o.sh;
+            const int64_t qt = r0 / TILE, q_tiles = blocks / (TILE / SP_ROWS);
+            float* st = g.stats + ((int64_t)bh * q_tiles + qt) * 2 * TILE + r0 % TILE;
+            const bool live = lane < 8 && row_counts(a, x, b, r0 + lane);
+            const float lse = live ? a.lse[(int64_t)bh * a.nq + r0 + lane] : -INFINITY;
+            float d = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const bool on = row_counts(a, x, b, r0 + k);
+                float dot = 0.f;
+#pragma unroll
+                for (int f = 0; f < HALVES; ++f) {
+                    const int col = c + 64 * f;
+                    if (on && col < a.d) dot = fmaf(u[k][f], o[(r0 + k) * a.o.ss + col * a.o.sd], dot);
+                    if (on && col + 1 < a.d) dot = fmaf(w[k][f], o[(r0 + k) * a.o.ss + (col + 1) * a.o.sd], dot);
+                }
+#pragma unroll
+                for (int m = 16; m; m >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, m);
+                if (lane == k) d = dot;
+            }
+            if (lane < 8) {
+                // a row that sees nothing has p = 2^-inf = 0 everywhere
+                st[lane] = lse == -INFINITY ? -INFINITY : PLift<__half>::log2 - lse * kLog2e;
+                st[TILE + lane] = -d;
+            }
+        }
         float top = 0.f, norm = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -82,6 +111,7 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
                 norm = fmaxf(norm, n2);
             }
         }
+        wait_for_previous();   // the maxima start at 0
         // non-negative floats order like their bits; a maximum does not depend on the order
         const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
         if (lane == 0) {
@@ -107,10 +137,13 @@ SplitPlan::SplitPlan(const AttnCall& a, bool backward) {
     data[3] = take(backward ? q : 0);
 }
 
-tl_status launch_split(tl_ctx* c, const AttnCall& a, bool backward, uint8_t* ws, HeadMap* maps, cudaStream_t s) {
+tl_status launch_split(tl_ctx* c, const AttnCall& a, float* stats, uint8_t* ws, HeadMap* maps, DocRange* q_ranges, DocRange* k_ranges,
+                       cudaStream_t s) {
+    const bool backward = stats != nullptr;
     const SplitPlan plan(a, backward);
     SplitArgs g;
     g.a = a;
+    g.stats = stats;
     uint32_t* top = reinterpret_cast<uint32_t*>(ws + plan.top);
     g.norms = reinterpret_cast<uint32_t*>(ws + plan.norms);
     const int count = backward ? 4 : 3;
@@ -126,17 +159,17 @@ tl_status launch_split(tl_ctx* c, const AttnCall& a, bool backward, uint8_t* ws,
         x.out = reinterpret_cast<__half*>(ws + plan.data[i]);
         x.top = top;
         top += (size_t)a.b * a.hkv;
-        grid = std::max<int64_t>(grid, (int64_t)a.b * x.h * ((x.n + SP_ROWS - 1) / SP_ROWS));
+        grid = std::max<int64_t>(grid, (int64_t)a.b * x.h * ((x.n + TILE - 1) / TILE * (TILE / SP_ROWS)));
         const int64_t w = split_width(a.d);
         const HeadsView flat = {x.out, x.h * x.n * w, x.n * w, w, 1};
         if (!make_head_map(&maps[i], flat, TL_TYPE_F16, a.b, x.h, x.n, (int)w)) return fail(c, TL_ERR_CUDA, "attention: tensor maps");
     }
-    TL_CK(c, cudaMemsetAsync(ws + plan.top, 0, (size_t)a.b * a.hkv * (4 * 4 + 8), s));
+    TL_TRY(launch_attn_begin(c, a, q_ranges, k_ranges, reinterpret_cast<uint32_t*>(ws + plan.top), (int64_t)a.b * a.hkv * 6, s));
     const double bytes = (double)a.b * a.d * ((double)(backward ? 2 : 1) * a.hq * a.nq + 2.0 * a.hkv * a.nk);
     cudaEvent_t ev[2];
     launch_begin_on(c, s, "attention_split_top", 4 * bytes, 0, ev);
     const bool wide = a.d > 64;
-    TL_CK(c, launch_with(wide ? k_split<false, 2> : k_split<false, 1>, dim3((unsigned)grid, count), 1, 256, 0, false, s, g));
+    TL_CK(c, launch_with(wide ? k_split<false, 2> : k_split<false, 1>, dim3((unsigned)grid, count), 1, 256, 0, true, s, g));
     TL_TRY(launch_end_on(c, s, ev));
     launch_begin_on(c, s, "attention_split", 8 * bytes, 0, ev);
     TL_CK(c, launch_with(wide ? k_split<true, 2> : k_split<true, 1>, dim3((unsigned)grid, count), 1, 256, 0, true, s, g));

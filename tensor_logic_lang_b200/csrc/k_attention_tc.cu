@@ -76,13 +76,28 @@ struct Fw {
     static_assert(STATS + TILE * 8 <= BAR, "the rows to add fit where Q, K and V were");
 };
 
-// the smallest / largest document of each tile of 128 keys (queries), a warp per tile
-__global__ void __launch_bounds__(256) k_doc_ranges(const int32_t* __restrict__ doc, int n, int tiles, int64_t total,
-                                                    DocRange* __restrict__ out) {
+// Behind which a call's other kernels start early: the smallest and largest
+// document of each query and key tile (a warp a tile; null: not wanted), and
+// words that maxima are taken in.
+struct BeginArgs {
+    const int32_t *q_doc, *k_doc;
+    int nq, nk;
+    int64_t q_total, k_total;      // tiles of all sequences
+    DocRange *q_out, *k_out;
+    uint32_t* zero;
+    int64_t words;
+};
+__global__ void __launch_bounds__(256) k_attn_begin(const __grid_constant__ BeginArgs g) {
     let_next_start();
     const int lane = threadIdx.x & 31;
-    const int64_t t = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    if (t >= total) return;
+    const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    for (int64_t w = at; w < g.words; w += (int64_t)gridDim.x * blockDim.x) g.zero[w] = 0;
+    int64_t t = at >> 5;
+    if (t >= g.q_total + g.k_total) return;
+    const bool keys = t >= g.q_total;
+    if (keys) t -= g.q_total;
+    const int32_t* doc = keys ? g.k_doc : g.q_doc;
+    const int n = keys ? g.nk : g.nq, tiles = (n + TILE - 1) / TILE;
     const int64_t b = t / tiles;
     const int j0 = (int)(t % tiles) * TILE;
     DocRange r = no_docs();
@@ -96,7 +111,7 @@ __global__ void __launch_bounds__(256) k_doc_ranges(const int32_t* __restrict__ 
     r.lo = __reduce_min_sync(0xffffffffu, r.lo);
     r.hi = __reduce_max_sync(0xffffffffu, r.hi);
     r.pad = __reduce_max_sync(0xffffffffu, r.pad);
-    if (lane == 0) out[t] = r;
+    if (lane == 0) (keys ? g.k_out : g.q_out)[t] = r;
 }
 
 // 64 scores of this thread's row: x (q.k) in registers becomes the
@@ -667,12 +682,16 @@ size_t attn_tc_workspace(const AttnCall& a) {
     return ranges_bytes(a) + (a.dtype == TL_TYPE_F32 ? SplitPlan(a, false).bytes : 0);
 }
 
-tl_status launch_doc_ranges(tl_ctx* c, const int32_t* doc, int b, int n, DocRange* out, cudaStream_t s) {
-    const int tiles = (n + TILE - 1) / TILE;
-    const int64_t total = (int64_t)b * tiles;
+tl_status launch_attn_begin(tl_ctx* c, const AttnCall& a, DocRange* q_out, DocRange* k_out, uint32_t* zero, int64_t words,
+                            cudaStream_t s) {
+    BeginArgs g = {a.q_doc, a.k_doc, a.nq, a.nk, 0, 0, q_out, k_out, zero, words};
+    if (a.q_doc && q_out) g.q_total = (int64_t)a.b * ((a.nq + TILE - 1) / TILE);
+    if (a.k_doc && k_out) g.k_total = (int64_t)a.b * ((a.nk + TILE - 1) / TILE);
+    const int64_t total = g.q_total + g.k_total, zeros = std::min<int64_t>((words + 255) / 256, 64);
+    if (!total && !words) return TL_OK;
     cudaEvent_t ev[2];
-    launch_begin_on(c, s, "attention_doc_ranges", 4.0 * b * n, 0, ev);
-    k_doc_ranges<<<(unsigned)((total + 7) / 8), 256, 0, s>>>(doc, n, tiles, total, out);
+    launch_begin_on(c, s, "attention_begin", 4.0 * total * TILE, 0, ev);
+    k_attn_begin<<<(unsigned)std::max((total + 7) / 8, zeros), 256, 0, s>>>(g);
     return launch_end_on(c, s, ev);
 }
 
@@ -682,18 +701,18 @@ tl_status launch_attn_tc(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s)
     g.k_ranges = static_cast<DocRange*>(ws);
     g.key_tiles = (a.nk + TILE - 1) / TILE;
     g.err = c->d_flags + 8;
-    if (a.k_doc) TL_TRY(launch_doc_ranges(c, a.k_doc, a.b, a.nk, static_cast<DocRange*>(ws), s));
     c->flags_armed = true;
     HeadMap m[4];
     if (a.dtype == TL_TYPE_F32) {
         uint8_t* w = static_cast<uint8_t*>(ws) + ranges_bytes(a);
-        TL_TRY(launch_split(c, a, false, w, m, s));
+        TL_TRY(launch_split(c, a, nullptr, w, m, nullptr, static_cast<DocRange*>(ws), s));
         g.tops.q = reinterpret_cast<const uint32_t*>(w + SplitPlan(a, false).top);
         g.tops.k = g.tops.q + (size_t)a.b * a.hkv;
         g.tops.v = g.tops.k + (size_t)a.b * a.hkv;
         g.tops.dout = nullptr;
         return a.d > 64 ? launch_tiles<__half, float, 256>(c, m, g, s) : launch_tiles<__half, float, 128>(c, m, g, s);
     }
+    TL_TRY(launch_attn_begin(c, a, nullptr, static_cast<DocRange*>(ws), nullptr, 0, s));
     g.tops = {nullptr, nullptr, nullptr, nullptr};
     if (!make_head_map(&m[0], a.q, a.dtype, a.b, a.hq, a.nq, a.d) || !make_head_map(&m[1], a.k, a.dtype, a.b, a.hkv, a.nk, a.d) ||
         !make_head_map(&m[2], a.v, a.dtype, a.b, a.hkv, a.nk, a.d))

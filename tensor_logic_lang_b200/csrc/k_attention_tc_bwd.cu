@@ -42,11 +42,6 @@ namespace {
 constexpr int BW_COMPUTE = 512, BW_THREADS = BW_COMPUTE + 64, BW_STAGES = 2;
 constexpr int BW_MMA = BW_COMPUTE / 32, BW_TMA = BW_MMA + 1;   // warps
 constexpr int BW_COLS = 32;   // scores of a thread
-constexpr int STAT_BYTES = 2 * TILE * 4;   // of a query tile: -log2(e) lse (+ lift), -D
-
-template <typename T> struct PLift { static constexpr float log2 = 0.f, back = 1.f; };
-template <> struct PLift<__half> { static constexpr float log2 = 14.f, back = 1.f / 16384.f; };
-
 struct BwArgs {
     AttnCall a;
     const float* stats;          // [b, hq, query tiles][2][128]
@@ -164,45 +159,16 @@ __global__ void __launch_bounds__(256)
             top = fmaxf(top, xx);
         }
     }
+    wait_for_previous();   // the norms start at 0; the documents' ranges, which the kernel behind this one reads
     if (norms) {
         // non-negative floats order like their bits; a maximum does not depend on the order
+        __shared__ uint32_t most[8];
         const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-        if ((threadIdx.x & 31) == 0) atomicMax(&norms[2 * group_of + (keys ? 1 : 0)], m);
-    }
-}
-
-// The statistics of fp32 arrays of any layout: a warp takes 8 rows, a lane
-// columns 2 lane and 2 lane + 1 of every 64.
-__global__ void __launch_bounds__(256) k_attn_prep_f32(const __grid_constant__ AttnCall a, float* __restrict__ stats, int q_tiles) {
-    let_next_start();
-    wait_for_previous();   // the split operands, which the kernel behind this one reads
-    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, c = 2 * lane;
-    const int64_t blk = blockIdx.x / 2;   // half a tile a block
-    const int qt = (int)(blk % q_tiles), h = (int)(blk / q_tiles % a.hq), b = (int)(blk / q_tiles / a.hq);
-    const int r0 = (blockIdx.x % 2) * 64 + warp * 8;
-    const float* x = static_cast<const float*>(a.dout.p) + b * a.dout.sb + h * a.dout.sh;
-    const float* y = static_cast<const float*>(a.o.p) + b * a.o.sb + h * a.o.sh;
-    float dot[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const int64_t i = qt * TILE + r0 + k;
-        const bool on = i < a.nq && (!a.q_doc || a.q_doc[(int64_t)b * a.nq + i] >= 0);
-        dot[k] = 0.f;
-        for (int e = c; on && e < a.d; e += 64) {
-            dot[k] = fmaf(x[i * a.dout.ss + e * a.dout.sd], y[i * a.o.ss + e * a.o.sd], dot[k]);
-            if (e + 1 < a.d) dot[k] = fmaf(x[i * a.dout.ss + (e + 1) * a.dout.sd], y[i * a.o.ss + (e + 1) * a.o.sd], dot[k]);
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-#pragma unroll
-        for (int w = 16; w; w >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], w);
-        const int64_t i = qt * TILE + r0 + k;
-        if (lane == 0) {
-            const bool on = i < a.nq && (!a.q_doc || a.q_doc[(int64_t)b * a.nq + i] >= 0);
-            const float lse = on ? a.lse[((int64_t)b * a.hq + h) * a.nq + i] : -INFINITY;
-            stats[blk * 2 * TILE + r0 + k] = lse == -INFINITY ? -INFINITY : PLift<__half>::log2 - lse * kLog2e;
-            stats[blk * 2 * TILE + TILE + r0 + k] = -dot[k];
+        if ((threadIdx.x & 31) == 0) most[threadIdx.x / 32] = m;
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            const uint32_t all = __reduce_max_sync(0xffffffffu, most[threadIdx.x & 7]);
+            if (threadIdx.x == 0) atomicMax(&norms[2 * group_of + (keys ? 1 : 0)], all);
         }
     }
 }
@@ -1114,8 +1080,6 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
     g.a = a;
     g.stats = stats;
     g.norms = norms;
-    g.q_ranges = reinterpret_cast<DocRange*>(w + plan.q_ranges);
-    g.k_ranges = reinterpret_cast<DocRange*>(w + plan.k_ranges);
     g.q_tiles = plan.q_tiles;
     g.k_tiles = plan.k_tiles;
     const int group = a.hq / a.hkv;
@@ -1144,10 +1108,9 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
     g.dv = a.dv;
     g.err = c->d_flags + 8;
     c->flags_armed = true;
-    if (a.q_doc) {
-        TL_TRY(launch_doc_ranges(c, a.q_doc, a.b, a.nq, reinterpret_cast<DocRange*>(w + plan.q_ranges), s));
-        TL_TRY(launch_doc_ranges(c, a.k_doc, a.b, a.nk, reinterpret_cast<DocRange*>(w + plan.k_ranges), s));
-    }
+    DocRange *q_ranges = reinterpret_cast<DocRange*>(w + plan.q_ranges), *k_ranges = reinterpret_cast<DocRange*>(w + plan.k_ranges);
+    g.q_ranges = q_ranges;
+    g.k_ranges = k_ranges;
     HeadMap m[4];
     const double rows = (double)a.b * a.hq * a.nq;
     const int64_t tiles = (int64_t)a.b * a.hq * plan.q_tiles;
@@ -1155,15 +1118,12 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
     if (a.dtype == TL_TYPE_F32) {
         uint8_t* sw = w + plan.split;
         const SplitPlan sp(a, true);
-        TL_TRY(launch_split(c, a, true, sw, m, s));
+        TL_TRY(launch_split(c, a, stats, sw, m, q_ranges, k_ranges, s));
         g.norms = reinterpret_cast<const uint32_t*>(sw + sp.norms);
         g.tops.q = reinterpret_cast<const uint32_t*>(sw + sp.top);
         g.tops.k = g.tops.q + (size_t)a.b * a.hkv;
         g.tops.v = g.tops.k + (size_t)a.b * a.hkv;
         g.tops.dout = g.tops.v + (size_t)a.b * a.hkv;
-        launch_begin_on(c, s, "attention_prep", 8.0 * rows * a.d, 2.0 * rows * a.d, ev);
-        TL_CK(c, launch_with(k_attn_prep_f32, dim3((unsigned)(2 * tiles)), 1, 256, 0, true, s, a, stats, plan.q_tiles));
-        TL_TRY(launch_end_on(c, s, ev));
         if (a.d > 64) {
             g.cluster = g.abreast = g.parts = 1;
             if (!sums_by_head(a)) return launch_scores<__half, float, 256>(c, m, g, s);
@@ -1184,11 +1144,12 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
     if (!make_head_map(&m[0], a.q, a.dtype, a.b, a.hq, a.nq, a.d) || !make_head_map(&m[1], a.k, a.dtype, a.b, a.hkv, a.nk, a.d) ||
         !make_head_map(&m[2], a.v, a.dtype, a.b, a.hkv, a.nk, a.d) || !make_head_map(&m[3], a.dout, a.dtype, a.b, a.hq, a.nq, a.d))
         return fail(c, TL_ERR_CUDA, "attention: tensor maps");
-    if (norms) TL_CK(c, cudaMemsetAsync(norms, 0, (size_t)a.b * a.hkv * 8, s));
+    TL_TRY(launch_attn_begin(c, a, q_ranges, k_ranges, norms, norms ? (int64_t)a.b * a.hkv * 2 : 0, s));
     const int64_t blocks = tiles + (norms ? (int64_t)a.b * a.hkv * plan.k_tiles : 0);
     launch_begin_on(c, s, "attention_prep", 4.0 * rows * a.d, 2.0 * rows * a.d, ev);
-    if (a.dtype == TL_TYPE_F16) k_attn_prep<__half><<<(unsigned)(2 * blocks), 256, 0, s>>>(a, stats, norms, plan.q_tiles, plan.k_tiles);
-    else k_attn_prep<__nv_bfloat16><<<(unsigned)(2 * blocks), 256, 0, s>>>(a, stats, norms, plan.q_tiles, plan.k_tiles);
+    // early behind launch_attn_begin's kernel where there is one
+    TL_CK(c, launch_with(a.dtype == TL_TYPE_F16 ? k_attn_prep<__half> : k_attn_prep<__nv_bfloat16>, dim3((unsigned)(2 * blocks)), 1, 256, 0,
+                         norms || a.q_doc, s, a, stats, norms, plan.q_tiles, plan.k_tiles));
     TL_TRY(launch_end_on(c, s, ev));
     if (a.dtype == TL_TYPE_F16)
         return a.d <= 64 ? launch_scores<__half, __half, 64>(c, m, g, s) : launch_scores<__half, __half, 128>(c, m, g, s);
