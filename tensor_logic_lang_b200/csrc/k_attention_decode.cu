@@ -2,7 +2,7 @@
 // over its cache): bound by reading the cache once.
 //
 // The queries of a group's heads that read one key head are the rows of a
-// unit (16 or 32 of them; more rows make more units).  A unit's keys are cut
+// unit (16, 32 or 64 of them; on the CUDA cores 4 or 16, and more rows make more units).  A unit's keys are cut
 // into tiles (of 64, or 128 of head sizes up to 64), the tiles of all units form one line, and each block takes
 // an equal piece of it, whatever the sequences' lengths: all blocks run at
 // once and end together.  A piece that covers a unit whole writes its output;
@@ -413,12 +413,12 @@ __global__ void __launch_bounds__(256) k_doc_spans(const __grid_constant__ AttnC
 template <int DP, int MT>
 struct DmSmem {
     static constexpr int KW = DP == 64 ? 32 : 16, DT = 4 * KW;   // keys of a warp, of a tile
-    // sets of four warps take the tiles in turn; one warp of TMA
-    static constexpr int SETS = MT, WARPS = 4 * SETS, THREADS = 32 * (WARPS + 1), PER_SM = MT == 1 ? 2 : 1;
-    static constexpr int CH = DP / 64, CHUNK = DT * 128, TILE_B = CH * CHUNK, STAGES = 2 * SETS;
+    // four warps for each 16 rows; one of TMA
+    static constexpr int WARPS = 4 * MT, THREADS = 32 * (WARPS + 1), PER_SM = MT == 1 ? 2 : 1;
+    static constexpr int CH = DP / 64, CHUNK = DT * 128, TILE_B = CH * CHUNK, STAGES = MT == 1 ? 2 : 4;
     static constexpr int LQ = DP + 8;   // 16-bit query rows, padded by 16 bytes
     static constexpr int KV = 0, Q = STAGES * 2 * TILE_B, MERGE = Q + 16 * MT * LQ * 2, LO = DP + 4,
-                         STAT = MERGE + WARPS * 16 * LO * 4, PART = STAT + 2 * WARPS * 16 * 4, BAR = PART + 16 * MT * (DP + 2) * 4, BYTES = BAR + 256 + 1024;
+                         STAT = MERGE + 4 * 16 * LO * 4, PART = STAT + 2 * 4 * 16 * 4, BAR = PART + 16 * MT * (DP + 2) * 4, BYTES = BAR + 256 + 1024;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t at, uint32_t* r) {
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     let_next_start();
     if (threadIdx.x == 0) {
-        for (int s = 0; s < L::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 4); }
+        for (int s = 0; s < L::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], L::WARPS); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     PieceWalk walk = block_pieces<L::THREADS / 32>(g, red, found);
@@ -499,8 +499,8 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
     const int ksteps = (a.d + 15) / 16;
     T* qs = reinterpret_cast<T*>(smem + L::Q);
     float* merge = reinterpret_cast<float*>(smem + L::MERGE);
-    float *m_s = reinterpret_cast<float*>(smem + L::STAT), *l_s = m_s + L::WARPS * 16;
-    const int set = warp / 4, sub = warp % 4;
+    float *m_s = reinterpret_cast<float*>(smem + L::STAT), *l_s = m_s + 4 * 16;
+    const int u = warp / 4, sub = warp % 4;   // 16 rows of the unit, a quarter of a tile's keys
     while (walk.next(g, &pc)) {
         const SeqMask mask(a, pc.b);
         const int32_t* kd = a.k_doc ? a.k_doc + (int64_t)pc.b * a.nk : nullptr;
@@ -516,29 +516,32 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
             *reinterpret_cast<uint4*>(qs + r * L::LQ + c) = v;
         }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * L::WARPS) : "memory");
-        DecRow row[MT][2];
-        float m[MT][2], l[MT][2], o[MT][DP / 8][4];
+        DecRow row[2];
+        float m[2], l[2], o[DP / 8][4];
+        const int left = a.nq * (a.hq / a.hkv) - pc.rb * g.rows - 16 * u;   // rows from this warp's first on
+        int all_see = 0x7fffffff;                                           // keys that every row sees
 #pragma unroll
-        for (int u = 0; u < MT; ++u)
+        for (int e = 0; e < 2; ++e) {
+            row[e].set(a, mask, pc.b, pc.kvh, pc.rb * g.rows + 16 * u + gid + 8 * e);
+            if (row[e].on) all_see = min(all_see, row[e].limit);
+            m[e] = -INFINITY;
+            l[e] = 0.f;
+        }
+        all_see = __reduce_min_sync(0xffffffffu, all_see);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                row[u][e].set(a, mask, pc.b, pc.kvh, pc.rb * g.rows + 16 * u + gid + 8 * e);
-                m[u][e] = -INFINITY;
-                l[u][e] = 0.f;
-            }
+        for (int c = 0; c < DP / 8; ++c)
 #pragma unroll
-        for (int u = 0; u < MT; ++u)
-#pragma unroll
-            for (int c = 0; c < DP / 8; ++c)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[u][c][e] = 0.f;
+            for (int e = 0; e < 4; ++e) o[c][e] = 0.f;
         for (int t = pc.t0; t < pc.t1 && ok; ++t, ++n) {
-            if (n % L::SETS != set) continue;
             constexpr int KW = L::KW, NK = KW / 8;   // tiles of 8 keys of a warp
             const int st = n % L::STAGES, j0 = t * L::DT + sub * KW;
             ok = mbar_wait(&full[st], (n / L::STAGES) & 1, g.err);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
+            if (left <= 0) {   // none of the unit's rows are this warp's
+                if (lane == 0) mbar_arrive(&empty[st]);
+                continue;
+            }
             uint8_t* kt = smem + L::KV + 2 * st * L::TILE_B;
             uint8_t* vt = kt + L::TILE_B;
             // keys whose values must not count: 0 times what they hold could be NaN
@@ -555,15 +558,13 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
                 __syncwarp();
             }
             // scores of the warp's keys, 8 to a tile
-            float s[MT][NK][4];
+            float s[NK][4];
 #pragma unroll
-            for (int u = 0; u < MT; ++u)
-#pragma unroll
-                for (int e = 0; e < 4 * NK; ++e) s[u][e / 4][e % 4] = 0.f;
+            for (int e = 0; e < 4 * NK; ++e) s[e / 4][e % 4] = 0.f;
             {
                 const int key = sub * KW + (mi >> 1) * 8 + mr;
                 const uint32_t kb = smem_u32(kt) + key * 128;
-                const uint32_t qb = smem_u32(qs) + ((mi & 1) * 8 + mr) * (L::LQ * 2) + (mi >> 1) * 16;
+                const uint32_t qb = smem_u32(qs) + (16 * u + (mi & 1) * 8 + mr) * (L::LQ * 2) + (mi >> 1) * 16;
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
                     if (k >= ksteps) break;
@@ -572,66 +573,87 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
 #pragma unroll
                     for (int x = 0; x < NK / 2; ++x)
                         ldsm4(kb + x * 16 * 128 + (k / 4) * L::CHUNK + ((c16 ^ (key & 7)) << 4), kf[x]);
+                    uint32_t qf[4];
+                    ldsm4(qb + k * 32, qf);
 #pragma unroll
-                    for (int u = 0; u < MT; ++u) {
-                        uint32_t qf[4];
-                        ldsm4(qb + u * 16 * L::LQ * 2 + k * 32, qf);
-#pragma unroll
-                        for (int x = 0; x < NK / 2; ++x) {
-                            mma16816<T>(s[u][2 * x], qf, kf[x][0], kf[x][1]);
-                            mma16816<T>(s[u][2 * x + 1], qf, kf[x][2], kf[x][3]);
-                        }
+                    for (int x = 0; x < NK / 2; ++x) {
+                        mma16816<T>(s[2 * x], qf, kf[x][0], kf[x][1]);
+                        mma16816<T>(s[2 * x + 1], qf, kf[x][2], kf[x][3]);
                     }
                 }
             }
-            uint32_t p[MT][NK / 2][4];
-#pragma unroll
-            for (int u = 0; u < MT; ++u) {
+            uint32_t p[NK / 2][4];
+            // scores to probabilities; E: 4, or 2 where rows 8..15 are not there
+            auto soft = [&](auto e_count) {
+                constexpr int E = decltype(e_count)::value;
+                const bool masked = kd || j0 + KW > all_see;
                 float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const DecRow& w = row[e >> 1];
+                    const float at = (float)(w.p - j0 - 2 * tid - (e & 1));
+#pragma unroll
+                    for (int x = 0; x < NK; ++x) {
+                        float y = s[x][e];
+                        y = a.cap > 0.f ? cap.top * wide_tanh(y, cap.wide) : y * cap.mul;
+                        s[x][e] = fmaf(-w.slope2, fabsf(at - (float)(8 * x)), y);
+                    }
+                }
+                if (masked) {
+#pragma unroll
+                    for (int x = 0; x < NK; ++x)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            const DecRow& w = row[e >> 1];
+                            const int col = 8 * x + 2 * tid + (e & 1);
+                            const int cdoc = kd ? __shfl_sync(0xffffffffu, jdoc, col) : -1;
+                            if (!(j0 + col < w.limit && (!kd || (w.doc >= 0 && cdoc == w.doc)))) s[x][e] = -INFINITY;
+                        }
+                }
 #pragma unroll
                 for (int x = 0; x < NK; ++x)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int col = 8 * x + 2 * tid + (e & 1);
-                        const int cdoc = kd ? __shfl_sync(0xffffffffu, jdoc, col) : -1;
-                        s[u][x][e] = row[u][e >> 1].score(s[u][x][e], j0 + col, cdoc, a, cap);
-                        top[e >> 1] = fmaxf(top[e >> 1], s[u][x][e]);
-                    }
+                    for (int e = 0; e < E; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[x][e]);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
+                for (int e = 0; e < E / 2; ++e) {
                     top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
                     top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
                 }
                 // the reference maximum moves for a row's first key and by steps of 2^8
-                const bool move = top[0] > m[u][0] + 8.f || top[1] > m[u][1] + 8.f || (m[u][0] == -INFINITY && top[0] > m[u][0]) ||
-                                  (m[u][1] == -INFINITY && top[1] > m[u][1]);
+                bool move = false;
+#pragma unroll
+                for (int e = 0; e < E / 2; ++e) move |= top[e] > m[e] + 8.f || (m[e] == -INFINITY && top[e] > m[e]);
                 if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float nm = fmaxf(m[u][e], top[e]);
-                        const float by = nm == -INFINITY ? 1.f : ex2(m[u][e] - nm);
-                        m[u][e] = nm;
-                        l[u][e] *= by;
+                    for (int e = 0; e < E / 2; ++e) {
+                        const float nm = fmaxf(m[e], top[e]);
+                        const float by = nm == -INFINITY ? 1.f : ex2(m[e] - nm);
+                        m[e] = nm;
+                        l[e] *= by;
 #pragma unroll
                         for (int c = 0; c < DP / 8; ++c) {
-                            o[u][c][2 * e] *= by;
-                            o[u][c][2 * e + 1] *= by;
+                            o[c][2 * e] *= by;
+                            o[c][2 * e + 1] *= by;
                         }
                     }
                 }
+                float ref[2];
+#pragma unroll
+                for (int e = 0; e < E / 2; ++e) ref[e] = (m[e] == -INFINITY ? 0.f : m[e]) - Lift<T>::log2;
 #pragma unroll
                 for (int x = 0; x < NK; ++x) {
-                    float pr[4];
+                    float pr[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float ref = (m[u][e >> 1] == -INFINITY ? 0.f : m[u][e >> 1]) - Lift<T>::log2;
-                        pr[e] = ex2(s[u][x][e] - ref);
-                        l[u][e >> 1] += pr[e];
+                    for (int e = 0; e < E; ++e) {
+                        pr[e] = ex2(s[x][e] - ref[e >> 1]);
+                        l[e >> 1] += pr[e];
                     }
-                    p[u][x / 2][2 * (x % 2)] = pack16<T>(pr[0], pr[1]);
-                    p[u][x / 2][2 * (x % 2) + 1] = pack16<T>(pr[2], pr[3]);
+                    p[x / 2][2 * (x % 2)] = pack16<T>(pr[0], pr[1]);
+                    p[x / 2][2 * (x % 2) + 1] = E == 4 ? pack16<T>(pr[2], pr[3]) : 0u;
                 }
-            }
+            };
+            if (left > 8) soft(std::integral_constant<int, 4>());
+            else soft(std::integral_constant<int, 2>());
             {
                 const int key = sub * KW + (mi & 1) * 8 + mr;
                 const uint32_t vb = smem_u32(vt) + key * 128;
@@ -643,11 +665,8 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
                     for (int x = 0; x < NK / 2; ++x) {
                         uint32_t vf[4];
                         ldsm4t(vb + x * 16 * 128 + (c / 8) * L::CHUNK + ((c16 ^ (key & 7)) << 4), vf);
-#pragma unroll
-                        for (int u = 0; u < MT; ++u) {
-                            mma16816<T>(o[u][c], p[u][x], vf[0], vf[1]);
-                            mma16816<T>(o[u][c + 1], p[u][x], vf[2], vf[3]);
-                        }
+                        mma16816<T>(o[c], p[x], vf[0], vf[1]);
+                        mma16816<T>(o[c + 1], p[x], vf[2], vf[3]);
                     }
                 }
             }
@@ -657,24 +676,27 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
         }
         // the warps' sums, 16 rows at a time
 #pragma unroll
-        for (int u = 0; u < MT; ++u) {
+        for (int e = 0; e < 2; ++e) {
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+        }
+        for (int v = 0; v < MT; ++v) {
+            if (u == v) {
+                float* mw = merge + sub * 16 * L::LO;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                l[u][e] += __shfl_xor_sync(0xffffffffu, l[u][e], 1);
-                l[u][e] += __shfl_xor_sync(0xffffffffu, l[u][e], 2);
-                if (tid == 0) {
-                    m_s[warp * 16 + gid + 8 * e] = m[u][e] == -INFINITY ? -INFINITY : m[u][e] - Lift<T>::log2;
-                    l_s[warp * 16 + gid + 8 * e] = l[u][e];
+                for (int e = 0; e < 2; ++e)
+                    if (tid == 0) {
+                        m_s[sub * 16 + gid + 8 * e] = m[e] == -INFINITY ? -INFINITY : m[e] - Lift<T>::log2;
+                        l_s[sub * 16 + gid + 8 * e] = l[e];
+                    }
+#pragma unroll
+                for (int c = 0; c < DP / 8; ++c) {
+                    *reinterpret_cast<float2*>(mw + gid * L::LO + 8 * c + 2 * tid) = make_float2(o[c][0], o[c][1]);
+                    *reinterpret_cast<float2*>(mw + (gid + 8) * L::LO + 8 * c + 2 * tid) = make_float2(o[c][2], o[c][3]);
                 }
             }
-            float* mw = merge + warp * 16 * L::LO;
-#pragma unroll
-            for (int c = 0; c < DP / 8; ++c) {
-                *reinterpret_cast<float2*>(mw + gid * L::LO + 8 * c + 2 * tid) = make_float2(o[u][c][0], o[u][c][1]);
-                *reinterpret_cast<float2*>(mw + (gid + 8) * L::LO + 8 * c + 2 * tid) = make_float2(o[u][c][2], o[u][c][3]);
-            }
             asm volatile("bar.sync 1, %0;" ::"n"(32 * L::WARPS) : "memory");
-            if (ok) finish_piece<T>(g, pc, merge, L::WARPS, 16 * L::LO, L::LO, m_s, l_s, 16 * u, 16, threadIdx.x, 32 * L::WARPS,
+            if (ok) finish_piece<T>(g, pc, merge, 4, 16 * L::LO, L::LO, m_s, l_s, 16 * v, 16, threadIdx.x, 32 * L::WARPS,
                                     reinterpret_cast<float*>(smem + L::PART));
             asm volatile("bar.sync 1, %0;" ::"n"(32 * L::WARPS) : "memory");
         }
@@ -892,7 +914,7 @@ __global__ void __launch_bounds__(DA_THREADS) k_decode_any(const __grid_constant
 bool few_takes_mma(const AttnCall& a) { return a.dtype != TL_TYPE_F32 && attn_tc_takes(a); }
 int few_rows(const AttnCall& a) {
     const int64_t rows = (int64_t)a.nq * (a.hq / a.hkv);
-    if (few_takes_mma(a)) return rows <= 16 ? 16 : 32;
+    if (few_takes_mma(a)) return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     return rows <= 4 ? 4 : 16;
 }
 int few_blocks(const AttnCall& a) { return (few_takes_mma(a) ? few_rows(a) > 16 : a.d > 128) ? kSms : 2 * kSms; }
@@ -951,8 +973,10 @@ tl_status launch_type(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
     launch_begin_on(c, s, "attention_decode", 2.0 * a.b * a.hkv * (double)a.nk * a.d * sizeof(T), 4.0 * a.d * attn_pairs(a), ev);
     if constexpr (!std::is_same<T, float>::value) {
         if (few_takes_mma(a)) {
-            if (a.d <= 64) TL_TRY((g.rows == 16 ? launch_mma<T, 64, 1>(c, g, s) : launch_mma<T, 64, 2>(c, g, s)));
-            else TL_TRY((g.rows == 16 ? launch_mma<T, 128, 1>(c, g, s) : launch_mma<T, 128, 2>(c, g, s)));
+            if (a.d <= 64)
+                TL_TRY((g.rows == 16 ? launch_mma<T, 64, 1>(c, g, s) : g.rows == 32 ? launch_mma<T, 64, 2>(c, g, s) : launch_mma<T, 64, 4>(c, g, s)));
+            else
+                TL_TRY((g.rows == 16 ? launch_mma<T, 128, 1>(c, g, s) : g.rows == 32 ? launch_mma<T, 128, 2>(c, g, s) : launch_mma<T, 128, 4>(c, g, s)));
             return launch_end_on(c, s, ev);
         }
     }

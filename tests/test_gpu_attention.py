@@ -476,6 +476,16 @@ def test_more_tiles_than_the_gpu_holds_at_once(ctx, hq, hkv, nq, nk, d, names, d
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("names", ["cap causal start len", "slopes docs len", "ids", "prefix start"])
+@pytest.mark.parametrize("b,hq,hkv,nq,nk,d", [
+    (3, 8, 1, 1, 900, 128), (2, 18, 2, 1, 333, 64), (4, 8, 2, 6, 700, 128), (2, 8, 1, 5, 1300, 64), (3, 4, 4, 50, 260, 72),
+    (2, 32, 1, 2, 5000, 128), (40, 6, 2, 11, 150, 128)])
+def test_few_rows(ctx, b, hq, hkv, nq, nk, d, names, dtype):
+    # 1 to 64 rows a key head
+    compare(ctx, b, hq, hkv, nq, nk, d, dtype, names, seed=nq + nk, backward=False)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("b,hq,hkv,nq,nk,d,names", [
     (1, 1, 1, 130, 4300, 64, "len start"), (2, 2, 1, 200, 1200, 128, "cap causal start"), (5, 1, 1, 140, 1031, 40, "slopes len"),
     (1, 2, 2, 260, 4200, 72, "docs"), (2, 1, 1, 300, 4100, 64, "ids"), (3, 2, 1, 150, 2100, 96, "cap slopes prefix len start"),
