@@ -425,6 +425,8 @@ tl_status tl_closure_noalloc(int64_t n, const int64_t* d_rowptr, const int32_t* 
 /* buffer for that stream, which it allocates as needed (and keeps for the   */
 /* 16 streams used last); a stream in capture and the per-thread default     */
 /* stream need one of the caller's (TL_ERR_INVALID) unless the size is 0.    */
+/* A stream whose calls took the context's buffer is destroyed only when its */
+/* work is done: another may get its handle, and with it the buffer.         */
 /* ------------------------------------------------------------------------ */
 #define TL_TYPE_F32  0
 #define TL_TYPE_F16  1

@@ -393,21 +393,51 @@ struct HalfRing {
         }
     }
 };
-// A row's columns col0 .. col0 + N - 1 of an fp32 output (+)= N TMEM columns times mul.
+// A row's columns col0 .. col0 + N - 1 of an fp32 output (+)= N TMEM columns times
+// mul.  32 loads before the first store: a round trip each took 15 us a tile of 96
+// columns, all of them 2.
 template <int N>
 __device__ __forceinline__ void add_row(const HeadsView& v, int b, int h, int64_t row, int col0, bool on, int d, uint32_t taddr, float mul,
                                         bool fresh) {
-    float* p = static_cast<float*>(v.p) + b * v.sb + h * v.sh + row * v.ss;
-    for (int k = 0; k < N; k += 16) {
-        uint32_t o[16];
-        tmem_ld16(taddr + k, o);
-        tmem_wait_ld();
-        if (on)
+    float* p = static_cast<float*>(v.p) + b * v.sb + h * v.sh + row * v.ss + col0 * v.sd;
+    const bool wide = v.sd == 1 && d % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+#pragma unroll 1
+    for (int k = 0; k < N; k += 32) {
+        const int left = on ? d - col0 - k : 0;   // columns from here on
+        float old[32];
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
-                const int c = col0 + k + q;
-                if (c < d) p[c * v.sd] = __uint_as_float(o[q]) * mul + (fresh ? 0.f : p[c * v.sd]);
+        for (int q = 0; q < 32; ++q) old[q] = 0.f;
+        if (!fresh) {
+            if (wide) {
+#pragma unroll
+                for (int q = 0; q < 32; q += 4)
+                    if (q < left) {
+                        const float4 x = *reinterpret_cast<const float4*>(p + k + q);
+                        old[q] = x.x; old[q + 1] = x.y; old[q + 2] = x.z; old[q + 3] = x.w;
+                    }
+            } else {
+#pragma unroll
+                for (int q = 0; q < 32; ++q)
+                    if (q < left) old[q] = p[(k + q) * v.sd];
             }
+        }
+#pragma unroll
+        for (int f = 0; f < 32; f += 16) {
+            uint32_t o[16];
+            tmem_ld16(taddr + k + f, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int q = 0; q < 16; ++q) old[f + q] = fmaf(__uint_as_float(o[q]), mul, old[f + q]);
+        }
+        if (wide) {
+#pragma unroll
+            for (int q = 0; q < 32; q += 4)
+                if (q < left) *reinterpret_cast<float4*>(p + k + q) = make_float4(old[q], old[q + 1], old[q + 2], old[q + 3]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 32; ++q)
+                if (q < left) p[(k + q) * v.sd] = old[q];
+        }
     }
 }
 
@@ -1001,18 +1031,25 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 }
 
 // dk and dv of a key head: the sums of its group's heads, in their order.
+// Blocks of 8 rows of a key head, a warp a row.
 __global__ void __launch_bounds__(256) k_sum_heads(const __grid_constant__ AttnCall a, const float* __restrict__ dk, const float* __restrict__ dv) {
-    const int64_t n = (int64_t)a.nk * a.d, total = (int64_t)a.b * a.hkv * n;
-    const int group = a.hq / a.hkv;
+    const int64_t n = (int64_t)a.nk * a.d;
+    const int group = a.hq / a.hkv, lane = threadIdx.x & 31, blocks = (a.nk + 7) / 8;
+    const int bh = blockIdx.x / blocks, row = blockIdx.x % blocks * 8 + threadIdx.x / 32;
     wait_for_previous();
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < 2 * total; e += (int64_t)gridDim.x * 256) {
-        const bool is_v = e >= total;
-        const int64_t x = is_v ? e - total : e, bh = x / n, at = x % n;
-        const float* p = (is_v ? dv : dk) + bh * group * n + at;
-        float sum = 0.f;
-        for (int q = 0; q < group; ++q) sum += p[q * n];
-        const HeadsView& v = is_v ? a.dv : a.dk;
-        static_cast<float*>(v.p)[bh / a.hkv * v.sb + bh % a.hkv * v.sh + at / a.d * v.ss + at % a.d * v.sd] = sum;
+    if (row >= a.nk) return;
+    for (int w = 0; w < 2; ++w) {
+        const float* p = (w ? dv : dk) + bh * group * n + (int64_t)row * a.d;
+        const HeadsView& v = w ? a.dv : a.dk;
+        float* out = static_cast<float*>(v.p) + bh / a.hkv * v.sb + bh % a.hkv * v.sh + row * v.ss;
+        float sum[4] = {};   // columns lane, lane + 32, ...
+        for (int q = 0; q < group; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (lane + 32 * e < a.d) sum[e] += p[q * n + lane + 32 * e];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (lane + 32 * e < a.d) out[(lane + 32 * e) * v.sd] = sum[e];
     }
 }
 
@@ -1134,8 +1171,8 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
             g.dv = {sums + one, g.dk.sb, g.dk.sh, g.dk.ss, 1};
             TL_TRY((launch_scores<__half, float, 256>(c, m, g, s)));
             launch_begin_on(c, s, "attention_sum_heads", 4.0 * 2 * (one + one / a.hq * a.hkv), 0, ev);
-            TL_CK(c, launch_with(k_sum_heads, dim3((unsigned)std::min<int64_t>((2 * one / a.hq * a.hkv + 255) / 256, 148 * 8)), 1, 256, 0,
-                                 false, s, a, static_cast<const float*>(sums), static_cast<const float*>(sums + one)));
+            TL_CK(c, launch_with(k_sum_heads, dim3((unsigned)((int64_t)a.b * a.hkv * ((a.nk + 7) / 8))), 1, 256, 0, false, s, a,
+                                 static_cast<const float*>(sums), static_cast<const float*>(sums + one)));
             return launch_end_on(c, s, ev);
         }
         return launch_scores<__half, float, 128>(c, m, g, s);
