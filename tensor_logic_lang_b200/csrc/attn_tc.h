@@ -501,7 +501,7 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int chunks, F bad) {
 }
 
 // host: the tensor map of one array (k_attention_tc.cu)
-bool make_head_map(HeadMap* m, const HeadsView& v, int dtype, int b, int h, int64_t n, int d, int box_rows = TILE);
+bool make_head_map(HeadMap* m, const HeadsView& v, int dtype, int b, int h, int64_t n, int d, int box_rows = TILE, int box_heads = 1);
 // the arrays a tensor-core kernel takes: 16-bit, head size contiguous, 16-byte
 // aligned rows
 bool tc_array(const HeadsView& v, int b, int h, int64_t n);

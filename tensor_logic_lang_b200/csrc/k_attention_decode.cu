@@ -2,7 +2,7 @@
 // over its cache): bound by reading the cache once.
 //
 // The queries of a group's heads that read one key head are the rows of a
-// unit (16, 32 or 64 of them; on the CUDA cores 4 or 16, and more rows make more units).  A unit's keys are cut
+// unit (16 of them, or 4 on the CUDA cores; more rows make more units).  A unit's keys are cut
 // into tiles (of 64, or 128 of head sizes up to 64), the tiles of all units form one line, and each block takes
 // an equal piece of it, whatever the sequences' lengths: all blocks run at
 // once and end together.  A piece that covers a unit whole writes its output;
@@ -410,15 +410,14 @@ __global__ void __launch_bounds__(256) k_doc_spans(const __grid_constant__ AttnC
 
 // ---------------------------------------------------------------- tensor cores
 
-template <int DP, int MT>
+template <int DP>
 struct DmSmem {
     static constexpr int KW = DP == 64 ? 32 : 16, DT = 4 * KW;   // keys of a warp, of a tile
-    // four warps for each 16 rows; one of TMA
-    static constexpr int WARPS = 4 * MT, THREADS = 32 * (WARPS + 1), PER_SM = MT == 1 ? 2 : 1;
-    static constexpr int CH = DP / 64, CHUNK = DT * 128, TILE_B = CH * CHUNK, STAGES = MT == 1 ? 2 : 4;
+    static constexpr int WARPS = 4, THREADS = 32 * (WARPS + 1), PER_SM = 2;   // and one of TMA
+    static constexpr int CH = DP / 64, CHUNK = DT * 128, TILE_B = CH * CHUNK, STAGES = 2;
     static constexpr int LQ = DP + 8;   // 16-bit query rows, padded by 16 bytes
-    static constexpr int KV = 0, Q = STAGES * 2 * TILE_B, MERGE = Q + 16 * MT * LQ * 2, LO = DP + 4,
-                         STAT = MERGE + 4 * 16 * LO * 4, PART = STAT + 2 * 4 * 16 * 4, BAR = PART + 16 * MT * (DP + 2) * 4, BYTES = BAR + 256 + 1024;
+    static constexpr int KV = 0, Q = STAGES * 2 * TILE_B, MERGE = Q + 16 * LQ * 2, LO = DP + 4,
+                         STAT = MERGE + WARPS * 16 * LO * 4, PART = STAT + 2 * WARPS * 16 * 4, BAR = PART + 16 * (DP + 2) * 4, BYTES = BAR + 256 + 1024;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t at, uint32_t* r) {
@@ -445,11 +444,10 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// MT: tiles of 16 rows of a unit
-template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_SM)
+template <typename T, int DP>
+__global__ void __launch_bounds__(DmSmem<DP>::THREADS, DmSmem<DP>::PER_SM)
     k_decode_mma(const __grid_constant__ HeadMap mk, const __grid_constant__ HeadMap mv, const __grid_constant__ DecArgs g) {
-    using L = DmSmem<DP, MT>;
+    using L = DmSmem<DP>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR);
@@ -499,13 +497,12 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
     const int ksteps = (a.d + 15) / 16;
     T* qs = reinterpret_cast<T*>(smem + L::Q);
     float* merge = reinterpret_cast<float*>(smem + L::MERGE);
-    float *m_s = reinterpret_cast<float*>(smem + L::STAT), *l_s = m_s + 4 * 16;
-    const int u = warp / 4, sub = warp % 4;   // 16 rows of the unit, a quarter of a tile's keys
+    float *m_s = reinterpret_cast<float*>(smem + L::STAT), *l_s = m_s + L::WARPS * 16;
     while (walk.next(g, &pc)) {
         const SeqMask mask(a, pc.b);
         const int32_t* kd = a.k_doc ? a.k_doc + (int64_t)pc.b * a.nk : nullptr;
         // the unit's query rows (zeros past the last one and past the head size)
-        for (int e = threadIdx.x; e < 16 * MT * DP / 8; e += 32 * L::WARPS) {
+        for (int e = threadIdx.x; e < 16 * DP / 8; e += 32 * L::WARPS) {
             const int r = e / (DP / 8), c = e % (DP / 8) * 8, row = pc.rb * g.rows + r;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (row < a.nq * (a.hq / a.hkv) && c < a.d) {
@@ -518,11 +515,11 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
         asm volatile("bar.sync 1, %0;" ::"n"(32 * L::WARPS) : "memory");
         DecRow row[2];
         float m[2], l[2], o[DP / 8][4];
-        const int left = a.nq * (a.hq / a.hkv) - pc.rb * g.rows - 16 * u;   // rows from this warp's first on
-        int all_see = 0x7fffffff;                                           // keys that every row sees
+        const int left = a.nq * (a.hq / a.hkv) - pc.rb * g.rows;   // rows from the unit's first on
+        int all_see = 0x7fffffff;                                  // keys that every row sees
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            row[e].set(a, mask, pc.b, pc.kvh, pc.rb * g.rows + 16 * u + gid + 8 * e);
+            row[e].set(a, mask, pc.b, pc.kvh, pc.rb * g.rows + gid + 8 * e);
             if (row[e].on) all_see = min(all_see, row[e].limit);
             m[e] = -INFINITY;
             l[e] = 0.f;
@@ -534,14 +531,10 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
             for (int e = 0; e < 4; ++e) o[c][e] = 0.f;
         for (int t = pc.t0; t < pc.t1 && ok; ++t, ++n) {
             constexpr int KW = L::KW, NK = KW / 8;   // tiles of 8 keys of a warp
-            const int st = n % L::STAGES, j0 = t * L::DT + sub * KW;
+            const int st = n % L::STAGES, j0 = t * L::DT + warp * KW;
             ok = mbar_wait(&full[st], (n / L::STAGES) & 1, g.err);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            if (left <= 0) {   // none of the unit's rows are this warp's
-                if (lane == 0) mbar_arrive(&empty[st]);
-                continue;
-            }
             uint8_t* kt = smem + L::KV + 2 * st * L::TILE_B;
             uint8_t* vt = kt + L::TILE_B;
             // keys whose values must not count: 0 times what they hold could be NaN
@@ -554,7 +547,7 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
                     for (int c = 0; c < L::CH; ++c)
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
-                            *reinterpret_cast<uint4*>(vt + c * L::CHUNK + (sub * KW + lane) * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(vt + c * L::CHUNK + (warp * KW + lane) * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
                 __syncwarp();
             }
             // scores of the warp's keys, 8 to a tile
@@ -562,9 +555,9 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
 #pragma unroll
             for (int e = 0; e < 4 * NK; ++e) s[e / 4][e % 4] = 0.f;
             {
-                const int key = sub * KW + (mi >> 1) * 8 + mr;
+                const int key = warp * KW + (mi >> 1) * 8 + mr;
                 const uint32_t kb = smem_u32(kt) + key * 128;
-                const uint32_t qb = smem_u32(qs) + (16 * u + (mi & 1) * 8 + mr) * (L::LQ * 2) + (mi >> 1) * 16;
+                const uint32_t qb = smem_u32(qs) + ((mi & 1) * 8 + mr) * (L::LQ * 2) + (mi >> 1) * 16;
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
                     if (k >= ksteps) break;
@@ -655,7 +648,7 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
             if (left > 8) soft(std::integral_constant<int, 4>());
             else soft(std::integral_constant<int, 2>());
             {
-                const int key = sub * KW + (mi & 1) * 8 + mr;
+                const int key = warp * KW + (mi & 1) * 8 + mr;
                 const uint32_t vb = smem_u32(vt) + key * 128;
 #pragma unroll
                 for (int c = 0; c < DP / 8; c += 2) {
@@ -674,32 +667,26 @@ __global__ void __launch_bounds__(DmSmem<DP, MT>::THREADS, DmSmem<DP, MT>::PER_S
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[st]);
         }
-        // the warps' sums, 16 rows at a time
+        // the warps' sums
+        float* mw = merge + warp * 16 * L::LO;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
             l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-        }
-        for (int v = 0; v < MT; ++v) {
-            if (u == v) {
-                float* mw = merge + sub * 16 * L::LO;
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    if (tid == 0) {
-                        m_s[sub * 16 + gid + 8 * e] = m[e] == -INFINITY ? -INFINITY : m[e] - Lift<T>::log2;
-                        l_s[sub * 16 + gid + 8 * e] = l[e];
-                    }
-#pragma unroll
-                for (int c = 0; c < DP / 8; ++c) {
-                    *reinterpret_cast<float2*>(mw + gid * L::LO + 8 * c + 2 * tid) = make_float2(o[c][0], o[c][1]);
-                    *reinterpret_cast<float2*>(mw + (gid + 8) * L::LO + 8 * c + 2 * tid) = make_float2(o[c][2], o[c][3]);
-                }
+            if (tid == 0) {
+                m_s[warp * 16 + gid + 8 * e] = m[e] == -INFINITY ? -INFINITY : m[e] - Lift<T>::log2;
+                l_s[warp * 16 + gid + 8 * e] = l[e];
             }
-            asm volatile("bar.sync 1, %0;" ::"n"(32 * L::WARPS) : "memory");
-            if (ok) finish_piece<T>(g, pc, merge, 4, 16 * L::LO, L::LO, m_s, l_s, 16 * v, 16, threadIdx.x, 32 * L::WARPS,
-                                    reinterpret_cast<float*>(smem + L::PART));
-            asm volatile("bar.sync 1, %0;" ::"n"(32 * L::WARPS) : "memory");
         }
+#pragma unroll
+        for (int c = 0; c < DP / 8; ++c) {
+            *reinterpret_cast<float2*>(mw + gid * L::LO + 8 * c + 2 * tid) = make_float2(o[c][0], o[c][1]);
+            *reinterpret_cast<float2*>(mw + (gid + 8) * L::LO + 8 * c + 2 * tid) = make_float2(o[c][2], o[c][3]);
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * L::WARPS) : "memory");
+        if (ok) finish_piece<T>(g, pc, merge, L::WARPS, 16 * L::LO, L::LO, m_s, l_s, 0, 16, threadIdx.x, 32 * L::WARPS,
+                                reinterpret_cast<float*>(smem + L::PART));
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * L::WARPS) : "memory");
     }
     if (g.cluster > 1) join_cluster<T>(g, pc, reinterpret_cast<float*>(smem + L::PART), 32 * L::WARPS);
 }
@@ -914,10 +901,9 @@ __global__ void __launch_bounds__(DA_THREADS) k_decode_any(const __grid_constant
 bool few_takes_mma(const AttnCall& a) { return a.dtype != TL_TYPE_F32 && attn_tc_takes(a); }
 int few_rows(const AttnCall& a) {
     const int64_t rows = (int64_t)a.nq * (a.hq / a.hkv);
-    if (few_takes_mma(a)) return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-    return rows <= 4 ? 4 : 16;
+    return !few_takes_mma(a) && rows <= 4 ? 4 : 16;
 }
-int few_blocks(const AttnCall& a) { return (few_takes_mma(a) ? few_rows(a) > 16 : a.d > 128) ? kSms : 2 * kSms; }
+int few_blocks(const AttnCall& a) { return a.d > 128 ? kSms : 2 * kSms; }
 
 struct DecPlan {
     size_t part, spans, bytes;
@@ -929,18 +915,18 @@ struct DecPlan {
     }
 };
 
-template <typename T, int DP, int MT>
+template <typename T, int DP>
 tl_status launch_mma(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
-    constexpr int smem = DmSmem<DP, MT>::BYTES;
-    TL_TRY(kernel_smem(c, k_decode_mma<T, DP, MT>, smem, done));
+    constexpr int smem = DmSmem<DP>::BYTES;
+    TL_TRY(kernel_smem(c, k_decode_mma<T, DP>, smem, done));
     const AttnCall& a = g.a;
     HeadMap mk, mv;
-    if (!make_head_map(&mk, a.k, a.dtype, a.b, a.hkv, a.nk, a.d, DmSmem<DP, MT>::DT) ||
-        !make_head_map(&mv, a.v, a.dtype, a.b, a.hkv, a.nk, a.d, DmSmem<DP, MT>::DT))
+    if (!make_head_map(&mk, a.k, a.dtype, a.b, a.hkv, a.nk, a.d, DmSmem<DP>::DT) ||
+        !make_head_map(&mv, a.v, a.dtype, a.b, a.hkv, a.nk, a.d, DmSmem<DP>::DT))
         return fail(c, TL_ERR_CUDA, "attention: tensor maps");
     c->flags_armed = true;
-    TL_CK(c, launch_with(k_decode_mma<T, DP, MT>, dim3(g.blocks), g.cluster, DmSmem<DP, MT>::THREADS, smem, false, s, mk, mv, g));
+    TL_CK(c, launch_with(k_decode_mma<T, DP>, dim3(g.blocks), g.cluster, DmSmem<DP>::THREADS, smem, false, s, mk, mv, g));
     return TL_OK;
 }
 
@@ -973,10 +959,8 @@ tl_status launch_type(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
     launch_begin_on(c, s, "attention_decode", 2.0 * a.b * a.hkv * (double)a.nk * a.d * sizeof(T), 4.0 * a.d * attn_pairs(a), ev);
     if constexpr (!std::is_same<T, float>::value) {
         if (few_takes_mma(a)) {
-            if (a.d <= 64)
-                TL_TRY((g.rows == 16 ? launch_mma<T, 64, 1>(c, g, s) : g.rows == 32 ? launch_mma<T, 64, 2>(c, g, s) : launch_mma<T, 64, 4>(c, g, s)));
-            else
-                TL_TRY((g.rows == 16 ? launch_mma<T, 128, 1>(c, g, s) : g.rows == 32 ? launch_mma<T, 128, 2>(c, g, s) : launch_mma<T, 128, 4>(c, g, s)));
+            if (a.d <= 64) TL_TRY((launch_mma<T, 64>(c, g, s)));
+            else TL_TRY((launch_mma<T, 128>(c, g, s)));
             return launch_end_on(c, s, ev);
         }
     }
@@ -988,9 +972,22 @@ tl_status launch_type(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
 
 }  // namespace
 
+// Where these kernels are faster than the tiles of 128 queries, if the tensor
+// cores take the call at all.  us here / there, one head a group:
+//   bf16, d 128, 16 x 8 heads of 4096 keys: 4 rows 51 / 52, 12 rows 61 / 53; with
+//     lengths of their own the pieces here stay equal
+//   fp16, d 64, the same: 12 rows 37 / 41, 24 rows 52 / 42
+//   fp32, d 64, 4 x 16 heads of 4096 keys: 4 rows 49 / 147, 12 rows 172 / 148
+// and where few tiles, each shared by eight blocks at most, would walk a long
+// cache: 64 rows of one head, 65536 keys: bf16, d 128 50 / 134, fp16, d 64 28 / 109,
+// fp32, d 64 172 / 272; of two heads, 32768 keys: 42 / 72, 25 / 60, 168 / 155.
 bool attn_few_takes(const AttnCall& a) {
     const int64_t rows = (int64_t)a.nq * (a.hq / a.hkv);
-    return a.nk > 0 && rows <= 64;
+    if (a.nk == 0 || rows > 64) return false;
+    if (!attn_tc_takes(a)) return true;
+    const bool f32 = a.dtype == TL_TYPE_F32;
+    if (a.nk >= 8192 && (int64_t)a.b * a.hkv * ((rows + 15) / 16) <= (f32 ? 4 : a.d <= 64 ? 32 : 12)) return true;
+    return rows <= (f32 ? 4 : a.d <= 64 || a.kv_len ? 16 : 8);
 }
 
 size_t attn_few_workspace(const AttnCall& a) { return DecPlan(a).bytes; }
@@ -1009,8 +1006,11 @@ tl_status launch_attn_few(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s
     const int64_t units = (int64_t)a.b * a.hkv * g.row_blocks, rows = (int64_t)a.nq * (a.hq / a.hkv);
     g.tile = few_takes_mma(a) && a.d <= 64 ? 128 : 64;
     const int64_t tiles = (a.nk + g.tile - 1) / g.tile;
-    // a cluster a unit while all of them run at once and a block has few tiles
-    g.cluster = units * 8 <= kSms && tiles <= 32 ? 8 : 1;
+    // A cluster a unit while all of them run at once and a block has few tiles: one
+    // launch for two.  Cluster / line, us: bf16, 1 x 32 heads over 8, 512 keys 6.9 / 8.8,
+    // 2048 9.9 / 11.8, 2 x 32 heads, 4096 14.9 / 13.9; fp32, 512 keys 9.3 / 11.0, 1024 14.3 /
+    // 13.5, 2048 18 / 15.
+    g.cluster = units * 8 <= kSms && tiles <= (few_takes_mma(a) ? 32 : 8) ? 8 : 1;
     g.blocks = g.cluster > 1 ? (int)units * g.cluster : (int)std::min<int64_t>(few_blocks(a), units * tiles);
     cudaEvent_t ev[2];
     if (a.k_doc) {

@@ -49,6 +49,7 @@ struct FwArgs {
     AttnCall a;
     const DocRange* k_ranges;   // [b, key tiles] with documents
     int pair_heads;             // two tiles: heads h, h + 1 (else rows i0, i0 + 128)
+    int pack;                   // one tile: queries of it, of all heads of a group, head after head; 0: one head's
     int key_tiles;
     int parts;                  // one tile: blocks (a cluster) that share its keys
     SplitTops tops;             // fp32 arrays
@@ -178,11 +179,15 @@ __device__ __forceinline__ float score_row(f2 (&x)[32], float c1, const CapCoef<
 // block q, w_q = 2^(m_q - max m), o = sum w_q O_q / sum w_q l_q, added in the
 // order of the blocks.  Each block stores TILE / parts rows, a warp a row.
 template <typename T, typename U, typename L, bool FIX>
-__device__ void join_parts(uint8_t* smem, const AttnCall& a, const SplitTops& tops, int parts, int part, int b, int h, int kvh, int i0) {
+__device__ void join_parts(uint8_t* smem, const FwArgs& g, int part, int b, int h0, int kvh, int i0) {
+    const AttnCall& a = g.a;
+    const int parts = g.parts, rows = g.pack ? g.pack * (a.hq / a.hkv) : TILE;
     const int lane = threadIdx.x & 31, share = TILE / parts, d0 = 4 * lane;
     const float fix = FIX ? fixed_top(CapCoef<L::SPLIT>(a.scale, a.cap).top) : 0.f;
-    const float out_scale = L::SPLIT ? exp2f((float)-split_exp(tops.v, b * a.hkv + kvh)) : 1.f;
-    for (int r = part * share + threadIdx.x / 32; r < (part + 1) * share && i0 + r < a.nq; r += L::THREADS / 32) {
+    const float out_scale = L::SPLIT ? exp2f((float)-split_exp(g.tops.v, b * a.hkv + kvh)) : 1.f;
+    for (int r = part * share + threadIdx.x / 32; r < min((part + 1) * share, rows); r += L::THREADS / 32) {
+        const int i = g.pack ? i0 + r % g.pack : i0 + r, h = g.pack ? h0 + r / g.pack : h0;
+        if (i >= a.nq) continue;
         float m = -INFINITY, l = 0.f;
         if (lane < parts)
             asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m), "=f"(l) : "r"(in_block(smem_u32(smem + L::STATS) + r * 8, lane)));
@@ -203,7 +208,7 @@ __device__ void join_parts(uint8_t* smem, const AttnCall& a, const SplitTops& to
         }
         const bool none = sum == 0.f;
         const float inv = none ? 0.f : out_scale / sum;
-        U* p = static_cast<U*>(a.o.p) + b * a.o.sb + h * a.o.sh + (int64_t)(i0 + r) * a.o.ss;
+        U* p = static_cast<U*>(a.o.p) + b * a.o.sb + h * a.o.sh + i * a.o.ss;
         if constexpr (std::is_same<U, float>::value) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -213,7 +218,7 @@ __device__ void join_parts(uint8_t* smem, const AttnCall& a, const SplitTops& to
                 none ? make_uint2(0, 0) : make_uint2(pack16<U>(o[0] * inv, o[1] * inv), pack16<U>(o[2] * inv, o[3] * inv));
         }
         if (a.lse && lane == 0)
-            a.lse[((int64_t)b * a.hq + h) * a.nq + i0 + r] =
+            a.lse[((int64_t)b * a.hq + h) * a.nq + i] =
                 none ? -INFINITY : (FIX ? fix : top - Lift<T>::log2) * kLn2 + logf(sum);
     }
 }
@@ -240,15 +245,16 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
     // block -> (rows, heads, sequence); the last rows, which see the most keys
     // of a causal call, go first
     const int group = a.hq / a.hkv;
-    const int units = g.pair_heads ? a.hq / 2 : a.hq;
-    const int span = g.pair_heads ? TILE : NT * TILE;
+    const int pack = NT == 1 ? g.pack : 0;
+    const int units = pack ? a.hkv : g.pair_heads ? a.hq / 2 : a.hq;
+    const int span = pack ? pack : g.pair_heads ? TILE : NT * TILE;
     const int row_blocks = (a.nq + span - 1) / span;
     const unsigned per_row = (unsigned)units * a.b;
     const int parts = NT == 1 ? g.parts : 1, part = NT == 1 ? blockIdx.x % g.parts : 0;
     const unsigned block = NT == 1 ? blockIdx.x / g.parts : blockIdx.x;
     const int rb = row_blocks - 1 - (int)(block / per_row);
     const unsigned u = block % per_row;
-    const int b = u / units, h0 = (u % units) * (g.pair_heads ? 2 : 1), kvh = h0 / group;
+    const int b = u / units, h0 = (u % units) * (pack ? group : g.pair_heads ? 2 : 1), kvh = h0 / group;
     const int i0 = rb * span, rows = min(span, a.nq - i0);
     const SeqMask mask(a, b);
     const int32_t* qd = NT == 1 && a.q_doc ? a.q_doc + (int64_t)b * a.nq : nullptr;
@@ -304,7 +310,7 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
             int kt = walk.next(&masked);
             int n = 0;   // ring entries filled
             if (kt >= 0 && lane == 0) {
-                mbar_expect_tx(q_full, NT * HALVES * L::TILE_B);
+                mbar_expect_tx(q_full, pack ? HALVES * L::CH * pack * group * 128 : NT * HALVES * L::TILE_B);
                 for (int t = 0; t < NT; ++t)
                     for (int f = 0; f < HALVES; ++f)
                         tma_tile(smem_u32(smem + L::Q + (t * HALVES + f) * L::TILE_B), mq, q_full, L::CH,
@@ -413,7 +419,10 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
     } else {
         // ---------------------------------------------------- half a row per thread
         const int t = warp / 8, half = warp / 4 % 2, r = threadIdx.x % TILE;
-        const int i = i0 + r + (g.pair_heads ? 0 : t * TILE), h = h0 + (g.pair_heads ? t : 0);
+        const int head = pack ? r / pack : 0;   // of the group
+        const int i = pack ? i0 + r % pack : i0 + r + (g.pair_heads ? 0 : t * TILE);
+        const int h = h0 + (pack ? min(head, group - 1) : g.pair_heads ? t : 0);
+        const bool on = i < a.nq && (!pack || head < group);
         const int p = mask.p0 + i, limit = mask.key_end(i, 1);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         constexpr int DH = DO / 2;            // this thread's columns of O
@@ -552,8 +561,8 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
         } else if (ok) {
             HeadsView o = a.o;
             o.p = static_cast<U*>(o.p) + half * DH * o.sd;
-            store_row<U, DH>(o, b, h, i, i < a.nq, a.d - half * DH, acc, !none, it > 0, inv);
-            if (a.lse && i < a.nq && half == 0)
+            store_row<U, DH>(o, b, h, i, on, a.d - half * DH, acc, !none, it > 0, inv);
+            if (a.lse && on && half == 0)
                 a.lse[((int64_t)b * a.hq + h) * a.nq + i] = none ? -INFINITY : (FIX ? fix : m - Lift<T>::log2) * kLn2 + logf(l);
         }
     }
@@ -567,7 +576,7 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
         if (parts > 1) {
             // TMEM is given back: no block holds any while it waits for its cluster
             cluster_sync();
-            if (ok) join_parts<T, U, L, FIX>(smem, a, g.tops, parts, part, b, h0, kvh, i0);
+            if (ok) join_parts<T, U, L, FIX>(smem, g, part, b, h0, kvh, i0);
             cluster_sync();   // its rows are read
         }
     }
@@ -579,8 +588,8 @@ tl_status launch(tl_ctx* c, const HeadMap* m, const FwArgs& g, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     TL_TRY(kernel_smem(c, k_attn_tc<T, U, DP, NT, CAP, BIAS, FIX>, L::BYTES, done));
     const AttnCall& a = g.a;
-    const int span = g.pair_heads ? TILE : NT * TILE;
-    const int64_t grid = (int64_t)a.b * (g.pair_heads ? a.hq / 2 : a.hq) * ((a.nq + span - 1) / span) * g.parts;
+    const int span = g.pack ? g.pack : g.pair_heads ? TILE : NT * TILE;
+    const int64_t grid = (int64_t)a.b * (g.pack ? a.hkv : g.pair_heads ? a.hq / 2 : a.hq) * ((a.nq + span - 1) / span) * g.parts;
     cudaEvent_t ev[2];
     launch_begin_on(c, s, "attention_tc", 0, 4.0 * a.d * attn_pairs(a), ev);
     // early behind a kernel of this call
@@ -610,8 +619,8 @@ tl_status launch_tiles(tl_ctx* c, const HeadMap* m, FwArgs g, cudaStream_t s) {
     // tiles 87 / 82; 512 causal tiles of 4096 keys in 16 documents 28 / 31, in 4
     // 44 / 46, in one 95 / 81.  Lengths of documents are not known here: many
     // (and two tiles a block have no documents).
-    const int64_t tiles = (int64_t)a.b * a.hq * ((a.nq + TILE - 1) / TILE);
-    const bool one = tiles <= c->sm_count || (a.causal && (tiles <= 2 * c->sm_count || a.nk <= 1024)) || (a.q_doc && a.k_doc);
+    const int64_t tiles = g.pack ? (int64_t)a.b * a.hkv * ((a.nq + g.pack - 1) / g.pack) : (int64_t)a.b * a.hq * ((a.nq + TILE - 1) / TILE);
+    const bool one = g.pack || tiles <= c->sm_count || (a.causal && (tiles <= 2 * c->sm_count || a.nk <= 1024)) || (a.q_doc && a.k_doc);
     g.pair_heads = 0;
     g.parts = 1;
     if constexpr (DP <= 128)
@@ -650,7 +659,7 @@ bool attn_tc_takes(const AttnCall& a) {
            tc_array(a.v, a.b, a.hkv, a.nk) && tc_array(a.o, a.b, a.hq, a.nq);
 }
 
-bool make_head_map(HeadMap* m, const HeadsView& v, int dtype, int b, int h, int64_t n, int d, int box_rows) {
+bool make_head_map(HeadMap* m, const HeadsView& v, int dtype, int b, int h, int64_t n, int d, int box_rows, int box_heads) {
     typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -668,7 +677,7 @@ bool make_head_map(HeadMap* m, const HeadsView& v, int dtype, int b, int h, int6
     cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)n, m->mh ? (cuuint64_t)h : 1, m->mb ? (cuuint64_t)b : 1};
     const int64_t row = n > 1 ? v.ss : (d + 7) / 8 * 8;
     cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)(m->mh ? v.sh : row) * 2, (cuuint64_t)(m->mb ? v.sb : row) * 2};
-    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, one[4] = {1, 1, 1, 1};
+    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_heads, 1}, one[4] = {1, 1, 1, 1};
     return enc(&m->map, dtype == TL_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, v.p, dims,
                strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -695,6 +704,16 @@ tl_status launch_attn_begin(tl_ctx* c, const AttnCall& a, DocRange* q_out, DocRa
     return launch_end_on(c, s, ev);
 }
 
+// Queries of a tile that holds them for all heads of a group, where that makes
+// fewer tiles (0: it does not): 16 x 64 heads over 8, 8 queries over 4096 keys of
+// bf16, d 128, 260 us by head, 54 packed.
+static int packed_queries(const AttnCall& a) {
+    const int group = a.hq / a.hkv;
+    if (group < 2 || group > TILE || (a.dtype != TL_TYPE_F32 && a.q.sh == 0)) return 0;
+    const int n = std::min(a.nq, TILE / group);
+    return (a.nq + n - 1) / n < (int64_t)group * ((a.nq + TILE - 1) / TILE) ? n : 0;
+}
+
 tl_status launch_attn_tc(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s) {
     FwArgs g;
     g.a = a;
@@ -703,6 +722,8 @@ tl_status launch_attn_tc(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s)
     g.err = c->d_flags + 8;
     c->flags_armed = true;
     HeadMap m[4];
+    g.pack = packed_queries(a);
+    const int group = a.hq / a.hkv, q_rows = g.pack ? g.pack : TILE, q_heads = g.pack ? group : 1;
     if (a.dtype == TL_TYPE_F32) {
         uint8_t* w = static_cast<uint8_t*>(ws) + ranges_bytes(a);
         TL_TRY(launch_split(c, a, nullptr, w, m, nullptr, static_cast<DocRange*>(ws), s));
@@ -710,11 +731,15 @@ tl_status launch_attn_tc(tl_ctx* c, const AttnCall& a, void* ws, cudaStream_t s)
         g.tops.k = g.tops.q + (size_t)a.b * a.hkv;
         g.tops.v = g.tops.k + (size_t)a.b * a.hkv;
         g.tops.dout = nullptr;
+        const int64_t width = split_width(a.d);
+        const HeadsView q = {w + SplitPlan(a, false).data[0], a.hq * a.nq * width, a.nq * width, width, 1};
+        if (g.pack && !make_head_map(&m[0], q, TL_TYPE_F16, a.b, a.hq, a.nq, (int)width, q_rows, q_heads))
+            return fail(c, TL_ERR_CUDA, "attention: tensor maps");
         return a.d > 64 ? launch_tiles<__half, float, 256>(c, m, g, s) : launch_tiles<__half, float, 128>(c, m, g, s);
     }
     TL_TRY(launch_attn_begin(c, a, nullptr, static_cast<DocRange*>(ws), nullptr, 0, s));
     g.tops = {nullptr, nullptr, nullptr, nullptr};
-    if (!make_head_map(&m[0], a.q, a.dtype, a.b, a.hq, a.nq, a.d) || !make_head_map(&m[1], a.k, a.dtype, a.b, a.hkv, a.nk, a.d) ||
+    if (!make_head_map(&m[0], a.q, a.dtype, a.b, a.hq, a.nq, a.d, q_rows, q_heads) || !make_head_map(&m[1], a.k, a.dtype, a.b, a.hkv, a.nk, a.d) ||
         !make_head_map(&m[2], a.v, a.dtype, a.b, a.hkv, a.nk, a.d))
         return fail(c, TL_ERR_CUDA, "attention: tensor maps");
     if (a.dtype == TL_TYPE_F16)

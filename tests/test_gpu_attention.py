@@ -486,6 +486,27 @@ def test_few_rows(ctx, b, hq, hkv, nq, nk, d, names, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("names", ["cap causal start len", "slopes docs len", "ids", "prefix start", ""])
+@pytest.mark.parametrize("b,hq,hkv,nq,nk,d,layout", [
+    (2, 6, 2, 50, 700, 128, "bhsd"), (1, 40, 2, 30, 260, 64, "bshd"), (3, 8, 1, 16, 1000, 128, "packed"), (2, 10, 2, 27, 520, 40, "bshd"),
+    (1, 128, 1, 3, 1100, 64, "bhsd"), (5, 4, 2, 65, 130, 96, "odd")])
+def test_heads_of_a_group_in_one_tile(ctx, b, hq, hkv, nq, nk, d, layout, names, dtype):
+    compare(ctx, b, hq, hkv, nq, nk, d, dtype, names, layout=layout, seed=nq + nk, backward=False)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_queries_broadcast_over_heads(ctx, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    for nq in (2, 20, 150):
+        q = heads(gen, 1, 1, nq, 64, dtype).expand(2, 8, nq, 64)
+        k, v = heads(gen, 2, 2, 300, 64, dtype), heads(gen, 2, 2, 300, 64, dtype)
+        m = {"causal": True, "softcap": 2.0}
+        want, got = reference(q, k, v, **m), run(ctx, q, k, v, None, m)
+        for n in want:
+            check(got[n], want[n], n)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("b,hq,hkv,nq,nk,d,names", [
     (1, 1, 1, 130, 4300, 64, "len start"), (2, 2, 1, 200, 1200, 128, "cap causal start"), (5, 1, 1, 140, 1031, 40, "slopes len"),
     (1, 2, 2, 260, 4200, 72, "docs"), (2, 1, 1, 300, 4100, 64, "ids"), (3, 2, 1, 150, 2100, 96, "cap slopes prefix len start"),
