@@ -1,6 +1,7 @@
 // Attention with modified scores for any type, stride and head size up to
-// 256 (where the tensor-core kernels' rules do not hold, attn_tc_takes): tiles of queries against tiles of keys in shared memory, fp32 FFMA
-// products, one pass over the keys with a running maximum and sum.
+// 256 (where the tensor-core kernels' rules do not hold, attn_tc_takes): tiles of
+// queries against tiles of keys in shared memory, fp32 FFMA products, one pass
+// over the keys with a running maximum and sum.
 //
 //   forward   a block per (sequence, head, query tile):
 //               s = scores(q k), m' = max(m, s), l = l e^{m-m'} + sum e^{s-m'},

@@ -5,7 +5,7 @@
 //
 //   k_attn_prep    by tile of 128 queries: log2(e) lse and D, ready for the
 //                  kernels below; the largest row norms of dout and v (fp16;
-//                  fp32 arrays: k_attn_prep_f32, norms with the splitting)
+//                  fp32 arrays: all of it falls out of the splitting)
 //   k_attn_tc_dkv  a block per (key tile, head): dk and dv stay in TMEM while
 //                  the query tiles pass; the heads of a group form a cluster
 //                  and add their sums through distributed shared memory in a
@@ -32,6 +32,11 @@
 // ones come in halves, each as often as a product needs it (twice, from the L2
 // cache), and dk and dv, which leave no room for sums in TMEM, are added to
 // the outputs every 4 tiles.
+//
+// Bound by the element work between the products: a pair of tiles takes 4500 clocks
+// in either kernel, of which the products fill 2048 (dk, dv) and 1536.  16 heads of 16384
+// queries and keys, bf16, causal, five products counted: d 128 3930 us, 700 TFLOP/s,
+// cap 50 4620; d 64 3030 us, 454 TFLOP/s, cap 50 3710.  fp32, 8 heads of 4096: d 64 278 us, d 96 456.
 #include <algorithm>
 
 #include "attn_tc.h"

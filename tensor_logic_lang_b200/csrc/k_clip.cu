@@ -9,13 +9,12 @@
 //
 // HBM-bound: the list is read once for the norm, and read and written once
 // more where it is scaled, the last chunks first: the L2 cache still holds
-// those.  The blocks take the chunks in turn: runs of chunks for each block were
-// slower.  400M bf16 into fp32, one array: 515 us, 6.2 TB/s of the 3.2 GB that
+// those.  The blocks take the chunks in turn.  400M bf16 into fp32, one array: 515 us, 6.2 TB/s of the 3.2 GB that
 // two reads and a write are; 291 arrays: 546 us; 360 MB of fp32 under the limit:
 // 61 us, 5.9 TB/s.  A chunk is a piece of one array; the list travels in the launch's
 // parameters (no copy, so a captured call keeps it).  128-bit loads, eight
-// in flight a thread (four: 585 us), stores of up to 256 bits; a chunk whose array starts between 16-byte boundaries
-// peels its first elements.
+// in flight a thread (four: 585 us), stores of up to 256 bits; a chunk whose array
+// starts between 16-byte boundaries peels its first elements.
 //
 // The squares of a 128-bit load are added in fp32 and go into a 64-bit sum;
 // where they could leave the range of fp32 (a sum outside 2^-90 .. 2^120, zeros
@@ -39,7 +38,6 @@ struct ClipEntry {
     uint32_t first;      // chunk number of its first element within the launch
     uint16_t in_type, out_type;
 };
-// 32-byte entries in at most 32764 bytes of parameters
 // The elements before an array's first 16-byte boundary belong to its first
 // chunk, so every other chunk starts on one and the full ones are equal.
 __host__ __device__ inline int64_t head_of(const void* p, int64_t n, int type) {
@@ -56,6 +54,7 @@ struct Run {
     }
 };
 
+// 32-byte entries: 1000 of them stay below the 32764 bytes of a launch's parameters.
 template <int CAP>
 struct ClipList {
     int32_t count;
