@@ -35,7 +35,7 @@
 // Bound by the softmax threads' chain (TMEM loads, maximum, exponentials, TMEM
 // stores; with a cap the tanh's polynomial too), not by the products, which keep
 // the tensor pipe busy for 50 to 70 %.  16 heads of 16384 queries and keys, bf16, causal:
-// d 128 1020 us, 1080 TFLOP/s, cap 50 1210 to 1410; d 64 830 us, 664 TFLOP/s, cap 50 1240.
+// d 128 950 to 1030 us, 1160 to 1070 TFLOP/s, cap 50 1270; d 64 783 us, 702 TFLOP/s, cap 50 963.
 // With a thread a whole row, and MMAs issued by lane 0 with descriptors made for
 // each, 910 and 669 TFLOP/s where this reached 1083 and 867 (not causal).
 #include <algorithm>
@@ -71,7 +71,11 @@ struct Fw {
     static constexpr bool SPLIT = !std::is_same<T, U>::value;
     static constexpr int HALVES = DP > 128 ? 2 : 1;   // split operands of more than 64 columns: a tile is two, one behind the other
     static constexpr int DO = SPLIT ? DP / 2 : DP;    // columns of O
-    static constexpr int SOFTMAX = 256 * NT, THREADS = SOFTMAX + 64, MMA = SOFTMAX / 32, TMA = MMA + 1;   // threads, warps
+    static constexpr int SOFTMAX = 256 * NT, THREADS = SOFTMAX + (HALVES == 2 ? 64 : 128), MMA = SOFTMAX / 32, TMA = MMA + 1;   // threads, warps
+    // registers a thread: at launch, of the softmax warps, of the last warpgroup (bf16, 32/8
+    // heads of 4096, d 128, cap 50: 182 us without a split, 165 with; fp32, 8 heads of 2048, d 64: 65, 60)
+    static constexpr int REGS = HALVES == 2 ? 0 : NT == 2 ? 96 : 80, MORE = NT == 2 ? 112 : 104, FEWER = 32;
+    static_assert(!REGS || SOFTMAX * MORE + 128 * FEWER <= THREADS * REGS, "the split waits for ever");
     static constexpr int CH = DP / HALVES / 64, TILE_B = CH * CHUNK_BYTES;
     static constexpr int PER_SM = NT == 1 && HALVES == 1 ? 2 : 1;
     static constexpr int STAGES = PER_SM == 2 && CH == 2 ? 2 : 4;
@@ -313,6 +317,7 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
     bool masked, ok = true;
 
     if (warp >= L::MMA) {
+        if constexpr (L::REGS > 0) fewer_registers<L::FEWER>();
         if (warp == L::TMA) {
             // ------------------------------------------------ TMA
             int kt = walk.next(&masked);
@@ -426,6 +431,7 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
         }
     } else {
         // ---------------------------------------------------- half a row per thread
+        if constexpr (L::REGS > 0) more_registers<L::MORE>();
         const int t = warp / 8, half = warp / 4 % 2, r = threadIdx.x % TILE;
         const int head = pack ? r / pack : 0;   // of the group
         const int i = pack ? i0 + r % pack : i0 + r + (g.pair_heads ? 0 : t * TILE);
@@ -594,7 +600,7 @@ template <typename T, typename U, int DP, int NT, bool CAP, bool BIAS, bool FIX 
 tl_status launch(tl_ctx* c, const HeadMap* m, const FwArgs& g, cudaStream_t s) {
     using L = Fw<T, U, DP, NT>;
     static std::atomic<uint64_t> done{0};
-    TL_TRY(kernel_smem(c, k_attn_tc<T, U, DP, NT, CAP, BIAS, FIX>, L::BYTES, done));
+    TL_TRY(kernel_smem(c, k_attn_tc<T, U, DP, NT, CAP, BIAS, FIX>, L::BYTES, done, L::REGS));
     const AttnCall& a = g.a;
     const int span = g.pack ? g.pack : g.pair_heads ? TILE : NT * TILE;
     const int64_t grid = (int64_t)a.b * (g.pack ? a.hkv : g.pair_heads ? a.hq / 2 : a.hq) * ((a.nq + span - 1) / span) * g.parts;

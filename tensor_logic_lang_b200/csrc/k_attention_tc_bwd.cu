@@ -33,10 +33,10 @@
 // cache), and dk and dv, which leave no room for sums in TMEM, are added to
 // the outputs every 4 tiles.
 //
-// Bound by the element work between the products: a pair of tiles takes 4500 clocks
+// Bound by the element work between the products: a pair of tiles takes about 4300 clocks
 // in either kernel, of which the products fill 2048 (dk, dv) and 1536.  16 heads of 16384
-// queries and keys, bf16, causal, five products counted: d 128 3930 us, 700 TFLOP/s,
-// cap 50 4620; d 64 3030 us, 454 TFLOP/s, cap 50 3710.  fp32, 8 heads of 4096: d 64 278 us, d 96 456.
+// queries and keys, bf16, causal, five products counted: d 128 3860 us, 712 TFLOP/s,
+// cap 50 4460; d 64 2890 us, 475 TFLOP/s, cap 50 3600.  fp32, 8 heads of 4096: d 64 212 us, d 96 447.
 #include <algorithm>
 
 #include "attn_tc.h"
@@ -44,9 +44,19 @@
 namespace tl {
 namespace {
 
-constexpr int BW_COMPUTE = 512, BW_THREADS = BW_COMPUTE + 64, BW_STAGES = 2;
+constexpr int BW_COMPUTE = 512, BW_THREADS = BW_COMPUTE + 128, BW_STAGES = 2;
 constexpr int BW_MMA = BW_COMPUTE / 32, BW_TMA = BW_MMA + 1;   // warps
 constexpr int BW_COLS = 32;   // scores of a thread
+// Registers a thread: at launch, of the computing warps, of the last warpgroup.
+// fp32 (hi and lo of everything) gains most from the larger share (causal backward of 8 heads x
+// 4096 x 64: 278 us without a split, 223 with 104 and 64, 213 with 112 and 32); with
+// 16 bits, and in halves, the MMA and TMA warps need more than 32 (2 x 16 heads over 4 x 2048 x
+// 128, step of both passes: 235 us, 231, 240).
+constexpr int BW_REGS = 96;
+template <bool FP32> struct BwRegs {
+    static constexpr int MORE = FP32 ? 112 : 104, FEWER = FP32 ? 32 : 64;
+    static_assert(BW_COMPUTE * MORE + 128 * FEWER <= BW_THREADS * BW_REGS, "the split waits for ever");
+};
 struct BwArgs {
     AttnCall a;
     const float* stats;          // [b, hq, query tiles][2][128]
@@ -519,6 +529,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     const bool any = qt >= 0;
 
     if (warp >= BW_MMA) {
+        fewer_registers<BwRegs<SPLIT && !WIDE>::FEWER>();
         if (warp == BW_TMA) {
             // ------------------------------------------------ TMA
             if (any && lane == 0) {
@@ -577,7 +588,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             if (!WIDE && !ok)   // copies in flight land before the block ends
                 for (int e = max(0, n - 1 - BW_STAGES); e < n - 1; ++e)
                     mbar_wait(&bb.full[e % BW_STAGES], (e / BW_STAGES) & 1, g.err);
-        } else {
+        } else if (warp == BW_MMA) {
             // ------------------------------------------------ tensor cores
             const int ksteps = (a.d + 15) / 16;
             const uint32_t idesc = f16_idesc<T>(16 * ksteps, true);
@@ -665,6 +676,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         }
     } else {
         // ---------------------------------------------------- 32 queries of a key per thread
+        more_registers<BwRegs<SPLIT && !WIDE>::MORE>();
         const int wg = warp / 4, r = threadIdx.x % TILE, j = j0 + r;
         // at the end: dv (dk) and half of its columns
         constexpr int DH = DO / 2;
@@ -845,6 +857,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     const bool any = kt >= 0;
 
     if (warp >= BW_MMA) {
+        fewer_registers<BwRegs<SPLIT && !WIDE>::FEWER>();
         if (warp == BW_TMA) {
             // ------------------------------------------------ TMA
             if (any && lane == 0) {
@@ -879,7 +892,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             if (!WIDE && !ok)
                 for (int e = max(0, n - 1 - BW_STAGES); e < n - 1; ++e)
                     mbar_wait(&bb.full[e % BW_STAGES], (e / BW_STAGES) & 1, g.err);
-        } else {
+        } else if (warp == BW_MMA) {
             // ------------------------------------------------ tensor cores
             const int ksteps = (a.d + 15) / 16;
             const uint32_t idesc = f16_idesc<T>(16 * ksteps, true);
@@ -962,6 +975,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         }
     } else {
         // ---------------------------------------------------- 32 keys of a query per thread
+        more_registers<BwRegs<SPLIT && !WIDE>::MORE>();
         const int wg = warp / 4, r = threadIdx.x % TILE, i = i0 + r;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const SplitExps ex = split_exps<SPLIT>(g, b, kvh);
@@ -1081,8 +1095,8 @@ template <typename T, typename U, int DP, bool CAP, bool BIAS>
 tl_status launch(tl_ctx* c, const HeadMap* m, const BwArgs& g, cudaStream_t s) {
     static std::atomic<uint64_t> done_kv{0}, done_q{0};
     constexpr int smem = BwSmem<DP>::BYTES;
-    TL_TRY(kernel_smem(c, k_attn_tc_dkv<T, U, DP, CAP, BIAS>, smem, done_kv));
-    TL_TRY(kernel_smem(c, k_attn_tc_dq<T, U, DP, CAP, BIAS>, smem, done_q));
+    TL_TRY(kernel_smem(c, k_attn_tc_dkv<T, U, DP, CAP, BIAS>, smem, done_kv, BW_REGS));
+    TL_TRY(kernel_smem(c, k_attn_tc_dq<T, U, DP, CAP, BIAS>, smem, done_q, BW_REGS));
     const AttnCall& a = g.a;
     cudaEvent_t ev[2];
     launch_begin_on(c, s, "attention_tc_dkv", 0, 8.0 * a.d * attn_pairs(a), ev);
