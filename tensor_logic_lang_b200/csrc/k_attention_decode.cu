@@ -978,13 +978,13 @@ tl_status launch_type(tl_ctx* c, const DecArgs& g, cudaStream_t s) {
 
 // Where these kernels are faster than the tiles of 128 queries, if the tensor
 // cores take the call at all.  us here / there, one head a group:
-//   bf16, d 128, 16 x 8 heads of 4096 keys: 4 rows 51 / 52, 12 rows 61 / 53; with
+//   bf16, d 128, 16 x 8 heads of 4096 keys: 4 rows 51 / 55, 12 rows 60 / 55; with
 //     lengths of their own the pieces here stay equal
-//   fp16, d 64, the same: 12 rows 37 / 41, 24 rows 52 / 42
-//   fp32, d 64, 4 x 16 heads of 4096 keys: 4 rows 49 / 147, 12 rows 172 / 148
+//   fp16, d 64, the same: 12 rows 37 / 39, 48 rows 80 / 42
+//   fp32, d 64, 4 x 16 heads of 4096 keys: 4 rows 49 / 141, 12 rows 172 / 141
 // and where few tiles, each shared by eight blocks at most, would walk a long
-// cache: 64 rows of one head, 65536 keys: bf16, d 128 50 / 134, fp16, d 64 28 / 109,
-// fp32, d 64 172 / 272; of two heads, 32768 keys: 42 / 72, 25 / 60, 168 / 155.
+// cache: 64 rows of one head, 65536 keys: bf16, d 128 50 / 123, fp16, d 64 28 / 105,
+// fp32, d 64 171 / 211; of two heads, 32768 keys: 42 / 68, 25 / 57, 169 / 126.
 bool attn_few_takes(const AttnCall& a) {
     const int64_t rows = (int64_t)a.nq * (a.hq / a.hkv);
     if (a.nk == 0 || rows > 64) return false;

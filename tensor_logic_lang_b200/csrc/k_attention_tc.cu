@@ -197,7 +197,7 @@ __device__ void join_parts(uint8_t* smem, const FwArgs& g, int part, int b, int 
     const int lane = threadIdx.x & 31, share = TILE / parts, d0 = 4 * lane;
     const float fix = FIX ? fixed_top(CapCoef<L::SPLIT>(a.scale, a.cap).top) : 0.f;
     const float out_scale = L::SPLIT ? exp2f((float)-split_exp(g.tops.v, b * a.hkv + kvh)) : 1.f;
-    for (int r = part * share + threadIdx.x / 32; r < min((part + 1) * share, rows); r += L::THREADS / 32) {
+    for (int r = part * share + threadIdx.x / 32; r < min((part + 1) * share, rows); r += L::SOFTMAX / 32) {
         const int i = g.pack ? i0 + r % g.pack : i0 + r, h = g.pack ? h0 + r / g.pack : h0;
         if (i >= a.nq) continue;
         float m = -INFINITY, l = 0.f;
@@ -315,6 +315,15 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
         walk.start(0, end, 0, clear, kd ? g.k_ranges + (int64_t)b * g.key_tiles : nullptr, mine, parts, part);
     }
     bool masked, ok = true;
+    // by every warp: gives the TMEM back
+    auto end_of_walk = [&]() {
+        tc_fence_before();
+        __syncthreads();
+        if (warp == L::MMA) {
+            tc_fence_after();
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::TMEM));
+        }
+    };
 
     if (warp >= L::MMA) {
         if constexpr (L::REGS > 0) fewer_registers<L::FEWER>();
@@ -428,6 +437,12 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
                 kt = next;
                 masked = next_masked;
             }
+        }
+        __syncwarp();
+        end_of_walk();
+        if (NT == 1 && parts > 1) {   // as the softmax warps below, which keep their registers to the end
+            cluster_sync();
+            cluster_sync();
         }
     } else {
         // ---------------------------------------------------- half a row per thread
@@ -579,18 +594,12 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
             if (a.lse && on && half == 0)
                 a.lse[((int64_t)b * a.hq + h) * a.nq + i] = none ? -INFINITY : (FIX ? fix : m - Lift<T>::log2) * kLn2 + logf(l);
         }
-    }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == L::MMA) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)L::TMEM));
-    }
-    if constexpr (NT == 1) {
-        if (parts > 1) {
+        end_of_walk();
+        if (NT == 1 && parts > 1) {
             // TMEM is given back: no block holds any while it waits for its cluster
             cluster_sync();
             if (ok) join_parts<T, U, L, FIX>(smem, g, part, b, h0, kvh, i0);
+            __syncwarp();
             cluster_sync();   // its rows are read
         }
     }
@@ -628,13 +637,14 @@ tl_status launch_tiles(tl_ctx* c, const HeadMap* m, FwArgs g, cudaStream_t s) {
     // Two tiles a block read each key tile once for both and keep the tensor
     // cores busier; one leaves two blocks an SM, which even out walks of
     // different lengths.  bf16, d 128, one tile / two, us: 128 tiles of 2048
-    // keys 38 / 42; causal, 288 tiles 40 / 44, 512 tiles of 512 keys 29 / 32,
-    // of 1024 39 / 40, of 2048 58 / 52; not causal, 192 tiles 47 / 42, 512
-    // tiles 87 / 82; 512 causal tiles of 4096 keys in 16 documents 28 / 31, in 4
-    // 44 / 46, in one 95 / 81.  Lengths of documents are not known here: many
-    // (and two tiles a block have no documents).
+    // keys 36 / 40; causal, 288 tiles 39 / 42, 512 tiles of 512 keys 29 / 30,
+    // of 1024 36 / 38, of 2048 50 / 50; not causal, 192 tiles 46 / 41, 512
+    // tiles 85 / 79.  fp32, d 64: causal, 288 tiles 86 / 83, 512 112 / 107; 128 tiles 79 /
+    // 73, but 58 with keys shared by two blocks.  Documents (when two tiles had them): 512
+    // causal tiles of 4096 keys in 16 28 / 31, in 4 44 / 46, in one 95 / 81; their
+    // lengths are not known here: many.
     const int64_t tiles = g.pack ? (int64_t)a.b * a.hkv * ((a.nq + g.pack - 1) / g.pack) : (int64_t)a.b * a.hq * ((a.nq + TILE - 1) / TILE);
-    const bool one = g.pack || tiles <= c->sm_count || (a.causal && (tiles <= 2 * c->sm_count || a.nk <= 1024)) || (a.q_doc && a.k_doc);
+    const bool one = g.pack || tiles <= c->sm_count || (a.causal && !L::SPLIT && (tiles <= 2 * c->sm_count || a.nk <= 1024)) || (a.q_doc && a.k_doc);
     g.pair_heads = 0;
     g.parts = 1;
     if constexpr (DP <= 128)
@@ -643,13 +653,13 @@ tl_status launch_tiles(tl_ctx* c, const HeadMap* m, FwArgs g, cudaStream_t s) {
             return launch_scores<T, U, DP, 2>(c, m, g, s);
         }
     // Blocks that would leave the GPU half empty share the keys of a tile among
-    // up to eight, a cluster, which add their rows in shared memory (3 to 4 us).
-    // 1, 2, 4, 8 blocks a tile, us: bf16, d 128, 16 tiles of 32768 keys 496,
-    // 262, 137, 86, of 2048 38, 27, 19, 17; 128 tiles of 2048 38, 30; 32 tiles of 512 keys
-    // 15, 17, 15, 15, of 256 13, 15; fp32, d 64, of 512 32, 31, 26.  A tile of
-    // packed documents meets few of the keys: 64 tiles of 2048 keys in four 17,
-    // 19, 18, 18.  Where a block fills an SM (fp32, d 128, 16 tiles of 2048 keys) 82,
-    // 59, 44, 52: few clusters of eight find their SMs.
+    // up to eight, a cluster, which add their rows in shared memory (2 to 4 us).
+    // One block a tile / shared, us: bf16, d 128, 16 tiles of 32768 keys 507 / 78 (two 267,
+    // four 139), of 2048 35 / 17; 128 tiles of 2048 36 / 33; 32 tiles of 512 keys, four 16 / 15,
+    // two 17, of 256, two 13 / 15; fp32, d 64, of 512 28 / 25, 64 tiles of 1024 41 / 31.  A tile of
+    // packed documents meets few of the keys: 64 tiles of 2048 keys in four 17 / 19.
+    // Where a block fills an SM (fp32, d 128, 16 tiles of 2048 keys) 80, 57, 42, 48 by 1, 2, 4, 8:
+    // few clusters of eight find their SMs.
     const int least = a.q_doc ? 32 : L::SPLIT ? 4 : 8;   // key tiles
     while (g.key_tiles >= least && g.parts < (L::PER_SM == 1 ? 4 : 8) && tiles * g.parts * 2 <= c->sm_count * L::PER_SM &&
            g.parts * 2 <= g.key_tiles)
@@ -720,7 +730,7 @@ tl_status launch_attn_begin(tl_ctx* c, const AttnCall& a, DocRange* q_out, DocRa
 
 // Queries of a tile that holds them for all heads of a group, where that makes
 // fewer tiles (0: it does not): 16 x 64 heads over 8, 8 queries over 4096 keys of
-// bf16, d 128, 260 us by head, 54 packed.
+// bf16, d 128, 260 us by head, 61 packed.
 static int packed_queries(const AttnCall& a) {
     const int group = a.hq / a.hkv;
     if (group < 2 || group > TILE || (a.dtype != TL_TYPE_F32 && a.q.sh == 0)) return 0;

@@ -674,6 +674,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 ++n;
             }
         }
+        __syncwarp();
+        if (g.cluster > 1) {   // as the computing warps below, which keep their registers to the end
+            cluster_sync();
+            cluster_sync();
+        }
     } else {
         // ---------------------------------------------------- 32 queries of a key per thread
         more_registers<BwRegs<SPLIT && !WIDE>::MORE>();
@@ -785,12 +790,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                                     __uint_as_float(o[4 * q + 2]) * mul, __uint_as_float(o[4 * q + 3]) * mul);
             }
         }
-    }
-    __syncwarp();
-    if (g.cluster > 1) {
-        // each block adds its share of the rows over the cluster, in the order of the heads
-        cluster_sync();
-        if (warp < BW_MMA) {
+        __syncwarp();
+        if (g.cluster > 1) {
+            // each block adds its share of the rows over the cluster, in the order of the heads
+            cluster_sync();
             const int share = TILE / g.cluster, r0 = rank * share;
             const uint32_t sums = smem_u32(smem);
             constexpr int V = DO / 4;
@@ -814,10 +817,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                     *reinterpret_cast<uint2*>(p + 4 * c) = make_uint2(pack16<T>(s[0], s[1]), pack16<T>(s[2], s[3]));
                 }
             }
+            __syncwarp();
+            // a block's sums stay until the others have read them
+            cluster_sync();
         }
-        __syncwarp();
-        // a block's sums stay until the others have read them
-        cluster_sync();
     }
     bb.finish(tmem);
 }
@@ -1148,9 +1151,9 @@ tl_status launch_attn_tc_backward(tl_ctx* c, const AttnCall& a, void* ws, cudaSt
         g.cluster *= 2;
     // two blocks of the cluster for a head's query tiles where they and dq's
     // blocks find SMs of their own (2 x 512 x 4 heads over 2: bf16 24 -> 21, fp32
-    // 57 -> 45 us; 2 x 512 x 8 heads, too many: bf16 22 -> 28); fp32 walks, twice
-    // as long a tile, gain from a causal call's shorter longest one for longer (1024
-    // x 8 heads 82 -> 61, x 16 over 4 88 -> 104).  Four never paid.
+    // 42 -> 33 us; 2 x 512 x 8 heads, too many: bf16 22 -> 28); fp32 walks, longer
+    // a tile, gain from a causal call's shorter longest one for longer (2048 x 4 heads 78 -> 62,
+    // 1024 x 8 54 -> 49, but 2 x 512 x 8 42 -> 43, 1024 x 16 over 4 60 -> 81).  Four never paid.
     const int64_t kv_blocks = (int64_t)plan.k_tiles * a.b * a.hkv * g.cluster, q_blocks = (int64_t)plan.q_tiles * a.b * a.hq;
     g.abreast = g.cluster;
     g.parts = 1;
