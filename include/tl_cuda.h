@@ -469,7 +469,8 @@ tl_status tl_tensor_array(tl_tensor* t, int32_t write, tl_array* out);
  * Arrays of rank 4, [batch, heads, positions, head size], of one type, head
  * size 1..256, any strides (k and v may have strides of 0; arrays that are
  * written may not overlap themselves, one another or an input).  Sums, the
- * softmax and its statistics are in 32 bits.  16-bit types take their products
+ * softmax and its statistics are in 32 bits (so the backward pass's exponentials
+ * are good to 2^-24 of |s| and |lse|).  16-bit types take their products
  * from 16-bit operands (exponentials, and dx of the backward pass, rounded to
  * them).  fp32 arrays of head size up to 128 take 22 bits of each operand of a
  * product, or 2^-39 of the largest of its kind in the heads that share a key

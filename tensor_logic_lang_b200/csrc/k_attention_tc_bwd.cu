@@ -31,12 +31,13 @@
 // operands fill shared memory but for two tiles of 64 columns, so the passing
 // ones come in halves, each as often as a product needs it (twice, from the L2
 // cache), and dk and dv, which leave no room for sums in TMEM, are added to
-// the outputs every 4 tiles.
+// the outputs tile by tile (sums of 4 tiles on the tensor cores lost 2.4e-6 of dk
+// and dv, of one 6e-7).
 //
 // Bound by the element work between the products: a pair of tiles takes about 4300 clocks
 // in either kernel, of which the products fill 2048 (dk, dv) and 1536.  16 heads of 16384
 // queries and keys, bf16, causal, five products counted: d 128 3860 us, 712 TFLOP/s,
-// cap 50 4460; d 64 2890 us, 475 TFLOP/s, cap 50 3600.  fp32, 8 heads of 4096: d 64 212 us, d 96 447.
+// cap 50 4460; d 64 2890 us, 475 TFLOP/s, cap 50 3600.  fp32, 8 heads of 4096: d 64 215 us, d 96 440.
 #include <algorithm>
 
 #include "attn_tc.h"
@@ -352,7 +353,6 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 
 // WIDE: the ring of two halves (64 columns, hi and lo) that pass, entry by entry
 // in the same order for the warp that loads and the one that multiplies.
-constexpr int WIDE_FLUSH = 4;   // tiles whose dk and dv the tensor cores add
 struct HalfRing {
     static constexpr int HALF = 2 * CHUNK_BYTES;
     const BwBlock& bb;
@@ -394,64 +394,55 @@ struct HalfRing {
             __syncwarp();
         }
     }
-    // columns 0..63 and 64.. of D (+)= A Y: Y passes
+    // columns 0..63 and 64.. of D = A Y: Y passes
     template <typename T>
-    __device__ __forceinline__ void parts2(uint32_t d, uint32_t a, int ksteps, bool more, bool& ok) {
+    __device__ __forceinline__ void parts2(uint32_t d, uint32_t a, int ksteps, bool& ok) {
         for (int f = 0; f < 2; ++f, ++e) {
             const int s = e % 2;
             ok = warp_wait(&bb.full[s], (e / 2) & 1, ok, err);
             if (ok && elect_one()) {
-                mma_parts_split<BW_COLS>(d + 64 * f, a, smem_u32(at + s * HALF), f16_idesc<T>(f ? 16 * (ksteps - 4) : 64, true), more);
+                mma_parts_split<BW_COLS>(d + 64 * f, a, smem_u32(at + s * HALF), f16_idesc<T>(f ? 16 * (ksteps - 4) : 64, true), 0);
                 umma_commit(&bb.empty[s]);
             }
             __syncwarp();
         }
     }
 };
+
 // A row's columns col0 .. col0 + N - 1 of an fp32 output (+)= N TMEM columns times
-// mul.  32 loads before the first store: a round trip each took 15 us a tile of 96
-// columns, all of them 2.
+// mul.  The thread alone owns them, so additions that the L2 makes, which nothing
+// waits for, come in one order (loads and stores took 6 us more a tile of 96 columns).
 template <int N>
 __device__ __forceinline__ void add_row(const HeadsView& v, int b, int h, int64_t row, int col0, bool on, int d, uint32_t taddr, float mul,
                                         bool fresh) {
     float* p = static_cast<float*>(v.p) + b * v.sb + h * v.sh + row * v.ss + col0 * v.sd;
     const bool wide = v.sd == 1 && d % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
 #pragma unroll 1
-    for (int k = 0; k < N; k += 32) {
+    for (int k = 0; k < N; k += 16) {
         const int left = on ? d - col0 - k : 0;   // columns from here on
-        float old[32];
+        uint32_t o[16];
+        tmem_ld16(taddr + k, o);
+        tmem_wait_ld();
 #pragma unroll
-        for (int q = 0; q < 32; ++q) old[q] = 0.f;
-        if (!fresh) {
-            if (wide) {
+        for (int q = 0; q < 16; q += 4) {
+            float x[4];
 #pragma unroll
-                for (int q = 0; q < 32; q += 4)
-                    if (q < left) {
-                        const float4 x = *reinterpret_cast<const float4*>(p + k + q);
-                        old[q] = x.x; old[q + 1] = x.y; old[q + 2] = x.z; old[q + 3] = x.w;
-                    }
+            for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(o[q + e]) * mul;
+            float* at = p + (k + q) * v.sd;
+            if (wide && fresh) {
+                if (q < left) *reinterpret_cast<float4*>(at) = make_float4(x[0], x[1], x[2], x[3]);
+            } else if (wide) {
+                if (q < left)
+                    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3])
+                                 : "memory");
             } else {
 #pragma unroll
-                for (int q = 0; q < 32; ++q)
-                    if (q < left) old[q] = p[(k + q) * v.sd];
+                for (int e = 0; e < 4; ++e)
+                    if (q + e < left) {
+                        if (fresh) at[e * v.sd] = x[e];
+                        else asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(at + e * v.sd), "f"(x[e]) : "memory");
+                    }
             }
-        }
-#pragma unroll
-        for (int f = 0; f < 32; f += 16) {
-            uint32_t o[16];
-            tmem_ld16(taddr + k + f, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int q = 0; q < 16; ++q) old[f + q] = fmaf(__uint_as_float(o[q]), mul, old[f + q]);
-        }
-        if (wide) {
-#pragma unroll
-            for (int q = 0; q < 32; q += 4)
-                if (q < left) *reinterpret_cast<float4*>(p + k + q) = make_float4(old[q], old[q + 1], old[q + 2], old[q + 3]);
-        } else {
-#pragma unroll
-            for (int q = 0; q < 32; ++q)
-                if (q < left) p[(k + q) * v.sd] = old[q];
         }
     }
 }
@@ -618,11 +609,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 ring.rows2<T>(t_dp, sv, ksteps, bb.dp_full, ok);
                 while (qt >= 0 && ok) {
                     ok = warp_wait(bb.p_full, n & 1, ok, g.err);
-                    ring.parts2<T>(t_dv, t_s, ksteps, n % WIDE_FLUSH != 0, ok);
+                    ring.parts2<T>(t_dv, t_s, ksteps, ok);
                     next();
                     if (qt >= 0) ring.rows2<T>(t_s, sk, ksteps, &bb.s_full[0], ok);
                     ok = warp_wait(bb.dx_full, n & 1, ok, g.err);
-                    ring.parts2<T>(t_dk, t_dp, ksteps, n % WIDE_FLUSH != 0, ok);
+                    ring.parts2<T>(t_dk, t_dp, ksteps, ok);
                     if (qt >= 0) ring.rows2<T>(t_dp, sv, ksteps, bb.dp_full, ok);
                     else if (ok && elect_one()) umma_commit(bb.done);
                     __syncwarp();
@@ -720,8 +711,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             {
                 // dv of the tile before, done before this S
                 if (WIDE) {
-                    if (which == 0 && n > 0 && n % WIDE_FLUSH == 0)
-                        add_row<DH>(g.dv, b, out_h, j, col0, j < a.nk, a.d, t_dv + lanes + col0, mul, n == WIDE_FLUSH);
+                    if (which == 0 && n > 0)
+                        add_row<DH>(g.dv, b, out_h, j, col0, j < a.nk, a.d, t_dv + lanes + col0, mul, n == 1);
                 } else if (SPLIT && which == 0 && n > 0) {
                     tmem_add<DH>(t_dva + lanes + col0, t_dv + lanes + col0, n == 1);
                 }
@@ -740,8 +731,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             {
                 // dk of the tile before, done before this dp
                 if (WIDE) {
-                    if (which == 1 && n > 0 && n % WIDE_FLUSH == 0)
-                        add_row<DH>(g.dk, b, out_h, j, col0, j < a.nk, a.d, t_dk + lanes + col0, mul, n == WIDE_FLUSH);
+                    if (which == 1 && n > 0)
+                        add_row<DH>(g.dk, b, out_h, j, col0, j < a.nk, a.d, t_dk + lanes + col0, mul, n == 1);
                 } else if (SPLIT && which == 1 && n > 0) {
                     tmem_add<DH>(t_dka + lanes + col0, t_dk + lanes + col0, n == 1);
                 }
@@ -770,7 +761,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             mine_at = acc;
         }
         if (WIDE && any) {
-            if (ok) add_row<DH>(which ? g.dk : g.dv, b, out_h, j, col0, j < a.nk, a.d, mine_at, mul, n <= WIDE_FLUSH);
+            if (ok) add_row<DH>(which ? g.dk : g.dv, b, out_h, j, col0, j < a.nk, a.d, mine_at, mul, n <= 1);
         } else if (g.cluster == 1) {
             HeadsView v = which ? g.dk : g.dv;
             v.p = static_cast<U*>(v.p) + col0 * v.sd;
@@ -926,7 +917,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                     ring.rows2<T>(tmem, sq, ksteps, &bb.s_full[0], ok);
                     ring.rows2<T>(t_dp, sdo, ksteps, bb.dp_full, ok);
                     ok = warp_wait(bb.dx_full, n & 1, ok, g.err);
-                    ring.parts2<T>(t_dq, t_dp, ksteps, false, ok);
+                    ring.parts2<T>(t_dq, t_dp, ksteps, ok);
                     ++n;
                     kt = walk.next(&masked);
                 }

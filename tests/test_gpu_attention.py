@@ -540,6 +540,23 @@ def test_values_of_very_different_size(ctx, dtype):
         check(got[n], want[n], n)
 
 
+@pytest.mark.parametrize("d", [64, 80, 128])
+def test_fp32_errors_do_not_grow_with_the_tiles(ctx, d):
+    # of the norm of a result: a tile's sums are cut 24 times (8 steps of 3 products) by half a
+    # last place, 2^-24 each, whatever the number of tiles, and either operand has 22 bits
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    q, dout = heads(gen, 1, 4, 1300, d, "f32"), heads(gen, 1, 4, 1300, d, "f32")
+    k, v = heads(gen, 1, 2, 1300, d, "f32"), heads(gen, 1, 2, 1300, d, "f32")
+    got = run(ctx, q, k, v, dout, {"causal": True})
+    q6, k6, v6 = (x.double().requires_grad_() for x in (q, k, v))
+    s = (q6 @ k6.repeat_interleave(2, 1).transpose(2, 3)) * d ** -0.5
+    seen = torch.ones(1300, 1300, dtype=torch.bool, device="cuda").tril()
+    o6 = s.masked_fill(~seen, -torch.inf).softmax(-1) @ v6.repeat_interleave(2, 1)
+    o6.backward(dout.double())
+    for n, want in (("out", o6), ("dq", q6.grad), ("dk", k6.grad), ("dv", v6.grad)):
+        assert ((got[n].double() - want).norm() / want.norm()).item() <= 24 * 2.0 ** -24 + 2 * 2.0 ** -22, n
+
+
 def test_fp32_on_the_cuda_cores():
     # a context of that precision keeps all 24 bits of the operands
     from tensor_logic_lang_b200 import abi
