@@ -350,8 +350,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_decode_join(const __grid_const
     const int64_t per = max((int64_t)1, (all + g.blocks - 1) / g.blocks);
     const int64_t u0 = before + (int64_t)unit * n, u1 = u0 + n;
     const int first = (int)(u0 / per), last = n ? (int)((u1 - 1) / per) : first;
-    if (n && first == last) return;   // one block wrote it
+    // before any return: where no row is split over blocks, what follows this
+    // kernel would else start before the outputs are written
     wait_for_previous();
+    if (n && first == last) return;   // one block wrote it
     int i, h;
     unit_row(a, kvh, row, &i, &h);
     // a block's second piece is the one that starts inside it

@@ -272,6 +272,43 @@ def test_captured_and_replayed(ctx, nq):
                 check(x, want[n], n)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("b,hkv,nk", [
+    (4, 8, 50),        # more units than clusters find SMs for, a tile each: every unit lies in one block
+    (64, 8, 30), (37, 8, 64),
+    (3, 8, 333)])      # units that lie over several blocks
+def test_few_rows_are_written_when_the_call_ends(ctx, b, hkv, nk, dtype):
+    # the next node of a captured graph takes what the call wrote
+    gen = torch.Generator(device="cuda").manual_seed(b)
+    q, k, v = heads(gen, b, 2 * hkv, 1, 128, dtype), heads(gen, b, hkv, nk, 128, dtype), heads(gen, b, hkv, nk, 128, dtype)
+    out, lse = like(q, "bhsd"), torch.empty(q.shape[:3], device="cuda")
+    kept, kept_lse = torch.empty_like(out), torch.empty_like(lse)
+    m = {"causal": True, "softcap": 3.0}
+    ws = torch.empty(256 + ctx.attention_workspace(q, k, v, out, lse, **m), dtype=torch.uint8, device="cuda")
+    ws = ws[-ws.data_ptr() % 256:]
+
+    def step():
+        out.fill_(float("nan")), lse.fill_(float("nan"))
+        ctx.attention(q, k, v, out, lse, stream=stream(), workspace=ws, **m)
+        kept.copy_(out), kept_lse.copy_(lse)
+        k.mul_(-1.0)                            # the cache moves on
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(10):
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=gen, device="cuda"))
+        want = reference(q, k, v, **m)
+        graph.replay()
+        check(kept, want["out"], "out")
+        check(kept_lse, want["lse"], "lse")
+
+
 def test_capture_needs_a_workspace(ctx):
     from tensor_logic_lang_b200 import abi
     gen = torch.Generator(device="cuda").manual_seed(4)
