@@ -240,7 +240,13 @@ tl_status check_attention(tl_ctx* c, const tl_attention& t, bool backward, AttnC
     return TL_OK;
 }
 
+// No query (backward: and no key) to write for.
+bool nothing_to_do(const AttnCall& a, bool backward) {
+    return (int64_t)a.b * a.hq * a.nq == 0 && (!backward || (int64_t)a.b * a.hkv * a.nk == 0);
+}
+
 size_t attention_need(const AttnCall& a, bool backward) {
+    if (nothing_to_do(a, backward)) return 0;
     if (backward && attn_tc_backward_takes(a)) return attn_tc_backward_workspace(a);
     if (!backward && attn_few_takes(a)) return attn_few_workspace(a);
     if (!backward && attn_tc_takes(a)) return attn_tc_workspace(a);
@@ -251,8 +257,7 @@ tl_status run_attention(tl_ctx* c, const tl_attention* t, bool backward) {
     if (!t) return fail(c, TL_ERR_INVALID, "attention: no descriptor");
     AttnCall a;
     TL_TRY(check_attention(c, *t, backward, &a));
-    const int64_t queries = (int64_t)a.b * a.hq * a.nq, keys = (int64_t)a.b * a.hkv * a.nk;
-    if (queries == 0 && (!backward || keys == 0)) return TL_OK;
+    if (nothing_to_do(a, backward)) return TL_OK;
     DeviceGuard dev(c->device);
     if (!dev.ok) return fail(c, TL_ERR_CUDA, "cannot make device %d current", c->device);
     cudaStream_t s = static_cast<cudaStream_t>(t->stream);

@@ -87,6 +87,16 @@ def test_refused_sizes(lib):
     assert need(lib, a) == -abi.TL_ERR_TOO_LARGE
 
 
+@pytest.mark.parametrize("dtype", [abi.TL_TYPE_F32, abi.TL_TYPE_F16, abi.TL_TYPE_BF16])
+def test_no_heads_need_no_workspace(lib, dtype):
+    # heads, queries or sequences that are not there: nothing is divided by their number
+    for backward in (0, 1):
+        for none in (dict(hq=0, hkv=0), dict(b=0), dict(b=0, hq=0, hkv=0), dict(hq=0, hkv=0, nq=0, nk=0)):
+            assert need(lib, attention(dtype=dtype, **none), backward) == 0, none
+        assert need(lib, attention(dtype=dtype, hq=0), backward) == 0    # keys without queries: dk, dv of zeros
+        assert need(lib, attention(dtype=dtype, nq=0), backward) == 0
+
+
 def test_refused_counts(lib):
     # more queries than blocks can be numbered, without the memory for them
     def wide(b, h, n):
