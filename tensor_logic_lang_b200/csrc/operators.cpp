@@ -189,10 +189,11 @@ tl_status check_attention(tl_ctx* c, const tl_attention& t, bool backward, AttnC
         return fail(c, TL_ERR_UNSUPPORTED, "attention: head size %lld, 1 to %d are supported", (long long)d, kAttnMaxHead);
     if (hkv == 0 ? hq != 0 : hq % hkv != 0)
         return fail(c, TL_ERR_INVALID, "attention: %lld query heads over %lld key heads", (long long)hq, (long long)hkv);
-    if (b > kMaxCount || hq > kMaxCount || nq > kMaxCount || nk > kMaxCount)
+    if (b > kMaxCount || hq > kMaxCount || hkv > kMaxCount || nq > kMaxCount || nk > kMaxCount)
         return fail(c, TL_ERR_TOO_LARGE, "attention: more than 2^29 sequences, heads or positions");
     // blocks are numbered in 31 bits: one a query, or 16 keys of a head, at the least
-    if (b * hq > kMaxCount / 2 || (double)b * hq * nq > 2147483647.0 || (double)b * hq * ((nk + 15) / 16) > 2147483647.0)
+    const int64_t heads = std::max(hq, hkv);   // keys without queries have gradients of 0 to write
+    if (b * heads > kMaxCount / 2 || (double)b * hq * nq > 2147483647.0 || (double)b * heads * ((nk + 15) / 16) > 2147483647.0)
         return fail(c, TL_ERR_TOO_LARGE, "attention: batch x heads x queries above 2^31, or x keys above 2^35");
     TL_TRY(check_heads(c, t.q, "q", t, b, hq, nq, d, false));
     TL_TRY(check_heads(c, t.k, "k", t, b, hkv, nk, d, false));

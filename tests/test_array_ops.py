@@ -108,6 +108,17 @@ def test_refused_counts(lib):
     assert need(lib, a) == -abi.TL_ERR_TOO_LARGE
 
 
+def test_refused_counts_of_keys_without_queries(lib):
+    # key heads of calls without query heads count like query heads
+    for b, h, n in ((1 << 14, 1 << 15, 1), (1 << 14, 1 << 14, 1 << 20), (1, 1 << 40, 1)):
+        a = attention(b=1, hq=1, hkv=1, nq=1, nk=1, d=1)
+        for i, name in enumerate(("q", "o", "dout", "dq")):
+            setattr(a, name, array((b, 0, 1, 1), data=0x1000 * (i + 1)))
+        a.k = a.v = array((b, h, n, 1), (0, 0, 0, 1))
+        a.dk, a.dv = array((b, h, n, 1), data=1 << 40), array((b, h, n, 1), data=1 << 41)
+        assert need(lib, a, 1) == -abi.TL_ERR_TOO_LARGE, (b, h, n)
+
+
 def test_refused_outputs(lib):
     # written arrays that overlap themselves, an input or one another
     assert need(lib, attention(o=array((2, 4, 8, 32), (0, 256, 32, 1)))) == -abi.TL_ERR_INVALID
