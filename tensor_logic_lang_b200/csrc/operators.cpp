@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "attention.h"
@@ -220,7 +221,11 @@ tl_status check_attention(tl_ctx* c, const tl_attention& t, bool backward, AttnC
             if (wr[i]->data == wr[w]->data && numel(*wr[i]) > 0)
                 return fail(c, TL_ERR_INVALID, "attention: two written arrays are one");
     }
-    if (reinterpret_cast<uintptr_t>(t.lse) % 4) return fail(c, TL_ERR_INVALID, "attention: lse is misaligned");
+    const std::pair<const void*, const char*> words[] = {
+        {t.lse, "lse"}, {t.slopes, "slopes"}, {t.prefix_len, "prefix_len"}, {t.q_doc, "q_doc"},
+        {t.k_doc, "k_doc"}, {t.kv_len, "kv_len"}, {t.q_start, "q_start"}};
+    for (const auto& w : words)
+        if (reinterpret_cast<uintptr_t>(w.first) % 4) return fail(c, TL_ERR_INVALID, "attention: %s is misaligned", w.second);
     if (!isfinite(t.scale)) return fail(c, TL_ERR_INVALID, "attention: scale is not finite");
     if (!isfinite(t.softcap) || t.softcap < 0) return fail(c, TL_ERR_INVALID, "attention: softcap is negative or not finite");
     if (t.causal != 0 && t.causal != 1) return fail(c, TL_ERR_INVALID, "attention: causal is 0 or 1");

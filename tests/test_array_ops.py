@@ -77,6 +77,16 @@ def test_refused(lib, bad, backward):
     assert st in (-abi.TL_ERR_INVALID, -abi.TL_ERR_UNSUPPORTED), st
 
 
+@pytest.mark.parametrize("name", ["slopes", "prefix_len", "kv_len", "q_start", "q_doc", "k_doc"])
+def test_refused_addresses(lib, name):
+    # 32-bit values that do not lie on 4 bytes would fault the GPU
+    both = {"q_doc": 0x1000, "k_doc": 0x2000} if "doc" in name else {}
+    for off in (1, 2):
+        a = attention(causal=1, **dict(both, **{name: 0x3000 + off}))
+        assert need(lib, a) == need(lib, a, 1) == -abi.TL_ERR_INVALID
+    assert need(lib, attention(causal=1, **dict(both, **{name: 0x3004}))) >= 0
+
+
 def test_refused_sizes(lib):
     assert need(lib, attention(d=257)) == -abi.TL_ERR_UNSUPPORTED
     assert need(lib, attention(d=256)) >= 0
