@@ -514,7 +514,8 @@ tl_status tl_attention_forward(tl_ctx* ctx, const tl_attention* a);
 tl_status tl_attention_backward(tl_ctx* ctx, const tl_attention* a);
 /* Bytes of workspace of a forward (backward = 0) or backward call with these */
 /* arrays, or minus the status with which the call would be refused.  Checks  */
-/* the arguments and does no device work; ctx may be NULL (no error text).    */
+/* the arguments and does no device work; ctx may be NULL (no error text, and */
+/* a size that is enough for any context).                                    */
 int64_t tl_attention_workspace(tl_ctx* ctx, const tl_attention* a, int32_t backward);
 
 /*

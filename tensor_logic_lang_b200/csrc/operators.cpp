@@ -373,7 +373,13 @@ extern "C" int64_t tl_attention_workspace(tl_ctx* c, const tl_attention* t, int3
         if (!t) return -(int64_t)fail(c, TL_ERR_INVALID, "attention: no descriptor");
         AttnCall a;
         const tl_status st = check_attention(c, *t, backward != 0, &a);
-        return st == TL_OK ? (int64_t)attention_need(a, backward != 0) : -(int64_t)st;
+        if (st != TL_OK) return -(int64_t)st;
+        size_t n = attention_need(a, backward != 0);
+        if (!c && a.dtype == TL_TYPE_F32) {   // enough for a context of either precision
+            a.cuda_cores = 1;
+            n = std::max(n, attention_need(a, backward != 0));
+        }
+        return (int64_t)n;
     });
 }
 

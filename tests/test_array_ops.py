@@ -97,6 +97,14 @@ def test_refused_sizes(lib):
     assert need(lib, a) == -abi.TL_ERR_TOO_LARGE
 
 
+def test_workspace_without_a_context_is_enough_for_any(lib):
+    # a TL_PREC_FP32 context keeps fp32 arrays on the CUDA cores, as every context does at a head size of 200,
+    # where a row's part is 202 words (of head size 64: 66)
+    for rows in (1, 8, 32):
+        on_cuda_cores = need(lib, attention(b=1, hq=rows, hkv=1, nq=1, nk=64, d=200)) * 66 // 202
+        assert need(lib, attention(b=1, hq=rows, hkv=1, nq=1, nk=64, d=64)) >= on_cuda_cores
+
+
 @pytest.mark.parametrize("dtype", [abi.TL_TYPE_F32, abi.TL_TYPE_F16, abi.TL_TYPE_BF16])
 def test_no_heads_need_no_workspace(lib, dtype):
     # heads, queries or sequences that are not there: nothing is divided by their number

@@ -608,6 +608,27 @@ def test_fp32_on_the_cuda_cores():
         c.close()
 
 
+def test_workspace_of_either_precision(ctx):
+    # without a context the size is enough for a context of any precision
+    import ctypes as C
+    from tensor_logic_lang_b200 import abi
+    from tensor_logic_lang_b200.runtime import Context
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    c = Context(device=0, precision=abi.PREC_FP32)
+    try:
+        for hq, nq, nk, d in ((32, 1, 64, 64), (2, 20, 70, 128), (2, 100, 100, 96), (2, 1, 900, 200)):
+            q, k, v = heads(gen, 1, hq, nq, d, "f32"), heads(gen, 1, 1, nk, d, "f32"), heads(gen, 1, 1, nk, d, "f32")
+            out, lse, dout = like(q, "bhsd"), torch.empty(q.shape[:3], device="cuda"), like(q, "bhsd")
+            g = (dout, like(q, "bhsd"), like(k, "bhsd"), like(v, "bhsd"))
+            for grads in (None, g):
+                fields = ctx._attention(q, k, v, out, lse, grads, None, 0.0, None, False, None, None, None, None, None,
+                                        None, None, True)
+                any_context = ctx.lib.tl_attention_workspace(None, C.c_char_p(fields), 1 if grads else 0)
+                assert any_context >= max(x.attention_workspace(q, k, v, out, lse, grads) for x in (ctx, c))
+    finally:
+        c.close()
+
+
 def test_kernels_that_run(ctx):
     # the kernels the rules of the entry point's documentation name
     gen = torch.Generator(device="cuda").manual_seed(1)
