@@ -8,6 +8,7 @@ fallback: without the built library or a GPU, construction raises.
 """
 import ctypes as C
 import struct
+from math import prod
 from operator import methodcaller
 
 import numpy as np
@@ -26,6 +27,17 @@ _DATA, _NUMEL, _DEVICE, _IS_CONTIGUOUS = (methodcaller(n) for n in ("data_ptr", 
 _ATTENTION = struct.Struct("=" + "Qii4q4q" * 8 + "QffiiQQQQQQQqQ")
 _NO_GRADS = (0,) * (11 * 4)
 _PAD = [(0,) * (abi.TL_ARRAY_RANK - r) for r in range(abi.TL_ARRAY_RANK + 1)]
+
+
+def _in_a_row(shape, strides):
+    """Whether an array's elements lie behind one another in the order of its indices."""
+    n = 1
+    for k, s in zip(reversed(shape), reversed(strides)):
+        if k != 1 and s != n:
+            return False
+        n *= k
+    return True
+
 
 
 class Context:
@@ -332,10 +344,10 @@ class Context:
         for x in arrays:
             p, t, shape, strides = self._view(x, what, write)
             r = len(shape)
-            if r > abi.TL_ARRAY_RANK:
-                if not x.is_contiguous():
-                    raise abi.TLError(abi.TL_ERR_INVALID, f"{what}: rank {r} and not contiguous")
-                shape, strides, r = (x.numel(),), (1,), 1
+            if _in_a_row(shape, strides) if isinstance(x, str) else x.is_contiguous():
+                shape, strides, r = (prod(shape),), (1,), 1
+            elif r > abi.TL_ARRAY_RANK:
+                raise abi.TLError(abi.TL_ERR_INVALID, f"{what}: rank {r} and not contiguous")
             parts.append(_ARRAY.pack(p, t, r, *shape, *_PAD[r], *strides, *_PAD[r]))
         return b"".join(parts)
 
@@ -347,7 +359,8 @@ class Context:
     def clip_gradients(self, grads, max_norm, out=None, norm=None, workspace=None, stream=None):
         """Scales the arrays so that their global norm is at most max_norm (tl_clip_gradients).
 
-        In place, or into the arrays of `out` (same dims and strides, any type).  norm: a device fp32 scalar that
+        In place, or into the arrays of `out` (any type; the same dims and strides, or contiguous like the gradient and
+        with as many elements).  norm: a device fp32 scalar that
         receives the norm before the scaling.  Nothing is copied to the host.
         """
         stream = self._stream(stream)

@@ -184,6 +184,56 @@ def test_clip_checks(lib):
     assert lib.tl_clip_workspace(None, None, None, 2, 1.0) == -abi.TL_ERR_INVALID
 
 
+class DeviceArray:
+    """What Context reads of a contiguous device tensor."""
+    device = "cuda:0"
+
+    def __init__(self, at, shape, dtype="float32"):
+        self.at, self.shape, self.dtype = at, shape, dtype
+
+    def data_ptr(self):
+        return self.at
+
+    def numel(self):
+        return math.prod(self.shape)
+
+    def get_device(self):
+        return 0
+
+    def is_contiguous(self):
+        return True
+
+    def stride(self):
+        return tuple(math.prod(self.shape[i + 1:]) for i in range(len(self.shape)))
+
+
+@pytest.mark.parametrize("count", [1, 2, 16, 17, 60])
+def test_clip_lists_of_names_and_arrays(lib, count):
+    # names and device arrays pair up the same way in lists of any length
+    from tensor_logic_lang_b200.runtime import Context
+    shapes = [((40, 3), (7,), (2, 5, 3, 4), (1, 9))[i % 4] for i in range(count)]
+
+    def arrays(at):
+        return [DeviceArray(at + 0x1000 * i, s) for i, s in enumerate(shapes)]
+
+    class Named(Context):
+        def __init__(self):
+            self.device, self.lib, self.h = 0, lib, None
+            self.held = dict(zip((f"W{i}" for i in range(count)), arrays(0x10000000)))
+
+        def _view(self, x, what, write=False):
+            return super()._view(self.held[x] if isinstance(x, str) else x, what)
+
+    c = Named()
+    names, there = list(c.held), arrays(0x20000000)
+    mixed = [n if i % 2 else a for i, (n, a) in enumerate(zip(names, arrays(0x30000000)))]
+    for grads, out in ((names, there), (there, names), (names, None), (mixed, there), (there, mixed)):
+        a, o = c._clip_lists(grads, out)
+        assert lib.tl_clip_workspace(None, a, o, count, 1.0) > 0, (grads is names, out is names)
+    a, o = c._clip_lists(names, there[1:] + [DeviceArray(0x40000000, (41, 3))])
+    assert lib.tl_clip_workspace(None, a, o, count, 1.0) == -abi.TL_ERR_INVALID
+
+
 def test_null_arguments(lib):
     assert lib.tl_attention_forward(None, None) == abi.TL_ERR_INVALID
     assert lib.tl_attention_backward(None, None) == abi.TL_ERR_INVALID
