@@ -194,19 +194,25 @@ class Context:
     # current stream: torch.cuda.current_stream().cuda_stream), or None for the
     # context's own stream, on which its programs run.  Device tensors that
     # another stream wrote need that stream's work done or waited for first.
-    def _view(self, x, what, write=False):
+    def _view(self, x, what):
         """(data, type, shape, strides) of an array argument."""
         if isinstance(x, str):
             if self._foreign:
                 raise abi.TLError(abi.TL_ERR_INVALID, f"{what}: a tensor's storage is used on the context's own stream")
             a = abi.Array()
-            self.check(self.lib.tl_tensor_array(self._lookup(x), 1 if write else 0, C.byref(a)), f"{what} {x}")
+            self.check(self.lib.tl_tensor_array(self._lookup(x), 0, C.byref(a)), f"{what} {x}")
             return a.data or 0, a.dtype, tuple(a.dims[:a.rank]), tuple(a.strides[:a.rank])
         t = _type_of.get(x.dtype)
         if t is None:
             t = self._type(x.dtype, what)
         self._on_device(x, what)
         return x.data_ptr(), t, x.shape, x.stride()
+
+    def _wrote(self, xs, what):
+        """Tells the tensors among the arrays that a call has been queued which writes their storage."""
+        for x in xs:
+            if isinstance(x, str):
+                self.check(self.lib.tl_tensor_array(self._lookup(x), 1, C.byref(abi.Array())), f"{what} {x}")
 
     def _type(self, dtype, what):
         t = _TYPES.get(str(dtype))
@@ -219,9 +225,9 @@ class Context:
         if x.get_device() != self.device:
             raise abi.TLError(abi.TL_ERR_INVALID, f"{what} is on {x.device}, the context on cuda:{self.device}")
 
-    def _heads(self, x, what, write=False):
+    def _heads(self, x, what):
         """The fields of an array of rank 2 to 4 as [batch, heads, positions, head size]."""
-        p, t, shape, strides = self._view(x, what, write)
+        p, t, shape, strides = self._view(x, what)
         r = len(shape)
         if r != 4:
             if r < 2 or r > 4:
@@ -234,7 +240,7 @@ class Context:
         if isinstance(x, str):
             if kind != "float32":
                 raise abi.TLError(abi.TL_ERR_INVALID, f"{what} is an array of {kind}, not a tensor's name")
-            p, _, have, _ = self._view(x, what, what in ("lse", "norm"))
+            p, _, have, _ = self._view(x, what)
         else:
             self._on_device(x, what)
             if str(x.dtype).rpartition(".")[2] != kind or not x.is_contiguous():
@@ -268,14 +274,14 @@ class Context:
         return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
     def _attention(self, q, k, v, out, lse, grads, scale, softcap, slopes, causal, prefix_len, q_doc, k_doc, kv_len,
-                   q_start, workspace, stream, writes_out):
+                   q_start, workspace, stream):
         stream = self._stream(stream)
-        qa, ka, va, oa = self._heads(q, "q"), self._heads(k, "k"), self._heads(v, "v"), self._heads(out, "out", writes_out)
+        qa, ka, va, oa = self._heads(q, "q"), self._heads(k, "k"), self._heads(v, "v"), self._heads(out, "out")
         b, hq, nq, d = qa[3:7]
         nk = ka[5]
         ga = _NO_GRADS
         if grads:
-            ga = sum((self._heads(x, n, n != "dout") for x, n in zip(grads, ("dout", "dq", "dk", "dv"))), ())
+            ga = sum((self._heads(x, n) for x, n in zip(grads, ("dout", "dq", "dk", "dv"))), ())
         if scale is None:
             scale = d ** -0.5 if d else 1.0
         ws, room = self._room(workspace)
@@ -301,8 +307,9 @@ class Context:
         kv_len - Nq when None.  lse [batch, Hq, Nq] fp32 receives what the backward pass needs.
         """
         d = self._attention(q, k, v, out, lse, None, scale, softcap, slopes, causal, prefix_len, q_doc, k_doc, kv_len,
-                            q_start, workspace, stream, True)
+                            q_start, workspace, stream)
         self.check(self.lib.tl_attention_forward(self.h, d), "attention")
+        self._wrote((out, lse), "attention")
         return out
 
     def attention_backward(self, q, k, v, out, lse, dout, dq, dk, dv, *, scale=None, softcap=0.0, slopes=None,
@@ -310,20 +317,21 @@ class Context:
                            workspace=None, stream=None):
         """Writes dq, dk, dv, the gradient of sum(out * dout) (tl_attention_backward); out and lse are the forward's."""
         d = self._attention(q, k, v, out, lse, (dout, dq, dk, dv), scale, softcap, slopes, causal, prefix_len, q_doc,
-                            k_doc, kv_len, q_start, workspace, stream, False)
+                            k_doc, kv_len, q_start, workspace, stream)
         self.check(self.lib.tl_attention_backward(self.h, d), "attention_backward")
+        self._wrote((dq, dk, dv), "attention_backward")
         return dq, dk, dv
 
     def attention_workspace(self, q, k, v, out, lse=None, grads=None, *, scale=None, softcap=0.0, slopes=None,
                             causal=False, prefix_len=None, q_doc=None, k_doc=None, kv_len=None, q_start=None):
         """Bytes of workspace of an attention call, with grads = (dout, dq, dk, dv) of its backward pass."""
         d = self._attention(q, k, v, out, lse, grads, scale, softcap, slopes, causal, prefix_len, q_doc, k_doc, kv_len,
-                            q_start, None, None, grads is None)
+                            q_start, None, None)
         n = self.lib.tl_attention_workspace(self.h, d, 1 if grads else 0)
         self.check(max(0, -n), "attention_workspace")
         return n
 
-    def _list(self, arrays, what, write):
+    def _list(self, arrays, what):
         """Packs arrays as tl_array (a contiguous one as its elements in a row)."""
         n = len(arrays)
         if n > 16 and not any(isinstance(x, str) for x in arrays) and all(map(_IS_CONTIGUOUS, arrays)):
@@ -342,7 +350,7 @@ class Context:
             return out.tobytes()
         parts = []
         for x in arrays:
-            p, t, shape, strides = self._view(x, what, write)
+            p, t, shape, strides = self._view(x, what)
             r = len(shape)
             if _in_a_row(shape, strides) if isinstance(x, str) else x.is_contiguous():
                 shape, strides, r = (prod(shape),), (1,), 1
@@ -354,7 +362,7 @@ class Context:
     def _clip_lists(self, grads, out):
         if out is not None and len(out) != len(grads):
             raise abi.TLError(abi.TL_ERR_INVALID, f"clip: {len(out)} outputs for {len(grads)} gradients")
-        return self._list(grads, "gradient", out is None), None if out is None else self._list(out, "output", True)
+        return self._list(grads, "gradient"), None if out is None else self._list(out, "output")
 
     def clip_gradients(self, grads, max_norm, out=None, norm=None, workspace=None, stream=None):
         """Scales the arrays so that their global norm is at most max_norm (tl_clip_gradients).
@@ -368,6 +376,8 @@ class Context:
         at = None if norm is None else self._plain(norm, "norm", "float32", ())
         self.check(self.lib.tl_clip_gradients(self.h, a, o, len(grads), max_norm,
                                               at, *self._room(workspace), stream), "clip_gradients")
+        self._wrote(grads if out is None else out, "clip_gradients")
+        self._wrote((norm,), "clip_gradients")
         return grads if out is None else out
 
     def clip_workspace(self, grads, max_norm, out=None):

@@ -622,7 +622,7 @@ def test_workspace_of_either_precision(ctx):
             g = (dout, like(q, "bhsd"), like(k, "bhsd"), like(v, "bhsd"))
             for grads in (None, g):
                 fields = ctx._attention(q, k, v, out, lse, grads, None, 0.0, None, False, None, None, None, None, None,
-                                        None, None, True)
+                                        None, None)
                 any_context = ctx.lib.tl_attention_workspace(None, C.c_char_p(fields), 1 if grads else 0)
                 assert any_context >= max(x.attention_workspace(q, k, v, out, lse, grads) for x in (ctx, c))
     finally:
@@ -677,6 +677,48 @@ def test_named_tensors_stay_on_their_stream(ctx):
     x = torch.zeros((8, 16), device="cuda")
     with pytest.raises(abi.TLError):
         ctx.attention("Xq", x, x, torch.empty_like(x), stream=stream())
+
+
+def test_names_are_marked_as_written_by_calls_that_write(ctx):
+    # asking for a workspace, a refused call and reading leave a 0/1 tensor one (with its bit rows)
+    from tensor_logic_lang_b200 import abi
+    rows, d = 24, 16
+    gen = np.random.default_rng(1)
+    for n in ("Mq", "Mk", "Mv", "Mdo"):
+        ctx.create(n, (rows, d))
+        ctx.upload(n, gen.standard_normal((rows, d)))
+    out, lse, grads = "Mo", "Mlse", ("Mdq", "Mdk", "Mdv")
+    marked = (out, *grads)
+    for n in marked:
+        ctx.create(n, (rows, d))
+    ctx.create(lse, (1, rows))
+    ctx.create("Mnorm", (1, 1))
+    for n in (*marked, lse, "Mnorm"):
+        ctx.upload(n, np.ones(ctx.shape(n)))
+
+    def still(names):
+        for n in names:
+            assert (ctx.tensor(n) == 1).all()
+            ctx.bits(n)                         # refused where a tensor may hold other values
+    ctx.attention_workspace("Mq", "Mk", "Mv", out, lse)
+    ctx.attention_workspace("Mq", "Mk", "Mv", out, lse, ("Mdo", *grads))
+    ctx.clip_workspace(list(grads), 1.0)
+    for bad in (dict(softcap=-1.0), dict(prefix_len=ints([3]))):
+        with pytest.raises(abi.TLError):
+            ctx.attention("Mq", "Mk", "Mv", out, lse, **bad)
+        with pytest.raises(abi.TLError):
+            ctx.attention_backward("Mq", "Mk", "Mv", out, lse, "Mdo", *grads, **bad)
+    with pytest.raises(abi.TLError):
+        ctx.clip_gradients(list(grads), -1.0, norm="Mnorm")
+    still((*marked, lse, "Mnorm"))
+    ctx.attention_backward("Mq", "Mk", "Mv", out, lse, "Mdo", *grads)
+    still((out, lse))
+    ctx.attention("Mq", "Mk", "Mv", out, lse)
+    ctx.clip_gradients(list(grads), 0.5, norm="Mnorm")
+    for n in (*marked, lse, "Mnorm"):
+        assert not (ctx.tensor(n) == 1).all()
+        with pytest.raises(abi.TLError):
+            ctx.bits(n)
 
 
 def test_second_device():
