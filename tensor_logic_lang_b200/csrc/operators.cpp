@@ -269,6 +269,7 @@ tl_status run_attention(tl_ctx* c, const tl_attention* t, bool backward) {
     cudaStream_t s = static_cast<cudaStream_t>(t->stream);
     bool capturing;
     TL_TRY(check_stream(c, s, &capturing));
+    if (capturing) c->flags_captured = true;
     void* ws = nullptr;
     TL_TRY(op_workspace(c, s, capturing, attention_need(a, backward), t->workspace, t->workspace_bytes, &ws));
     if (backward)

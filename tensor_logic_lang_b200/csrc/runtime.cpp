@@ -379,11 +379,11 @@ extern "C" const char* tl_last_error(const tl_ctx* c) { return c ? c->err.c_str(
 namespace tl {
 // Device-side error words: [8] a tensor-core pipeline wait gave up.
 tl_status check_device_flags(tl_ctx* c) {
-    // only the tensor-core GEMM and the message-passing SpMM write the error
-    // word (1: a pipeline wait ran out, 2: a wait for another rank's tiles
-    // ran out): without one since the last read there is nothing to read
+    // only the tensor-core GEMM, attention and the message-passing SpMM write
+    // the error word (1: a pipeline wait ran out, 2: a wait for another rank's
+    // tiles ran out): without one since the last read there is nothing to read
     // (and no reason to wait for the stream)
-    if (!c->flags_armed) return TL_OK;
+    if (!c->flags_armed && !c->flags_captured) return TL_OK;
     c->flags_armed = false;
     TL_CK(c, cudaMemcpyAsync(c->h_flags + 8, c->d_flags + 8, sizeof(int), cudaMemcpyDeviceToHost, c->stream));
     TL_CK(c, cudaStreamSynchronize(c->stream));

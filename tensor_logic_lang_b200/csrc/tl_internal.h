@@ -194,6 +194,8 @@ struct tl_ctx {
     int fix_shape_teams = -1, fix_wpb = 0, fix_per_sm = 0;
     // a tensor-core GEMM was given the device error word since it was last read
     bool flags_armed = false;
+    // a captured graph of the caller's holds kernels that were: it may run at any time
+    bool flags_captured = false;
     // a closure fixpoint whose control block has not been read yet (fix_resolve)
     bool fix_pending = false, fix_prof = false, fix_last_changed = false;
     double fix_sweep_bytes = 0;

@@ -721,6 +721,39 @@ def test_names_are_marked_as_written_by_calls_that_write(ctx):
             ctx.bits(n)
 
 
+def test_replayed_graphs_report_to_sync():
+    # tl_sync reads the device's error word after work that may write it: a captured call's replays too
+    from tensor_logic_lang_b200.runtime import Context
+    c = Context(device=0)
+
+    def read_by_sync():
+        with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+            c.sync()
+            torch.cuda.synchronize()
+        return any("DtoH" in e.name for e in prof.events())
+    try:
+        gen = torch.Generator(device="cuda").manual_seed(4)
+        q, k, v = (heads(gen, 1, 2, 200, 64, "bf16") for _ in range(3))
+        out = like(q, "bhsd")
+        c.sync()
+        read_by_sync()
+        c.attention(q, k, v, out, stream=stream())
+        torch.cuda.synchronize()
+        if not read_by_sync():
+            pytest.skip("the profiler sees no copies here")
+        assert not read_by_sync()               # nothing since
+        ws = torch.empty(256 + c.attention_workspace(q, k, v, out), dtype=torch.uint8, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c.attention(q, k, v, out, stream=stream(), workspace=ws)
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert read_by_sync()
+    finally:
+        c.close()
+
+
 def test_second_device():
     if torch.cuda.device_count() < 2:
         pytest.skip("needs two GPUs")
