@@ -321,8 +321,10 @@ __device__ __forceinline__ void tma_tile(uint32_t dst, const HeadMap& m, uint64_
 // over a Chebyshev grid gives it).  16-bit probabilities: |u| <= 0.75, degree 3,
 // 1.1e-5, far below the rounding of p.  Fp32: |u| <= 0.625, degree 5, 3.9e-9, below
 // the rounding of fp32.  Tiles that hold a larger score take tanh u =
-// 1 - 2 / (1 + e^2u) (fp32: for those scores alone; there 1.2e-7 off is
-// relative to more than 0.55).
+// 1 - 2 / (1 + e^2u), which is off by 1.2e-7 of 1, so its scores by 1.2e-7 of the
+// cap: fp32, and 16-bit types where that counts beside P's error (top above
+// kFarTop), take it for the larger scores alone, 16-bit types with small caps for
+// all of the tile.
 template <bool FINE>
 __device__ __forceinline__ constexpr float tanh_coef(int i) {
     if (FINE)
@@ -331,6 +333,7 @@ __device__ __forceinline__ constexpr float tanh_coef(int i) {
     return i == 0 ? 0.9999889731407166f : i == 1 ? -0.33269670605659485f : i == 2 ? 0.12742698192596436f : -0.035452794283628464f;
 }
 
+constexpr float kFarTop = 128.f;
 template <bool FINE>
 struct CapCoef {
     static constexpr int N = FINE ? 5 : 3;
@@ -341,7 +344,6 @@ struct CapCoef {
     float top;         // softcap log2 e
     float c[N + 1];    // 16-bit: P's coefficients times scale log2(e) k2^i
     __device__ __forceinline__ CapCoef(float scale, float cap) {
-        limit = (FINE ? 0.625f : 0.75f) * (cap / scale);
         k2 = (scale / cap) * (scale / cap);
         mul = scale * kLog2e;
         wide = 2.f * kLog2e * scale / cap;
@@ -352,7 +354,7 @@ struct CapCoef {
             c[i] = tanh_coef<FINE>(i) * f;
             if (!FINE) f *= k2;
         }
-        if (!(fabsf(c[N]) < 3e38f)) limit = -1.f;   // out of range: never the polynomial
+        limit = fabsf(c[N]) < 3e38f ? (FINE ? 0.625f : 0.75f) * (cap / scale) : -1.f;   // out of range: never the polynomial
     }
     // score / x in base 2 of a pair within the limit
     __device__ __forceinline__ f2 ratio(f2 x) const {
@@ -377,19 +379,34 @@ __device__ __forceinline__ float largest(const f2 (&x)[N]) {
     }
     return big;
 }
-// The score in base 2 of a pair in a tile with scores past the limit.
-template <bool FINE>
+// The score in base 2 of a pair in a tile with scores past the limit; EACH: those within
+// it take the polynomial.
+template <bool EACH, bool FINE>
 __device__ __forceinline__ f2 wide_score(f2 x, const CapCoef<FINE>& cap) {
     float lo, hi;
     unpack2(x, lo, hi);
     float y = cap.top * wide_tanh(lo, cap.wide), z = cap.top * wide_tanh(hi, cap.wide);
-    if (FINE) {
+    if (EACH) {
         float a, b;
         unpack2(mul2(x, cap.ratio(x)), a, b);
         y = fabsf(lo) <= cap.limit ? a : y;
         z = fabsf(hi) <= cap.limit ? b : z;
     }
     return pack2(y, z);
+}
+// The scores in base 2 of a row, in place; one choice for all of a warp's rows.
+template <bool FINE, int N>
+__device__ __forceinline__ void cap_scores(f2 (&x)[N], const CapCoef<FINE>& cap) {
+    if (!__any_sync(0xffffffffu, !(largest(x) <= cap.limit))) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = mul2(x[i], cap.ratio(x[i]));
+    } else if (FINE || cap.top > kFarTop) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = wide_score<true>(x[i], cap);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = wide_score<false>(x[i], cap);
+    }
 }
 
 // ---------------------------------------------------------------- documents

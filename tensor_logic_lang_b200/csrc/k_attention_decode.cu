@@ -587,16 +587,24 @@ __global__ void __launch_bounds__(DmSmem<DP>::THREADS, DmSmem<DP>::PER_SM)
                 constexpr int E = decltype(e_count)::value;
                 const bool masked = kd || j0 + KW > all_see;
                 float top[2] = {-INFINITY, -INFINITY};
+                f2 y[NK * E / 2];   // pairs of keys of a row
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
+                for (int i = 0; i < NK * E / 2; ++i) y[i] = pack2(s[i % NK][i / NK * 2], s[i % NK][i / NK * 2 + 1]);
+                if (a.cap > 0.f) {
+                    cap_scores(y, cap);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NK * E / 2; ++i) y[i] = mul2(y[i], pack2(cap.mul, cap.mul));
+                }
+#pragma unroll
+                for (int i = 0; i < NK * E / 2; ++i) {
+                    const int x = i % NK, e = i / NK * 2;
                     const DecRow& w = row[e >> 1];
-                    const float at = (float)(w.p - j0 - 2 * tid - (e & 1));
-#pragma unroll
-                    for (int x = 0; x < NK; ++x) {
-                        float y = s[x][e];
-                        y = a.cap > 0.f ? cap.top * wide_tanh(y, cap.wide) : y * cap.mul;
-                        s[x][e] = fmaf(-w.slope2, fabsf(at - (float)(8 * x)), y);
-                    }
+                    const float at = (float)(w.p - j0 - 8 * x - 2 * tid);
+                    float lo, hi;
+                    unpack2(y[i], lo, hi);
+                    s[x][e] = fmaf(-w.slope2, fabsf(at), lo);
+                    s[x][e + 1] = fmaf(-w.slope2, fabsf(at - 1.f), hi);
                 }
                 if (masked) {
 #pragma unroll

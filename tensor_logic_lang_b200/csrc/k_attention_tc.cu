@@ -135,13 +135,14 @@ __global__ void __launch_bounds__(256) k_attn_begin(const __grid_constant__ Begi
 template <bool CAP, bool BIAS, bool FINE, bool FIX>
 __device__ __forceinline__ float score_row(f2 (&x)[32], float c1, const CapCoef<FINE>& cap, f2 shift, float slope2, int p, int j0,
                                            bool masked, uint32_t bits0, uint32_t bits1) {
-    if (CAP) {
+    if (CAP && !FIX) cap_scores(x, cap);
+    if (CAP && FIX) {   // its caps are small (kFixTop)
         if (__any_sync(0xffffffffu, !(largest(x) <= cap.limit))) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = FIX ? add2(wide_score<FINE>(x[i], cap), shift) : wide_score<FINE>(x[i], cap);
+            for (int i = 0; i < 32; ++i) x[i] = add2(wide_score<false>(x[i], cap), shift);
         } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = FIX ? fma2(x[i], cap.ratio(x[i]), shift) : mul2(x[i], cap.ratio(x[i]));
+            for (int i = 0; i < 32; ++i) x[i] = fma2(x[i], cap.ratio(x[i]), shift);
         }
     }
     if (BIAS) {

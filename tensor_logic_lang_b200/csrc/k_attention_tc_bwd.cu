@@ -209,13 +209,7 @@ __device__ __forceinline__ void grad_row(f2 (&x)[16], uint32_t (&p16)[16], uint3
                                          bool masked, uint32_t bits, NL nl) {
     f2 bend[CAP ? 16 : 1];
     if (CAP) {
-        if (__any_sync(0xffffffffu, !(largest(x) <= cap.limit))) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = wide_score<SPLIT>(x[i], cap);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = mul2(x[i], cap.ratio(x[i]));
-        }
+        cap_scores(x, cap);
         // 1 - tanh^2, the tanh from the score
         const float inv = -1.f / (cap.top * cap.top);
 #pragma unroll

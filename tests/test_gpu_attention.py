@@ -491,6 +491,40 @@ def test_cap_at_the_ends_of_the_tanh(ctx, cap):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cap", [200.0, 1e4, 1e6, 3e7, 1e8, 1e12])
+def test_caps_far_above_the_scores(ctx, cap, dtype):
+    # a cap that bends nothing changes nothing: the scores keep their digits beside it
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for b, nq, d in ((1, 1, 64), (3, 3, 128), (1, 150, 128), (2, 300, 64)):
+        q, k, v = heads(gen, b, 4, nq, d, dtype), heads(gen, b, 2, 400, d, dtype), heads(gen, b, 2, 400, d, dtype)
+        q.mul_(2.0)
+        dout = heads(gen, b, 4, nq, d, dtype)
+        m = {"softcap": cap, "causal": True}
+        want = reference(q, k, v, dout, **m)
+        got = run(ctx, q, k, v, dout, m)
+        for n in want:
+            check(got[n], want[n], (nq, n))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cap", [100.0, 1e4, 1e5])
+def test_large_and_small_scores_in_one_tile(ctx, cap, dtype):
+    # every third query's scores pass the cap; the rows beside it keep the digits of theirs
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for nq in (1, 3, 150):
+        q, k, v = heads(gen, 1, 4, nq, 64, dtype), heads(gen, 1, 2, 300, 64, dtype), heads(gen, 1, 2, 300, 64, dtype)
+        k.mul_(4.0)
+        q.mul_(0.5)
+        q[:, 0, ::3].mul_(min(cap, 1e4))        # fp16 ends at 65504
+        dout = heads(gen, 1, 4, nq, 64, dtype)
+        m = {"softcap": cap, "causal": True}
+        want = reference(q, k, v, dout, **m)
+        got = run(ctx, q, k, v, dout, m)
+        for n in want:
+            check(got[n], want[n], (nq, n))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_many_sequences(ctx, dtype):
     # more sequences than a block has threads, most of them short or empty
     for b, nq in ((700, 1), (300, 3), (90, 40)):
