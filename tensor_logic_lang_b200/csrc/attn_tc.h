@@ -354,7 +354,18 @@ struct CapCoef {
             c[i] = tanh_coef<FINE>(i) * f;
             if (!FINE) f *= k2;
         }
-        limit = fabsf(c[N]) < 3e38f ? (FINE ? 0.625f : 0.75f) * (cap / scale) : -1.f;   // out of range: never the polynomial
+        // 16-bit: a coefficient below fp32's normal numbers (scale much smaller than
+        // the cap) is left out, and the polynomial ends where its term is 1e-6 of the score
+        float end = FINE ? 0.625f : 0.75f;
+        if (!FINE) {
+#pragma unroll
+            for (int i = N; i >= 1; --i)
+                if (fabsf(c[i]) < 0x1p-126f) {
+                    c[i] = 0.f;
+                    end = i == 3 ? 0.1f : i == 2 ? 0.05f : 1e-3f;
+                }
+        }
+        limit = fabsf(c[N]) < 3e38f ? end * (cap / scale) : -1.f;   // out of range: never the polynomial
     }
     // score / x in base 2 of a pair within the limit
     __device__ __forceinline__ f2 ratio(f2 x) const {

@@ -524,6 +524,21 @@ def test_large_and_small_scores_in_one_tile(ctx, cap, dtype):
             check(got[n], want[n], (nq, n))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cap", [1e6, 3e7, 1e9])
+def test_bent_scores_of_a_large_cap(ctx, cap, dtype):
+    # scores up to three quarters of a cap that is 1e7 to 1e10 times the scale: a row's one large weight is
+    # that of its largest score, so lse is the bent score itself
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    for nq in (1, 150):
+        q, k, v = heads(gen, 1, 4, nq, 64, dtype), heads(gen, 1, 2, 300, 64, dtype), heads(gen, 1, 2, 300, 64, dtype)
+        x = (q.double() @ k.double().repeat_interleave(2, 1).transpose(-1, -2)).abs().amax().item() * 64 ** -0.5
+        q.mul_(0.74 * cap / x)
+        m = {"softcap": cap}
+        got = run(ctx, q, k, v, None, m)
+        check(got["lse"], reference(q, k, v, **m)["lse"], nq)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_many_sequences(ctx, dtype):
     # more sequences than a block has threads, most of them short or empty
