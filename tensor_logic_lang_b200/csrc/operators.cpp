@@ -228,6 +228,11 @@ tl_status check_attention(tl_ctx* c, const tl_attention& t, bool backward, AttnC
         if (reinterpret_cast<uintptr_t>(w.first) % 4) return fail(c, TL_ERR_INVALID, "attention: %s is misaligned", w.second);
     if (!isfinite(t.scale)) return fail(c, TL_ERR_INVALID, "attention: scale is not finite");
     if (!isfinite(t.softcap) || t.softcap < 0) return fail(c, TL_ERR_INVALID, "attention: softcap is negative or not finite");
+    // what the kernels make of the two (their quotient, its squares, the cap's
+    // square) stays within fp32's normal numbers
+    const double sc = fabs((double)t.scale), cap = t.softcap;
+    if (cap > 0 && (cap < 0x1p-60 || cap > 0x1p100 || sc > cap * 0x1p60))
+        return fail(c, TL_ERR_UNSUPPORTED, "attention: softcap %g with scale %g is out of range", cap, (double)t.scale);
     if (t.causal != 0 && t.causal != 1) return fail(c, TL_ERR_INVALID, "attention: causal is 0 or 1");
     if (t.prefix_len && !t.causal) return fail(c, TL_ERR_INVALID, "attention: prefix_len is for causal calls");
     if (!t.q_doc != !t.k_doc) return fail(c, TL_ERR_INVALID, "attention: q_doc and k_doc come together");
@@ -238,7 +243,9 @@ tl_status check_attention(tl_ctx* c, const tl_attention& t, bool backward, AttnC
     a.q = view(t.q); a.k = view(t.k); a.v = view(t.v); a.o = view(t.o);
     if (backward) { a.dout = view(t.dout); a.dq = view(t.dq); a.dk = view(t.dk); a.dv = view(t.dv); }
     a.lse = t.lse;
-    a.scale = t.scale; a.cap = t.softcap; a.causal = t.causal;
+    a.scale = t.scale; a.causal = t.causal;
+    // q.k below 2^47 is then below 2^-13 of the cap, where the tanh is its argument to 2^-27
+    a.cap = cap > sc * 0x1p60 ? 0.f : t.softcap;
     a.slopes = t.slopes; a.prefix_len = t.prefix_len; a.q_doc = t.q_doc; a.k_doc = t.k_doc;
     a.kv_len = t.kv_len; a.q_start = t.q_start;
     a.cuda_cores = c && c->opts.precision == TL_PREC_FP32 && a.dtype == TL_TYPE_F32;

@@ -87,6 +87,15 @@ def test_refused_addresses(lib, name):
     assert need(lib, attention(causal=1, **dict(both, **{name: 0x3004}))) >= 0
 
 
+def test_refused_caps(lib):
+    # caps whose quotients with the scale, or squares, leave fp32
+    for scale, softcap in ((1.0, 1e-30), (1.0, 2.0 ** -61), (1e-20, 1e-40), (1e30, 2.0 ** 101), (1e20, 1.0), (-1e20, 1.0)):
+        for backward in (0, 1):
+            assert need(lib, attention(scale=scale, softcap=softcap), backward) == -abi.TL_ERR_UNSUPPORTED
+    for scale, softcap in ((1.0, 2.0 ** -60), (1.0, 2.0 ** 100), (0.0, 1.0), (1e-30, 1e30), (2.0 ** 60, 1.0)):
+        assert need(lib, attention(scale=scale, softcap=softcap)) >= 0
+
+
 def test_refused_sizes(lib):
     assert need(lib, attention(d=257)) == -abi.TL_ERR_UNSUPPORTED
     assert need(lib, attention(d=256)) >= 0

@@ -540,6 +540,27 @@ def test_bent_scores_of_a_large_cap(ctx, cap, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_caps_at_the_ends_of_their_range(ctx, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    for nq in (1, 3, 150):
+        q, k, v = heads(gen, 1, 4, nq, 64, dtype), heads(gen, 1, 2, 300, 64, dtype), heads(gen, 1, 2, 300, 64, dtype)
+        q[:, 1] = 0.0                           # scores of 0
+        dout = heads(gen, 1, 4, nq, 64, dtype)
+        for scale, cap in ((0.125, 2.0 ** -60), (0.125, 2.0 ** -40), (0.125, 2.0 ** 56), (0.125, 2.0 ** 100), (2.0 ** 30, 2.0 ** -30),
+                           (-0.125, 2.0 ** -60), (-0.125, 2.0 ** 100)):
+            m = {"softcap": cap, "causal": True, "scale": scale}
+            want = reference(q, k, v, dout, **m)
+            got = run(ctx, q, k, v, dout, m)
+            for n in ("out", "lse", "dv"):
+                check(got[n], want[n], (nq, scale, cap, n))
+            for n in ("dq", "dk"):
+                # at q = 0 the tanh is its argument, so dq is 2^30 dx k under a scale of 2^30: past 65504, fp16's
+                # largest number, where dx k is above 2^-14
+                past = want[n][0].abs() + want[n][1] > torch.finfo(got[n].dtype).max
+                assert (torch.isfinite(got[n]) | (past & torch.isinf(got[n]))).all(), (nq, scale, cap, n)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_many_sequences(ctx, dtype):
     # more sequences than a block has threads, most of them short or empty
     for b, nq in ((700, 1), (300, 3), (90, 40)):
