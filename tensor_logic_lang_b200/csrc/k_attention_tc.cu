@@ -51,6 +51,7 @@ namespace {
 // on them, no rescaling.
 constexpr float kFixTop = 72.5f;
 __device__ __forceinline__ float fixed_top(float top) { return top - 20.f; }
+constexpr float kFuseTop = 0x1p12f;   // half a step of it is 2^-12, less than P's rounding
 constexpr float kGrow = 8.f;   // rescale when the maximum grew by 2^8
 
 struct FwArgs {
@@ -526,7 +527,17 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
             }
             // p = 2^(c x - m), -inf gives 0; a row with no key yet keeps m = 0 here
             const float ref = (m == -INFINITY ? 0.f : m) - Lift<T>::log2;
-            const f2 c2 = pack2(c, c), ref2 = pack2(-ref, -ref);
+            // c x - m in one step keeps what rounding m cut off, half a step of m: nothing of
+            // the row's sum is left, or more than fp16 holds, where that is many powers of two.
+            // Large scores are rounded before, as m was (rows beside theirs then too, by at
+            // most 2^-12 of a power of two).
+            float by = c;
+            if (!CAP && !BIAS && __any_sync(0xffffffffu, m > -INFINITY && fabsf(m) > kFuseTop)) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) x[i] = mul2(x[i], pack2(c, c));
+                by = 1.f;
+            }
+            const f2 c2 = pack2(by, by), ref2 = pack2(-ref, -ref);
             f2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
             for (int k = 0; k < 2; ++k) {

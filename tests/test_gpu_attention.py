@@ -561,6 +561,40 @@ def test_caps_at_the_ends_of_their_range(ctx, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [2.0 ** 12, 2.0 ** 21, 2.0 ** 24, 2.0 ** 30, 2.0 ** 60])
+def test_scores_without_a_fraction(ctx, scale, dtype):
+    # q.k are whole numbers: a row's weight lies on the keys of its largest score alone, in equal parts, so
+    # what is off is v's bits (fp32: 22), the sums' and the result's rounding
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    for hq, nq, nk in ((2, 1, 300), (4, 150, 700), (1, 130, 4300), (8, 600, 600)):
+        q, k, v = heads(gen, 2, hq, nq, 64, dtype), heads(gen, 2, 1, nk, 64, dtype), heads(gen, 2, 1, nk, 64, dtype)
+        q.mul_(2.0).round_(), k.mul_(2.0).round_()
+        m = {"scale": scale, "causal": True}
+        got = run(ctx, q, k, v, None, m)
+        # (softmax of 64-bit scores of 2^37 would lose bits of the logarithm of the number of equal parts)
+        x = q.double() @ k.double().transpose(-1, -2)
+        x = x.masked_fill(~torch.ones((nq, nk), dtype=torch.bool, device="cuda").tril(nk - nq), -np.inf)
+        largest = x.amax(-1, keepdim=True)
+        w = (x == largest).double()
+        out = (w / w.sum(-1, keepdim=True)) @ v.double()
+        one = torch.finfo(v.dtype).eps / 2 + 2.0 ** -20
+        check(got["out"], (out, one * (out.abs() + v.double().abs().amax())), "out")
+        lse = largest[..., 0] * scale + w.sum(-1).log()
+        check(got["lse"], (lse, 2.0 ** -22 * lse.abs() + 2.0 ** -16), "lse")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_products_whose_squares_pass_fp32(ctx, dtype):
+    # under a cap far above them, which counts as none
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    for nq in (1, 3, 150):
+        q, k, v = heads(gen, 1, 4, nq, 64, dtype), heads(gen, 1, 2, 300, 64, dtype), heads(gen, 1, 2, 300, 64, dtype)
+        q.mul_(2.0 ** 40), k.mul_(2.0 ** 40)
+        m = {"softcap": 2.0 ** 99, "scale": 2.0 ** -10}
+        check(run(ctx, q, k, v, None, m)["lse"], reference(q, k, v, **m)["lse"], nq)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_many_sequences(ctx, dtype):
     # more sequences than a block has threads, most of them short or empty
     for b, nq in ((700, 1), (300, 3), (90, 40)):
