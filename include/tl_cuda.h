@@ -472,7 +472,9 @@ tl_status tl_tensor_array(tl_tensor* t, int32_t write, tl_array* out);
  * softmax and its statistics are in 32 bits (so the backward pass's exponentials
  * are good to 2^-24 of |s| and |lse|).  16-bit types take their products
  * from 16-bit operands (exponentials, and dx of the backward pass, rounded to
- * them).  fp32 arrays of head size up to 128 take 22 bits of each operand of a
+ * them).  bf16 calls with a softcap up to 50.2 and no slopes may take exponentials of the
+ * scores themselves, 2^-72 to 2^72: values of v below 2^-44 then lose bits in rows whose
+ * scores all lie near -softcap, and above 2^54 / Nk they may overflow near +softcap.  fp32 arrays of head size up to 128 take 22 bits of each operand of a
  * product, or 2^-39 of the largest of its kind in the heads that share a key
  * head where that is more (a value that is not finite then makes the results that
  * depend on it NaN); larger ones, and all of a TL_PREC_FP32 context, 24 bits on

@@ -491,6 +491,26 @@ def test_cap_at_the_ends_of_the_tanh(ctx, cap):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("power", [-40, -30, -20, -12, 12, 30])
+def test_values_of_any_size_under_a_cap(ctx, power, dtype):
+    # rows whose scores all lie near the lower end of the tanh, all near the upper one, or anywhere, and rows
+    # that see one key: the exponentials' size does not show in what they weigh
+    if dtype == "f16" and not -12 <= power <= 12:
+        pytest.skip("outside fp16")
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    for hq, nq, nk in ((4, 1, 300), (4, 150, 300), (2, 130, 4300), (32, 700, 700)):
+        q, k, v = heads(gen, 1, hq, nq, 64, dtype), heads(gen, 1, 2, nk, 64, dtype), heads(gen, 1, 2, nk, 64, dtype)
+        k[:, 0].abs_()
+        q[:, 0].abs_().neg_(), q[:, hq // 2 - 1].abs_()
+        q.mul_(40.0)
+        v.mul_(2.0 ** power)
+        m = {"softcap": 50.0, "causal": True}
+        got, want = run(ctx, q, k, v, None, m), reference(q, k, v, **m)
+        for n in ("out", "lse"):
+            check(got[n], want[n], (hq, nq, n))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("cap", [200.0, 1e4, 1e6, 3e7, 1e8, 1e12])
 def test_caps_far_above_the_scores(ctx, cap, dtype):
     # a cap that bends nothing changes nothing: the scores keep their digits beside it
