@@ -9,6 +9,8 @@
 // rows contracted: p v, dx k, p^T dout, dx^T q).
 #pragma once
 
+#include <float.h>
+
 #include "attention.h"
 #include "tc_ptx.h"
 
@@ -64,6 +66,9 @@ template <> __device__ __forceinline__ uint32_t pack16<__half>(float lo, float h
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+
+// 2^e, of e in fp32's normal numbers (their ends beyond)
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
 
 // ---------------------------------------------------------------- tcgen05
 // One lane of a converged warp.  ptxas knows that the branch it guards has one
@@ -255,12 +260,12 @@ __device__ __forceinline__ void tmem_add(uint32_t acc, uint32_t from, bool fresh
     }
 }
 
-// A row of DP fp32 sums in TMEM, scaled, as values of an array: 16-bit rows
-// are 16-byte aligned (tc_array), fp32 ones may lie anyhow.  any: there are sums
+// A row of DP fp32 sums in TMEM, scaled (by mul and then by post, of fp32 arrays, whose product may pass fp32), as
+// values of an array: 16-bit rows are 16-byte aligned (tc_array), fp32 ones may lie anyhow.  any: there are sums
 // (else zeros); live: the columns may be read (the same for the whole warp).
 template <typename U, int DP>
 __device__ __forceinline__ void store_row(const HeadsView& v, int b, int h, int64_t row, bool on, int d, uint32_t taddr, bool any,
-                                          bool live, float mul) {
+                                          bool live, float mul, float post = 1.f) {
     U* p = static_cast<U*>(v.p) + b * v.sb + h * v.sh + row * v.ss;
     const bool wide = std::is_same<U, float>::value && v.sd == 1 && d % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
     for (int k = 0; k < DP / 16; ++k) {
@@ -277,7 +282,7 @@ __device__ __forceinline__ void store_row(const HeadsView& v, int b, int h, int6
                 if (c >= d) break;
                 float w[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = any ? __uint_as_float(o[4 * q + e]) * mul : 0.f;
+                for (int e = 0; e < 4; ++e) w[e] = any ? __uint_as_float(o[4 * q + e]) * mul * post : 0.f;
                 if (wide) {
                     *reinterpret_cast<float4*>(p + c) = make_float4(w[0], w[1], w[2], w[3]);
                 } else {
@@ -344,9 +349,11 @@ struct CapCoef {
     float top;         // softcap log2 e
     float c[N + 1];    // 16-bit: P's coefficients times scale log2(e) k2^i
     __device__ __forceinline__ CapCoef(float scale, float cap) {
-        k2 = (scale / cap) * (scale / cap);
+        // split operands have scales of any size; their products are 0 or above 2^-48, so 2^63 bends alike
+        const float u = FINE ? fminf(scale / cap, 0x1p63f) : scale / cap;
+        k2 = u * u;
         mul = scale * kLog2e;
-        wide = 2.f * kLog2e * scale / cap;
+        wide = FINE ? 2.f * kLog2e * u : 2.f * kLog2e * scale / cap;
         top = cap * kLog2e;
         float f = FINE ? 1.f : mul;
 #pragma unroll
@@ -565,11 +572,16 @@ struct SplitPlan {
 // stats: of the backward pass, null in a forward one
 tl_status launch_split(tl_ctx* c, const AttnCall& a, float* stats, uint8_t* ws, HeadMap* maps, DocRange* q_ranges, DocRange* k_ranges,
                        cudaStream_t s);
-// the power of two of a group, from its largest value
+// the power of two of a group, from its largest value (below 2^-112, where fp32 itself ends, it stays smaller)
 __device__ __forceinline__ int split_exp(const uint32_t* top, int group) {
     const float m = __uint_as_float(top[group]);
-    if (!(m > 0.f) || m > 3.4e38f) return 0;
-    return min(max(14 - ilogbf(m), -60), 60);
+    if (!(m > 0.f) || !(m <= FLT_MAX)) return 0;
+    return min(14 - ilogbf(m), 126);
+}
+// the scale of scores whose operands carry the powers of two e together.  Within 2^-126 .. 2^126 whatever they
+// are: products of split operands, below 2^37, are scores of 0 at the lower end, and pass fp32 past the upper one
+__device__ __forceinline__ float split_scale(float scale, int e) {
+    return fminf(fmaxf(scale * pow2(-e / 2) * pow2(-e - -e / 2), 0x1p-126f), 0x1p126f);
 }
 struct SplitTops {
     const uint32_t *q, *k, *v, *dout;    // null: operands are the arrays themselves

@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
             u[k][f] = on ? two(p + (r0 + k) * x.v.ss, x.v.sd, c + 64 * f, a.d, pairs) : make_float2(0.f, 0.f);
     }
     if (WRITE) {
-        const float up = exp2f((float)split_exp(x.top, group));
+        const float up = pow2(split_exp(x.top, group));
         __half* out = x.out + ((int64_t)bh * x.n + r0) * (128 * HALVES) + c;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {

@@ -188,7 +188,7 @@ __device__ void join_parts(uint8_t* smem, const FwArgs& g, int part, int b, int 
     const AttnCall& a = g.a;
     const int parts = g.parts, rows = g.pack ? g.pack * (a.hq / a.hkv) : TILE;
     const int lane = threadIdx.x & 31, share = TILE / parts, d0 = 4 * lane;
-    const float out_scale = L::SPLIT ? exp2f((float)-split_exp(g.tops.v, b * a.hkv + kvh)) : 1.f;
+    const float out_scale = L::SPLIT ? pow2(-split_exp(g.tops.v, b * a.hkv + kvh)) : 1.f;
     for (int r = part * share + threadIdx.x / 32; r < min((part + 1) * share, rows); r += L::SOFTMAX / 32) {
         const int i = g.pack ? i0 + r % g.pack : i0 + r, h = g.pack ? h0 + r / g.pack : h0;
         if (i >= a.nq) continue;
@@ -211,12 +211,12 @@ __device__ void join_parts(uint8_t* smem, const FwArgs& g, int part, int b, int 
             }
         }
         const bool none = sum == 0.f;
-        const float inv = none ? 0.f : out_scale / sum;
+        const float inv = none ? 0.f : 1.f / sum;
         U* p = static_cast<U*>(a.o.p) + b * a.o.sb + h * a.o.sh + i * a.o.ss;
         if constexpr (std::is_same<U, float>::value) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (d0 + e < a.d) p[(d0 + e) * a.o.sd] = none ? 0.f : o[e] * inv;
+                if (d0 + e < a.d) p[(d0 + e) * a.o.sd] = none ? 0.f : o[e] * inv * out_scale;
         } else if (d0 < a.d) {   // d is a multiple of 8, the rows lie on 16 bytes
             *reinterpret_cast<uint2*>(p + d0) =
                 none ? make_uint2(0, 0) : make_uint2(pack16<U>(o[0] * inv, o[1] * inv), pack16<U>(o[2] * inv, o[3] * inv));
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
         float* rows_at = reinterpret_cast<float*>(smem + L::ROWS) + t * 2 * TILE + r;   // [parity][tile][half][row]
         // split operands carry powers of two of their heads
         const int e_qk = SPLIT ? split_exp(g.tops.q, b * a.hkv + kvh) + split_exp(g.tops.k, b * a.hkv + kvh) : 0;
-        const float scale = SPLIT ? a.scale * exp2f((float)-e_qk) : a.scale;
+        const float scale = SPLIT ? split_scale(a.scale, e_qk) : a.scale;
         const float c1 = scale * kLog2e, c = CAP || BIAS ? 1.f : c1;
         const CapCoef<SPLIT> cap(scale, CAP ? a.cap : 1.f);
         const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
@@ -563,11 +563,12 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
         asm volatile("bar.sync %0, 256;" ::"r"(1 + t) : "memory");
         l += mine_at[(1 - half) * TILE];
         const bool none = it == 0 || l == 0.f;   // no key seen
-        float inv = none ? 0.f : 1.f / l;
+        const float inv = none ? 0.f : 1.f / l;
+        float post = 1.f;
         if (ok && SPLIT && it > 0) {
             tmem_add<DH>(acc, to, it == 1);
             tmem_wait_st();
-            inv *= exp2f((float)-split_exp(g.tops.v, b * a.hkv + kvh));
+            post = pow2(-split_exp(g.tops.v, b * a.hkv + kvh));
         }
         if (NT == 1 && parts > 1) {
             if (ok) {
@@ -590,7 +591,7 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
         } else if (ok) {
             HeadsView o = a.o;
             o.p = static_cast<U*>(o.p) + half * DH * o.sd;
-            store_row<U, DH>(o, b, h, i, on, a.d - half * DH, acc, !none, it > 0, inv);
+            store_row<U, DH>(o, b, h, i, on, a.d - half * DH, acc, !none, it > 0, inv, post);
             if (a.lse && on && half == 0)
                 a.lse[((int64_t)b * a.hq + h) * a.nq + i] = none ? -INFINITY : (FIX ? 0.f : m - Lift<T>::log2) * kLn2 + logf(l);
         }

@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         const int which = wg / 2, col0 = wg % 2 * DH;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const SplitExps ex = split_exps<SPLIT>(g, b, kvh);
-        const float scale = SPLIT ? a.scale * exp2f((float)-(ex.q + ex.k)) : a.scale, c1 = scale * kLog2e;
+        const float scale = SPLIT ? split_scale(a.scale, ex.q + ex.k) : a.scale, c1 = scale * kLog2e;
         const CapCoef<SPLIT> cap(scale, CAP ? a.cap : 1.f);
         const float lift = dx_lift<T>(g, b, kvh), up = lift * PLift<T>::back;
         const float up_dp = SPLIT ? up * exp2f((float)-(ex.dout + ex.v)) : up;   // dp carries the powers of dout and v
@@ -967,7 +967,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         const int wg = warp / 4, r = threadIdx.x % TILE, i = i0 + r;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const SplitExps ex = split_exps<SPLIT>(g, b, kvh);
-        const float scale = SPLIT ? a.scale * exp2f((float)-(ex.q + ex.k)) : a.scale, c1 = scale * kLog2e;
+        const float scale = SPLIT ? split_scale(a.scale, ex.q + ex.k) : a.scale, c1 = scale * kLog2e;
         const CapCoef<SPLIT> cap(scale, CAP ? a.cap : 1.f);
         const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
         const float lift = dx_lift<T>(g, b, kvh), up = lift * PLift<T>::back;

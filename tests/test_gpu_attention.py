@@ -701,6 +701,22 @@ def test_values_of_very_different_size(ctx, dtype):
         check(got[n], want[n], n)
 
 
+@pytest.mark.parametrize("sizes", [(1, 1, 1e-30), (1, 1, 1e30), (1, 1, 1e-37), (1e-25, 1e25, 1), (1e27, 1e-27, 1e20), (1e-30, 1, 1),
+                                   (1e-25, 1e-25, 1), (1e17, 1e17, 1e-20), (1e-19, 1e20, 1e-24)])
+@pytest.mark.parametrize("d", [64, 100])
+def test_fp32_values_of_any_size(ctx, d, sizes):
+    # q, k and v anywhere in the range of fp32 keep their digits
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    for hq, nq, nk, names in ((2, 1, 300, ""), (4, 150, 150, "causal"), (2, 130, 4300, "slopes"), (8, 300, 700, "cap causal")):
+        q, k, v = heads(gen, 1, hq, nq, d, "f32"), heads(gen, 1, 2, nk, d, "f32"), heads(gen, 1, 2, nk, d, "f32")
+        for x, by in zip((q, k, v), sizes):
+            x.mul_(by)
+        m = modifiers(names, 1, hq, nq, nk, 0)
+        got, want = run(ctx, q, k, v, None, m), reference(q, k, v, **m)
+        for n in ("out", "lse"):
+            check(got[n], want[n], (hq, nq, n))
+
+
 @pytest.mark.parametrize("d", [64, 80, 128])
 def test_fp32_errors_do_not_grow_with_the_tiles(ctx, d):
     # of the norm of a result: a tile's sums are cut 24 times (8 steps of 3 products) by half a
