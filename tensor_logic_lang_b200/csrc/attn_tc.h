@@ -560,7 +560,7 @@ struct SplitArray {
     HeadsView v;
     int h, n;
     bool keys;          // rows count below kv_len and in documents of k_doc (else of q_doc)
-    int norm;           // largest row norm^2 into norms[2 * (b * hkv + key head) + norm]; -1: none
+    int norm;           // largest row norm^2, of what out holds, into norms[2 * (b * hkv + key head) + norm]; -1: none
     __half* out;
     uint32_t* top;      // [b, hkv] largest |x| of the group's heads as bits
 };

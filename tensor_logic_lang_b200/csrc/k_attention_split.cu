@@ -1,6 +1,6 @@
 // fp32 arrays as pairs of fp16 for the tensor-core attention kernels: the
 // largest value of every group of heads, then hi and lo of every value (attn_tc.h,
-// SplitArray).  HBM-bound: the arrays are read twice (the second time mostly
+// SplitArray), and what the backward pass needs of the rows.  HBM-bound: the arrays are read twice (the second time mostly
 // from the L2 cache) and their 4 bytes a value written once.
 //
 // Three fp16 products of 11-bit parts give 22 bits; TF32 would take the same
@@ -17,8 +17,9 @@ constexpr int SP_ROWS = 64;   // of a block of 8 warps
 struct SplitArgs {
     AttnCall a;
     SplitArray arr[4];
+    // backward: of operands with their powers of two, so that no square leaves fp32
     uint32_t* norms;
-    float* stats;     // backward: [b, hq, query tiles][2][128], -log2(e) lse + lift and -D = -dout.out of each row
+    float* stats;     // [b, hq, query tiles][2][128], -log2(e) lse + lift and -D = -dout.out of each row
 };
 
 __device__ __forceinline__ bool row_counts(const AttnCall& a, const SplitArray& x, int b, int64_t r) {
@@ -36,6 +37,20 @@ __device__ __forceinline__ float2 two(const float* row, int64_t sd, int c, int d
 }
 __device__ __forceinline__ bool in_pairs(const HeadsView& v, int d) {
     return v.sd == 1 && d % 2 == 0 && (v.ss | v.sh | v.sb) % 2 == 0 && reinterpret_cast<uintptr_t>(v.p) % 8 == 0;
+}
+
+// The largest of a block's values into *to.  Non-negative floats order like their
+// bits; a maximum does not depend on the order.
+__device__ __forceinline__ void block_max(float v, uint32_t* to) {
+    __shared__ uint32_t most[8];
+    const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+    if ((threadIdx.x & 31) == 0) most[threadIdx.x / 32] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint32_t all = 0;
+        for (int k = 0; k < 8; ++k) all = max(all, most[k]);
+        atomicMax(to, all);
+    }
 }
 
 // A warp takes 8 rows, a lane columns 2 lane and 2 lane + 1 of every 64.
@@ -63,6 +78,10 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
     }
     if (WRITE) {
         const float up = pow2(split_exp(x.top, group));
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int f = 0; f < HALVES; ++f) u[k][f] = make_float2(u[k][f].x * up, u[k][f].y * up);
         __half* out = x.out + ((int64_t)bh * x.n + r0) * (128 * HALVES) + c;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -70,15 +89,15 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
 #pragma unroll
             for (int f = 0; f < HALVES; ++f) {
                 uint32_t hi, lo;
-                split16(u[k][f].x * up, u[k][f].y * up, hi, lo);
+                split16(u[k][f].x, u[k][f].y, hi, lo);
                 *reinterpret_cast<uint32_t*>(out + (k * HALVES + f) * 128) = hi;
                 *reinterpret_cast<uint32_t*>(out + (k * HALVES + f) * 128 + 64) = lo;
             }
         }
-    } else {
         if (g.stats && blockIdx.y == 3) {
             // dout: D of its rows, and the statistics of whole tiles
             const float* o = static_cast<const float*>(a.o.p) + b * a.o.sb + h * a.o.sh;
+            const float up_o = pow2(split_exp(g.arr[2].top, group));   // o's values are within those of v
             const int64_t qt = r0 / TILE, q_tiles = blocks / (TILE / SP_ROWS);
             float* st = g.stats + ((int64_t)bh * q_tiles + qt) * 2 * TILE + r0 % TILE;
             const bool live = lane < 8 && row_counts(a, x, b, r0 + lane);
@@ -92,7 +111,7 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
 #pragma unroll
                 for (int f = 0; f < HALVES; ++f) {
                     const float2 y = two(o + (r0 + k) * a.o.ss, a.o.sd, c + 64 * f, a.d, o_pairs);
-                    dot[k] = fmaf(u[k][f].x, y.x, fmaf(u[k][f].y, y.y, dot[k]));
+                    dot[k] = fmaf(u[k][f].x, y.x * up_o, fmaf(u[k][f].y, y.y * up_o, dot[k]));
                 }
             }
             float d = 0.f;
@@ -108,36 +127,27 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
                 st[TILE + lane] = -d;
             }
         }
-        float top = 0.f, norm = 0.f;
+        if (x.norm >= 0) {
+            float norm = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            float n2 = 0.f;
+            for (int k = 0; k < 8; ++k) {
+                float n2 = 0.f;
 #pragma unroll
-            for (int f = 0; f < HALVES; ++f) {
-                top = fmaxf(top, fmaxf(fabsf(u[k][f].x), fabsf(u[k][f].y)));
-                n2 = fmaf(u[k][f].x, u[k][f].x, fmaf(u[k][f].y, u[k][f].y, n2));
-            }
-            if (x.norm >= 0) {
+                for (int f = 0; f < HALVES; ++f) n2 = fmaf(u[k][f].x, u[k][f].x, fmaf(u[k][f].y, u[k][f].y, n2));
 #pragma unroll
-                for (int o = 16; o; o >>= 1) n2 += __shfl_xor_sync(0xffffffffu, n2, o);
+                for (int m = 16; m; m >>= 1) n2 += __shfl_xor_sync(0xffffffffu, n2, m);
                 norm = fmaxf(norm, n2);
             }
+            block_max(norm, &g.norms[2 * group + x.norm]);
         }
+    } else {
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int f = 0; f < HALVES; ++f) top = fmaxf(top, fmaxf(fabsf(u[k][f].x), fabsf(u[k][f].y)));
         wait_for_previous();   // the maxima start at 0
-        // non-negative floats order like their bits; a maximum does not depend on the order
-        __shared__ uint32_t most[2][8];
-        const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-        if (lane == 0) {
-            most[0][warp] = m;
-            most[1][warp] = __float_as_uint(norm);
-        }
-        __syncthreads();
-        if (threadIdx.x < 2) {
-            uint32_t all = 0;
-            for (int k = 0; k < 8; ++k) all = max(all, most[threadIdx.x][k]);
-            if (threadIdx.x == 0) atomicMax(&x.top[group], all);
-            else if (x.norm >= 0) atomicMax(&g.norms[2 * group + x.norm], all);
-        }
+        block_max(top, &x.top[group]);
     }
 }
 

@@ -189,15 +189,24 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// The power of two that dx is written with (see the top of the file).
+// The power of two that dx is written with (see the top of the file), as its
+// exponent.  Split operands: beside those that dout and v carry.
 template <typename T>
-__device__ __forceinline__ float dx_lift(const BwArgs& g, int b, int kvh) {
-    if (PLift<T>::log2 == 0.f) return 1.f;
+__device__ __forceinline__ int dx_exp(const BwArgs& g, int b, int kvh) {
+    if (PLift<T>::log2 == 0.f) return 0;
     const uint32_t* n = g.norms + 2 * ((int64_t)b * g.a.hkv + kvh);
     const float bound = 2.f * sqrtf(__uint_as_float(n[0])) * sqrtf(__uint_as_float(n[1]));
-    if (!(bound > 0.f) || bound > 3e38f) return 1.f;
-    return exp2f(fminf(fmaxf(floorf(15.f - log2f(bound)), -100.f), 100.f));
+    if (!(bound > 0.f) || bound > 3e38f) return 0;
+    return (int)fminf(fmaxf(floorf(15.f - log2f(bound)), -100.f), 100.f);
 }
+
+// a 2^e, of split operands in two factors, each within fp32
+template <bool SPLIT>
+struct Factors {
+    float mul, post;
+    __device__ __forceinline__ Factors(float a, int e) : mul(a * pow2(SPLIT ? e / 2 : e)), post(SPLIT ? pow2(e - e / 2) : 1.f) {}
+    __device__ __forceinline__ float of(uint32_t bits) const { return __uint_as_float(bits) * mul * post; }
+};
 
 // ---------------------------------------------------------------- elements
 // 32 scores q.k of a row -> p in base 2 (16-bit pairs) and p (1 - tanh^2).
@@ -404,11 +413,11 @@ struct HalfRing {
 };
 
 // A row's columns col0 .. col0 + N - 1 of an fp32 output (+)= N TMEM columns times
-// mul.  The thread alone owns them, so additions that the L2 makes, which nothing
+// f.  The thread alone owns them, so additions that the L2 makes, which nothing
 // waits for, come in one order (loads and stores took 6 us more a tile of 96 columns).
-template <int N>
-__device__ __forceinline__ void add_row(const HeadsView& v, int b, int h, int64_t row, int col0, bool on, int d, uint32_t taddr, float mul,
-                                        bool fresh) {
+template <int N, bool SPLIT>
+__device__ __forceinline__ void add_row(const HeadsView& v, int b, int h, int64_t row, int col0, bool on, int d, uint32_t taddr,
+                                        const Factors<SPLIT>& f, bool fresh) {
     float* p = static_cast<float*>(v.p) + b * v.sb + h * v.sh + row * v.ss + col0 * v.sd;
     const bool wide = v.sd == 1 && d % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
 #pragma unroll 1
@@ -421,7 +430,7 @@ __device__ __forceinline__ void add_row(const HeadsView& v, int b, int h, int64_
         for (int q = 0; q < 16; q += 4) {
             float x[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(o[q + e]) * mul;
+            for (int e = 0; e < 4; ++e) x[e] = f.of(o[q + e]);
             float* at = p + (k + q) * v.sd;
             if (wide && fresh) {
                 if (q < left) *reinterpret_cast<float4*>(at) = make_float4(x[0], x[1], x[2], x[3]);
@@ -675,10 +684,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         const SplitExps ex = split_exps<SPLIT>(g, b, kvh);
         const float scale = SPLIT ? split_scale(a.scale, ex.q + ex.k) : a.scale, c1 = scale * kLog2e;
         const CapCoef<SPLIT> cap(scale, CAP ? a.cap : 1.f);
-        const float lift = dx_lift<T>(g, b, kvh), up = lift * PLift<T>::back;
-        const float up_dp = SPLIT ? up * exp2f((float)-(ex.dout + ex.v)) : up;   // dp carries the powers of dout and v
+        const int e_dx = dx_exp<T>(g, b, kvh);
+        const float up = pow2(e_dx) * PLift<T>::back;   // (split operands: dp and D carry the powers of dout and v)
         const int doc = kd && j < a.nk ? kd[j] : -1;
-        const float mul = (which ? a.scale / lift : PLift<T>::back) * (SPLIT ? exp2f((float)-(which ? ex.q : ex.dout)) : 1.f);
+        // dk = scale dx^T q, dv = p^T dout
+        const Factors<SPLIT> f(which ? a.scale : PLift<T>::back, which ? -(e_dx + ex.dout + ex.v + ex.q) : -ex.dout);
         int n = 0;
         for (; qt >= 0 && ok; next(), ++n) {
             const int i0 = qt * TILE + wg * BW_COLS;
@@ -706,7 +716,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 // dv of the tile before, done before this S
                 if (WIDE) {
                     if (which == 0 && n > 0)
-                        add_row<DH>(g.dv, b, out_h, j, col0, j < a.nk, a.d, t_dv + lanes + col0, mul, n == 1);
+                        add_row<DH>(g.dv, b, out_h, j, col0, j < a.nk, a.d, t_dv + lanes + col0, f, n == 1);
                 } else if (SPLIT && which == 0 && n > 0) {
                     tmem_add<DH>(t_dva + lanes + col0, t_dv + lanes + col0, n == 1);
                 }
@@ -726,14 +736,14 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 // dk of the tile before, done before this dp
                 if (WIDE) {
                     if (which == 1 && n > 0)
-                        add_row<DH>(g.dk, b, out_h, j, col0, j < a.nk, a.d, t_dk + lanes + col0, mul, n == 1);
+                        add_row<DH>(g.dk, b, out_h, j, col0, j < a.nk, a.d, t_dk + lanes + col0, f, n == 1);
                 } else if (SPLIT && which == 1 && n > 0) {
                     tmem_add<DH>(t_dka + lanes + col0, t_dk + lanes + col0, n == 1);
                 }
                 uint32_t dp[32], dx[16], low[16];
                 tmem_load(t_dp + lanes + wg * BW_COLS, dp);
                 const f2 up2 = pack2(up, up);
-                grad_dx<T, SPLIT>(x, dp, dx, low, up_dp, masked, bits, [&](int i) {
+                grad_dx<T, SPLIT>(x, dp, dx, low, up, masked, bits, [&](int i) {
                     const f2 d = *reinterpret_cast<const f2*>(st + TILE + 2 * i);
                     return PLift<T>::log2 == 0.f ? d : mul2(d, up2);
                 });
@@ -755,11 +765,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             mine_at = acc;
         }
         if (WIDE && any) {
-            if (ok) add_row<DH>(which ? g.dk : g.dv, b, out_h, j, col0, j < a.nk, a.d, mine_at, mul, n <= 1);
+            if (ok) add_row<DH>(which ? g.dk : g.dv, b, out_h, j, col0, j < a.nk, a.d, mine_at, f, n <= 1);
         } else if (g.cluster == 1) {
             HeadsView v = which ? g.dk : g.dv;
             v.p = static_cast<U*>(v.p) + col0 * v.sd;
-            if (ok) store_row<U, DH>(v, b, out_h, j, j < a.nk, a.d - col0, mine_at, any, any, mul);
+            if (ok) store_row<U, DH>(v, b, out_h, j, j < a.nk, a.d - col0, mine_at, any, any, f.mul, f.post);
         } else if (ok) {
             float* row = reinterpret_cast<float*>(smem) + (which * TILE + r) * L::SUM_LD + col0;
             for (int k = 0; k < DH / 16; ++k) {
@@ -771,8 +781,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                     *reinterpret_cast<float4*>(row + 16 * k + 4 * q) =
-                        make_float4(__uint_as_float(o[4 * q]) * mul, __uint_as_float(o[4 * q + 1]) * mul,
-                                    __uint_as_float(o[4 * q + 2]) * mul, __uint_as_float(o[4 * q + 3]) * mul);
+                        make_float4(f.of(o[4 * q]), f.of(o[4 * q + 1]), f.of(o[4 * q + 2]), f.of(o[4 * q + 3]));
             }
         }
         __syncwarp();
@@ -970,8 +979,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         const float scale = SPLIT ? split_scale(a.scale, ex.q + ex.k) : a.scale, c1 = scale * kLog2e;
         const CapCoef<SPLIT> cap(scale, CAP ? a.cap : 1.f);
         const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
-        const float lift = dx_lift<T>(g, b, kvh), up = lift * PLift<T>::back;
-        const float up_dp = SPLIT ? up * exp2f((float)-(ex.dout + ex.v)) : up;   // dp carries the powers of dout and v
+        const int e_dx = dx_exp<T>(g, b, kvh);
+        const float up = pow2(e_dx) * PLift<T>::back;   // (split operands: dp and D carry the powers of dout and v)
         const float* st = g.stats + (((int64_t)b * a.hq + h) * g.q_tiles + qt) * 2 * TILE;
         const float nl = st[r], nd = st[TILE + r] * up;
         const f2 nl2 = pack2(nl, nl), nd2 = pack2(nd, nd);
@@ -1006,7 +1015,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 if (SPLIT && n > 0) tmem_add<DO / 4>(t_dqa + lanes + wg * (DO / 4), t_dq + lanes + wg * (DO / 4), n == 1);
                 uint32_t dp[32], dx[16], low[16];
                 tmem_load(t_dp + lanes + wg * BW_COLS, dp);
-                grad_dx<T, SPLIT>(x, dp, dx, low, up_dp, masked, bits, [&](int) { return nd2; });
+                grad_dx<T, SPLIT>(x, dp, dx, low, up, masked, bits, [&](int) { return nd2; });
                 tmem_st16(t_dp + lanes + wg * BW_COLS, dx);
                 if (SPLIT) tmem_st16(t_dp + lanes + wg * BW_COLS + 16, low);
             }
@@ -1019,18 +1028,17 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         if (ok) {
             constexpr int PART = DO / 4;
             uint32_t at = t_dq + lanes + wg * PART;
-            float mul = a.scale / lift;
             if (SPLIT) {
                 if (any) {
                     tmem_add<PART>(t_dqa + lanes + wg * PART, at, n == 1);
                     tmem_wait_st();
                 }
                 at = t_dqa + lanes + wg * PART;
-                mul *= exp2f((float)-ex.k);
             }
+            const Factors<SPLIT> f(a.scale, -(e_dx + ex.dout + ex.v + ex.k));
             HeadsView v = a.dq;
             v.p = static_cast<U*>(v.p) + wg * PART * v.sd;
-            store_row<U, PART>(v, b, h, i, i < a.nq, a.d - wg * PART, at, any, any, mul);
+            store_row<U, PART>(v, b, h, i, i < a.nq, a.d - wg * PART, at, any, any, f.mul, f.post);
         }
     }
     wait_for_previous();   // the dk, dv kernel, which this one did not need, so that its end is the call's

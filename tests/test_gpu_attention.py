@@ -717,6 +717,22 @@ def test_fp32_values_of_any_size(ctx, d, sizes):
             check(got[n], want[n], (hq, nq, n))
 
 
+@pytest.mark.parametrize("sizes", [(1, 1, 1, 1e-24), (1, 1, 1, 1e20), (1, 1, 1e-20, 1e-10), (1, 1, 1e25, 1e-20), (1, 1, 1e20, 1e15),
+                                   (1e-10, 1e10, 1e-15, 1e-15), (1e10, 1e-10, 1e-18, 1e10), (1e-20, 1e20, 1e-30, 1e25), (1, 1, 1e-25, 1e-9)])
+@pytest.mark.parametrize("d", [64, 100])
+def test_fp32_gradients_of_any_size(ctx, d, sizes):
+    gen = torch.Generator(device="cuda").manual_seed(22)
+    for hq, nq, nk, names in ((2, 150, 150, "causal"), (4, 300, 260, "cap"), (8, 130, 700, "slopes"), (6, 520, 520, "cap causal")):
+        q, k, v = heads(gen, 1, hq, nq, d, "f32"), heads(gen, 1, 2, nk, d, "f32"), heads(gen, 1, 2, nk, d, "f32")
+        dout = heads(gen, 1, hq, nq, d, "f32")
+        for x, by in zip((q, k, v, dout), sizes):
+            x.mul_(by)
+        m = modifiers(names, 1, hq, nq, nk, 0)
+        got, want = run(ctx, q, k, v, dout, m), reference(q, k, v, dout, **m)
+        for n in want:
+            check(got[n], want[n], (hq, nq, n))
+
+
 @pytest.mark.parametrize("d", [64, 80, 128])
 def test_fp32_errors_do_not_grow_with_the_tiles(ctx, d):
     # of the norm of a result: a tile's sums are cut 24 times (8 steps of 3 products) by half a
