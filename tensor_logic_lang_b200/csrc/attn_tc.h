@@ -70,6 +70,10 @@ template <> __device__ __forceinline__ uint32_t pack16<__half>(float lo, float h
 // 2^e, of e in fp32's normal numbers (their ends beyond)
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
 
+// a value >= 0, or 0 for one that is not finite: a power of two taken from the largest of many then stays
+// that of the others
+__device__ __forceinline__ float finite(float x) { return x <= FLT_MAX ? x : 0.f; }
+
 // ---------------------------------------------------------------- tcgen05
 // One lane of a converged warp.  ptxas knows that the branch it guards has one
 // thread and keeps descriptors in uniform registers there (a branch on the lane
@@ -575,7 +579,7 @@ tl_status launch_split(tl_ctx* c, const AttnCall& a, float* stats, uint8_t* ws, 
 // the power of two of a group, from its largest value (below 2^-112, where fp32 itself ends, it stays smaller)
 __device__ __forceinline__ int split_exp(const uint32_t* top, int group) {
     const float m = __uint_as_float(top[group]);
-    if (!(m > 0.f) || !(m <= FLT_MAX)) return 0;
+    if (!(m > 0.f)) return 0;
     return min(14 - ilogbf(m), 126);
 }
 // the scale of scores whose operands carry the powers of two e together.  Within 2^-126 .. 2^126 whatever they

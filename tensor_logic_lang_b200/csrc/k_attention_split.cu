@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
                 for (int f = 0; f < HALVES; ++f) n2 = fmaf(u[k][f].x, u[k][f].x, fmaf(u[k][f].y, u[k][f].y, n2));
 #pragma unroll
                 for (int m = 16; m; m >>= 1) n2 += __shfl_xor_sync(0xffffffffu, n2, m);
-                norm = fmaxf(norm, n2);
+                norm = fmaxf(norm, finite(n2));
             }
             block_max(norm, &g.norms[2 * group + x.norm]);
         }
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(256) k_split(const __grid_constant__ SplitArgs
 #pragma unroll
         for (int k = 0; k < 8; ++k)
 #pragma unroll
-            for (int f = 0; f < HALVES; ++f) top = fmaxf(top, fmaxf(fabsf(u[k][f].x), fabsf(u[k][f].y)));
+            for (int f = 0; f < HALVES; ++f) top = fmaxf(top, fmaxf(finite(fabsf(u[k][f].x)), finite(fabsf(u[k][f].y))));
         wait_for_previous();   // the maxima start at 0
         block_max(top, &x.top[group]);
     }

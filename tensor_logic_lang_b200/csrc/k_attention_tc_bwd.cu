@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(256)
                 xy += __shfl_xor_sync(0xffffffffu, xy, w);
                 xx += __shfl_xor_sync(0xffffffffu, xx, w);
             }
-            top = fmaxf(top, xx);
+            top = fmaxf(top, finite(xx));
             if (sub == k) mine = xy;
         }
         if (sub < R) {
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(256)
             dot8<T>(x[k], x[k], xy, xx);
 #pragma unroll
             for (int w = 8; w; w >>= 1) xx += __shfl_xor_sync(0xffffffffu, xx, w);
-            top = fmaxf(top, xx);
+            top = fmaxf(top, finite(xx));
         }
     }
     wait_for_previous();   // the norms start at 0; the documents' ranges, which the kernel behind this one reads
@@ -196,7 +196,7 @@ __device__ __forceinline__ int dx_exp(const BwArgs& g, int b, int kvh) {
     if (PLift<T>::log2 == 0.f) return 0;
     const uint32_t* n = g.norms + 2 * ((int64_t)b * g.a.hkv + kvh);
     const float bound = 2.f * sqrtf(__uint_as_float(n[0])) * sqrtf(__uint_as_float(n[1]));
-    if (!(bound > 0.f) || bound > 3e38f) return 0;
+    if (!(bound > 0.f)) return 0;
     return (int)fminf(fmaxf(floorf(15.f - log2f(bound)), -100.f), 100.f);
 }
 

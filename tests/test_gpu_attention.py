@@ -733,6 +733,44 @@ def test_fp32_gradients_of_any_size(ctx, d, sizes):
             check(got[n], want[n], (hq, nq, n))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("size", [2.0 ** -10, 1.0, 2.0 ** 20])
+def test_one_infinity_stays_in_its_tiles(ctx, dtype, bad, size):
+    # a document of one tile holds values that are not finite; the next document's results are its own
+    if dtype == "f16" and size > 1:
+        pytest.skip("outside fp16")
+    gen = torch.Generator(device="cuda").manual_seed(23)
+    for d in (64, 128) if dtype != "f32" else (64, 100):
+        for names in ("", "cap", "slopes"):
+            q, k = heads(gen, 1, 4, 400, d, dtype), heads(gen, 1, 2, 400, d, dtype)
+            v, dout = heads(gen, 1, 2, 400, d, dtype), heads(gen, 1, 4, 400, d, dtype)
+            v.mul_(size), dout.mul_(size)
+            for x in (q, k, v, dout):
+                x[0, 1, 5, 3] = bad
+            m = modifiers(names, 1, 4, 400, 400, 0)
+            docs = ints([[0] * 128 + [1] * 272])
+            got = run(ctx, q, k, v, dout, dict(m, causal=True, q_doc=docs, k_doc=docs))
+            want = reference(*(x[:, :, 128:] for x in (q, k, v, dout)), causal=True, **m)
+            for n in want:
+                check(got[n][:, :, 128:], want[n], n)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("where", ["dout", "v"])
+def test_one_infinity_leaves_small_gradients_their_bits(ctx, where, d):
+    # fp16: dx of 2^-22 and keys of 2^12, beside a document with an infinity
+    gen = torch.Generator(device="cuda").manual_seed(24)
+    q, k = heads(gen, 1, 4, 400, d, "f16"), heads(gen, 1, 2, 400, d, "f16")
+    v, dout = heads(gen, 1, 2, 400, d, "f16"), heads(gen, 1, 4, 400, d, "f16")
+    q.mul_(2.0 ** -12), k.mul_(2.0 ** 12), dout.mul_(2.0 ** -14)
+    (dout if where == "dout" else v)[0, 1, 5, 3] = float("inf")
+    docs = ints([[0] * 128 + [1] * 272])
+    got = run(ctx, q, k, v, dout, dict(causal=True, q_doc=docs, k_doc=docs))
+    want = reference(*(x[:, :, 128:] for x in (q, k, v, dout)), causal=True)
+    check(got["dq"][:, :, 128:], want["dq"], "dq")
+
+
 @pytest.mark.parametrize("d", [64, 80, 128])
 def test_fp32_errors_do_not_grow_with_the_tiles(ctx, d):
     # of the norm of a result: a tile's sums are cut 24 times (8 steps of 3 products) by half a
