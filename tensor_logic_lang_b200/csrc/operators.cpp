@@ -279,10 +279,13 @@ tl_status run_attention(tl_ctx* c, const tl_attention* t, bool backward) {
     if (capturing) c->flags_captured = true;
     void* ws = nullptr;
     TL_TRY(op_workspace(c, s, capturing, attention_need(a, backward), t->workspace, t->workspace_bytes, &ws));
-    if (backward)
-        return attn_tc_backward_takes(a) ? launch_attn_tc_backward(c, a, ws, s) : launch_attn_general_backward(c, a, ws, s);
-    if (attn_few_takes(a)) return launch_attn_few(c, a, ws, s);
-    return attn_tc_takes(a) ? launch_attn_tc(c, a, ws, s) : launch_attn_general(c, a, ws, s);
+    if (!backward && attn_few_takes(a)) return launch_attn_few(c, a, ws, s);
+    const bool tc = backward ? attn_tc_backward_takes(a) : attn_tc_takes(a);
+    if (tc) {
+        const tl_status st = backward ? launch_attn_tc_backward(c, a, ws, s) : launch_attn_tc(c, a, ws, s);
+        if (st != kNoSplit) return st;   // (what was queued only prepares operands; the general kernels need less workspace)
+    }
+    return backward ? launch_attn_general_backward(c, a, ws, s) : launch_attn_general(c, a, ws, s);
 }
 
 // ---------------------------------------------------------------------------
