@@ -474,8 +474,10 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
                     bits1 &= same[1];
                 }
             }
+            // a warp whose wait runs out walks on without waiting: the other warps of the tile meet it at
+            // the barrier of the maxima once a key tile, which has no limit
             ok = ok && mbar_wait(&s_full[t], it & 1, g.err);
-            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
             if (SPLIT && it > 0) tmem_add<DH>(acc, to, it == 1);   // P V of the tile before, done before this S
             f2 x[32];
