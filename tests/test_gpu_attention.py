@@ -161,6 +161,23 @@ def test_layouts(ctx, layout, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("step", [8, 3, 0])
+def test_rows_that_overlap(ctx, step, dtype):
+    # windows over one row of memory: neighbouring positions share elements, or all of them
+    gen = torch.Generator(device="cuda").manual_seed(11)
+
+    def windows(b, h, n, d):
+        room = n * step + d + 8 - d % 8
+        return torch.randn((b, h, room), generator=gen, device="cuda").to(TYPES[dtype]).as_strided((b, h, n, d), (h * room, room, step, 1))
+    for nq in (1, 5, 140):
+        q, k, v, dout = windows(2, 4, nq, 64), windows(2, 2, 140, 64), windows(2, 2, 140, 64), windows(2, 4, nq, 64)
+        m = {"causal": True, "softcap": 3.0}
+        got, want = run(ctx, q, k, v, dout, m, "bshd"), reference(q, k, v, dout, **m)
+        for n in want:
+            check(got[n], want[n], (nq, n))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("nq,nk", [(0, 5), (5, 0), (0, 0)])
 def test_nothing_to_attend(ctx, nq, nk, dtype):
     got = compare(ctx, 2, 2, 1, nq, nk, 64, dtype)
