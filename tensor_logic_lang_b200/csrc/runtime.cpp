@@ -38,6 +38,7 @@ tl_status fail(tl_ctx* c, tl_status code, const char* fmt, ...) {
 }
 
 tl_status cuda_fail(tl_ctx* c, cudaError_t e, const char* what) {
+    cudaGetLastError();   // reported here: the check after the next launch is for that launch
     return fail(c, e == cudaErrorMemoryAllocation ? TL_ERR_OOM : TL_ERR_CUDA, "%s: %s", what,
                 cudaGetErrorString(e));
 }

@@ -391,6 +391,21 @@ def test_streams_side_by_side(ctx):
             check(x, want[n], n)
 
 
+def test_calls_after_one_that_found_no_memory(ctx):
+    from tensor_logic_lang_b200 import abi
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    # dk and dv of 8192 heads that share their keys, 430 GB, before they are added up
+    q, k = torch.zeros((1, 8192, 1, 100), device="cuda"), torch.zeros((1, 1, 65536, 100), device="cuda")
+    lse, dk, dv = torch.zeros(q.shape[:3], device="cuda"), torch.empty_like(k), torch.empty_like(k)
+    assert ctx.attention_workspace(q, k, k, q, lse, (q, torch.empty_like(q), dk, dv)) > torch.cuda.get_device_properties(0).total_memory
+    with pytest.raises(abi.TLError) as said:
+        ctx.attention_backward(q, k, k, q, lse, q, torch.empty_like(q), dk, dv, stream=stream())
+    assert said.value.status == abi.TL_ERR_OOM
+    compare(ctx, 1, 2, 1, 100, 100, 64, "f32", "causal")
+    compare(ctx, 1, 2, 1, 100, 100, 64, "bf16", "causal")
+    torch.cuda.synchronize()
+
+
 def test_refusals_do_nothing(ctx):
     from tensor_logic_lang_b200 import abi
     gen = torch.Generator(device="cuda").manual_seed(4)
