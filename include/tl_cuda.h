@@ -486,8 +486,8 @@ tl_status tl_tensor_array(tl_tensor* t, int32_t write, tl_array* out);
  * k_doc [batch, Nk] int32 are contiguous.  kv_len NULL: all Nk keys; its values
  * are clamped to 0..Nk, those of q_start to +-2^30.  q_start NULL: kv_len[b] - Nq, so that the last query
  * stands at the last key (a cache that already holds the new tokens); a batch
- * padded on the right passes zeros.  softcap is 0 or within 2^-60 .. 2^100, and
- * at least 2^-60 |scale| (else TL_ERR_UNSUPPORTED); above 2^60 |scale| it is as 0.
+ * padded on the right passes zeros.  |scale| is at most 2^120 and softcap is 0 or within 2^-60 .. 2^100, and
+ * at least 2^-60 |scale| (else TL_ERR_UNSUPPORTED); a softcap above 2^60 |scale| is as 0.
  */
 typedef struct tl_attention {
     tl_array q, k, v, o;                /* o: forward writes, backward reads  */

@@ -227,6 +227,8 @@ tl_status check_attention(tl_ctx* c, const tl_attention& t, bool backward, AttnC
     for (const auto& w : words)
         if (reinterpret_cast<uintptr_t>(w.first) % 4) return fail(c, TL_ERR_INVALID, "attention: %s is misaligned", w.second);
     if (!isfinite(t.scale)) return fail(c, TL_ERR_INVALID, "attention: scale is not finite");
+    if (fabsf(t.scale) > 0x1p120f)   // times log2(e) it has to stay in fp32
+        return fail(c, TL_ERR_UNSUPPORTED, "attention: scale %g is out of range", (double)t.scale);
     if (!isfinite(t.softcap) || t.softcap < 0) return fail(c, TL_ERR_INVALID, "attention: softcap is negative or not finite");
     // what the kernels make of the two (their quotient, its squares, the cap's
     // square) stays within fp32's normal numbers

@@ -87,6 +87,15 @@ def test_refused_addresses(lib, name):
     assert need(lib, attention(causal=1, **dict(both, **{name: 0x3004}))) >= 0
 
 
+def test_refused_scales(lib):
+    # times log2(e), 3e38 is infinite, and 0 times that no score
+    for scale in (3e38, -3e38, 2.0 ** 121):
+        for backward in (0, 1):
+            assert need(lib, attention(scale=scale), backward) == -abi.TL_ERR_UNSUPPORTED
+    for scale in (2.0 ** 120, -2.0 ** 120, 0.0, 1e-44):
+        assert need(lib, attention(scale=scale)) >= 0
+
+
 def test_refused_caps(lib):
     # caps whose quotients with the scale, or squares, leave fp32
     for scale, softcap in ((1.0, 1e-30), (1.0, 2.0 ** -61), (1e-20, 1e-40), (1e30, 2.0 ** 101), (1e20, 1.0), (-1e20, 1.0)):
