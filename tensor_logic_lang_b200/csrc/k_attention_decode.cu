@@ -249,12 +249,6 @@ struct DecRow {
         doc = a.q_doc ? a.q_doc[(int64_t)b * a.nq + i] : -1;
         slope2 = a.slopes ? a.slopes[h] * kLog2e : 0.f;
     }
-    // q.k -> score in base 2, -inf when not seen
-    __device__ __forceinline__ float score(float x, int j, int jdoc, const AttnCall& a, const CapCoef<false>& cap) const {
-        float y = a.cap > 0.f ? cap.top * wide_tanh(x, cap.wide) : x * cap.mul;
-        y -= slope2 * fabsf((float)(p - j));
-        return j < limit && (!a.k_doc || (doc >= 0 && jdoc == doc)) ? y : -INFINITY;
-    }
 };
 
 // The end of a piece: `warps` sums of o (rows x ld fp32 each), m, l in shared
