@@ -390,6 +390,9 @@ __device__ __forceinline__ float largest(const f2 (&x)[N]) {
     }
     return big;
 }
+// 16-bit calls whose cap is far above the scores take the kernels with slopes, of 0 where there are none: the code for
+// both forms in one tile costs the others 1 to 4 % (backward, 16 x 2048 x 128 over 4, cap 30: 113.1 us, 115.5 with it).
+inline bool takes_slopes(const AttnCall& a) { return a.slopes || (a.dtype != TL_TYPE_F32 && a.cap * kLog2e > kFarTop); }
 // The score in base 2 of a pair in a tile with scores past the limit; EACH: those within
 // it take the polynomial.
 template <bool EACH, bool FINE>
@@ -406,12 +409,13 @@ __device__ __forceinline__ f2 wide_score(f2 x, const CapCoef<FINE>& cap) {
     return pack2(y, z);
 }
 // The scores in base 2 of a row, in place; one choice for all of a warp's rows.
-template <bool FINE, int N>
+// FAR: caps above kFarTop come here too.
+template <bool FAR, bool FINE, int N>
 __device__ __forceinline__ void cap_scores(f2 (&x)[N], const CapCoef<FINE>& cap) {
     if (!__any_sync(0xffffffffu, !(largest(x) <= cap.limit))) {
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = mul2(x[i], cap.ratio(x[i]));
-    } else if (FINE || cap.top > kFarTop) {
+    } else if (FINE || (FAR && cap.top > kFarTop)) {
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = wide_score<true>(x[i], cap);
     } else {

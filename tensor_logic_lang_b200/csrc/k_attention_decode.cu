@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(DmSmem<DP>::THREADS, DmSmem<DP>::PER_SM)
 #pragma unroll
                 for (int i = 0; i < NK * E / 2; ++i) y[i] = pack2(s[i % NK][i / NK * 2], s[i % NK][i / NK * 2 + 1]);
                 if (a.cap > 0.f) {
-                    cap_scores(y, cap);
+                    cap_scores<true>(y, cap);
                 } else {
 #pragma unroll
                     for (int i = 0; i < NK * E / 2; ++i) y[i] = mul2(y[i], pack2(cap.mul, cap.mul));

@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(256) k_attn_begin(const __grid_constant__ Begi
 template <bool CAP, bool BIAS, bool FINE, bool FIX>
 __device__ __forceinline__ float score_row(f2 (&x)[32], float c1, const CapCoef<FINE>& cap, float slope2, int p, int j0,
                                            bool masked, uint32_t bits0, uint32_t bits1) {
-    if (CAP) cap_scores(x, cap);
+    if (CAP) cap_scores<BIAS>(x, cap);
     if (BIAS) {
         // -slope |p - j| is linear in j on either side of p
         const bool before = __all_sync(0xffffffffu, j0 + 63 <= p), after = __all_sync(0xffffffffu, j0 >= p);
@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
         const float scale = SPLIT ? split_scale(a.scale, e_qk) : a.scale;
         const float c1 = scale * kLog2e, c = CAP || BIAS ? 1.f : c1;
         const CapCoef<SPLIT> cap(scale, CAP ? a.cap : 1.f);
-        const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
+        const float slope2 = BIAS && a.slopes ? a.slopes[h] * kLog2e : 0.f;
         const int doc = qd && i < a.nq ? qd[i] : -1;
         float m = -INFINITY, l = 0.f;
         int it = 0;
@@ -626,7 +626,7 @@ tl_status launch(tl_ctx* c, const HeadMap* m, const FwArgs& g, cudaStream_t s) {
 
 template <typename T, typename U, int DP, int NT>
 tl_status launch_scores(tl_ctx* c, const HeadMap* m, const FwArgs& g, cudaStream_t s) {
-    const bool bias = g.a.slopes != nullptr;
+    const bool bias = takes_slopes(g.a);
     if constexpr (std::is_same<T, __nv_bfloat16>::value)
         if (g.a.cap > 0.f && !bias && g.a.cap * kLog2e <= kFixTop) return launch<T, U, DP, NT, true, false, true>(c, m, g, s);
     if (g.a.cap > 0.f) return bias ? launch<T, U, DP, NT, true, true>(c, m, g, s) : launch<T, U, DP, NT, true, false>(c, m, g, s);

@@ -189,22 +189,22 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// The power of two that dx is written with (see the top of the file), as its
-// exponent.  Split operands: beside those that dout and v carry.
+// The power of two that dx is written with (see the top of the file).  Split
+// operands: beside those that dout and v carry.
 template <typename T>
-__device__ __forceinline__ int dx_exp(const BwArgs& g, int b, int kvh) {
-    if (PLift<T>::log2 == 0.f) return 0;
+__device__ __forceinline__ float dx_lift(const BwArgs& g, int b, int kvh) {
+    if (PLift<T>::log2 == 0.f) return 1.f;
     const uint32_t* n = g.norms + 2 * ((int64_t)b * g.a.hkv + kvh);
     const float bound = 2.f * sqrtf(__uint_as_float(n[0])) * sqrtf(__uint_as_float(n[1]));
-    if (!(bound > 0.f)) return 0;
-    return (int)fminf(fmaxf(floorf(15.f - log2f(bound)), -100.f), 100.f);
+    if (!(bound > 0.f)) return 1.f;
+    return exp2f(fminf(fmaxf(floorf(15.f - log2f(bound)), -100.f), 100.f));
 }
 
-// a 2^e, of split operands in two factors, each within fp32
+// a, of split operands times 2^e in two factors, each within fp32
 template <bool SPLIT>
 struct Factors {
     float mul, post;
-    __device__ __forceinline__ Factors(float a, int e) : mul(a * pow2(SPLIT ? e / 2 : e)), post(SPLIT ? pow2(e - e / 2) : 1.f) {}
+    __device__ __forceinline__ Factors(float a, int e) : mul(SPLIT ? a * pow2(e / 2) : a), post(SPLIT ? pow2(e - e / 2) : 1.f) {}
     __device__ __forceinline__ float of(uint32_t bits) const { return __uint_as_float(bits) * mul * post; }
 };
 
@@ -218,7 +218,7 @@ __device__ __forceinline__ void grad_row(f2 (&x)[16], uint32_t (&p16)[16], uint3
                                          bool masked, uint32_t bits, NL nl) {
     f2 bend[CAP ? 16 : 1];
     if (CAP) {
-        cap_scores(x, cap);
+        cap_scores<BIAS>(x, cap);
         // 1 - tanh^2, the tanh from the score
         const float inv = -1.f / (cap.top * cap.top);
 #pragma unroll
@@ -684,11 +684,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         const SplitExps ex = split_exps<SPLIT>(g, b, kvh);
         const float scale = SPLIT ? split_scale(a.scale, ex.q + ex.k) : a.scale, c1 = scale * kLog2e;
         const CapCoef<SPLIT> cap(scale, CAP ? a.cap : 1.f);
-        const int e_dx = dx_exp<T>(g, b, kvh);
-        const float up = pow2(e_dx) * PLift<T>::back;   // (split operands: dp and D carry the powers of dout and v)
+        const float lift = dx_lift<T>(g, b, kvh), up = lift * PLift<T>::back;   // (split operands: dp and D carry the powers of dout and v)
         const int doc = kd && j < a.nk ? kd[j] : -1;
         // dk = scale dx^T q, dv = p^T dout
-        const Factors<SPLIT> f(which ? a.scale : PLift<T>::back, which ? -(e_dx + ex.dout + ex.v + ex.q) : -ex.dout);
+        const Factors<SPLIT> f(which ? (SPLIT ? a.scale : a.scale / lift) : PLift<T>::back,
+                               SPLIT ? -(which ? ilogbf(lift) + ex.dout + ex.v + ex.q : ex.dout) : 0);
         int n = 0;
         for (; qt >= 0 && ok; next(), ++n) {
             const int i0 = qt * TILE + wg * BW_COLS;
@@ -705,7 +705,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                     bits &= same[0];
                 }
             }
-            const float slope2 = BIAS ? __ldg(a.slopes + h) * kLog2e : 0.f;
+            const float slope2 = BIAS && a.slopes ? __ldg(a.slopes + h) * kLog2e : 0.f;
             const float* st = reinterpret_cast<const float*>(smem + L::STAT + (n % BW_STAGES) * STAT_BYTES) + wg * BW_COLS;
             uint64_t* landed = WIDE ? &bb.stat_full[n & 1] : &bb.full[n % BW_STAGES];   // the statistics
             ok = warp_wait(landed, (n / 2) & 1, ok, g.err);
@@ -978,9 +978,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         const SplitExps ex = split_exps<SPLIT>(g, b, kvh);
         const float scale = SPLIT ? split_scale(a.scale, ex.q + ex.k) : a.scale, c1 = scale * kLog2e;
         const CapCoef<SPLIT> cap(scale, CAP ? a.cap : 1.f);
-        const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
-        const int e_dx = dx_exp<T>(g, b, kvh);
-        const float up = pow2(e_dx) * PLift<T>::back;   // (split operands: dp and D carry the powers of dout and v)
+        const float slope2 = BIAS && a.slopes ? a.slopes[h] * kLog2e : 0.f;
+        const float lift = dx_lift<T>(g, b, kvh), up = lift * PLift<T>::back;   // (split operands: dp and D carry the powers of dout and v)
         const float* st = g.stats + (((int64_t)b * a.hq + h) * g.q_tiles + qt) * 2 * TILE;
         const float nl = st[r], nd = st[TILE + r] * up;
         const f2 nl2 = pack2(nl, nl), nd2 = pack2(nd, nd);
@@ -1035,7 +1034,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                 }
                 at = t_dqa + lanes + wg * PART;
             }
-            const Factors<SPLIT> f(a.scale, -(e_dx + ex.dout + ex.v + ex.k));
+            const Factors<SPLIT> f(SPLIT ? a.scale : a.scale / lift, SPLIT ? -(ilogbf(lift) + ex.dout + ex.v + ex.k) : 0);
             HeadsView v = a.dq;
             v.p = static_cast<U*>(v.p) + wg * PART * v.sd;
             store_row<U, PART>(v, b, h, i, i < a.nq, a.d - wg * PART, at, any, any, f.mul, f.post);
@@ -1107,7 +1106,7 @@ tl_status launch(tl_ctx* c, const HeadMap* m, const BwArgs& g, cudaStream_t s) {
 
 template <typename T, typename U, int DP>
 tl_status launch_scores(tl_ctx* c, const HeadMap* m, const BwArgs& g, cudaStream_t s) {
-    const bool bias = g.a.slopes != nullptr;
+    const bool bias = takes_slopes(g.a);
     if (g.a.cap > 0.f) return bias ? launch<T, U, DP, true, true>(c, m, g, s) : launch<T, U, DP, true, false>(c, m, g, s);
     return bias ? launch<T, U, DP, false, true>(c, m, g, s) : launch<T, U, DP, false, false>(c, m, g, s);
 }
