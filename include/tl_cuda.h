@@ -459,35 +459,44 @@ tl_status tl_tensor_array(tl_tensor* t, int32_t write, tl_array* out);
  *     or j < prefix_len[b]), and (no documents, or q_doc[b,i] == k_doc[b,j] >= 0)
  *   o_i = sum over seen j of softmax(s)_j v_j,  lse_i = log sum exp(s)
  *
- * A query that sees no key gives o = 0 and lse = -inf, and takes and gives no
- * gradient.  What k and v hold at and after kv_len[b] and at keys of a negative
- * document, and q and dout at queries of a negative document, does not matter,
- * not even infinities or NaN; elsewhere a value that is not finite reaches
- * every result it would reach in the formulas (0 times infinity included), and
- * may reach others of the same tile of queries or keys.
+ * A query that sees no key (or keys with scores of -infinity alone) gives o = 0
+ * and lse = -inf, and takes and gives no gradient.  What k and v hold at and after
+ * kv_len[b] and at keys of a negative document, and q and dout at queries of a
+ * negative document, does not matter, not even infinities or NaN; elsewhere a value
+ * that is not finite reaches every result it would reach in the formulas (0 times
+ * infinity included), and may reach others of the same tile of queries or keys.
  *
  * Arrays of rank 4, [batch, heads, positions, head size], of one type, head
  * size 1..256, any strides (k and v may have strides of 0; arrays that are
- * written may not overlap themselves, one another or an input).  Sums, the
- * softmax and its statistics are in 32 bits (so the backward pass's exponentials
- * are good to 2^-24 of |s| and |lse|).  16-bit types take their products
- * from 16-bit operands (exponentials, and dx of the backward pass, rounded to
- * them).  bf16 calls with a softcap up to 50.2 and no slopes may take exponentials of the
- * scores themselves, 2^-72 to 2^72: values of v below 2^-44 then lose bits in rows whose
- * scores all lie near -softcap, and above 2^54 / Nk they may overflow near +softcap.  fp32 arrays of head size up to 128 take 22 bits of each operand of a
- * product, or 2^-39 of the largest of its kind in the heads that share a key
- * head where that is more (a value that is not finite then makes the results that
- * depend on it NaN); larger ones, and all of a TL_PREC_FP32 context, 24 bits on
- * the CUDA cores.  The tensor cores need scale > 0 and, of 16-bit arrays, a
- * contiguous head size that is a multiple of 8, at most 128, and 16-byte
- * aligned rows; other calls take a general kernel, tens of times slower.
+ * written may not overlap themselves, one another or an input).
+ *
+ * Sums, the softmax and its statistics are in 32 bits (so the backward pass's
+ * exponentials are good to 2^-24 of |s| and |lse|, and say nothing where these pass
+ * 2^24).  16-bit types take their products from 16-bit operands (exponentials, and dx
+ * of the backward pass, rounded to them; a capped score is good to 1.1e-5 of itself).
+ * fp32 arrays of head size up to 128 take 22 bits of each operand of a product, or
+ * 2^-39 of the largest of its kind in the heads that share a key head where that is
+ * more (of the forward's exponentials 2^-31 of a row's largest; a value that is not
+ * finite then makes the results that depend on it NaN); larger ones, and all of a
+ * TL_PREC_FP32 context, 24 bits on the CUDA cores.  The tensor cores cut their 32-bit
+ * sums: a sum of one sign over n keys (of dk and dv: n queries) of 16-bit arrays may lose
+ * up to n 2^-27 of itself (5e-4 of 131072 measured, 7e-3 of 2^20).  bf16 calls with a
+ * softcap up to 50.2 and no slopes may take exponentials of the scores themselves, 2^-72
+ * to 2^72: values of v below 2^-44 then lose bits in rows whose scores all lie near
+ * -softcap, and above 2^54 / Nk they may overflow near +softcap.
+ *
+ * The tensor cores need scale > 0 and, of 16-bit arrays, a contiguous head size that
+ * is a multiple of 8, at most 128, and 16-byte aligned rows; other calls take a general
+ * kernel, tens of times slower.
+ *
  * The device arrays slopes [Hq] fp32 (constants: they get no gradient),
  * prefix_len, kv_len, q_start [batch] int32, q_doc [batch, Nq] and
- * k_doc [batch, Nk] int32 are contiguous.  kv_len NULL: all Nk keys; its values
- * are clamped to 0..Nk, those of q_start to +-2^30.  q_start NULL: kv_len[b] - Nq, so that the last query
- * stands at the last key (a cache that already holds the new tokens); a batch
- * padded on the right passes zeros.  |scale| is at most 2^120 and softcap is 0 or within 2^-60 .. 2^100, and
- * at least 2^-60 |scale| (else TL_ERR_UNSUPPORTED); a softcap above 2^60 |scale| is as 0.
+ * k_doc [batch, Nk] int32 are contiguous and lie on 4 bytes.  kv_len NULL: all Nk keys;
+ * its values are clamped to 0..Nk, those of q_start to +-2^30.  q_start NULL:
+ * kv_len[b] - Nq, so that the last query stands at the last key (a cache that already
+ * holds the new tokens); a batch padded on the right passes zeros.  |scale| is at most
+ * 2^120, and softcap 0 or within 2^-60 .. 2^100 and at least 2^-60 |scale| (else
+ * TL_ERR_UNSUPPORTED); a softcap above 2^60 |scale| is as 0.
  */
 typedef struct tl_attention {
     tl_array q, k, v, o;                /* o: forward writes, backward reads  */
@@ -522,7 +531,8 @@ tl_status tl_attention_backward(tl_ctx* ctx, const tl_attention* a);
 int64_t tl_attention_workspace(tl_ctx* ctx, const tl_attention* a, int32_t backward);
 
 /*
- * norm = sqrt(sum of x^2 over all elements of the n arrays), in 64 bits;
+ * norm = sqrt(sum of x^2 over all elements of the n arrays), in 64 bits (the squares
+ * of 16 neighbouring bytes are added in 32 first, where they stay within fp32);
  * out = x min(1, max_norm / norm).  out NULL: in place (nothing is written when
  * norm <= max_norm).  A norm that is not finite leaves the values as they are.
  * The arrays may have different types and ranks; each is dense (its elements

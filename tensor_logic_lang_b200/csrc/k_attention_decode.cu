@@ -17,11 +17,11 @@
 //                  warps takes a quarter of a tile's keys for all rows, with
 //                  mma.sync.m16n8k16 (at a few rows a key the tensor work is a
 //                  fraction of the time the key's bytes take)
-//                  16 x 32 heads over 8, caches up to 32768, d 128: 181 us, 6.6 TB/s; 5
-//                  sequences x 3 tokens of 16 heads, 4099, d 64: 18 us with the join, 2.6
+//                  16 x 32 heads over 8, caches up to 32768, d 128: 186 us, 6.5 TB/s; 5
+//                  sequences x 3 tokens of 16 heads, 4099, d 64: 20 us with the join, 2.4
 //                  TB/s: starts and ends of pieces of a few tiles
 //   k_decode_any   any type, stride and head size: tiles as fp32 in shared
-//                  memory, FFMA; fp32, 16 x 32 heads over 8, 4096, d 128: 85 us, 3.6 TB/s, its
+//                  memory, FFMA; fp32, 16 x 32 heads over 8, 4096, d 128: 85 us, 3.6 TB/s of 6.5, its
 //                  five barriers a tile leave the loads uneven
 #include <algorithm>
 

@@ -33,9 +33,10 @@
 // thread adds them to the sum, also in TMEM, behind S, with rounded additions.
 //
 // Bound by the softmax threads' chain (TMEM loads, maximum, exponentials, TMEM
-// stores; with a cap the tanh's polynomial too), not by the products, which keep
-// the tensor pipe busy for 50 to 70 %.  16 heads of 16384 queries and keys, bf16, causal:
-// d 128 950 to 1030 us, 1160 to 1070 TFLOP/s, cap 50 1270; d 64 783 us, 702 TFLOP/s, cap 50 963.
+// stores; with a cap the tanh's polynomial too), not by the products: 1 x 32/8 heads x 4096 x
+// 128, cap 50, keep the tensor pipe busy for 41 % of the clocks, the exponentials' pipe for 42 %.
+// 16 heads of 16384 queries and keys, bf16, causal: d 128 950 to 1070 us (the power cap), 1160 to
+// 1030 TFLOP/s, cap 50 1260; d 64 780 us, 705 TFLOP/s, cap 50 946.
 // With a thread a whole row, and MMAs issued by lane 0 with descriptors made for
 // each, 910 and 669 TFLOP/s where this reached 1083 and 867 (not causal).
 #include <algorithm>

@@ -34,10 +34,12 @@
 // the outputs tile by tile (sums of 4 tiles on the tensor cores lost 2.4e-6 of dk
 // and dv, of one 6e-7).
 //
-// Bound by the element work between the products: a pair of tiles takes about 4300 clocks
-// in either kernel, of which the products fill 2048 (dk, dv) and 1536.  16 heads of 16384
-// queries and keys, bf16, causal, five products counted: d 128 3860 us, 712 TFLOP/s,
-// cap 50 4460; d 64 2890 us, 475 TFLOP/s, cap 50 3600.  fp32, 8 heads of 4096: d 64 215 us, d 96 440.
+// Bound by the element work between the products: a pair of tiles takes about 4600 clocks
+// in the dq kernel and 5700 in the other (2 x 16/4 heads x 2048 x 128, cap 30, starts and ends
+// of walks of 1 to 16 tiles among them), of which the products fill 1536 and 2048; instructions
+// issue in 52 % of the clocks.  16 heads of 16384 queries and keys, bf16, causal, five products
+// counted: d 128 3400 to 3900 us (the power cap), 810 to 710 TFLOP/s, cap 50 4490; d 64 2870 us, 479 TFLOP/s,
+// cap 50 3510.  fp32, 8 heads of 4096: d 64 214 us, d 96 455.
 #include <algorithm>
 
 #include "attn_tc.h"

@@ -9,9 +9,9 @@
 //
 // HBM-bound: the list is read once for the norm, and read and written once
 // more where it is scaled, the last chunks first: the L2 cache still holds
-// those.  The blocks take the chunks in turn.  400M bf16 into fp32, one array: 515 us, 6.2 TB/s of the 3.2 GB that
-// two reads and a write are; 291 arrays: 546 us; 360 MB of fp32 under the limit:
-// 61 us, 5.9 TB/s.  A chunk is a piece of one array; the list travels in the launch's
+// those.  The blocks take the chunks in turn.  400M bf16 into fp32, one array: 514 us, 6.2 TB/s of the 3.2 GB that
+// two reads and a write are; 291 arrays of six sizes: 563 to 573 us; 360 MB of fp32 under the limit:
+// 64 to 67 us, 5.5 TB/s, in place over it 193 us, 5.6 TB/s.  A chunk is a piece of one array; the list travels in the launch's
 // parameters (no copy, so a captured call keeps it).  128-bit loads, eight
 // in flight a thread (four: 585 us), stores of up to 256 bits; a chunk whose array
 // starts between 16-byte boundaries peels its first elements.
