@@ -276,6 +276,14 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)L::TMEM));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    if (pack) {
+        // rows of no query: what they hold would have a say in their warp's common choices
+        // (rescaling, the tanh's form), and so in the last bits of the others
+        const int first = pack * group * 128, n = (CHUNK_BYTES - first) / 16;
+        for (int e = threadIdx.x; e < HALVES * L::CH * n; e += L::THREADS)
+            *reinterpret_cast<uint4*>(smem + L::Q + e / n * CHUNK_BYTES + first + e % n * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+    }
     if (warp == L::TMA && lane == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mq.map)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&mk.map)) : "memory");

@@ -247,6 +247,26 @@ def test_runs_repeat_bit_for_bit(ctx, dtype):
                 assert torch.equal(first[n], again[n]), n
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hq,hkv,nq,nk,d", [(8, 2, 30, 700, 64), (8, 1, 9, 1300, 128), (4, 1, 18, 155, 128), (64, 8, 3, 300, 64),
+                                            (24, 8, 17, 600, 100), (16, 2, 40, 40, 32)])
+def test_what_ran_before_leaves_no_trace(ctx, hq, hkv, nq, nk, d, dtype):
+    # tiles that hold fewer queries than rows: shared memory that other calls left behind does not show in a bit
+    gen = torch.Generator(device="cuda").manual_seed(nq)
+    q, k, v = heads(gen, 2, hq, nq, d, dtype), heads(gen, 2, hkv, nk, d, dtype), heads(gen, 2, hkv, nk, d, dtype)
+    q.mul_(4.0)
+    others = [[x.mul_(by) for x in (heads(gen, 2, 16, 256, 128, t), *(heads(gen, 2, 4, 512, 128, t) for _ in range(2)))]
+              for t in ("bf16", "f32") for by in (0.0, 1.0, 30.0)]
+    for m in ({"causal": True}, {"softcap": 3.0}, {"slopes": torch.full((hq,), 0.02, device="cuda")}):
+        first = run(ctx, q, k, v, None, m)
+        for a, b, c in others:
+            for _ in range(2):
+                ctx.attention(a, b, c, torch.empty_like(a), stream=stream())
+            again = run(ctx, q, k, v, None, m)
+            for n in first:
+                assert torch.equal(first[n], again[n]), n
+
+
 @pytest.mark.parametrize("nq", [1, 200])
 def test_captured_and_replayed(ctx, nq):
     # two graphs with workspaces of their own, replayed side by side on new values
