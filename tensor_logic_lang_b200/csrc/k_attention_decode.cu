@@ -501,14 +501,15 @@ __global__ void __launch_bounds__(DmSmem<DP>::THREADS, DmSmem<DP>::PER_SM)
     while (walk.next(g, &pc)) {
         const SeqMask mask(a, pc.b);
         const int32_t* kd = a.k_doc ? a.k_doc + (int64_t)pc.b * a.nk : nullptr;
-        // the unit's query rows (zeros past the last one and past the head size)
+        // the unit's query rows (zeros past the last one, past the head size and of padding)
         for (int e = threadIdx.x; e < 16 * DP / 8; e += 32 * L::WARPS) {
             const int r = e / (DP / 8), c = e % (DP / 8) * 8, row = pc.rb * g.rows + r;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (row < a.nq * (a.hq / a.hkv) && c < a.d) {
                 int i, h;
                 unit_row(a, pc.kvh, row, &i, &h);
-                v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.p) + pc.b * a.q.sb + h * a.q.sh + i * a.q.ss + c);
+                if (!a.q_doc || a.q_doc[(int64_t)pc.b * a.nq + i] >= 0)
+                    v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.p) + pc.b * a.q.sb + h * a.q.sh + i * a.q.ss + c);
             }
             *reinterpret_cast<uint4*>(qs + r * L::LQ + c) = v;
         }
@@ -537,17 +538,23 @@ __global__ void __launch_bounds__(DmSmem<DP>::THREADS, DmSmem<DP>::PER_SM)
             if (!ok) break;
             uint8_t* kt = smem + L::KV + 2 * st * L::TILE_B;
             uint8_t* vt = kt + L::TILE_B;
-            // keys whose values must not count: 0 times what they hold could be NaN
+            // keys that must not count: 0 times what V holds could be NaN, and scores of what K
+            // holds would have a say in the tanh's form
             const int jl = j0 + lane % KW;
             const int jdoc = kd && jl < a.nk ? __ldg(kd + jl) : -1;
             const bool bad = jl >= mask.kv || (kd && jdoc < 0);
             const bool dirty = __any_sync(0xffffffffu, bad);
             if (dirty) {
-                if (bad && lane < KW)
+                auto clear = [&](uint8_t* tile) {
                     for (int c = 0; c < L::CH; ++c)
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
-                            *reinterpret_cast<uint4*>(vt + c * L::CHUNK + (warp * KW + lane) * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(tile + c * L::CHUNK + (warp * KW + lane) * 128 + 16 * k) = make_uint4(0, 0, 0, 0);
+                };
+                if (bad && lane < KW) {
+                    clear(vt);
+                    if (a.cap > 0.f) clear(kt);
+                }
                 __syncwarp();
             }
             // scores of the warp's keys, 8 to a tile

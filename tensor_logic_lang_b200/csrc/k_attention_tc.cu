@@ -387,9 +387,30 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
             auto wait_entries = [&](int e) {
                 for (int f = 0; f < HALVES; ++f) wait_full(full, e + f, L::STAGES);
             };
+            // Rows of padding are zeros where they count: those of V, since 0 probability times
+            // what they hold could be NaN; with a cap those of K and Q, whose scores would
+            // have a say in the tanh's form of their warps, and so in the others' last bits.
+            auto padded = [&](int tile, bool mk) { return !SPLIT && ((kd && mk) || (mask.kv < a.nk && (tile + 1) * TILE > mask.kv)); };
+            auto clean = [&](int e, int tile) {
+                clear_rows(smem + L::KV + e % L::STAGES * L::TILE_B, L::CH, [&](int r) {
+                    const int j = tile * TILE + r;
+                    return j >= mask.kv || (kd && kd[j] < 0);
+                });
+                fence_proxy_async_smem();
+                __syncwarp();
+            };
             if (kt >= 0) {
                 wait_full(q_full, 0, 1);
+                if (CAP && !SPLIT && ok && qd && mine.pad) {
+                    clear_rows(smem + L::Q, L::CH, [&](int r) {
+                        const int i = i0 + (pack ? r % pack : r);
+                        return i < a.nq && qd[i] < 0;
+                    });
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
                 wait_entries(n);
+                if (CAP && ok && padded(kt, masked)) clean(n, kt);
                 for (int t = 0; t < NT; ++t) scores(t, n);
                 if (ok && elect_one()) free_entries(n);
                 n += HALVES;
@@ -398,18 +419,13 @@ __global__ void __launch_bounds__(Fw<T, U, DP, NT>::THREADS, Fw<T, U, DP, NT>::P
                 const int vs = n;   // V's entries
                 wait_entries(n);
                 n += HALVES;
-                // rows of V that must not count: 0 probability times what they hold could be NaN
-                if (!SPLIT && ok && ((kd && masked) || (mask.kv < a.nk && (kt + 1) * TILE > mask.kv))) {
-                    clear_rows(smem + L::KV + vs % L::STAGES * L::TILE_B, L::CH, [&](int r) {
-                        const int j = kt * TILE + r;
-                        return j >= mask.kv || (kd && kd[j] < 0);
-                    });
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                }
+                if (ok && padded(kt, masked)) clean(vs, kt);
                 bool next_masked;
                 const int next = walk.next(&next_masked);
-                if (next >= 0) wait_entries(n);   // the next keys: nothing waits between P V and S
+                if (next >= 0) {
+                    wait_entries(n);   // the next keys: nothing waits between P V and S
+                    if (CAP && ok && padded(next, next_masked)) clean(n, next);
+                }
                 for (int t = 0; t < NT; ++t) {
                     ok = ok && mbar_wait(&p_full[t], it & 1, g.err);
                     ok = __all_sync(0xffffffffu, ok);

@@ -627,6 +627,12 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             }
             if (!WIDE && any) {
                 ok = warp_wait(bb.fix, 0, ok, g.err);
+                // keys of padding: their scores would have a say in the tanh's form of their warps
+                if (CAP && !SPLIT && ((kd && mine.pad) || (mask.kv < a.nk && j0 + TILE > mask.kv))) {
+                    clear_rows(smem + L::FIX, L::CH, [&](int r) { return j0 + r < a.nk && (j0 + r >= mask.kv || (kd && kd[j0 + r] < 0)); });
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
                 ok = warp_wait(&bb.full[0], 0, ok, g.err);
                 if (ok) clean(0);
                 const uint32_t sq = smem_u32(smem + L::RING);
@@ -931,6 +937,12 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
             }
             if (!WIDE && any) {
                 ok = warp_wait(bb.fix, 0, ok, g.err);
+                // queries of padding, likewise
+                if (CAP && !SPLIT && qd && mine.pad) {
+                    clear_rows(smem + L::FIX, L::CH, [&](int r) { return i0 + r < a.nq && qd[i0 + r] < 0; });
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
                 ok = warp_wait(&bb.full[0], 0, ok, g.err);
                 if (ok) clean(0);
                 const uint32_t sk = smem_u32(smem + L::RING);

@@ -267,6 +267,32 @@ def test_what_ran_before_leaves_no_trace(ctx, hq, hkv, nq, nk, d, dtype):
                 assert torch.equal(first[n], again[n]), n
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("names", ["len cap", "docs cap", "ids cap causal", "len docs cap slopes", "len docs", "ids causal slopes"])
+@pytest.mark.parametrize("size", [(3, 8, 2, 1, 700, 64), (3, 4, 2, 3, 300, 128), (2, 4, 1, 60, 60, 40), (2, 2, 2, 300, 300, 128),
+                                  (3, 4, 2, 150, 333, 64), (2, 6, 2, 11, 150, 192)])
+def test_padding_leaves_no_trace(ctx, size, names, dtype):
+    # what padding holds does not show in a bit of any result
+    b, hq, hkv, nq, nk, d = size
+    gen = torch.Generator(device="cuda").manual_seed(nk)
+    arrays = [heads(gen, b, h, n, d, dtype) for h, n in ((hq, nq), (hkv, nk), (hkv, nk), (hq, nq))]
+    m = modifiers(names, b, hq, nq, nk, 1)
+    k_ok = torch.arange(nk, device="cuda")[None] < m.get("kv_len", ints([nk] * b))[:, None]
+    q_ok = torch.ones((b, nq), dtype=torch.bool, device="cuda")
+    if "k_doc" in m:
+        k_ok, q_ok = k_ok & (m["k_doc"] >= 0), m["q_doc"] >= 0
+    first = {}
+    for fill in (0.0, -3.0, 1000.0, float("inf"), float("nan")):
+        q, k, v, dout = (torch.where(ok[:, None, :, None], x, torch.full_like(x, fill))
+                         for x, ok in zip(arrays, (q_ok, k_ok, k_ok, q_ok)))
+        for softcap in (6.0, 30.0) if "cap" in names else (0.0,):
+            got = run(ctx, q, k, v, dout, dict(m, softcap=softcap))
+            if fill == 0.0:
+                first[softcap] = got
+            for n in got:
+                assert torch.equal(got[n], first[softcap][n]), (fill, softcap, n)
+
+
 @pytest.mark.parametrize("nq", [1, 200])
 def test_captured_and_replayed(ctx, nq):
     # two graphs with workspaces of their own, replayed side by side on new values
