@@ -50,7 +50,7 @@ namespace {
 // needs no maximum: p = 2^s lies in 2^-top .. 2^top, and up to top = 72.5 (softcap 50.2)
 // its products with v and their sums stay normal numbers of fp32 for |v| of 2^-53 to
 // 2^54 / keys.  No maxima, no agreeing on them, no rescaling (1 x 32/8 heads x 4096 x 128,
-// causal, cap 50: 163 us, 174 with them).
+// causal, cap 50: 161 us, 174 with them).
 constexpr float kFixTop = 72.5f;
 constexpr float kFuseTop = 0x1p12f;   // half a step of it is 2^-12, less than P's rounding
 constexpr float kGrow = 8.f;   // rescale when the maximum grew by 2^8
