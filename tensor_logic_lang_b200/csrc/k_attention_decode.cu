@@ -45,12 +45,15 @@ struct DecArgs {
     int* err;
 };
 
+// Documents' spans come out of the workspace.  Where a caller lets other work write there
+// meanwhile, results are lost, but what is made of the spans stays within the
+// arrays: here, in find_place and in the join.
 __device__ __forceinline__ int2 seq_tiles(const DecArgs& g, int b) {
     const SeqMask mask(g.a, b);
     int end = max(mask.key_end(0, g.a.nq), 0), begin = 0;
     if (g.spans) {
         const int2 s = g.spans[b];
-        begin = min(s.x, end);
+        begin = min(max(s.x, 0), end);
         end = min(s.y, end);
     }
     if (end <= begin) return make_int2(0, 0);
@@ -153,11 +156,15 @@ __device__ __forceinline__ Place find_place(const DecArgs& g, int64_t* left, int
         if (found[0] >= 0) break;
         before += total;
     }
+    if (found[0] < 0) {
+        *left = 0;
+        return p;
+    }
     p.b = (int)found[0];
     p.span = seq_tiles(g, p.b);
-    const int n = p.span.y - p.span.x;
+    const int n = max(p.span.y - p.span.x, 1);
     const int64_t in = at - found[1];
-    p.unit = (int)(in / n);
+    p.unit = (int)min(in / n, (int64_t)units - 1);
     p.tile = p.span.x + in % n;
     return p;
 }
@@ -343,7 +350,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_decode_join(const __grid_const
     const int n = span.y - span.x, d2 = a.d + 2;
     const int64_t per = max((int64_t)1, (all + g.blocks - 1) / g.blocks);
     const int64_t u0 = before + (int64_t)unit * n, u1 = u0 + n;
-    const int first = (int)(u0 / per), last = n ? (int)((u1 - 1) / per) : first;
+    const int first = (int)min(u0 / per, (int64_t)g.blocks - 1), last = n ? (int)min((u1 - 1) / per, (int64_t)g.blocks - 1) : first;
     // before any return: where no row is split over blocks, what follows this
     // kernel would else start before the outputs are written
     wait_for_previous();

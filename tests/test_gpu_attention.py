@@ -372,6 +372,30 @@ def test_few_rows_are_written_when_the_call_ends(ctx, b, hkv, nk, dtype):
         check(kept_lse, want["lse"], "lse")
 
 
+@pytest.mark.parametrize("names", ["docs", "docs len causal", ""])
+def test_graphs_that_take_turns_share_a_workspace(ctx, names):
+    # two captured calls of different sizes, one replayed when the other's work is done
+    gen = torch.Generator(device="cuda").manual_seed(14)
+    kept, ws = [], torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+    for b, hkv, nq, nk, dtype in ((3, 8, 2, 900, "bf16"), (2, 2, 60, 300, "f32")):
+        q, k, v = heads(gen, b, 2 * hkv, nq, 64, dtype), heads(gen, b, hkv, nk, 64, dtype), heads(gen, b, hkv, nk, 64, dtype)
+        out, lse = like(q, "bhsd"), torch.empty(q.shape[:3], device="cuda")
+        m = modifiers(names, b, 2 * hkv, nq, nk, 3)
+        assert ctx.attention_workspace(q, k, v, out, lse, **m) <= ws.numel()
+        ctx.attention(q, k, v, out, lse, workspace=ws, stream=stream(), **m)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ctx.attention(q, k, v, out, lse, workspace=ws, stream=stream(), **m)
+        kept.append((graph, q, k, v, out, lse, m))
+    for _ in range(3):
+        for graph, q, k, v, out, lse, m in kept:
+            v.copy_(torch.randn(v.shape, generator=gen, device="cuda"))
+            graph.replay()
+            want = reference(q, k, v, **m)
+            check(out, want["out"], "out")
+            check(lse, want["lse"], "lse")
+
+
 def test_capture_needs_a_workspace(ctx):
     from tensor_logic_lang_b200 import abi
     gen = torch.Generator(device="cuda").manual_seed(4)
